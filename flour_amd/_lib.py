@@ -11,7 +11,7 @@ from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "libflour_hip.so"
 
-F32, BF16, F16 = 0, 1, 2
+F32, BF16, F16, E4M3, I8 = 0, 1, 2, 3, 4
 OK = 0
 ERR_INVALID_ARGUMENT = -1
 ERR_UNSUPPORTED = -2
@@ -52,6 +52,33 @@ SIGNATURES: dict[str, tuple] = {
                                              _vp, _vp, _vp, _vp, _vp, _c_int, _c_int, _c_int,
                                              _c_int, _c_int, _c_int, _c_int, _c_int, _c_i64, _c_f,
                                              _c_int, _vp, _c_sz, _vp]),
+    "flour_hip_kv_write_q8": (_c_int, [_vp, _vp, _c_i64, _c_i64, _c_int, _vp, _vp, _vp, _vp, _c_int,
+                                       _vp, _vp, _vp, _c_int, _c_int, _c_int, _c_int, _c_int,
+                                       _c_int, _c_i64, _vp]),
+    "flour_hip_kv_dequant": (_c_int, [_vp, _vp, _c_int, _vp, _c_int, _c_i64, _vp, _vp, _vp, _vp,
+                                      _c_int, _vp, _c_int, _vp, _c_int, _c_int, _c_int, _c_int,
+                                      _c_int, _c_i64, _vp]),
+    "flour_hip_paged_decode_q8": (_c_int, [_vp, _c_int, _vp, _c_int, _vp, _vp, _vp, _vp, _c_int,
+                                           _vp, _c_int, _vp, _c_int, _c_int, _c_int, _c_int,
+                                           _c_int, _c_i64, _c_int, _c_f, _vp, _c_i64, _vp, _c_int,
+                                           _vp, _c_sz, _vp]),
+    "flour_hip_paged_decode_weights": (_c_int, [_vp, _c_int, _vp, _vp, _vp, _vp, _c_int, _vp,
+                                                _c_int, _c_int, _c_int, _c_int, _c_int, _c_i64,
+                                                _c_int, _c_f, _c_int, _vp, _c_i64, _vp, _c_int,
+                                                _vp, _c_sz, _vp]),
+    "flour_hip_decode_weights_workspace_size": (_c_int, [_c_int, _c_int, _c_int, _c_int, _c_int,
+                                                         _c_int, ctypes.POINTER(ctypes.c_size_t)]),
+    "flour_hip_varlen_prefill_q8": (_c_int, [_vp, _c_int, _c_i64, _c_i64, _vp, _c_i64, _c_i64,
+                                             _c_int, _vp, _vp, _vp, _vp, _c_int, _vp, _vp, _vp,
+                                             _c_int, _c_int, _c_int, _c_int, _c_int, _c_int,
+                                             _c_int, _c_int, _c_i64, _c_int, _c_f, _vp, _c_sz,
+                                             _vp]),
+    "flour_hip_varlen_prefill_q8_workspace_size": (_c_int, [_c_int, _c_int, _c_int, _c_int, _c_int,
+                                                            _c_int, _c_int, _c_int, _c_int,
+                                                            ctypes.POINTER(ctypes.c_size_t)]),
+    "flour_hip_kv_evict": (_c_int, [_vp, _vp, _vp, _vp, _c_int, _vp, _vp, _c_i64, _vp, _c_int, _vp,
+                                    _c_int, _vp, _vp, _vp, _c_int, _vp, _c_int, _c_int, _c_int,
+                                    _c_int, _c_i64, _c_int, _c_int, _c_int, _vp]),
     # include/flour_cache.h
     "flour_block_allocator_create": (_c_int, [_c_int, _vp]),
     "flour_block_allocator_destroy": (None, [_vp]),

@@ -1,0 +1,387 @@
+// attn_pools.hip — attention over pools of any element type and shape, with the scores kept for the
+// attention-weight sums where they are asked for.
+//
+// The kernels that every other one is checked against, and what runs where the streamed decode
+// (decode_pools.hip) does not take a shape: any head_dim up to 512, block size, group size,
+// alignment. One workgroup a (row, query head): 256 positions at a time, a thread's whole dot
+// product each, then a thread's output dims each over the 256 weights in LDS.
+#include <math.h>
+
+#include "cache8.h"
+#include "decode_pools.h"
+
+namespace flour {
+
+static constexpr int AP_THREADS = 256;
+static constexpr int AP_MAX_D = 512;
+
+template <typename T>
+__device__ __forceinline__ float pool_f32(const T* p) {
+    return to_f32(*p);
+}
+template <>
+__device__ __forceinline__ float pool_f32<e4m3_t>(const e4m3_t* p) {
+    return Elem8<e4m3_t>::widen1(p->bits);
+}
+template <>
+__device__ __forceinline__ float pool_f32<i8_t>(const i8_t* p) {
+    return (float)p->v;
+}
+
+template <typename F>
+__device__ __forceinline__ float ap_reduce(float x, float* red, F op) {
+    for (int o = 32; o > 0; o >>= 1) x = op(x, __shfl_xor(x, o, 64));
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = x;
+    __syncthreads();
+    float r = red[0];
+    for (int i = 1; i < AP_THREADS / 64; i++) r = op(r, red[i]);
+    return r;
+}
+
+// scores (or null): (batch, num_heads, score_stride) in the exp2 domain, ml (batch, num_heads, 2)
+// their maximum and sum: decode steps only.
+template <typename TQ, typename TP>
+__global__ __launch_bounds__(AP_THREADS) void attn_pools_kernel(
+    void* __restrict__ out, int out_dtype, int64_t o_st, int64_t o_sh, const TQ* __restrict__ q,
+    int64_t q_st, int64_t q_sh, const TP* __restrict__ k_pool, const TP* __restrict__ v_pool,
+    const float* __restrict__ k_scale, const float* __restrict__ v_scale,
+    const int32_t* __restrict__ cu, const int32_t* __restrict__ kv_lens,
+    const int32_t* __restrict__ block_tables, int max_blocks, int num_seqs, int num_heads,
+    int n_rep, int head_dim, int block_size, int64_t num_slots, int max_kv, float scale_log2,
+    float* __restrict__ scores, int64_t score_stride, float* __restrict__ ml) {
+    __shared__ float qs[AP_MAX_D];
+    __shared__ float ps[AP_THREADS];
+    __shared__ int64_t rows[AP_THREADS];
+    __shared__ float red[AP_THREADS / 64];
+    const int64_t r = blockIdx.x;
+    const int h = blockIdx.y, tid = threadIdx.x;
+    int s = (int)r, i = 0, q_len = 1;
+    if (cu) {
+        int lo = 0, hi = num_seqs;
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (cu[mid] <= r)
+                lo = mid;
+            else
+                hi = mid;
+        }
+        s = lo;
+        i = (int)(r - cu[s]);
+        q_len = cu[s + 1] - cu[s];
+    }
+    const int kv_len = (int)min((int64_t)min(kv_lens[s], max_kv), (int64_t)max_blocks * block_size);
+    const int64_t n_vis = kv_len >= q_len ? (int64_t)kv_len - q_len + i + 1 : 0;
+    const int g = h / n_rep;
+    const int64_t nb = num_slots / block_size;
+    const int32_t* bt = block_tables + (int64_t)s * max_blocks;
+    for (int d = tid; d < head_dim; d += AP_THREADS) qs[d] = to_f32(q[r * q_st + h * q_sh + d]);
+    __syncthreads();
+
+    float m = -3.402823466e38f, l = 0.0f, acc[AP_MAX_D / AP_THREADS] = {};
+    for (int64_t c0 = 0; c0 < n_vis; c0 += AP_THREADS) {
+        const int64_t j = c0 + tid;
+        float sc = -INFINITY, vs = 1.0f;
+        int64_t row = 0;
+        if (j < n_vis) {
+            const int64_t lb = j / block_size;
+            int64_t id = bt[lb];
+            id = id < 0 ? 0 : (id >= nb ? nb - 1 : id);
+            row = ((int64_t)g * num_slots + id * block_size + (j - lb * block_size)) * head_dim;
+            float dot = 0.0f;
+            for (int d = 0; d < head_dim; d++) dot = fmaf(qs[d], pool_f32(k_pool + row + d), dot);
+            if (k_scale) {
+                dot *= k_scale[g * nb + id];
+                vs = v_scale[g * nb + id];
+            }
+            sc = dot * scale_log2;
+            if (scores) scores[(r * num_heads + h) * score_stride + j] = sc;
+        }
+        rows[tid] = row;
+        const float m_new =
+            fmaxf(m, ap_reduce(sc, red, [](float a, float b) { return fmaxf(a, b); }));
+        const float corr = fast_exp2(m - m_new);
+        const float p = j < n_vis ? fast_exp2(sc - m_new) : 0.0f;
+        ps[tid] = p * vs;
+        // (its barriers also publish ps and rows)
+        l = l * corr + ap_reduce(p, red, [](float a, float b) { return a + b; });
+        const int nj = (int)min(n_vis - c0, (int64_t)AP_THREADS);
+#pragma unroll
+        for (int x = 0; x < AP_MAX_D / AP_THREADS; x++) {
+            const int d = tid + x * AP_THREADS;
+            if (d < head_dim) {
+                float pv = 0.0f;
+                for (int jj = 0; jj < nj; jj++)
+                    pv = fmaf(ps[jj], pool_f32(v_pool + rows[jj] + d), pv);
+                acc[x] = acc[x] * corr + pv;
+            }
+        }
+        m = m_new;
+        __syncthreads();  // ps and rows are written again by the next chunk
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // (a NaN is handed on)
+#pragma unroll
+    for (int x = 0; x < AP_MAX_D / AP_THREADS; x++) {
+        const int d = tid + x * AP_THREADS;
+        if (d < head_dim) {
+            const int64_t at = r * o_st + h * o_sh + d;
+            const float y = l == 0.0f ? 0.0f : acc[x] * inv;
+            if (out_dtype == FLOUR_DTYPE_F32)
+                static_cast<float*>(out)[at] = y;
+            else if (out_dtype == FLOUR_DTYPE_BF16)
+                static_cast<bf16_t*>(out)[at] = from_f32<bf16_t>(y);
+            else
+                static_cast<f16_t*>(out)[at] = from_f32<f16_t>(y);
+        }
+    }
+    if (scores && tid == 0) {
+        ml[(r * num_heads + h) * 2] = m;
+        ml[(r * num_heads + h) * 2 + 1] = l;
+    }
+}
+
+// weights[r, g, j] += sum over kv head g's query heads of exp2(score - max) / sum, in their order.
+__global__ __launch_bounds__(AP_THREADS) void weights_add_kernel(
+    float* __restrict__ weights, int64_t width, const int32_t* __restrict__ weight_rows,
+    int num_rows, const int32_t* __restrict__ context_lens, int max_ctx, int kv_heads, int n_rep,
+    const float* __restrict__ scores, int64_t score_stride, const float* __restrict__ ml) {
+    const int b = blockIdx.z, g = blockIdx.y;
+    const int r = weight_rows ? weight_rows[b] : b;
+    const int64_t j = (int64_t)blockIdx.x * AP_THREADS + threadIdx.x;
+    if (r < 0 || r >= num_rows || j >= min(context_lens[b], max_ctx)) return;
+    float sum = 0.0f;
+    for (int i = 0; i < n_rep; i++) {
+        const int64_t h = ((int64_t)b * kv_heads + g) * n_rep + i;
+        const float l = ml[2 * h + 1];
+        const float p = fast_exp2(scores[h * score_stride + j] - ml[2 * h]);
+        sum += l == 0.0f ? 0.0f : p / l;
+    }
+    weights[((int64_t)r * kv_heads + g) * width + j] += sum;
+}
+
+int launch_weights_add(float* weights, int64_t width, const int32_t* weight_rows, int num_rows,
+                       const int32_t* context_lens, int max_ctx, int batch, int kv_heads,
+                       int n_rep, const float* scores, int64_t score_stride, const float* ml,
+                       hipStream_t stream) {
+    if (max_ctx <= 0) return FLOUR_OK;
+    weights_add_kernel<<<dim3((unsigned)((max_ctx + AP_THREADS - 1) / AP_THREADS), kv_heads, batch),
+                         dim3(AP_THREADS), 0, stream>>>(weights, width, weight_rows, num_rows,
+                                                        context_lens, max_ctx, kv_heads, n_rep,
+                                                        scores, score_stride, ml);
+    return check_hip(hipGetLastError(), "attention weights launch");
+}
+
+int launch_attn_pools(const PoolAttn& a, hipStream_t stream) {
+    if (a.head_dim > AP_MAX_D) {
+        set_error("attention over 8-bit pools or with weights: head_dim %d > %d is not supported",
+                  a.head_dim, AP_MAX_D);
+        return FLOUR_ERR_UNSUPPORTED;
+    }
+    if (a.num_heads > 65535 || (a.scores && (a.batch > 65535 || a.kv_heads > 65535))) {
+        set_error("attention: %d heads of %d sequences are too many", a.num_heads, a.batch);
+        return FLOUR_ERR_UNSUPPORTED;
+    }
+    const int n_rep = a.num_heads / a.kv_heads;
+#define FLOUR_AP(TQ, TP)                                                                          \
+    attn_pools_kernel<TQ, TP><<<dim3(a.rows, a.num_heads), dim3(AP_THREADS), 0, stream>>>(        \
+        a.out, a.out_dtype, a.o_st, a.o_sh, static_cast<const TQ*>(a.q), a.q_st, a.q_sh,          \
+        static_cast<const TP*>(a.k_pool), static_cast<const TP*>(a.v_pool), a.k_scale, a.v_scale, \
+        a.cu, a.kv_lens, a.block_tables, a.max_blocks, a.batch, a.num_heads, n_rep, a.head_dim,   \
+        a.block_size, a.num_slots, a.max_kv, a.scale * LOG2_E, a.scores, a.score_stride, a.ml)
+#define FLOUR_AP_Q(TQ)                                                                            \
+    do {                                                                                          \
+        if (a.pool_dtype == FLOUR_DTYPE_E4M3) FLOUR_AP(TQ, e4m3_t);                               \
+        else if (a.pool_dtype == FLOUR_DTYPE_I8) FLOUR_AP(TQ, i8_t);                              \
+        else FLOUR_AP(TQ, TQ);                                                                    \
+    } while (0)
+    if (a.dtype == FLOUR_DTYPE_F32) FLOUR_AP_Q(float);
+    else if (a.dtype == FLOUR_DTYPE_BF16) FLOUR_AP_Q(bf16_t);
+    else FLOUR_AP_Q(f16_t);
+#undef FLOUR_AP_Q
+#undef FLOUR_AP
+    return check_hip(hipGetLastError(), "attention (any pool) launch");
+}
+
+}  // namespace flour
+
+using namespace flour;
+
+namespace flour {
+
+static size_t up256(size_t x) { return (x + 255) & ~(size_t)255; }
+
+static int64_t score_stride_of(int max_ctx) { return ((int64_t)max_ctx + 63) / 64 * 64; }
+
+static size_t decode_pools_ws(int batch, int num_heads, int max_ctx, bool with_weights) {
+    if (!with_weights) return 0;
+    const size_t rows = (size_t)batch * num_heads;
+    return up256(rows * 2 * sizeof(float)) + up256(rows * score_stride_of(max_ctx) * sizeof(float));
+}
+
+static int decode_pools(const char* what, PoolAttn a, float* weights, int64_t width,
+                        const int32_t* weight_rows, int num_rows, void* workspace,
+                        size_t workspace_bytes, hipStream_t stream) {
+    if (!valid_dtype(a.dtype) || !valid_dtype(a.out_dtype)) {
+        set_error("%s: unknown dtype (%d, out %d)", what, a.dtype, a.out_dtype);
+        return FLOUR_ERR_INVALID_ARGUMENT;
+    }
+    if (a.batch < 0 || a.num_heads <= 0 || a.kv_heads <= 0 || a.num_heads % a.kv_heads != 0 ||
+        a.head_dim <= 0 || a.block_size <= 0 || a.num_slots <= 0 ||
+        a.num_slots % a.block_size != 0 || a.max_blocks <= 0 || a.max_kv < 0 ||
+        (int64_t)a.max_kv > (int64_t)a.max_blocks * a.block_size) {
+        set_error("%s: bad shape (batch=%d heads=%d kv_heads=%d head_dim=%d bs=%d num_slots=%lld "
+                  "max_blocks=%d max_ctx=%d)",
+                  what, a.batch, a.num_heads, a.kv_heads, a.head_dim, a.block_size,
+                  (long long)a.num_slots, a.max_blocks, a.max_kv);
+        return FLOUR_ERR_INVALID_ARGUMENT;
+    }
+    if (weights && (width < a.max_kv || num_rows < 0 || (!weight_rows && num_rows < a.batch))) {
+        set_error("%s: weights of %d rows of width %lld for %d sequences of up to %d positions",
+                  what, num_rows, (long long)width, a.batch, a.max_kv);
+        return FLOUR_ERR_INVALID_ARGUMENT;
+    }
+    if (a.batch == 0) return FLOUR_OK;
+    if (!a.out || !a.q || !a.k_pool || !a.v_pool || !a.block_tables || !a.kv_lens) {
+        set_error("%s: null pointer", what);
+        return FLOUR_ERR_INVALID_ARGUMENT;
+    }
+    const size_t need = decode_pools_ws(a.batch, a.num_heads, a.max_kv, weights != nullptr);
+    if (need > 0 && (!workspace || workspace_bytes < need || (uintptr_t)workspace % 256 != 0)) {
+        set_error("%s: workspace of %zu bytes (256-byte aligned) required, got %zu at %p", what,
+                  need, workspace_bytes, workspace);
+        return FLOUR_ERR_WORKSPACE;
+    }
+    a.rows = a.batch;
+    a.q_st = a.o_st = (int64_t)a.num_heads * a.head_dim;
+    a.q_sh = a.o_sh = a.head_dim;
+    if (weights) {
+        a.ml = static_cast<float*>(workspace);
+        a.scores = reinterpret_cast<float*>(
+            static_cast<char*>(workspace) +
+            up256((size_t)a.batch * a.num_heads * 2 * sizeof(float)));
+        a.score_stride = score_stride_of(a.max_kv);
+    }
+    const int rc = launch_attn_pools(a, stream);
+    if (rc != FLOUR_OK || !weights) return rc;
+    return launch_weights_add(weights, width, weight_rows, num_rows, a.kv_lens, a.max_kv, a.batch,
+                              a.kv_heads, a.num_heads / a.kv_heads, a.scores, a.score_stride, a.ml,
+                              stream);
+}
+
+}  // namespace flour
+
+extern "C" int flour_hip_decode_weights_workspace_size(int batch, int num_heads, int kv_heads,
+                                                       int head_dim, int max_context_len,
+                                                       int with_weights, size_t* bytes) {
+    clear_error();
+    if (!bytes || batch < 0 || num_heads <= 0 || kv_heads <= 0 || num_heads % kv_heads != 0 ||
+        head_dim <= 0 || max_context_len < 0) {
+        set_error("decode_weights_workspace_size: bad arguments");
+        return FLOUR_ERR_INVALID_ARGUMENT;
+    }
+    *bytes = decode_pools_ws(batch, num_heads, max_context_len, with_weights != 0);
+    return FLOUR_OK;
+}
+
+extern "C" int flour_hip_paged_decode_q8(
+    void* out, int out_dtype, const void* q, int dtype, const void* k_pool, const void* v_pool,
+    const float* k_scale, const float* v_scale, int pool_dtype, const int32_t* block_tables,
+    int max_blocks_per_seq, const int32_t* context_lens, int batch, int num_heads, int kv_heads,
+    int head_dim, int block_size, int64_t num_slots, int max_context_len, float scale,
+    float* weights, int64_t weights_width, const int32_t* weight_rows, int num_weight_rows,
+    void* workspace, size_t workspace_bytes, void* stream) {
+    clear_error();
+    if (!check_pool8("paged_decode_q8", pool_dtype, k_pool, v_pool, k_scale, v_scale, kv_heads,
+                     head_dim, block_size, num_slots))
+        return FLOUR_ERR_INVALID_ARGUMENT;
+    PoolAttn a{};
+    a.out = out, a.out_dtype = out_dtype, a.q = q, a.dtype = dtype;
+    a.k_pool = k_pool, a.v_pool = v_pool, a.k_scale = k_scale, a.v_scale = v_scale;
+    a.pool_dtype = pool_dtype, a.block_tables = block_tables, a.max_blocks = max_blocks_per_seq;
+    a.kv_lens = context_lens, a.batch = batch, a.num_heads = num_heads, a.kv_heads = kv_heads;
+    a.head_dim = head_dim, a.block_size = block_size, a.num_slots = num_slots;
+    a.max_kv = max_context_len, a.scale = scale;
+    return decode_pools("paged_decode_q8", a, weights, weights_width, weight_rows, num_weight_rows,
+                        workspace, workspace_bytes, static_cast<hipStream_t>(stream));
+}
+
+extern "C" int flour_hip_paged_decode_weights(
+    void* out, int out_dtype, const void* q, const void* k_pool, const void* v_pool,
+    const int32_t* block_tables, int max_blocks_per_seq, const int32_t* context_lens, int batch,
+    int num_heads, int kv_heads, int head_dim, int block_size, int64_t num_slots,
+    int max_context_len, float scale, int dtype, float* weights, int64_t weights_width,
+    const int32_t* weight_rows, int num_weight_rows, void* workspace, size_t workspace_bytes,
+    void* stream) {
+    clear_error();
+    if (!weights) {
+        set_error("paged_decode_weights: null weights");
+        return FLOUR_ERR_INVALID_ARGUMENT;
+    }
+    PoolAttn a{};
+    a.out = out, a.out_dtype = out_dtype, a.q = q, a.dtype = dtype;
+    a.k_pool = k_pool, a.v_pool = v_pool, a.pool_dtype = dtype;
+    a.block_tables = block_tables, a.max_blocks = max_blocks_per_seq;
+    a.kv_lens = context_lens, a.batch = batch, a.num_heads = num_heads, a.kv_heads = kv_heads;
+    a.head_dim = head_dim, a.block_size = block_size, a.num_slots = num_slots;
+    a.max_kv = max_context_len, a.scale = scale;
+    return decode_pools("paged_decode_weights", a, weights, weights_width, weight_rows,
+                        num_weight_rows, workspace, workspace_bytes,
+                        static_cast<hipStream_t>(stream));
+}
+
+extern "C" int flour_hip_varlen_prefill_q8_workspace_size(int num_seqs, int max_seqlen_q,
+                                                          int total_q, int max_kv_len,
+                                                          int num_heads, int kv_heads,
+                                                          int head_dim, int block_size, int dtype,
+                                                          size_t* bytes) {
+    clear_error();
+    if (!bytes || num_seqs < 0 || max_seqlen_q < 0 || total_q < 0 || max_kv_len < 0 ||
+        num_heads <= 0 || kv_heads <= 0 || num_heads % kv_heads != 0 || head_dim <= 0 ||
+        block_size <= 0 || !valid_dtype(dtype)) {
+        set_error("varlen_prefill_q8_workspace_size: bad arguments");
+        return FLOUR_ERR_INVALID_ARGUMENT;
+    }
+    *bytes = 0;
+    return FLOUR_OK;
+}
+
+extern "C" int flour_hip_varlen_prefill_q8(
+    void* out, int out_dtype, int64_t o_stride_tok, int64_t o_stride_head, const void* q,
+    int64_t q_stride_tok, int64_t q_stride_head, int dtype, const void* k_pool, const void* v_pool,
+    const float* k_scale, const float* v_scale, int pool_dtype, const int32_t* cu_seqlens_q,
+    const int32_t* kv_lens, const int32_t* block_tables, int max_blocks_per_seq, int num_seqs,
+    int max_seqlen_q, int total_q, int num_heads, int kv_heads, int head_dim, int block_size,
+    int64_t num_slots, int max_kv_len, float scale, void* workspace, size_t workspace_bytes,
+    void* stream) {
+    clear_error();
+    if (!valid_dtype(dtype) || !valid_dtype(out_dtype)) {
+        set_error("varlen_prefill_q8: unknown dtype (%d, out %d)", dtype, out_dtype);
+        return FLOUR_ERR_INVALID_ARGUMENT;
+    }
+    if (!check_pool8("varlen_prefill_q8", pool_dtype, k_pool, v_pool, k_scale, v_scale, kv_heads,
+                     head_dim, block_size, num_slots))
+        return FLOUR_ERR_INVALID_ARGUMENT;
+    if (num_seqs < 0 || total_q < 0 || max_seqlen_q < 0 || num_heads <= 0 ||
+        num_heads % kv_heads != 0 || max_blocks_per_seq <= 0 || max_kv_len < 0 ||
+        (int64_t)max_kv_len > (int64_t)max_blocks_per_seq * block_size) {
+        set_error("varlen_prefill_q8: bad shape (seqs=%d total_q=%d max_q=%d heads=%d kv_heads=%d "
+                  "max_blocks=%d max_kv=%d)",
+                  num_seqs, total_q, max_seqlen_q, num_heads, kv_heads, max_blocks_per_seq,
+                  max_kv_len);
+        return FLOUR_ERR_INVALID_ARGUMENT;
+    }
+    if (num_seqs == 0 || total_q == 0) return FLOUR_OK;
+    if (!out || !q || !cu_seqlens_q || !kv_lens || !block_tables) {
+        set_error("varlen_prefill_q8: null pointer");
+        return FLOUR_ERR_INVALID_ARGUMENT;
+    }
+    PoolAttn a{};
+    a.out = out, a.out_dtype = out_dtype, a.o_st = o_stride_tok, a.o_sh = o_stride_head;
+    a.q = q, a.dtype = dtype, a.q_st = q_stride_tok, a.q_sh = q_stride_head;
+    a.k_pool = k_pool, a.v_pool = v_pool, a.k_scale = k_scale, a.v_scale = v_scale;
+    a.pool_dtype = pool_dtype, a.cu = cu_seqlens_q, a.kv_lens = kv_lens;
+    a.block_tables = block_tables, a.max_blocks = max_blocks_per_seq, a.batch = num_seqs;
+    a.rows = total_q, a.num_heads = num_heads, a.kv_heads = kv_heads, a.head_dim = head_dim;
+    a.block_size = block_size, a.num_slots = num_slots, a.max_kv = max_kv_len, a.scale = scale;
+    return launch_attn_pools(a, static_cast<hipStream_t>(stream));
+}

@@ -8,6 +8,11 @@ call into libflour_hip.so. Shapes follow the C-ABI (include/flour_hip.h):
 * ``kv_write``        <- PagedKvPool::write (paged.rs:186-204), scatter semantics.
 * ``paged_decode``    <- paged_attention (src/backend/cpu.rs:57-112) for seq_q == 1, batched.
 * ``varlen_prefill``  <- paged_attention for seq_q >= 1, batched over packed sequences.
+
+A cache in 8 bits (``kv_write_q8``, ``kv_dequant``, ``paged_decode_q8``, ``varlen_prefill_q8``) has
+pools of torch.float8_e4m3fn or torch.int8 and fp32 scales (kv_heads, num_blocks);
+``paged_decode_weights`` and ``kv_evict`` sum attention weights and evict by them. These have no
+counterpart in the reference.
 """
 from __future__ import annotations
 
@@ -143,15 +148,20 @@ class Workspace:
     the prefill V staging copy); grows on demand and is reused.
 
     Calls sharing one workspace must not overlap in time (one stream, or explicit ordering).
+    A buffer that a captured graph uses stays with the workspace when it grows.
     """
 
     def __init__(self, device: torch.device | str = "cuda"):
         self.device = torch.device(device)
         self.buf: torch.Tensor | None = None
+        self.captured: list[torch.Tensor] = []
 
     def get(self, nbytes: int) -> torch.Tensor:
         if self.buf is None or self.buf.numel() < nbytes:
             self.buf = torch.empty(max(nbytes, 256), dtype=torch.uint8, device=self.device)
+        if torch.cuda.is_current_stream_capturing() and \
+                not any(self.buf is t for t in self.captured):
+            self.captured.append(self.buf)
         return self.buf
 
 
@@ -296,3 +306,327 @@ def _check_block_size(num_slots: int, block_size: int) -> None:
     if block_size <= 0 or num_slots % block_size != 0:
         raise _lib.FlourError(_lib.ERR_INVALID_ARGUMENT,
                               f"num_slots {num_slots} is not a multiple of block_size {block_size}")
+
+
+# ------------------------------------------------------------------ caches kept small
+# 8-bit pools (an element stands for itself times its (kv head, block)'s scale) and eviction by
+# accumulated attention weight. These run on the tensors' own device, on its current stream.
+_POOL_DT = {torch.float8_e4m3fn: _lib.E4M3, torch.int8: _lib.I8}
+
+
+def _invalid(msg: str) -> _lib.FlourError:
+    return _lib.FlourError(_lib.ERR_INVALID_ARGUMENT, msg)
+
+
+def _same_device(first: torch.Tensor, *rest: torch.Tensor | None) -> None:
+    dev = first.device
+    for t in (first, *rest):
+        if t is not None and not t.is_cuda:
+            raise _invalid("flour_amd ops take device tensors (got a CPU tensor)")
+        if t is not None and t.device != dev:
+            raise _invalid(f"tensors on {dev} and {t.device}")
+
+
+def _launch(fn, device: torch.device, *args) -> None:
+    """fn(*args, stream) on the device's current stream."""
+    if device.index == torch.cuda.current_device():
+        check(fn(*args, ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)))
+        return
+    with torch.cuda.device(device):
+        check(fn(*args, ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)))
+
+
+def _table(t: torch.Tensor, rows: int, what: str) -> None:
+    if t.dim() != 2 or t.shape[0] != rows:
+        raise _invalid(f"{what} must be (sequences, blocks), got {tuple(t.shape)} for {rows}")
+
+
+def _lens(t: torch.Tensor, n: int, what: str) -> None:
+    if t.dim() != 1 or t.shape[0] != n:
+        raise _invalid(f"{what} must hold {n} lengths, got {tuple(t.shape)}")
+
+
+def _pools(k_pool: torch.Tensor, v_pool: torch.Tensor, block_size: int,
+           what: str = "pools") -> tuple[int, int, int]:
+    if k_pool.dim() != 3 or v_pool.shape != k_pool.shape or v_pool.dtype != k_pool.dtype or \
+            not k_pool.is_contiguous() or not v_pool.is_contiguous():
+        raise _invalid(f"{what} must be contiguous (kv_heads, num_slots, head_dim) of one dtype")
+    _check_block_size(k_pool.shape[1], block_size)
+    return k_pool.shape
+
+
+def _pools8(k_pool: torch.Tensor, v_pool: torch.Tensor, k_scale: torch.Tensor,
+            v_scale: torch.Tensor, block_size: int) -> tuple[int, int, int, int]:
+    """(dtype code, kv_heads, num_slots, head_dim) of an 8-bit cache's pools."""
+    G, slots, D = _pools(k_pool, v_pool, block_size)
+    code = _POOL_DT.get(k_pool.dtype)
+    if code is None:
+        raise _invalid(f"8-bit pools are torch.float8_e4m3fn or torch.int8, not {k_pool.dtype}")
+    for t in (k_scale, v_scale):
+        if t is None or t.dtype != torch.float32 or t.shape != (G, slots // block_size) or \
+                not t.is_contiguous():
+            raise _invalid(f"scales must be contiguous fp32 (kv_heads, num_blocks) = "
+                           f"{(G, slots // block_size)}")
+    return code, G, slots, D
+
+
+def _out(out: torch.Tensor | None, shape, dtype: torch.dtype, device) -> torch.Tensor:
+    if out is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    if out.shape != shape or out.device != device:
+        raise _invalid(f"out must be {tuple(shape)} on {device}")
+    return out
+
+
+def _weights_args(weights: torch.Tensor | None, weight_rows: torch.Tensor | None, kv_heads: int,
+                  batch: int, max_len: int, what: str = "weights") -> tuple:
+    """(pointer, width, row pointer, rows) of the sums of attention weights."""
+    if weights is None:
+        if weight_rows is not None:
+            raise _invalid("weight_rows without weights")
+        return _ptr(None), 0, _ptr(None), 0
+    if weights.dtype != torch.float32 or weights.dim() != 3 or weights.shape[1] != kv_heads or \
+            not weights.is_contiguous() or weights.shape[2] < max_len:
+        raise _invalid(f"{what} must be contiguous fp32 (rows, {kv_heads} kv heads, positions >= "
+                       f"{max_len}), got {tuple(weights.shape)} {weights.dtype}")
+    if weight_rows is not None:
+        _need_i32(weight_rows)
+        _lens(weight_rows, batch, "weight_rows")
+    elif weights.shape[0] < batch:
+        raise _invalid(f"{what} has {weights.shape[0]} rows for {batch} sequences")
+    return _ptr(weights), weights.shape[2], _ptr(weight_rows), weights.shape[0]
+
+
+def kv_write_q8(k: torch.Tensor, v: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
+                k_scale: torch.Tensor, v_scale: torch.Tensor, cu_seqlens_q: torch.Tensor,
+                kv_lens: torch.Tensor, block_tables: torch.Tensor, block_size: int = 16) -> None:
+    """Quantises new K/V rows into the blocks of an 8-bit cache.
+
+    ``k``/``v`` are (num_tokens, kv_heads, head_dim) of f32, bf16 or f16 with a unit last stride;
+    sequence s brings rows cu_seqlens_q[s]:cu_seqlens_q[s+1] as its positions up to kv_lens[s].
+    Each written block's scale becomes the smallest power of two with which its new rows and the
+    rows it holds of the sequence from before fit the 8-bit type (those are requantised if it
+    grows); a non-finite row gives NaN. A block written by one call belongs to one sequence of it.
+    """
+    _same_device(k, v, k_pool, v_pool, k_scale, v_scale, cu_seqlens_q, kv_lens, block_tables)
+    _need_i32(cu_seqlens_q, kv_lens, block_tables)
+    code, G, slots, D = _pools8(k_pool, v_pool, k_scale, v_scale, block_size)
+    if k.dim() != 3 or k.shape[1:] != (G, D) or v.shape != k.shape or v.stride() != k.stride() or \
+            v.dtype != k.dtype or k.stride(2) != 1:
+        raise _invalid("k/v must be (num_tokens, kv_heads, head_dim) sharing dtype and strides, "
+                       "unit last stride")
+    n = cu_seqlens_q.numel() - 1
+    _lens(kv_lens, n, "kv_lens")
+    _table(block_tables, n, "block_tables")
+    _launch(lib().flour_hip_kv_write_q8, k.device, _ptr(k), _ptr(v), k.stride(0), k.stride(1),
+            dtype_code(k.dtype), _ptr(k_pool), _ptr(v_pool), _ptr(k_scale), _ptr(v_scale), code,
+            _ptr(cu_seqlens_q), _ptr(kv_lens), _ptr(block_tables), block_tables.shape[1], n,
+            k.shape[0], G, D, block_size, slots)
+
+
+def kv_dequant(k_pool: torch.Tensor, v_pool: torch.Tensor, k_scale: torch.Tensor,
+               v_scale: torch.Tensor, block_tables: torch.Tensor, kv_lens: torch.Tensor,
+               k_out: torch.Tensor, v_out: torch.Tensor, out_tables: torch.Tensor,
+               max_kv_len: int, block_size: int = 16) -> None:
+    """The values of sequences in an 8-bit cache, into the blocks that ``out_tables`` gives them in
+    the plain pools ``k_out``/``v_out`` (kv_heads, out_slots, head_dim) of f32, bf16 or f16.
+    ``max_kv_len`` bounds kv_lens."""
+    _same_device(k_pool, v_pool, k_scale, v_scale, block_tables, kv_lens, k_out, v_out, out_tables)
+    _need_i32(block_tables, kv_lens, out_tables)
+    code, G, slots, D = _pools8(k_pool, v_pool, k_scale, v_scale, block_size)
+    Go, out_slots, Do = _pools(k_out, v_out, block_size, "k_out and v_out")
+    if (Go, Do) != (G, D):
+        raise _invalid("k_out and v_out must have the cache's kv_heads and head_dim")
+    n = kv_lens.numel()
+    _table(block_tables, n, "block_tables")
+    _table(out_tables, n, "out_tables")
+    _launch(lib().flour_hip_kv_dequant, k_pool.device, _ptr(k_out), _ptr(v_out),
+            dtype_code(k_out.dtype), _ptr(out_tables), out_tables.shape[1], out_slots,
+            _ptr(k_pool), _ptr(v_pool), _ptr(k_scale), _ptr(v_scale), code, _ptr(block_tables),
+            block_tables.shape[1], _ptr(kv_lens), n, max_kv_len, G, D, block_size, slots)
+
+
+def decode_weights_workspace_bytes(batch: int, num_heads: int, kv_heads: int, head_dim: int,
+                                   max_context_len: int, with_weights: bool) -> int:
+    """Bytes of workspace of paged_decode_q8 and paged_decode_weights."""
+    n = ctypes.c_size_t(0)
+    check(lib().flour_hip_decode_weights_workspace_size(batch, num_heads, kv_heads, head_dim,
+                                                        max_context_len, int(with_weights),
+                                                        ctypes.byref(n)))
+    return n.value
+
+
+def _scratch(workspace: Workspace | None, nbytes: int, device: torch.device) -> torch.Tensor:
+    # Without a caller's workspace each call has scratch of its own, in its stream's order.
+    if workspace is None:
+        return torch.empty(max(nbytes, 256), dtype=torch.uint8, device=device)
+    ws = workspace.get(nbytes)
+    if ws.device != device:
+        raise _invalid(f"workspace on {ws.device}, tensors on {device}")
+    return ws
+
+
+def _decode_q(q: torch.Tensor, D: int, G: int) -> tuple[int, int]:
+    if q.dim() != 3 or q.shape[2] != D or not q.is_contiguous() or q.shape[1] == 0 or \
+            q.shape[1] % G != 0:
+        raise _invalid("q must be contiguous (batch, num_heads, head_dim), num_heads a multiple "
+                       "of the pools' kv_heads")
+    return q.shape[0], q.shape[1]
+
+
+def paged_decode_q8(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
+                    k_scale: torch.Tensor, v_scale: torch.Tensor, block_tables: torch.Tensor,
+                    context_lens: torch.Tensor, scale: float, max_context_len: int,
+                    block_size: int = 16, out_dtype: torch.dtype | None = None,
+                    out: torch.Tensor | None = None, workspace: Workspace | None = None,
+                    weights: torch.Tensor | None = None,
+                    weight_rows: torch.Tensor | None = None) -> torch.Tensor:
+    """paged_decode over an 8-bit cache: q (batch, num_heads, head_dim) of f32, bf16 or f16. With
+    ``weights`` the step's attention weights are added to it, as paged_decode_weights does."""
+    _same_device(q, k_pool, v_pool, k_scale, v_scale, block_tables, context_lens, out, weights,
+                 weight_rows)
+    _need_i32(block_tables, context_lens)
+    code, G, slots, D = _pools8(k_pool, v_pool, k_scale, v_scale, block_size)
+    B, H = _decode_q(q, D, G)
+    _lens(context_lens, B, "context_lens")
+    _table(block_tables, B, "block_tables")
+    wargs = _weights_args(weights, weight_rows, G, B, max_context_len)
+    out = _out(out, q.shape, out_dtype or q.dtype, q.device)
+    if not out.is_contiguous():
+        raise _invalid("out must be contiguous")
+    ws = _scratch(workspace, decode_weights_workspace_bytes(B, H, G, D, max_context_len,
+                                                            weights is not None), q.device)
+    _launch(lib().flour_hip_paged_decode_q8, q.device, _ptr(out), dtype_code(out.dtype), _ptr(q),
+            dtype_code(q.dtype), _ptr(k_pool), _ptr(v_pool), _ptr(k_scale), _ptr(v_scale), code,
+            _ptr(block_tables), block_tables.shape[1], _ptr(context_lens), B, H, G, D, block_size,
+            slots, max_context_len, float(scale), *wargs, _ptr(ws), ws.numel())
+    return out
+
+
+def paged_decode_weights(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
+                         block_tables: torch.Tensor, context_lens: torch.Tensor, scale: float,
+                         max_context_len: int, weights: torch.Tensor, block_size: int = 16,
+                         out_dtype: torch.dtype | None = None, out: torch.Tensor | None = None,
+                         workspace: Workspace | None = None,
+                         weight_rows: torch.Tensor | None = None) -> torch.Tensor:
+    """paged_decode that also adds the step's attention weights to ``weights``, fp32 (rows,
+    kv_heads, positions): weights[r, g, j] += the sum over kv head g's query heads of their softmax
+    weight on position j, r = weight_rows[b] or b. Rows of one call must differ; one outside the
+    tensor adds nothing."""
+    _same_device(q, k_pool, v_pool, block_tables, context_lens, out, weights, weight_rows)
+    _need_i32(block_tables, context_lens)
+    G, slots, D = _pools(k_pool, v_pool, block_size)
+    B, H = _decode_q(q, D, G)
+    if q.dtype != k_pool.dtype:
+        raise _invalid("q and pools must share a dtype")
+    if weights is None:
+        raise _invalid("paged_decode_weights needs weights")
+    _lens(context_lens, B, "context_lens")
+    _table(block_tables, B, "block_tables")
+    wargs = _weights_args(weights, weight_rows, G, B, max_context_len)
+    out = _out(out, q.shape, out_dtype or q.dtype, q.device)
+    if not out.is_contiguous():
+        raise _invalid("out must be contiguous")
+    ws = _scratch(workspace, decode_weights_workspace_bytes(B, H, G, D, max_context_len, True),
+                  q.device)
+    _launch(lib().flour_hip_paged_decode_weights, q.device, _ptr(out), dtype_code(out.dtype),
+            _ptr(q), _ptr(k_pool), _ptr(v_pool), _ptr(block_tables), block_tables.shape[1],
+            _ptr(context_lens), B, H, G, D, block_size, slots, max_context_len, float(scale),
+            dtype_code(q.dtype), *wargs, _ptr(ws), ws.numel())
+    return out
+
+
+def prefill_q8_workspace_bytes(num_seqs: int, max_seqlen_q: int, total_q: int, max_kv_len: int,
+                               num_heads: int, kv_heads: int, head_dim: int, block_size: int,
+                               dtype: torch.dtype) -> int:
+    """Bytes of workspace of varlen_prefill_q8."""
+    n = ctypes.c_size_t(0)
+    check(lib().flour_hip_varlen_prefill_q8_workspace_size(
+        num_seqs, max_seqlen_q, total_q, max_kv_len, num_heads, kv_heads, head_dim, block_size,
+        dtype_code(dtype), ctypes.byref(n)))
+    return n.value
+
+
+def varlen_prefill_q8(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
+                      k_scale: torch.Tensor, v_scale: torch.Tensor, cu_seqlens_q: torch.Tensor,
+                      kv_lens: torch.Tensor, block_tables: torch.Tensor, max_seqlen_q: int,
+                      max_kv_len: int, scale: float, block_size: int = 16,
+                      out_dtype: torch.dtype | None = None, out: torch.Tensor | None = None,
+                      workspace: Workspace | None = None) -> torch.Tensor:
+    """varlen_prefill over an 8-bit cache that already holds the rows' K/V (kv_write_q8): packed q
+    (total_q, num_heads, head_dim), any view with a unit last stride. ``max_seqlen_q`` bounds the
+    rows of a sequence, ``max_kv_len`` kv_lens."""
+    _same_device(q, k_pool, v_pool, k_scale, v_scale, cu_seqlens_q, kv_lens, block_tables, out)
+    _need_i32(cu_seqlens_q, kv_lens, block_tables)
+    code, G, slots, D = _pools8(k_pool, v_pool, k_scale, v_scale, block_size)
+    if q.dim() != 3 or q.shape[2] != D or q.stride(2) != 1 or q.shape[1] == 0 or \
+            q.shape[1] % G != 0:
+        raise _invalid("q must be (total_q, num_heads, head_dim) with a unit last stride, "
+                       "num_heads a multiple of the pools' kv_heads")
+    T, H, _ = q.shape
+    n = cu_seqlens_q.numel() - 1
+    _lens(kv_lens, n, "kv_lens")
+    _table(block_tables, n, "block_tables")
+    out = _out(out, q.shape, out_dtype or q.dtype, q.device)
+    if out.stride(2) != 1:
+        raise _invalid("out must have a unit last stride")
+    ws = _scratch(workspace, prefill_q8_workspace_bytes(n, max_seqlen_q, T, max_kv_len, H, G, D,
+                                                        block_size, q.dtype), q.device)
+    _launch(lib().flour_hip_varlen_prefill_q8, q.device, _ptr(out), dtype_code(out.dtype),
+            out.stride(0), out.stride(1), _ptr(q), q.stride(0), q.stride(1), dtype_code(q.dtype),
+            _ptr(k_pool), _ptr(v_pool), _ptr(k_scale), _ptr(v_scale), code, _ptr(cu_seqlens_q),
+            _ptr(kv_lens), _ptr(block_tables), block_tables.shape[1], n, max_seqlen_q, T, H, G, D,
+            block_size, slots, max_kv_len, float(scale), _ptr(ws), ws.numel())
+    return out
+
+
+def kv_evict(k_pool: torch.Tensor, v_pool: torch.Tensor, weights: torch.Tensor,
+             block_tables: torch.Tensor, context_lens: torch.Tensor, keep_lens: torch.Tensor,
+             out_tables: torch.Tensor, max_context_len: int, max_keep_len: int, recent: int = 0,
+             block_size: int = 16, k_scale: torch.Tensor | None = None,
+             v_scale: torch.Tensor | None = None, weights_out: torch.Tensor | None = None,
+             weight_rows: torch.Tensor | None = None,
+             kept: torch.Tensor | None = None) -> torch.Tensor:
+    """Gathers, for every sequence and kv head, the ``recent`` latest positions and the heaviest
+    of the others by ``weights`` (rows, kv_heads, positions) into the blocks of ``out_tables``:
+    n = min(keep_lens[b], context_lens[b]) in all, in their order, ties to the lower position.
+    ``weights_out`` (default: ``weights`` itself) takes the kept positions' sums in front, zeros up
+    to the old length behind. Pools are plain, or 8-bit with ``k_scale``/``v_scale``. Destination
+    blocks must be new: in no sequence of the call and not twice among themselves.
+
+    Returns the kept positions (batch, kv_heads, max_keep_len) int32, -1 behind the n-th.
+    """
+    _same_device(k_pool, v_pool, weights, block_tables, context_lens, keep_lens, out_tables,
+                 k_scale, v_scale, weights_out, weight_rows, kept)
+    _need_i32(block_tables, context_lens, keep_lens, out_tables)
+    if k_pool.dtype in _POOL_DT:
+        code, G, slots, D = _pools8(k_pool, v_pool, k_scale, v_scale, block_size)
+    else:
+        G, slots, D = _pools(k_pool, v_pool, block_size)
+        code = dtype_code(k_pool.dtype)
+        if k_scale is not None or v_scale is not None:
+            raise _invalid("scales go with 8-bit pools")
+    B = context_lens.numel()
+    _lens(context_lens, B, "context_lens")
+    _lens(keep_lens, B, "keep_lens")
+    _table(block_tables, B, "block_tables")
+    _table(out_tables, B, "out_tables")
+    w, width, rows, n_rows = _weights_args(weights, weight_rows, G, B, max_context_len)
+    if weights_out is None:
+        weights_out = weights
+    elif weights_out.shape != weights.shape or weights_out.dtype != torch.float32 or \
+            not weights_out.is_contiguous():
+        raise _invalid("weights_out must be contiguous fp32 of the shape of weights")
+    shape = (B, G, max(max_keep_len, 0))
+    if kept is None:
+        kept = torch.empty(shape, dtype=torch.int32, device=k_pool.device)
+    else:
+        _need_i32(kept)
+        if kept.shape != shape:
+            raise _invalid(f"kept must be {shape}")
+    _launch(lib().flour_hip_kv_evict, k_pool.device, _ptr(k_pool), _ptr(v_pool), _ptr(k_scale),
+            _ptr(v_scale), code, w, _ptr(weights_out), width, rows, n_rows, _ptr(block_tables),
+            block_tables.shape[1], _ptr(context_lens), _ptr(keep_lens), _ptr(out_tables),
+            out_tables.shape[1], _ptr(kept), B, G, D, block_size, slots, max_context_len,
+            max_keep_len, recent)
+    return kept

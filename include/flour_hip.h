@@ -46,6 +46,9 @@ enum flour_dtype {
     FLOUR_DTYPE_F32 = 0,
     FLOUR_DTYPE_BF16 = 1,
     FLOUR_DTYPE_F16 = 2,
+    /* elements of the 8-bit pools (the functions that take a pool_dtype; no others) */
+    FLOUR_DTYPE_E4M3 = 3, /* OCP e4m3: 448 the largest, no infinities */
+    FLOUR_DTYPE_I8 = 4,   /* two's complement, -127 .. 127 */
 };
 
 #define FLOUR_OK 0
@@ -223,6 +226,135 @@ int flour_hip_varlen_prefill_ws(void* out, int out_dtype, int64_t o_stride_tok,
                                 int kv_heads, int head_dim, int block_size, int64_t num_slots,
                                 float scale, int dtype, void* workspace, size_t workspace_bytes,
                                 void* stream);
+
+/* ------------------------------------------------------------------------------------------
+ * 8-bit KV pools. The reference keeps K/V in the model's dtype only; these functions have no
+ * counterpart there. A pool of one layer is K and V, (kv_heads, num_slots, head_dim) in
+ * pool_dtype (FLOUR_DTYPE_E4M3 or FLOUR_DTYPE_I8), with k_scale and v_scale, fp32 (kv_heads,
+ * num_slots / block_size): an element of block b and kv head h stands for itself times
+ * scale[h, b]. Tables, lengths, slots and q / out are those of the plain pools.
+ *
+ * Functions that read a pool take any scale that is not negative. Those that write one
+ * (flour_hip_kv_write_q8, flour_hip_kv_evict) store powers of two: the smallest S >= 2^-126 with
+ * which no element exceeds 448 (e4m3) or 127 (int8) times S, 0 for a block of zeros. A block that
+ * takes an infinity or a NaN gets the scale NaN: whoever attends to one of its positions reads
+ * NaN, until the block is started again.
+ * ---------------------------------------------------------------------------------------- */
+
+/* New rows into an 8-bit cache. As in flour_hip_varlen_prefill, sequence s brings the packed rows
+ * cu_seqlens_q[s] .. cu_seqlens_q[s+1]-1, its positions kv_lens[s] - q_len .. kv_lens[s]-1; row t,
+ * head h of k and v at t*stride_tok + h*stride_head (elements), in `dtype`. total_q =
+ * cu_seqlens_q[num_seqs].
+ * A block that the call writes gets the scale max(S_kept, S_new): S_kept the stored scale if the
+ * block holds positions of the sequence from before the call (0 otherwise, whatever the block
+ * held), S_new the one the new rows need. Rows kept from before are requantised where that is
+ * larger than their scale; new rows are rounded once, to nearest even. Rows of a block behind the
+ * sequence's last position keep their bits.
+ * Nothing is written for a sequence with kv_len < q_len, for positions past the table, or to blocks
+ * whose id lies outside the pool. Several sequences may share blocks that the call only keeps
+ * whole; a block that it writes must belong to one sequence of the call. */
+int flour_hip_kv_write_q8(const void* k, const void* v, int64_t stride_tok, int64_t stride_head,
+                          int dtype, void* k_pool, void* v_pool, float* k_scale, float* v_scale,
+                          int pool_dtype, const int32_t* cu_seqlens_q, const int32_t* kv_lens,
+                          const int32_t* block_tables, int max_blocks_per_seq, int num_seqs,
+                          int total_q, int kv_heads, int head_dim, int block_size,
+                          int64_t num_slots, void* stream);
+
+/* The way back: positions 0 .. kv_lens[s]-1 of each sequence as the values they stand for, rounded
+ * to `dtype` (f16: values beyond its largest number become that number), into the slots of a plain
+ * pool (kv_heads, out_slots, head_dim) that out_tables gives them; other slots are left as they
+ * are. max_kv_len bounds kv_lens (a longer sequence is read up to it). Ids of block_tables outside
+ * the pool read a block inside it, as in attention; ids of out_tables outside theirs are skipped. */
+int flour_hip_kv_dequant(void* k_out, void* v_out, int dtype, const int32_t* out_tables,
+                         int out_max_blocks, int64_t out_slots, const void* k_pool,
+                         const void* v_pool, const float* k_scale, const float* v_scale,
+                         int pool_dtype, const int32_t* block_tables, int max_blocks_per_seq,
+                         const int32_t* kv_lens, int num_seqs, int max_kv_len, int kv_heads,
+                         int head_dim, int block_size, int64_t num_slots, void* stream);
+
+/* flour_hip_paged_decode over an 8-bit cache: q in `dtype` (f32, bf16 or f16), the products and
+ * sums as there. `weights` (NULL for none) is described at flour_hip_paged_decode_weights.
+ * A workspace of flour_hip_decode_weights_workspace_size bytes is required. */
+int flour_hip_paged_decode_q8(void* out, int out_dtype, const void* q, int dtype,
+                              const void* k_pool, const void* v_pool, const float* k_scale,
+                              const float* v_scale, int pool_dtype, const int32_t* block_tables,
+                              int max_blocks_per_seq, const int32_t* context_lens, int batch,
+                              int num_heads, int kv_heads, int head_dim, int block_size,
+                              int64_t num_slots, int max_context_len, float scale, float* weights,
+                              int64_t weights_width, const int32_t* weight_rows,
+                              int num_weight_rows, void* workspace, size_t workspace_bytes,
+                              void* stream);
+
+/* flour_hip_paged_decode over a plain pool that also adds the step's attention weights to a sum
+ * per cached position, what an eviction goes by:
+ *     weights[r, g, j] += sum over the query heads of kv head g of softmax weight (head, j)
+ * for the sequence's positions j < context_len, r = weight_rows[b] (b itself if weight_rows is
+ * NULL). weights is fp32 (num_weight_rows, kv_heads, weights_width) contiguous, weights_width >=
+ * max_context_len. Entries of one call must have different rows; one whose row lies outside
+ * [0, num_weight_rows) adds nothing (its attention is computed all the same).
+ * A workspace of flour_hip_decode_weights_workspace_size bytes (256-byte aligned, no
+ * initialisation needed) is required; calls that share one must not overlap in time. */
+int flour_hip_paged_decode_weights(void* out, int out_dtype, const void* q, const void* k_pool,
+                                   const void* v_pool, const int32_t* block_tables,
+                                   int max_blocks_per_seq, const int32_t* context_lens, int batch,
+                                   int num_heads, int kv_heads, int head_dim, int block_size,
+                                   int64_t num_slots, int max_context_len, float scale, int dtype,
+                                   float* weights, int64_t weights_width,
+                                   const int32_t* weight_rows, int num_weight_rows,
+                                   void* workspace, size_t workspace_bytes, void* stream);
+
+/* Workspace of the two functions above; with_weights != 0 where `weights` is given. */
+int flour_hip_decode_weights_workspace_size(int batch, int num_heads, int kv_heads, int head_dim,
+                                            int max_context_len, int with_weights, size_t* bytes);
+
+/* flour_hip_varlen_prefill over an 8-bit cache, whose new rows flour_hip_kv_write_q8 has written:
+ * every row attends to the quantised values, its own among them. max_kv_len bounds kv_lens (a
+ * longer sequence is taken to end there). A workspace of
+ * flour_hip_varlen_prefill_q8_workspace_size bytes (256-byte aligned, no initialisation needed)
+ * is required; calls that share one must not overlap in time. */
+int flour_hip_varlen_prefill_q8(void* out, int out_dtype, int64_t o_stride_tok,
+                                int64_t o_stride_head, const void* q, int64_t q_stride_tok,
+                                int64_t q_stride_head, int dtype, const void* k_pool,
+                                const void* v_pool, const float* k_scale, const float* v_scale,
+                                int pool_dtype, const int32_t* cu_seqlens_q,
+                                const int32_t* kv_lens, const int32_t* block_tables,
+                                int max_blocks_per_seq, int num_seqs, int max_seqlen_q,
+                                int total_q, int num_heads, int kv_heads, int head_dim,
+                                int block_size, int64_t num_slots, int max_kv_len, float scale,
+                                void* workspace, size_t workspace_bytes, void* stream);
+
+int flour_hip_varlen_prefill_q8_workspace_size(int num_seqs, int max_seqlen_q, int total_q,
+                                               int max_kv_len, int num_heads, int kv_heads,
+                                               int head_dim, int block_size, int dtype,
+                                               size_t* bytes);
+
+/* ------------------------------------------------------------------------------------------
+ * Eviction by accumulated attention weight (no counterpart in the reference). Of sequence b's L =
+ * context_lens[b] positions each kv head keeps n = min(keep_lens[b], L) of its own: the last
+ * min(recent, n), and of the others those with the largest weights[r, g, .], ties to the lower
+ * position, NaN below every number. In their order, the kept rows of K and V go to the slots that
+ * out_tables gives positions 0 .. n-1; keys keep the rotation of their old positions.
+ * Blocks of out_tables must not be among any block_tables of the call, nor twice among their own;
+ * rows of a destination block behind position n-1 keep their bits. The old blocks are not written: shared prefix
+ * blocks may be evicted from.
+ *   weights      fp32 (num_weight_rows, kv_heads, weights_width), r = weight_rows[b] (b if NULL;
+ *                outside [0, num_weight_rows): the entry is skipped, its kept row is all -1)
+ *   weights_out  same shape, or weights itself: [r, g, i] = the i-th kept position's sum for i < n
+ *                and 0 for n <= i < L; the rest is left as it is
+ *   kept         [batch, kv_heads, max_keep_len]: the kept positions, -1 behind the n-th
+ * Plain pools (pool_dtype f32, bf16 or f16; k_scale = v_scale = NULL) are copied bit for bit. Over
+ * an 8-bit pool each destination block gets a scale of its own from the kept values, which are
+ * rounded once more where it differs from theirs.
+ * max_context_len bounds context_lens, max_keep_len keep_lens (larger ones are clamped).
+ * ---------------------------------------------------------------------------------------- */
+int flour_hip_kv_evict(void* k_pool, void* v_pool, float* k_scale, float* v_scale, int pool_dtype,
+                       const float* weights, float* weights_out, int64_t weights_width,
+                       const int32_t* weight_rows, int num_weight_rows,
+                       const int32_t* block_tables, int max_blocks_per_seq,
+                       const int32_t* context_lens, const int32_t* keep_lens,
+                       const int32_t* out_tables, int out_max_blocks, int32_t* kept, int batch,
+                       int kv_heads, int head_dim, int block_size, int64_t num_slots,
+                       int max_context_len, int max_keep_len, int recent, void* stream);
 
 #ifdef __cplusplus
 }

@@ -18,6 +18,9 @@ use std::os::raw::{c_char, c_int, c_void};
 pub const FLOUR_DTYPE_F32: c_int = 0;
 pub const FLOUR_DTYPE_BF16: c_int = 1;
 pub const FLOUR_DTYPE_F16: c_int = 2;
+/// Elements of the 8-bit pools (`pool_dtype` arguments only).
+pub const FLOUR_DTYPE_E4M3: c_int = 3;
+pub const FLOUR_DTYPE_I8: c_int = 4;
 
 pub const FLOUR_OK: c_int = 0;
 pub const FLOUR_ERR_INVALID_ARGUMENT: c_int = -1;
@@ -91,6 +94,53 @@ extern "C" {
         max_seqlen_q: c_int, total_q: c_int, num_heads: c_int, kv_heads: c_int, head_dim: c_int,
         block_size: c_int, num_slots: i64, scale: f32, dtype: c_int, workspace: *mut c_void,
         workspace_bytes: usize, stream: *mut c_void) -> c_int;
+    pub fn flour_hip_kv_write_q8(k: *const c_void, v: *const c_void, stride_tok: i64,
+        stride_head: i64, dtype: c_int, k_pool: *mut c_void, v_pool: *mut c_void,
+        k_scale: *mut f32, v_scale: *mut f32, pool_dtype: c_int, cu_seqlens_q: *const i32,
+        kv_lens: *const i32, block_tables: *const i32, max_blocks_per_seq: c_int, num_seqs: c_int,
+        total_q: c_int, kv_heads: c_int, head_dim: c_int, block_size: c_int, num_slots: i64,
+        stream: *mut c_void) -> c_int;
+    pub fn flour_hip_kv_dequant(k_out: *mut c_void, v_out: *mut c_void, dtype: c_int,
+        out_tables: *const i32, out_max_blocks: c_int, out_slots: i64, k_pool: *const c_void,
+        v_pool: *const c_void, k_scale: *const f32, v_scale: *const f32, pool_dtype: c_int,
+        block_tables: *const i32, max_blocks_per_seq: c_int, kv_lens: *const i32, num_seqs: c_int,
+        max_kv_len: c_int, kv_heads: c_int, head_dim: c_int, block_size: c_int, num_slots: i64,
+        stream: *mut c_void) -> c_int;
+    pub fn flour_hip_paged_decode_q8(out: *mut c_void, out_dtype: c_int, q: *const c_void,
+        dtype: c_int, k_pool: *const c_void, v_pool: *const c_void, k_scale: *const f32,
+        v_scale: *const f32, pool_dtype: c_int, block_tables: *const i32,
+        max_blocks_per_seq: c_int, context_lens: *const i32, batch: c_int, num_heads: c_int,
+        kv_heads: c_int, head_dim: c_int, block_size: c_int, num_slots: i64,
+        max_context_len: c_int, scale: f32, weights: *mut f32, weights_width: i64,
+        weight_rows: *const i32, num_weight_rows: c_int, workspace: *mut c_void,
+        workspace_bytes: usize, stream: *mut c_void) -> c_int;
+    pub fn flour_hip_paged_decode_weights(out: *mut c_void, out_dtype: c_int, q: *const c_void,
+        k_pool: *const c_void, v_pool: *const c_void, block_tables: *const i32,
+        max_blocks_per_seq: c_int, context_lens: *const i32, batch: c_int, num_heads: c_int,
+        kv_heads: c_int, head_dim: c_int, block_size: c_int, num_slots: i64,
+        max_context_len: c_int, scale: f32, dtype: c_int, weights: *mut f32, weights_width: i64,
+        weight_rows: *const i32, num_weight_rows: c_int, workspace: *mut c_void,
+        workspace_bytes: usize, stream: *mut c_void) -> c_int;
+    pub fn flour_hip_decode_weights_workspace_size(batch: c_int, num_heads: c_int, kv_heads: c_int,
+        head_dim: c_int, max_context_len: c_int, with_weights: c_int, bytes: *mut usize) -> c_int;
+    pub fn flour_hip_varlen_prefill_q8(out: *mut c_void, out_dtype: c_int, o_stride_tok: i64,
+        o_stride_head: i64, q: *const c_void, q_stride_tok: i64, q_stride_head: i64, dtype: c_int,
+        k_pool: *const c_void, v_pool: *const c_void, k_scale: *const f32, v_scale: *const f32,
+        pool_dtype: c_int, cu_seqlens_q: *const i32, kv_lens: *const i32, block_tables: *const i32,
+        max_blocks_per_seq: c_int, num_seqs: c_int, max_seqlen_q: c_int, total_q: c_int,
+        num_heads: c_int, kv_heads: c_int, head_dim: c_int, block_size: c_int, num_slots: i64,
+        max_kv_len: c_int, scale: f32, workspace: *mut c_void, workspace_bytes: usize,
+        stream: *mut c_void) -> c_int;
+    pub fn flour_hip_varlen_prefill_q8_workspace_size(num_seqs: c_int, max_seqlen_q: c_int,
+        total_q: c_int, max_kv_len: c_int, num_heads: c_int, kv_heads: c_int, head_dim: c_int,
+        block_size: c_int, dtype: c_int, bytes: *mut usize) -> c_int;
+    pub fn flour_hip_kv_evict(k_pool: *mut c_void, v_pool: *mut c_void, k_scale: *mut f32,
+        v_scale: *mut f32, pool_dtype: c_int, weights: *const f32, weights_out: *mut f32,
+        weights_width: i64, weight_rows: *const i32, num_weight_rows: c_int,
+        block_tables: *const i32, max_blocks_per_seq: c_int, context_lens: *const i32,
+        keep_lens: *const i32, out_tables: *const i32, out_max_blocks: c_int, kept: *mut i32,
+        batch: c_int, kv_heads: c_int, head_dim: c_int, block_size: c_int, num_slots: i64,
+        max_context_len: c_int, max_keep_len: c_int, recent: c_int, stream: *mut c_void) -> c_int;
 }
 
 // include/flour_cache.h

@@ -1,0 +1,569 @@
+"""The 8-bit cache on the GPU: the quantising write and the way back bit for bit, decode, prefill and
+the sums of attention weights within the bounds of fp32 arithmetic, against tests/_cache8.py."""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+from _cache8 import Cache, attend, close, values
+from flour_amd import ops
+from flour_amd._lib import ERR_INVALID_ARGUMENT, ERR_UNSUPPORTED, FlourError
+
+pytestmark = pytest.mark.gpu
+
+E, I = torch.float8_e4m3fn, torch.int8
+BF, HF, F = torch.bfloat16, torch.float16, torch.float32
+
+
+def i32(x, device):
+    return torch.tensor(x, dtype=torch.int32, device=device)
+
+
+def tables(lens, bs, blocks, gen, extra=0):
+    """Disjoint random tables of sequences of `lens` positions, padded with ids outside the pool."""
+    perm = torch.randperm(blocks, generator=gen).tolist()
+    width = max((n + bs - 1) // bs for n in lens) + extra
+    rows, at = [], 0
+    for n in lens:
+        nb = (n + bs - 1) // bs
+        rows.append(perm[at:at + nb] + [2 ** 31 - 1, -1][:width - nb] + [-7] * (width - nb - 2))
+        at += nb
+    assert at <= blocks
+    return rows
+
+
+def random_pool(G, blocks, bs, D, dtype, gen, device, scales="pow2"):
+    """An 8-bit pool of every byte but e4m3's NaN, and its scales."""
+    b = torch.randint(0, 256, (G, blocks * bs, D), generator=gen).to(torch.uint8)
+    if dtype == E:
+        b[(b & 127) == 127] = 5
+        b &= 0xBF  # |values| < 2: mixed magnitudes without a few that decide everything
+    else:
+        b[b == 128] = 1
+    e = torch.randint(-7, -4, (G, blocks), generator=gen).float() + (5 if dtype == E else 0)
+    s = torch.exp2(e)
+    if scales == "any":
+        s *= 1 + torch.rand((G, blocks), generator=gen)
+        s[:, ::7] = 0.0
+    return b.view(dtype).to(device), s.to(device)
+
+
+def packed(x):
+    cu = [0]
+    for n in x:
+        cu.append(cu[-1] + n)
+    return cu
+
+
+# ------------------------------------------------------------------ write
+WRITES = [  # (G, D, bs, [(rows, kv)])
+    (2, 128, 16, [(1, 1), (1, 16), (1, 17), (1, 40), (33, 33), (20, 30), (0, 9), (0, 0)]),
+    (3, 64, 16, [(48, 48), (16, 32), (5, 100)]),
+    (1, 128, 32, [(1, 31), (1, 33), (64, 70)]),
+    (2, 20, 16, [(7, 9), (1, 3), (30, 31)]),
+    (2, 72, 5, [(1, 6), (11, 13), (1, 5)]),
+    (2, 256, 16, [(17, 35)]),
+    (1, 8, 1, [(3, 5), (1, 1)]),
+]
+
+
+@pytest.mark.parametrize("shape", range(len(WRITES)))
+@pytest.mark.parametrize("dtype", [BF, HF, F])
+@pytest.mark.parametrize("pool", [E, I])
+def test_write_bits(device, pool, dtype, shape):
+    G, D, bs, seqs = WRITES[shape]
+    gen = torch.Generator().manual_seed(shape)
+    rows, lens = [n for n, _ in seqs], [kv for _, kv in seqs]
+    blocks = sum((n + bs - 1) // bs for n in lens) + 3
+    tab = tables(lens, bs, blocks, gen)
+    kp, ks = random_pool(G, blocks, bs, D, pool, gen, device)
+    vp, vs = random_pool(G, blocks, bs, D, pool, gen, device)
+    T = sum(rows)
+    # magnitudes from far below the blocks' present scales to far above
+    mag = torch.exp2(torch.randint(-12, 6, (T, G, 1), generator=gen).float())
+    k = (torch.randn((T, G, D), generator=gen) * mag).to(dtype).to(device)
+    v = (torch.randn((T, G, D), generator=gen) * mag).to(dtype).to(device)
+    v[: T // 2] = 0  # blocks of zeros
+    want = [Cache(kp, ks, bs), Cache(vp, vs, bs)]
+    cu = packed(rows)
+    for w, x in zip(want, (k, v)):
+        for s, (n, kv) in enumerate(seqs):
+            w.write(x[cu[s]:cu[s + 1]].cpu().double().numpy(), tab[s], kv)
+    before = [kp.clone(), vp.clone()]
+    if shape == 0:  # the reference's head-major rows
+        k = k.transpose(0, 1).contiguous().transpose(0, 1)
+        v = v.transpose(0, 1).contiguous().transpose(0, 1)
+    ops.kv_write_q8(k, v, kp, vp, ks, vs, i32(cu, device), i32(lens, device), i32(tab, device), bs)
+    torch.cuda.synchronize()
+    for w, p, s, old in zip(want, (kp, vp), (ks, vs), before):
+        assert np.array_equal(s.cpu().double().numpy(), w.s)
+        assert np.array_equal(values(p).reshape(w.q.shape), w.q)
+    # blocks that no sequence writes keep their bytes, and so do the rows behind a sequence's last
+    touched = torch.zeros(blocks * bs, dtype=torch.bool)
+    for s, (n, kv) in enumerate(seqs):
+        for j in range((kv - n) // bs * bs if n else kv, kv):
+            touched[tab[s][j // bs] * bs + j % bs] = True
+    for p, old in zip((kp, vp), before):
+        a, b = p.view(torch.uint8).cpu()[:, ~touched], old.view(torch.uint8).cpu()[:, ~touched]
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("pool", [E, I])
+def test_write_non_finite_and_extremes(device, pool):
+    G, D, bs = 1, 64, 16
+    kp = torch.zeros((G, 4 * bs, D), dtype=torch.int8, device=device).view(pool)
+    vp, ks = kp.clone(), torch.ones((G, 4), device=device)
+    vs = ks.clone()
+    x = torch.ones((3 * bs, G, D), device=device)
+    x[3, 0, 5] = float("nan")
+    x[bs + 1, 0, 0] = float("-inf")
+    x[2 * bs:] = 3.4e38
+    y = torch.full((3 * bs, G, D), 1e-45, device=device)
+    y[bs:] = 0.0
+    tab, cu, kv = i32([[2, 0, 3]], device), i32([0, 3 * bs], device), i32([3 * bs], device)
+    ops.kv_write_q8(x, y, kp, vp, ks, vs, cu, kv, tab)
+    s = ks[0].cpu()
+    assert torch.isnan(s[2]) and torch.isnan(s[0]) and s[1] == 1.0
+    # 127 * 2^121 = 3.376e38 and 448 * 2^119 = 2.977e38 are below 3.4e38
+    assert s[3] == (2.0 ** 122 if pool == I else 2.0 ** 120)
+    assert vs[0].cpu().tolist() == [0.0, 1.0, 2.0 ** -126, 0.0]
+    # one more row into a poisoned block keeps it so; a fresh start clears it
+    one = torch.ones((1, G, D), device=device)
+    ops.kv_write_q8(one, one, kp, vp, ks, vs, i32([0, 1], device), i32([5], device), tab)
+    assert torch.isnan(ks[0, 2])
+    ops.kv_write_q8(one, one, kp, vp, ks, vs, i32([0, 1], device), i32([1], device), tab)
+    assert ks[0, 2] == (2.0 ** -6 if pool == I else 2.0 ** -8)
+
+
+def test_write_skips_what_it_must_not_touch(device):
+    """kv < q_len, ids outside the pool, positions past the table, rows past total_q's sequences."""
+    G, D, bs = 2, 64, 16
+    kp = torch.full((G, 4 * bs, D), 3, dtype=torch.int8, device=device)
+    vp, ks = kp.clone(), torch.ones((G, 4), device=device)
+    vs = ks.clone()
+    x = torch.randn((40, G, D), device=device)
+    tab = i32([[0, 1], [-1, 4], [2, 3]], device)
+    # sequence 0: kv < rows; 1: bad ids; 2: rows end past its table of two blocks
+    ops.kv_write_q8(x, x, kp, vp, ks, vs, i32([0, 10, 20, 40], device), i32([9, 20, 50], device),
+                    tab)
+    assert (kp[:, :2 * bs] == 3).all() and (ks[:, :3] == 1).all() and (kp[:, 2 * bs:3 * bs] == 3).all()
+    assert (ks[:, 3] == 1).all()  # its new rows start at position 30: block 3's rows 14 and 15
+    assert not (kp[:, 3 * bs + 14:] == 3).all() and (kp[:, 3 * bs:3 * bs + 14] == 3).all()
+
+
+# ------------------------------------------------------------------ read back
+@pytest.mark.parametrize("dtype", [BF, HF, F])
+@pytest.mark.parametrize("pool", [E, I])
+@pytest.mark.parametrize("D,bs", [(128, 16), (20, 16), (64, 5)])
+def test_dequant(device, D, bs, pool, dtype):
+    gen = torch.Generator().manual_seed(D)
+    G, lens = 2, [1, 0, 33, 16]
+    blocks = sum((n + bs - 1) // bs for n in lens) + 1
+    kp, ks = random_pool(G, blocks, bs, D, pool, gen, device, "any")
+    vp, vs = random_pool(G, blocks, bs, D, pool, gen, device)
+    tab, out_tab = tables(lens, bs, blocks, gen), tables(lens, bs, blocks + 2, gen)
+    ko = torch.full((G, (blocks + 2) * bs, D), 7.0, dtype=dtype, device=device)
+    vo = ko.clone()
+    ops.kv_dequant(kp, vp, ks, vs, i32(tab, device), i32(lens, device), ko, vo,
+                   i32(out_tab, device), max(lens), bs)
+    for p, s, o in ((kp, ks, ko), (vp, vs, vo)):
+        c, want = Cache(p, s, bs), np.full(o.shape, 7.0)
+        for t, ot, n in zip(tab, out_tab, lens):
+            for j, row in enumerate(c.rows(t, n)):
+                want[:, ot[j // bs] * bs + j % bs] = row
+        w = torch.from_numpy(want).float().to(dtype)  # products of two fp32 rounded to fp32 first
+        assert torch.equal(o.cpu(), w)
+
+
+def test_dequant_every_byte_and_f16_saturates(device):
+    G, D, bs = 1, 256, 1
+    for pool in (E, I):
+        b = torch.arange(256, dtype=torch.int32).to(torch.uint8).view(1, 1, 256)
+        kp = b.view(pool).to(device)
+        s = torch.full((1, 1), 2.0 ** 10, device=device)
+        one = i32([[0]], device)
+        ko = torch.zeros((1, 1, 256), dtype=HF, device=device)
+        vo = torch.zeros_like(ko)
+        ops.kv_dequant(kp, kp, s, s, one, i32([1], device), ko, vo, one, 1, bs)
+        want = np.clip(values(b.view(pool)) * 1024.0, -65504, 65504)
+        assert np.array_equal(ko.cpu().double().numpy(), want, equal_nan=True)
+
+
+# ------------------------------------------------------------------ decode
+DECODES = [  # (H, G, D, bs, context lengths)
+    (8, 2, 128, 16, [1, 0, 15, 16, 17, 64, 33]),
+    (14, 2, 64, 16, [100, 31, 1]),
+    (4, 4, 64, 16, [5, 700]),
+    (32, 8, 128, 16, [1030]),
+    (28, 4, 128, 16, [65, 2, 129]),
+    (16, 1, 128, 32, [40, 90]),
+    (17, 1, 64, 16, [37]),
+    (6, 3, 128, 48, [100, 47]),
+    (4, 2, 96, 16, [50, 3]),
+    (2, 1, 20, 5, [23, 4]),
+    (4, 2, 256, 16, [33]),
+    (2, 2, 64, 8, [19, 70]),
+]
+
+
+def decode_case(shape, pool, dtype, device, scales="pow2"):
+    H, G, D, bs, lens = DECODES[shape]
+    gen = torch.Generator().manual_seed(100 + shape)
+    blocks = sum((n + bs - 1) // bs for n in lens) + 2
+    tab = tables(lens, bs, blocks, gen, extra=1)
+    kp, ks = random_pool(G, blocks, bs, D, pool, gen, device, scales)
+    vp, vs = random_pool(G, blocks, bs, D, pool, gen, device, scales)
+    q = torch.randn((len(lens), H, D), generator=gen).to(dtype).to(device)
+    # positions behind a sequence's end hold NaN bytes (e4m3) and whatever else
+    if pool == E:
+        flat = kp.view(torch.uint8), vp.view(torch.uint8)
+        for t, n in zip(tab, lens):
+            if n % bs:
+                lo = t[n // bs] * bs + n % bs
+                for f in flat:
+                    f[:, lo:lo + bs - n % bs] = 127
+    return q, kp, vp, ks, vs, tab, lens, bs
+
+
+def want_decode(q, kp, vp, ks, vs, tab, lens, bs, scale):
+    """(output, bound, weights (b, G, L), their bound) in 64 bits."""
+    ck, cv, G = Cache(kp, ks, bs), Cache(vp, vs, bs), kp.shape[0]
+    B, H, D = q.shape
+    out, bound = np.zeros((B, H, D)), np.zeros((B, H, D))
+    w, wb = np.zeros((B, G, max(lens))), np.zeros((B, G, max(lens)))
+    for b, n in enumerate(lens):
+        if n == 0:
+            continue
+        k, v = ck.rows(tab[b], n), cv.rows(tab[b], n)
+        o, p, err = attend(q[b:b + 1].cpu().double().numpy(), k, v, scale)
+        out[b], p = o[0], p[0]
+        big = np.abs(v).max()
+        bound[b] = 2 * err[0][:, None] * big
+        w[b, :, :n] = p.reshape(G, H // G, n).sum(1)
+        wb[b, :, :n] = (p * 2 * err[0][:, None]).reshape(G, H // G, n).sum(1) + 2.0 ** -40
+    return out, bound, w, wb
+
+
+@pytest.mark.parametrize("shape", range(len(DECODES)))
+@pytest.mark.parametrize("dtype", [BF, HF, F])
+@pytest.mark.parametrize("pool", [E, I])
+def test_decode(device, pool, dtype, shape):
+    q, kp, vp, ks, vs, tab, lens, bs = decode_case(shape, pool, dtype, device,
+                                                   "any" if shape % 2 else "pow2")
+    scale = q.shape[2] ** -0.5
+    want, bound, w, wb = want_decode(q, kp, vp, ks, vs, tab, lens, bs, scale)
+    args = (q, kp, vp, ks, vs, i32(tab, device), i32(lens, device), scale, max(lens), bs)
+    ws = ops.Workspace(device)
+    for out_dtype in {F, dtype}:
+        close(ops.paged_decode_q8(*args, out_dtype=out_dtype, workspace=ws), want, bound)
+    # the same with the weights added to sums, twice
+    sums = torch.rand((len(lens) + 1, kp.shape[0], max(lens) + 3), device=device)
+    before = sums.cpu().double().numpy()
+    for _ in range(2):
+        out = ops.paged_decode_q8(*args, out_dtype=F, workspace=ws, weights=sums)
+    close(out, want, bound)
+    after = before.copy()
+    after[:len(lens), :, :max(lens)] += 2 * w
+    wbound = np.zeros_like(before)
+    wbound[:len(lens), :, :max(lens)] = 2 * wb + 2.0 ** -23 * after[:len(lens), :, :max(lens)]
+    close(sums, after, wbound)
+    for b, n in enumerate(lens):  # nothing behind a sequence's end, nothing in the spare row
+        assert np.array_equal(sums[b, :, n:].cpu().double().numpy(), before[b, :, n:])
+    assert np.array_equal(sums[len(lens)].cpu().double().numpy(), before[len(lens)])
+
+
+@pytest.mark.parametrize("shape", [0, 1, 3, 5, 6, 8, 9])
+@pytest.mark.parametrize("dtype", [BF, HF, F])
+def test_decode_weights_over_plain_pools(device, dtype, shape):
+    H, G, D, bs, lens = DECODES[shape]
+    gen = torch.Generator().manual_seed(200 + shape)
+    blocks = sum((n + bs - 1) // bs for n in lens) + 2
+    tab = tables(lens, bs, blocks, gen, extra=1)
+    kp = torch.randn((G, blocks * bs, D), generator=gen).to(dtype).to(device)
+    vp = torch.randn((G, blocks * bs, D), generator=gen).to(dtype).to(device)
+    q = torch.randn((len(lens), H, D), generator=gen).to(dtype).to(device)
+    scale = D ** -0.5
+    rows = list(range(len(lens), 0, -1))
+    rows[0] = len(lens) + 5  # no such row
+    if len(rows) > 2:
+        rows[2] = -1
+    sums = torch.rand((len(lens) + 1, G, max(lens)), device=device)
+    before = sums.cpu().double().numpy()
+    out = ops.paged_decode_weights(q, kp, vp, i32(tab, device), i32(lens, device), scale, max(lens),
+                                   sums, bs, out_dtype=F, weight_rows=i32(rows, device))
+    after, wbound = before.copy(), np.zeros_like(before)
+    for b, n in enumerate(lens):
+        o, bound = np.zeros((1, H, D)), np.zeros((1, H, D))
+        if n:
+            j = np.arange(n)
+            at = np.array(tab[b])[j // bs] * bs + j % bs
+            k, v = (p.cpu().double().numpy()[:, at].transpose(1, 0, 2) for p in (kp, vp))
+            o, p, err = attend(q[b:b + 1].cpu().double().numpy(), k, v, scale)
+            bound[0] = 2 * err[0][:, None] * np.abs(v).max()
+            if 0 <= rows[b] <= len(lens):
+                add = p[0].reshape(G, H // G, n)
+                after[rows[b], :, :n] += add.sum(1)
+                wbound[rows[b], :, :n] = (add * 2 * err[0].reshape(G, -1, 1)).sum(1) + 2.0 ** -22
+        close(out[b:b + 1], o, bound)
+    close(sums, after, wbound)
+
+
+@pytest.mark.parametrize("shape", [0, 8])
+def test_decode_poisoned_block_reaches_only_those_that_attend_to_it(device, shape):
+    q, kp, vp, ks, vs, tab, lens, bs = decode_case(shape, I, BF, device)
+    b = len(lens) - 1 if lens[-1] > 1 else 0
+    args = (kp, vp, ks, vs, i32(tab, device), i32(lens, device), 0.1, max(lens), bs)
+    clean = ops.paged_decode_q8(q, *args)
+    for s in (ks, vs):
+        keep = s.clone()
+        s[0, tab[b][0]] = float("nan")
+        # blocks that no sequence holds
+        used = {x for t, n in zip(tab, lens) for x in t[:(n + bs - 1) // bs]}
+        for x in set(range(s.shape[1])) - used:
+            s[:, x] = float("nan")
+        got = ops.paged_decode_q8(q, *args)
+        rep = q.shape[1] // kp.shape[0]
+        assert torch.isnan(got[b, :rep]).all()
+        got[b, :rep] = clean[b, :rep]
+        assert torch.equal(got, clean)
+        s.copy_(keep)
+
+
+@pytest.mark.parametrize("dtype", [BF, F])
+def test_decode_range_of_scales(device, dtype):
+    """Blocks whose V scales lie 2^60 apart, the heaviest position in the smallest, one block of
+    zeros: each weight still counts."""
+    H, G, D, bs, n = 4, 2, 64, 16, 64
+    gen = torch.Generator().manual_seed(3)
+    kp, ks = random_pool(G, 4, bs, D, I, gen, device)
+    vp, vs = random_pool(G, 4, bs, D, I, gen, device)
+    vs[:] = torch.tensor([2.0 ** -50, 0.0, 2.0 ** 10, 1.0], device=device)
+    vp[:, bs:2 * bs] = 0
+    q = (3 * torch.randn((1, H, D), generator=gen)).to(dtype).to(device)
+    tab = [[0, 1, 2, 3]]
+    want, bound, _, _ = want_decode(q, kp, vp, ks, vs, tab, [n], bs, 1.0)
+    got = ops.paged_decode_q8(q, kp, vp, ks, vs, i32(tab, device), i32([n], device), 1.0, n, bs,
+                              out_dtype=F)
+    close(got, want, bound)
+
+
+def test_decode_queries_beyond_f16(device):
+    """bf16 and fp32 queries whose elements f16 could not hold."""
+    H, G, D, bs, n = 4, 2, 128, 16, 40
+    gen = torch.Generator().manual_seed(4)
+    kp, ks = random_pool(G, 3, bs, D, E, gen, device)
+    vp, vs = random_pool(G, 3, bs, D, E, gen, device)
+    for dtype in (BF, F):
+        for mag in (1e20, 1e-20):
+            q = (mag * torch.randn((1, H, D), generator=gen)).to(dtype).to(device)
+            scale = 0.1 / mag
+            want, bound, _, _ = want_decode(q, kp, vp, ks, vs, [[0, 1, 2]], [n], bs, scale)
+            got = ops.paged_decode_q8(q, kp, vp, ks, vs, i32([[0, 1, 2]], device),
+                                      i32([n], device), scale, n, bs, out_dtype=F)
+            close(got, want, bound)
+    q = torch.zeros((1, H, D), dtype=BF, device=device)  # all scores alike
+    want, bound, _, _ = want_decode(q, kp, vp, ks, vs, [[0, 1, 2]], [n], bs, 1.0)
+    close(ops.paged_decode_q8(q, kp, vp, ks, vs, i32([[0, 1, 2]], device), i32([n], device), 1.0,
+                              n, bs, out_dtype=F), want, bound)
+    q[0, 1, 3] = float("nan")
+    got = ops.paged_decode_q8(q, kp, vp, ks, vs, i32([[0, 1, 2]], device), i32([n], device), 1.0, n)
+    assert torch.isnan(got[0, 1]).all() and not torch.isnan(got[0, [0, 2, 3]]).any()
+
+
+def test_decode_context_clamped_and_offsets_past_32_bits(device):
+    """max_context_len bounds the contexts; a pool of more than 2^32 elements a pool."""
+    H, G, D, bs = 2, 2, 128, 16
+    blocks = (1 << 32) // (G * bs * D) + 64
+    kp = torch.zeros((G, blocks * bs, D), dtype=torch.int8, device=device)
+    vp = torch.zeros_like(kp)
+    ks = torch.ones((G, blocks), device=device)
+    gen = torch.Generator().manual_seed(5)
+    tab = [[blocks - 1, 3, blocks // 2 + 7]]
+    small_k, _ = random_pool(G, 3, bs, D, I, gen, device)
+    small_v, _ = random_pool(G, 3, bs, D, I, gen, device)
+    for i, b in enumerate(tab[0]):
+        kp[:, b * bs:(b + 1) * bs] = small_k[:, i * bs:(i + 1) * bs]
+        vp[:, b * bs:(b + 1) * bs] = small_v[:, i * bs:(i + 1) * bs]
+    s3 = torch.ones((G, 3), device=device)
+    q = torch.randn((1, H, D), generator=gen).to(BF).to(device)
+    want, bound, _, _ = want_decode(q, small_k, small_v, s3, s3, [[0, 1, 2]], [40], bs, 0.001)
+    got = ops.paged_decode_q8(q, kp, vp, ks, ks, i32(tab, device), i32([47], device), 0.001, 40)
+    close(got, want, bound)
+    x = torch.randn((4, G, D), generator=gen).to(BF).to(device)
+    c = Cache(small_k, s3, bs)
+    c.write(x.cpu().double().numpy(), [0, 1, 2], 47)
+    ops.kv_write_q8(x, x, kp, vp, ks, torch.ones_like(ks), i32([0, 4], device), i32([47], device),
+                    i32(tab, device))
+    b = tab[0][2]
+    assert np.array_equal(values(kp[:, b * bs:(b + 1) * bs]), c.q[:, 2])
+    del kp, vp
+
+
+# ------------------------------------------------------------------ prefill
+PREFILLS = [  # (H, G, D, bs, [(rows, kv)])
+    (8, 2, 128, 16, [(1, 1), (5, 40), (0, 12), (17, 17), (3, 2), (2, 100)]),
+    (14, 2, 64, 16, [(4, 33), (7, 130)]),
+    (28, 4, 128, 16, [(130, 200), (1, 64)]),
+    (4, 2, 128, 16, [(300, 300)]),
+    (4, 4, 64, 32, [(40, 70), (8, 8)]),
+    (6, 2, 96, 16, [(9, 20)]),
+    (2, 1, 20, 5, [(6, 13), (2, 2)]),
+    (17, 1, 128, 16, [(3, 50)]),
+    (16, 2, 128, 16, [(8, 600), (2, 900)]),
+]
+
+
+@pytest.mark.parametrize("shape", range(len(PREFILLS)))
+@pytest.mark.parametrize("dtype", [BF, HF, F])
+@pytest.mark.parametrize("pool", [E, I])
+def test_prefill(device, pool, dtype, shape):
+    H, G, D, bs, seqs = PREFILLS[shape]
+    gen = torch.Generator().manual_seed(300 + shape)
+    rows, lens = [n for n, _ in seqs], [kv for _, kv in seqs]
+    blocks = sum((n + bs - 1) // bs for n in lens) + 2
+    tab = tables(lens, bs, blocks, gen, extra=1)
+    kp, ks = random_pool(G, blocks, bs, D, pool, gen, device)
+    vp, vs = random_pool(G, blocks, bs, D, pool, gen, device)
+    q = torch.randn((sum(rows), H, D), generator=gen).to(dtype).to(device)
+    if shape % 2:  # head-major
+        q = q.transpose(0, 1).contiguous().transpose(0, 1)
+    scale, cu = D ** -0.5, packed(rows)
+    ck, cv = Cache(kp, ks, bs), Cache(vp, vs, bs)
+    want, bound = np.zeros((sum(rows), H, D)), np.zeros((sum(rows), H, D))
+    for s, (n, kv) in enumerate(seqs):
+        if n and kv >= n:
+            k, v = ck.rows(tab[s], kv), cv.rows(tab[s], kv)
+            o, _, err = attend(q[cu[s]:cu[s + 1]].cpu().double().numpy(), k, v, scale)
+            want[cu[s]:cu[s + 1]] = o
+            # longer calls over 16-bit queries round each probability to f16 once (2^-11)
+            p_eps = 2.0 ** -11 if dtype != F else 0.0
+            bound[cu[s]:cu[s + 1]] = (2 * err[:, :, None] + p_eps) * np.abs(v).max()
+    for out_dtype in {F, dtype}:
+        out = torch.full((sum(rows) + 2, H, D), 9.0, dtype=out_dtype, device=device)
+        ops.varlen_prefill_q8(q, kp, vp, ks, vs, i32(cu, device), i32(lens, device),
+                              i32(tab, device), max(rows), max(lens), scale, bs,
+                              out=out[:sum(rows)], workspace=ops.Workspace(device))
+        close(out[:sum(rows)], want, bound)
+        assert (out[sum(rows):] == 9.0).all()
+
+
+# ------------------------------------------------------------------ streams and graphs
+def test_decode_captured_and_replayed(device):
+    """Two captured steps that share a workspace, replayed among eager calls of their own and of a
+    larger step that makes the workspace grow."""
+    q, kp, vp, ks, vs, tab, lens, bs = decode_case(0, E, BF, device)
+    big = decode_case(3, E, BF, device)
+    ws = ops.Workspace(device)
+    t, n = i32(tab, device), i32(lens, device)
+    sums = torch.zeros((len(lens), kp.shape[0], max(lens)), device=device)
+    cu = i32(packed([1] * len(lens)), device)
+
+    def step(w):
+        o = ops.paged_decode_q8(q, kp, vp, ks, vs, t, n, 0.09, max(lens), bs, workspace=ws,
+                                weights=w)
+        p = ops.varlen_prefill_q8(q, kp, vp, ks, vs, cu, n, t, 1, max(lens), 0.09, bs, workspace=ws)
+        return o, p
+
+    eager = torch.zeros_like(sums)
+    want = step(eager)
+    graphs = []
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        step(sums)
+    torch.cuda.synchronize()
+    sums.zero_()
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            got = step(sums)
+        graphs.append((g, got))
+    total = torch.zeros_like(sums)
+    for i in range(6):
+        g, got = graphs[i % 2]
+        for x in got:
+            x.fill_(5.0)
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        total += eager
+        assert torch.allclose(sums, total, rtol=2.0 ** -20, atol=0)
+        ops.paged_decode_q8(big[0], *big[1:5], i32(big[5], device), i32(big[6], device), 0.1,
+                            max(big[6]), big[7], workspace=ws,
+                            weights=torch.zeros((1, 8, max(big[6])), device=device))
+        torch.cuda.synchronize()
+
+
+def test_two_streams_without_a_workspace(device):
+    """Calls without a workspace share no scratch: two streams at once."""
+    a, b = decode_case(3, I, HF, device), decode_case(0, E, HF, device)
+
+    def call(c):
+        q, kp, vp, ks, vs, tab, lens, bs = c
+        w = torch.zeros((len(lens), kp.shape[0], max(lens)), device=device)
+        return ops.paged_decode_q8(q, kp, vp, ks, vs, i32(tab, device), i32(lens, device), 0.1,
+                                   max(lens), bs, weights=w), w
+
+    want = [call(a), call(b)]
+    torch.cuda.synchronize()
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+    got = []
+    for _ in range(4):
+        with torch.cuda.stream(s1):
+            x = call(a)
+        with torch.cuda.stream(s2):
+            y = call(b)
+        got.append((x, y))
+    torch.cuda.synchronize()
+    for pair in got:
+        for g, w in zip(pair, want):
+            assert torch.equal(g[0], w[0]) and torch.equal(g[1], w[1])
+
+
+
+# ------------------------------------------------------------------ refusals (nothing is launched)
+def test_tensor_refusals(device):
+    G, D, bs = 2, 64, 16
+    kp = torch.zeros((G, 4 * bs, D), dtype=torch.int8, device=device)
+    s = torch.ones((G, 4), device=device)
+    t, n, cu = i32([[0, 1]], device), i32([20], device), i32([0, 1], device)
+    q = torch.zeros((1, 4, D), dtype=BF, device=device)
+    x = torch.zeros((1, G, D), dtype=BF, device=device)
+    plain = torch.zeros((G, 4 * bs, D), dtype=BF, device=device)
+    w = torch.zeros((1, G, 32), device=device)
+    bad = [
+        lambda: ops.paged_decode_q8(q, plain, plain, s, s, t, n, 1.0, 32),
+        lambda: ops.paged_decode_q8(q, kp, kp, s[:, :3], s, t, n, 1.0, 32),
+        lambda: ops.paged_decode_q8(q, kp, kp, s.double(), s, t, n, 1.0, 32),
+        lambda: ops.paged_decode_q8(q, kp, kp, s, s.cpu(), t, n, 1.0, 32),
+        lambda: ops.paged_decode_q8(q[:, :3], kp, kp, s, s, t, n, 1.0, 32),
+        lambda: ops.paged_decode_q8(q, kp, kp, s, s, t, n, 1.0, 33),  # beyond the table
+        lambda: ops.paged_decode_q8(q, kp, kp, s, s, t.long(), n, 1.0, 32),
+        lambda: ops.paged_decode_q8(q, kp, kp, s, s, t, i32([20, 3], device), 1.0, 32),
+        lambda: ops.paged_decode_q8(q, kp, kp, s, s, t, n, 1.0, 32, block_size=24),
+        lambda: ops.paged_decode_q8(q, kp, kp, s, s, t, n, 1.0, 32, weights=w[:, :, :31]),
+        lambda: ops.paged_decode_q8(q, kp, kp, s, s, t, n, 1.0, 32, weights=w[:0]),
+        lambda: ops.paged_decode_q8(q, kp, kp, s, s, t, n, 1.0, 32, weight_rows=n),
+        lambda: ops.paged_decode_q8(q.to(torch.float64), kp, kp, s, s, t, n, 1.0, 32),
+        lambda: ops.paged_decode_weights(q, plain, plain, t, n, 1.0, 32, None),
+        lambda: ops.paged_decode_weights(q.half(), plain, plain, t, n, 1.0, 32, w),
+        lambda: ops.paged_decode_weights(q, kp, kp, t, n, 1.0, 32, w),
+        lambda: ops.kv_write_q8(x, x[:, :1], kp, kp, s, s, cu, n, t),
+        lambda: ops.kv_write_q8(x, x.half(), kp, kp, s, s, cu, n, t),
+        lambda: ops.kv_write_q8(x, x, kp, kp, s, s, cu, i32([1, 2], device), t),
+        lambda: ops.kv_write_q8(x, x, plain, plain, s, s, cu, n, t),
+        lambda: ops.kv_dequant(kp, kp, s, s, t, n, plain, plain, t, 40),
+        lambda: ops.kv_dequant(kp, kp, s, s, t, n, plain[:1], plain[:1], t, 32),
+        lambda: ops.kv_dequant(kp, kp, s, s, t, n, kp, kp, t, 32),
+        lambda: ops.varlen_prefill_q8(q, kp, kp, s, s, cu, n, t, 1, 33, 1.0),
+        lambda: ops.varlen_prefill_q8(q[..., ::2], kp, kp, s, s, cu, n, t, 1, 32, 1.0),
+        lambda: ops.kv_evict(kp, kp, w, t, n, n, t, 32, 32),  # no scales
+        lambda: ops.kv_evict(plain, plain, w, t, n, n, t, 32, 32, k_scale=s, v_scale=s),
+        lambda: ops.kv_evict(plain, plain, w, t, n, n, t, 32, 33),
+        lambda: ops.kv_evict(plain, plain, w, t, n, n, t, 32, 32, recent=-1),
+        lambda: ops.kv_evict(plain, plain, w, t, n, n, t, 32, 32, weights_out=w.half()),
+    ]
+    for i, f in enumerate(bad):
+        with pytest.raises(FlourError) as e:
+            f()
+        assert e.value.code in (ERR_INVALID_ARGUMENT, ERR_UNSUPPORTED), i
