@@ -212,8 +212,8 @@ static size_t up256(size_t x) { return (x + 255) & ~(size_t)255; }
 
 static int64_t score_stride_of(int max_ctx) { return ((int64_t)max_ctx + 63) / 64 * 64; }
 
-static size_t decode_pools_ws(int batch, int num_heads, int max_ctx, bool with_weights) {
-    if (!with_weights) return 0;
+// Scores and their maxima and sums, behind the streamed kernel's part.
+static size_t weights_bytes(int batch, int num_heads, int max_ctx) {
     const size_t rows = (size_t)batch * num_heads;
     return up256(rows * 2 * sizeof(float)) + up256(rows * score_stride_of(max_ctx) * sizeof(float));
 }
@@ -245,7 +245,10 @@ static int decode_pools(const char* what, PoolAttn a, float* weights, int64_t wi
         set_error("%s: null pointer", what);
         return FLOUR_ERR_INVALID_ARGUMENT;
     }
-    const size_t need = decode_pools_ws(a.batch, a.num_heads, a.max_kv, weights != nullptr);
+    const int n_rep = a.num_heads / a.kv_heads;
+    const size_t stream_part = decode_stream_bytes(a.batch, n_rep, a.head_dim);
+    const size_t need =
+        stream_part + (weights ? weights_bytes(a.batch, a.num_heads, a.max_kv) : 0);
     if (need > 0 && (!workspace || workspace_bytes < need || (uintptr_t)workspace % 256 != 0)) {
         set_error("%s: workspace of %zu bytes (256-byte aligned) required, got %zu at %p", what,
                   need, workspace_bytes, workspace);
@@ -255,17 +258,17 @@ static int decode_pools(const char* what, PoolAttn a, float* weights, int64_t wi
     a.q_st = a.o_st = (int64_t)a.num_heads * a.head_dim;
     a.q_sh = a.o_sh = a.head_dim;
     if (weights) {
-        a.ml = static_cast<float*>(workspace);
+        char* ws = static_cast<char*>(workspace) + stream_part;
+        a.ml = reinterpret_cast<float*>(ws);
         a.scores = reinterpret_cast<float*>(
-            static_cast<char*>(workspace) +
-            up256((size_t)a.batch * a.num_heads * 2 * sizeof(float)));
+            ws + up256((size_t)a.batch * a.num_heads * 2 * sizeof(float)));
         a.score_stride = score_stride_of(a.max_kv);
     }
-    const int rc = launch_attn_pools(a, stream);
+    const int rc = decode_stream_takes(a) ? launch_decode_stream(a, 1, workspace, stream)
+                                          : launch_attn_pools(a, stream);
     if (rc != FLOUR_OK || !weights) return rc;
     return launch_weights_add(weights, width, weight_rows, num_rows, a.kv_lens, a.max_kv, a.batch,
-                              a.kv_heads, a.num_heads / a.kv_heads, a.scores, a.score_stride, a.ml,
-                              stream);
+                              a.kv_heads, n_rep, a.scores, a.score_stride, a.ml, stream);
 }
 
 }  // namespace flour
@@ -279,7 +282,8 @@ extern "C" int flour_hip_decode_weights_workspace_size(int batch, int num_heads,
         set_error("decode_weights_workspace_size: bad arguments");
         return FLOUR_ERR_INVALID_ARGUMENT;
     }
-    *bytes = decode_pools_ws(batch, num_heads, max_context_len, with_weights != 0);
+    *bytes = decode_stream_bytes(batch, num_heads / kv_heads, head_dim) +
+             (with_weights ? weights_bytes(batch, num_heads, max_context_len) : 0);
     return FLOUR_OK;
 }
 

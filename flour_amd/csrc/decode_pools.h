@@ -32,6 +32,14 @@ struct PoolAttn {
     float* ml;
 };
 
+// The streamed kernel (decode_pools.hip): whether it takes a call, the workspace it needs for groups of
+// up to max_cols columns (rows x query heads of a kv head), and its launch (max_rows bounds the rows of
+// a sequence). launch_attn_pools (attn_pools.hip) takes every shape.
+bool decode_stream_takes(const PoolAttn& a);
+size_t decode_stream_bytes(int batch, int max_cols, int head_dim);
+int launch_decode_stream(const PoolAttn& a, int max_rows, void* workspace, hipStream_t stream);
+int launch_attn_pools(const PoolAttn& a, hipStream_t stream);
+
 bool check_pool8(const char* what, int pool_dtype, const void* k_pool, const void* v_pool,
                  const void* k_scale, const void* v_scale, int kv_heads, int head_dim,
                  int block_size, int64_t num_slots);

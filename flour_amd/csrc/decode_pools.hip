@@ -1,0 +1,801 @@
+// decode_pools.hip — attention of few query rows over an 8-bit cache, streamed from HBM on the f16
+// matrix cores: decode steps and short runs of new rows (drafted tokens, short turns).
+//
+// With few rows per sequence the step reads each K/V byte once and is bound by that; everything
+// else has to fit beside the stream. Work split: as in paged_decode.hip, the chunks of every
+// (sequence, kv head, column group) laid end to end and cut into equal wave ranges, one-wave
+// workgroups, pieces of pairs cut by a range end merged by a second kernel.
+//
+// Inside a piece, for a column = (query row, query head of the kv head), 16 to a matrix tile, NT
+// tiles to a wave:
+//  * A chunk is TILES tiles of 16 tokens, 2 KB of K and of V each at head_dim 128. Two register
+//    buffers: the next chunk's loads are in flight while one is computed.
+//  * S = K Q^T on v_mfma_f32_16x16x32_f16. K is loaded in the A layout as it lies in memory: lane
+//    (g, c) = (lane / 16, lane % 16) holds bytes 16g .. of token c's row, and the columns of Q^T are
+//    permuted to match, so K passes through no LDS. Bytes become f16 exactly: e4m3 by the
+//    converter, int8 by placing x + 128 under the exponent of 1,024 and subtracting 1,152.
+//  * Queries are f16: f16 ones as they are; bf16 ones times a power of two per (row, head) that puts
+//    the largest element just below 2^15 (exact down to 2^-31 of it); fp32 ones as two f16 parts of that
+//    (22 bits, two products).
+//  * A block's K scale multiplies its 16 tokens' scores, one factor per tile. Its V scale S_v goes
+//    into the exponent: P' = 2^(s + log2 S_v - m'), with a running maximum m' of its own beside the
+//    maximum m of s that the sum of 2^(s - m) uses. So P' stays in (0, 1], f16 keeps it exact relative to
+//    the row's largest contribution whatever the blocks' scales, and V stays the integers and
+//    e4m3 values that it is. P' is scaled by 2^14 (clear of f16's subnormals) and split into two f16
+//    parts: two products, 22 bits.
+//  * The score registers are the B operand of O^T = V^T P'^T as they stand; the V^T operand is built
+//    in-lane, pairs of tokens' bytes by v_perm_b32, then the same conversion.
+#include <math.h>
+
+#include <algorithm>
+
+#include "cache8.h"
+#include "decode_pools.h"
+#include "decode_ranges.h"
+
+namespace flour {
+
+static constexpr int DP_MAX_BATCH = 4096;  // per-sequence chunk sums live in LDS
+static constexpr float DP_SHIFT = 14.0f;   // P' times 2^14
+static constexpr int DP_XCD_W = 2;         // the wave ranges' weight (paged_decode.hip)
+
+struct DpArgs {
+    void* out;
+    int out_dtype;
+    int64_t o_st, o_sh;
+    const void* q;
+    int64_t q_st, q_sh;
+    const uint8_t *k_pool, *v_pool;
+    const float *k_scale, *v_scale;
+    const int32_t *cu, *kv_lens, *block_tables;
+    int max_blocks, batch, num_heads, kv_heads, n_rep, block_size;
+    int64_t num_slots;
+    int max_kv;
+    float scale_log2;
+    float* scores;  // kept scores (or null): (batch, num_heads, score_stride)
+    int64_t score_stride;
+    float* ml;    // with scores: (batch, num_heads, 2)
+    float* p_ml;  // pieces: [2 * waves][16 NT][3] maximum, sum, maximum with the V scales
+    float* p_o;   // pieces: [2 * waves][16 NT][D]
+    int* pre;     // [batch + 1] chunks per kv head of the sequences before
+};
+
+// Rows of sequence s, its kv length (0 where its rows see nothing).
+struct DpSeq {
+    int row0, rows, kv;
+};
+__device__ __forceinline__ DpSeq dp_seq(const int32_t* cu, const int32_t* kv_lens, int max_kv, int s) {
+    const int r0 = cu ? cu[s] : s, n = cu ? cu[s + 1] - r0 : 1;
+    const int kv = min(kv_lens[s], max_kv);
+    return DpSeq{r0, max(n, 0), kv >= n && kv > 0 ? kv : 0};
+}
+// Column groups of n rows of n_rep heads; chunks of all of them over kv positions.
+template <int NT>
+__device__ __forceinline__ int dp_groups(int rows, int n_rep) {
+    return (rows * n_rep + 16 * NT - 1) / (16 * NT);
+}
+
+// Four bytes to two f16 pairs.
+template <typename TP>
+__device__ __forceinline__ u32x2 to_f16x4(uint32_t w);
+template <>
+__device__ __forceinline__ u32x2 to_f16x4<e4m3_t>(uint32_t w) {
+    return u32x2{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, false)),
+                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, true))};
+}
+template <>
+__device__ __forceinline__ u32x2 to_f16x4<i8_t>(uint32_t w) {
+    const uint32_t x = w ^ 0x80808080u;  // x + 128
+    const f16x2 off = {(_Float16)-1152.0f, (_Float16)-1152.0f};
+    const uint32_t a = __builtin_amdgcn_perm(0x64646464u, x, 0x04010400u);
+    const uint32_t b = __builtin_amdgcn_perm(0x64646464u, x, 0x04030402u);
+    return u32x2{__builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, a) + off),
+                 __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, b) + off)};
+}
+
+template <typename TQ, typename TP, int D, int TILES, int NT, bool BS16, bool W>
+__global__ __launch_bounds__(64, NT == 4 ? 1 : 2) void decode_pools_kernel(DpArgs a) {
+    constexpr int CHUNK = 16 * TILES;
+    constexpr int KL = D / 64;   // 16-byte K loads of a lane and tile
+    constexpr int NV = D / 16;   // O^T products of a chunk's half
+    constexpr int KK = D / 32;   // products of a score tile
+    constexpr int QP = sizeof(TQ) == 4 ? 2 : 1;  // parts of a query
+    typedef typename std::conditional<D == 128, u32x2, uint32_t>::type Vd;
+    extern __shared__ int pre[];
+    const int lane = threadIdx.x, lg = lane >> 4, lc = lane & 15;
+    const int n_rep = a.n_rep, batch = a.batch;
+
+    auto seq_chunks = [&](int s) -> int {
+        const DpSeq q = dp_seq(a.cu, a.kv_lens, a.max_kv, s);
+        return dp_groups<NT>(q.rows, n_rep) * ((q.kv + CHUNK - 1) / CHUNK);
+    };
+    // ---- exclusive prefix sums of the sequences' chunks (per kv head); up to 64 sequences stay in
+    // registers, one a lane
+    const bool in_lanes = batch <= 64;
+    int my_pre = 0, all_chunks;
+    if (in_lanes) {
+        const int n = lane < batch ? seq_chunks(lane) : 0;
+        const int incl = wave_incl_sum(n);
+        my_pre = incl - n;
+        all_chunks = __builtin_amdgcn_readlane(incl, 63);
+        if (blockIdx.x == 0) {
+            if (lane < batch) a.pre[lane] = my_pre;
+            if (lane == 63) a.pre[batch] = incl;
+        }
+    } else {
+        const int per = (batch + 63) / 64;
+        int local = 0;
+        for (int i = 0; i < per; i++) {
+            const int b = lane * per + i;
+            if (b < batch) {
+                const int n = seq_chunks(b);
+                pre[b] = n;
+                local += n;
+            }
+        }
+        const int incl = wave_incl_sum(local);
+        int run = incl - local;
+        for (int i = 0; i < per; i++) {
+            const int b = lane * per + i;
+            if (b < batch) {
+                const int n = pre[b];
+                pre[b] = run;
+                run += n;
+            }
+        }
+        if (lane == 63) pre[batch] = incl;
+        __syncthreads();
+        all_chunks = __builtin_amdgcn_readlane(incl, 63);
+        if (blockIdx.x == 0)
+            for (int b = lane; b <= batch; b += 64) a.pre[b] = pre[b];
+    }
+    const int64_t total = (int64_t)a.kv_heads * all_chunks;
+    const int64_t nwg = range_count(total, gridDim.x), wgi = blockIdx.x;
+    if (total == 0 || wgi >= nwg) return;
+    const bool narrow = ranges_narrow(total, nwg, DP_XCD_W);
+    int64_t lo;
+    int len;
+    if (narrow) {
+        const WaveRanges<uint32_t> wr(total, nwg, DP_XCD_W);
+        const uint32_t x = wr.lo((uint32_t)wgi);
+        lo = (uint32_t)__builtin_amdgcn_readfirstlane((int)x);
+        len = __builtin_amdgcn_readfirstlane((int)(wr.lo((uint32_t)wgi + 1) - x));
+    } else {
+        const WaveRanges<int64_t> wr(total, nwg, DP_XCD_W);
+        const int64_t x = wr.lo(wgi);
+        lo = ((int64_t)__builtin_amdgcn_readfirstlane((int)(x >> 32)) << 32) |
+             (uint32_t)__builtin_amdgcn_readfirstlane((int)x);
+        len = __builtin_amdgcn_readfirstlane((int)(wr.lo(wgi + 1) - x));
+    }
+
+    // ---- segments: up to SEG chunks (64 tiles, one a lane) of one (sequence, kv head, group)
+    constexpr int SEG = 64 / TILES;
+    struct Seg {
+        int b, g, grp, cb, ce, nch, row0, rows, kv;
+    };
+    auto seg_at = [&](int at) -> Seg {
+        const int64_t x = lo + at;
+        Seg sg;
+        int before;
+        if (in_lanes) {
+            const uint64_t le = __ballot(lane < batch && (int64_t)a.kv_heads * my_pre <= x);
+            sg.b = 63 - __builtin_clzll(le);
+            before = __builtin_amdgcn_readlane(my_pre, sg.b);
+        } else {
+            int l0 = 0, h0 = batch;
+            while (h0 - l0 > 1) {
+                const int mid = (l0 + h0) >> 1;
+                if ((int64_t)a.kv_heads * pre[mid] <= x)
+                    l0 = mid;
+                else
+                    h0 = mid;
+            }
+            sg.b = __builtin_amdgcn_readfirstlane(l0);
+            before = __builtin_amdgcn_readfirstlane(pre[l0]);
+        }
+        const DpSeq q = dp_seq(a.cu, a.kv_lens, a.max_kv, sg.b);
+        sg.row0 = __builtin_amdgcn_readfirstlane(q.row0);
+        sg.rows = __builtin_amdgcn_readfirstlane(q.rows);
+        sg.kv = __builtin_amdgcn_readfirstlane(q.kv);
+        sg.nch = (sg.kv + CHUNK - 1) / CHUNK;
+        const int64_t rel = x - (int64_t)a.kv_heads * before;
+        const int pair = __builtin_amdgcn_readfirstlane(
+            narrow ? (int)((uint32_t)rel / (uint32_t)sg.nch) : (int)(rel / sg.nch));
+        sg.cb = (int)(rel - (int64_t)pair * sg.nch);
+        // a head's groups next to each other: they read the same K/V
+        const int groups = dp_groups<NT>(sg.rows, n_rep);
+        sg.g = groups == 1 ? pair : pair / groups;
+        sg.grp = pair - sg.g * groups;
+        sg.ce = sg.cb + min(min(sg.nch - sg.cb, SEG), len - at);
+        return sg;
+    };
+    const int max_id = (int)(a.num_slots / a.block_size - 1);
+    const int64_t nb = a.num_slots / a.block_size;
+    struct Slots {
+        int id, off;  // lane i: block id as loaded and in-block offset of tile i's first token
+    };
+    auto seg_slots = [&](const Seg& sg) -> Slots {
+        const int32_t* bt = a.block_tables + (int64_t)sg.b * a.max_blocks;
+        const int tok0 = min(sg.cb * CHUNK + lane * 16, ((sg.kv - 1) >> 4) << 4);
+        const int lb = BS16 ? (tok0 >> 4) : tok0 / a.block_size;
+        return Slots{bt[lb], BS16 ? 0 : tok0 - lb * a.block_size};
+    };
+    auto clamp_id = [&](int id) -> int { return id < 0 ? 0 : (id > max_id ? max_id : id); };
+    struct Scales {
+        float k, v;  // lane i: the scales of tile i's block
+    };
+    auto seg_scales = [&](const Seg& sg, const Slots& sl) -> Scales {
+        const int64_t at = (int64_t)sg.g * nb + clamp_id(sl.id);
+        return Scales{a.k_scale[at], a.v_scale[at]};
+    };
+
+    const uint32_t head_bytes = (uint32_t)(a.num_slots * D);
+    // K: bytes 16 lg + 64 i of row lc. V: bytes (D / 16) lc of row 4 lg + j.
+    uint32_t k_off = (uint32_t)(lc * D + 16 * lg);
+    uint32_t v_off = (uint32_t)(4 * lg * D + (D / 16) * lc);
+    asm volatile("" : "+v"(k_off), "+v"(v_off));  // (row offsets stay immediates of the loads)
+    auto load_chunk = [&](int g, const Slots& sl, int tile0, u32x4 (*kd)[KL], Vd (*vd)[4]) {
+        const __amdgpu_buffer_rsrc_t k_rsrc = __builtin_amdgcn_make_buffer_rsrc(
+            (void*)(a.k_pool + (int64_t)g * a.num_slots * D), (short)0, (int)head_bytes, BUF_DWORD3);
+        const __amdgpu_buffer_rsrc_t v_rsrc = __builtin_amdgcn_make_buffer_rsrc(
+            (void*)(a.v_pool + (int64_t)g * a.num_slots * D), (short)0, (int)head_bytes, BUF_DWORD3);
+#pragma unroll
+        for (int t = 0; t < TILES; t++) {
+            const int id = clamp_id(__builtin_amdgcn_readlane(sl.id, tile0 + t));
+            const uint32_t slot =
+                BS16 ? (uint32_t)(id * 16)
+                     : (uint32_t)(id * a.block_size + __builtin_amdgcn_readlane(sl.off, tile0 + t));
+            const uint32_t soff = slot * (uint32_t)D;
+#pragma unroll
+            for (int i = 0; i < KL; i++)
+                kd[t][i] = __builtin_amdgcn_raw_buffer_load_b128(k_rsrc, k_off + 64 * i, soff, BUF_NT);
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                if constexpr (D == 128)
+                    vd[t][j] = __builtin_amdgcn_raw_buffer_load_b64(v_rsrc, v_off + j * D, soff, BUF_NT);
+                else
+                    vd[t][j] = __builtin_amdgcn_raw_buffer_load_b32(v_rsrc, v_off + j * D, soff, BUF_NT);
+            }
+        }
+    };
+
+    // ---- queries: lane (lg, lc) holds column lc of each tile, dims 16 lg + 64 i + 8 h .. + 7 for
+    // product kk = 2 i + h
+    u32x4 qb[NT][QP][KK];
+    float qf[NT];  // what turns a column's products into exp2-domain scores (times the K scale)
+    int vis[NT];   // positions that the column sees
+    int min_vis;   // that every column sees
+    auto load_q = [&](const Seg& sg) {
+        const TQ* q = static_cast<const TQ*>(a.q);
+#pragma unroll
+        for (int ct = 0; ct < NT; ct++) {
+            const int col = (sg.grp * NT + ct) * 16 + lc;
+            const bool real = col < sg.rows * n_rep;
+            const int i = real ? col / n_rep : 0, r = real ? col - i * n_rep : 0;
+            vis[ct] = real ? sg.kv - sg.rows + i + 1 : sg.kv;
+            const TQ* row = q + (int64_t)(sg.row0 + i) * a.q_st + (int64_t)(sg.g * n_rep + r) * a.q_sh;
+            if constexpr (std::is_same<TQ, f16_t>::value) {
+                qf[ct] = a.scale_log2;
+#pragma unroll
+                for (int kk = 0; kk < KK; kk++)
+                    qb[ct][0][kk] = real ? *reinterpret_cast<const u32x4*>(
+                                               row + 64 * (kk >> 1) + 16 * lg + 8 * (kk & 1))
+                                         : u32x4{0, 0, 0, 0};
+            } else {
+                float x[KK][8];
+                float top = 0.0f;
+#pragma unroll
+                for (int kk = 0; kk < KK; kk++) {
+                    const TQ* p = row + 64 * (kk >> 1) + 16 * lg + 8 * (kk & 1);
+                    if constexpr (sizeof(TQ) == 4) {
+                        const f32x4 u = *reinterpret_cast<const f32x4*>(p);
+                        const f32x4 v = *reinterpret_cast<const f32x4*>(p + 4);
+#pragma unroll
+                        for (int e = 0; e < 4; e++) x[kk][e] = u[e], x[kk][4 + e] = v[e];
+                    } else {
+                        const u32x4 u = *reinterpret_cast<const u32x4*>(p);
+#pragma unroll
+                        for (int e = 0; e < 4; e++)
+                            x[kk][2 * e] = lo_f32<TQ>(u[e]), x[kk][2 * e + 1] = hi_f32<TQ>(u[e]);
+                    }
+#pragma unroll
+                    for (int e = 0; e < 8; e++) top = fmaxf(top, fabsf(x[kk][e]));
+                }
+                top = max_across_rows(top);
+                // 2^up * top in [2^14, 2^15) (f16 holds twice that); infinities and NaN as they come
+                const int ex = (int)(__float_as_uint(top) >> 23);
+                const int up = top > 0.0f ? min(14 + 127 - ex, 126) : 0;
+                const float f = __uint_as_float((uint32_t)(up + 127) << 23);
+                qf[ct] = a.scale_log2 * __uint_as_float((uint32_t)(127 - up) << 23);
+#pragma unroll
+                for (int kk = 0; kk < KK; kk++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const float y0 = real ? x[kk][2 * e] * f : 0.0f;
+                        const float y1 = real ? x[kk][2 * e + 1] * f : 0.0f;
+                        const uint32_t hi = pack2<f16_t>(y0, y1);
+                        qb[ct][0][kk][e] = hi;
+                        if constexpr (QP == 2)
+                            qb[ct][1][kk][e] =
+                                pack2<f16_t>(y0 - lo_f32<f16_t>(hi), y1 - hi_f32<f16_t>(hi));
+                    }
+            }
+        }
+        min_vis = sg.kv - sg.rows + 1 + sg.grp * NT * 16 / n_rep;
+    };
+
+    float m[NT], lsum[NT], mv[NT];
+    f32x4 acc[NT][NV];
+    auto clear = [&]() {
+#pragma unroll
+        for (int ct = 0; ct < NT; ct++) {
+            m[ct] = mv[ct] = DEC_M0;
+            lsum[ct] = 0.0f;
+#pragma unroll
+            for (int nn = 0; nn < NV; nn++) acc[ct][nn] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        }
+    };
+    clear();
+
+    auto compute_chunk = [&](const Seg& sg, int c, const Scales& sc, u32x4 (*ka)[KL], Vd (*va)[4]) {
+        const int tok0 = c * CHUNK, tile0 = TILES * (c - sg.cb);
+        const bool full = tok0 + CHUNK <= min_vis;
+        if (tok0 + CHUNK > sg.kv) {  // tokens past the sequence: no bits of theirs
+#pragma unroll
+            for (int t = 0; t < TILES; t++)
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    if (tok0 + 16 * t + 4 * lg + j >= sg.kv) va[t][j] = Vd{};
+        }
+        f32x4 s[NT][TILES];
+#pragma unroll
+        for (int t = 0; t < TILES; t++) {
+            u32x4 kA[KK];
+#pragma unroll
+            for (int kk = 0; kk < KK; kk++) {
+                const u32x2 x = to_f16x4<TP>(ka[t][kk >> 1][2 * (kk & 1)]);
+                const u32x2 y = to_f16x4<TP>(ka[t][kk >> 1][2 * (kk & 1) + 1]);
+                kA[kk] = u32x4{x[0], x[1], y[0], y[1]};
+            }
+#pragma unroll
+            for (int ct = 0; ct < NT; ct++) {
+                f32x4 z = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int p = QP - 1; p >= 0; p--)
+#pragma unroll
+                    for (int kk = 0; kk < KK; kk++) z = mfma16x16x32<f16_t>(kA[kk], qb[ct][p][kk], z);
+                s[ct][t] = z;
+            }
+        }
+        float kf[TILES], lv[TILES];
+#pragma unroll
+        for (int t = 0; t < TILES; t++) {
+            kf[t] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(sc.k), tile0 + t));
+            lv[t] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(sc.v), tile0 + t));
+        }
+        u32x4 PH[NT][TILES / 2], PL[NT][TILES / 2];
+#pragma unroll
+        for (int ct = 0; ct < NT; ct++) {
+            float x[4 * TILES];  // scores
+            float top = -INFINITY, topv = -INFINITY;
+#pragma unroll
+            for (int t = 0; t < TILES; t++) {
+                const float f = qf[ct] * kf[t];
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    const bool ok = full || tok0 + 16 * t + 4 * lg + r < vis[ct];
+                    x[4 * t + r] = ok ? s[ct][t][r] * f : -INFINITY;
+                    top = fmaxf(top, x[4 * t + r]);
+                }
+            }
+            if constexpr (W) {
+                if (lc < n_rep - 16 * sg.grp) {
+                    float* to = a.scores +
+                                ((int64_t)sg.row0 * a.num_heads + sg.g * n_rep + 16 * sg.grp + lc) *
+                                    a.score_stride + tok0 + 4 * lg;
+#pragma unroll
+                    for (int t = 0; t < TILES; t++)
+                        *reinterpret_cast<f32x4*>(to + 16 * t) =
+                            f32x4{x[4 * t], x[4 * t + 1], x[4 * t + 2], x[4 * t + 3]};
+                }
+            }
+            const float m_new = fmaxf(m[ct], max_across_rows(top));
+            float psum = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 4 * TILES; i++) {
+                psum += fast_exp2(x[i] - m_new);
+                // (a position that the column does not see takes nothing from its block, a scale of NaN
+                // least of all)
+                const bool ok = full || tok0 + 16 * (i >> 2) + 4 * lg + (i & 3) < vis[ct];
+                x[i] = ok ? x[i] + lv[i >> 2] : -INFINITY;
+                topv = fmaxf(topv, x[i]);
+            }
+            lsum[ct] = lsum[ct] * fast_exp2(m[ct] - m_new) + psum;
+            m[ct] = m_new;
+            const float mv_new = fmaxf(mv[ct], max_across_rows(topv));
+            if (__builtin_amdgcn_ballot_w64(mv_new > mv[ct]) != 0) {
+                const float alpha = fast_exp2(mv[ct] - mv_new);
+#pragma unroll
+                for (int nn = 0; nn < NV; nn++) acc[ct][nn] *= alpha;
+            }
+            mv[ct] = mv_new;
+#pragma unroll
+            for (int i = 0; i < 4 * TILES; i += 2) {
+                const float p0 = fast_exp2(x[i] - mv_new + DP_SHIFT);
+                const float p1 = fast_exp2(x[i + 1] - mv_new + DP_SHIFT);
+                const uint32_t hi = pack2<f16_t>(p0, p1);
+                PH[ct][i >> 3][(i & 7) >> 1] = hi;
+                PL[ct][i >> 3][(i & 7) >> 1] =
+                    pack2<f16_t>(p0 - lo_f32<f16_t>(hi), p1 - hi_f32<f16_t>(hi));
+            }
+        }
+        // V^T: lane (lg, lc) holds dim (D / 16) lc + nn of tokens 4lg .. 4lg + 3 of two tiles
+#pragma unroll
+        for (int u = 0; u < TILES / 2; u++)
+#pragma unroll
+            for (int w = 0; w < NV / 4; w++) {
+                u32x4 A[4];  // of the dword's four dims
+#pragma unroll
+                for (int t = 0; t < 2; t++) {
+                    uint32_t r[4];
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        if constexpr (D == 128)
+                            r[j] = va[2 * u + t][j][w];
+                        else
+                            r[j] = va[2 * u + t][j];
+                    }
+                    // bytes (row 0, row 1) of dims 0 and 1, of dims 2 and 3; the same of rows 2 and 3
+                    const u32x2 a01 = to_f16x4<TP>(__builtin_amdgcn_perm(r[1], r[0], 0x05010400u));
+                    const u32x2 a23 = to_f16x4<TP>(__builtin_amdgcn_perm(r[1], r[0], 0x07030602u));
+                    const u32x2 b01 = to_f16x4<TP>(__builtin_amdgcn_perm(r[3], r[2], 0x05010400u));
+                    const u32x2 b23 = to_f16x4<TP>(__builtin_amdgcn_perm(r[3], r[2], 0x07030602u));
+                    A[0][2 * t] = a01[0], A[0][2 * t + 1] = b01[0];
+                    A[1][2 * t] = a01[1], A[1][2 * t + 1] = b01[1];
+                    A[2][2 * t] = a23[0], A[2][2 * t + 1] = b23[0];
+                    A[3][2 * t] = a23[1], A[3][2 * t + 1] = b23[1];
+                }
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+#pragma unroll
+                    for (int ct = 0; ct < NT; ct++) {
+                        f32x4& o = acc[ct][4 * w + e];
+                        o = mfma16x16x32<f16_t>(A[e], PH[ct][u], o);
+                        o = mfma16x16x32<f16_t>(A[e], PL[ct][u], o);
+                    }
+            }
+    };
+
+    // ---- a piece's end: lane (lg, lc) holds column lc, dims (D / 4) lg + NV r + nn
+    auto epilogue = [&](const Seg& sg, bool complete, bool first_piece) {
+        int lgo = lg;
+        asm volatile("" : "+v"(lgo));  // (addresses formed here, not kept through the stream)
+#pragma unroll
+        for (int ct = 0; ct < NT; ct++) {
+            const float l = sum_across_rows(lsum[ct]);
+            const int col = (sg.grp * NT + ct) * 16 + lc;
+            if (col >= sg.rows * n_rep) continue;
+            const int i = col / n_rep, r0 = col - i * n_rep;
+            const int h = sg.g * n_rep + r0;
+            if (complete) {
+                const float f = l == 0.0f ? 0.0f : fast_exp2(mv[ct] - m[ct] - DP_SHIFT) / l;
+                const int64_t at = (int64_t)(sg.row0 + i) * a.o_st + (int64_t)h * a.o_sh + (D / 4) * lgo;
+#pragma unroll
+                for (int r = 0; r < 4; r++)
+#pragma unroll
+                    for (int h4 = 0; h4 < NV; h4 += 4) {
+                        float v[4];
+#pragma unroll
+                        for (int e = 0; e < 4; e++)
+                            v[e] = l == 0.0f ? 0.0f : acc[ct][h4 + e][r] * f;
+                        store_run<4>(a.out, a.out_dtype, at + NV * r + h4, v);
+                    }
+                if constexpr (W)
+                    if (lg == 0) {
+                        float* ml = a.ml + 2 * ((int64_t)(sg.row0 + i) * a.num_heads + h);
+                        ml[0] = m[ct];
+                        ml[1] = l;
+                    }
+            } else {
+                const int64_t slot = (2 * wgi + (first_piece ? 0 : 1)) * (16 * NT) + 16 * ct + lc;
+                float* o = a.p_o + slot * D + (D / 4) * lgo;
+#pragma unroll
+                for (int r = 0; r < 4; r++)
+#pragma unroll
+                    for (int h4 = 0; h4 < NV; h4 += 4)
+                        *reinterpret_cast<f32x4*>(o + NV * r + h4) =
+                            f32x4{acc[ct][h4][r], acc[ct][h4 + 1][r], acc[ct][h4 + 2][r],
+                                  acc[ct][h4 + 3][r]};
+                if (lg == 0) {
+                    a.p_ml[3 * slot] = m[ct];
+                    a.p_ml[3 * slot + 1] = l;
+                    a.p_ml[3 * slot + 2] = mv[ct];
+                }
+            }
+        }
+        clear();
+    };
+
+    // ---- the stream. A segment's ids are requested two segments ahead, its scales one ahead (they
+    // need the ids), and every chunk's rows one chunk ahead; waits are in the order of the requests.
+    auto log_scales = [&](Scales s) -> Scales { return Scales{s.k, __builtin_amdgcn_logf(s.v)}; };
+    Seg cur = seg_at(0);
+    Slots cur_slots = seg_slots(cur);
+    int nx = cur.ce - cur.cb;
+    bool has_nxt = nx < len;
+    Seg nxt = cur;
+    Slots nxt_slots{0, 0};
+    if (has_nxt) {
+        nxt = seg_at(nx);
+        nxt_slots = seg_slots(nxt);
+    }
+    load_q(cur);
+    Scales cur_raw = seg_scales(cur, cur_slots);
+    u32x4 ka[TILES][KL], kb[TILES][KL];
+    Vd va[TILES][4], vb[TILES][4];
+    load_chunk(cur.g, cur_slots, 0, ka, va);
+    Scales nxt_raw = cur_raw;
+    if (has_nxt) nxt_raw = seg_scales(nxt, nxt_slots);
+    Scales cur_sc = log_scales(cur_raw);
+    int pc0 = cur.cb;
+    bool first_piece = true;
+    int c = cur.cb;
+
+    auto step = [&](auto prefetch, u32x4 (*kc)[KL], Vd (*vc)[4], u32x4 (*kn)[KL], Vd (*vn)[4]) {
+        const bool seg_end = c + 1 >= cur.ce;
+        int nn_x = nx;
+        bool has_nn = false;
+        Seg nn = nxt;
+        Slots nn_slots = nxt_slots;
+        if (seg_end && has_nxt) {
+            nn_x = nx + (nxt.ce - nxt.cb);
+            has_nn = nn_x < len;
+            if (has_nn) {
+                nn = seg_at(nn_x);
+                nn_slots = seg_slots(nn);
+            }
+        }
+        if constexpr (decltype(prefetch)::value) {
+            const bool in_cur = c + 1 < cur.ce;
+            const Slots ps = in_cur ? cur_slots : nxt_slots;
+            load_chunk(in_cur ? cur.g : nxt.g, ps, in_cur ? TILES * (c + 1 - cur.cb) : 0, kn, vn);
+        }
+        compute_chunk(cur, c, cur_sc, kc, vc);
+        if (!seg_end) {
+            c += 1;
+            return;
+        }
+        const bool piece_end =
+            !has_nxt || nxt.b != cur.b || nxt.g != cur.g || nxt.grp != cur.grp;
+        if (piece_end) epilogue(cur, pc0 == 0 && cur.ce == cur.nch, first_piece);
+        if (!has_nxt) return;
+        if (piece_end) {
+            pc0 = nxt.cb;
+            first_piece = false;
+            load_q(nxt);
+        }
+        cur = nxt;
+        cur_slots = nxt_slots;
+        cur_sc = log_scales(nxt_raw);
+        c = cur.cb;
+        nx = nn_x;
+        has_nxt = has_nn;
+        if (has_nn) {
+            nxt = nn;
+            nxt_slots = nn_slots;
+            nxt_raw = seg_scales(nxt, nxt_slots);
+        }
+    };
+    using pf_on = std::integral_constant<bool, true>;
+    using pf_off = std::integral_constant<bool, false>;
+    int remaining = len;
+    for (; remaining > 2; remaining -= 2) {
+        step(pf_on{}, ka, va, kb, vb);
+        step(pf_on{}, kb, vb, ka, va);
+    }
+    if (remaining == 2) {
+        step(pf_on{}, ka, va, kb, vb);
+        step(pf_off{}, kb, vb, ka, va);
+    } else {
+        step(pf_off{}, ka, va, kb, vb);
+    }
+}
+
+// Merge of the pieces of cut pairs, and the rows that see nothing: one workgroup a (query head, packed
+// row), its waves sharing the pieces; lane i owns dims (D / 64) i .. .
+static constexpr int DP_MERGE_WAVES = 8;
+template <int D, int TILES, int NT, bool W>
+__global__ __launch_bounds__(64 * DP_MERGE_WAVES) void decode_pools_merge_kernel(DpArgs a, int cap) {
+    constexpr int E = D / 64, CHUNK = 16 * TILES;
+    const int h = blockIdx.x, row = blockIdx.y, lane = threadIdx.x & 63;
+    const int w_id = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
+    int s = row;
+    if (a.cu) s = wave_find_last(a.batch, row, [&](int i) -> int64_t { return a.cu[i]; });
+    const DpSeq q = dp_seq(a.cu, a.kv_lens, a.max_kv, s);
+    const int i = row - q.row0;
+    if (i < 0 || i >= q.rows) return;  // (rows of no sequence)
+    const int64_t at = (int64_t)row * a.o_st + (int64_t)h * a.o_sh + E * lane;
+    auto put = [&](const float* v) {
+#pragma unroll
+        for (int e = 0; e < E; e++) {
+            if (a.out_dtype == FLOUR_DTYPE_F32)
+                static_cast<float*>(a.out)[at + e] = v[e];
+            else if (a.out_dtype == FLOUR_DTYPE_BF16)
+                static_cast<bf16_t*>(a.out)[at + e] = from_f32<bf16_t>(v[e]);
+            else
+                static_cast<f16_t*>(a.out)[at + e] = from_f32<f16_t>(v[e]);
+        }
+    };
+    if (q.kv == 0) {
+        const float zero[E] = {};
+        if (w_id == 0) put(zero);
+        if (W && threadIdx.x == 0) {
+            a.ml[2 * ((int64_t)row * a.num_heads + h)] = DEC_M0;
+            a.ml[2 * ((int64_t)row * a.num_heads + h) + 1] = 0.0f;
+        }
+        return;
+    }
+    const int n_rep = a.n_rep, g = h / n_rep, col = i * n_rep + (h - g * n_rep);
+    const int grp = col / (16 * NT), cc = col - grp * (16 * NT);
+    const int groups = dp_groups<NT>(q.rows, n_rep), nch = (q.kv + CHUNK - 1) / CHUNK;
+    const int64_t total = (int64_t)a.kv_heads * a.pre[a.batch], nwg = range_count(total, cap);
+    const int64_t from = (int64_t)a.kv_heads * a.pre[s] + ((int64_t)g * groups + grp) * nch;
+    const int64_t to = from + nch;
+    const bool narrow = ranges_narrow(total, nwg, DP_XCD_W);
+    const WaveRanges<uint32_t> r32(narrow ? total : 1, nwg, DP_XCD_W);
+    const WaveRanges<int64_t> r64(total, nwg, DP_XCD_W);
+    const int64_t f = narrow ? (int64_t)r32.owner((uint32_t)from) : r64.owner(from);
+    const int64_t l = narrow ? (int64_t)r32.owner((uint32_t)(to - 1)) : r64.owner(to - 1);
+    if (f == l) return;  // finished inside one wave range
+    const bool f_first = from == (narrow ? (int64_t)r32.lo((uint32_t)f) : r64.lo(f));
+    const int np = (int)(l - f + 1);
+    auto slot_of = [&](int p) -> int64_t {  // (the last piece of a range but the first: its second)
+        return (2 * (f + p) + (p == 0 && !f_first ? 1 : 0)) * (16 * NT) + cc;
+    };
+    float M = DEC_M0, MV = DEC_M0, L = 0.0f, O[E] = {};
+    const int per = (np + waves - 1) / waves, p_end = min(np, (w_id + 1) * per);
+    for (int p0 = w_id * per; p0 < p_end; p0 += 64) {
+        const bool on = p0 + lane < p_end;
+        const int64_t sl = slot_of(on ? p0 + lane : p0);
+        const float mx = on ? a.p_ml[3 * sl] : DEC_M0, mvx = on ? a.p_ml[3 * sl + 2] : DEC_M0;
+        const float lx = on ? a.p_ml[3 * sl + 1] : 0.0f;
+        const float Mn = fmaxf(M, wave_max(mx)), MVn = fmaxf(MV, wave_max(mvx));
+        L = L * fast_exp2(M - Mn) + wave_sum(on ? fast_exp2(mx - Mn) * lx : 0.0f);
+        const float w = on ? fast_exp2(mvx - MVn) : 0.0f, old = fast_exp2(MV - MVn);
+#pragma unroll
+        for (int e = 0; e < E; e++) O[e] *= old;
+        const int n = min(64, p_end - p0);
+        for (int x = 0; x < n; x += 8) {
+            float v[8][E];
+#pragma unroll
+            for (int y = 0; y < 8; y++) {  // loads together; past the end the first piece again
+                const float* o = a.p_o + slot_of(p0 + (x + y < n ? x + y : 0)) * D + E * lane;
+#pragma unroll
+                for (int e = 0; e < E; e++) v[y][e] = o[e];
+            }
+#pragma unroll
+            for (int y = 0; y < 8; y++) {
+                const float wy = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w), (x + y) & 63));
+                if (x + y < n)
+#pragma unroll
+                    for (int e = 0; e < E; e++) O[e] = fmaf(wy, v[y][e], O[e]);
+            }
+        }
+        M = Mn;
+        MV = MVn;
+    }
+    if (waves > 1) {
+        __shared__ float wM[DP_MERGE_WAVES][3], wO[DP_MERGE_WAVES][E][64];
+        if (lane == 0) wM[w_id][0] = M, wM[w_id][1] = L, wM[w_id][2] = MV;
+#pragma unroll
+        for (int e = 0; e < E; e++) wO[w_id][e][lane] = O[e];
+        __syncthreads();
+        if (w_id != 0) return;
+        for (int x = 1; x < waves; x++) {  // (a wave without pieces: sum 0 at the lowest maximum)
+            const float Mn = fmaxf(M, wM[x][0]), MVn = fmaxf(MV, wM[x][2]);
+            L = L * fast_exp2(M - Mn) + wM[x][1] * fast_exp2(wM[x][0] - Mn);
+            const float c0 = fast_exp2(MV - MVn), c1 = fast_exp2(wM[x][2] - MVn);
+#pragma unroll
+            for (int e = 0; e < E; e++) O[e] = O[e] * c0 + wO[x][e][lane] * c1;
+            M = Mn;
+            MV = MVn;
+        }
+    }
+    float v[E];
+#pragma unroll
+    for (int e = 0; e < E; e++)
+        v[e] = L == 0.0f ? 0.0f : O[e] * (fast_exp2(MV - M - DP_SHIFT) / L);
+    put(v);
+    if (W && lane == 0) {
+        a.ml[2 * ((int64_t)row * a.num_heads + h)] = M;
+        a.ml[2 * ((int64_t)row * a.num_heads + h) + 1] = L;
+    }
+}
+
+static constexpr size_t up256(size_t x) { return (x + 255) & ~(size_t)255; }
+
+static int stream_waves() { return std::min(device_cus() * 4, 4096); }
+
+// Workspace of a streamed call of `cols` columns a group.
+static size_t stream_bytes(int batch, int cols, int head_dim) {
+    const size_t slots = 2 * (size_t)stream_waves() * cols;
+    return up256(slots * 3 * sizeof(float)) + up256(slots * head_dim * sizeof(float)) +
+           up256(((size_t)batch + 1) * sizeof(int));
+}
+
+bool decode_stream_takes(const PoolAttn& a) {
+    const int es = elem_bytes(a.dtype), oes = elem_bytes(a.out_dtype);
+    return valid_pool8(a.pool_dtype) && (a.head_dim == 64 || a.head_dim == 128) &&
+           a.block_size % 16 == 0 && a.batch <= DP_MAX_BATCH && a.rows <= 65535 &&
+           a.num_slots * a.head_dim <= (int64_t)0x7fffffff &&
+           (((uintptr_t)a.q | (uintptr_t)a.out | (uintptr_t)a.k_pool | (uintptr_t)a.v_pool |
+             (uint64_t)(a.q_st * es) | (uint64_t)(a.q_sh * es) | (uint64_t)(a.o_st * oes) |
+             (uint64_t)(a.o_sh * oes)) & 15) == 0;
+}
+
+size_t decode_stream_bytes(int batch, int max_cols, int head_dim) {
+    return head_dim == 64 || head_dim == 128
+               ? stream_bytes(batch, max_cols <= 16 ? 16 : max_cols <= 32 ? 32 : 64, head_dim) : 0;
+}
+
+template <typename TQ, typename TP, int D, int TILES, int NT, bool W>
+static int launch_stream(const DpArgs& a, int max_rows, int rows, hipStream_t stream) {
+    const int64_t groups = ((int64_t)max_rows * a.n_rep + 16 * NT - 1) / (16 * NT);
+    const int64_t chunks = (a.max_kv + 16 * TILES - 1) / (16 * TILES);
+    const int64_t half = (int64_t)a.batch * a.kv_heads * groups * chunks / 2;
+    const int per_cu = 3, cap = std::min(device_cus() * per_cu, 4096);
+    const int grid = (int)std::max<int64_t>(1, std::min<int64_t>(half, cap));
+    const size_t lds = a.batch <= 64 ? 0 : (size_t)(a.batch + 1) * sizeof(int);
+    auto kern = a.block_size == 16 ? decode_pools_kernel<TQ, TP, D, TILES, NT, true, W>
+                                   : decode_pools_kernel<TQ, TP, D, TILES, NT, false, W>;
+    kern<<<dim3(grid), dim3(64), lds, stream>>>(a);
+    const int rc = check_hip(hipGetLastError(), "8-bit decode launch");
+    if (rc != FLOUR_OK) return rc;
+    const int64_t pieces = 2 * (int64_t)grid / ((int64_t)a.batch * a.kv_heads);
+    int waves = 1;
+    while (waves < DP_MERGE_WAVES && 8 * waves < pieces) waves *= 2;
+    decode_pools_merge_kernel<D, TILES, NT, W>
+        <<<dim3(a.num_heads, rows), dim3(64 * waves), 0, stream>>>(a, grid);
+    return check_hip(hipGetLastError(), "8-bit decode merge launch");
+}
+
+template <typename TQ, typename TP, int D>
+static int launch_stream_d(const DpArgs& a, int max_rows, int rows, hipStream_t s) {
+    if (a.scores) return launch_stream<TQ, TP, D, 4, 1, true>(a, max_rows, rows, s);
+    return launch_stream<TQ, TP, D, 4, 1, false>(a, max_rows, rows, s);
+}
+
+int launch_decode_stream(const PoolAttn& p, int max_rows, void* workspace, hipStream_t stream) {
+    DpArgs a{};
+    a.out = p.out, a.out_dtype = p.out_dtype, a.o_st = p.o_st, a.o_sh = p.o_sh;
+    a.q = p.q, a.q_st = p.q_st, a.q_sh = p.q_sh;
+    a.k_pool = static_cast<const uint8_t*>(p.k_pool);
+    a.v_pool = static_cast<const uint8_t*>(p.v_pool);
+    a.k_scale = p.k_scale, a.v_scale = p.v_scale;
+    a.cu = p.cu, a.kv_lens = p.kv_lens, a.block_tables = p.block_tables;
+    a.max_blocks = p.max_blocks, a.batch = p.batch, a.num_heads = p.num_heads;
+    a.kv_heads = p.kv_heads, a.n_rep = p.num_heads / p.kv_heads, a.block_size = p.block_size;
+    a.num_slots = p.num_slots, a.scale_log2 = p.scale * LOG2_E;
+    a.max_kv = (int)std::min<int64_t>(p.max_kv, (int64_t)p.max_blocks * p.block_size);
+    a.scores = p.scores, a.score_stride = p.score_stride, a.ml = p.ml;
+    const int cols = 16;
+    const size_t slots = 2 * (size_t)stream_waves() * cols;
+    char* ws = static_cast<char*>(workspace);
+    a.p_ml = reinterpret_cast<float*>(ws);
+    ws += up256(slots * 3 * sizeof(float));
+    a.p_o = reinterpret_cast<float*>(ws);
+    ws += up256(slots * p.head_dim * sizeof(float));
+    a.pre = reinterpret_cast<int*>(ws);
+#define FLOUR_DS(TQ)                                                                              \
+    (p.pool_dtype == FLOUR_DTYPE_E4M3                                                             \
+         ? (p.head_dim == 64 ? launch_stream_d<TQ, e4m3_t, 64>(a, max_rows, p.rows, stream)       \
+                             : launch_stream_d<TQ, e4m3_t, 128>(a, max_rows, p.rows, stream))     \
+         : (p.head_dim == 64 ? launch_stream_d<TQ, i8_t, 64>(a, max_rows, p.rows, stream)         \
+                             : launch_stream_d<TQ, i8_t, 128>(a, max_rows, p.rows, stream)))
+    if (p.dtype == FLOUR_DTYPE_F32) return FLOUR_DS(float);
+    if (p.dtype == FLOUR_DTYPE_BF16) return FLOUR_DS(bf16_t);
+    return FLOUR_DS(f16_t);
+#undef FLOUR_DS
+}
+
+}  // namespace flour

@@ -105,7 +105,9 @@ __global__ __launch_bounds__(64 * KQ_WAVES) void kv_write_q8_kernel(
         const int i = x / runs;
         float y[N];
         load_run<T, N>(src + i * st + (x - i * runs) * N, y);
-        // (a block of scale NaN: zeros, which read as NaN)
+        if (!(S >= 0.0f))  // a block of scale NaN holds zeros: only those that attend to it see NaN
+#pragma unroll
+            for (int j = 0; j < N; j++) y[j] = 0.0f;
         store_run8<TP, N>(dst + (int64_t)x * N, y, inv);
     }
     if (S != old && S > 0.0f) {  // the kept rows, if the scale grew
