@@ -2,7 +2,7 @@
 // attention-weight sums where they are asked for.
 //
 // The kernels that every other one is checked against, and what runs where the streamed decode
-// (decode_pools.hip) does not take a shape: any head_dim up to 512, block size, group size,
+// (decode_stream.h) does not take a shape: any head_dim up to 512, block size, group size,
 // alignment. One workgroup a (row, query head): 256 positions at a time, a thread's whole dot
 // product each, then a thread's output dims each over the 256 weights in LDS.
 #include <math.h>
@@ -203,189 +203,3 @@ int launch_attn_pools(const PoolAttn& a, hipStream_t stream) {
 }
 
 }  // namespace flour
-
-using namespace flour;
-
-namespace flour {
-
-static size_t up256(size_t x) { return (x + 255) & ~(size_t)255; }
-
-static int64_t score_stride_of(int max_ctx) { return ((int64_t)max_ctx + 63) / 64 * 64; }
-
-// Scores and their maxima and sums, behind the streamed kernel's part.
-static size_t weights_bytes(int batch, int num_heads, int max_ctx) {
-    const size_t rows = (size_t)batch * num_heads;
-    return up256(rows * 2 * sizeof(float)) + up256(rows * score_stride_of(max_ctx) * sizeof(float));
-}
-
-static int decode_pools(const char* what, PoolAttn a, float* weights, int64_t width,
-                        const int32_t* weight_rows, int num_rows, void* workspace,
-                        size_t workspace_bytes, hipStream_t stream) {
-    if (!valid_dtype(a.dtype) || !valid_dtype(a.out_dtype)) {
-        set_error("%s: unknown dtype (%d, out %d)", what, a.dtype, a.out_dtype);
-        return FLOUR_ERR_INVALID_ARGUMENT;
-    }
-    if (a.batch < 0 || a.num_heads <= 0 || a.kv_heads <= 0 || a.num_heads % a.kv_heads != 0 ||
-        a.head_dim <= 0 || a.block_size <= 0 || a.num_slots <= 0 ||
-        a.num_slots % a.block_size != 0 || a.max_blocks <= 0 || a.max_kv < 0 ||
-        (int64_t)a.max_kv > (int64_t)a.max_blocks * a.block_size) {
-        set_error("%s: bad shape (batch=%d heads=%d kv_heads=%d head_dim=%d bs=%d num_slots=%lld "
-                  "max_blocks=%d max_ctx=%d)",
-                  what, a.batch, a.num_heads, a.kv_heads, a.head_dim, a.block_size,
-                  (long long)a.num_slots, a.max_blocks, a.max_kv);
-        return FLOUR_ERR_INVALID_ARGUMENT;
-    }
-    if (weights && (width < a.max_kv || num_rows < 0 || (!weight_rows && num_rows < a.batch))) {
-        set_error("%s: weights of %d rows of width %lld for %d sequences of up to %d positions",
-                  what, num_rows, (long long)width, a.batch, a.max_kv);
-        return FLOUR_ERR_INVALID_ARGUMENT;
-    }
-    if (a.batch == 0) return FLOUR_OK;
-    if (!a.out || !a.q || !a.k_pool || !a.v_pool || !a.block_tables || !a.kv_lens) {
-        set_error("%s: null pointer", what);
-        return FLOUR_ERR_INVALID_ARGUMENT;
-    }
-    const int n_rep = a.num_heads / a.kv_heads;
-    const size_t stream_part = decode_stream_bytes(a.batch, n_rep, a.head_dim);
-    const size_t need =
-        stream_part + (weights ? weights_bytes(a.batch, a.num_heads, a.max_kv) : 0);
-    if (need > 0 && (!workspace || workspace_bytes < need || (uintptr_t)workspace % 256 != 0)) {
-        set_error("%s: workspace of %zu bytes (256-byte aligned) required, got %zu at %p", what,
-                  need, workspace_bytes, workspace);
-        return FLOUR_ERR_WORKSPACE;
-    }
-    a.rows = a.batch;
-    a.q_st = a.o_st = (int64_t)a.num_heads * a.head_dim;
-    a.q_sh = a.o_sh = a.head_dim;
-    if (weights) {
-        char* ws = static_cast<char*>(workspace) + stream_part;
-        a.ml = reinterpret_cast<float*>(ws);
-        a.scores = reinterpret_cast<float*>(
-            ws + up256((size_t)a.batch * a.num_heads * 2 * sizeof(float)));
-        a.score_stride = score_stride_of(a.max_kv);
-    }
-    const int rc = decode_stream_takes(a) ? launch_decode_stream(a, 1, workspace, stream)
-                                          : launch_attn_pools(a, stream);
-    if (rc != FLOUR_OK || !weights) return rc;
-    return launch_weights_add(weights, width, weight_rows, num_rows, a.kv_lens, a.max_kv, a.batch,
-                              a.kv_heads, n_rep, a.scores, a.score_stride, a.ml, stream);
-}
-
-}  // namespace flour
-
-extern "C" int flour_hip_decode_weights_workspace_size(int batch, int num_heads, int kv_heads,
-                                                       int head_dim, int max_context_len,
-                                                       int with_weights, size_t* bytes) {
-    clear_error();
-    if (!bytes || batch < 0 || num_heads <= 0 || kv_heads <= 0 || num_heads % kv_heads != 0 ||
-        head_dim <= 0 || max_context_len < 0) {
-        set_error("decode_weights_workspace_size: bad arguments");
-        return FLOUR_ERR_INVALID_ARGUMENT;
-    }
-    *bytes = decode_stream_bytes(batch, num_heads / kv_heads, head_dim) +
-             (with_weights ? weights_bytes(batch, num_heads, max_context_len) : 0);
-    return FLOUR_OK;
-}
-
-extern "C" int flour_hip_paged_decode_q8(
-    void* out, int out_dtype, const void* q, int dtype, const void* k_pool, const void* v_pool,
-    const float* k_scale, const float* v_scale, int pool_dtype, const int32_t* block_tables,
-    int max_blocks_per_seq, const int32_t* context_lens, int batch, int num_heads, int kv_heads,
-    int head_dim, int block_size, int64_t num_slots, int max_context_len, float scale,
-    float* weights, int64_t weights_width, const int32_t* weight_rows, int num_weight_rows,
-    void* workspace, size_t workspace_bytes, void* stream) {
-    clear_error();
-    if (!check_pool8("paged_decode_q8", pool_dtype, k_pool, v_pool, k_scale, v_scale, kv_heads,
-                     head_dim, block_size, num_slots))
-        return FLOUR_ERR_INVALID_ARGUMENT;
-    PoolAttn a{};
-    a.out = out, a.out_dtype = out_dtype, a.q = q, a.dtype = dtype;
-    a.k_pool = k_pool, a.v_pool = v_pool, a.k_scale = k_scale, a.v_scale = v_scale;
-    a.pool_dtype = pool_dtype, a.block_tables = block_tables, a.max_blocks = max_blocks_per_seq;
-    a.kv_lens = context_lens, a.batch = batch, a.num_heads = num_heads, a.kv_heads = kv_heads;
-    a.head_dim = head_dim, a.block_size = block_size, a.num_slots = num_slots;
-    a.max_kv = max_context_len, a.scale = scale;
-    return decode_pools("paged_decode_q8", a, weights, weights_width, weight_rows, num_weight_rows,
-                        workspace, workspace_bytes, static_cast<hipStream_t>(stream));
-}
-
-extern "C" int flour_hip_paged_decode_weights(
-    void* out, int out_dtype, const void* q, const void* k_pool, const void* v_pool,
-    const int32_t* block_tables, int max_blocks_per_seq, const int32_t* context_lens, int batch,
-    int num_heads, int kv_heads, int head_dim, int block_size, int64_t num_slots,
-    int max_context_len, float scale, int dtype, float* weights, int64_t weights_width,
-    const int32_t* weight_rows, int num_weight_rows, void* workspace, size_t workspace_bytes,
-    void* stream) {
-    clear_error();
-    if (!weights) {
-        set_error("paged_decode_weights: null weights");
-        return FLOUR_ERR_INVALID_ARGUMENT;
-    }
-    PoolAttn a{};
-    a.out = out, a.out_dtype = out_dtype, a.q = q, a.dtype = dtype;
-    a.k_pool = k_pool, a.v_pool = v_pool, a.pool_dtype = dtype;
-    a.block_tables = block_tables, a.max_blocks = max_blocks_per_seq;
-    a.kv_lens = context_lens, a.batch = batch, a.num_heads = num_heads, a.kv_heads = kv_heads;
-    a.head_dim = head_dim, a.block_size = block_size, a.num_slots = num_slots;
-    a.max_kv = max_context_len, a.scale = scale;
-    return decode_pools("paged_decode_weights", a, weights, weights_width, weight_rows,
-                        num_weight_rows, workspace, workspace_bytes,
-                        static_cast<hipStream_t>(stream));
-}
-
-extern "C" int flour_hip_varlen_prefill_q8_workspace_size(int num_seqs, int max_seqlen_q,
-                                                          int total_q, int max_kv_len,
-                                                          int num_heads, int kv_heads,
-                                                          int head_dim, int block_size, int dtype,
-                                                          size_t* bytes) {
-    clear_error();
-    if (!bytes || num_seqs < 0 || max_seqlen_q < 0 || total_q < 0 || max_kv_len < 0 ||
-        num_heads <= 0 || kv_heads <= 0 || num_heads % kv_heads != 0 || head_dim <= 0 ||
-        block_size <= 0 || !valid_dtype(dtype)) {
-        set_error("varlen_prefill_q8_workspace_size: bad arguments");
-        return FLOUR_ERR_INVALID_ARGUMENT;
-    }
-    *bytes = 0;
-    return FLOUR_OK;
-}
-
-extern "C" int flour_hip_varlen_prefill_q8(
-    void* out, int out_dtype, int64_t o_stride_tok, int64_t o_stride_head, const void* q,
-    int64_t q_stride_tok, int64_t q_stride_head, int dtype, const void* k_pool, const void* v_pool,
-    const float* k_scale, const float* v_scale, int pool_dtype, const int32_t* cu_seqlens_q,
-    const int32_t* kv_lens, const int32_t* block_tables, int max_blocks_per_seq, int num_seqs,
-    int max_seqlen_q, int total_q, int num_heads, int kv_heads, int head_dim, int block_size,
-    int64_t num_slots, int max_kv_len, float scale, void* workspace, size_t workspace_bytes,
-    void* stream) {
-    clear_error();
-    if (!valid_dtype(dtype) || !valid_dtype(out_dtype)) {
-        set_error("varlen_prefill_q8: unknown dtype (%d, out %d)", dtype, out_dtype);
-        return FLOUR_ERR_INVALID_ARGUMENT;
-    }
-    if (!check_pool8("varlen_prefill_q8", pool_dtype, k_pool, v_pool, k_scale, v_scale, kv_heads,
-                     head_dim, block_size, num_slots))
-        return FLOUR_ERR_INVALID_ARGUMENT;
-    if (num_seqs < 0 || total_q < 0 || max_seqlen_q < 0 || num_heads <= 0 ||
-        num_heads % kv_heads != 0 || max_blocks_per_seq <= 0 || max_kv_len < 0 ||
-        (int64_t)max_kv_len > (int64_t)max_blocks_per_seq * block_size) {
-        set_error("varlen_prefill_q8: bad shape (seqs=%d total_q=%d max_q=%d heads=%d kv_heads=%d "
-                  "max_blocks=%d max_kv=%d)",
-                  num_seqs, total_q, max_seqlen_q, num_heads, kv_heads, max_blocks_per_seq,
-                  max_kv_len);
-        return FLOUR_ERR_INVALID_ARGUMENT;
-    }
-    if (num_seqs == 0 || total_q == 0) return FLOUR_OK;
-    if (!out || !q || !cu_seqlens_q || !kv_lens || !block_tables) {
-        set_error("varlen_prefill_q8: null pointer");
-        return FLOUR_ERR_INVALID_ARGUMENT;
-    }
-    PoolAttn a{};
-    a.out = out, a.out_dtype = out_dtype, a.o_st = o_stride_tok, a.o_sh = o_stride_head;
-    a.q = q, a.dtype = dtype, a.q_st = q_stride_tok, a.q_sh = q_stride_head;
-    a.k_pool = k_pool, a.v_pool = v_pool, a.k_scale = k_scale, a.v_scale = v_scale;
-    a.pool_dtype = pool_dtype, a.cu = cu_seqlens_q, a.kv_lens = kv_lens;
-    a.block_tables = block_tables, a.max_blocks = max_blocks_per_seq, a.batch = num_seqs;
-    a.rows = total_q, a.num_heads = num_heads, a.kv_heads = kv_heads, a.head_dim = head_dim;
-    a.block_size = block_size, a.num_slots = num_slots, a.max_kv = max_kv_len, a.scale = scale;
-    return launch_attn_pools(a, static_cast<hipStream_t>(stream));
-}

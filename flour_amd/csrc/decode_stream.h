@@ -1,5 +1,6 @@
-// decode_pools.hip — attention of few query rows over an 8-bit cache, streamed from HBM on the f16
-// matrix cores: decode steps and short runs of new rows (drafted tokens, short turns).
+// decode_stream.h — attention of few query rows over an 8-bit cache, streamed from HBM on the f16
+// matrix cores: decode steps and short runs of new rows (drafted tokens, short turns). Instantiated
+// per type of the queries in decode_stream_*.hip.
 //
 // With few rows per sequence the step reads each K/V byte once and is bound by that; everything
 // else has to fit beside the stream. Work split: as in paged_decode.hip, the chunks of every
@@ -10,21 +11,25 @@
 // tiles to a wave:
 //  * A chunk is TILES tiles of 16 tokens, 2 KB of K and of V each at head_dim 128. Two register
 //    buffers: the next chunk's loads are in flight while one is computed.
-//  * S = K Q^T on v_mfma_f32_16x16x32_f16. K is loaded in the A layout as it lies in memory: lane
-//    (g, c) = (lane / 16, lane % 16) holds bytes 16g .. of token c's row, and the columns of Q^T are
-//    permuted to match, so K passes through no LDS. Bytes become f16 exactly: e4m3 by the
-//    converter, int8 by placing x + 128 under the exponent of 1,024 and subtracting 1,152.
+//  * S = K Q^T on v_mfma_f32_16x16x32_f16. K is loaded as it lies in memory, 1 KB an instruction, and
+//    turned into the A layout (lane (g, c) = (lane / 16, lane % 16): bytes 16g .. of token c's row, the
+//    columns of Q^T permuted to match) through LDS. Loaded in that layout, a 64-byte half of 16 rows an
+//    instruction, the stream alone stops at 4.2-4.6 TB/s against 4.9-5.3. Bytes become f16 exactly:
+//    e4m3 by the converter, int8 by placing x + 128 under the exponent of 1,024 and subtracting 1,152.
 //  * Queries are f16: f16 ones as they are; bf16 ones times a power of two per (row, head) that puts
 //    the largest element just below 2^15 (exact down to 2^-31 of it); fp32 ones as two f16 parts of that
 //    (22 bits, two products).
 //  * A block's K scale multiplies its 16 tokens' scores, one factor per tile. Its V scale S_v goes
 //    into the exponent: P' = 2^(s + log2 S_v - m'), with a running maximum m' of its own beside the
-//    maximum m of s that the sum of 2^(s - m) uses. So P' stays in (0, 1], f16 keeps it exact relative to
-//    the row's largest contribution whatever the blocks' scales, and V stays the integers and
-//    e4m3 values that it is. P' is scaled by 2^14 (clear of f16's subnormals) and split into two f16
-//    parts: two products, 22 bits.
+//    maximum m of s that the sum of p = 2^(s - m) uses, formed as p times a factor per tile. So P'
+//    stays in (0, 1], f16 keeps it relative to the row's largest contribution whatever the blocks'
+//    scales (up to 2^100 apart, where p leaves fp32's range), and V stays the integers and e4m3 values
+//    that it is. P' is scaled by 2^14 (clear of f16's subnormals) and split into two f16 parts: two
+//    products, 22 bits.
 //  * The score registers are the B operand of O^T = V^T P'^T as they stand; the V^T operand is built
 //    in-lane, pairs of tokens' bytes by v_perm_b32, then the same conversion.
+#pragma once
+
 #include <math.h>
 
 #include <algorithm>
@@ -39,35 +44,15 @@ static constexpr int DP_MAX_BATCH = 4096;  // per-sequence chunk sums live in LD
 static constexpr float DP_SHIFT = 14.0f;   // P' times 2^14
 static constexpr int DP_XCD_W = 2;         // the wave ranges' weight (paged_decode.hip)
 
-struct DpArgs {
-    void* out;
-    int out_dtype;
-    int64_t o_st, o_sh;
-    const void* q;
-    int64_t q_st, q_sh;
-    const uint8_t *k_pool, *v_pool;
-    const float *k_scale, *v_scale;
-    const int32_t *cu, *kv_lens, *block_tables;
-    int max_blocks, batch, num_heads, kv_heads, n_rep, block_size;
-    int64_t num_slots;
-    int max_kv;
-    float scale_log2;
-    float* scores;  // kept scores (or null): (batch, num_heads, score_stride)
-    int64_t score_stride;
-    float* ml;    // with scores: (batch, num_heads, 2)
-    float* p_ml;  // pieces: [2 * waves][16 NT][3] maximum, sum, maximum with the V scales
-    float* p_o;   // pieces: [2 * waves][16 NT][D]
-    int* pre;     // [batch + 1] chunks per kv head of the sequences before
-};
-
 // Rows of sequence s, its kv length (0 where its rows see nothing).
 struct DpSeq {
     int row0, rows, kv;
 };
-__device__ __forceinline__ DpSeq dp_seq(const int32_t* cu, const int32_t* kv_lens, int max_kv, int s) {
-    const int r0 = cu ? cu[s] : s, n = cu ? cu[s + 1] - r0 : 1;
-    const int kv = min(kv_lens[s], max_kv);
-    return DpSeq{r0, max(n, 0), kv >= n && kv > 0 ? kv : 0};
+__device__ __forceinline__ DpSeq dp_seq(const DpArgs& a, int s) {
+    const int r0 = a.cu ? a.cu[s] : s, n = a.cu ? a.cu[s + 1] - r0 : 1;
+    const int kv = min(a.kv_lens[s], a.max_kv);
+    // (the pieces' slots hold the columns of max_rows rows)
+    return DpSeq{r0, min(max(n, 0), a.max_rows), kv >= n && kv > 0 ? kv : 0};
 }
 // Column groups of n rows of n_rep heads; chunks of all of them over kv positions.
 template <int NT>
@@ -93,32 +78,52 @@ __device__ __forceinline__ u32x2 to_f16x4<i8_t>(uint32_t w) {
                  __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, b) + off)};
 }
 
-template <typename TQ, typename TP, int D, int TILES, int NT, bool BS16, bool W>
-__global__ __launch_bounds__(64, NT == 4 ? 1 : 2) void decode_pools_kernel(DpArgs a) {
+// Resident waves per CU. Decode steps and 32 columns: two per SIMD. With 64 columns, or 32 of fp32 queries
+// in two parts, the accumulators and queries leave room for one.
+template <typename TQ, int NT>
+__host__ __device__ constexpr int dp_waves() {
+    return NT == 4 || (NT == 2 && sizeof(TQ) == 4) ? 4 : 8;
+}
+
+// MULTI: several rows of a sequence, or more query heads of a kv head than a tile has columns;
+// otherwise a decode step whose columns are one tile's.
+template <typename TQ, typename TP, int D, int TILES, int NT, bool MULTI, bool BS16, bool W>
+__global__ __launch_bounds__(64, (dp_waves<TQ, NT>() / 4)) void decode_pools_kernel(DpArgs a) {
     constexpr int CHUNK = 16 * TILES;
     constexpr int KL = D / 64;   // 16-byte K loads of a lane and tile
     constexpr int NV = D / 16;   // O^T products of a chunk's half
     constexpr int KK = D / 32;   // products of a score tile
     constexpr int QP = sizeof(TQ) == 4 ? 2 : 1;  // parts of a query
     typedef typename std::conditional<D == 128, u32x2, uint32_t>::type Vd;
+    constexpr int KP = D + 16;  // bytes of a K row in LDS: 16-byte reads of 16 rows spread over the banks
     extern __shared__ int pre[];
+    __shared__ __attribute__((aligned(16))) unsigned char kt[16 * KP];  // one K tile
     const int lane = threadIdx.x, lg = lane >> 4, lc = lane & 15;
     const int n_rep = a.n_rep, batch = a.batch;
+    // (opaque: where it is known to be 0, joins with paths where it is not would make it per lane)
+    int wg = blockIdx.x;
+    asm volatile("" : "+s"(wg));
 
-    auto seq_chunks = [&](int s) -> int {
-        const DpSeq q = dp_seq(a.cu, a.kv_lens, a.max_kv, s);
-        return dp_groups<NT>(q.rows, n_rep) * ((q.kv + CHUNK - 1) / CHUNK);
+    auto seq_of = [&](int s) -> DpSeq {
+        if constexpr (MULTI) return dp_seq(a, s);
+        return DpSeq{s, 1, max(min(a.kv_lens[s], a.max_kv), 0)};
+    };
+    auto groups_of = [&](int rows) -> int { return MULTI ? dp_groups<NT>(rows, n_rep) : 1; };
+    auto seq_chunks = [&](const DpSeq& q) -> int {
+        return groups_of(q.rows) * ((q.kv + CHUNK - 1) / CHUNK);
     };
     // ---- exclusive prefix sums of the sequences' chunks (per kv head); up to 64 sequences stay in
     // registers, one a lane
     const bool in_lanes = batch <= 64;
+    DpSeq my = {0, 0, 0};
     int my_pre = 0, all_chunks;
     if (in_lanes) {
-        const int n = lane < batch ? seq_chunks(lane) : 0;
+        if (lane < batch) my = seq_of(lane);
+        const int n = seq_chunks(my);
         const int incl = wave_incl_sum(n);
         my_pre = incl - n;
         all_chunks = __builtin_amdgcn_readlane(incl, 63);
-        if (blockIdx.x == 0) {
+        if (wg == 0) {
             if (lane < batch) a.pre[lane] = my_pre;
             if (lane == 63) a.pre[batch] = incl;
         }
@@ -128,7 +133,7 @@ __global__ __launch_bounds__(64, NT == 4 ? 1 : 2) void decode_pools_kernel(DpArg
         for (int i = 0; i < per; i++) {
             const int b = lane * per + i;
             if (b < batch) {
-                const int n = seq_chunks(b);
+                const int n = seq_chunks(seq_of(b));
                 pre[b] = n;
                 local += n;
             }
@@ -146,11 +151,14 @@ __global__ __launch_bounds__(64, NT == 4 ? 1 : 2) void decode_pools_kernel(DpArg
         if (lane == 63) pre[batch] = incl;
         __syncthreads();
         all_chunks = __builtin_amdgcn_readlane(incl, 63);
-        if (blockIdx.x == 0)
+        if (wg == 0)
             for (int b = lane; b <= batch; b += 64) a.pre[b] = pre[b];
     }
-    const int64_t total = (int64_t)a.kv_heads * all_chunks;
-    const int64_t nwg = range_count(total, gridDim.x), wgi = blockIdx.x;
+    // (scalar again: the paths above join under per-lane stores, and a divergent value here makes
+    // every branch and register of the stream per lane)
+    const int64_t total = (int64_t)a.kv_heads * __builtin_amdgcn_readfirstlane(all_chunks);
+    const int64_t nwg = range_count(total, gridDim.x);
+    const int64_t wgi = wg;
     if (total == 0 || wgi >= nwg) return;
     const bool narrow = ranges_narrow(total, nwg, DP_XCD_W);
     int64_t lo;
@@ -171,9 +179,20 @@ __global__ __launch_bounds__(64, NT == 4 ? 1 : 2) void decode_pools_kernel(DpArg
     // ---- segments: up to SEG chunks (64 tiles, one a lane) of one (sequence, kv head, group)
     constexpr int SEG = 64 / TILES;
     struct Seg {
-        int b, g, grp, cb, ce, nch, row0, rows, kv;
+        int b, g, grp_, cb, ce, nch, row0_, rows_, kv;
+        Seg() = default;
+        // (copied by field: a copy in pieces of other widths keeps the struct in memory)
+        __device__ Seg(const Seg& o) { *this = o; }
+        __device__ Seg& operator=(const Seg& o) {
+            b = o.b, g = o.g, grp_ = o.grp_, cb = o.cb, ce = o.ce, nch = o.nch;
+            row0_ = o.row0_, rows_ = o.rows_, kv = o.kv;
+            return *this;
+        }
+        __device__ int grp() const { return MULTI ? grp_ : 0; }
+        __device__ int row0() const { return MULTI ? row0_ : b; }
+        __device__ int rows() const { return MULTI ? rows_ : 1; }
     };
-    auto seg_at = [&](int at) -> Seg {
+    auto seg_at = [&](int at) __attribute__((always_inline)) -> Seg {
         const int64_t x = lo + at;
         Seg sg;
         int before;
@@ -181,6 +200,9 @@ __global__ __launch_bounds__(64, NT == 4 ? 1 : 2) void decode_pools_kernel(DpArg
             const uint64_t le = __ballot(lane < batch && (int64_t)a.kv_heads * my_pre <= x);
             sg.b = 63 - __builtin_clzll(le);
             before = __builtin_amdgcn_readlane(my_pre, sg.b);
+            sg.kv = __builtin_amdgcn_readlane(my.kv, sg.b);
+            sg.row0_ = MULTI ? __builtin_amdgcn_readlane(my.row0, sg.b) : 0;
+            sg.rows_ = MULTI ? __builtin_amdgcn_readlane(my.rows, sg.b) : 0;
         } else {
             int l0 = 0, h0 = batch;
             while (h0 - l0 > 1) {
@@ -192,20 +214,21 @@ __global__ __launch_bounds__(64, NT == 4 ? 1 : 2) void decode_pools_kernel(DpArg
             }
             sg.b = __builtin_amdgcn_readfirstlane(l0);
             before = __builtin_amdgcn_readfirstlane(pre[l0]);
+            const DpSeq q = seq_of(sg.b);
+            sg.kv = __builtin_amdgcn_readfirstlane(q.kv);
+            sg.row0_ = MULTI ? __builtin_amdgcn_readfirstlane(q.row0) : 0;
+            sg.rows_ = MULTI ? __builtin_amdgcn_readfirstlane(q.rows) : 0;
         }
-        const DpSeq q = dp_seq(a.cu, a.kv_lens, a.max_kv, sg.b);
-        sg.row0 = __builtin_amdgcn_readfirstlane(q.row0);
-        sg.rows = __builtin_amdgcn_readfirstlane(q.rows);
-        sg.kv = __builtin_amdgcn_readfirstlane(q.kv);
         sg.nch = (sg.kv + CHUNK - 1) / CHUNK;
         const int64_t rel = x - (int64_t)a.kv_heads * before;
         const int pair = __builtin_amdgcn_readfirstlane(
             narrow ? (int)((uint32_t)rel / (uint32_t)sg.nch) : (int)(rel / sg.nch));
         sg.cb = (int)(rel - (int64_t)pair * sg.nch);
         // a head's groups next to each other: they read the same K/V
-        const int groups = dp_groups<NT>(sg.rows, n_rep);
-        sg.g = groups == 1 ? pair : pair / groups;
-        sg.grp = pair - sg.g * groups;
+        const int groups = __builtin_amdgcn_readfirstlane(groups_of(sg.rows()));
+        // (scalar: a divergent value would put every buffer load into a per-lane loop)
+        sg.g = !MULTI || groups == 1 ? pair : __builtin_amdgcn_readfirstlane(pair / groups);
+        sg.grp_ = MULTI ? pair - sg.g * groups : 0;
         sg.ce = sg.cb + min(min(sg.nch - sg.cb, SEG), len - at);
         return sg;
     };
@@ -214,7 +237,7 @@ __global__ __launch_bounds__(64, NT == 4 ? 1 : 2) void decode_pools_kernel(DpArg
     struct Slots {
         int id, off;  // lane i: block id as loaded and in-block offset of tile i's first token
     };
-    auto seg_slots = [&](const Seg& sg) -> Slots {
+    auto seg_slots = [&](Seg sg) -> Slots {
         const int32_t* bt = a.block_tables + (int64_t)sg.b * a.max_blocks;
         const int tok0 = min(sg.cb * CHUNK + lane * 16, ((sg.kv - 1) >> 4) << 4);
         const int lb = BS16 ? (tok0 >> 4) : tok0 / a.block_size;
@@ -224,17 +247,19 @@ __global__ __launch_bounds__(64, NT == 4 ? 1 : 2) void decode_pools_kernel(DpArg
     struct Scales {
         float k, v;  // lane i: the scales of tile i's block
     };
-    auto seg_scales = [&](const Seg& sg, const Slots& sl) -> Scales {
+    auto seg_scales = [&](Seg sg, Slots sl) -> Scales {
         const int64_t at = (int64_t)sg.g * nb + clamp_id(sl.id);
         return Scales{a.k_scale[at], a.v_scale[at]};
     };
 
     const uint32_t head_bytes = (uint32_t)(a.num_slots * D);
-    // K: bytes 16 lg + 64 i of row lc. V: bytes (D / 16) lc of row 4 lg + j.
-    uint32_t k_off = (uint32_t)(lc * D + 16 * lg);
+    // K: bytes 16 lane + 1024 i of the tile. V: bytes (D / 16) lc of row 4 lg + j.
+    uint32_t k_off = (uint32_t)(16 * lane);
     uint32_t v_off = (uint32_t)(4 * lg * D + (D / 16) * lc);
     asm volatile("" : "+v"(k_off), "+v"(v_off));  // (row offsets stay immediates of the loads)
-    auto load_chunk = [&](int g, const Slots& sl, int tile0, u32x4 (*kd)[KL], Vd (*vd)[4]) {
+    auto load_chunk = [&](int head, Slots sl, int tile0, u32x4 (*kd)[KL],
+                          Vd (*vd)[4]) __attribute__((always_inline)) {
+        const int g = __builtin_amdgcn_readfirstlane(head);
         const __amdgpu_buffer_rsrc_t k_rsrc = __builtin_amdgcn_make_buffer_rsrc(
             (void*)(a.k_pool + (int64_t)g * a.num_slots * D), (short)0, (int)head_bytes, BUF_DWORD3);
         const __amdgpu_buffer_rsrc_t v_rsrc = __builtin_amdgcn_make_buffer_rsrc(
@@ -248,7 +273,7 @@ __global__ __launch_bounds__(64, NT == 4 ? 1 : 2) void decode_pools_kernel(DpArg
             const uint32_t soff = slot * (uint32_t)D;
 #pragma unroll
             for (int i = 0; i < KL; i++)
-                kd[t][i] = __builtin_amdgcn_raw_buffer_load_b128(k_rsrc, k_off + 64 * i, soff, BUF_NT);
+                kd[t][i] = __builtin_amdgcn_raw_buffer_load_b128(k_rsrc, k_off + 1024 * i, soff, BUF_NT);
 #pragma unroll
             for (int j = 0; j < 4; j++) {
                 if constexpr (D == 128)
@@ -265,15 +290,15 @@ __global__ __launch_bounds__(64, NT == 4 ? 1 : 2) void decode_pools_kernel(DpArg
     float qf[NT];  // what turns a column's products into exp2-domain scores (times the K scale)
     int vis[NT];   // positions that the column sees
     int min_vis;   // that every column sees
-    auto load_q = [&](const Seg& sg) {
+    auto load_q = [&](Seg sg) __attribute__((always_inline)) {
         const TQ* q = static_cast<const TQ*>(a.q);
 #pragma unroll
         for (int ct = 0; ct < NT; ct++) {
-            const int col = (sg.grp * NT + ct) * 16 + lc;
-            const bool real = col < sg.rows * n_rep;
-            const int i = real ? col / n_rep : 0, r = real ? col - i * n_rep : 0;
-            vis[ct] = real ? sg.kv - sg.rows + i + 1 : sg.kv;
-            const TQ* row = q + (int64_t)(sg.row0 + i) * a.q_st + (int64_t)(sg.g * n_rep + r) * a.q_sh;
+            const int col = (sg.grp() * NT + ct) * 16 + lc;
+            const bool real = col < sg.rows() * n_rep;
+            const int i = MULTI && real ? col / n_rep : 0, r = real ? col - i * n_rep : 0;
+            vis[ct] = real ? sg.kv - sg.rows() + i + 1 : sg.kv;
+            const TQ* row = q + (int64_t)(sg.row0() + i) * a.q_st + (int64_t)(sg.g * n_rep + r) * a.q_sh;
             if constexpr (std::is_same<TQ, f16_t>::value) {
                 qf[ct] = a.scale_log2;
 #pragma unroll
@@ -321,12 +346,14 @@ __global__ __launch_bounds__(64, NT == 4 ? 1 : 2) void decode_pools_kernel(DpArg
                     }
             }
         }
-        min_vis = sg.kv - sg.rows + 1 + sg.grp * NT * 16 / n_rep;
+        min_vis = MULTI ? sg.kv - sg.rows() + 1 +
+                              __builtin_amdgcn_readfirstlane(sg.grp() * NT * 16 / n_rep)
+                        : sg.kv;
     };
 
     float m[NT], lsum[NT], mv[NT];
     f32x4 acc[NT][NV];
-    auto clear = [&]() {
+    auto clear = [&]() __attribute__((always_inline)) {
 #pragma unroll
         for (int ct = 0; ct < NT; ct++) {
             m[ct] = mv[ct] = DEC_M0;
@@ -337,7 +364,12 @@ __global__ __launch_bounds__(64, NT == 4 ? 1 : 2) void decode_pools_kernel(DpArg
     };
     clear();
 
-    auto compute_chunk = [&](const Seg& sg, int c, const Scales& sc, u32x4 (*ka)[KL], Vd (*va)[4]) {
+    auto compute_chunk = [&](Seg sg, int c, Scales sc, u32x4 (*ka)[KL],
+                             Vd (*va)[4]) __attribute__((always_inline)) {
+        // (several column tiles: the compiler would have all of a chunk's conversions in registers)
+        auto phase = [] {
+            if constexpr (NT > 1) __builtin_amdgcn_sched_barrier(0);
+        };
         const int tok0 = c * CHUNK, tile0 = TILES * (c - sg.cb);
         const bool full = tok0 + CHUNK <= min_vis;
         if (tok0 + CHUNK > sg.kv) {  // tokens past the sequence: no bits of theirs
@@ -350,13 +382,25 @@ __global__ __launch_bounds__(64, NT == 4 ? 1 : 2) void decode_pools_kernel(DpArg
         f32x4 s[NT][TILES];
 #pragma unroll
         for (int t = 0; t < TILES; t++) {
+            // One wave a workgroup, whose LDS operations complete in order: the barriers only keep
+            // the compiler from moving them.
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll
+            for (int i = 0; i < KL; i++)
+                *reinterpret_cast<u32x4*>(
+                    &kt[(lane / (D / 16) + (1024 / D) * i) * KP + 16 * (lane % (D / 16))]) = ka[t][i];
+            __builtin_amdgcn_wave_barrier();
             u32x4 kA[KK];
 #pragma unroll
-            for (int kk = 0; kk < KK; kk++) {
-                const u32x2 x = to_f16x4<TP>(ka[t][kk >> 1][2 * (kk & 1)]);
-                const u32x2 y = to_f16x4<TP>(ka[t][kk >> 1][2 * (kk & 1) + 1]);
-                kA[kk] = u32x4{x[0], x[1], y[0], y[1]};
+            for (int i = 0; i < KL; i++) {
+                const u32x4 w = *reinterpret_cast<const u32x4*>(&kt[lc * KP + 64 * i + 16 * lg]);
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    const u32x2 x = to_f16x4<TP>(w[2 * h]), y = to_f16x4<TP>(w[2 * h + 1]);
+                    kA[2 * i + h] = u32x4{x[0], x[1], y[0], y[1]};
+                }
             }
+            __builtin_amdgcn_wave_barrier();
 #pragma unroll
             for (int ct = 0; ct < NT; ct++) {
                 f32x4 z = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -366,6 +410,7 @@ __global__ __launch_bounds__(64, NT == 4 ? 1 : 2) void decode_pools_kernel(DpArg
                     for (int kk = 0; kk < KK; kk++) z = mfma16x16x32<f16_t>(kA[kk], qb[ct][p][kk], z);
                 s[ct][t] = z;
             }
+            phase();
         }
         float kf[TILES], lv[TILES];
 #pragma unroll
@@ -374,25 +419,31 @@ __global__ __launch_bounds__(64, NT == 4 ? 1 : 2) void decode_pools_kernel(DpArg
             lv[t] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(sc.v), tile0 + t));
         }
         u32x4 PH[NT][TILES / 2], PL[NT][TILES / 2];
-#pragma unroll
-        for (int ct = 0; ct < NT; ct++) {
+        auto softmax = [&](auto all_seen, int ct) __attribute__((always_inline)) {
             float x[4 * TILES];  // scores
-            float top = -INFINITY, topv = -INFINITY;
+            float top = DEC_M0, topv = -INFINITY;
 #pragma unroll
             for (int t = 0; t < TILES; t++) {
                 const float f = qf[ct] * kf[t];
+                float tile = -INFINITY;
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
-                    const bool ok = full || tok0 + 16 * t + 4 * lg + r < vis[ct];
-                    x[4 * t + r] = ok ? s[ct][t][r] * f : -INFINITY;
-                    top = fmaxf(top, x[4 * t + r]);
+                    x[4 * t + r] = s[ct][t][r] * f;
+                    if constexpr (!decltype(all_seen)::value)
+                        if (tok0 + 16 * t + 4 * lg + r >= vis[ct]) x[4 * t + r] = -INFINITY;
+                    tile = fmaxf(tile, x[4 * t + r]);
                 }
+                top = fmaxf(top, tile);
+                // a tile that the column does not see takes nothing from its block, least of all a
+                // scale of NaN (fmaxf hands that on to nothing here, so it is selected away)
+                topv = fmaxf(topv, tile + lv[t]);
             }
             if constexpr (W) {
-                if (lc < n_rep - 16 * sg.grp) {
+                const int r = (sg.grp() * NT + ct) * 16 + lc;  // (decode steps: the query head)
+                if (r < n_rep) {
                     float* to = a.scores +
-                                ((int64_t)sg.row0 * a.num_heads + sg.g * n_rep + 16 * sg.grp + lc) *
-                                    a.score_stride + tok0 + 4 * lg;
+                                ((int64_t)sg.b * a.num_heads + sg.g * n_rep + r) * a.score_stride +
+                                tok0 + 4 * lg;
 #pragma unroll
                     for (int t = 0; t < TILES; t++)
                         *reinterpret_cast<f32x4*>(to + 16 * t) =
@@ -400,34 +451,47 @@ __global__ __launch_bounds__(64, NT == 4 ? 1 : 2) void decode_pools_kernel(DpArg
                 }
             }
             const float m_new = fmaxf(m[ct], max_across_rows(top));
+            const float mv_new = fmaxf(mv[ct], max_across_rows(topv));
             float psum = 0.0f;
 #pragma unroll
-            for (int i = 0; i < 4 * TILES; i++) {
-                psum += fast_exp2(x[i] - m_new);
-                // (a position that the column does not see takes nothing from its block, a scale of NaN
-                // least of all)
-                const bool ok = full || tok0 + 16 * (i >> 2) + 4 * lg + (i & 3) < vis[ct];
-                x[i] = ok ? x[i] + lv[i >> 2] : -INFINITY;
-                topv = fmaxf(topv, x[i]);
+            for (int t = 0; t < TILES; t++) {
+                // P' = p 2^(m + log2 S_v - m'): a factor per tile. It is at most 2^(m - the tile's
+                // maximum); the bound keeps it finite where every p of the tile is 0.
+                const bool none = !decltype(all_seen)::value && tok0 + 16 * t >= vis[ct];
+                const float e = none ? 0.0f : (m_new - mv_new) + (lv[t] + DP_SHIFT);
+                const float gt = fast_exp2(e > 126.0f ? 126.0f : e);
+                float p[4];
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    p[r] = fast_exp2(x[4 * t + r] - m_new);
+                    psum += p[r];
+                    p[r] *= gt;
+                }
+#pragma unroll
+                for (int r = 0; r < 4; r += 2) {
+                    const uint32_t hi = pack2<f16_t>(p[r], p[r + 1]);
+                    PH[ct][t >> 1][2 * (t & 1) + (r >> 1)] = hi;
+                    PL[ct][t >> 1][2 * (t & 1) + (r >> 1)] =
+                        pack2<f16_t>(fmaf(lo_f32<f16_t>(hi), -1.0f, p[r]),
+                                     fmaf(hi_f32<f16_t>(hi), -1.0f, p[r + 1]));
+                }
             }
             lsum[ct] = lsum[ct] * fast_exp2(m[ct] - m_new) + psum;
             m[ct] = m_new;
-            const float mv_new = fmaxf(mv[ct], max_across_rows(topv));
             if (__builtin_amdgcn_ballot_w64(mv_new > mv[ct]) != 0) {
                 const float alpha = fast_exp2(mv[ct] - mv_new);
 #pragma unroll
                 for (int nn = 0; nn < NV; nn++) acc[ct][nn] *= alpha;
             }
             mv[ct] = mv_new;
+        };
 #pragma unroll
-            for (int i = 0; i < 4 * TILES; i += 2) {
-                const float p0 = fast_exp2(x[i] - mv_new + DP_SHIFT);
-                const float p1 = fast_exp2(x[i + 1] - mv_new + DP_SHIFT);
-                const uint32_t hi = pack2<f16_t>(p0, p1);
-                PH[ct][i >> 3][(i & 7) >> 1] = hi;
-                PL[ct][i >> 3][(i & 7) >> 1] =
-                    pack2<f16_t>(p0 - lo_f32<f16_t>(hi), p1 - hi_f32<f16_t>(hi));
-            }
+        for (int ct = 0; ct < NT; ct++) {
+            if (full)
+                softmax(std::integral_constant<bool, true>{}, ct);
+            else
+                softmax(std::integral_constant<bool, false>{}, ct);
+            phase();
         }
         // V^T: lane (lg, lc) holds dim (D / 16) lc + nn of tokens 4lg .. 4lg + 3 of two tiles
 #pragma unroll
@@ -463,23 +527,24 @@ __global__ __launch_bounds__(64, NT == 4 ? 1 : 2) void decode_pools_kernel(DpArg
                         o = mfma16x16x32<f16_t>(A[e], PH[ct][u], o);
                         o = mfma16x16x32<f16_t>(A[e], PL[ct][u], o);
                     }
+                phase();
             }
     };
 
     // ---- a piece's end: lane (lg, lc) holds column lc, dims (D / 4) lg + NV r + nn
-    auto epilogue = [&](const Seg& sg, bool complete, bool first_piece) {
+    auto epilogue = [&](Seg sg, bool complete, bool first_piece) __attribute__((always_inline)) {
         int lgo = lg;
         asm volatile("" : "+v"(lgo));  // (addresses formed here, not kept through the stream)
 #pragma unroll
         for (int ct = 0; ct < NT; ct++) {
             const float l = sum_across_rows(lsum[ct]);
-            const int col = (sg.grp * NT + ct) * 16 + lc;
-            if (col >= sg.rows * n_rep) continue;
-            const int i = col / n_rep, r0 = col - i * n_rep;
+            const int col = (sg.grp() * NT + ct) * 16 + lc;
+            if (col >= sg.rows() * n_rep) continue;
+            const int i = MULTI ? col / n_rep : 0, r0 = col - i * n_rep;
             const int h = sg.g * n_rep + r0;
             if (complete) {
                 const float f = l == 0.0f ? 0.0f : fast_exp2(mv[ct] - m[ct] - DP_SHIFT) / l;
-                const int64_t at = (int64_t)(sg.row0 + i) * a.o_st + (int64_t)h * a.o_sh + (D / 4) * lgo;
+                const int64_t at = (int64_t)(sg.row0() + i) * a.o_st + (int64_t)h * a.o_sh + (D / 4) * lgo;
 #pragma unroll
                 for (int r = 0; r < 4; r++)
 #pragma unroll
@@ -492,12 +557,12 @@ __global__ __launch_bounds__(64, NT == 4 ? 1 : 2) void decode_pools_kernel(DpArg
                     }
                 if constexpr (W)
                     if (lg == 0) {
-                        float* ml = a.ml + 2 * ((int64_t)(sg.row0 + i) * a.num_heads + h);
+                        float* ml = a.ml + 2 * ((int64_t)(sg.row0() + i) * a.num_heads + h);
                         ml[0] = m[ct];
                         ml[1] = l;
                     }
             } else {
-                const int64_t slot = (2 * wgi + (first_piece ? 0 : 1)) * (16 * NT) + 16 * ct + lc;
+                const int64_t slot = (2 * wgi + (first_piece ? 0 : 1)) * a.cols + 16 * ct + lc;
                 float* o = a.p_o + slot * D + (D / 4) * lgo;
 #pragma unroll
                 for (int r = 0; r < 4; r++)
@@ -541,7 +606,8 @@ __global__ __launch_bounds__(64, NT == 4 ? 1 : 2) void decode_pools_kernel(DpArg
     bool first_piece = true;
     int c = cur.cb;
 
-    auto step = [&](auto prefetch, u32x4 (*kc)[KL], Vd (*vc)[4], u32x4 (*kn)[KL], Vd (*vn)[4]) {
+    auto step = [&](auto prefetch, u32x4 (*kc)[KL], Vd (*vc)[4], u32x4 (*kn)[KL],
+                    Vd (*vn)[4]) __attribute__((always_inline)) {
         const bool seg_end = c + 1 >= cur.ce;
         int nn_x = nx;
         bool has_nn = false;
@@ -557,7 +623,10 @@ __global__ __launch_bounds__(64, NT == 4 ? 1 : 2) void decode_pools_kernel(DpArg
         }
         if constexpr (decltype(prefetch)::value) {
             const bool in_cur = c + 1 < cur.ce;
-            const Slots ps = in_cur ? cur_slots : nxt_slots;
+            // (selected by value: a choice between two structs keeps them in memory)
+            Slots ps;
+            ps.id = in_cur ? cur_slots.id : nxt_slots.id;
+            ps.off = in_cur ? cur_slots.off : nxt_slots.off;
             load_chunk(in_cur ? cur.g : nxt.g, ps, in_cur ? TILES * (c + 1 - cur.cb) : 0, kn, vn);
         }
         compute_chunk(cur, c, cur_sc, kc, vc);
@@ -566,7 +635,7 @@ __global__ __launch_bounds__(64, NT == 4 ? 1 : 2) void decode_pools_kernel(DpArg
             return;
         }
         const bool piece_end =
-            !has_nxt || nxt.b != cur.b || nxt.g != cur.g || nxt.grp != cur.grp;
+            !has_nxt || nxt.b != cur.b || nxt.g != cur.g || nxt.grp() != cur.grp();
         if (piece_end) epilogue(cur, pc0 == 0 && cur.ce == cur.nch, first_piece);
         if (!has_nxt) return;
         if (piece_end) {
@@ -611,7 +680,7 @@ __global__ __launch_bounds__(64 * DP_MERGE_WAVES) void decode_pools_merge_kernel
     const int w_id = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
     int s = row;
     if (a.cu) s = wave_find_last(a.batch, row, [&](int i) -> int64_t { return a.cu[i]; });
-    const DpSeq q = dp_seq(a.cu, a.kv_lens, a.max_kv, s);
+    const DpSeq q = dp_seq(a, s);
     const int i = row - q.row0;
     if (i < 0 || i >= q.rows) return;  // (rows of no sequence)
     const int64_t at = (int64_t)row * a.o_st + (int64_t)h * a.o_sh + E * lane;
@@ -650,7 +719,7 @@ __global__ __launch_bounds__(64 * DP_MERGE_WAVES) void decode_pools_merge_kernel
     const bool f_first = from == (narrow ? (int64_t)r32.lo((uint32_t)f) : r64.lo(f));
     const int np = (int)(l - f + 1);
     auto slot_of = [&](int p) -> int64_t {  // (the last piece of a range but the first: its second)
-        return (2 * (f + p) + (p == 0 && !f_first ? 1 : 0)) * (16 * NT) + cc;
+        return (2 * (f + p) + (p == 0 && !f_first ? 1 : 0)) * a.cols + cc;
     };
     float M = DEC_M0, MV = DEC_M0, L = 0.0f, O[E] = {};
     const int per = (np + waves - 1) / waves, p_end = min(np, (w_id + 1) * per);
@@ -712,90 +781,86 @@ __global__ __launch_bounds__(64 * DP_MERGE_WAVES) void decode_pools_merge_kernel
     }
 }
 
-static constexpr size_t up256(size_t x) { return (x + 255) & ~(size_t)255; }
-
-static int stream_waves() { return std::min(device_cus() * 4, 4096); }
-
-// Workspace of a streamed call of `cols` columns a group.
-static size_t stream_bytes(int batch, int cols, int head_dim) {
-    const size_t slots = 2 * (size_t)stream_waves() * cols;
-    return up256(slots * 3 * sizeof(float)) + up256(slots * head_dim * sizeof(float)) +
-           up256(((size_t)batch + 1) * sizeof(int));
+// The grid's waves at most: what the workspace is sized for and what a launch is cut to.
+template <typename TQ, int NT>
+static int stream_waves() {
+    return std::min(device_cus() * dp_waves<TQ, NT>(), 4096);
 }
 
-bool decode_stream_takes(const PoolAttn& a) {
-    const int es = elem_bytes(a.dtype), oes = elem_bytes(a.out_dtype);
-    return valid_pool8(a.pool_dtype) && (a.head_dim == 64 || a.head_dim == 128) &&
-           a.block_size % 16 == 0 && a.batch <= DP_MAX_BATCH && a.rows <= 65535 &&
-           a.num_slots * a.head_dim <= (int64_t)0x7fffffff &&
-           (((uintptr_t)a.q | (uintptr_t)a.out | (uintptr_t)a.k_pool | (uintptr_t)a.v_pool |
-             (uint64_t)(a.q_st * es) | (uint64_t)(a.q_sh * es) | (uint64_t)(a.o_st * oes) |
-             (uint64_t)(a.o_sh * oes)) & 15) == 0;
+static constexpr size_t dp_up256(size_t x) { return (x + 255) & ~(size_t)255; }
+
+// Bytes of a streamed call's workspace (null: its size alone).
+template <typename TQ, int NT>
+static size_t stream_layout(DpArgs* a, void* workspace, int batch, int cols, int head_dim) {
+    const size_t slots = 2 * (size_t)stream_waves<TQ, NT>() * cols;
+    const size_t ml = dp_up256(slots * 3 * sizeof(float));
+    const size_t o = dp_up256(slots * head_dim * sizeof(float));
+    if (a) {
+        char* ws = static_cast<char*>(workspace);
+        a->cols = cols;
+        a->p_ml = reinterpret_cast<float*>(ws);
+        a->p_o = reinterpret_cast<float*>(ws + ml);
+        a->pre = reinterpret_cast<int*>(ws + ml + o);
+    }
+    return ml + o + dp_up256(((size_t)batch + 1) * sizeof(int));
 }
 
-size_t decode_stream_bytes(int batch, int max_cols, int head_dim) {
-    return head_dim == 64 || head_dim == 128
-               ? stream_bytes(batch, max_cols <= 16 ? 16 : max_cols <= 32 ? 32 : 64, head_dim) : 0;
-}
-
-template <typename TQ, typename TP, int D, int TILES, int NT, bool W>
-static int launch_stream(const DpArgs& a, int max_rows, int rows, hipStream_t stream) {
-    const int64_t groups = ((int64_t)max_rows * a.n_rep + 16 * NT - 1) / (16 * NT);
+template <typename TQ, typename TP, int D, int NT, bool MULTI, bool W>
+static int launch_stream(DpArgs a, void* workspace, int max_rows, int rows, hipStream_t stream) {
+    constexpr int TILES = 2;
+    const int64_t max_cols = (int64_t)max_rows * a.n_rep, groups = (max_cols + 16 * NT - 1) / (16 * NT);
+    a.max_rows = max_rows;
+    stream_layout<TQ, NT>(&a, workspace, a.batch, (int)std::min<int64_t>(max_cols, 16 * NT), D);
     const int64_t chunks = (a.max_kv + 16 * TILES - 1) / (16 * TILES);
     const int64_t half = (int64_t)a.batch * a.kv_heads * groups * chunks / 2;
-    const int per_cu = 3, cap = std::min(device_cus() * per_cu, 4096);
-    const int grid = (int)std::max<int64_t>(1, std::min<int64_t>(half, cap));
+    const int grid = (int)std::max<int64_t>(1, std::min<int64_t>(half, stream_waves<TQ, NT>()));
     const size_t lds = a.batch <= 64 ? 0 : (size_t)(a.batch + 1) * sizeof(int);
-    auto kern = a.block_size == 16 ? decode_pools_kernel<TQ, TP, D, TILES, NT, true, W>
-                                   : decode_pools_kernel<TQ, TP, D, TILES, NT, false, W>;
+    auto kern = a.block_size == 16 ? decode_pools_kernel<TQ, TP, D, TILES, NT, MULTI, true, W>
+                                   : decode_pools_kernel<TQ, TP, D, TILES, NT, MULTI, false, W>;
     kern<<<dim3(grid), dim3(64), lds, stream>>>(a);
-    const int rc = check_hip(hipGetLastError(), "8-bit decode launch");
+    const int rc = check_hip(hipGetLastError(), "8-bit attention launch");
     if (rc != FLOUR_OK) return rc;
-    const int64_t pieces = 2 * (int64_t)grid / ((int64_t)a.batch * a.kv_heads);
+    const int64_t pieces = 2 * (int64_t)grid / ((int64_t)a.batch * a.kv_heads * groups);
     int waves = 1;
     while (waves < DP_MERGE_WAVES && 8 * waves < pieces) waves *= 2;
     decode_pools_merge_kernel<D, TILES, NT, W>
         <<<dim3(a.num_heads, rows), dim3(64 * waves), 0, stream>>>(a, grid);
-    return check_hip(hipGetLastError(), "8-bit decode merge launch");
+    return check_hip(hipGetLastError(), "8-bit attention merge launch");
 }
 
 template <typename TQ, typename TP, int D>
-static int launch_stream_d(const DpArgs& a, int max_rows, int rows, hipStream_t s) {
-    if (a.scores) return launch_stream<TQ, TP, D, 4, 1, true>(a, max_rows, rows, s);
-    return launch_stream<TQ, TP, D, 4, 1, false>(a, max_rows, rows, s);
+static int launch_stream_d(const DpArgs& a, void* ws, int max_rows, int rows, hipStream_t s) {
+    const int64_t cols = (int64_t)max_rows * a.n_rep;
+    if (a.scores)
+        return cols <= 16 ? launch_stream<TQ, TP, D, 1, false, true>(a, ws, max_rows, rows, s)
+                          : launch_stream<TQ, TP, D, 2, true, true>(a, ws, max_rows, rows, s);
+    if (!a.cu && cols <= 16)
+        return launch_stream<TQ, TP, D, 1, false, false>(a, ws, max_rows, rows, s);
+    return cols <= 32 ? launch_stream<TQ, TP, D, 2, true, false>(a, ws, max_rows, rows, s)
+                      : launch_stream<TQ, TP, D, 4, true, false>(a, ws, max_rows, rows, s);
 }
 
-int launch_decode_stream(const PoolAttn& p, int max_rows, void* workspace, hipStream_t stream) {
-    DpArgs a{};
-    a.out = p.out, a.out_dtype = p.out_dtype, a.o_st = p.o_st, a.o_sh = p.o_sh;
-    a.q = p.q, a.q_st = p.q_st, a.q_sh = p.q_sh;
-    a.k_pool = static_cast<const uint8_t*>(p.k_pool);
-    a.v_pool = static_cast<const uint8_t*>(p.v_pool);
-    a.k_scale = p.k_scale, a.v_scale = p.v_scale;
-    a.cu = p.cu, a.kv_lens = p.kv_lens, a.block_tables = p.block_tables;
-    a.max_blocks = p.max_blocks, a.batch = p.batch, a.num_heads = p.num_heads;
-    a.kv_heads = p.kv_heads, a.n_rep = p.num_heads / p.kv_heads, a.block_size = p.block_size;
-    a.num_slots = p.num_slots, a.scale_log2 = p.scale * LOG2_E;
-    a.max_kv = (int)std::min<int64_t>(p.max_kv, (int64_t)p.max_blocks * p.block_size);
-    a.scores = p.scores, a.score_stride = p.score_stride, a.ml = p.ml;
-    const int cols = 16;
-    const size_t slots = 2 * (size_t)stream_waves() * cols;
-    char* ws = static_cast<char*>(workspace);
-    a.p_ml = reinterpret_cast<float*>(ws);
-    ws += up256(slots * 3 * sizeof(float));
-    a.p_o = reinterpret_cast<float*>(ws);
-    ws += up256(slots * p.head_dim * sizeof(float));
-    a.pre = reinterpret_cast<int*>(ws);
-#define FLOUR_DS(TQ)                                                                              \
-    (p.pool_dtype == FLOUR_DTYPE_E4M3                                                             \
-         ? (p.head_dim == 64 ? launch_stream_d<TQ, e4m3_t, 64>(a, max_rows, p.rows, stream)       \
-                             : launch_stream_d<TQ, e4m3_t, 128>(a, max_rows, p.rows, stream))     \
-         : (p.head_dim == 64 ? launch_stream_d<TQ, i8_t, 64>(a, max_rows, p.rows, stream)         \
-                             : launch_stream_d<TQ, i8_t, 128>(a, max_rows, p.rows, stream)))
-    if (p.dtype == FLOUR_DTYPE_F32) return FLOUR_DS(float);
-    if (p.dtype == FLOUR_DTYPE_BF16) return FLOUR_DS(bf16_t);
-    return FLOUR_DS(f16_t);
-#undef FLOUR_DS
+template <typename TQ>
+static int launch_stream_q(const DpArgs& a, int pool_dtype, int head_dim, void* ws, int max_rows,
+                           int rows, hipStream_t s) {
+    if (pool_dtype == FLOUR_DTYPE_E4M3)
+        return head_dim == 64 ? launch_stream_d<TQ, e4m3_t, 64>(a, ws, max_rows, rows, s)
+                              : launch_stream_d<TQ, e4m3_t, 128>(a, ws, max_rows, rows, s);
+    return head_dim == 64 ? launch_stream_d<TQ, i8_t, 64>(a, ws, max_rows, rows, s)
+                          : launch_stream_d<TQ, i8_t, 128>(a, ws, max_rows, rows, s);
+}
+
+// The largest workspace of calls of up to max_cols columns.
+template <typename TQ>
+static size_t stream_bytes_q(int batch, int64_t max_cols, int head_dim) {
+    size_t n = 0;
+    if (max_cols <= 16) n = stream_layout<TQ, 1>(nullptr, nullptr, batch, (int)max_cols, head_dim);
+    n = std::max(n, stream_layout<TQ, 2>(nullptr, nullptr, batch,
+                                         (int)std::min<int64_t>(max_cols, 32), head_dim));
+    if (max_cols > 32)
+        n = std::max(n, stream_layout<TQ, 4>(nullptr, nullptr, batch,
+                                             (int)std::min<int64_t>(max_cols, 64), head_dim));
+    return n;
 }
 
 }  // namespace flour

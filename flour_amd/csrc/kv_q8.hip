@@ -7,6 +7,7 @@
 // The units of a call are listed without a pass over it: sequence s owns the blocks from index
 // cu[s] / bs + 2 s on, which leaves room for the n / bs + 2 blocks that n rows can touch.
 #include "cache8.h"
+#include "decode_pools.h"
 
 namespace flour {
 
@@ -121,15 +122,18 @@ __global__ __launch_bounds__(64 * KQ_WAVES) void kv_write_q8_kernel(
     if (lane == 0) *scale = S;
 }
 
-// One wave a (sequence, block, kv head): rows of K and of V.
-template <typename T, typename TP, int N>
+// One wave a (sequence, block, kv head): rows of K and of V. STAGE: a copy for an attention kernel (out
+// blocks by position, the table and lengths that go with them). What a block of scale NaN stands for
+// must reach those that attend to it and nobody else, so it goes into the scores: K is NaN, V 0.
+template <typename T, typename TP, int N, bool STAGE>
 __global__ __launch_bounds__(64 * KQ_WAVES) void kv_dequant_kernel(
     T* __restrict__ k_out, T* __restrict__ v_out, const int32_t* __restrict__ out_tables,
     int out_max_blocks, int64_t out_slots, const uint8_t* __restrict__ k_pool,
     const uint8_t* __restrict__ v_pool, const float* __restrict__ k_scale,
     const float* __restrict__ v_scale, const int32_t* __restrict__ block_tables, int max_blocks,
     const int32_t* __restrict__ kv_lens, int num_seqs, int max_kv, int blocks_per_seq,
-    int kv_heads, int head_dim, int block_size, int64_t num_slots) {
+    int kv_heads, int head_dim, int block_size, int64_t num_slots, int32_t* __restrict__ staged_table,
+    int32_t* __restrict__ staged_lens) {
     const int lane = threadIdx.x & 63;
     const int64_t u = (int64_t)blockIdx.x * KQ_WAVES +
                       __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -138,17 +142,25 @@ __global__ __launch_bounds__(64 * KQ_WAVES) void kv_dequant_kernel(
     if (s >= num_seqs) return;
     const int rest = (int)(u - s * per_seq), lb = rest / kv_heads, g = rest - lb * kv_heads;
     const int kv = min(kv_lens[s], max_kv);
+    if constexpr (STAGE) {
+        if (g == 0 && lane == 0) {
+            staged_table[(int64_t)s * out_max_blocks + lb] = s * out_max_blocks + lb;
+            if (lb == 0) staged_lens[s] = kv;
+        }
+    }
     const int64_t first = (int64_t)lb * block_size;
     if (first >= kv || lb >= max_blocks || lb >= out_max_blocks) return;
     const int64_t nb = num_slots / block_size;
     const int64_t raw = block_tables[(int64_t)s * max_blocks + lb];
     const int64_t id = raw < 0 ? 0 : (raw >= nb ? nb - 1 : raw);
-    const int64_t to = out_tables[(int64_t)s * out_max_blocks + lb];
+    const int64_t to = STAGE ? (int64_t)s * out_max_blocks + lb
+                             : (int64_t)out_tables[(int64_t)s * out_max_blocks + lb];
     if (to < 0 || to >= out_slots / block_size) return;
     const int rows = (int)min((int64_t)kv - first, (int64_t)block_size);
     const int64_t src = ((int64_t)g * num_slots + id * block_size) * head_dim;
     const int64_t dst = ((int64_t)g * out_slots + to * block_size) * head_dim;
-    const float ks = k_scale[g * nb + id], vs = v_scale[g * nb + id];
+    float ks = k_scale[g * nb + id], vs = v_scale[g * nb + id];
+    if (STAGE && !(fabsf(vs) < INFINITY)) ks = __uint_as_float(0x7fc00000u), vs = 0.0f;
     auto put = [&](T* out, const uint8_t* in, float S) {
         float y[N];
         load_run8<TP, N>(in, y);
@@ -213,7 +225,8 @@ int launch_kv_dequant(void* k_out, void* v_out, int dtype, const int32_t* out_ta
                       const void* v_pool, const float* k_scale, const float* v_scale,
                       int pool_dtype, const int32_t* bt, int max_blocks, const int32_t* kv_lens,
                       int num_seqs, int max_kv, int kv_heads, int head_dim, int block_size,
-                      int64_t num_slots, hipStream_t s) {
+                      int64_t num_slots, int32_t* staged_table, int32_t* staged_lens,
+                      hipStream_t s) {
     const int per_seq = (int)(((int64_t)max_kv + block_size - 1) / block_size);
     const int64_t waves = (int64_t)num_seqs * per_seq * kv_heads;
     const int64_t grid = (waves + KQ_WAVES - 1) / KQ_WAVES;
@@ -225,11 +238,12 @@ int launch_kv_dequant(void* k_out, void* v_out, int dtype, const int32_t* out_ta
     const bool wide = head_dim % 8 == 0 && (((uintptr_t)k_out | (uintptr_t)v_out) & 15) == 0 &&
                       (((uintptr_t)k_pool | (uintptr_t)v_pool) & 7) == 0;
 #define FLOUR_DQ(T, TP, N)                                                                        \
-    kv_dequant_kernel<T, TP, N><<<dim3((unsigned)grid), dim3(64 * KQ_WAVES), 0, s>>>(             \
+    (staged_table ? kv_dequant_kernel<T, TP, N, true>                                             \
+                  : kv_dequant_kernel<T, TP, N, false>)<<<dim3((unsigned)grid), dim3(64 * KQ_WAVES), 0, s>>>(             \
         static_cast<T*>(k_out), static_cast<T*>(v_out), out_tables, out_max_blocks, out_slots,    \
         static_cast<const uint8_t*>(k_pool), static_cast<const uint8_t*>(v_pool), k_scale,        \
         v_scale, bt, max_blocks, kv_lens, num_seqs, max_kv, per_seq, kv_heads, head_dim,          \
-        block_size, num_slots)
+        block_size, num_slots, staged_table, staged_lens)
 #define FLOUR_DQ_T(T)                                                                             \
     do {                                                                                          \
         if (pool_dtype == FLOUR_DTYPE_E4M3) {                                                     \
@@ -340,5 +354,6 @@ extern "C" int flour_hip_kv_dequant(void* k_out, void* v_out, int dtype,
     return launch_kv_dequant(k_out, v_out, dtype, out_tables, out_max_blocks, out_slots, k_pool,
                              v_pool, k_scale, v_scale, pool_dtype, block_tables,
                              max_blocks_per_seq, kv_lens, num_seqs, max_kv_len, kv_heads, head_dim,
-                             block_size, num_slots, static_cast<hipStream_t>(stream));
+                             block_size, num_slots, nullptr, nullptr,
+                             static_cast<hipStream_t>(stream));
 }

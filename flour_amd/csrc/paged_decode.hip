@@ -115,6 +115,11 @@ struct DecodeWs {
     int64_t new_st, new_sh;
     const int32_t* new_slots;
     int xcd_w;  // wave-range weight w (WaveRanges): even ranges 32 + w, odd 32 - w
+    // A step whose attention weights are wanted (the kernels' WTS instantiations): every score in the
+    // exp2 domain, row b * num_heads + h at scores + row * score_stride, and each row's (max, sum).
+    float* scores;
+    int64_t score_stride;
+    float* row_ml;
 };
 
 static int g_wg_override = 0;  // tuning / test hook: number of waves (0 = one resident round)
@@ -161,7 +166,7 @@ __device__ __forceinline__ f32x4 mfma16x16x4_f32(float a, float b, f32x4 c) {
 // One wave per workgroup; each wave owns one contiguous range of the chunk list. D is the head
 // dim, 128 or 64. A lane's K/V share of a 16-token tile is rows 4lg .. 4lg + 3 at 16-byte
 // (D 128: dims 8lc ..) or 8-byte (D 64: dims 4lc ..) width, so a wave reads whole rows.
-template <typename T, typename TO, bool BS16, int D, bool FUSE>
+template <typename T, typename TO, bool BS16, int D, bool FUSE, bool WTS>
 __global__ __launch_bounds__(64, 2) void paged_decode_mfma_kernel(
     TO* __restrict__ out, const T* __restrict__ q, const T* __restrict__ k_pool,
     const T* __restrict__ v_pool, const int32_t* __restrict__ block_tables, int max_blocks,
@@ -352,7 +357,11 @@ __global__ __launch_bounds__(64, 2) void paged_decode_mfma_kernel(
     // 16kk + 4lg .. + 3, one per k-step 4kk .. 4kk + 3.
     constexpr int NQ = D * (int)sizeof(T) / 64;
     u32x4 qb[NQ];
+    float* score_to = nullptr;  // WTS: where the lane's scores of a chunk at token 0 go
     auto load_q = [&](int b, int g) {
+        if constexpr (WTS)
+            score_to = ws.scores + ((int64_t)b * num_heads + (int64_t)g * n_rep + lc) * ws.score_stride +
+                       4 * lg;
         const int64_t row = ws.rows ? (int64_t)ws.rows[b] : (int64_t)b;
         const T* qh = q + (row * num_heads + (int64_t)g * n_rep + lc) * D + (F32 ? 4 : 8) * lg;
 #pragma unroll
@@ -436,6 +445,13 @@ __global__ __launch_bounds__(64, 2) void paged_decode_mfma_kernel(
                 sv[4 * t + r] = ok ? s[t][r] * scale_log2 : -INFINITY;
                 tmax = fmaxf(tmax, sv[4 * t + r]);
             }
+        if constexpr (WTS) {
+            if (lc < n_rep)
+#pragma unroll
+                for (int t = 0; t < TILES; t++)
+                    *reinterpret_cast<f32x4*>(score_to + tok0 + 16 * t) =
+                        f32x4{sv[4 * t], sv[4 * t + 1], sv[4 * t + 2], sv[4 * t + 3]};
+        }
         tmax = max_across_rows(tmax);
         const float m_new = fmaxf(m, tmax);
         const float alpha = fast_exp2(m - m_new);
@@ -510,6 +526,12 @@ __global__ __launch_bounds__(64, 2) void paged_decode_mfma_kernel(
         asm volatile("" : "+v"(lgo));
         if (lc < n_rep) {
             if (complete) {  // whole pair in this range: final output
+                if constexpr (WTS)
+                    if (lg == 0) {
+                        float* ml = ws.row_ml + 2 * ((int64_t)b * num_heads + (int64_t)g * n_rep + lc);
+                        ml[0] = m;
+                        ml[1] = lsum;
+                    }
                 const int64_t row = ws.rows ? (int64_t)ws.rows[b] : (int64_t)b;
                 TO* o = out + (row * num_heads + (int64_t)g * n_rep + lc) * D +
                         (F32 ? 16 : D / 4) * lgo;
@@ -751,7 +773,7 @@ __global__ __launch_bounds__(64, 2) void paged_decode_mfma_kernel(
 // workgroup's waves split them, since one wave reads them 8 rows a memory round trip, and fold
 // their states through LDS; with one wave there is no LDS and no barrier.
 static constexpr int DEC_MERGE_WAVES = 8;
-template <typename TO, int D, bool F32>
+template <typename TO, int D, bool F32, bool WTS>
 __global__ __launch_bounds__(64 * DEC_MERGE_WAVES) void paged_decode_merge_kernel(
     TO* __restrict__ out, int batch, int num_heads, int kv_heads, int n_rep, int nwg_i,
     DecodeWs ws) {
@@ -895,6 +917,11 @@ __global__ __launch_bounds__(64 * DEC_MERGE_WAVES) void paged_decode_merge_kerne
             }
         }
     }
+    if constexpr (WTS)
+        if (lane == 0) {
+            ws.row_ml[2 * ((int64_t)b * num_heads + h)] = M;
+            ws.row_ml[2 * ((int64_t)b * num_heads + h) + 1] = L;
+        }
 #pragma unroll
     for (int i = 0; i < E; i++) {
         const float x = O[i] / divisor<F32>(L);
@@ -923,10 +950,14 @@ static int launch_decode_mfma_d(void* out, const void* q, const void* k_pool, co
         set_error("paged_decode: the fused KV write needs 16-token pages of a 16-bit pool");
         return FLOUR_ERR_UNSUPPORTED;
     }
-    auto kern = block_size == 16 ? paged_decode_mfma_kernel<T, TO, true, D, false>
-                                 : paged_decode_mfma_kernel<T, TO, false, D, false>;
+    const bool wts = ws.scores != nullptr;
+    auto kern = block_size == 16 ? paged_decode_mfma_kernel<T, TO, true, D, false, false>
+                                 : paged_decode_mfma_kernel<T, TO, false, D, false, false>;
     if constexpr (!std::is_same<T, float>::value)
-        if (fuse) kern = paged_decode_mfma_kernel<T, TO, true, D, true>;
+        if (fuse) kern = paged_decode_mfma_kernel<T, TO, true, D, true, false>;
+    if (wts)
+        kern = block_size == 16 ? paged_decode_mfma_kernel<T, TO, true, D, false, true>
+                                : paged_decode_mfma_kernel<T, TO, false, D, false, true>;
     // no more waves than ranges (range_count) for contexts of max_ctx
     const int64_t chunk = dec_chunk(sizeof(T));
     const int64_t half = (int64_t)batch * kv_heads * ((max_ctx + chunk - 1) / chunk) / 2;
@@ -938,9 +969,11 @@ static int launch_decode_mfma_d(void* out, const void* q, const void* k_pool, co
     int rc = check_hip(hipGetLastError(), "paged_decode launch");
     if (rc != FLOUR_OK) return rc;
     const int mw = decode_merge_waves(grid, batch, kv_heads);
-    paged_decode_merge_kernel<TO, D, std::is_same<T, float>::value>
-        <<<dim3(num_heads, batch), dim3(64 * mw), 0, stream>>>(
-            static_cast<TO*>(out), batch, num_heads, kv_heads, n_rep, grid, ws);
+    constexpr bool F32 = std::is_same<T, float>::value;
+    auto merge = wts ? paged_decode_merge_kernel<TO, D, F32, true>
+                     : paged_decode_merge_kernel<TO, D, F32, false>;
+    merge<<<dim3(num_heads, batch), dim3(64 * mw), 0, stream>>>(
+        static_cast<TO*>(out), batch, num_heads, kv_heads, n_rep, grid, ws);
     return check_hip(hipGetLastError(), "paged_decode merge launch");
 }
 
@@ -1160,7 +1193,7 @@ static int paged_decode_impl(void* out, int out_dtype, const void* q, const void
     const int n_rep = num_heads / kv_heads;
     const bool mfma = decode_mfma_supported(dtype, head_dim, block_size, n_rep, batch, num_heads,
                                             num_slots, q, k_pool, v_pool);
-    if (!mfma && (rows || fused)) {
+    if (!mfma && (rows || (fused && !fused->scores))) {
         set_error("paged_decode: row indices and the fused KV write need the matrix-core path");
         return FLOUR_ERR_UNSUPPORTED;
     }
@@ -1170,11 +1203,12 @@ static int paged_decode_impl(void* out, int out_dtype, const void* q, const void
                                        : workspace && workspace_bytes >= need &&
                                              ((uintptr_t)workspace % 256) == 0;
     // (an fp32 call without a workspace never touches the library's shared one)
+    const bool wts = fused && fused->scores;
     const bool f32_split =
-        dtype == FLOUR_DTYPE_F32 &&
+        dtype == FLOUR_DTYPE_F32 && !wts &&
         decode_f32_split(head_dim, block_size, n_rep, batch, num_heads, num_slots, max_context_len,
                          out, q, k_pool, v_pool, ws_ok && !ws_from_scratch);
-    if (!mfma && !f32_split) {
+    if (!mfma && !f32_split && !wts) {
         // one query row per sequence: cu_seqlens == nullptr
         const int64_t qs = (int64_t)num_heads * head_dim;
         if (simt_supported(dtype, head_dim, q, qs, head_dim, k_pool, v_pool))
@@ -1220,6 +1254,9 @@ static int paged_decode_impl(void* out, int out_dtype, const void* q, const void
     ws.new_st = fused ? fused->new_st : 0;
     ws.new_sh = fused ? fused->new_sh : 0;
     ws.new_slots = fused ? fused->new_slots : nullptr;
+    ws.scores = fused ? fused->scores : nullptr;
+    ws.score_stride = fused ? fused->score_stride : 0;
+    ws.row_ml = fused ? fused->row_ml : nullptr;
 #define FLOUR_DEC(T)                                                                            \
     do {                                                                                        \
         if (out_dtype == FLOUR_DTYPE_F32)                                                       \
@@ -1266,6 +1303,38 @@ int paged_decode_rows(void* out, int out_dtype, const void* q, const void* k_poo
                              context_lens, batch, num_heads, kv_heads, head_dim, block_size,
                              num_slots, max_context_len, scale, dtype, workspace, workspace_bytes,
                              false, rows, nullptr, stream);
+}
+
+bool paged_decode_scores_takes(int dtype, int head_dim, int block_size, int n_rep, int batch,
+                               int num_heads, int64_t num_slots, const void* out, const void* q,
+                               const void* k_pool, const void* v_pool) {
+    if (dtype != FLOUR_DTYPE_F32)
+        return decode_mfma_supported(dtype, head_dim, block_size, n_rep, batch, num_heads, num_slots,
+                                     q, k_pool, v_pool);
+    return (head_dim == 128 || head_dim == 64) && block_size % 16 == 0 && n_rep <= 16 &&
+           batch <= DEC_MAX_BATCH && num_heads <= 65535 &&
+           num_slots * head_dim * 4 <= (int64_t)0x7fffffff &&
+           (((uintptr_t)out | (uintptr_t)q | (uintptr_t)k_pool | (uintptr_t)v_pool) & 15) == 0;
+}
+
+size_t paged_decode_scores_bytes(int batch, int n_rep, int head_dim) {
+    return decode_ws_bytes(decode_workgroups(FLOUR_DTYPE_F32), n_rep, head_dim, batch);
+}
+
+int paged_decode_scores(void* out, int out_dtype, const void* q, const void* k_pool,
+                        const void* v_pool, const int32_t* block_tables, int max_blocks_per_seq,
+                        const int32_t* context_lens, int batch, int num_heads, int kv_heads,
+                        int head_dim, int block_size, int64_t num_slots, int max_context_len,
+                        float scale, int dtype, void* workspace, size_t workspace_bytes,
+                        float* scores, int64_t score_stride, float* row_ml, void* stream) {
+    DecodeWs wz{};
+    wz.scores = scores;
+    wz.score_stride = score_stride;
+    wz.row_ml = row_ml;
+    return paged_decode_impl(out, out_dtype, q, k_pool, v_pool, block_tables, max_blocks_per_seq,
+                             context_lens, batch, num_heads, kv_heads, head_dim, block_size,
+                             num_slots, max_context_len, scale, dtype, workspace, workspace_bytes,
+                             false, nullptr, &wz, stream);
 }
 
 int paged_decode_write_kv(void* out, int out_dtype, const void* q, void* k_pool, void* v_pool,

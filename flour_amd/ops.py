@@ -159,7 +159,7 @@ class Workspace:
     def get(self, nbytes: int) -> torch.Tensor:
         if self.buf is None or self.buf.numel() < nbytes:
             self.buf = torch.empty(max(nbytes, 256), dtype=torch.uint8, device=self.device)
-        if torch.cuda.is_current_stream_capturing() and \
+        if self.buf.is_cuda and torch.cuda.is_current_stream_capturing() and \
                 not any(self.buf is t for t in self.captured):
             self.captured.append(self.buf)
         return self.buf
