@@ -119,6 +119,11 @@ SHAPES = [  # (lens, keeps, recent, G, D, bs)
     ([90], [48], 7, 1, 8, 32),
     ([30, 31], [9, 16], 3, 2, 3, 1),
     ([5000], [17], 5, 1, 256, 16),
+    ([9000, 40], [8000, 39], 3, 1, 64, 16),
+    ([40000, 300], [2000, 200], 100, 1, 16, 16),
+    ([66000], [65000], 64900, 1, 8, 16),
+    ([200, 90], [150, 90], 9, 2, 64, 80),
+    ([100], [70], 9, 2, 33, 128),
 ]
 
 
