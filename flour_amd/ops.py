@@ -17,6 +17,7 @@ counterpart in the reference.
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import torch
 
@@ -318,22 +319,34 @@ def _invalid(msg: str) -> _lib.FlourError:
     return _lib.FlourError(_lib.ERR_INVALID_ARGUMENT, msg)
 
 
-def _same_device(first: torch.Tensor, *rest: torch.Tensor | None) -> None:
-    dev = first.device
-    for t in (first, *rest):
-        if t is not None and not t.is_cuda:
-            raise _invalid("flour_amd ops take device tensors (got a CPU tensor)")
-        if t is not None and t.device != dev:
-            raise _invalid(f"tensors on {dev} and {t.device}")
+def _same_device(*ts: torch.Tensor | None) -> int:
+    """The index of the one device that all tensors are on."""
+    dev = ts[0].get_device()
+    for t in ts:
+        if t is not None and t.get_device() != dev or dev < 0:
+            if not all(x is None or x.is_cuda for x in ts):
+                raise _invalid("flour_amd ops take device tensors (got a CPU tensor)")
+            raise _invalid(f"tensors on {ts[0].device} and {t.device}")
+    return dev
 
 
-def _launch(fn, device: torch.device, *args) -> None:
+def _at(t: torch.Tensor | None) -> int | None:
+    return None if t is None else t.data_ptr()
+
+
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+def _launch(fn, dev: int, *args) -> None:
     """fn(*args, stream) on the device's current stream."""
-    if device.index == torch.cuda.current_device():
-        check(fn(*args, ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)))
-        return
-    with torch.cuda.device(device):
-        check(fn(*args, ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)))
+    stream = _raw_stream(dev) if _raw_stream else torch.cuda.current_stream(dev).cuda_stream
+    if dev == torch.cuda.current_device():
+        rc = fn(*args, stream)
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, stream)
+    if rc:
+        check(rc)
 
 
 def _table(t: torch.Tensor, rows: int, what: str) -> None:
@@ -384,7 +397,7 @@ def _weights_args(weights: torch.Tensor | None, weight_rows: torch.Tensor | None
     if weights is None:
         if weight_rows is not None:
             raise _invalid("weight_rows without weights")
-        return _ptr(None), 0, _ptr(None), 0
+        return None, 0, None, 0
     if weights.dtype != torch.float32 or weights.dim() != 3 or weights.shape[1] != kv_heads or \
             not weights.is_contiguous() or weights.shape[2] < max_len:
         raise _invalid(f"{what} must be contiguous fp32 (rows, {kv_heads} kv heads, positions >= "
@@ -394,7 +407,7 @@ def _weights_args(weights: torch.Tensor | None, weight_rows: torch.Tensor | None
         _lens(weight_rows, batch, "weight_rows")
     elif weights.shape[0] < batch:
         raise _invalid(f"{what} has {weights.shape[0]} rows for {batch} sequences")
-    return _ptr(weights), weights.shape[2], _ptr(weight_rows), weights.shape[0]
+    return weights.data_ptr(), weights.shape[2], _at(weight_rows), weights.shape[0]
 
 
 def kv_write_q8(k: torch.Tensor, v: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
@@ -408,7 +421,7 @@ def kv_write_q8(k: torch.Tensor, v: torch.Tensor, k_pool: torch.Tensor, v_pool: 
     rows it holds of the sequence from before fit the 8-bit type (those are requantised if it
     grows); a non-finite row gives NaN. A block written by one call belongs to one sequence of it.
     """
-    _same_device(k, v, k_pool, v_pool, k_scale, v_scale, cu_seqlens_q, kv_lens, block_tables)
+    dev = _same_device(k, v, k_pool, v_pool, k_scale, v_scale, cu_seqlens_q, kv_lens, block_tables)
     _need_i32(cu_seqlens_q, kv_lens, block_tables)
     code, G, slots, D = _pools8(k_pool, v_pool, k_scale, v_scale, block_size)
     if k.dim() != 3 or k.shape[1:] != (G, D) or v.shape != k.shape or v.stride() != k.stride() or \
@@ -418,9 +431,9 @@ def kv_write_q8(k: torch.Tensor, v: torch.Tensor, k_pool: torch.Tensor, v_pool: 
     n = cu_seqlens_q.numel() - 1
     _lens(kv_lens, n, "kv_lens")
     _table(block_tables, n, "block_tables")
-    _launch(lib().flour_hip_kv_write_q8, k.device, _ptr(k), _ptr(v), k.stride(0), k.stride(1),
-            dtype_code(k.dtype), _ptr(k_pool), _ptr(v_pool), _ptr(k_scale), _ptr(v_scale), code,
-            _ptr(cu_seqlens_q), _ptr(kv_lens), _ptr(block_tables), block_tables.shape[1], n,
+    _launch(lib().flour_hip_kv_write_q8, dev, _at(k), _at(v), k.stride(0), k.stride(1),
+            dtype_code(k.dtype), _at(k_pool), _at(v_pool), _at(k_scale), _at(v_scale), code,
+            _at(cu_seqlens_q), _at(kv_lens), _at(block_tables), block_tables.shape[1], n,
             k.shape[0], G, D, block_size, slots)
 
 
@@ -431,7 +444,7 @@ def kv_dequant(k_pool: torch.Tensor, v_pool: torch.Tensor, k_scale: torch.Tensor
     """The values of sequences in an 8-bit cache, into the blocks that ``out_tables`` gives them in
     the plain pools ``k_out``/``v_out`` (kv_heads, out_slots, head_dim) of f32, bf16 or f16.
     ``max_kv_len`` bounds kv_lens."""
-    _same_device(k_pool, v_pool, k_scale, v_scale, block_tables, kv_lens, k_out, v_out, out_tables)
+    dev = _same_device(k_pool, v_pool, k_scale, v_scale, block_tables, kv_lens, k_out, v_out, out_tables)
     _need_i32(block_tables, kv_lens, out_tables)
     code, G, slots, D = _pools8(k_pool, v_pool, k_scale, v_scale, block_size)
     Go, out_slots, Do = _pools(k_out, v_out, block_size, "k_out and v_out")
@@ -440,12 +453,13 @@ def kv_dequant(k_pool: torch.Tensor, v_pool: torch.Tensor, k_scale: torch.Tensor
     n = kv_lens.numel()
     _table(block_tables, n, "block_tables")
     _table(out_tables, n, "out_tables")
-    _launch(lib().flour_hip_kv_dequant, k_pool.device, _ptr(k_out), _ptr(v_out),
-            dtype_code(k_out.dtype), _ptr(out_tables), out_tables.shape[1], out_slots,
-            _ptr(k_pool), _ptr(v_pool), _ptr(k_scale), _ptr(v_scale), code, _ptr(block_tables),
-            block_tables.shape[1], _ptr(kv_lens), n, max_kv_len, G, D, block_size, slots)
+    _launch(lib().flour_hip_kv_dequant, dev, _at(k_out), _at(v_out),
+            dtype_code(k_out.dtype), _at(out_tables), out_tables.shape[1], out_slots,
+            _at(k_pool), _at(v_pool), _at(k_scale), _at(v_scale), code, _at(block_tables),
+            block_tables.shape[1], _at(kv_lens), n, max_kv_len, G, D, block_size, slots)
 
 
+@functools.lru_cache(maxsize=1024)
 def decode_weights_workspace_bytes(batch: int, num_heads: int, kv_heads: int, head_dim: int,
                                    max_context_len: int, with_weights: bool) -> int:
     """Bytes of workspace of paged_decode_q8 and paged_decode_weights."""
@@ -483,7 +497,7 @@ def paged_decode_q8(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
                     weight_rows: torch.Tensor | None = None) -> torch.Tensor:
     """paged_decode over an 8-bit cache: q (batch, num_heads, head_dim) of f32, bf16 or f16. With
     ``weights`` the step's attention weights are added to it, as paged_decode_weights does."""
-    _same_device(q, k_pool, v_pool, k_scale, v_scale, block_tables, context_lens, out, weights,
+    dev = _same_device(q, k_pool, v_pool, k_scale, v_scale, block_tables, context_lens, out, weights,
                  weight_rows)
     _need_i32(block_tables, context_lens)
     code, G, slots, D = _pools8(k_pool, v_pool, k_scale, v_scale, block_size)
@@ -496,10 +510,10 @@ def paged_decode_q8(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
         raise _invalid("out must be contiguous")
     ws = _scratch(workspace, decode_weights_workspace_bytes(B, H, G, D, max_context_len,
                                                             weights is not None), q.device)
-    _launch(lib().flour_hip_paged_decode_q8, q.device, _ptr(out), dtype_code(out.dtype), _ptr(q),
-            dtype_code(q.dtype), _ptr(k_pool), _ptr(v_pool), _ptr(k_scale), _ptr(v_scale), code,
-            _ptr(block_tables), block_tables.shape[1], _ptr(context_lens), B, H, G, D, block_size,
-            slots, max_context_len, float(scale), *wargs, _ptr(ws), ws.numel())
+    _launch(lib().flour_hip_paged_decode_q8, dev, _at(out), dtype_code(out.dtype), _at(q),
+            dtype_code(q.dtype), _at(k_pool), _at(v_pool), _at(k_scale), _at(v_scale), code,
+            _at(block_tables), block_tables.shape[1], _at(context_lens), B, H, G, D, block_size,
+            slots, max_context_len, float(scale), *wargs, _at(ws), ws.numel())
     return out
 
 
@@ -513,7 +527,7 @@ def paged_decode_weights(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Te
     kv_heads, positions): weights[r, g, j] += the sum over kv head g's query heads of their softmax
     weight on position j, r = weight_rows[b] or b. Rows of one call must differ; one outside the
     tensor adds nothing."""
-    _same_device(q, k_pool, v_pool, block_tables, context_lens, out, weights, weight_rows)
+    dev = _same_device(q, k_pool, v_pool, block_tables, context_lens, out, weights, weight_rows)
     _need_i32(block_tables, context_lens)
     G, slots, D = _pools(k_pool, v_pool, block_size)
     B, H = _decode_q(q, D, G)
@@ -529,13 +543,14 @@ def paged_decode_weights(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Te
         raise _invalid("out must be contiguous")
     ws = _scratch(workspace, decode_weights_workspace_bytes(B, H, G, D, max_context_len, True),
                   q.device)
-    _launch(lib().flour_hip_paged_decode_weights, q.device, _ptr(out), dtype_code(out.dtype),
-            _ptr(q), _ptr(k_pool), _ptr(v_pool), _ptr(block_tables), block_tables.shape[1],
-            _ptr(context_lens), B, H, G, D, block_size, slots, max_context_len, float(scale),
-            dtype_code(q.dtype), *wargs, _ptr(ws), ws.numel())
+    _launch(lib().flour_hip_paged_decode_weights, dev, _at(out), dtype_code(out.dtype),
+            _at(q), _at(k_pool), _at(v_pool), _at(block_tables), block_tables.shape[1],
+            _at(context_lens), B, H, G, D, block_size, slots, max_context_len, float(scale),
+            dtype_code(q.dtype), *wargs, _at(ws), ws.numel())
     return out
 
 
+@functools.lru_cache(maxsize=1024)
 def prefill_q8_workspace_bytes(num_seqs: int, max_seqlen_q: int, total_q: int, max_kv_len: int,
                                num_heads: int, kv_heads: int, head_dim: int, block_size: int,
                                dtype: torch.dtype) -> int:
@@ -556,7 +571,7 @@ def varlen_prefill_q8(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tenso
     """varlen_prefill over an 8-bit cache that already holds the rows' K/V (kv_write_q8): packed q
     (total_q, num_heads, head_dim), any view with a unit last stride. ``max_seqlen_q`` bounds the
     rows of a sequence, ``max_kv_len`` kv_lens."""
-    _same_device(q, k_pool, v_pool, k_scale, v_scale, cu_seqlens_q, kv_lens, block_tables, out)
+    dev = _same_device(q, k_pool, v_pool, k_scale, v_scale, cu_seqlens_q, kv_lens, block_tables, out)
     _need_i32(cu_seqlens_q, kv_lens, block_tables)
     code, G, slots, D = _pools8(k_pool, v_pool, k_scale, v_scale, block_size)
     if q.dim() != 3 or q.shape[2] != D or q.stride(2) != 1 or q.shape[1] == 0 or \
@@ -572,11 +587,11 @@ def varlen_prefill_q8(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tenso
         raise _invalid("out must have a unit last stride")
     ws = _scratch(workspace, prefill_q8_workspace_bytes(n, max_seqlen_q, T, max_kv_len, H, G, D,
                                                         block_size, q.dtype), q.device)
-    _launch(lib().flour_hip_varlen_prefill_q8, q.device, _ptr(out), dtype_code(out.dtype),
-            out.stride(0), out.stride(1), _ptr(q), q.stride(0), q.stride(1), dtype_code(q.dtype),
-            _ptr(k_pool), _ptr(v_pool), _ptr(k_scale), _ptr(v_scale), code, _ptr(cu_seqlens_q),
-            _ptr(kv_lens), _ptr(block_tables), block_tables.shape[1], n, max_seqlen_q, T, H, G, D,
-            block_size, slots, max_kv_len, float(scale), _ptr(ws), ws.numel())
+    _launch(lib().flour_hip_varlen_prefill_q8, dev, _at(out), dtype_code(out.dtype),
+            out.stride(0), out.stride(1), _at(q), q.stride(0), q.stride(1), dtype_code(q.dtype),
+            _at(k_pool), _at(v_pool), _at(k_scale), _at(v_scale), code, _at(cu_seqlens_q),
+            _at(kv_lens), _at(block_tables), block_tables.shape[1], n, max_seqlen_q, T, H, G, D,
+            block_size, slots, max_kv_len, float(scale), _at(ws), ws.numel())
     return out
 
 
@@ -596,7 +611,7 @@ def kv_evict(k_pool: torch.Tensor, v_pool: torch.Tensor, weights: torch.Tensor,
 
     Returns the kept positions (batch, kv_heads, max_keep_len) int32, -1 behind the n-th.
     """
-    _same_device(k_pool, v_pool, weights, block_tables, context_lens, keep_lens, out_tables,
+    dev = _same_device(k_pool, v_pool, weights, block_tables, context_lens, keep_lens, out_tables,
                  k_scale, v_scale, weights_out, weight_rows, kept)
     _need_i32(block_tables, context_lens, keep_lens, out_tables)
     if k_pool.dtype in _POOL_DT:
@@ -624,9 +639,9 @@ def kv_evict(k_pool: torch.Tensor, v_pool: torch.Tensor, weights: torch.Tensor,
         _need_i32(kept)
         if kept.shape != shape:
             raise _invalid(f"kept must be {shape}")
-    _launch(lib().flour_hip_kv_evict, k_pool.device, _ptr(k_pool), _ptr(v_pool), _ptr(k_scale),
-            _ptr(v_scale), code, w, _ptr(weights_out), width, rows, n_rows, _ptr(block_tables),
-            block_tables.shape[1], _ptr(context_lens), _ptr(keep_lens), _ptr(out_tables),
-            out_tables.shape[1], _ptr(kept), B, G, D, block_size, slots, max_context_len,
+    _launch(lib().flour_hip_kv_evict, dev, _at(k_pool), _at(v_pool), _at(k_scale),
+            _at(v_scale), code, w, _at(weights_out), width, rows, n_rows, _at(block_tables),
+            block_tables.shape[1], _at(context_lens), _at(keep_lens), _at(out_tables),
+            out_tables.shape[1], _at(kept), B, G, D, block_size, slots, max_context_len,
             max_keep_len, recent)
     return kept
