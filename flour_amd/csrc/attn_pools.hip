@@ -140,23 +140,38 @@ __global__ __launch_bounds__(AP_THREADS) void attn_pools_kernel(
     }
 }
 
-// weights[r, g, j] += sum over kv head g's query heads of exp2(score - max) / sum, in their order.
+// weights[r, g, j] += sum over kv head g's query heads of exp2(score - max) / sum, in their order. A
+// thread takes WA_POS positions, AP_THREADS apart, so that several scores of a head are in flight.
+static constexpr int WA_POS = 4;
 __global__ __launch_bounds__(AP_THREADS) void weights_add_kernel(
     float* __restrict__ weights, int64_t width, const int32_t* __restrict__ weight_rows,
     int num_rows, const int32_t* __restrict__ context_lens, int max_ctx, int kv_heads, int n_rep,
     const float* __restrict__ scores, int64_t score_stride, const float* __restrict__ ml) {
     const int b = blockIdx.z, g = blockIdx.y;
+    const int ctx = min(context_lens[b], max_ctx), j0 = blockIdx.x * AP_THREADS * WA_POS;
     const int r = weight_rows ? weight_rows[b] : b;
-    const int64_t j = (int64_t)blockIdx.x * AP_THREADS + threadIdx.x;
-    if (r < 0 || r >= num_rows || j >= min(context_lens[b], max_ctx)) return;
-    float sum = 0.0f;
-    for (int i = 0; i < n_rep; i++) {
-        const int64_t h = ((int64_t)b * kv_heads + g) * n_rep + i;
-        const float l = ml[2 * h + 1];
-        const float p = fast_exp2(scores[h * score_stride + j] - ml[2 * h]);
-        sum += l == 0.0f ? 0.0f : p / l;
+    if (j0 >= ctx || r < 0 || r >= num_rows) return;
+    const int64_t h0 = ((int64_t)b * kv_heads + g) * n_rep;
+    float* w = weights + ((int64_t)r * kv_heads + g) * width;
+    float old[WA_POS], sum[WA_POS];
+    int j[WA_POS];
+#pragma unroll
+    for (int x = 0; x < WA_POS; x++) {  // (past the end: the last position's, for nothing)
+        j[x] = min(j0 + x * AP_THREADS + (int)threadIdx.x, ctx - 1);
+        old[x] = w[j[x]];
+        sum[x] = 0.0f;
     }
-    weights[((int64_t)r * kv_heads + g) * width + j] += sum;
+#pragma unroll 4
+    for (int i = 0; i < n_rep; i++) {
+        const float* s = scores + (h0 + i) * score_stride;
+        const float m = ml[2 * (h0 + i)], l = ml[2 * (h0 + i) + 1];
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+        for (int x = 0; x < WA_POS; x++) sum[x] = fmaf(fast_exp2(s[j[x]] - m), inv, sum[x]);
+    }
+#pragma unroll
+    for (int x = 0; x < WA_POS; x++)
+        if (j0 + x * AP_THREADS + (int)threadIdx.x < ctx) w[j[x]] = old[x] + sum[x];
 }
 
 int launch_weights_add(float* weights, int64_t width, const int32_t* weight_rows, int num_rows,
@@ -164,7 +179,8 @@ int launch_weights_add(float* weights, int64_t width, const int32_t* weight_rows
                        int n_rep, const float* scores, int64_t score_stride, const float* ml,
                        hipStream_t stream) {
     if (max_ctx <= 0) return FLOUR_OK;
-    weights_add_kernel<<<dim3((unsigned)((max_ctx + AP_THREADS - 1) / AP_THREADS), kv_heads, batch),
+    const int per = AP_THREADS * WA_POS;
+    weights_add_kernel<<<dim3((unsigned)((max_ctx + per - 1) / per), kv_heads, batch),
                          dim3(AP_THREADS), 0, stream>>>(weights, width, weight_rows, num_rows,
                                                         context_lens, max_ctx, kv_heads, n_rep,
                                                         scores, score_stride, ml);

@@ -78,11 +78,11 @@ __device__ __forceinline__ u32x2 to_f16x4<i8_t>(uint32_t w) {
                  __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, b) + off)};
 }
 
-// Resident waves per CU. Decode steps and 32 columns: two per SIMD. With 64 columns, or 32 of fp32 queries
-// in two parts, the accumulators and queries leave room for one.
+// Resident waves per CU: two per SIMD with one column tile, one with more (whose accumulators take the
+// registers; and fewer waves leave fewer pieces of 32 or 64 rows to merge).
 template <typename TQ, int NT>
 __host__ __device__ constexpr int dp_waves() {
-    return NT == 4 || (NT == 2 && sizeof(TQ) == 4) ? 4 : 8;
+    return NT > 1 ? 4 : 8;
 }
 
 // MULTI: several rows of a sequence, or more query heads of a kv head than a tile has columns;
@@ -722,32 +722,43 @@ __global__ __launch_bounds__(64 * DP_MERGE_WAVES) void decode_pools_merge_kernel
         return (2 * (f + p) + (p == 0 && !f_first ? 1 : 0)) * a.cols + cc;
     };
     float M = DEC_M0, MV = DEC_M0, L = 0.0f, O[E] = {};
+    // this wave's pieces, 64 at a time (one a lane for the maxima and sums), their rows 8 at a time, the
+    // first 8 requested beside the maxima
     const int per = (np + waves - 1) / waves, p_end = min(np, (w_id + 1) * per);
+    typedef typename std::conditional<E == 2, f32x2, float>::type RowV;
+    auto row_of = [&](int p) -> RowV {  // (past the end a row that exists, for nothing)
+        return *reinterpret_cast<const RowV*>(a.p_o + slot_of(min(p, np - 1)) * D + E * lane);
+    };
+    auto add = [&](float w, RowV v) {
+        if constexpr (E == 2) {
+            O[0] = fmaf(w, v[0], O[0]);
+            O[1] = fmaf(w, v[1], O[1]);
+        } else {
+            O[0] = fmaf(w, v, O[0]);
+        }
+    };
     for (int p0 = w_id * per; p0 < p_end; p0 += 64) {
         const bool on = p0 + lane < p_end;
-        const int64_t sl = slot_of(on ? p0 + lane : p0);
-        const float mx = on ? a.p_ml[3 * sl] : DEC_M0, mvx = on ? a.p_ml[3 * sl + 2] : DEC_M0;
-        const float lx = on ? a.p_ml[3 * sl + 1] : 0.0f;
-        const float Mn = fmaxf(M, wave_max(mx)), MVn = fmaxf(MV, wave_max(mvx));
+        const float* ml = a.p_ml + 3 * slot_of(on ? p0 + lane : p0);
+        const float mx = ml[0], lx = ml[1], mvx = ml[2];
+        RowV v[8];
+#pragma unroll
+        for (int y = 0; y < 8; y++) v[y] = row_of(p0 + y);
+        const float Mn = fmaxf(M, wave_max(on ? mx : DEC_M0));
+        const float MVn = fmaxf(MV, wave_max(on ? mvx : DEC_M0));
         L = L * fast_exp2(M - Mn) + wave_sum(on ? fast_exp2(mx - Mn) * lx : 0.0f);
         const float w = on ? fast_exp2(mvx - MVn) : 0.0f, old = fast_exp2(MV - MVn);
 #pragma unroll
         for (int e = 0; e < E; e++) O[e] *= old;
         const int n = min(64, p_end - p0);
         for (int x = 0; x < n; x += 8) {
-            float v[8][E];
+            if (x > 0)
 #pragma unroll
-            for (int y = 0; y < 8; y++) {  // loads together; past the end the first piece again
-                const float* o = a.p_o + slot_of(p0 + (x + y < n ? x + y : 0)) * D + E * lane;
-#pragma unroll
-                for (int e = 0; e < E; e++) v[y][e] = o[e];
-            }
+                for (int y = 0; y < 8; y++) v[y] = row_of(p0 + x + y);
 #pragma unroll
             for (int y = 0; y < 8; y++) {
-                const float wy = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w), (x + y) & 63));
-                if (x + y < n)
-#pragma unroll
-                    for (int e = 0; e < E; e++) O[e] = fmaf(wy, v[y][e], O[e]);
+                const float wy = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w), x + y));
+                if (x + y < n) add(wy, v[y]);
             }
         }
         M = Mn;
