@@ -22,11 +22,8 @@ static bool stream_takes(const PoolAttn& a) {
              (uint64_t)(a.o_st * oes) | (uint64_t)(a.o_sh * oes)) & 15) == 0;
 }
 
-static size_t stream_bytes(int dtype, int batch, int64_t max_cols, int head_dim) {
-    if (head_dim != 64 && head_dim != 128) return 0;
-    if (dtype == FLOUR_DTYPE_F32) return decode_stream_bytes_f32(batch, max_cols, head_dim);
-    if (dtype == FLOUR_DTYPE_BF16) return decode_stream_bytes_bf16(batch, max_cols, head_dim);
-    return decode_stream_bytes_f16(batch, max_cols, head_dim);
+static size_t stream_bytes(int batch, int64_t max_cols, int head_dim) {
+    return head_dim == 64 || head_dim == 128 ? decode_stream_bytes(batch, max_cols, head_dim) : 0;
 }
 
 static int launch_stream_call(const PoolAttn& p, int max_rows, void* ws, hipStream_t stream) {
@@ -51,10 +48,8 @@ static int launch_stream_call(const PoolAttn& p, int max_rows, void* ws, hipStre
 // Workspace: whichever kernel's part is the larger, then (with weights) the scores' maxima and sums
 // and the scores.
 static size_t decode_part(int batch, int n_rep, int head_dim) {
-    size_t n = paged_decode_scores_bytes(batch, n_rep, head_dim);
-    for (int t : {FLOUR_DTYPE_F32, FLOUR_DTYPE_BF16, FLOUR_DTYPE_F16})
-        n = std::max(n, stream_bytes(t, batch, n_rep, head_dim));
-    return up256(n);
+    return up256(std::max(paged_decode_scores_bytes(batch, n_rep, head_dim),
+                          stream_bytes(batch, n_rep, head_dim)));
 }
 static size_t weights_part(int batch, int num_heads, int max_ctx) {
     const size_t rows = (size_t)batch * num_heads;
@@ -301,8 +296,7 @@ extern "C" int flour_hip_varlen_prefill_q8_workspace_size(int num_seqs, int max_
     const size_t staged =
         stage_of(num_seqs, max_seqlen_q, max_kv_len, kv_heads, head_dim, block_size, dtype, &st)
             ? st.total : 0;
-    *bytes = std::max(staged, stream_bytes(dtype, num_seqs,
-                                           (int64_t)max_seqlen_q * (num_heads / kv_heads), head_dim));
+    *bytes = std::max(staged, stream_bytes(num_seqs, (int64_t)max_seqlen_q * (num_heads / kv_heads), head_dim));
     return FLOUR_OK;
 }
 

@@ -76,16 +76,14 @@ int launch_weights_add(float* weights, int64_t width, const int32_t* weight_rows
                        hipStream_t stream);
 
 // Per type of the queries (decode_stream_*.hip): launches, and the workspace of calls whose sequences
-// bring up to max_cols columns (rows x query heads of a kv head).
+// bring up to max_cols columns (rows x query heads of a kv head), whatever the type.
 int launch_decode_stream_f32(const DpArgs& a, int pool_dtype, int head_dim, void* ws, int max_rows,
                              int rows, hipStream_t s);
 int launch_decode_stream_bf16(const DpArgs& a, int pool_dtype, int head_dim, void* ws, int max_rows,
                               int rows, hipStream_t s);
 int launch_decode_stream_f16(const DpArgs& a, int pool_dtype, int head_dim, void* ws, int max_rows,
                              int rows, hipStream_t s);
-size_t decode_stream_bytes_f32(int batch, int64_t max_cols, int head_dim);
-size_t decode_stream_bytes_bf16(int batch, int64_t max_cols, int head_dim);
-size_t decode_stream_bytes_f16(int batch, int64_t max_cols, int head_dim);
+size_t decode_stream_bytes(int batch, int64_t max_cols, int head_dim);
 
 // Decode over a plain pool that keeps its scores (paged_decode.hip): whether it takes a shape, its
 // workspace, the call (scores of row b * num_heads + h at row * score_stride, in chunks of up to 64

@@ -78,17 +78,17 @@ __device__ __forceinline__ u32x2 to_f16x4<i8_t>(uint32_t w) {
                  __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, b) + off)};
 }
 
-// Resident waves per CU: two per SIMD with one column tile, one with more (whose accumulators take the
-// registers; and fewer waves leave fewer pieces of 32 or 64 rows to merge).
-template <typename TQ, int NT>
+// Resident waves per CU: two per SIMD, or one where a wave's registers hold several column tiles or two
+// chunks of 64 tokens at head_dim 128 (and fewer waves leave fewer pieces to merge).
+template <int D, int TILES, int NT>
 __host__ __device__ constexpr int dp_waves() {
-    return NT > 1 ? 4 : 8;
+    return NT > 1 || (TILES == 4 && D == 128) ? 4 : 8;
 }
 
 // MULTI: several rows of a sequence, or more query heads of a kv head than a tile has columns;
 // otherwise a decode step whose columns are one tile's.
 template <typename TQ, typename TP, int D, int TILES, int NT, bool MULTI, bool BS16, bool W>
-__global__ __launch_bounds__(64, (dp_waves<TQ, NT>() / 4)) void decode_pools_kernel(DpArgs a) {
+__global__ __launch_bounds__(64, (dp_waves<D, TILES, NT>() / 4)) void decode_pools_kernel(DpArgs a) {
     constexpr int CHUNK = 16 * TILES;
     constexpr int KL = D / 64;   // 16-byte K loads of a lane and tile
     constexpr int NV = D / 16;   // O^T products of a chunk's half
@@ -793,17 +793,16 @@ __global__ __launch_bounds__(64 * DP_MERGE_WAVES) void decode_pools_merge_kernel
 }
 
 // The grid's waves at most: what the workspace is sized for and what a launch is cut to.
-template <typename TQ, int NT>
+template <int D, int TILES, int NT>
 static int stream_waves() {
-    return std::min(device_cus() * dp_waves<TQ, NT>(), 4096);
+    return std::min(device_cus() * dp_waves<D, TILES, NT>(), 4096);
 }
 
 static constexpr size_t dp_up256(size_t x) { return (x + 255) & ~(size_t)255; }
 
-// Bytes of a streamed call's workspace (null: its size alone).
-template <typename TQ, int NT>
-static size_t stream_layout(DpArgs* a, void* workspace, int batch, int cols, int head_dim) {
-    const size_t slots = 2 * (size_t)stream_waves<TQ, NT>() * cols;
+// Bytes of a streamed call's workspace for `waves` waves; its parts go to *a if that is not null.
+static size_t stream_layout(DpArgs* a, void* workspace, int waves, int batch, int cols, int head_dim) {
+    const size_t slots = 2 * (size_t)waves * cols;
     const size_t ml = dp_up256(slots * 3 * sizeof(float));
     const size_t o = dp_up256(slots * head_dim * sizeof(float));
     if (a) {
@@ -816,15 +815,15 @@ static size_t stream_layout(DpArgs* a, void* workspace, int batch, int cols, int
     return ml + o + dp_up256(((size_t)batch + 1) * sizeof(int));
 }
 
-template <typename TQ, typename TP, int D, int NT, bool MULTI, bool W>
+template <typename TQ, typename TP, int D, int TILES, int NT, bool MULTI, bool W>
 static int launch_stream(DpArgs a, void* workspace, int max_rows, int rows, hipStream_t stream) {
-    constexpr int TILES = 2;
     const int64_t max_cols = (int64_t)max_rows * a.n_rep, groups = (max_cols + 16 * NT - 1) / (16 * NT);
+    const int waves = stream_waves<D, TILES, NT>();
     a.max_rows = max_rows;
-    stream_layout<TQ, NT>(&a, workspace, a.batch, (int)std::min<int64_t>(max_cols, 16 * NT), D);
+    stream_layout(&a, workspace, waves, a.batch, (int)std::min<int64_t>(max_cols, 16 * NT), D);
     const int64_t chunks = (a.max_kv + 16 * TILES - 1) / (16 * TILES);
     const int64_t half = (int64_t)a.batch * a.kv_heads * groups * chunks / 2;
-    const int grid = (int)std::max<int64_t>(1, std::min<int64_t>(half, stream_waves<TQ, NT>()));
+    const int grid = (int)std::max<int64_t>(1, std::min<int64_t>(half, waves));
     const size_t lds = a.batch <= 64 ? 0 : (size_t)(a.batch + 1) * sizeof(int);
     auto kern = a.block_size == 16 ? decode_pools_kernel<TQ, TP, D, TILES, NT, MULTI, true, W>
                                    : decode_pools_kernel<TQ, TP, D, TILES, NT, MULTI, false, W>;
@@ -832,23 +831,33 @@ static int launch_stream(DpArgs a, void* workspace, int max_rows, int rows, hipS
     const int rc = check_hip(hipGetLastError(), "8-bit attention launch");
     if (rc != FLOUR_OK) return rc;
     const int64_t pieces = 2 * (int64_t)grid / ((int64_t)a.batch * a.kv_heads * groups);
-    int waves = 1;
-    while (waves < DP_MERGE_WAVES && 8 * waves < pieces) waves *= 2;
+    int mw = 1;
+    while (mw < DP_MERGE_WAVES && 8 * mw < pieces) mw *= 2;
     decode_pools_merge_kernel<D, TILES, NT, W>
-        <<<dim3(a.num_heads, rows), dim3(64 * waves), 0, stream>>>(a, grid);
+        <<<dim3(a.num_heads, rows), dim3(64 * mw), 0, stream>>>(a, grid);
     return check_hip(hipGetLastError(), "8-bit attention merge launch");
+}
+
+// One tile of columns: chunks of 64 tokens for contexts of more than 1,024 (a bound on them, that is),
+// of 32 for shorter ones, which they cut finer. 64 / 32 in us: 8 x 16-32K tokens of 64 / 8 heads of
+// 128 83.5 / 87.7, 64 x 512-4,096 of 32 / 8 59.4 / 60.4, 1 x 2,000 11.0 / 11.6, 32 x 512-4,096 of 32 /
+// 32 heads of 64 65.5 / 69.7; 128 x 20-300 of 32 / 8 of 128 28.8 / 26.3, 8 x 100-300 11.6 / 10.4, 16 x
+// 16-1,024 of 8 / 8 of 64 12.1 / 11.4.
+template <typename TQ, typename TP, int D, bool W>
+static int launch_stream_1(const DpArgs& a, void* ws, int rows, hipStream_t s) {
+    return a.max_kv > 1024 ? launch_stream<TQ, TP, D, 4, 1, false, W>(a, ws, 1, rows, s)
+                           : launch_stream<TQ, TP, D, 2, 1, false, W>(a, ws, 1, rows, s);
 }
 
 template <typename TQ, typename TP, int D>
 static int launch_stream_d(const DpArgs& a, void* ws, int max_rows, int rows, hipStream_t s) {
     const int64_t cols = (int64_t)max_rows * a.n_rep;
     if (a.scores)
-        return cols <= 16 ? launch_stream<TQ, TP, D, 1, false, true>(a, ws, max_rows, rows, s)
-                          : launch_stream<TQ, TP, D, 2, true, true>(a, ws, max_rows, rows, s);
-    if (!a.cu && cols <= 16)
-        return launch_stream<TQ, TP, D, 1, false, false>(a, ws, max_rows, rows, s);
-    return cols <= 32 ? launch_stream<TQ, TP, D, 2, true, false>(a, ws, max_rows, rows, s)
-                      : launch_stream<TQ, TP, D, 4, true, false>(a, ws, max_rows, rows, s);
+        return cols <= 16 ? launch_stream_1<TQ, TP, D, true>(a, ws, rows, s)
+                          : launch_stream<TQ, TP, D, 2, 2, true, true>(a, ws, max_rows, rows, s);
+    if (!a.cu && cols <= 16) return launch_stream_1<TQ, TP, D, false>(a, ws, rows, s);
+    return cols <= 32 ? launch_stream<TQ, TP, D, 2, 2, true, false>(a, ws, max_rows, rows, s)
+                      : launch_stream<TQ, TP, D, 2, 4, true, false>(a, ws, max_rows, rows, s);
 }
 
 template <typename TQ>
@@ -861,16 +870,20 @@ static int launch_stream_q(const DpArgs& a, int pool_dtype, int head_dim, void* 
                           : launch_stream_d<TQ, i8_t, 128>(a, ws, max_rows, rows, s);
 }
 
-// The largest workspace of calls of up to max_cols columns.
-template <typename TQ>
-static size_t stream_bytes_q(int batch, int64_t max_cols, int head_dim) {
-    size_t n = 0;
-    if (max_cols <= 16) n = stream_layout<TQ, 1>(nullptr, nullptr, batch, (int)max_cols, head_dim);
-    n = std::max(n, stream_layout<TQ, 2>(nullptr, nullptr, batch,
-                                         (int)std::min<int64_t>(max_cols, 32), head_dim));
+// The largest workspace of the launches above for calls of up to max_cols columns.
+static inline size_t stream_bytes_for(int batch, int64_t max_cols, int head_dim) {
+    auto bytes = [&](int waves, int cols) {
+        return stream_layout(nullptr, nullptr, waves, batch, (int)std::min<int64_t>(max_cols, cols),
+                             head_dim);
+    };
+    size_t n = bytes(head_dim == 64 ? stream_waves<64, 2, 2>() : stream_waves<128, 2, 2>(), 32);
+    if (max_cols <= 16)
+        n = std::max(n, head_dim == 64 ? std::max(bytes(stream_waves<64, 2, 1>(), 16),
+                                                  bytes(stream_waves<64, 4, 1>(), 16))
+                                       : std::max(bytes(stream_waves<128, 2, 1>(), 16),
+                                                  bytes(stream_waves<128, 4, 1>(), 16)));
     if (max_cols > 32)
-        n = std::max(n, stream_layout<TQ, 4>(nullptr, nullptr, batch,
-                                             (int)std::min<int64_t>(max_cols, 64), head_dim));
+        n = std::max(n, bytes(head_dim == 64 ? stream_waves<64, 2, 4>() : stream_waves<128, 2, 4>(), 64));
     return n;
 }
 

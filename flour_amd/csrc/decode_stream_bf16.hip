@@ -8,8 +8,4 @@ int launch_decode_stream_bf16(const DpArgs& a, int pool_dtype, int head_dim, voi
     return launch_stream_q<bf16_t>(a, pool_dtype, head_dim, ws, max_rows, rows, s);
 }
 
-size_t decode_stream_bytes_bf16(int batch, int64_t max_cols, int head_dim) {
-    return stream_bytes_q<bf16_t>(batch, max_cols, head_dim);
-}
-
 }  // namespace flour

@@ -8,8 +8,8 @@ int launch_decode_stream_f16(const DpArgs& a, int pool_dtype, int head_dim, void
     return launch_stream_q<f16_t>(a, pool_dtype, head_dim, ws, max_rows, rows, s);
 }
 
-size_t decode_stream_bytes_f16(int batch, int64_t max_cols, int head_dim) {
-    return stream_bytes_q<f16_t>(batch, max_cols, head_dim);
+size_t decode_stream_bytes(int batch, int64_t max_cols, int head_dim) {
+    return stream_bytes_for(batch, max_cols, head_dim);
 }
 
 }  // namespace flour

@@ -8,8 +8,4 @@ int launch_decode_stream_f32(const DpArgs& a, int pool_dtype, int head_dim, void
     return launch_stream_q<float>(a, pool_dtype, head_dim, ws, max_rows, rows, s);
 }
 
-size_t decode_stream_bytes_f32(int batch, int64_t max_cols, int head_dim) {
-    return stream_bytes_q<float>(batch, max_cols, head_dim);
-}
-
 }  // namespace flour
