@@ -20,12 +20,11 @@
 //    the largest element just below 2^15 (exact down to 2^-31 of it); fp32 ones as two f16 parts of that
 //    (22 bits, two products).
 //  * A block's K scale multiplies its 16 tokens' scores, one factor per tile. Its V scale S_v goes
-//    into the exponent: P' = 2^(s + log2 S_v - m'), with a running maximum m' of its own beside the
-//    maximum m of s that the sum of p = 2^(s - m) uses, formed as p times a factor per tile. So P'
-//    stays in (0, 1], f16 keeps it relative to the row's largest contribution whatever the blocks'
+//    into the exponent: P' = 2^(s + log2 S_v - m'), with a reference m' of its own (within 2^8 of the
+//    running maximum) beside the maximum m of s that the sum of p = 2^(s - m) uses, formed as p times a
+//    factor per tile. So f16 keeps P' relative to the row's largest contribution whatever the blocks'
 //    scales (up to 2^100 apart, where p leaves fp32's range), and V stays the integers and e4m3 values
-//    that it is. P' is scaled by 2^14 (clear of f16's subnormals) and split into two f16 parts: two
-//    products, 22 bits.
+//    that it is. P' is split into two f16 parts: two products, 22 bits.
 //  * The score registers are the B operand of O^T = V^T P'^T as they stand; the V^T operand is built
 //    in-lane, pairs of tokens' bytes by v_perm_b32, then the same conversion.
 #pragma once
@@ -41,7 +40,9 @@
 namespace flour {
 
 static constexpr int DP_MAX_BATCH = 4096;  // per-sequence chunk sums live in LDS
-static constexpr float DP_SHIFT = 14.0f;   // P' times 2^14
+// P' times 2^7: clear of f16's subnormals down to 2^-21 of the largest, with room for a reference that lags
+// the running maximum by up to 2^8.
+static constexpr float DP_SHIFT = 7.0f, DP_LAG = 8.0f;
 static constexpr int DP_XCD_W = 2;         // the wave ranges' weight (paged_decode.hip)
 
 // Rows of sequence s, its kv length (0 where its rows see nothing).
@@ -451,12 +452,17 @@ __global__ __launch_bounds__(64, (dp_waves<D, TILES, NT>() / 4)) void decode_poo
                 }
             }
             const float m_new = fmaxf(m[ct], max_across_rows(top));
-            const float mv_new = fmaxf(mv[ct], max_across_rows(topv));
+            // The reference of P' moves only when the maximum has left it by more than 2^8: with 16
+            // columns some column's maximum rises in most chunks, and the accumulators would be
+            // rescaled in each.
+            const float mv_max = max_across_rows(topv);
+            const bool lag = mv_max > mv[ct] + DP_LAG;
+            const float mv_new = lag ? mv_max : mv[ct];
             float psum = 0.0f;
 #pragma unroll
             for (int t = 0; t < TILES; t++) {
                 // P' = p 2^(m + log2 S_v - m'): a factor per tile. It is at most 2^(m - the tile's
-                // maximum); the bound keeps it finite where every p of the tile is 0.
+                // maximum + 15); the bound keeps it finite where every p of the tile is 0.
                 const bool none = !decltype(all_seen)::value && tok0 + 16 * t >= vis[ct];
                 const float e = none ? 0.0f : (m_new - mv_new) + (lv[t] + DP_SHIFT);
                 const float gt = fast_exp2(e > 126.0f ? 126.0f : e);
@@ -478,7 +484,7 @@ __global__ __launch_bounds__(64, (dp_waves<D, TILES, NT>() / 4)) void decode_poo
             }
             lsum[ct] = lsum[ct] * fast_exp2(m[ct] - m_new) + psum;
             m[ct] = m_new;
-            if (__builtin_amdgcn_ballot_w64(mv_new > mv[ct]) != 0) {
+            if (__builtin_amdgcn_ballot_w64(lag) != 0) {
                 const float alpha = fast_exp2(mv[ct] - mv_new);
 #pragma unroll
                 for (int nn = 0; nn < NV; nn++) acc[ct][nn] *= alpha;
