@@ -185,7 +185,7 @@ extern "C" int flour_hip_paged_decode_weights(
 namespace flour {
 
 // ---- prefill
-// Few rows run on the streamed kernel, which reads the 8-bit rows once per group of up to 64 columns;
+// Few rows run on the streamed kernel, which reads the 8-bit rows once per group of up to 32 columns;
 // others stage the sequences' values once as a plain pool, whose blocks lie in order, for the prefill
 // kernels. A batch whose staged copy would be larger than STAGE_BYTES goes slice by slice (whole
 // sequences) through one copy.
@@ -227,9 +227,30 @@ static bool stage_of(int num_seqs, int max_seqlen_q, int max_kv, int kv_heads, i
     return true;
 }
 
-// Whether a call runs streamed rather than staged.
+// Whether a call runs streamed rather than staged: estimates of both in us, from the bounds that the host
+// knows.
+//  * Streamed: 10, the cache once per group of 32 columns, 7.8e-5 us a position and kv head at head_dim 128
+//    (9.4e-5 with fp32 queries), 6.1e-5 at 64, and up to 14 for the pieces of the groups.
+//  * Staged: 10, the copy at 5 TB/s, and the prefill kernel: at least one item's walk over the kv
+//    positions (24 ns each at head_dim 128, 13.5 at 64; fp32 55 and 24), or its products at 650 TFLOP/s
+//    (fp32 70, rows in tiles of 32).
+// Measured, streamed / staged, 32 / 8 heads of 128 in bf16: 1 x 4,096 tokens with 32 rows 35 / 109, 8 x
+// 4,096 with 8 39 / 132 and with 128 268 / 159, 32 x 512 with 32 76 / 45; fp32 32 x 2,048 with 32 185 /
+// 637; 14 / 2 heads of 64 8 x 1,024 with 64 41 / 26. Of 390 such calls five are more than 10% slower than
+// on the other path (15%, one 33%).
 static bool prefer_stream(const PoolAttn& a, int max_rows) {
-    return (int64_t)max_rows * (a.num_heads / a.kv_heads) <= 64;
+    const bool f32 = a.dtype == FLOUR_DTYPE_F32, d64 = a.head_dim == 64;
+    const double units = (double)a.batch * a.kv_heads * a.max_kv;
+    const int64_t cols = (int64_t)max_rows * (a.num_heads / a.kv_heads);
+    const double groups = (double)((cols + 31) / 32);
+    const double streamed = 10 + units * groups * (d64 ? 6.1e-5 : f32 ? 9.4e-5 : 7.8e-5) +
+                            std::min(2 * groups, 14.0);
+    const double walk = a.max_kv * (f32 ? (d64 ? 0.024 : 0.055) : (d64 ? 0.0135 : 0.024));
+    const double rows = f32 ? (max_rows + 31) / 32 * 32.0 : max_rows;
+    const double flops = 4.0 * a.batch * rows * a.max_kv * a.num_heads * a.head_dim;
+    const double staged = 10 + units * a.head_dim * 2 * (1 + elem_bytes(a.dtype)) / 5e6 +
+                          std::max(walk, flops / (f32 ? 7e7 : 6.5e8));
+    return streamed < staged;
 }
 
 static int prefill_staged(const PoolAttn& a, const Stage& st, int max_rows, char* ws,

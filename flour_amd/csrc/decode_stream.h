@@ -862,8 +862,10 @@ static int launch_stream_d(const DpArgs& a, void* ws, int max_rows, int rows, hi
         return cols <= 16 ? launch_stream_1<TQ, TP, D, true>(a, ws, rows, s)
                           : launch_stream<TQ, TP, D, 2, 2, true, true>(a, ws, max_rows, rows, s);
     if (!a.cu && cols <= 16) return launch_stream_1<TQ, TP, D, false>(a, ws, rows, s);
-    return cols <= 32 ? launch_stream<TQ, TP, D, 2, 2, true, false>(a, ws, max_rows, rows, s)
-                      : launch_stream<TQ, TP, D, 2, 4, true, false>(a, ws, max_rows, rows, s);
+    // More than 32 columns: groups of 32, each of which reads the cache again (a head's groups are next to
+    // each other in the list). Tiles for 64 at once spill: 32 x 2,048 tokens of 32 / 8 heads of 128, 32
+    // columns 51 us, 64 as one group 161, as two 95.
+    return launch_stream<TQ, TP, D, 2, 2, true, false>(a, ws, max_rows, rows, s);
 }
 
 template <typename TQ>
@@ -888,8 +890,6 @@ static inline size_t stream_bytes_for(int batch, int64_t max_cols, int head_dim)
                                                   bytes(stream_waves<64, 4, 1>(), 16))
                                        : std::max(bytes(stream_waves<128, 2, 1>(), 16),
                                                   bytes(stream_waves<128, 4, 1>(), 16)));
-    if (max_cols > 32)
-        n = std::max(n, bytes(head_dim == 64 ? stream_waves<64, 2, 4>() : stream_waves<128, 2, 4>(), 64));
     return n;
 }
 

@@ -8,7 +8,7 @@ import torch
 
 from _cache8 import Cache, attend, close, values
 from flour_amd import ops
-from flour_amd._lib import ERR_INVALID_ARGUMENT, ERR_UNSUPPORTED, FlourError
+from flour_amd._lib import ERR_INVALID_ARGUMENT, ERR_UNSUPPORTED, FlourError, lib
 
 pytestmark = pytest.mark.gpu
 
@@ -414,10 +414,20 @@ PREFILLS = [  # (H, G, D, bs, [(rows, kv)])
 ]
 
 
+@pytest.fixture
+def prefill_mode():
+    """Sets the path of 8-bit prefill (0 by the rule, 1 streamed, 2 staged, 3 the kernel for every
+    shape); back to the rule afterwards."""
+    yield lib().flour_hip_set_prefill_q8
+    lib().flour_hip_set_prefill_q8(0)
+
+
 @pytest.mark.parametrize("shape", range(len(PREFILLS)))
 @pytest.mark.parametrize("dtype", [BF, HF, F])
 @pytest.mark.parametrize("pool", [E, I])
-def test_prefill(device, pool, dtype, shape):
+@pytest.mark.parametrize("mode", [0, 1, 2])
+def test_prefill(device, prefill_mode, mode, pool, dtype, shape):
+    prefill_mode(mode)
     H, G, D, bs, seqs = PREFILLS[shape]
     gen = torch.Generator().manual_seed(300 + shape)
     rows, lens = [n for n, _ in seqs], [kv for _, kv in seqs]
@@ -441,11 +451,145 @@ def test_prefill(device, pool, dtype, shape):
             bound[cu[s]:cu[s + 1]] = (2 * err[:, :, None] + p_eps) * np.abs(v).max()
     for out_dtype in {F, dtype}:
         out = torch.full((sum(rows) + 2, H, D), 9.0, dtype=out_dtype, device=device)
+        ws = ops.Workspace(device)  # whose bytes are NaN in every type
+        ws.get(ops.prefill_q8_workspace_bytes(len(seqs), max(rows), sum(rows), max(lens), H, G, D,
+                                              bs, dtype)).fill_(255)
         ops.varlen_prefill_q8(q, kp, vp, ks, vs, i32(cu, device), i32(lens, device),
                               i32(tab, device), max(rows), max(lens), scale, bs,
-                              out=out[:sum(rows)], workspace=ops.Workspace(device))
+                              out=out[:sum(rows)], workspace=ws)
         close(out[:sum(rows)], want, bound)
         assert (out[sum(rows):] == 9.0).all()
+
+
+@pytest.mark.parametrize("dtype", [BF, F])
+@pytest.mark.parametrize("mode", [1, 2, 3])
+@pytest.mark.parametrize("D,bs", [(128, 16), (64, 32)])
+def test_prefill_poisoned_block_reaches_only_the_rows_that_see_it(device, prefill_mode, D, bs, mode,
+                                                                  dtype):
+    H, G, rows, kv = 6, 2, 90, 150
+    gen = torch.Generator().manual_seed(11)
+    nb = (kv + bs - 1) // bs
+    kp, ks = random_pool(G, nb + 1, bs, D, E, gen, device)
+    vp, vs = random_pool(G, nb + 1, bs, D, E, gen, device)
+    q = torch.randn((rows, H, D), generator=gen).to(dtype).to(device)
+    tab = torch.randperm(nb, generator=gen).tolist()
+    args = (i32([0, rows], device), i32([kv], device), i32([tab], device), rows, kv, 0.1, bs)
+    prefill_mode(mode)
+    clean = ops.varlen_prefill_q8(q, kp, vp, ks, vs, *args)
+    assert not torch.isnan(clean).any()
+    for s in (ks, vs):
+        for lb in (0, nb // 2 + 1, nb - 1):
+            keep = s.clone()
+            s[1, tab[lb]] = float("nan")
+            got = ops.varlen_prefill_q8(q, kp, vp, ks, vs, *args)
+            sees = torch.arange(kv - rows, kv, device=device) >= lb * bs
+            assert torch.isnan(got[sees, H // G:]).all()
+            got[sees, H // G:] = clean[sees, H // G:]
+            s.copy_(keep)
+            if mode != 2:
+                assert torch.equal(got, clean)
+                continue
+            # the prefill kernel recomputes an item with an output that is not finite, with each
+            # probability in two parts instead of once rounded to f16 (off by at most 2^-11 of the
+            # largest |v|, as the weights sum to 1); both results are rounded to the type once
+            big = float(np.abs(Cache(vp, vs, bs).rows(tab, kv)).max())
+            off = (got.double() - clean.double()).abs()
+            assert (off <= 1.01 * 2.0 ** -11 * big + torch.finfo(dtype).eps * clean.double().abs()).all()
+
+
+@pytest.mark.parametrize("mode", [1, 2])
+def test_prefill_and_decode_of_many_sequences(device, prefill_mode, mode):
+    """More sequences than a wave has lanes, some empty, some without rows."""
+    H, G, D, bs, B = 4, 2, 64, 16, 83
+    gen = torch.Generator().manual_seed(12)
+    lens = torch.randint(0, 60, (B,), generator=gen).tolist()
+    rows = [min(n, int(r)) for n, r in zip(lens, torch.randint(0, 9, (B,), generator=gen))]
+    blocks = sum((n + bs - 1) // bs for n in lens) + 1
+    tab = tables(lens, bs, blocks, gen)
+    kp, ks = random_pool(G, blocks, bs, D, I, gen, device)
+    vp, vs = random_pool(G, blocks, bs, D, I, gen, device)
+    q = torch.randn((sum(rows), H, D), generator=gen).to(HF).to(device)
+    cu, ck, cv = packed(rows), Cache(kp, ks, bs), Cache(vp, vs, bs)
+    want, bound = np.zeros(q.shape), np.zeros(q.shape)
+    for s, (n, kv) in enumerate(zip(rows, lens)):
+        if n:
+            k, v = ck.rows(tab[s], kv), cv.rows(tab[s], kv)
+            o, _, err = attend(q[cu[s]:cu[s + 1]].cpu().double().numpy(), k, v, 0.125)
+            want[cu[s]:cu[s + 1]] = o
+            bound[cu[s]:cu[s + 1]] = (2 * err[:, :, None] + 2.0 ** -11) * np.abs(v).max()
+    prefill_mode(mode)
+    got = ops.varlen_prefill_q8(q, kp, vp, ks, vs, i32(cu, device), i32(lens, device),
+                                i32(tab, device), max(rows), max(lens), 0.125, bs)
+    close(got, want, bound)
+    q = torch.randn((B, H, D), generator=gen).to(HF).to(device)
+    sums = torch.zeros((B, G, max(lens)), device=device)
+    want, bound, w, wb = want_decode(q, kp, vp, ks, vs, tab, lens, bs, 0.125)
+    got = ops.paged_decode_q8(q, kp, vp, ks, vs, i32(tab, device), i32(lens, device), 0.125,
+                              max(lens), bs, weights=sums)
+    close(got, want, bound)
+    close(sums, w, wb)
+
+
+def test_staged_prefill_in_slices(device, prefill_mode):
+    """Six sequences whose bound of 2^20 positions allows four in a staged copy: two slices."""
+    H, G, D, bs, B, most = 4, 1, 64, 16, 6, 1 << 20
+    gen = torch.Generator().manual_seed(13)
+    lens, rows = [40, 33, 500, 7, 64, 130], [40, 2, 70, 7, 0, 129]
+    blocks = sum((n + bs - 1) // bs for n in lens)
+    tab = tables(lens, bs, blocks, gen)
+    wide = torch.full((B, most // bs), -1, dtype=torch.int32)
+    for s, t in enumerate(tab):
+        wide[s, :len(t)] = torch.tensor(t)
+    kp, ks = random_pool(G, blocks, bs, D, E, gen, device)
+    vp, vs = random_pool(G, blocks, bs, D, E, gen, device)
+    q = torch.randn((sum(rows), H, D), generator=gen).to(BF).to(device)
+    nbytes = ops.prefill_q8_workspace_bytes(B, max(rows), sum(rows), most, H, G, D, bs, BF)
+    assert nbytes < (1 << 30) + (1 << 25)
+    outs = []
+    for mode, bound in ((2, max(lens)), (2, most)):
+        prefill_mode(mode)
+        outs.append(ops.varlen_prefill_q8(q, kp, vp, ks, vs, i32(packed(rows), device),
+                                          i32(lens, device), wide.to(device), max(rows), bound, 0.1,
+                                          bs))
+    assert torch.equal(*outs)
+
+
+@pytest.mark.parametrize("shape", [0, 1, 2, 4, 5, 7])
+@pytest.mark.parametrize("dtype", [BF, F])
+def test_decode_by_chunks_of_64(device, dtype, shape):
+    """A bound far above the contexts picks the kernel for long ones: the same output and sums."""
+    q, kp, vp, ks, vs, tab, lens, bs = decode_case(shape, E, dtype, device, "any")
+    want, bound, w, wb = want_decode(q, kp, vp, ks, vs, tab, lens, bs, 0.1)
+    wide = torch.zeros((len(lens), 4096 // bs + 1), dtype=torch.int32)
+    for s, t in enumerate(tab):
+        wide[s, :len(t)] = torch.tensor(t)
+    sums = torch.zeros((len(lens), kp.shape[0], 4096), device=device)
+    got = ops.paged_decode_q8(q, kp, vp, ks, vs, wide.to(device), i32(lens, device), 0.1, 4096, bs,
+                              out_dtype=F, weights=sums)
+    close(got, want, bound)
+    close(sums[:, :, :max(lens)], w, wb)
+    assert (sums[:, :, max(lens):] == 0).all()
+    plain = ops.paged_decode_q8(q, kp, vp, ks, vs, wide.to(device), i32(lens, device), 0.1, 4096, bs,
+                                out_dtype=F)
+    close(plain, want, bound)  # (a kernel of its own: the same within the bound, not bit for bit)
+
+
+def test_rows_beyond_their_bound_stay_in_bounds(device, prefill_mode):
+    """More rows than max_seqlen_q says: nothing is written outside the call's own rows."""
+    H, G, D, bs = 4, 2, 64, 16
+    gen = torch.Generator().manual_seed(14)
+    kp, ks = random_pool(G, 4, bs, D, I, gen, device)
+    q = torch.randn((20, H, D), generator=gen).to(BF).to(device)
+    prefill_mode(1)
+    n = ops.prefill_q8_workspace_bytes(1, 2, 20, 60, H, G, D, bs, BF)
+    ws = ops.Workspace(device)
+    buf = ws.get(n + 4096)
+    buf.fill_(77)
+    out = torch.full((22, H, D), 9.0, dtype=BF, device=device)
+    ops.varlen_prefill_q8(q, kp, kp, ks, ks, i32([0, 20], device), i32([60], device),
+                          i32([[0, 1, 2, 3]], device), 2, 60, 0.1, bs, out=out[:20], workspace=ws)
+    torch.cuda.synchronize()
+    assert (out[20:] == 9.0).all() and (buf[n:] == 77).all()
 
 
 # ------------------------------------------------------------------ streams and graphs
