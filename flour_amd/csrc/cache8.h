@@ -23,6 +23,13 @@ inline bool valid_pool8(int dtype) {
     return dtype == FLOUR_DTYPE_E4M3 || dtype == FLOUR_DTYPE_I8;
 }
 
+// The larger of two dwords' 16-bit halves, as unsigned (magnitudes of 16-bit floats are ordered as their
+// patterns, infinities and NaN above the finite ones).
+__device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
+    return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, a),
+                                                                  __builtin_bit_cast(u16x2, b)));
+}
+
 template <typename T>
 struct Elem8;
 
@@ -41,6 +48,11 @@ struct Elem8<e4m3_t> {
         const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
         return __builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], lo, true);
     }
+    // m's halves: the larger of them and of the magnitudes (bit patterns) in w; what a half stands for
+    static __device__ __forceinline__ uint32_t max_halves(uint32_t w, uint32_t m) {
+        return max_u16x2(max_u16x2(m, w & 0x007f007fu), (w >> 8) & 0x007f007fu);
+    }
+    static __device__ __forceinline__ float half_value(uint32_t h) { return widen1((uint8_t)h); }
     static __device__ __forceinline__ float widen1(uint8_t b) {
         return __builtin_amdgcn_cvt_f32_fp8(b, 0);
     }
@@ -54,6 +66,16 @@ struct Elem8<i8_t> {
     static constexpr float TOP = 0.9921875f;  // 127 / 128
     static constexpr int EXP = 7;
     static __device__ __forceinline__ float widen1(uint8_t b) { return (float)(int8_t)b; }
+    static __device__ __forceinline__ uint32_t max_halves(uint32_t w, uint32_t m) {
+        typedef __attribute__((ext_vector_type(2))) int16_t i16x2;
+        const i16x2 odd = __builtin_bit_cast(i16x2, w) >> (int16_t)8;
+        const i16x2 even = __builtin_bit_cast(i16x2, w << 8) >> (int16_t)8;
+        i16x2 x = __builtin_elementwise_max(__builtin_bit_cast(i16x2, m), odd);
+        x = __builtin_elementwise_max(x, (i16x2)(-odd));
+        x = __builtin_elementwise_max(x, even);
+        return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(x, (i16x2)(-even)));
+    }
+    static __device__ __forceinline__ float half_value(uint32_t h) { return (float)h; }
     static __device__ __forceinline__ uint8_t narrow1(float y) {  // |y| <= 127 (a NaN: some number)
         return (uint8_t)(int8_t)(int)__builtin_amdgcn_fmed3f(rintf(y), -127.0f, 127.0f);
     }

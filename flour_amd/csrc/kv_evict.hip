@@ -285,29 +285,31 @@ __global__ __launch_bounds__(256) void evict_gather8_kernel(
     if (u >= units) return;
     const int64_t nb = num_slots / block_size;
     const int vecs = head_dim / N;  // pieces of a row
+    // the largest magnitude of a piece (all of one row) under its row's scale
     auto amax_of = [&](Vt w, float S, uint32_t amax) -> uint32_t {
         if constexpr (N == 1) return max(amax, magnitude(Elem8<TP>::widen1(w) * S));
         else {
+            uint32_t m = 0;
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                float y[4];
-                Elem8<TP>::widen(w[j], y);
-#pragma unroll
-                for (int e = 0; e < 4; e++) amax = max(amax, magnitude(y[e] * S));
-            }
-            return amax;
+            for (int j = 0; j < 4; j++) m = Elem8<TP>::max_halves(w[j], m);
+            return max(amax, magnitude(Elem8<TP>::half_value(max(m & 0xffffu, m >> 16)) * S));
         }
     };
-    auto requantised = [&](Vt w, float S, float inv) -> Vt {
-        if constexpr (N == 1) return Elem8<TP>::narrow1(Elem8<TP>::widen1(w) * S * inv);
+    // (0 for a block of zeros and for a poisoned one; bounded, since a row of zeros can have any scale)
+    auto ratio = [](float S, float inv) { return inv > 0.0f ? fminf(S * inv, 0x1p100f) : 0.0f; };
+    // f: the row's scale over the new one. Most rows come from blocks of the scale that theirs gets: where
+    // all of a wave's do, the bits are copied.
+    auto requantised = [&](Vt w, float f) -> Vt {
+        if constexpr (N == 1) return Elem8<TP>::narrow1(Elem8<TP>::widen1(w) * f);
         else {
+            if (__builtin_amdgcn_ballot_w64(f != 1.0f) == 0) return w;
             Vt z;
 #pragma unroll
             for (int j = 0; j < 4; j++) {
                 float y[4];
                 Elem8<TP>::widen(w[j], y);
 #pragma unroll
-                for (int e = 0; e < 4; e++) y[e] = y[e] * S * inv;
+                for (int e = 0; e < 4; e++) y[e] *= f;
                 z[j] = Elem8<TP>::narrow(y);
             }
             return z;
@@ -356,8 +358,8 @@ __global__ __launch_bounds__(256) void evict_gather8_kernel(
         for (int j = 0; j < EV_HELD; j++) {
             const int e = 64 * j + lane;
             if (e < all) {
-                k[dst + e] = requantised(kh[j], skh[j], ki);
-                v[dst + e] = requantised(vh[j], svh[j], vi);
+                k[dst + e] = requantised(kh[j], ratio(skh[j], ki));
+                v[dst + e] = requantised(vh[j], ratio(svh[j], vi));
             }
         }
         for (int e0 = 64 * EV_HELD; e0 < all; e0 += 64) {
@@ -366,8 +368,8 @@ __global__ __launch_bounds__(256) void evict_gather8_kernel(
             const int e = e0 + lane;
             piece(min(e, all - 1), from, sk, sv);
             if (e < all) {
-                k[dst + e] = requantised(k[from], sk, ki);
-                v[dst + e] = requantised(v[from], sv, vi);
+                k[dst + e] = requantised(k[from], ratio(sk, ki));
+                v[dst + e] = requantised(v[from], ratio(sv, vi));
             }
         }
         if (lane == 0) {
@@ -399,8 +401,8 @@ __global__ __launch_bounds__(256) void evict_gather8_kernel(
                     ka = amax_of(k[from], sk, ka);
                     va = amax_of(v[from], sv, va);
                 } else if (e < all) {
-                    k[dst + e] = requantised(k[from], sk, inv_scale(K));
-                    v[dst + e] = requantised(v[from], sv, inv_scale(V));
+                    k[dst + e] = requantised(k[from], ratio(sk, inv_scale(K)));
+                    v[dst + e] = requantised(v[from], ratio(sv, inv_scale(V)));
                 }
             }
             if (pass == 1 && row0 == 0 && lane == 0) {

@@ -2,8 +2,9 @@
 //
 // Write: a unit is one (block that the call writes, kv head, K or V). A block's scale depends on
 // all of its new rows and on the scale that its kept rows have, so the unit finds the largest
-// magnitude first and then rounds the rows to q = rne(x / S); both walk the same rows. A wave
-// takes a unit: the maximum is a wave reduction, no unit waits for another, nothing is atomic.
+// magnitude first (on the bit patterns, two 16-bit elements an instruction) and then rounds the rows to
+// q = rne(x / S); they stay in registers in between. A wave takes a unit: the maximum is a wave
+// reduction, no unit waits for another, nothing is atomic.
 // The units of a call are listed without a pass over it: sequence s owns the blocks from index
 // cu[s] / bs + 2 s on, which leaves room for the n / bs + 2 blocks that n rows can touch.
 #include "cache8.h"
@@ -12,24 +13,51 @@
 namespace flour {
 
 static constexpr int KQ_WAVES = 4;  // units of a workgroup, one a wave
+static constexpr int KQ_HELD = 4;   // runs of a lane between the walks: 16 rows of 128 as 8-element runs
 
-// N elements of a row at p, widened.
+// N elements of a row, as they lie in memory. N is 8, or 1 where rows or pointers are not aligned.
 template <typename T, int N>
-__device__ __forceinline__ void load_run(const T* p, float (&y)[N]) {
-    if constexpr (N == 1) {
-        y[0] = to_f32(*p);
-    } else if constexpr (sizeof(T) == 4) {
-#pragma unroll
-        for (int i = 0; i < N; i += 4) {
-            const f32x4 v = *reinterpret_cast<const f32x4*>(p + i);
-            y[i] = v[0], y[i + 1] = v[1], y[i + 2] = v[2], y[i + 3] = v[3];
-        }
-    } else {
-        const u32x4 v = *reinterpret_cast<const u32x4*>(p);
-#pragma unroll
-        for (int i = 0; i < 4; i++) y[2 * i] = lo_f32<T>(v[i]), y[2 * i + 1] = hi_f32<T>(v[i]);
+struct Run {
+    u32x4 w[sizeof(T) == 4 ? 2 : 1];
+    __device__ __forceinline__ void clear() {
+        for (auto& x : w) x = u32x4{0, 0, 0, 0};
     }
-}
+    __device__ __forceinline__ void load(const T* p) {
+#pragma unroll
+        for (int i = 0; i < (int)(sizeof(w) / 16); i++) w[i] = reinterpret_cast<const u32x4*>(p)[i];
+    }
+    // the largest magnitude, as an fp32 pattern (inf and NaN stay above the finite ones)
+    __device__ __forceinline__ uint32_t amax() const {
+        uint32_t m = 0;
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) m = max(m, w[i >> 2][i & 3] & 0x7fffffffu);
+            return m;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; i++) m = max_u16x2(m, w[0][i] & 0x7fff7fffu);
+            m = max(m & 0xffffu, m >> 16);
+            return __float_as_uint(to_f32(T{(uint16_t)m}));
+        }
+    }
+    __device__ __forceinline__ void widen(float (&y)[N]) const {
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) y[i] = __uint_as_float(w[i >> 2][i & 3]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; i++) y[2 * i] = lo_f32<T>(w[0][i]), y[2 * i + 1] = hi_f32<T>(w[0][i]);
+        }
+    }
+};
+template <typename T>
+struct Run<T, 1> {
+    float v;
+    __device__ __forceinline__ void clear() { v = 0.0f; }
+    __device__ __forceinline__ void load(const T* p) { v = to_f32(*p); }
+    __device__ __forceinline__ uint32_t amax() const { return magnitude(v); }
+    __device__ __forceinline__ void widen(float (&y)[1]) const { y[0] = v; }
+};
 
 // N elements q = rne(y * inv) at p.
 template <typename TP, int N>
@@ -91,25 +119,57 @@ __global__ __launch_bounds__(64 * KQ_WAVES) void kv_write_q8_kernel(
     float* scale = (is_v ? v_scale : k_scale) + (int64_t)g * (num_slots / block_size) + id;
     const float old = kept > 0 ? *scale : 0.0f;
     const int runs = head_dim / N;  // of a row
-
+    // a lane's runs: lane, lane + 64, .. of the new rows' (row i, run c), the first KQ_HELD of them held
+    // between the two walks
+    const int64_t step_i = 64 / runs * st;
+    const int step_c = 64 % runs, all = (end - kept) * runs;
+    int c = lane % runs;
+    const T* row = src + (int64_t)(kept + lane / runs) * st;
+    auto next = [&]() {
+        c += step_c;
+        row += step_i;
+        if (c >= runs) c -= runs, row += st;
+    };
+    Run<T, N> held[KQ_HELD];
     uint32_t amax = 0;
-    for (int x = kept * runs + lane; x < end * runs; x += 64) {
-        const int i = x / runs;
-        float y[N];
-        load_run<T, N>(src + i * st + (x - i * runs) * N, y);
 #pragma unroll
-        for (int j = 0; j < N; j++) amax = max(amax, magnitude(y[j]));
+    for (int j = 0; j < KQ_HELD; j++) {
+        held[j].clear();
+        if (64 * j + lane < all) held[j].load(row + c * N);
+        next();
+    }
+    const int c1 = c;
+    const T* row1 = row;
+#pragma unroll
+    for (int j = 0; j < KQ_HELD; j++) amax = max(amax, held[j].amax());
+    for (int x = 64 * KQ_HELD + lane; x < all; x += 64) {
+        Run<T, N> r;
+        r.load(row + c * N);
+        amax = max(amax, r.amax());
+        next();
     }
     const float S = max_scale(pow2_scale(old), scale_for<TP>(wave_max_u32(amax)));
     const float inv = inv_scale(S);
-    for (int x = kept * runs + lane; x < end * runs; x += 64) {
-        const int i = x / runs;
+    const bool poisoned = !(S >= 0.0f);  // (then zeros: only those that attend to the block see NaN)
+    uint8_t* to = dst + (int64_t)kept * head_dim;
+    auto store = [&](const Run<T, N>& r, int x) {
         float y[N];
-        load_run<T, N>(src + i * st + (x - i * runs) * N, y);
-        if (!(S >= 0.0f))  // a block of scale NaN holds zeros: only those that attend to it see NaN
+        r.widen(y);
+        if (poisoned)
 #pragma unroll
-            for (int j = 0; j < N; j++) y[j] = 0.0f;
-        store_run8<TP, N>(dst + (int64_t)x * N, y, inv);
+            for (int e = 0; e < N; e++) y[e] = 0.0f;
+        store_run8<TP, N>(to + (int64_t)x * N, y, inv);
+    };
+#pragma unroll
+    for (int j = 0; j < KQ_HELD; j++)
+        if (64 * j + lane < all) store(held[j], 64 * j + lane);
+    c = c1;
+    row = row1;
+    for (int x = 64 * KQ_HELD + lane; x < all; x += 64) {
+        Run<T, N> r;
+        r.load(row + c * N);
+        store(r, x);
+        next();
     }
     if (S != old && S > 0.0f) {  // the kept rows, if the scale grew
         const float ratio = old * inv;

@@ -183,6 +183,27 @@ def test_evict_nan_values_stay_where_they_are(device, pool):
         assert not torch.isnan(vs[0, out_tab[0][lb]])
 
 
+@pytest.mark.parametrize("bs,D", [(16, 64), (16, 40), (128, 64)])
+@pytest.mark.parametrize("pool", [E, I])
+def test_evict_zero_rows_of_a_huge_scale(device, pool, bs, D):
+    """Rows of zeros under a scale of 2^120 beside rows under 2^-100: zeros stay zeros, the others keep
+    their bits where the scale that they need is theirs (their quotient of 2^220 is no fp32 number)."""
+    b = torch.randint(0, 256, (2, 1, 3 * bs, D), generator=torch.Generator().manual_seed(3)).to(torch.uint8)
+    b[(b & 127) == 127] = 3
+    b[b == 128] = 2
+    b[:, :, :bs] = 0
+    b[:, :, bs:, 0] = 0x7e if pool is E else 0x7f  # the largest element: the scale is needed
+    kv = b.view(pool).to(device)
+    s = torch.tensor([[[2.0 ** 120, 2.0 ** -100, 1.0]]] * 2, device=device)
+    w = torch.ones((1, 1, 2 * bs), device=device)
+    w[0, 0, ::2] = 2.0  # every other row is kept
+    kept = ops.kv_evict(kv[0], kv[1], w, i32([[0, 1]], device), i32([2 * bs], device), i32([bs], device),
+                        i32([[2]], device), 2 * bs, bs, 0, bs, k_scale=s[0], v_scale=s[1])
+    assert kept[0, 0].tolist() == list(range(0, 2 * bs, 2))
+    assert torch.equal(s[:, 0, 2].cpu(), torch.full((2,), 2.0 ** -100))
+    assert torch.equal(kv.view(torch.uint8).cpu()[:, 0, 2 * bs:], b[:, 0, 0:2 * bs:2])
+
+
 def test_evict_captured(device):
     lens, keeps = [1500, 90], [400, 64]
     kp, vp, ks, vs, w, tab, out_tab = make(lens, keeps, 2, 128, 16, E, device, 4)
