@@ -140,38 +140,48 @@ __global__ __launch_bounds__(AP_THREADS) void attn_pools_kernel(
     }
 }
 
-// weights[r, g, j] += sum over kv head g's query heads of exp2(score - max) / sum, in their order. A
-// thread takes WA_POS positions, AP_THREADS apart, so that several scores of a head are in flight.
+// weights[r, g, j] += sum over kv head g's query heads of exp2(score - max) / sum, in their order. It moves
+// 4 (n_rep + 2) bytes a position and kv head and computes little: a thread takes four consecutive
+// positions, 16 bytes a load (rows of any width: the loads need 4-byte alignment only), the last of a
+// row one at a time.
 static constexpr int WA_POS = 4;
+typedef f32x4 __attribute__((aligned(4))) f32x4_any;
 __global__ __launch_bounds__(AP_THREADS) void weights_add_kernel(
     float* __restrict__ weights, int64_t width, const int32_t* __restrict__ weight_rows,
     int num_rows, const int32_t* __restrict__ context_lens, int max_ctx, int kv_heads, int n_rep,
     const float* __restrict__ scores, int64_t score_stride, const float* __restrict__ ml) {
     const int b = blockIdx.z, g = blockIdx.y;
-    const int ctx = min(context_lens[b], max_ctx), j0 = blockIdx.x * AP_THREADS * WA_POS;
+    const int ctx = min(context_lens[b], max_ctx);
+    const int j0 = (blockIdx.x * AP_THREADS + (int)threadIdx.x) * WA_POS;
     const int r = weight_rows ? weight_rows[b] : b;
     if (j0 >= ctx || r < 0 || r >= num_rows) return;
     const int64_t h0 = ((int64_t)b * kv_heads + g) * n_rep;
-    float* w = weights + ((int64_t)r * kv_heads + g) * width;
-    float old[WA_POS], sum[WA_POS];
-    int j[WA_POS];
-#pragma unroll
-    for (int x = 0; x < WA_POS; x++) {  // (past the end: the last position's, for nothing)
-        j[x] = min(j0 + x * AP_THREADS + (int)threadIdx.x, ctx - 1);
-        old[x] = w[j[x]];
-        sum[x] = 0.0f;
-    }
+    float* w = weights + ((int64_t)r * kv_heads + g) * width + j0;
+    scores += h0 * score_stride + j0;
+    ml += 2 * h0;
+    auto inv_of = [&](int i) { return ml[2 * i + 1] == 0.0f ? 0.0f : 1.0f / ml[2 * i + 1]; };
+    if (j0 + WA_POS <= ctx) {
+        const f32x4 old = *reinterpret_cast<const f32x4_any*>(w);
+        f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 4
-    for (int i = 0; i < n_rep; i++) {
-        const float* s = scores + (h0 + i) * score_stride;
-        const float m = ml[2 * (h0 + i)], l = ml[2 * (h0 + i) + 1];
-        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        for (int i = 0; i < n_rep; i++) {
+            const f32x4 s = *reinterpret_cast<const f32x4_any*>(scores + i * score_stride);
+            const float m = ml[2 * i], inv = inv_of(i);
 #pragma unroll
-        for (int x = 0; x < WA_POS; x++) sum[x] = fmaf(fast_exp2(s[j[x]] - m), inv, sum[x]);
+            for (int x = 0; x < WA_POS; x++) sum[x] = fmaf(fast_exp2(s[x] - m), inv, sum[x]);
+        }
+        f32x4 y;
+#pragma unroll
+        for (int x = 0; x < WA_POS; x++) y[x] = old[x] + sum[x];
+        *reinterpret_cast<f32x4_any*>(w) = y;
+        return;
     }
-#pragma unroll
-    for (int x = 0; x < WA_POS; x++)
-        if (j0 + x * AP_THREADS + (int)threadIdx.x < ctx) w[j[x]] = old[x] + sum[x];
+    for (int x = 0; x < ctx - j0; x++) {
+        float sum = 0.0f;
+        for (int i = 0; i < n_rep; i++)
+            sum = fmaf(fast_exp2(scores[i * score_stride + x] - ml[2 * i]), inv_of(i), sum);
+        w[x] += sum;
+    }
 }
 
 int launch_weights_add(float* weights, int64_t width, const int32_t* weight_rows, int num_rows,
