@@ -104,7 +104,7 @@ static int decode_pools(const char* what, PoolAttn a, float* weights, int64_t wi
     int rc;
     if (stream_takes(a))
         rc = launch_stream_call(a, 1, workspace, stream);
-    else if (!valid_pool8(a.pool_dtype) &&
+    else if (!valid_pool8(a.pool_dtype) && a.score_stride <= 0x7fffffff / 16 &&  // (a lane's 32-bit offset)
              paged_decode_scores_takes(a.dtype, a.head_dim, a.block_size, n_rep, a.batch, a.num_heads,
                                        a.num_slots, a.out, a.q, a.k_pool, a.v_pool))
         rc = paged_decode_scores(a.out, a.out_dtype, a.q, a.k_pool, a.v_pool, a.block_tables,

@@ -357,11 +357,12 @@ __global__ __launch_bounds__(64, 2) void paged_decode_mfma_kernel(
     // 16kk + 4lg .. + 3, one per k-step 4kk .. 4kk + 3.
     constexpr int NQ = D * (int)sizeof(T) / 64;
     u32x4 qb[NQ];
-    float* score_to = nullptr;  // WTS: where the lane's scores of a chunk at token 0 go
+    // WTS: where the scores of a chunk at token 0 go, and the lane's there
+    float* score_to = nullptr;
+    const uint32_t score_lane = WTS ? (uint32_t)(lc * ws.score_stride + 4 * lg) : 0;
     auto load_q = [&](int b, int g) {
         if constexpr (WTS)
-            score_to = ws.scores + ((int64_t)b * num_heads + (int64_t)g * n_rep + lc) * ws.score_stride +
-                       4 * lg;
+            score_to = ws.scores + ((int64_t)b * num_heads + (int64_t)g * n_rep) * ws.score_stride;
         const int64_t row = ws.rows ? (int64_t)ws.rows[b] : (int64_t)b;
         const T* qh = q + (row * num_heads + (int64_t)g * n_rep + lc) * D + (F32 ? 4 : 8) * lg;
 #pragma unroll
@@ -449,7 +450,7 @@ __global__ __launch_bounds__(64, 2) void paged_decode_mfma_kernel(
             if (lc < n_rep)
 #pragma unroll
                 for (int t = 0; t < TILES; t++)
-                    *reinterpret_cast<f32x4*>(score_to + tok0 + 16 * t) =
+                    *reinterpret_cast<f32x4*>(score_to + tok0 + 16 * t + score_lane) =
                         f32x4{sv[4 * t], sv[4 * t + 1], sv[4 * t + 2], sv[4 * t + 3]};
         }
         tmax = max_across_rows(tmax);
