@@ -69,6 +69,7 @@ __global__ __launch_bounds__(AP_THREADS) void attn_pools_kernel(
         s = lo;
         i = (int)(r - cu[s]);
         q_len = cu[s + 1] - cu[s];
+        if (i < 0 || i >= q_len) return;  // (rows of no sequence)
     }
     const int kv_len = (int)min((int64_t)min(kv_lens[s], max_kv), (int64_t)max_blocks * block_size);
     const int64_t n_vis = kv_len >= q_len ? (int64_t)kv_len - q_len + i + 1 : 0;
@@ -203,8 +204,8 @@ int launch_attn_pools(const PoolAttn& a, hipStream_t stream) {
                   a.head_dim, AP_MAX_D);
         return FLOUR_ERR_UNSUPPORTED;
     }
-    if (a.num_heads > 65535 || (a.scores && (a.batch > 65535 || a.kv_heads > 65535))) {
-        set_error("attention: %d heads of %d sequences are too many", a.num_heads, a.batch);
+    if (a.num_heads > 65535) {
+        set_error("attention: %d heads are too many", a.num_heads);
         return FLOUR_ERR_UNSUPPORTED;
     }
     const int n_rep = a.num_heads / a.kv_heads;

@@ -12,9 +12,12 @@ static size_t up256(size_t x) { return (x + 255) & ~(size_t)255; }
 static int64_t score_stride_of(int max_ctx) { return ((int64_t)max_ctx + 63) / 64 * 64; }
 
 // ---- the streamed kernel
-static bool stream_takes(const PoolAttn& a) {
+static bool stream_takes(const PoolAttn& a, int max_rows) {
     const int es = elem_bytes(a.dtype), oes = elem_bytes(a.out_dtype);
-    return valid_pool8(a.pool_dtype) && (a.head_dim == 64 || a.head_dim == 128) &&
+    // (chunks of 32 positions, or more, of groups of 16 columns, or more: counted in 32 bits)
+    const double chunks = (double)a.batch * (a.max_kv / 32 + 1.0) *
+                          ((double)max_rows * (a.num_heads / a.kv_heads) / 16 + 1.0);
+    return valid_pool8(a.pool_dtype) && (a.head_dim == 64 || a.head_dim == 128) && chunks < 2e9 &&
            a.block_size % 16 == 0 && a.batch <= 4096 && a.rows <= 65535 &&
            a.num_slots * a.head_dim <= (int64_t)0x7fffffff &&
            (((uint64_t)(uintptr_t)a.q | (uint64_t)(uintptr_t)a.out | (uint64_t)(uintptr_t)a.k_pool |
@@ -78,6 +81,11 @@ static int decode_pools(const char* what, PoolAttn a, float* weights, int64_t wi
                   what, num_rows, (long long)width, a.batch, a.max_kv);
         return FLOUR_ERR_INVALID_ARGUMENT;
     }
+    if (weights && (a.batch > 65535 || a.kv_heads > 65535)) {
+        set_error("%s: weights of %d kv heads of %d sequences are too many for one call", what,
+                  a.kv_heads, a.batch);
+        return FLOUR_ERR_UNSUPPORTED;
+    }
     if (a.batch == 0) return FLOUR_OK;
     if (!a.out || !a.q || !a.k_pool || !a.v_pool || !a.block_tables || !a.kv_lens) {
         set_error("%s: null pointer", what);
@@ -102,7 +110,7 @@ static int decode_pools(const char* what, PoolAttn a, float* weights, int64_t wi
         a.score_stride = score_stride_of(a.max_kv);
     }
     int rc;
-    if (stream_takes(a))
+    if (stream_takes(a, 1))
         rc = launch_stream_call(a, 1, workspace, stream);
     else if (!valid_pool8(a.pool_dtype) && a.score_stride <= 0x7fffffff / 16 &&  // (a lane's 32-bit offset)
              paged_decode_scores_takes(a.dtype, a.head_dim, a.block_size, n_rep, a.batch, a.num_heads,
@@ -377,7 +385,7 @@ extern "C" int flour_hip_varlen_prefill_q8(
                         stage_of(num_seqs, max_seqlen_q, max_kv_len, kv_heads, head_dim, block_size,
                                  dtype, &st) &&
                         stage_takes(a, st, max_seqlen_q);
-    const bool streamed = mode != 3 && stream_takes(a);
+    const bool streamed = mode != 3 && stream_takes(a, max_seqlen_q);
     if (streamed && (mode == 1 || !staged || (mode == 0 && prefer_stream(a, max_seqlen_q))))
         return launch_stream_call(a, max_seqlen_q, workspace, s);
     if (staged) return prefill_staged(a, st, max_seqlen_q, static_cast<char*>(workspace), s);

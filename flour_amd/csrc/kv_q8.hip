@@ -104,9 +104,10 @@ __global__ __launch_bounds__(64 * KQ_WAVES) void kv_write_q8_kernel(
     const int r0 = cu[s], n = cu[s + 1] - r0, kv = kv_lens[s];
     if (n <= 0 || kv < n || r0 < 0 || r0 + n > total_q) return;
     const int p0 = kv - n;  // the first new position
-    const int64_t lb = p0 / block_size + (item - (r0 / block_size + 2 * s));
+    const int64_t nth = item - (r0 / block_size + 2 * s);  // of the sequence's blocks
+    const int64_t lb = p0 / block_size + nth;
     const int64_t first = lb * block_size;  // the block's first position
-    if (first >= kv || lb >= max_blocks) return;
+    if (nth < 0 || first >= kv || lb >= max_blocks) return;
     const int64_t id = block_tables[(int64_t)s * max_blocks + lb];
     if (id < 0 || id >= num_slots / block_size) return;
     const int kept = (int)max((int64_t)p0 - first, (int64_t)0);
@@ -268,7 +269,8 @@ bool check_pool8(const char* what, int pool_dtype, const void* k_pool, const voi
         return false;
     }
     if (kv_heads <= 0 || head_dim <= 0 || block_size <= 0 || num_slots <= 0 ||
-        num_slots % block_size != 0 || num_slots > 0x7fffffff) {
+        num_slots % block_size != 0 || num_slots > 0x7fffffff ||
+        (int64_t)block_size * head_dim > 0x7fffffff) {
         set_error("%s: bad pool shape (kv_heads=%d head_dim=%d bs=%d num_slots=%lld)", what,
                   kv_heads, head_dim, block_size, (long long)num_slots);
         return false;

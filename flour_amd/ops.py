@@ -570,7 +570,8 @@ def varlen_prefill_q8(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tenso
                       workspace: Workspace | None = None) -> torch.Tensor:
     """varlen_prefill over an 8-bit cache that already holds the rows' K/V (kv_write_q8): packed q
     (total_q, num_heads, head_dim), any view with a unit last stride. ``max_seqlen_q`` bounds the
-    rows of a sequence, ``max_kv_len`` kv_lens."""
+    rows of a sequence, ``max_kv_len`` kv_lens; rows of q behind the last sequence's (a padded
+    batch) leave ``out`` as it was."""
     dev = _same_device(q, k_pool, v_pool, k_scale, v_scale, cu_seqlens_q, kv_lens, block_tables, out)
     _need_i32(cu_seqlens_q, kv_lens, block_tables)
     code, G, slots, D = _pools8(k_pool, v_pool, k_scale, v_scale, block_size)
@@ -606,7 +607,7 @@ def kv_evict(k_pool: torch.Tensor, v_pool: torch.Tensor, weights: torch.Tensor,
     of the others by ``weights`` (rows, kv_heads, positions) into the blocks of ``out_tables``:
     n = min(keep_lens[b], context_lens[b]) in all, in their order, ties to the lower position.
     ``weights_out`` (default: ``weights`` itself) takes the kept positions' sums in front, zeros up
-    to the old length behind. Pools are plain, or 8-bit with ``k_scale``/``v_scale``. Destination
+    to the old length behind; ``weight_rows`` gives each sequence a row of its own. Pools are plain, or 8-bit with ``k_scale``/``v_scale``. Destination
     blocks must be new: in no sequence of the call and not twice among themselves.
 
     Returns the kept positions (batch, kv_heads, max_keep_len) int32, -1 behind the n-th.

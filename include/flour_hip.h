@@ -234,7 +234,8 @@ int flour_hip_varlen_prefill_ws(void* out, int out_dtype, int64_t o_stride_tok,
  * num_slots / block_size): an element of block b and kv head h stands for itself times
  * scale[h, b]. Tables, lengths, slots and q / out are those of the plain pools.
  *
- * Functions that read a pool take any scale that is not negative. Those that write one
+ * Functions that read a pool take any scale that is not negative, and elements that are numbers (the
+ * writing ones store no others). Those that write one
  * (flour_hip_kv_write_q8, flour_hip_kv_evict) store powers of two: the smallest S >= 2^-126 with
  * which no element exceeds 448 (e4m3) or 127 (int8) times S, 0 for a block of zeros. A block that
  * takes an infinity or a NaN gets the scale NaN: whoever attends to one of its positions reads
@@ -309,7 +310,8 @@ int flour_hip_decode_weights_workspace_size(int batch, int num_heads, int kv_hea
 
 /* flour_hip_varlen_prefill over an 8-bit cache, whose new rows flour_hip_kv_write_q8 has written:
  * every row attends to the quantised values, its own among them. max_kv_len bounds kv_lens (a
- * longer sequence is taken to end there). A workspace of
+ * longer sequence is taken to end there); rows behind the last sequence's, where total_q is larger
+ * than cu_seqlens_q[num_seqs], leave out as it was. A workspace of
  * flour_hip_varlen_prefill_q8_workspace_size bytes (256-byte aligned, no initialisation needed)
  * is required; calls that share one must not overlap in time. */
 int flour_hip_varlen_prefill_q8(void* out, int out_dtype, int64_t o_stride_tok,
@@ -338,7 +340,8 @@ int flour_hip_varlen_prefill_q8_workspace_size(int num_seqs, int max_seqlen_q, i
  * rows of a destination block behind position n-1 keep their bits. The old blocks are not written: shared prefix
  * blocks may be evicted from.
  *   weights      fp32 (num_weight_rows, kv_heads, weights_width), r = weight_rows[b] (b if NULL;
- *                outside [0, num_weight_rows): the entry is skipped, its kept row is all -1)
+ *                outside [0, num_weight_rows): the entry is skipped, its kept row is all -1);
+ *                entries of one call must have different rows
  *   weights_out  same shape, or weights itself: [r, g, i] = the i-th kept position's sum for i < n
  *                and 0 for n <= i < L; the rest is left as it is
  *   kept         [batch, kv_heads, max_keep_len]: the kept positions, -1 behind the n-th

@@ -131,3 +131,14 @@ def test_the_tables_of_the_64_bit_form():
         for e in (-100, -7, 0, 30):
             assert scale_for(top * 2.0 ** e, d) == 2.0 ** e
             assert scale_for(top * 2.0 ** e * (1 + 2.0 ** -20), d) == 2.0 ** (e + 1)
+
+
+def test_shapes_beyond_the_kernels_counts_are_refused():
+    for name, args in (("flour_hip_kv_write_q8", WRITE), ("flour_hip_paged_decode_q8", DECODE),
+                       ("flour_hip_varlen_prefill_q8", PREFILL), ("flour_hip_kv_dequant", DEQUANT)):
+        # a block of 2^23 x 256 = 2^31 elements
+        assert call(name, args, bs=1 << 23, D=256, slots=1 << 24) == _lib.ERR_INVALID_ARGUMENT, name
+    for change in (dict(batch=65536, rows=65536), dict(G=65536, H=65536)):
+        assert call("flour_hip_paged_decode_weights", WEIGHTS, **change) == _lib.ERR_UNSUPPORTED
+        assert "too many" in _lib.last_error()
+    assert call("flour_hip_kv_evict", EVICT, batch=65536, rows=65536) == _lib.ERR_UNSUPPORTED

@@ -592,6 +592,39 @@ def test_rows_beyond_their_bound_stay_in_bounds(device, prefill_mode):
     assert (out[20:] == 9.0).all() and (buf[n:] == 77).all()
 
 
+@pytest.mark.parametrize("D,bs", [(128, 16), (64, 32), (20, 5)])
+@pytest.mark.parametrize("mode", [0, 1, 2, 3])
+def test_padded_batch(device, prefill_mode, mode, D, bs):
+    """Rows behind the last sequence and empty sequences at the end: the rows are neither written nor
+    stored, their blocks and results stay as they were."""
+    H, G, T = 4, 2, 64
+    gen = torch.Generator().manual_seed(15)
+    prefill_mode(mode)
+    kp, ks = random_pool(G, 12, bs, D, I, gen, device)
+    vp, vs = random_pool(G, 12, bs, D, I, gen, device)
+    rows, lens = [3, 6, 0, 0], [bs + 3, 6, 0, 0]
+    tab = [[3, 7, -1, -1], [5, 8, -1, -1], [-1] * 4, [-1] * 4]
+    cu, n = packed(rows), sum(rows)
+    k = torch.randn((T, G, D), generator=gen).to(BF).to(device)
+    k[n:] = float("nan")
+    q = torch.randn((T, H, D), generator=gen).to(BF).to(device)
+    q[n:] = float("nan")
+    before = kp.clone()
+    ops.kv_write_q8(k, k, kp, vp, ks, vs, i32(cu, device), i32(lens, device), i32(tab, device), bs)
+    others = [b for b in range(12) if b not in (3, 7, 5, 8)]
+    assert torch.equal(kp.view(G, 12, bs, D)[:, others], before.view(G, 12, bs, D)[:, others])
+    assert torch.isfinite(ks).all() and torch.isfinite(vs).all()
+    out = torch.full((T, H, D), 9.0, dtype=F, device=device)
+    ops.varlen_prefill_q8(q, kp, vp, ks, vs, i32(cu, device), i32(lens, device), i32(tab, device), 8,
+                          2 * bs, 0.1, bs, out=out)
+    ck, cv = Cache(kp, ks, bs), Cache(vp, vs, bs)
+    for s in range(2):
+        v = cv.rows(tab[s], lens[s])
+        o, _, err = attend(q[cu[s]:cu[s + 1]].cpu().double().numpy(), ck.rows(tab[s], lens[s]), v, 0.1)
+        close(out[cu[s]:cu[s + 1]], o, (2 * err[:, :, None] + 2.0 ** -11) * np.abs(v).max())
+    assert (out[n:] == 9.0).all()
+
+
 # ------------------------------------------------------------------ streams and graphs
 def test_decode_captured_and_replayed(device):
     """Two captured steps that share a workspace, replayed among eager calls of their own and of a
