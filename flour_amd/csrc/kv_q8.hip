@@ -70,12 +70,13 @@ __device__ __forceinline__ void store_run8(uint8_t* p, const float (&y)[N], floa
         *reinterpret_cast<u32x2*>(p) = u32x2{Elem8<TP>::narrow(a), Elem8<TP>::narrow(b)};
     }
 }
+template <int N>
+using Raw8 = typename std::conditional<N == 1, uint8_t, u32x2>::type;  // N elements of a pool
 template <typename TP, int N>
-__device__ __forceinline__ void load_run8(const uint8_t* p, float (&y)[N]) {
+__device__ __forceinline__ void widen8(Raw8<N> w, float (&y)[N]) {
     if constexpr (N == 1) {
-        y[0] = Elem8<TP>::widen1(*p);
+        y[0] = Elem8<TP>::widen1(w);
     } else {
-        const u32x2 w = *reinterpret_cast<const u32x2*>(p);
         float a[4], b[4];
         Elem8<TP>::widen(w[0], a);
         Elem8<TP>::widen(w[1], b);
@@ -176,7 +177,7 @@ __global__ __launch_bounds__(64 * KQ_WAVES) void kv_write_q8_kernel(
         const float ratio = old * inv;
         for (int x = lane; x < kept * runs; x += 64) {
             float y[N];
-            load_run8<TP, N>(dst + (int64_t)x * N, y);
+            widen8<TP, N>(*reinterpret_cast<const Raw8<N>*>(dst + (int64_t)x * N), y);
             store_run8<TP, N>(dst + (int64_t)x * N, y, ratio);
         }
     }
@@ -222,9 +223,9 @@ __global__ __launch_bounds__(64 * KQ_WAVES) void kv_dequant_kernel(
     const int64_t dst = ((int64_t)g * out_slots + to * block_size) * head_dim;
     float ks = k_scale[g * nb + id], vs = v_scale[g * nb + id];
     if (STAGE && !(fabsf(vs) < INFINITY)) ks = __uint_as_float(0x7fc00000u), vs = 0.0f;
-    auto put = [&](T* out, const uint8_t* in, float S) {
+    auto put = [&](T* out, Raw8<N> w, float S) {
         float y[N];
-        load_run8<TP, N>(in, y);
+        widen8<TP, N>(w, y);
 #pragma unroll
         for (int j = 0; j < N; j++) {
             y[j] *= S;
@@ -241,9 +242,23 @@ __global__ __launch_bounds__(64 * KQ_WAVES) void kv_dequant_kernel(
                                                    pack2<T>(y[4], y[5]), pack2<T>(y[6], y[7])};
         }
     };
-    for (int64_t x = (int64_t)lane * N; x < (int64_t)rows * head_dim; x += 64 * N) {
-        put(k_out + dst + x, k_pool + src + x, ks);
-        put(v_out + dst + x, v_pool + src + x, vs);
+    const int64_t all = (int64_t)rows * head_dim;
+    for (int64_t x0 = (int64_t)lane * N; x0 < all; x0 += 64 * N * KQ_HELD) {
+        Raw8<N> kw[KQ_HELD], vw[KQ_HELD];
+#pragma unroll
+        for (int j = 0; j < KQ_HELD; j++) {  // (past the end: the first again, for nothing)
+            const int64_t x = x0 + 64 * N * j < all ? x0 + 64 * N * j : x0;
+            kw[j] = *reinterpret_cast<const Raw8<N>*>(k_pool + src + x);
+            vw[j] = *reinterpret_cast<const Raw8<N>*>(v_pool + src + x);
+        }
+#pragma unroll
+        for (int j = 0; j < KQ_HELD; j++) {
+            const int64_t x = x0 + 64 * N * j;
+            if (x < all) {
+                put(k_out + dst + x, kw[j], ks);
+                put(v_out + dst + x, vw[j], vs);
+            }
+        }
     }
 }
 
