@@ -76,18 +76,19 @@ struct Elem8<i8_t> {
         return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(x, (i16x2)(-even)));
     }
     static __device__ __forceinline__ float half_value(uint32_t h) { return (float)h; }
-    static __device__ __forceinline__ uint8_t narrow1(float y) {  // |y| <= 127 (a NaN: some number)
-        return (uint8_t)(int8_t)(int)__builtin_amdgcn_fmed3f(rintf(y), -127.0f, 127.0f);
+    // |y| <= 127 (a NaN: some number). At 1.5 * 2^23 fp32 counts in ones: the sum rounds y to the nearest
+    // even integer and its lowest byte is that in two's complement.
+    static __device__ __forceinline__ uint32_t whole(float y) {
+        return __float_as_uint(y + 12582912.0f);
     }
+    static __device__ __forceinline__ uint8_t narrow1(float y) { return (uint8_t)whole(y); }
     static __device__ __forceinline__ void widen(uint32_t w, float (&y)[4]) {
 #pragma unroll
         for (int i = 0; i < 4; i++) y[i] = (float)(int8_t)(w >> (8 * i));
     }
     static __device__ __forceinline__ uint32_t narrow(const float (&y)[4]) {
-        uint32_t w = 0;
-#pragma unroll
-        for (int i = 0; i < 4; i++) w |= (uint32_t)narrow1(y[i]) << (8 * i);
-        return w;
+        return __builtin_amdgcn_perm(whole(y[1]), whole(y[0]), 0x0c0c0400u) |
+               __builtin_amdgcn_perm(whole(y[3]), whole(y[2]), 0x04000c0cu);
     }
 };
 

@@ -335,6 +335,7 @@ __global__ __launch_bounds__(256) void evict_gather8_kernel(
         uint32_t ka = 0, va = 0;
 #pragma unroll
         for (int j = 0; j < EV_HELD; j++) {  // (past the end: the last piece again)
+            if (64 * j >= all) break;
             int64_t from;
             piece(min(64 * j + lane, all - 1), from, skh[j], svh[j]);
             kh[j] = k[from];
@@ -342,6 +343,7 @@ __global__ __launch_bounds__(256) void evict_gather8_kernel(
         }
 #pragma unroll
         for (int j = 0; j < EV_HELD; j++) {
+            if (64 * j >= all) break;
             ka = amax_of(kh[j], skh[j], ka);
             va = amax_of(vh[j], svh[j], va);
         }
