@@ -4,7 +4,9 @@
 // The kernels that every other one is checked against, and what runs where the streamed decode
 // (decode_stream.h) does not take a shape: any head_dim up to 512, block size, group size,
 // alignment. One workgroup a (row, query head): 256 positions at a time, a thread's whole dot
-// product each, then a thread's output dims each over the 256 weights in LDS.
+// product each, then a thread's output dims each over the 256 weights in LDS. Bound by the vector
+// units and by reading K/V once a query head: 64 x 512-4,096 tokens of 32 / 8 heads of 128 in e4m3 take
+// 807 us where the streamed kernel takes 58.
 #include <math.h>
 
 #include "cache8.h"
@@ -144,7 +146,8 @@ __global__ __launch_bounds__(AP_THREADS) void attn_pools_kernel(
 // weights[r, g, j] += sum over kv head g's query heads of exp2(score - max) / sum, in their order. It moves
 // 4 (n_rep + 2) bytes a position and kv head and computes little: a thread takes four consecutive
 // positions, 16 bytes a load (rows of any width: the loads need 4-byte alignment only), the last of a
-// row one at a time.
+// row one at a time. 64 x 512-4,096 positions of 32 / 8 heads (26 MB): 8.5 us, 3 TB/s; with four positions
+// AP_THREADS apart 13.6.
 static constexpr int WA_POS = 4;
 typedef f32x4 __attribute__((aligned(4))) f32x4_any;
 __global__ __launch_bounds__(AP_THREADS) void weights_add_kernel(

@@ -116,7 +116,9 @@ struct DecodeWs {
     const int32_t* new_slots;
     int xcd_w;  // wave-range weight w (WaveRanges): even ranges 32 + w, odd 32 - w
     // A step whose attention weights are wanted (the kernels' WTS instantiations): every score in the
-    // exp2 domain, row b * num_heads + h at scores + row * score_stride, and each row's (max, sum).
+    // exp2 domain, row b * num_heads + h at scores + row * score_stride, and each row's (max, sum). Kept
+    // rather than computed again: 64 x 512-4,096 tokens of 32 / 8 heads of 128 in bf16 105 us where a
+    // step without weights takes 91, and a second pass over K would take half of that again.
     float* scores;
     int64_t score_stride;
     float* row_ml;

@@ -1,6 +1,6 @@
 //! Raw FFI bindings of `libflour_hip.so`: the C-ABI declared in `include/flour_hip.h` (the
 //! attention hot path: KV-cache write, fused RoPE + KV write, paged decode, causal varlen
-//! prefill) and `include/flour_cache.h` (block allocator, block table, per-sequence cache and
+//! prefill, the same over 8-bit caches, attention-weight sums and eviction by them) and `include/flour_cache.h` (block allocator, block table, per-sequence cache and
 //! many sequences over one device pool).
 //!
 //! These replace, in the flour crate, `paged_attention` (`src/backend/cpu.rs:57-112`),
