@@ -320,7 +320,8 @@ int launch_kv_dequant(void* k_out, void* v_out, int dtype, const int32_t* out_ta
                       (((uintptr_t)k_pool | (uintptr_t)v_pool) & 7) == 0;
 #define FLOUR_DQ(T, TP, N)                                                                        \
     (staged_table ? kv_dequant_kernel<T, TP, N, true>                                             \
-                  : kv_dequant_kernel<T, TP, N, false>)<<<dim3((unsigned)grid), dim3(64 * KQ_WAVES), 0, s>>>(             \
+                  : kv_dequant_kernel<T, TP, N, false>)                                           \
+        <<<dim3((unsigned)grid), dim3(64 * KQ_WAVES), 0, s>>>(                                    \
         static_cast<T*>(k_out), static_cast<T*>(v_out), out_tables, out_max_blocks, out_slots,    \
         static_cast<const uint8_t*>(k_pool), static_cast<const uint8_t*>(v_pool), k_scale,        \
         v_scale, bt, max_blocks, kv_lens, num_seqs, max_kv, per_seq, kv_heads, head_dim,          \

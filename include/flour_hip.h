@@ -337,8 +337,8 @@ int flour_hip_varlen_prefill_q8_workspace_size(int num_seqs, int max_seqlen_q, i
  * position, NaN below every number. In their order, the kept rows of K and V go to the slots that
  * out_tables gives positions 0 .. n-1; keys keep the rotation of their old positions.
  * Blocks of out_tables must not be among any block_tables of the call, nor twice among their own;
- * rows of a destination block behind position n-1 keep their bits. The old blocks are not written: shared prefix
- * blocks may be evicted from.
+ * rows of a destination block behind position n-1 keep their bits. The old blocks are not written:
+ * shared prefix blocks may be evicted from.
  *   weights      fp32 (num_weight_rows, kv_heads, weights_width), r = weight_rows[b] (b if NULL;
  *                outside [0, num_weight_rows): the entry is skipped, its kept row is all -1);
  *                entries of one call must have different rows
