@@ -32,10 +32,11 @@ __device__ __forceinline__ float key_weight(uint32_t k) {
     return __uint_as_float(k == 0 ? 0x7fc00000u : k & 0x80000000u ? k & 0x7fffffffu : ~k);
 }
 
-// E: keys that a thread holds in registers, for up to 1,024 E positions; 0: any length, the weights read
-// again for every count. Held / read again, in us: 16 x 8 heads of 8,000 positions 14 / 21, 4 x 8 of 32,000
-// 29 / 45, of 64,000 61 / 95; with 32 a thread instead of 8 16 x 8,000 take 22. A wave owns a run of consecutive positions, 64 at a step, so the ordered
-// pass needs its predecessors' totals and no barrier a step.
+// E: keys that a thread holds in registers, for up to 1,024 E positions; 0: any length, the weights
+// read again for every count. Held / read again, in us: 16 x 8 heads of 8,000 positions 14 / 21, 4 x 8
+// of 32,000 29 / 45, of 64,000 61 / 95; with 32 a thread instead of 8 16 x 8,000 take 22. A wave owns
+// a run of consecutive positions, 64 at a step, so the ordered pass needs its predecessors' totals and
+// no barrier a step.
 //
 // The m-th largest key is found eight bits at a time from the highest bit in which keys differ down: a
 // histogram of the digit over the keys that share the digits found so far, in LDS, then the bin that the

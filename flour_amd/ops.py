@@ -323,7 +323,7 @@ def _same_device(*ts: torch.Tensor | None) -> int:
     """The index of the one device that all tensors are on."""
     dev = ts[0].get_device()
     for t in ts:
-        if t is not None and t.get_device() != dev or dev < 0:
+        if dev < 0 or t is not None and t.get_device() != dev:
             if not all(x is None or x.is_cuda for x in ts):
                 raise _invalid("flour_amd ops take device tensors (got a CPU tensor)")
             raise _invalid(f"tensors on {ts[0].device} and {t.device}")
@@ -334,13 +334,15 @@ def _at(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 
 
+# (a call's host time is longer than its kernels' for small batches: no attribute is looked up twice)
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
 def _launch(fn, dev: int, *args) -> None:
     """fn(*args, stream) on the device's current stream."""
     stream = _raw_stream(dev) if _raw_stream else torch.cuda.current_stream(dev).cuda_stream
-    if dev == torch.cuda.current_device():
+    if dev == _current_device():
         rc = fn(*args, stream)
     else:
         with torch.cuda.device(dev):
@@ -349,23 +351,28 @@ def _launch(fn, dev: int, *args) -> None:
         check(rc)
 
 
-def _table(t: torch.Tensor, rows: int, what: str) -> None:
-    if t.dim() != 2 or t.shape[0] != rows:
+def _table(t: torch.Tensor, rows: int, what: str) -> int:
+    """The table's blocks of a sequence."""
+    shape = t.shape
+    if len(shape) != 2 or shape[0] != rows:
         raise _invalid(f"{what} must be (sequences, blocks), got {tuple(t.shape)} for {rows}")
+    return shape[1]
 
 
 def _lens(t: torch.Tensor, n: int, what: str) -> None:
-    if t.dim() != 1 or t.shape[0] != n:
+    if t.dim() != 1 or t.numel() != n:
         raise _invalid(f"{what} must hold {n} lengths, got {tuple(t.shape)}")
 
 
 def _pools(k_pool: torch.Tensor, v_pool: torch.Tensor, block_size: int,
            what: str = "pools") -> tuple[int, int, int]:
-    if k_pool.dim() != 3 or v_pool.shape != k_pool.shape or v_pool.dtype != k_pool.dtype or \
+    shape = k_pool.shape
+    if len(shape) != 3 or v_pool.shape != shape or v_pool.dtype != k_pool.dtype or \
             not k_pool.is_contiguous() or not v_pool.is_contiguous():
         raise _invalid(f"{what} must be contiguous (kv_heads, num_slots, head_dim) of one dtype")
-    _check_block_size(k_pool.shape[1], block_size)
-    return k_pool.shape
+    if block_size <= 0 or shape[1] % block_size != 0:
+        _check_block_size(shape[1], block_size)
+    return shape
 
 
 def _pools8(k_pool: torch.Tensor, v_pool: torch.Tensor, k_scale: torch.Tensor,
@@ -375,11 +382,10 @@ def _pools8(k_pool: torch.Tensor, v_pool: torch.Tensor, k_scale: torch.Tensor,
     code = _POOL_DT.get(k_pool.dtype)
     if code is None:
         raise _invalid(f"8-bit pools are torch.float8_e4m3fn or torch.int8, not {k_pool.dtype}")
+    shape = (G, slots // block_size)
     for t in (k_scale, v_scale):
-        if t is None or t.dtype != torch.float32 or t.shape != (G, slots // block_size) or \
-                not t.is_contiguous():
-            raise _invalid(f"scales must be contiguous fp32 (kv_heads, num_blocks) = "
-                           f"{(G, slots // block_size)}")
+        if t is None or t.dtype != torch.float32 or t.shape != shape or not t.is_contiguous():
+            raise _invalid(f"scales must be contiguous fp32 (kv_heads, num_blocks) = {shape}")
     return code, G, slots, D
 
 
@@ -424,17 +430,18 @@ def kv_write_q8(k: torch.Tensor, v: torch.Tensor, k_pool: torch.Tensor, v_pool: 
     dev = _same_device(k, v, k_pool, v_pool, k_scale, v_scale, cu_seqlens_q, kv_lens, block_tables)
     _need_i32(cu_seqlens_q, kv_lens, block_tables)
     code, G, slots, D = _pools8(k_pool, v_pool, k_scale, v_scale, block_size)
-    if k.dim() != 3 or k.shape[1:] != (G, D) or v.shape != k.shape or v.stride() != k.stride() or \
-            v.dtype != k.dtype or k.stride(2) != 1:
+    shape, strides = k.shape, k.stride()
+    if len(shape) != 3 or shape[1] != G or shape[2] != D or v.shape != shape or \
+            v.stride() != strides or v.dtype != k.dtype or strides[2] != 1:
         raise _invalid("k/v must be (num_tokens, kv_heads, head_dim) sharing dtype and strides, "
                        "unit last stride")
     n = cu_seqlens_q.numel() - 1
     _lens(kv_lens, n, "kv_lens")
-    _table(block_tables, n, "block_tables")
-    _launch(lib().flour_hip_kv_write_q8, dev, _at(k), _at(v), k.stride(0), k.stride(1),
-            dtype_code(k.dtype), _at(k_pool), _at(v_pool), _at(k_scale), _at(v_scale), code,
-            _at(cu_seqlens_q), _at(kv_lens), _at(block_tables), block_tables.shape[1], n,
-            k.shape[0], G, D, block_size, slots)
+    width = _table(block_tables, n, "block_tables")
+    _launch(lib().flour_hip_kv_write_q8, dev, k.data_ptr(), v.data_ptr(), strides[0], strides[1],
+            dtype_code(k.dtype), k_pool.data_ptr(), v_pool.data_ptr(), k_scale.data_ptr(),
+            v_scale.data_ptr(), code, cu_seqlens_q.data_ptr(), kv_lens.data_ptr(),
+            block_tables.data_ptr(), width, n, shape[0], G, D, block_size, slots)
 
 
 def kv_dequant(k_pool: torch.Tensor, v_pool: torch.Tensor, k_scale: torch.Tensor,
@@ -451,12 +458,13 @@ def kv_dequant(k_pool: torch.Tensor, v_pool: torch.Tensor, k_scale: torch.Tensor
     if (Go, Do) != (G, D):
         raise _invalid("k_out and v_out must have the cache's kv_heads and head_dim")
     n = kv_lens.numel()
-    _table(block_tables, n, "block_tables")
-    _table(out_tables, n, "out_tables")
-    _launch(lib().flour_hip_kv_dequant, dev, _at(k_out), _at(v_out),
-            dtype_code(k_out.dtype), _at(out_tables), out_tables.shape[1], out_slots,
-            _at(k_pool), _at(v_pool), _at(k_scale), _at(v_scale), code, _at(block_tables),
-            block_tables.shape[1], _at(kv_lens), n, max_kv_len, G, D, block_size, slots)
+    width = _table(block_tables, n, "block_tables")
+    out_width = _table(out_tables, n, "out_tables")
+    _launch(lib().flour_hip_kv_dequant, dev, k_out.data_ptr(), v_out.data_ptr(),
+            dtype_code(k_out.dtype), out_tables.data_ptr(), out_width, out_slots,
+            k_pool.data_ptr(), v_pool.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), code,
+            block_tables.data_ptr(), width, kv_lens.data_ptr(), n, max_kv_len, G, D, block_size,
+            slots)
 
 
 @functools.lru_cache(maxsize=1024)
@@ -481,11 +489,22 @@ def _scratch(workspace: Workspace | None, nbytes: int, device: torch.device) -> 
 
 
 def _decode_q(q: torch.Tensor, D: int, G: int) -> tuple[int, int]:
-    if q.dim() != 3 or q.shape[2] != D or not q.is_contiguous() or q.shape[1] == 0 or \
-            q.shape[1] % G != 0:
+    shape = q.shape
+    if len(shape) != 3 or shape[2] != D or not q.is_contiguous() or shape[1] == 0 or \
+            shape[1] % G != 0:
         raise _invalid("q must be contiguous (batch, num_heads, head_dim), num_heads a multiple "
                        "of the pools' kv_heads")
-    return q.shape[0], q.shape[1]
+    return shape[0], shape[1]
+
+
+def _decode_out(out: torch.Tensor | None, q: torch.Tensor,
+                dtype: torch.dtype | None) -> torch.Tensor:
+    if out is None:
+        return torch.empty_like(q, dtype=dtype)
+    out = _out(out, q.shape, q.dtype, q.device)
+    if not out.is_contiguous():
+        raise _invalid("out must be contiguous")
+    return out
 
 
 def paged_decode_q8(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
@@ -503,17 +522,16 @@ def paged_decode_q8(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
     code, G, slots, D = _pools8(k_pool, v_pool, k_scale, v_scale, block_size)
     B, H = _decode_q(q, D, G)
     _lens(context_lens, B, "context_lens")
-    _table(block_tables, B, "block_tables")
+    width = _table(block_tables, B, "block_tables")
     wargs = _weights_args(weights, weight_rows, G, B, max_context_len)
-    out = _out(out, q.shape, out_dtype or q.dtype, q.device)
-    if not out.is_contiguous():
-        raise _invalid("out must be contiguous")
+    out = _decode_out(out, q, out_dtype)
     ws = _scratch(workspace, decode_weights_workspace_bytes(B, H, G, D, max_context_len,
                                                             weights is not None), q.device)
-    _launch(lib().flour_hip_paged_decode_q8, dev, _at(out), dtype_code(out.dtype), _at(q),
-            dtype_code(q.dtype), _at(k_pool), _at(v_pool), _at(k_scale), _at(v_scale), code,
-            _at(block_tables), block_tables.shape[1], _at(context_lens), B, H, G, D, block_size,
-            slots, max_context_len, float(scale), *wargs, _at(ws), ws.numel())
+    _launch(lib().flour_hip_paged_decode_q8, dev, out.data_ptr(), dtype_code(out.dtype),
+            q.data_ptr(), dtype_code(q.dtype), k_pool.data_ptr(), v_pool.data_ptr(),
+            k_scale.data_ptr(), v_scale.data_ptr(), code, block_tables.data_ptr(), width,
+            context_lens.data_ptr(), B, H, G, D, block_size, slots, max_context_len, float(scale),
+            *wargs, ws.data_ptr(), ws.numel())
     return out
 
 
@@ -536,17 +554,15 @@ def paged_decode_weights(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Te
     if weights is None:
         raise _invalid("paged_decode_weights needs weights")
     _lens(context_lens, B, "context_lens")
-    _table(block_tables, B, "block_tables")
+    width = _table(block_tables, B, "block_tables")
     wargs = _weights_args(weights, weight_rows, G, B, max_context_len)
-    out = _out(out, q.shape, out_dtype or q.dtype, q.device)
-    if not out.is_contiguous():
-        raise _invalid("out must be contiguous")
+    out = _decode_out(out, q, out_dtype)
     ws = _scratch(workspace, decode_weights_workspace_bytes(B, H, G, D, max_context_len, True),
                   q.device)
-    _launch(lib().flour_hip_paged_decode_weights, dev, _at(out), dtype_code(out.dtype),
-            _at(q), _at(k_pool), _at(v_pool), _at(block_tables), block_tables.shape[1],
-            _at(context_lens), B, H, G, D, block_size, slots, max_context_len, float(scale),
-            dtype_code(q.dtype), *wargs, _at(ws), ws.numel())
+    _launch(lib().flour_hip_paged_decode_weights, dev, out.data_ptr(), dtype_code(out.dtype),
+            q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), block_tables.data_ptr(), width,
+            context_lens.data_ptr(), B, H, G, D, block_size, slots, max_context_len, float(scale),
+            dtype_code(q.dtype), *wargs, ws.data_ptr(), ws.numel())
     return out
 
 
@@ -575,24 +591,26 @@ def varlen_prefill_q8(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tenso
     dev = _same_device(q, k_pool, v_pool, k_scale, v_scale, cu_seqlens_q, kv_lens, block_tables, out)
     _need_i32(cu_seqlens_q, kv_lens, block_tables)
     code, G, slots, D = _pools8(k_pool, v_pool, k_scale, v_scale, block_size)
-    if q.dim() != 3 or q.shape[2] != D or q.stride(2) != 1 or q.shape[1] == 0 or \
-            q.shape[1] % G != 0:
+    shape, strides = q.shape, q.stride()
+    if len(shape) != 3 or shape[2] != D or strides[2] != 1 or shape[1] == 0 or shape[1] % G != 0:
         raise _invalid("q must be (total_q, num_heads, head_dim) with a unit last stride, "
                        "num_heads a multiple of the pools' kv_heads")
-    T, H, _ = q.shape
+    T, H, _ = shape
     n = cu_seqlens_q.numel() - 1
     _lens(kv_lens, n, "kv_lens")
-    _table(block_tables, n, "block_tables")
-    out = _out(out, q.shape, out_dtype or q.dtype, q.device)
-    if out.stride(2) != 1:
+    width = _table(block_tables, n, "block_tables")
+    out = _out(out, shape, out_dtype or q.dtype, q.device)
+    out_strides = out.stride()
+    if out_strides[2] != 1:
         raise _invalid("out must have a unit last stride")
     ws = _scratch(workspace, prefill_q8_workspace_bytes(n, max_seqlen_q, T, max_kv_len, H, G, D,
                                                         block_size, q.dtype), q.device)
-    _launch(lib().flour_hip_varlen_prefill_q8, dev, _at(out), dtype_code(out.dtype),
-            out.stride(0), out.stride(1), _at(q), q.stride(0), q.stride(1), dtype_code(q.dtype),
-            _at(k_pool), _at(v_pool), _at(k_scale), _at(v_scale), code, _at(cu_seqlens_q),
-            _at(kv_lens), _at(block_tables), block_tables.shape[1], n, max_seqlen_q, T, H, G, D,
-            block_size, slots, max_kv_len, float(scale), _at(ws), ws.numel())
+    _launch(lib().flour_hip_varlen_prefill_q8, dev, out.data_ptr(), dtype_code(out.dtype),
+            out_strides[0], out_strides[1], q.data_ptr(), strides[0], strides[1],
+            dtype_code(q.dtype), k_pool.data_ptr(), v_pool.data_ptr(), k_scale.data_ptr(),
+            v_scale.data_ptr(), code, cu_seqlens_q.data_ptr(), kv_lens.data_ptr(),
+            block_tables.data_ptr(), width, n, max_seqlen_q, T, H, G, D, block_size, slots,
+            max_kv_len, float(scale), ws.data_ptr(), ws.numel())
     return out
 
 
