@@ -478,13 +478,13 @@ def decode_weights_workspace_bytes(batch: int, num_heads: int, kv_heads: int, he
     return n.value
 
 
-def _scratch(workspace: Workspace | None, nbytes: int, device: torch.device) -> torch.Tensor:
+def _scratch(workspace: Workspace | None, nbytes: int, q: torch.Tensor) -> torch.Tensor:
     # Without a caller's workspace each call has scratch of its own, in its stream's order.
     if workspace is None:
-        return torch.empty(max(nbytes, 256), dtype=torch.uint8, device=device)
+        return torch.empty(max(nbytes, 256), dtype=torch.uint8, device=q.device)
     ws = workspace.get(nbytes)
-    if ws.device != device:
-        raise _invalid(f"workspace on {ws.device}, tensors on {device}")
+    if ws.get_device() != q.get_device():
+        raise _invalid(f"workspace on {ws.device}, tensors on {q.device}")
     return ws
 
 
@@ -526,7 +526,7 @@ def paged_decode_q8(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
     wargs = _weights_args(weights, weight_rows, G, B, max_context_len)
     out = _decode_out(out, q, out_dtype)
     ws = _scratch(workspace, decode_weights_workspace_bytes(B, H, G, D, max_context_len,
-                                                            weights is not None), q.device)
+                                                            weights is not None), q)
     _launch(lib().flour_hip_paged_decode_q8, dev, out.data_ptr(), dtype_code(out.dtype),
             q.data_ptr(), dtype_code(q.dtype), k_pool.data_ptr(), v_pool.data_ptr(),
             k_scale.data_ptr(), v_scale.data_ptr(), code, block_tables.data_ptr(), width,
@@ -557,8 +557,7 @@ def paged_decode_weights(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Te
     width = _table(block_tables, B, "block_tables")
     wargs = _weights_args(weights, weight_rows, G, B, max_context_len)
     out = _decode_out(out, q, out_dtype)
-    ws = _scratch(workspace, decode_weights_workspace_bytes(B, H, G, D, max_context_len, True),
-                  q.device)
+    ws = _scratch(workspace, decode_weights_workspace_bytes(B, H, G, D, max_context_len, True), q)
     _launch(lib().flour_hip_paged_decode_weights, dev, out.data_ptr(), dtype_code(out.dtype),
             q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), block_tables.data_ptr(), width,
             context_lens.data_ptr(), B, H, G, D, block_size, slots, max_context_len, float(scale),
@@ -604,7 +603,7 @@ def varlen_prefill_q8(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tenso
     if out_strides[2] != 1:
         raise _invalid("out must have a unit last stride")
     ws = _scratch(workspace, prefill_q8_workspace_bytes(n, max_seqlen_q, T, max_kv_len, H, G, D,
-                                                        block_size, q.dtype), q.device)
+                                                        block_size, q.dtype), q)
     _launch(lib().flour_hip_varlen_prefill_q8, dev, out.data_ptr(), dtype_code(out.dtype),
             out_strides[0], out_strides[1], q.data_ptr(), strides[0], strides[1],
             dtype_code(q.dtype), k_pool.data_ptr(), v_pool.data_ptr(), k_scale.data_ptr(),
