@@ -625,6 +625,51 @@ def test_padded_batch(device, prefill_mode, mode, D, bs):
     assert (out[n:] == 9.0).all()
 
 
+@pytest.mark.parametrize("D", [128, 64, 20])
+@pytest.mark.parametrize("mode", [0, 1, 2, 3])
+def test_prefill_strides(device, prefill_mode, mode, D):
+    """Queries that are one row for every head (stride 0), and outputs inside larger rows, head by head:
+    the bits of the contiguous call, nothing beside them written."""
+    H, G, bs, T = 4, 2, 16, 9
+    gen = torch.Generator().manual_seed(16)
+    prefill_mode(mode)
+    kp, ks = random_pool(G, 6, bs, D, E, gen, device)
+    row = torch.randn((T, 1, D), generator=gen).to(BF).to(device)
+    args = (kp, kp, ks, ks, i32([0, 4, T], device), i32([30, 40], device),
+            i32([[0, 3, -1], [5, 1, 2]], device), 5, 40, 0.1, bs)
+    want = ops.varlen_prefill_q8(row.expand(T, H, D).contiguous(), *args)
+    for shape, view in (((H, T, 2 * D), lambda x: x.transpose(0, 1)[:, :, :D]),
+                        ((T, 2 * H, D), lambda x: x[:, H:])):
+        buf = torch.full(shape, 9.0, dtype=BF, device=device)
+        out = ops.varlen_prefill_q8(row.expand(T, H, D), *args, out=view(buf))
+        assert torch.equal(out, want)
+        view(buf).fill_(9.0)
+        assert (buf == 9.0).all()
+
+
+@pytest.mark.parametrize("D", [128, 64, 20])
+def test_one_sequence_listed_twice(device, D):
+    """A sequence's table in two entries of a decode step (two samples of one prompt): equal rows, and each
+    entry's weights in its own row."""
+    H, G, bs = 8, 2, 16
+    gen = torch.Generator().manual_seed(17)
+    kp, ks = random_pool(G, 70, bs, D, I, gen, device)
+    q = torch.randn((1, H, D), generator=gen).to(BF).to(device).repeat(3, 1, 1)
+    tab = torch.randperm(70, generator=gen)[:63].to(torch.int32).to(device).repeat(3, 1)
+    w = torch.zeros((4, G, 1000), device=device)
+    out = ops.paged_decode_q8(q, kp, kp, ks, ks, tab, i32([1000, 1000, 7], device), 0.1, 1000, bs,
+                              out_dtype=F, weights=w, weight_rows=i32([3, 0, 7], device))
+    # The scores are the same bits. Cut into other pieces, sums of up to 1,000 terms, 32 or more an instruction,
+    # are rounded in another order (up to 32 additions and as many pieces: 64 * 2^-24 of the sum of
+    # magnitudes), and weights relative to another reference (2^-20): twice that of |v| < 4; of the
+    # denominator alone for the weights, at most H / G a position.
+    err = 2 * (64 * 2.0 ** -24 + 2.0 ** -20)
+    close(out[1], out[0].cpu().double().numpy(), 4 * err)
+    close(w[3], w[0].cpu().double().numpy(), H // G * err)
+    assert abs(float(w[0].double().sum()) - H) < H * err
+    assert (w[1:3] == 0).all()
+
+
 # ------------------------------------------------------------------ streams and graphs
 def test_decode_captured_and_replayed(device):
     """Two captured steps that share a workspace, replayed among eager calls of their own and of a
@@ -695,7 +740,6 @@ def test_two_streams_without_a_workspace(device):
     for pair in got:
         for g, w in zip(pair, want):
             assert torch.equal(g[0], w[0]) and torch.equal(g[1], w[1])
-
 
 
 # ------------------------------------------------------------------ refusals (nothing is launched)
