@@ -9,6 +9,8 @@
 // 807 us where the streamed kernel takes 58.
 #include <math.h>
 
+#include <algorithm>
+
 #include "cache8.h"
 #include "decode_pools.h"
 
@@ -41,44 +43,26 @@ __device__ __forceinline__ float ap_reduce(float x, float* red, F op) {
     return r;
 }
 
-// scores (or null): (batch, num_heads, score_stride) in the exp2 domain, ml (batch, num_heads, 2)
-// their maximum and sum: decode steps only.
+// Row r of q for query head h: row i of the q_len of sequence s. scores (or null): (batch, num_heads,
+// score_stride) in the exp2 domain, ml (batch, num_heads, 2) their maximum and sum: decode steps only.
 template <typename TQ, typename TP>
-__global__ __launch_bounds__(AP_THREADS) void attn_pools_kernel(
-    void* __restrict__ out, int out_dtype, int64_t o_st, int64_t o_sh, const TQ* __restrict__ q,
-    int64_t q_st, int64_t q_sh, const TP* __restrict__ k_pool, const TP* __restrict__ v_pool,
-    const float* __restrict__ k_scale, const float* __restrict__ v_scale,
-    const int32_t* __restrict__ cu, const int32_t* __restrict__ kv_lens,
-    const int32_t* __restrict__ block_tables, int max_blocks, int num_seqs, int num_heads,
-    int n_rep, int head_dim, int block_size, int64_t num_slots, int max_kv, float scale_log2,
-    float* __restrict__ scores, int64_t score_stride, float* __restrict__ ml) {
+__device__ __forceinline__ void attn_row(const PoolAttn& a, int64_t r, int h, int s, int i, int q_len) {
     __shared__ float qs[AP_MAX_D];
     __shared__ float ps[AP_THREADS];
     __shared__ int64_t rows[AP_THREADS];
     __shared__ float red[AP_THREADS / 64];
-    const int64_t r = blockIdx.x;
-    const int h = blockIdx.y, tid = threadIdx.x;
-    int s = (int)r, i = 0, q_len = 1;
-    if (cu) {
-        int lo = 0, hi = num_seqs;
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            if (cu[mid] <= r)
-                lo = mid;
-            else
-                hi = mid;
-        }
-        s = lo;
-        i = (int)(r - cu[s]);
-        q_len = cu[s + 1] - cu[s];
-        if (i < 0 || i >= q_len) return;  // (rows of no sequence)
-    }
-    const int kv_len = (int)min((int64_t)min(kv_lens[s], max_kv), (int64_t)max_blocks * block_size);
+    const TQ* __restrict__ q = static_cast<const TQ*>(a.q);
+    const TP* __restrict__ k_pool = static_cast<const TP*>(a.k_pool);
+    const TP* __restrict__ v_pool = static_cast<const TP*>(a.v_pool);
+    const int tid = threadIdx.x, head_dim = a.head_dim, block_size = a.block_size;
+    const float scale_log2 = a.scale * LOG2_E;
+    const int kv_len =
+        (int)min((int64_t)min(a.kv_lens[s], a.max_kv), (int64_t)a.max_blocks * block_size);
     const int64_t n_vis = kv_len >= q_len ? (int64_t)kv_len - q_len + i + 1 : 0;
-    const int g = h / n_rep;
-    const int64_t nb = num_slots / block_size;
-    const int32_t* bt = block_tables + (int64_t)s * max_blocks;
-    for (int d = tid; d < head_dim; d += AP_THREADS) qs[d] = to_f32(q[r * q_st + h * q_sh + d]);
+    const int g = h / (a.num_heads / a.kv_heads);
+    const int64_t nb = a.num_slots / block_size;
+    const int32_t* bt = a.block_tables + (int64_t)s * a.max_blocks;
+    for (int d = tid; d < head_dim; d += AP_THREADS) qs[d] = to_f32(q[r * a.q_st + h * a.q_sh + d]);
     __syncthreads();
 
     float m = -3.402823466e38f, l = 0.0f, acc[AP_MAX_D / AP_THREADS] = {};
@@ -90,15 +74,15 @@ __global__ __launch_bounds__(AP_THREADS) void attn_pools_kernel(
             const int64_t lb = j / block_size;
             int64_t id = bt[lb];
             id = id < 0 ? 0 : (id >= nb ? nb - 1 : id);
-            row = ((int64_t)g * num_slots + id * block_size + (j - lb * block_size)) * head_dim;
+            row = ((int64_t)g * a.num_slots + id * block_size + (j - lb * block_size)) * head_dim;
             float dot = 0.0f;
             for (int d = 0; d < head_dim; d++) dot = fmaf(qs[d], pool_f32(k_pool + row + d), dot);
-            if (k_scale) {
-                dot *= k_scale[g * nb + id];
-                vs = v_scale[g * nb + id];
+            if (a.k_scale) {
+                dot *= a.k_scale[g * nb + id];
+                vs = a.v_scale[g * nb + id];
             }
             sc = dot * scale_log2;
-            if (scores) scores[(r * num_heads + h) * score_stride + j] = sc;
+            if (a.scores) a.scores[(r * a.num_heads + h) * a.score_stride + j] = sc;
         }
         rows[tid] = row;
         const float m_new =
@@ -127,19 +111,68 @@ __global__ __launch_bounds__(AP_THREADS) void attn_pools_kernel(
     for (int x = 0; x < AP_MAX_D / AP_THREADS; x++) {
         const int d = tid + x * AP_THREADS;
         if (d < head_dim) {
-            const int64_t at = r * o_st + h * o_sh + d;
+            const int64_t at = r * a.o_st + h * a.o_sh + d;
             const float y = l == 0.0f ? 0.0f : acc[x] * inv;
-            if (out_dtype == FLOUR_DTYPE_F32)
-                static_cast<float*>(out)[at] = y;
-            else if (out_dtype == FLOUR_DTYPE_BF16)
-                static_cast<bf16_t*>(out)[at] = from_f32<bf16_t>(y);
+            if (a.out_dtype == FLOUR_DTYPE_F32)
+                static_cast<float*>(a.out)[at] = y;
+            else if (a.out_dtype == FLOUR_DTYPE_BF16)
+                static_cast<bf16_t*>(a.out)[at] = from_f32<bf16_t>(y);
             else
-                static_cast<f16_t*>(out)[at] = from_f32<f16_t>(y);
+                static_cast<f16_t*>(a.out)[at] = from_f32<f16_t>(y);
         }
     }
-    if (scores && tid == 0) {
-        ml[(r * num_heads + h) * 2] = m;
-        ml[(r * num_heads + h) * 2 + 1] = l;
+    if (a.scores && tid == 0) {
+        a.ml[(r * a.num_heads + h) * 2] = m;
+        a.ml[(r * a.num_heads + h) * 2 + 1] = l;
+    }
+}
+
+template <typename TQ, typename TP>
+__global__ __launch_bounds__(AP_THREADS) void attn_pools_kernel(PoolAttn a) {
+    const int r = blockIdx.x;
+    int s = r, i = 0, q_len = 1;
+    if (a.cu) {
+        int lo = 0, hi = a.batch;
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (a.cu[mid] <= r)
+                lo = mid;
+            else
+                hi = mid;
+        }
+        s = lo;
+        i = r - a.cu[s];
+        q_len = a.cu[s + 1] - a.cu[s];
+        if (i < 0 || i >= q_len) return;  // (rows of no sequence)
+    }
+    attn_row<TQ, TP>(a, r, blockIdx.y, s, i, q_len);
+}
+
+// Prefill with f16 queries whose copy of the cache in f16 (kv_q8.hip) may have lost values: the rows of the
+// (sequence, kv head) pairs that hold such a block, `share` workgroups each, from the 8 bits again. Other
+// pairs' workgroups read the scales and end, so that a call without such blocks takes a launch more: 16 x
+// 128-512 rows over 1,152-1,536 tokens of 28 / 4 heads of 128 125.5 -> 129 us, 4 x 256-512 over 512-1,024
+// of 14 / 2 of 64 28 -> 31, 1,024 rows over 32,768 of 32 / 8 of 128 942 -> 952.
+template <typename TP>
+__global__ __launch_bounds__(AP_THREADS) void attn_beyond_f16_kernel(PoolAttn a, int share) {
+    const int pair = blockIdx.x / share, part = blockIdx.x - pair * share;
+    const int s = pair / a.kv_heads, g = pair - s * a.kv_heads, n_rep = a.num_heads / a.kv_heads;
+    const int r0 = a.cu[s], q_len = a.cu[s + 1] - r0;
+    if (q_len <= 0 || r0 < 0 || r0 + q_len > a.rows) return;
+    const int64_t kv_len =
+        min((int64_t)min(a.kv_lens[s], a.max_kv), (int64_t)a.max_blocks * a.block_size);
+    const int64_t nb = a.num_slots / a.block_size;
+    const int blocks = (int)((kv_len + a.block_size - 1) / a.block_size);
+    bool beyond = false;
+    for (int lb = threadIdx.x; lb < blocks; lb += AP_THREADS) {
+        int64_t id = a.block_tables[(int64_t)s * a.max_blocks + lb];
+        id = g * nb + (id < 0 ? 0 : (id >= nb ? nb - 1 : id));
+        beyond |= beyond_f16<TP>(a.k_scale[id]) || beyond_f16<TP>(a.v_scale[id]);
+    }
+    if (!__syncthreads_or(beyond)) return;
+    for (int64_t x = part; x < (int64_t)q_len * n_rep; x += share) {
+        const int i = (int)(x / n_rep);
+        attn_row<f16_t, TP>(a, r0 + i, g * n_rep + (int)(x - (int64_t)i * n_rep), s, i, q_len);
     }
 }
 
@@ -211,13 +244,8 @@ int launch_attn_pools(const PoolAttn& a, hipStream_t stream) {
         set_error("attention: %d heads are too many", a.num_heads);
         return FLOUR_ERR_UNSUPPORTED;
     }
-    const int n_rep = a.num_heads / a.kv_heads;
 #define FLOUR_AP(TQ, TP)                                                                          \
-    attn_pools_kernel<TQ, TP><<<dim3(a.rows, a.num_heads), dim3(AP_THREADS), 0, stream>>>(        \
-        a.out, a.out_dtype, a.o_st, a.o_sh, static_cast<const TQ*>(a.q), a.q_st, a.q_sh,          \
-        static_cast<const TP*>(a.k_pool), static_cast<const TP*>(a.v_pool), a.k_scale, a.v_scale, \
-        a.cu, a.kv_lens, a.block_tables, a.max_blocks, a.batch, a.num_heads, n_rep, a.head_dim,   \
-        a.block_size, a.num_slots, a.max_kv, a.scale * LOG2_E, a.scores, a.score_stride, a.ml)
+    attn_pools_kernel<TQ, TP><<<dim3(a.rows, a.num_heads), dim3(AP_THREADS), 0, stream>>>(a)
 #define FLOUR_AP_Q(TQ)                                                                            \
     do {                                                                                          \
         if (a.pool_dtype == FLOUR_DTYPE_E4M3) FLOUR_AP(TQ, e4m3_t);                               \
@@ -230,6 +258,20 @@ int launch_attn_pools(const PoolAttn& a, hipStream_t stream) {
 #undef FLOUR_AP_Q
 #undef FLOUR_AP
     return check_hip(hipGetLastError(), "attention (any pool) launch");
+}
+
+int launch_attn_beyond_f16(const PoolAttn& a, int max_rows, hipStream_t stream) {
+    const int64_t pairs = (int64_t)a.batch * a.kv_heads;
+    const int64_t work = (int64_t)max_rows * (a.num_heads / a.kv_heads);
+    const int share = (int)std::max<int64_t>(1, std::min<int64_t>(1024 / pairs, work));
+    if (pairs > 0x7fffffff / share) {
+        set_error("attention: %d sequences of %d kv heads are too many", a.batch, a.kv_heads);
+        return FLOUR_ERR_UNSUPPORTED;
+    }
+    auto kern = a.pool_dtype == FLOUR_DTYPE_E4M3 ? attn_beyond_f16_kernel<e4m3_t>
+                                                 : attn_beyond_f16_kernel<i8_t>;
+    kern<<<dim3((unsigned)(pairs * share)), dim3(AP_THREADS), 0, stream>>>(a, share);
+    return check_hip(hipGetLastError(), "attention beyond f16 launch");
 }
 
 }  // namespace flour

@@ -38,6 +38,7 @@ struct Elem8<e4m3_t> {
     // amax = f 2^x, f in [1/2, 1): amax <= 448 2^e = 0.875 2^(9 + e)
     static constexpr float TOP = 0.875f;
     static constexpr int EXP = 9;
+    static constexpr float QMAX = 448.0f;
     // the four elements of a dword
     static __device__ __forceinline__ void widen(uint32_t w, float (&y)[4]) {
         const f32x2 a = __builtin_amdgcn_cvt_pk_f32_fp8(w, false);
@@ -65,6 +66,7 @@ template <>
 struct Elem8<i8_t> {
     static constexpr float TOP = 0.9921875f;  // 127 / 128
     static constexpr int EXP = 7;
+    static constexpr float QMAX = 127.0f;
     static __device__ __forceinline__ float widen1(uint8_t b) { return (float)(int8_t)b; }
     static __device__ __forceinline__ uint32_t max_halves(uint32_t w, uint32_t m) {
         typedef __attribute__((ext_vector_type(2))) int16_t i16x2;
@@ -123,6 +125,15 @@ __device__ __forceinline__ uint32_t wave_max_u32(uint32_t x) {  // of magnitudes
 
 // The larger of two scales; NaN if either is.
 __device__ __forceinline__ float max_scale(float a, float b) { return vmax(a, b); }
+
+// Whether a copy of a block's values in f16 could lose what f16 has for them: its largest possible
+// one, QMAX S, is beyond 65,504, or so small that f16's spacing near zero, 2^-24, rounds them by more than
+// 2^-12 of QMAX S / 2 (a scale that the write chose is used to half at least). No for 0 and NaN.
+template <typename T>
+__device__ __forceinline__ bool beyond_f16(float s) {
+    const float top = s * Elem8<T>::QMAX;
+    return top > 65504.0f || (top > 0.0f && top < 0x1p-12f);
+}
 
 // What x is multiplied by for x / S (0 where the block has no scale).
 __device__ __forceinline__ float inv_scale(float s) { return s > 0.0f ? 1.0f / s : 0.0f; }

@@ -194,8 +194,10 @@ namespace flour {
 
 // ---- prefill
 // Few rows run on the streamed kernel, which reads the 8-bit rows once per group of up to 32 columns;
-// others stage the sequences' values once as a plain pool, whose blocks lie in order, for the prefill
-// kernels. A batch whose staged copy would be larger than STAGE_BYTES goes slice by slice (whole
+// others stage the sequences' values once as a plain pool of the queries' type, whose blocks lie in order,
+// for the prefill kernels. bf16 and fp32 hold q * S of any block whose S is a power of two; f16 those
+// within its range, so with f16 queries the heads that have others are computed again from the 8 bits
+// (attn_beyond_f16_kernel). A batch whose staged copy would be larger than STAGE_BYTES goes slice by slice (whole
 // sequences) through one copy.
 static int g_prefill_q8 = 0;  // 0: by the rule, 1: streamed, 2: staged, 3: the kernel for every shape
 
@@ -239,7 +241,7 @@ static bool stage_of(int num_seqs, int max_seqlen_q, int max_kv, int kv_heads, i
 // knows.
 //  * Streamed: 10, the cache once per group of 32 columns, 7.8e-5 us a position and kv head at head_dim 128
 //    (9.4e-5 with fp32 queries), 6.1e-5 at 64, and up to 14 for the pieces of the groups.
-//  * Staged: 10, the copy at 5 TB/s, and the prefill kernel: at least one item's walk over the kv
+//  * Staged: 10, 3 with f16 queries (attn_beyond_f16_kernel), the copy at 5 TB/s, and the prefill kernel: at least one item's walk over the kv
 //    positions (24 ns each at head_dim 128, 13.5 at 64; fp32 55 and 24), or its products at 650 TFLOP/s
 //    (fp32 70, rows in tiles of 32).
 // Measured, streamed / staged, 32 / 8 heads of 128 in bf16: 1 x 4,096 tokens with 32 rows 35 / 109, 8 x
@@ -256,7 +258,7 @@ static bool prefer_stream(const PoolAttn& a, int max_rows) {
     const double walk = a.max_kv * (f32 ? (d64 ? 0.024 : 0.055) : (d64 ? 0.0135 : 0.024));
     const double rows = f32 ? (max_rows + 31) / 32 * 32.0 : max_rows;
     const double flops = 4.0 * a.batch * rows * a.max_kv * a.num_heads * a.head_dim;
-    const double staged = 10 + units * a.head_dim * 2 * (1 + elem_bytes(a.dtype)) / 5e6 +
+    const double staged = (a.dtype == FLOUR_DTYPE_F16 ? 13 : 10) + units * a.head_dim * 2 * (1 + elem_bytes(a.dtype)) / 5e6 +
                           std::max(walk, flops / (f32 ? 7e7 : 6.5e8));
     return streamed < staged;
 }
@@ -283,7 +285,7 @@ static int prefill_staged(const PoolAttn& a, const Stage& st, int max_rows, char
                                  st.slots, a.scale, a.dtype, v_stage, st.v_stage, a.max_kv, stream);
         if (rc != FLOUR_OK) return rc;
     }
-    return FLOUR_OK;
+    return a.dtype == FLOUR_DTYPE_F16 ? launch_attn_beyond_f16(a, max_rows, stream) : FLOUR_OK;
 }
 
 // Whether the prefill kernels that read rows by cu alone take the call's q and out.

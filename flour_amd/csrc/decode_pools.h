@@ -58,6 +58,8 @@ struct DpArgs {
 
 // Takes every shape (attn_pools.hip).
 int launch_attn_pools(const PoolAttn& a, hipStream_t stream);
+// After a staged prefill with f16 queries: the rows of the heads whose values f16 does not hold.
+int launch_attn_beyond_f16(const PoolAttn& a, int max_rows, hipStream_t stream);
 
 // flour_hip_kv_dequant's kernel; out_tables null: block lb of sequence s goes to block
 // s * out_max_blocks + lb, and staged_table and staged_lens (both or neither) take that table and the

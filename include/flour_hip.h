@@ -309,7 +309,12 @@ int flour_hip_decode_weights_workspace_size(int batch, int num_heads, int kv_hea
                                             int max_context_len, int with_weights, size_t* bytes);
 
 /* flour_hip_varlen_prefill over an 8-bit cache, whose new rows flour_hip_kv_write_q8 has written:
- * every row attends to the quantised values, its own among them. max_kv_len bounds kv_lens (a
+ * every row attends to the quantised values, its own among them. Which kernels run goes by the shape of
+ * the call; all take any scale. Calls of many rows round each value, element times scale, once to
+ * `dtype` (values of power-of-two scales are exact in f32 and bf16, and in f16 but for a last half step of
+ * 2^-25 near zero; a head whose blocks could hold values beyond f16's range, or so small that this half
+ * step would be more than 2^-12 of their largest, is computed from the 8 bits, which takes many times
+ * as long) and with 16-bit queries each probability once to f16. max_kv_len bounds kv_lens (a
  * longer sequence is taken to end there); rows behind the last sequence's, where total_q is larger
  * than cu_seqlens_q[num_seqs], leave out as it was. A workspace of
  * flour_hip_varlen_prefill_q8_workspace_size bytes (256-byte aligned, no initialisation needed)

@@ -1,0 +1,120 @@
+"""8-bit prefill over the whole range of scales and elements, on each of its paths: what a cache gives
+does not depend on which one the shape of the batch selects."""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+from _cache8 import Cache, attend, close
+from flour_amd import ops
+from flour_amd._lib import lib
+
+pytestmark = pytest.mark.gpu
+
+E, I = torch.float8_e4m3fn, torch.int8
+BF, HF, F = torch.bfloat16, torch.float16, torch.float32
+
+
+def i32(x, device):
+    return torch.tensor(x, dtype=torch.int32, device=device)
+
+
+def full_pool(G, blocks, bs, D, dtype, gen, device):
+    """An 8-bit pool of every byte but e4m3's NaN and int8's -128."""
+    b = torch.randint(0, 256, (G, blocks * bs, D), generator=gen).to(torch.uint8)
+    if dtype == E:
+        b[(b & 127) == 127] = 126
+    else:
+        b[b == 128] = 127
+    return b.view(dtype).to(device)
+
+
+@pytest.fixture
+def prefill_mode():
+    """Sets the path of 8-bit prefill (1 streamed, 2 staged, 3 the kernel for every shape); back to the
+    rule afterwards."""
+    yield lib().flour_hip_set_prefill_q8
+    lib().flour_hip_set_prefill_q8(0)
+
+
+def u_of(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+def check(device, pool, dtype, D, ks, vs, scale, stage_u, seed, qmag=1.0, H=6, lens=(130, 70),
+          rows=(40, 70), bs=16):
+    """Prefill of two sequences against 64 bits, each kv head by its own largest |v|; ks and vs (G,
+    blocks). stage_u: the half step to which a staged copy rounds K and V, 0 where it is exact."""
+    G, B = ks.shape[0], len(lens)
+    gen = torch.Generator().manual_seed(seed)
+    nb = [(n + bs - 1) // bs for n in lens]
+    perm = torch.randperm(sum(nb), generator=gen).tolist()
+    tab = [perm[sum(nb[:s]):sum(nb[:s + 1])] for s in range(B)]
+    kp, vp = (full_pool(G, sum(nb), bs, D, pool, gen, device) for _ in "kv")
+    q = (qmag * torch.randn((sum(rows), H, D), generator=gen)).to(dtype).to(device)
+    ks, vs = ks.to(device), vs.to(device)
+    cu = [0] + np.cumsum(rows).tolist()
+    wide = [t + [0] * (max(nb) - len(t)) for t in tab]
+    got = ops.varlen_prefill_q8(q, kp, vp, ks, vs, i32(cu, device), i32(lens, device),
+                                i32(wide, device), max(rows), max(lens), scale, bs, out_dtype=F)
+    ck, cv = Cache(kp, ks, bs), Cache(vp, vs, bs)
+    # longer calls over 16-bit queries round each probability to f16 once
+    p_u = 2.0 ** -11 if dtype != F else 0.0
+    for s in range(B):
+        k, v = ck.rows(tab[s], lens[s]), cv.rows(tab[s], lens[s])
+        qs = q[cu[s]:cu[s + 1]].cpu().double().numpy()
+        want, _, err = attend(qs, k, v, scale)
+        rep = H // G
+        big = np.repeat(np.abs(v).max((0, 2)), rep)  # of the query head's kv head
+        # K rounded by u: every score off by u sum |q k|, every weight by a factor within exp(2 that)
+        dots = np.einsum("ihd,jhd->ihj", np.abs(qs), np.abs(np.repeat(k, rep, 1))).max(2) * scale
+        bound = 2 * err + p_u + np.expm1(2 * stage_u * dots) + stage_u
+        close(got[cu[s]:cu[s + 1]], want, (bound * big)[:, :, None])
+
+
+def blocks_of(lens=(130, 70), bs=16):
+    return sum((n + bs - 1) // bs for n in lens)
+
+
+@pytest.mark.parametrize("mode", [1, 2, 3])
+@pytest.mark.parametrize("dtype", [BF, HF, F])
+@pytest.mark.parametrize("D", [128, 64])
+@pytest.mark.parametrize("pool", [E, I])
+def test_prefill_over_scales_that_f16_does_not_hold(device, prefill_mode, pool, D, dtype, mode):
+    """K blocks of values up to 2^20 and V blocks down to 2^-30 in some heads and sequences; one K block of
+    values around 2^-30 beside ordinary ones."""
+    prefill_mode(mode)
+    n = blocks_of()
+    one = 2.0 ** -9 if pool == E else 2.0 ** -7  # a block of values of about 1
+    for kf, vf, scale in ((2.0 ** 20, 1.0, 2.0 ** -26), (1.0, 2.0 ** -30, 0.05),
+                          (2.0 ** 12, 2.0 ** 18, 2.0 ** -18), (2.0 ** -30, 2.0 ** -40, 0.1),
+                          (2.0 ** 7, 2.0 ** -17, 2.0 ** -10)):
+        for part in range(3):
+            ks, vs = torch.full((2, n), one), torch.full((2, n), one)
+            if part == 0:
+                ks *= kf
+                vs *= vf
+            elif part == 1:  # one head
+                ks[1] *= kf
+                vs[1] *= vf
+            else:  # one block
+                ks[0, n // 2] *= kf
+                vs[0, n // 2] *= vf
+            check(device, pool, dtype, D, ks, vs, scale, 0.0, 40 + part)
+
+
+@pytest.mark.parametrize("mode", [1, 2, 3])
+@pytest.mark.parametrize("dtype", [BF, HF, F])
+@pytest.mark.parametrize("pool", [E, I])
+def test_prefill_over_every_element_and_any_scales(device, prefill_mode, pool, dtype, mode):
+    """Elements up to the type's largest under powers of two (exact on every path) and under scales that
+    are none (rounded once to the type of the queries on the staged one)."""
+    prefill_mode(mode)
+    n = blocks_of()
+    gen = torch.Generator().manual_seed(7)
+    for D in (128, 64):
+        s = torch.exp2(torch.randint(-9, -6, (2, 2, n), generator=gen).float())
+        check(device, pool, dtype, D, s[0], s[1], 0.02, 0.0, 50)
+        s = s * (1 + torch.rand((2, 2, n), generator=gen))
+        check(device, pool, dtype, D, s[0], s[1], 0.01, u_of(dtype) if mode == 2 else 0.0, 51)
