@@ -157,11 +157,12 @@ class FlourError(RuntimeError):
 
 
 _lib = None
+_switches = ctypes.c_uint(0)
 
 
 def lib() -> ctypes.CDLL:
     """Load libflour_hip.so once; raise if it has not been built."""
-    global _lib
+    global _lib, _switches
     if _lib is not None:
         return _lib
     path = Path(os.environ.get("FLOUR_HIP_LIB", LIB_PATH))
@@ -179,8 +180,17 @@ def lib() -> ctypes.CDLL:
         if fn is not None:
             fn.restype = res
             fn.argtypes = args
+    try:
+        _switches = ctypes.c_uint.in_dll(handle, "flour_hip_switches")
+    except ValueError:
+        pass
     _lib = handle
     return handle
+
+
+def switches() -> int:
+    """How often a switch that workspace sizes go by has been set: a kept size holds until it moves."""
+    return _switches.value
 
 
 # Optional, non-header helpers (test / tuning switches).

@@ -568,5 +568,6 @@ extern "C" int flour_hip_set_prefill_f32_mfma(int mode) {
         return FLOUR_ERR_INVALID_ARGUMENT;
     }
     g_prefill_f32_mfma = mode;
+    switch_set();
     return FLOUR_OK;
 }

@@ -312,6 +312,7 @@ inline int device_cus() {
 // Both are noexcept: the message lives in a fixed per-thread buffer.
 void set_error(const char* fmt, ...) noexcept __attribute__((format(printf, 1, 2)));
 void clear_error() noexcept;
+void switch_set() noexcept;  // a switch that workspace sizes go by (flour_errors.cpp)
 
 // Runs the body of a C entry point so that no C++ exception crosses the C ABI (the caller may
 // be C, ctypes or another language's FFI): a failed host allocation in a container or `new`

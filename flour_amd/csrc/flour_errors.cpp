@@ -1,6 +1,8 @@
-// flour_errors.cpp — per-thread error message and version of libflour_hip.so.
+// flour_errors.cpp — per-thread error message, version and switch count of libflour_hip.so.
 #include <stdarg.h>
 #include <stdio.h>
+
+#include <atomic>
 
 #include "flour_common.h"
 
@@ -25,6 +27,16 @@ int check_hip(hipError_t e, const char* what) {
     return FLOUR_ERR_HIP;
 }
 
+}  // namespace flour
+
+// Counts the settings of switches that workspace sizes go by: a size that a caller has kept holds as long
+// as this has not moved. (Exported for flour_amd; not in the header, as the switches are not.)
+extern "C" {
+std::atomic<unsigned> flour_hip_switches{0};
+}
+
+namespace flour {
+void switch_set() noexcept { flour_hip_switches.fetch_add(1, std::memory_order_relaxed); }
 }  // namespace flour
 
 extern "C" const char* flour_hip_last_error(void) { return flour::g_last_error; }

@@ -1019,6 +1019,7 @@ extern "C" int flour_hip_set_decode_xcd_weight(int w) {
 extern "C" int flour_hip_set_decode_workgroups(int n) {
     if (n < 0 || n > 4096) return FLOUR_ERR_INVALID_ARGUMENT;
     g_wg_override = n;
+    switch_set();
     return FLOUR_OK;
 }
 

@@ -22,7 +22,7 @@ import functools
 import torch
 
 from . import _lib
-from ._lib import check, lib
+from ._lib import check, lib, switches
 
 _DT = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
 
@@ -468,14 +468,34 @@ def kv_dequant(k_pool: torch.Tensor, v_pool: torch.Tensor, k_scale: torch.Tensor
 
 
 @functools.lru_cache(maxsize=1024)
+def _size(query: str, dev: int, set_count: int, *shape: int) -> int:
+    """The library's size query for device dev (-1: the current one, none being in use). A size goes by
+    the shape, the device's CUs and the library's switches (set_count: settings of them so far)."""
+    n = ctypes.c_size_t(0)
+    fn = getattr(lib(), query)
+    if dev < 0 or dev == _current_device():
+        check(fn(*shape, ctypes.byref(n)))
+    else:
+        with torch.cuda.device(dev):
+            check(fn(*shape, ctypes.byref(n)))
+    return n.value
+
+
+def _decode_size(dev: int, batch: int, num_heads: int, kv_heads: int, head_dim: int,
+                 max_context_len: int, with_weights: bool) -> int:
+    return _size("flour_hip_decode_weights_workspace_size", dev, switches(), batch, num_heads,
+                 kv_heads, head_dim, max_context_len, int(with_weights))
+
+
+def _device_in_use() -> int:
+    return torch.cuda.current_device() if torch.cuda.is_initialized() else -1
+
+
 def decode_weights_workspace_bytes(batch: int, num_heads: int, kv_heads: int, head_dim: int,
                                    max_context_len: int, with_weights: bool) -> int:
-    """Bytes of workspace of paged_decode_q8 and paged_decode_weights."""
-    n = ctypes.c_size_t(0)
-    check(lib().flour_hip_decode_weights_workspace_size(batch, num_heads, kv_heads, head_dim,
-                                                        max_context_len, int(with_weights),
-                                                        ctypes.byref(n)))
-    return n.value
+    """Bytes of workspace of paged_decode_q8 and paged_decode_weights on the current device."""
+    return _decode_size(_device_in_use(), batch, num_heads, kv_heads, head_dim, max_context_len,
+                        with_weights)
 
 
 def _scratch(workspace: Workspace | None, nbytes: int, q: torch.Tensor) -> torch.Tensor:
@@ -525,8 +545,7 @@ def paged_decode_q8(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
     width = _table(block_tables, B, "block_tables")
     wargs = _weights_args(weights, weight_rows, G, B, max_context_len)
     out = _decode_out(out, q, out_dtype)
-    ws = _scratch(workspace, decode_weights_workspace_bytes(B, H, G, D, max_context_len,
-                                                            weights is not None), q)
+    ws = _scratch(workspace, _decode_size(dev, B, H, G, D, max_context_len, weights is not None), q)
     _launch(lib().flour_hip_paged_decode_q8, dev, out.data_ptr(), dtype_code(out.dtype),
             q.data_ptr(), dtype_code(q.dtype), k_pool.data_ptr(), v_pool.data_ptr(),
             k_scale.data_ptr(), v_scale.data_ptr(), code, block_tables.data_ptr(), width,
@@ -557,7 +576,7 @@ def paged_decode_weights(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Te
     width = _table(block_tables, B, "block_tables")
     wargs = _weights_args(weights, weight_rows, G, B, max_context_len)
     out = _decode_out(out, q, out_dtype)
-    ws = _scratch(workspace, decode_weights_workspace_bytes(B, H, G, D, max_context_len, True), q)
+    ws = _scratch(workspace, _decode_size(dev, B, H, G, D, max_context_len, True), q)
     _launch(lib().flour_hip_paged_decode_weights, dev, out.data_ptr(), dtype_code(out.dtype),
             q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), block_tables.data_ptr(), width,
             context_lens.data_ptr(), B, H, G, D, block_size, slots, max_context_len, float(scale),
@@ -565,16 +584,16 @@ def paged_decode_weights(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Te
     return out
 
 
-@functools.lru_cache(maxsize=1024)
+def _prefill_size(dev: int, *shape: int) -> int:
+    return _size("flour_hip_varlen_prefill_q8_workspace_size", dev, switches(), *shape)
+
+
 def prefill_q8_workspace_bytes(num_seqs: int, max_seqlen_q: int, total_q: int, max_kv_len: int,
                                num_heads: int, kv_heads: int, head_dim: int, block_size: int,
                                dtype: torch.dtype) -> int:
-    """Bytes of workspace of varlen_prefill_q8."""
-    n = ctypes.c_size_t(0)
-    check(lib().flour_hip_varlen_prefill_q8_workspace_size(
-        num_seqs, max_seqlen_q, total_q, max_kv_len, num_heads, kv_heads, head_dim, block_size,
-        dtype_code(dtype), ctypes.byref(n)))
-    return n.value
+    """Bytes of workspace of varlen_prefill_q8 on the current device."""
+    return _prefill_size(_device_in_use(), num_seqs, max_seqlen_q, total_q, max_kv_len, num_heads,
+                         kv_heads, head_dim, block_size, dtype_code(dtype))
 
 
 def varlen_prefill_q8(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
@@ -602,8 +621,8 @@ def varlen_prefill_q8(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tenso
     out_strides = out.stride()
     if out_strides[2] != 1:
         raise _invalid("out must have a unit last stride")
-    ws = _scratch(workspace, prefill_q8_workspace_bytes(n, max_seqlen_q, T, max_kv_len, H, G, D,
-                                                        block_size, q.dtype), q)
+    ws = _scratch(workspace, _prefill_size(dev, n, max_seqlen_q, T, max_kv_len, H, G, D, block_size,
+                                           dtype_code(q.dtype)), q)
     _launch(lib().flour_hip_varlen_prefill_q8, dev, out.data_ptr(), dtype_code(out.dtype),
             out_strides[0], out_strides[1], q.data_ptr(), strides[0], strides[1],
             dtype_code(q.dtype), k_pool.data_ptr(), v_pool.data_ptr(), k_scale.data_ptr(),
