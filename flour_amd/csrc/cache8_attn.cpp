@@ -277,11 +277,12 @@ static int prefill_staged(const PoolAttn& a, const Stage& st, int max_rows, char
                                    a.kv_lens + s0, n, a.max_kv, a.kv_heads, a.head_dim, a.block_size,
                                    a.num_slots, table, lens, stream);
         if (rc != FLOUR_OK) return rc;
-        // (the matrix-core kernels take a sequence's rows from cu[s], cu[s + 1] alone; total_q is a
-        // bound and guides their choice)
+        // (the matrix-core kernels take a sequence's rows from cu[s], cu[s + 1] alone; total_q only guides
+        // their choice: the slice's share of the rows, which the host knows in all alone)
+        const int rows = (int)std::max<int64_t>(1, (int64_t)a.rows * n / a.batch);
         rc = varlen_prefill_rows(a.out, a.out_dtype, a.o_st, a.o_sh, a.q, a.q_st, a.q_sh, k, v,
                                  a.cu + s0, nullptr, lens, table, st.blocks, n, max_rows,
-                                 a.rows, a.num_heads, a.kv_heads, a.head_dim, a.block_size,
+                                 rows, a.num_heads, a.kv_heads, a.head_dim, a.block_size,
                                  st.slots, a.scale, a.dtype, v_stage, st.v_stage, a.max_kv, stream);
         if (rc != FLOUR_OK) return rc;
     }

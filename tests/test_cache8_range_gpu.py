@@ -1,5 +1,5 @@
-"""8-bit prefill over the whole range of scales and elements, on each of its paths: what a cache gives
-does not depend on which one the shape of the batch selects."""
+"""8-bit prefill over the whole range of scales and elements, on each of its paths (what a cache gives does
+not depend on which one the shape of the batch selects), and in slices."""
 from __future__ import annotations
 
 import numpy as np
@@ -118,3 +118,26 @@ def test_prefill_over_every_element_and_any_scales(device, prefill_mode, pool, d
         check(device, pool, dtype, D, s[0], s[1], 0.02, 0.0, 50)
         s = s * (1 + torch.rand((2, 2, n), generator=gen))
         check(device, pool, dtype, D, s[0], s[1], 0.01, u_of(dtype) if mode == 2 else 0.0, 51)
+
+
+def test_slices_choose_their_kernel_by_their_own_rows(device, prefill_mode):
+    """Six prompts whose bound of 2^20 positions allows four in a staged copy: the bits of the same prompts
+    in calls of four and of two, which run on the kernels for 6,000 and 3,000 rows (9,000 in one call
+    would run on another)."""
+    H, G, D, bs, n, most = 4, 1, 64, 16, 1500, 1 << 20
+    gen = torch.Generator().manual_seed(13)
+    nb = (n + bs - 1) // bs
+    kp, vp = (full_pool(G, 6 * nb, bs, D, E, gen, device) for _ in "kv")
+    s = torch.full((G, 6 * nb), 2.0 ** -9, device=device)
+    tab = torch.full((6, most // bs), -1, dtype=torch.int32)
+    tab[:, :nb] = torch.randperm(6 * nb, generator=gen).to(torch.int32).view(6, nb)
+    tab = tab.to(device)
+    q = torch.randn((6 * n, H, D), generator=gen).to(HF).to(device)
+    prefill_mode(2)
+
+    def call(a, b):
+        cu = i32([n * i for i in range(b - a + 1)], device)
+        return ops.varlen_prefill_q8(q[n * a:n * b], kp, vp, s, s, cu, i32([n] * (b - a), device),
+                                     tab[a:b], n, most, 0.05, bs, out_dtype=F)
+
+    assert torch.equal(call(0, 6), torch.cat([call(0, 4), call(4, 6)]))
