@@ -12,13 +12,21 @@ static size_t up256(size_t x) { return (x + 255) & ~(size_t)255; }
 static int64_t score_stride_of(int max_ctx) { return ((int64_t)max_ctx + 63) / 64 * 64; }
 
 // ---- the streamed kernel
+// What the shape says of it; a call's tensors can still refuse it (stream_takes).
+static bool stream_fits(int batch, int rows, int max_rows, int n_rep, int max_kv, int head_dim,
+                        int block_size) {
+    // (chunks of 32 positions, or more, of groups of 16 columns, or more: counted in 32 bits)
+    const double chunks =
+        (double)batch * (max_kv / 32 + 1.0) * ((double)max_rows * n_rep / 16 + 1.0);
+    return (head_dim == 64 || head_dim == 128) && chunks < 2e9 && block_size % 16 == 0 &&
+           batch <= 4096 && rows <= 65535;
+}
+
 static bool stream_takes(const PoolAttn& a, int max_rows) {
     const int es = elem_bytes(a.dtype), oes = elem_bytes(a.out_dtype);
-    // (chunks of 32 positions, or more, of groups of 16 columns, or more: counted in 32 bits)
-    const double chunks = (double)a.batch * (a.max_kv / 32 + 1.0) *
-                          ((double)max_rows * (a.num_heads / a.kv_heads) / 16 + 1.0);
-    return valid_pool8(a.pool_dtype) && (a.head_dim == 64 || a.head_dim == 128) && chunks < 2e9 &&
-           a.block_size % 16 == 0 && a.batch <= 4096 && a.rows <= 65535 &&
+    return valid_pool8(a.pool_dtype) &&
+           stream_fits(a.batch, a.rows, max_rows, a.num_heads / a.kv_heads, a.max_kv, a.head_dim,
+                       a.block_size) &&
            a.num_slots * a.head_dim <= (int64_t)0x7fffffff &&
            (((uint64_t)(uintptr_t)a.q | (uint64_t)(uintptr_t)a.out | (uint64_t)(uintptr_t)a.k_pool |
              (uint64_t)(uintptr_t)a.v_pool | (uint64_t)(a.q_st * es) | (uint64_t)(a.q_sh * es) |
@@ -211,8 +219,11 @@ struct Stage {
     size_t table, lens, v_stage, total;
 };
 
-static bool stage_of(int num_seqs, int max_seqlen_q, int max_kv, int kv_heads, int head_dim,
-                     int block_size, int dtype, Stage* st) {
+// The staged copy of a call within `limit` bytes: slices of as many sequences as STAGE_BYTES and the limit
+// allow, and the prefill kernel's own copy of V where it wants one; false where none fits or no such
+// kernel takes the shape.
+static bool stage_of(int num_seqs, int max_seqlen_q, int total_q, int max_kv, int kv_heads,
+                     int head_dim, int block_size, int dtype, size_t limit, Stage* st) {
     if (num_seqs <= 0 || max_kv <= 0 || (head_dim != 64 && head_dim != 128)) return false;
     st->blocks = (max_kv + block_size - 1) / block_size;
     const size_t seq = (size_t)st->blocks * block_size * head_dim * elem_bytes(dtype);  // of a head
@@ -220,21 +231,30 @@ static bool stage_of(int num_seqs, int max_seqlen_q, int max_kv, int kv_heads, i
     // (a head's part of the pool stays below 2^31 bytes: the kernels' limit)
     const size_t fit = std::min<size_t>(STAGE_BYTES / (2 * seq * kv_heads), 0x7fffffff / seq);
     st->slice = (int)std::min<size_t>(std::max<size_t>(fit, 1), num_seqs);
+    bool copy_v = prefill_wants_v_stage(num_seqs, total_q);
+    for (;;) {
+        size_t v = 0;
+        if (copy_v &&
+            flour_hip_varlen_prefill_workspace_size(st->slice, st->blocks, block_size, kv_heads,
+                                                    head_dim, dtype, &v) != FLOUR_OK)
+            return false;
+        st->pool = up256(seq * st->slice * kv_heads);
+        st->table = up256((size_t)st->slice * st->blocks * sizeof(int32_t));
+        st->lens = up256((size_t)st->slice * sizeof(int32_t));
+        st->v_stage = up256(v);
+        st->total = 2 * st->pool + st->table + st->lens + st->v_stage;
+        if (st->total <= limit) break;
+        if (st->slice > 1)
+            st->slice = std::max(1, std::min(st->slice - 1, (int)((double)st->slice * limit / st->total)));
+        else if (copy_v)
+            copy_v = false;
+        else
+            return false;
+    }
     st->slots = (int64_t)st->slice * st->blocks * block_size;
     const bool mfma = prefill_mfma_supported(dtype, head_dim, block_size, st->slots, 1.0f, 0);
-    if (!mfma && !prefill_f32_mfma_supported(dtype, head_dim, st->slice, max_seqlen_q, block_size,
-                                             st->slots))
-        return false;
-    st->pool = up256(seq * st->slice * kv_heads);
-    st->table = up256((size_t)st->slice * st->blocks * sizeof(int32_t));
-    st->lens = up256((size_t)st->slice * sizeof(int32_t));
-    size_t v = 0;
-    if (flour_hip_varlen_prefill_workspace_size(st->slice, st->blocks, block_size, kv_heads, head_dim,
-                                                dtype, &v) != FLOUR_OK)
-        return false;
-    st->v_stage = up256(v);
-    st->total = 2 * st->pool + st->table + st->lens + st->v_stage;
-    return true;
+    return mfma || prefill_f32_mfma_supported(dtype, head_dim, st->slice, max_seqlen_q, block_size,
+                                              st->slots);
 }
 
 // Whether a call runs streamed rather than staged: estimates of both in us, from the bounds that the host
@@ -248,17 +268,19 @@ static bool stage_of(int num_seqs, int max_seqlen_q, int max_kv, int kv_heads, i
 // 4,096 with 8 39 / 132 and with 128 268 / 159, 32 x 512 with 32 76 / 45; fp32 32 x 2,048 with 32 185 /
 // 637; 14 / 2 heads of 64 8 x 1,024 with 64 41 / 26. Of 390 such calls five are more than 10% slower than
 // on the other path (15%, one 33%).
-static bool prefer_stream(const PoolAttn& a, int max_rows) {
-    const bool f32 = a.dtype == FLOUR_DTYPE_F32, d64 = a.head_dim == 64;
-    const double units = (double)a.batch * a.kv_heads * a.max_kv;
-    const int64_t cols = (int64_t)max_rows * (a.num_heads / a.kv_heads);
+static bool prefer_stream(int batch, int max_rows, int max_kv, int num_heads, int kv_heads,
+                          int head_dim, int dtype) {
+    const bool f32 = dtype == FLOUR_DTYPE_F32, d64 = head_dim == 64;
+    const double units = (double)batch * kv_heads * max_kv;
+    const int64_t cols = (int64_t)max_rows * (num_heads / kv_heads);
     const double groups = (double)((cols + 31) / 32);
     const double streamed = 10 + units * groups * (d64 ? 6.1e-5 : f32 ? 9.4e-5 : 7.8e-5) +
                             std::min(2 * groups, 14.0);
-    const double walk = a.max_kv * (f32 ? (d64 ? 0.024 : 0.055) : (d64 ? 0.0135 : 0.024));
+    const double walk = max_kv * (f32 ? (d64 ? 0.024 : 0.055) : (d64 ? 0.0135 : 0.024));
     const double rows = f32 ? (max_rows + 31) / 32 * 32.0 : max_rows;
-    const double flops = 4.0 * a.batch * rows * a.max_kv * a.num_heads * a.head_dim;
-    const double staged = (a.dtype == FLOUR_DTYPE_F16 ? 13 : 10) + units * a.head_dim * 2 * (1 + elem_bytes(a.dtype)) / 5e6 +
+    const double flops = 4.0 * batch * rows * max_kv * num_heads * head_dim;
+    const double staged = (dtype == FLOUR_DTYPE_F16 ? 13 : 10) +
+                          units * head_dim * 2 * (1 + elem_bytes(dtype)) / 5e6 +
                           std::max(walk, flops / (f32 ? 7e7 : 6.5e8));
     return streamed < staged;
 }
@@ -309,6 +331,7 @@ extern "C" int flour_hip_set_prefill_q8(int mode) {
         return FLOUR_ERR_INVALID_ARGUMENT;
     }
     flour::g_prefill_q8 = mode;
+    flour::switch_set();
     return FLOUR_OK;
 }
 
@@ -324,11 +347,18 @@ extern "C" int flour_hip_varlen_prefill_q8_workspace_size(int num_seqs, int max_
         set_error("varlen_prefill_q8_workspace_size: bad arguments");
         return FLOUR_ERR_INVALID_ARGUMENT;
     }
+    const int n_rep = num_heads / kv_heads, mode = g_prefill_q8;
+    const bool streamed = mode != 3 && stream_fits(num_seqs, total_q, max_seqlen_q, n_rep, max_kv_len,
+                                                   head_dim, block_size);
+    const bool preferred =
+        streamed && (mode == 1 || (mode == 0 && prefer_stream(num_seqs, max_seqlen_q, max_kv_len,
+                                                              num_heads, kv_heads, head_dim, dtype)));
+    *bytes = streamed ? stream_bytes(num_seqs, (int64_t)max_seqlen_q * n_rep, head_dim) : 0;
     Stage st{};
-    const size_t staged =
-        stage_of(num_seqs, max_seqlen_q, max_kv_len, kv_heads, head_dim, block_size, dtype, &st)
-            ? st.total : 0;
-    *bytes = std::max(staged, stream_bytes(num_seqs, (int64_t)max_seqlen_q * (num_heads / kv_heads), head_dim));
+    if (mode != 3 && !preferred &&
+        stage_of(num_seqs, max_seqlen_q, total_q, max_kv_len, kv_heads, head_dim, block_size, dtype,
+                 SIZE_MAX, &st))
+        *bytes = std::max(*bytes, st.total);
     return FLOUR_OK;
 }
 
@@ -370,12 +400,13 @@ extern "C" int flour_hip_varlen_prefill_q8(
     a.block_tables = block_tables, a.max_blocks = max_blocks_per_seq, a.batch = num_seqs;
     a.rows = total_q, a.num_heads = num_heads, a.kv_heads = kv_heads, a.head_dim = head_dim;
     a.block_size = block_size, a.num_slots = num_slots, a.max_kv = max_kv_len, a.scale = scale;
-    size_t need = 0;
-    if (flour_hip_varlen_prefill_q8_workspace_size(num_seqs, max_seqlen_q, total_q, max_kv_len,
-                                                   num_heads, kv_heads, head_dim, block_size, dtype,
-                                                   &need) != FLOUR_OK)
-        return FLOUR_ERR_INVALID_ARGUMENT;
-    if (need > 0 && (!workspace || workspace_bytes < need || (uintptr_t)workspace % 256 != 0)) {
+    const int n_rep = num_heads / kv_heads, mode = g_prefill_q8;
+    const bool fits = mode != 3 && stream_fits(num_seqs, total_q, max_seqlen_q, n_rep, max_kv_len,
+                                               head_dim, block_size);
+    // (a staged copy takes what there is beyond that: workspaces of other shapes serve)
+    const size_t need = fits ? stream_bytes(num_seqs, (int64_t)max_seqlen_q * n_rep, head_dim) : 0;
+    if ((workspace && (uintptr_t)workspace % 256 != 0) || workspace_bytes < need ||
+        (!workspace && need > 0)) {
         set_error("varlen_prefill_q8: workspace of %zu bytes (256-byte aligned) required, got %zu at "
                   "%p",
                   need, workspace_bytes, workspace);
@@ -383,14 +414,15 @@ extern "C" int flour_hip_varlen_prefill_q8(
     }
     hipStream_t s = static_cast<hipStream_t>(stream);
     Stage st{};
-    const int mode = g_prefill_q8;
-    const bool staged = mode != 3 &&
-                        stage_of(num_seqs, max_seqlen_q, max_kv_len, kv_heads, head_dim, block_size,
-                                 dtype, &st) &&
-                        stage_takes(a, st, max_seqlen_q);
-    const bool streamed = mode != 3 && stream_takes(a, max_seqlen_q);
-    if (streamed && (mode == 1 || !staged || (mode == 0 && prefer_stream(a, max_seqlen_q))))
+    const bool streamed = fits && stream_takes(a, max_seqlen_q);
+    if (streamed && (mode == 1 || (mode == 0 && prefer_stream(num_seqs, max_seqlen_q, max_kv_len,
+                                                              num_heads, kv_heads, head_dim, dtype))))
         return launch_stream_call(a, max_seqlen_q, workspace, s);
-    if (staged) return prefill_staged(a, st, max_seqlen_q, static_cast<char*>(workspace), s);
+    if (mode != 3 &&
+        stage_of(num_seqs, max_seqlen_q, total_q, max_kv_len, kv_heads, head_dim, block_size, dtype,
+                 workspace ? workspace_bytes : 0, &st) &&
+        stage_takes(a, st, max_seqlen_q))
+        return prefill_staged(a, st, max_seqlen_q, static_cast<char*>(workspace), s);
+    if (streamed) return launch_stream_call(a, max_seqlen_q, workspace, s);
     return launch_attn_pools(a, s);
 }

@@ -353,6 +353,8 @@ bool decode_mfma_supported(int dtype, int head_dim, int block_size, int n_rep, i
                            const void* v_pool);
 bool prefill_mfma_supported(int dtype, int head_dim, int block_size, int64_t num_slots,
                             float scale, int64_t q_stride_tok);
+// Whether a prefill at head_dim 128 with a workspace for it copies V there first.
+bool prefill_wants_v_stage(int num_seqs, int64_t total_q);
 int paged_decode_rows(void* out, int out_dtype, const void* q, const void* k_pool,
                       const void* v_pool, const int32_t* block_tables, int max_blocks_per_seq,
                       const int32_t* context_lens, const int32_t* rows, int batch, int num_heads,

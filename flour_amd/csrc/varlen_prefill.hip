@@ -1603,6 +1603,11 @@ static int64_t prefill_stage_bytes(int64_t num_seqs, int64_t max_blocks, int64_t
     return bytes <= PF_STAGE_MAX_BYTES ? bytes : 0;
 }
 
+bool prefill_wants_v_stage(int num_seqs, int64_t total_q) {
+    return g_prefill_dma == 2 ||
+           (g_prefill_dma == 1 && total_q >= (int64_t)PF_DMA_MIN_MEAN_Q * num_seqs);
+}
+
 template <typename T, typename TO, int PV, int D>
 static int launch_prefill_mfma(void* out, int64_t o_st, int64_t o_sh, const void* q,
                                int64_t q_st, int64_t q_sh, const void* k_pool, const void* v_pool,
@@ -1628,9 +1633,7 @@ static int launch_prefill_mfma(void* out, int64_t o_st, int64_t o_sh, const void
         const int kv_heads = num_heads / n_rep;
         const int64_t pages_per_seq = 4 * (((int64_t)max_blocks * block_size + PF_KT - 1) / PF_KT);
         const int64_t need = prefill_stage_bytes(num_seqs, max_blocks, block_size, kv_heads);
-        const bool want = g_prefill_dma == 2 ||
-                          (g_prefill_dma == 1 && total_q >= (int64_t)PF_DMA_MIN_MEAN_Q * num_seqs);
-        if (want && persistent && ws != nullptr && need > 0 && (int64_t)ws_size >= need) {
+        if (prefill_wants_v_stage(num_seqs, total_q) && persistent && ws != nullptr && need > 0 && (int64_t)ws_size >= need) {
             prefill_v_stage_kernel<T><<<dim3((unsigned)(num_seqs * pages_per_seq / 4),
                                              (unsigned)kv_heads),
                                         dim3(256), 0, stream>>>(
@@ -1679,6 +1682,7 @@ extern "C" int flour_hip_set_prefill_dma(int mode) {
         return FLOUR_ERR_INVALID_ARGUMENT;
     }
     g_prefill_dma = mode;
+    switch_set();
     return FLOUR_OK;
 }
 

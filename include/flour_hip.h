@@ -317,8 +317,8 @@ int flour_hip_decode_weights_workspace_size(int batch, int num_heads, int kv_hea
  * as long) and with 16-bit queries each probability once to f16. max_kv_len bounds kv_lens (a
  * longer sequence is taken to end there); rows behind the last sequence's, where total_q is larger
  * than cu_seqlens_q[num_seqs], leave out as it was. A workspace of
- * flour_hip_varlen_prefill_q8_workspace_size bytes (256-byte aligned, no initialisation needed)
- * is required; calls that share one must not overlap in time. */
+ * flour_hip_varlen_prefill_q8_workspace_size bytes (256-byte aligned, no initialisation needed) goes with
+ * the call (FLOUR_ERR_WORKSPACE where it is too small for any kernel); calls that share one must not overlap in time. */
 int flour_hip_varlen_prefill_q8(void* out, int out_dtype, int64_t o_stride_tok,
                                 int64_t o_stride_head, const void* q, int64_t q_stride_tok,
                                 int64_t q_stride_head, int dtype, const void* k_pool,
@@ -330,6 +330,10 @@ int flour_hip_varlen_prefill_q8(void* out, int out_dtype, int64_t o_stride_tok,
                                 int block_size, int64_t num_slots, int max_kv_len, float scale,
                                 void* workspace, size_t workspace_bytes, void* stream);
 
+/* What the kernels take that the shape selects. Few rows read the 8-bit cache as it is, in tens of MB. More
+ * have a copy of the sequences in `dtype`, up to 1 GiB or one sequence, and for long prompts another of
+ * V. A call with less than that for its copy makes it in parts, or does without, and takes longer; so does
+ * one whose pool holds 2^31 bytes or more of a kv head with the size for few rows. */
 int flour_hip_varlen_prefill_q8_workspace_size(int num_seqs, int max_seqlen_q, int total_q,
                                                int max_kv_len, int num_heads, int kv_heads,
                                                int head_dim, int block_size, int dtype,

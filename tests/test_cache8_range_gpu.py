@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from _cache8 import Cache, attend, close
-from flour_amd import ops
+from flour_amd import _lib, ops
 from flour_amd._lib import lib
 
 pytestmark = pytest.mark.gpu
@@ -140,4 +140,55 @@ def test_slices_choose_their_kernel_by_their_own_rows(device, prefill_mode):
         return ops.varlen_prefill_q8(q[n * a:n * b], kp, vp, s, s, cu, i32([n] * (b - a), device),
                                      tab[a:b], n, most, 0.05, bs, out_dtype=F)
 
+    def call_with(nbytes):  # of workspace
+        ws = torch.full((nbytes,), 255, dtype=torch.uint8, device=device)
+        out = torch.empty((6 * n, H, D), dtype=F, device=device)
+        cu, lens = i32([n * i for i in range(7)], device), i32([n] * 6, device)
+        _lib.check(lib().flour_hip_varlen_prefill_q8(
+            out.data_ptr(), _lib.F32, H * D, D, q.data_ptr(), H * D, D, _lib.F16, kp.data_ptr(),
+            vp.data_ptr(), s.data_ptr(), s.data_ptr(), _lib.E4M3, cu.data_ptr(), lens.data_ptr(),
+            tab.data_ptr(), most // bs, 6, n, 6 * n, H, G, D, bs, kp.shape[1], most, 0.05,
+            ws.data_ptr(), nbytes, torch.cuda.current_stream().cuda_stream))
+        return out
+
     assert torch.equal(call(0, 6), torch.cat([call(0, 4), call(4, 6)]))
+    # a copy of one sequence takes 256 MiB and its table: parts of as many as the workspace holds
+    one = (1 << 28) + (1 << 20)
+    assert torch.equal(call_with(3 * one), torch.cat([call(0, 3), call(3, 6)]))
+    assert torch.equal(call_with(one), torch.cat([call(i, i + 1) for i in range(6)]))
+
+
+def test_few_rows_over_a_pool_of_2_31_bytes_a_head(device):
+    """Such a pool is staged where its shape would be streamed: within the streamed kernel's workspace, one
+    sequence of up to 65,536 positions (16 MiB of K, as much of V) at a time."""
+    H, G, D, bs, most = 4, 1, 128, 16, 1 << 16
+    blocks = (1 << 31) // (bs * D) + 40
+    kp = torch.zeros((G, blocks * bs, D), dtype=I, device=device)
+    s = torch.full((G, blocks), 2.0 ** -7, device=device)
+    gen = torch.Generator().manual_seed(14)
+    lens, rows = [600, 33, 100], [8, 3, 8]
+    nb = [(n + bs - 1) // bs for n in lens]
+    tab = torch.full((3, most // bs), -1, dtype=torch.int32)
+    small = full_pool(G, sum(nb), bs, D, I, gen, device)
+    where = [blocks - 1 - 7 * i for i in range(5)] + list(range(3, sum(nb) - 2))
+    at = 0
+    for x, n in enumerate(nb):
+        tab[x, :n] = torch.tensor(where[at:at + n])
+        at += n
+    for i, b in enumerate(where):
+        kp[:, b * bs:(b + 1) * bs] = small[:, i * bs:(i + 1) * bs]
+    q = torch.randn((sum(rows), H, D), generator=gen).to(BF).to(device)
+    cu = [0, 8, 11, 19]
+    size = ops.prefill_q8_workspace_bytes(3, 8, 19, most, H, G, D, bs, BF)
+    assert size < 3 * 2 * most * D * 2  # not all three at once
+    ws = ops.Workspace(device)
+    ws.get(size).fill_(255)
+    got = ops.varlen_prefill_q8(q, kp, kp, s, s, i32(cu, device), i32(lens, device), tab.to(device), 8,
+                                most, 0.03, bs, out_dtype=F, workspace=ws)
+    c = Cache(small, torch.full((G, sum(nb)), 2.0 ** -7), bs)
+    at = 0
+    for x in range(3):
+        v = c.rows(list(range(at, at + nb[x])), lens[x])
+        at += nb[x]
+        want, _, err = attend(q[cu[x]:cu[x + 1]].cpu().double().numpy(), v, v, 0.03)
+        close(got[cu[x]:cu[x + 1]], want, (2 * err[:, :, None] + 2.0 ** -11) * np.abs(v).max())
