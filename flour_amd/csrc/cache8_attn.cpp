@@ -258,30 +258,34 @@ static bool stage_of(int num_seqs, int max_seqlen_q, int total_q, int max_kv, in
 }
 
 // Whether a call runs streamed rather than staged: estimates of both in us, from the bounds that the host
-// knows.
+// knows (total_q rows in all, max_kv positions of each sequence).
 //  * Streamed: 10, the cache once per group of 32 columns, 7.8e-5 us a position and kv head at head_dim 128
-//    (9.4e-5 with fp32 queries), 6.1e-5 at 64, and up to 14 for the pieces of the groups.
-//  * Staged: 10, 3 with f16 queries (attn_beyond_f16_kernel), the copy at 5 TB/s, and the prefill kernel: at least one item's walk over the kv
-//    positions (24 ns each at head_dim 128, 13.5 at 64; fp32 55 and 24), or its products at 650 TFLOP/s
-//    (fp32 70, rows in tiles of 32).
+//    (9.4e-5 with fp32 queries), 6.1e-5 at 64, and up to 14 for the pieces of the groups. Positions that a
+//    group does not see are read all the same.
+//  * Staged: 11 (16 in fp32; 18 in f16, whose scales are looked at again, attn_beyond_f16_kernel), the copy at
+//    5 TB/s, and the prefill kernel: at least one item's walk over the kv positions (24 ns each at
+//    head_dim 128, 13.5 at 64; fp32 55 and 24), or the products of the causal range at 650 TFLOP/s (fp32
+//    110, rows in tiles of 32).
 // Measured, streamed / staged, 32 / 8 heads of 128 in bf16: 1 x 4,096 tokens with 32 rows 35 / 109, 8 x
 // 4,096 with 8 39 / 132 and with 128 268 / 159, 32 x 512 with 32 76 / 45; fp32 32 x 2,048 with 32 185 /
-// 637; 14 / 2 heads of 64 8 x 1,024 with 64 41 / 26. Of 390 such calls five are more than 10% slower than
-// on the other path (15%, one 33%).
-static bool prefer_stream(int batch, int max_rows, int max_kv, int num_heads, int kv_heads,
+// 637; 14 / 2 heads of 64 8 x 1,024 with 64 41 / 26. Of 1,500 drawn calls, cold prompts among them, 58 are
+// more than 10% slower than on the other path, 1.7 times the most; in the mean it is 1.7%.
+static bool prefer_stream(int batch, int total_q, int max_rows, int max_kv, int num_heads, int kv_heads,
                           int head_dim, int dtype) {
     const bool f32 = dtype == FLOUR_DTYPE_F32, d64 = head_dim == 64;
-    const double units = (double)batch * kv_heads * max_kv;
-    const int64_t cols = (int64_t)max_rows * (num_heads / kv_heads);
-    const double groups = (double)((cols + 31) / 32);
-    const double streamed = 10 + units * groups * (d64 ? 6.1e-5 : f32 ? 9.4e-5 : 7.8e-5) +
-                            std::min(2 * groups, 14.0);
+    const int n_rep = num_heads / kv_heads;
+    const double seqs = batch, rows = std::min((double)total_q, seqs * max_rows);
+    const double groups = std::max(rows * n_rep / 32 + 0.5 * seqs, seqs);
+    const double pieces = (double)(((int64_t)max_rows * n_rep + 31) / 32);
+    const double streamed =
+        10 + groups * kv_heads * max_kv * (d64 ? 6.1e-5 : f32 ? 9.4e-5 : 7.8e-5) +
+        std::min(2 * pieces, 14.0);
     const double walk = max_kv * (f32 ? (d64 ? 0.024 : 0.055) : (d64 ? 0.0135 : 0.024));
-    const double rows = f32 ? (max_rows + 31) / 32 * 32.0 : max_rows;
-    const double flops = 4.0 * batch * rows * max_kv * num_heads * head_dim;
-    const double staged = (dtype == FLOUR_DTYPE_F16 ? 13 : 10) +
-                          units * head_dim * 2 * (1 + elem_bytes(dtype)) / 5e6 +
-                          std::max(walk, flops / (f32 ? 7e7 : 6.5e8));
+    const double seen = std::max(max_kv - rows / seqs / 2, 0.0);  // by a row, in the mean
+    const double flops = 4.0 * (rows + (f32 ? 16 * seqs : 0)) * seen * num_heads * head_dim;
+    const double copy = seqs * kv_heads * max_kv * head_dim * 2 * (1 + elem_bytes(dtype)) / 5e6;
+    const double staged = (f32 ? 16 : dtype == FLOUR_DTYPE_F16 ? 18 : 11) + copy +
+                          std::max(walk, flops / (f32 ? 1.1e8 : 6.5e8));
     return streamed < staged;
 }
 
@@ -351,7 +355,7 @@ extern "C" int flour_hip_varlen_prefill_q8_workspace_size(int num_seqs, int max_
     const bool streamed = mode != 3 && stream_fits(num_seqs, total_q, max_seqlen_q, n_rep, max_kv_len,
                                                    head_dim, block_size);
     const bool preferred =
-        streamed && (mode == 1 || (mode == 0 && prefer_stream(num_seqs, max_seqlen_q, max_kv_len,
+        streamed && (mode == 1 || (mode == 0 && prefer_stream(num_seqs, total_q, max_seqlen_q, max_kv_len,
                                                               num_heads, kv_heads, head_dim, dtype)));
     *bytes = streamed ? stream_bytes(num_seqs, (int64_t)max_seqlen_q * n_rep, head_dim) : 0;
     Stage st{};
@@ -415,7 +419,7 @@ extern "C" int flour_hip_varlen_prefill_q8(
     hipStream_t s = static_cast<hipStream_t>(stream);
     Stage st{};
     const bool streamed = fits && stream_takes(a, max_seqlen_q);
-    if (streamed && (mode == 1 || (mode == 0 && prefer_stream(num_seqs, max_seqlen_q, max_kv_len,
+    if (streamed && (mode == 1 || (mode == 0 && prefer_stream(num_seqs, total_q, max_seqlen_q, max_kv_len,
                                                               num_heads, kv_heads, head_dim, dtype))))
         return launch_stream_call(a, max_seqlen_q, workspace, s);
     if (mode != 3 &&

@@ -94,3 +94,13 @@ def test_a_smaller_workspace_is_refused():
     for ws, size in ((None, 1 << 30), (4096, n - 1), (4096 + 128, 1 << 30)):
         rc = _lib.lib().flour_hip_varlen_prefill_q8(*args, ws, size, None)
         assert rc == _lib.ERR_WORKSPACE and "workspace" in _lib.last_error()
+
+
+def test_cold_prompts_are_staged():
+    """A prompt without cached positions has half the products of its rows times its positions (fp32 ones
+    were taken for streamed, at up to twice the time)."""
+    for seqs, rows, H, G, D in ((10, 1185, 8, 8, 64), (4, 2048, 32, 8, 128), (64, 506, 14, 2, 64)):
+        n = prefill_size(seqs, rows, seqs * rows, rows, H=H, G=G, D=D, dtype=F)
+        assert n >= 2 * seqs * rows * G * D * 4, (seqs, rows)
+    # few rows behind as many positions: as before
+    assert prefill_size(10, 16, 160, 1185, H=8, G=8, D=64, dtype=F) < 2 * 10 * 1185 * 8 * 64 * 4
