@@ -192,3 +192,79 @@ def test_few_rows_over_a_pool_of_2_31_bytes_a_head(device):
         at += nb[x]
         want, _, err = attend(q[cu[x]:cu[x + 1]].cpu().double().numpy(), v, v, 0.03)
         close(got[cu[x]:cu[x + 1]], want, (2 * err[:, :, None] + 2.0 ** -11) * np.abs(v).max())
+
+
+def decode_against_64_bits(q, kp, vp, ks, vs, tab, lens, scale, bs, weights=False):
+    """A decode step within the bounds of fp32 arithmetic relative to the sum of |weight v|, and its
+    weights."""
+    device = q.device
+    B, H, D = q.shape
+    G = kp.shape[0]
+    w = torch.zeros((B, G, max(lens)), device=device) if weights else None
+    got = ops.paged_decode_q8(q, kp, vp, ks, vs, i32(tab, device), i32(lens, device), scale, max(lens),
+                              bs, out_dtype=F, weights=w)
+    ck, cv = Cache(kp, ks, bs), Cache(vp, vs, bs)
+    for b, n in enumerate(lens):
+        k, v = ck.rows(tab[b], n), cv.rows(tab[b], n)
+        want, p, err = attend(q[b:b + 1].cpu().double().numpy(), k, v, scale)
+        av = np.abs(np.repeat(v, H // G, 1))  # (n, H, D)
+        bound = 2 * err[0][:, None] * np.einsum("hj,jhd->hd", p[0], av)
+        # probabilities as two f16 parts (2^-22) of the largest contribution to the head's row
+        bound += 2.0 ** -21 * (p[0].T[:, :, None] * av).max((0, 2))[:, None]
+        close(got[b:b + 1], want, bound[None])
+        if weights:
+            pg = p[0].reshape(G, H // G, n)
+            close(w[b, :, :n], pg.sum(1), (2 * err[0].reshape(G, -1, 1) * pg).sum(1) + 2.0 ** -40)
+
+
+@pytest.mark.parametrize("lens", [[48], [1500, 300]])
+@pytest.mark.parametrize("dtype", [BF, HF, F])
+@pytest.mark.parametrize("D", [128, 64])
+@pytest.mark.parametrize("pool", [E, I])
+def test_decode_over_v_scales_2_100_apart_that_all_count(device, pool, D, dtype, lens):
+    """Blocks under V scales of 2^50, 1 and 2^-50, with weights that make up for them: each contributes
+    about as much. One sequence is finished inside a wave's range, the others are merged from pieces."""
+    H, G, bs = 4, 2, 16
+    gen = torch.Generator().manual_seed(21)
+    nb = [(n + bs - 1) // bs for n in lens]
+    tab, at = [], 0
+    for x in nb:
+        tab.append(list(range(at, at + x)) + [0] * (max(nb) - x))
+        at += x
+    blocks = sum(nb)
+    kind = torch.arange(blocks) % 3  # 0: 2^50, 1: 1, 2: 2^-50
+    vs = torch.exp2(50.0 * (1 - kind)).repeat(G, 1).to(device)
+    vp = full_pool(G, blocks, bs, D, pool, gen, device)
+    # keys along one direction: the scores of the kinds are -50, 0 and 50 times ln 2 and some noise
+    sign = torch.randint(0, 2, (G, 1, D), generator=gen) * 2 - 1
+    noise = torch.randint(-2, 3, (G, blocks * bs, D), generator=gen)
+    k = (sign * (32 * (kind - 1)).repeat_interleave(bs)[:, None] + noise).float()
+    kp = k.to(E).to(device) if pool == E else k.to(I).to(device)
+    ks = torch.full((G, blocks), 2.0 ** -5, device=device)
+    q = sign.view(G, 1, D).repeat(1, H // G, 1).reshape(1, H, D).repeat(len(lens), 1, 1)
+    q = q.to(dtype).to(device)
+    decode_against_64_bits(q, kp, vp, ks, vs, tab, lens, 50 * np.log(2) / D, bs)
+
+
+@pytest.mark.parametrize("dtype", [BF, HF, F])
+@pytest.mark.parametrize("H,G,D", [(8, 2, 128), (4, 4, 64), (34, 2, 64), (4, 2, 96)])
+@pytest.mark.parametrize("pool", [E, I])
+def test_decode_over_every_element(device, pool, H, G, D, dtype):
+    """Elements up to the type's largest, under powers of two and other scales, K's and V's of a block far
+    apart; contexts in one piece and in several."""
+    gen = torch.Generator().manual_seed(22)
+    bs, lens = 16, [1, 17, 700, 64]
+    nb = [(n + bs - 1) // bs for n in lens]
+    tab, at = [], 0
+    for x in nb:
+        tab.append(list(range(at, at + x)) + [0] * (max(nb) - x))
+        at += x
+    kp, vp = (full_pool(G, sum(nb), bs, D, pool, gen, device) for _ in "kv")
+    q = torch.randn((len(lens), H, D), generator=gen).to(dtype).to(device)
+    for any_scale in (False, True):
+        s = torch.exp2(torch.randint(-9, -6, (2, G, sum(nb)), generator=gen).float())
+        s[1] *= 2.0 ** 12
+        if any_scale:
+            s *= 1 + torch.rand(s.shape, generator=gen)
+        decode_against_64_bits(q, kp, vp, s[0].to(device), s[1].to(device), tab, lens, 0.02, bs,
+                               weights=True)
