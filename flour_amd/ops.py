@@ -563,7 +563,7 @@ def paged_decode_weights(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Te
     """paged_decode that also adds the step's attention weights to ``weights``, fp32 (rows,
     kv_heads, positions): weights[r, g, j] += the sum over kv head g's query heads of their softmax
     weight on position j, r = weight_rows[b] or b. Rows of one call must differ; one outside the
-    tensor adds nothing."""
+    tensor adds nothing. A score of NaN or +inf makes its (row, kv head)'s sums NaN, for good."""
     dev = _same_device(q, k_pool, v_pool, block_tables, context_lens, out, weights, weight_rows)
     _need_i32(block_tables, context_lens)
     G, slots, D = _pools(k_pool, v_pool, block_size)

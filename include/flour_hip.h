@@ -292,7 +292,9 @@ int flour_hip_paged_decode_q8(void* out, int out_dtype, const void* q, int dtype
  * for the sequence's positions j < context_len, r = weight_rows[b] (b itself if weight_rows is
  * NULL). weights is fp32 (num_weight_rows, kv_heads, weights_width) contiguous, weights_width >=
  * max_context_len. Entries of one call must have different rows; one whose row lies outside
- * [0, num_weight_rows) adds nothing (its attention is computed all the same).
+ * [0, num_weight_rows) adds nothing (its attention is computed all the same). A query head of which a
+ * score is NaN or +inf adds NaN to every position of its kv head, also where an fp32 pool's output is a zero
+ * row: such sums stay NaN until the caller writes them, and to flour_hip_kv_evict are below every number.
  * A workspace of flour_hip_decode_weights_workspace_size bytes (256-byte aligned, no
  * initialisation needed) is required; calls that share one must not overlap in time. */
 int flour_hip_paged_decode_weights(void* out, int out_dtype, const void* q, const void* k_pool,
