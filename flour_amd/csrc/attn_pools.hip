@@ -227,7 +227,7 @@ int launch_weights_add(float* weights, int64_t width, const int32_t* weight_rows
                        hipStream_t stream) {
     if (max_ctx <= 0) return FLOUR_OK;
     const int per = AP_THREADS * WA_POS;
-    weights_add_kernel<<<dim3((unsigned)((max_ctx + per - 1) / per), kv_heads, batch),
+    weights_add_kernel<<<dim3((unsigned)(((int64_t)max_ctx + per - 1) / per), kv_heads, batch),
                          dim3(AP_THREADS), 0, stream>>>(weights, width, weight_rows, num_rows,
                                                         context_lens, max_ctx, kv_heads, n_rep,
                                                         scores, score_stride, ml);

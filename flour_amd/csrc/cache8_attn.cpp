@@ -225,7 +225,7 @@ struct Stage {
 static bool stage_of(int num_seqs, int max_seqlen_q, int total_q, int max_kv, int kv_heads,
                      int head_dim, int block_size, int dtype, size_t limit, Stage* st) {
     if (num_seqs <= 0 || max_kv <= 0 || (head_dim != 64 && head_dim != 128)) return false;
-    st->blocks = (max_kv + block_size - 1) / block_size;
+    st->blocks = (int)(((int64_t)max_kv + block_size - 1) / block_size);
     const size_t seq = (size_t)st->blocks * block_size * head_dim * elem_bytes(dtype);  // of a head
     if (seq > 0x7fffffff) return false;
     // (a head's part of the pool stays below 2^31 bytes: the kernels' limit)

@@ -833,7 +833,7 @@ static int launch_stream(DpArgs a, void* workspace, int max_rows, int rows, hipS
     const int waves = stream_waves<D, TILES, NT>();
     a.max_rows = max_rows;
     stream_layout(&a, workspace, waves, a.batch, (int)std::min<int64_t>(max_cols, 16 * NT), D);
-    const int64_t chunks = (a.max_kv + 16 * TILES - 1) / (16 * TILES);
+    const int64_t chunks = ((int64_t)a.max_kv + 16 * TILES - 1) / (16 * TILES);
     const int64_t half = (int64_t)a.batch * a.kv_heads * groups * chunks / 2;
     const int grid = (int)std::max<int64_t>(1, std::min<int64_t>(half, waves));
     const size_t lds = a.batch <= 64 ? 0 : (size_t)(a.batch + 1) * sizeof(int);

@@ -268,3 +268,29 @@ def test_decode_over_every_element(device, pool, H, G, D, dtype):
             s *= 1 + torch.rand(s.shape, generator=gen)
         decode_against_64_bits(q, kp, vp, s[0].to(device), s[1].to(device), tab, lens, 0.02, bs,
                                weights=True)
+
+
+@pytest.mark.parametrize("D,bs", [(64, 16), (20, 16)])
+def test_bounds_of_2_31_positions(device, D, bs):
+    """max_context_len and max_kv_len of 2^31 - 1 over a table that wide: decode and prefill as with the
+    sequence's own length."""
+    H, G, n, rows, most = 4, 2, 40, 5, (1 << 31) - 1
+    gen = torch.Generator().manual_seed(23)
+    kp, vp = (full_pool(G, 3, bs, D, I, gen, device) for _ in "kv")
+    s = torch.full((G, 3), 2.0 ** -7, device=device)
+    q = torch.randn((rows, H, D), generator=gen).to(BF).to(device)
+    wide = torch.zeros((1, (most + bs - 1) // bs), dtype=torch.int32, device=device)
+    wide[0, :3] = i32([2, 0, 1], device)
+    lens, cu = i32([n], device), i32([0, rows], device)
+
+    def calls(table, bound):
+        return (ops.paged_decode_q8(q[:1], kp, vp, s, s, table, lens, 0.05, bound, bs, out_dtype=F),
+                ops.varlen_prefill_q8(q, kp, vp, s, s, cu, lens, table, rows, bound, 0.05, bs,
+                                      out_dtype=F))
+
+    c, t = (Cache(x, s, bs) for x in (kp, vp)), [2, 0, 1]
+    k, v = (x.rows(t, n) for x in c)
+    got = calls(wide, most)
+    for x, qs in zip(got, (q[:1], q)):
+        want, _, err = attend(qs.cpu().double().numpy(), k, v, 0.05)
+        close(x, want, 2 * err[:, :, None] * np.abs(v).max())
