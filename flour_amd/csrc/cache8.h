@@ -107,11 +107,11 @@ __device__ __forceinline__ float scale_for(uint32_t amax) {
     return __uint_as_float((uint32_t)(e + 127) << 23);
 }
 
-// A stored scale as the write and the eviction take it: itself if it is a power of two or 0, the next
-// power of two otherwise (scales that a caller chose), NaN if it is negative, inf or NaN.
+// A stored scale as the write takes it: itself if it is a power of two from 2^-126 on or 0, the next one
+// otherwise (scales that a caller chose), NaN if it is negative, inf, NaN or beyond 2^127.
 __device__ __forceinline__ float pow2_scale(float s) {
-    const uint32_t u = __float_as_uint(s);
-    if (u >= 0x7f000000u) return __uint_as_float(0x7fc00000u);  // (negative ones too: the sign bit)
+    const uint32_t u = __float_as_uint(s + 0.0f);  // (-0 as 0)
+    if (u > 0x7f000000u) return __uint_as_float(0x7fc00000u);  // (negative ones too: the sign bit)
     if (u == 0) return 0.0f;
     const uint32_t up = (u + 0x007fffffu) & 0xff800000u;
     return __uint_as_float(up < 0x00800000u ? 0x00800000u : up);

@@ -234,8 +234,8 @@ int flour_hip_varlen_prefill_ws(void* out, int out_dtype, int64_t o_stride_tok,
  * num_slots / block_size): an element of block b and kv head h stands for itself times
  * scale[h, b]. Tables, lengths, slots and q / out are those of the plain pools.
  *
- * Functions that read a pool take any scale that is not negative, and elements that are numbers (the
- * writing ones store no others). Those that write one
+ * Functions that read a pool take any scale that is 0 or a positive normal number (of subnormal ones
+ * attention may make 0), and elements that are numbers (the writing ones store no others). Those that write one
  * (flour_hip_kv_write_q8, flour_hip_kv_evict) store powers of two: the smallest S >= 2^-126 with
  * which no element exceeds 448 (e4m3) or 127 (int8) times S, 0 for a block of zeros. A block that
  * takes an infinity or a NaN gets the scale NaN: whoever attends to one of its positions reads
@@ -246,8 +246,8 @@ int flour_hip_varlen_prefill_ws(void* out, int out_dtype, int64_t o_stride_tok,
  * cu_seqlens_q[s] .. cu_seqlens_q[s+1]-1, its positions kv_lens[s] - q_len .. kv_lens[s]-1; row t,
  * head h of k and v at t*stride_tok + h*stride_head (elements), in `dtype`. total_q =
  * cu_seqlens_q[num_seqs].
- * A block that the call writes gets the scale max(S_kept, S_new): S_kept the stored scale if the
- * block holds positions of the sequence from before the call (0 otherwise, whatever the block
+ * A block that the call writes gets the scale max(S_kept, S_new): S_kept the stored scale (the next power
+ * of two where it is none; NaN where that is beyond 2^127) if the block holds positions of the sequence from before the call (0 otherwise, whatever the block
  * held), S_new the one the new rows need. Rows kept from before are requantised where that is
  * larger than their scale; new rows are rounded once, to nearest even. Rows of a block behind the
  * sequence's last position keep their bits.
