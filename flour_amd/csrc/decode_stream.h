@@ -29,10 +29,10 @@
 //    in-lane, pairs of tokens' bytes by v_perm_b32, then the same conversion.
 //
 // Measured, kernel + merge: decode steps, 64 x 512-4,096 tokens of 32 / 8 heads of 128 in e4m3 (278
-// MB) 54 + 6.5 us, the stream at 5.1 TB/s; 8 x 16-32K of 64 / 8 in int8 (415 MB) 72 + 6 us, 5.7 TB/s;
-// one sequence of 2,000 tokens 7 + 5 us, launches and dependent loads. Drafted rows, 32 sequences of
-// 512-4,096 tokens with 3-8 rows of 32 / 8 heads (162 MB) 49 + 9.5 us: with two column tiles a SIMD
-// holds one wave, whose vector instructions take 47% of the time and its waits the rest.
+// MB) 54 + 6.5 us, the stream at 5.1 TB/s, what its loads reach alone; 8 x 16-32K of 64 / 8 in int8 (415
+// MB) 72 + 6 us, 5.7 TB/s; one sequence of 2,000 tokens 7 + 5 us, launches and dependent loads. Drafted
+// rows, 32 sequences of 512-4,096 tokens with 3-8 rows of 32 / 8 heads (162 MB) 49 + 9.5 us: with two
+// column tiles a SIMD holds one wave, whose vector instructions take 47% of the time and its waits the rest.
 #pragma once
 
 #include <math.h>

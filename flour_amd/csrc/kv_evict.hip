@@ -6,11 +6,13 @@
 // Gather, a wave a (sequence, kv head, destination block): kept rows are copied (plain pools) or
 // requantised under the destination block's own scale (8-bit pools).
 //
-// The gather is bound by memory: 16 sequences' 1,000 positions of 8 bf16 heads of 128 (131 MB) 22 us, 6.0
-// TB/s, 4 x 4,096 in e4m3 (67 MB, rows of 128 bytes apart) 15 us, 4.5. The selection is bound by what
-// one CU does: 16 x 8 heads of 2-4K positions 10 us, 4 x 8 of 16-32K, on 32 CUs, 31 (load 3, range 3,
-// digits 10, totals and kept positions 7, the latest and the zeros 4). More workgroups a head would have to
-// wait for each other, or be a row of small launches.
+// The gather of plain pools is bound by memory: 16 sequences' 1,000 positions of 8 bf16 heads of 128 (131
+// MB) 22 us, 6.0 TB/s, from sources that the Infinity Cache holds, about 9 more from others. That of 8-bit
+// pools is bound by vector issue (76% of its cycles: maxima and conversions): 4 x 4,096 in e4m3 (67 MB,
+// rows of 128 bytes apart) 15 us, 4.5 TB/s. The selection is bound by what one CU does: 16 x 8 heads of
+// 2-4K positions 10 us, 4 x 8 of 16-32K, on 32 CUs, 31 (load 3, range 3, digits 10, totals and kept
+// positions 7, the latest and the zeros 4). One launch with no wait between workgroups is what this form
+// has; several workgroups a head, in a few short launches, have not been measured.
 #include <type_traits>
 
 #include "cache8.h"

@@ -605,7 +605,8 @@ def varlen_prefill_q8(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tenso
     """varlen_prefill over an 8-bit cache that already holds the rows' K/V (kv_write_q8): packed q
     (total_q, num_heads, head_dim), any view with a unit last stride. ``max_seqlen_q`` bounds the
     rows of a sequence, ``max_kv_len`` kv_lens; rows of q behind the last sequence's (a padded
-    batch) leave ``out`` as it was."""
+    batch) leave ``out`` as it was. Calls of many rows round each value of the cache once to q's type,
+    exact for the scales that kv_write_q8 stores."""
     dev = _same_device(q, k_pool, v_pool, k_scale, v_scale, cu_seqlens_q, kv_lens, block_tables, out)
     _need_i32(cu_seqlens_q, kv_lens, block_tables)
     code, G, slots, D = _pools8(k_pool, v_pool, k_scale, v_scale, block_size)
