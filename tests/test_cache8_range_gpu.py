@@ -294,3 +294,47 @@ def test_bounds_of_2_31_positions(device, D, bs):
     for x, qs in zip(got, (q[:1], q)):
         want, _, err = attend(qs.cpu().double().numpy(), k, v, 0.05)
         close(x, want, 2 * err[:, :, None] * np.abs(v).max())
+
+
+def test_staged_prefill_captured_and_replayed_over_changing_scales(device, prefill_mode):
+    """A captured staged call with f16 queries looks at the scales in every replay: ordinary ones, a head
+    beyond f16, ordinary ones again, each as the eager call, with eager work between them."""
+    H, G, D, bs, rows, n = 4, 2, 128, 16, 70, 150
+    gen = torch.Generator().manual_seed(24)
+    nb = (n + bs - 1) // bs
+    kp, vp = (full_pool(G, nb, bs, D, E, gen, device) for _ in "kv")
+    q = torch.randn((rows, H, D), generator=gen).to(HF).to(device)
+    ks, vs = (torch.full((G, nb), 2.0 ** -9, device=device) for _ in "kv")
+    ws = ops.Workspace(device)
+    args = (i32([0, rows], device), i32([n], device), i32([list(range(nb))], device), rows, n, 0.05, bs)
+    prefill_mode(2)
+    out = torch.empty((rows, H, D), dtype=F, device=device)
+
+    def call(o):
+        return ops.varlen_prefill_q8(q, kp, vp, ks, vs, *args, out=o, workspace=ws)
+
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        call(out)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        call(out)
+    plain = None
+    for v in (2.0 ** -9, 2.0 ** -40, 2.0 ** -9, 2.0 ** 30, 2.0 ** -9):
+        vs[1] = v
+        out.fill_(7.0)
+        g.replay()
+        torch.cuda.synchronize()
+        got = out.clone()
+        want = call(torch.empty_like(out))
+        assert torch.equal(got, want)
+        if v == 2.0 ** -9:
+            plain = got if plain is None else plain
+            assert torch.equal(got, plain)
+        else:  # V under another power of two: the output times it, but for the probabilities' rounding
+            assert torch.equal(got[:, :2], plain[:, :2])
+            c = Cache(vp, torch.full((G, nb), v, device=device), bs)
+            big = float(np.abs(c.rows(list(range(nb)), n)).max())
+            off = (got[:, 2:].double() - plain[:, 2:].double() * (v * 2.0 ** 9)).abs().max()
+            assert off <= 1.01 * 2.0 ** -11 * big
