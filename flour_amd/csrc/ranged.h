@@ -1,0 +1,44 @@
+// ranged.h — attention over parts of the cached positions, as the kernels that compute it share a call:
+// a sliding window with sinks, or a prefix that groups of sequences have in common.
+#pragma once
+
+#include "flour_common.h"
+
+namespace flour {
+
+struct RangedAttn {
+    void* out;
+    int out_dtype;
+    int64_t o_st, o_sh;
+    const void* q;
+    int64_t q_st, q_sh;
+    const void *k_pool, *v_pool;
+    int dtype;
+    const int32_t* cu;  // null: a decode step, row b of sequence b
+    const int32_t* kv_lens;
+    const int32_t* block_tables;
+    int max_blocks, num_seqs, max_rows, rows, num_heads, kv_heads, head_dim, block_size;
+    int64_t num_slots;
+    int max_kv;  // bounds kv_lens
+    float scale;
+    // A row at position p sees j <= p with p - j < window or j < sinks.
+    int window, sinks;
+    // Groups of sequences with the first shared_lens[g] positions in common (num_groups 0: none).
+    const int32_t *group_starts, *shared_lens;
+    int num_groups, max_shared;
+};
+
+// Rows of sequence s, its kv length (0 where its rows see nothing).
+struct RangedSeq {
+    int row0, rows, kv;
+};
+__device__ __forceinline__ RangedSeq ranged_seq(const RangedAttn& a, int s) {
+    const int r0 = a.cu ? a.cu[s] : s, n = a.cu ? a.cu[s + 1] - r0 : 1;
+    const int kv = min(a.kv_lens[s], a.max_kv);
+    return RangedSeq{r0, max(n, 0), kv >= n && kv > 0 ? kv : 0};
+}
+
+// Takes every shape (ranged_generic.hip).
+int launch_ranged_generic(const RangedAttn& a, hipStream_t stream);
+
+}  // namespace flour

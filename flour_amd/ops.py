@@ -11,8 +11,10 @@ call into libflour_hip.so. Shapes follow the C-ABI (include/flour_hip.h):
 
 A cache in 8 bits (``kv_write_q8``, ``kv_dequant``, ``paged_decode_q8``, ``varlen_prefill_q8``) has
 pools of torch.float8_e4m3fn or torch.int8 and fp32 scales (kv_heads, num_blocks);
-``paged_decode_weights`` and ``kv_evict`` sum attention weights and evict by them. These have no
-counterpart in the reference.
+``paged_decode_weights`` and ``kv_evict`` sum attention weights and evict by them.
+``paged_decode_window`` and ``varlen_prefill_window`` attend to a sliding window and the first few
+positions, ``paged_decode_shared`` and ``varlen_prefill_shared`` to prefixes that sequences have in
+common, once for all of them. These have no counterpart in the reference.
 """
 from __future__ import annotations
 
@@ -683,3 +685,177 @@ def kv_evict(k_pool: torch.Tensor, v_pool: torch.Tensor, weights: torch.Tensor,
             out_tables.shape[1], _at(kept), B, G, D, block_size, slots, max_context_len,
             max_keep_len, recent)
     return kept
+
+
+# ------------------------------------------------------------------ parts of the cache
+# A sliding window with sinks, and prefixes that groups of sequences share. These too run on the
+# tensors' own device, on its current stream.
+def _window_size(dev: int, *shape: int) -> int:
+    return _size("flour_hip_window_workspace_size", dev, switches(), *shape)
+
+
+def _shared_size(dev: int, *shape: int) -> int:
+    return _size("flour_hip_shared_workspace_size", dev, switches(), *shape)
+
+
+def window_workspace_bytes(num_seqs: int, max_seqlen_q: int, total_q: int, num_heads: int,
+                           kv_heads: int, head_dim: int, max_kv_len: int, window: int, sinks: int,
+                           dtype: torch.dtype) -> int:
+    """Bytes of workspace of varlen_prefill_window on the current device, and of
+    paged_decode_window (max_seqlen_q 1, total_q = num_seqs)."""
+    return _window_size(_device_in_use(), num_seqs, max_seqlen_q, total_q, num_heads, kv_heads,
+                        head_dim, max_kv_len, window, sinks, dtype_code(dtype))
+
+
+def shared_workspace_bytes(num_seqs: int, num_groups: int, max_seqlen_q: int, total_q: int,
+                           num_heads: int, kv_heads: int, head_dim: int, max_kv_len: int,
+                           max_shared_len: int, dtype: torch.dtype) -> int:
+    """Bytes of workspace of varlen_prefill_shared on the current device, and of
+    paged_decode_shared (max_seqlen_q 1, total_q = num_seqs)."""
+    return _shared_size(_device_in_use(), num_seqs, num_groups, max_seqlen_q, total_q, num_heads,
+                        kv_heads, head_dim, max_kv_len, max_shared_len, dtype_code(dtype))
+
+
+def _plain_pools(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
+                 block_size: int) -> tuple[int, int, int]:
+    shape = _pools(k_pool, v_pool, block_size)
+    if q.dtype != k_pool.dtype:
+        raise _invalid("q and pools must share a dtype")
+    return shape
+
+
+def _prefill_q(q: torch.Tensor, D: int, G: int) -> tuple:
+    shape, strides = q.shape, q.stride()
+    if len(shape) != 3 or shape[2] != D or strides[2] != 1 or shape[1] == 0 or shape[1] % G != 0:
+        raise _invalid("q must be (total_q, num_heads, head_dim) with a unit last stride, "
+                       "num_heads a multiple of the pools' kv_heads")
+    return shape, strides
+
+
+def _groups(group_starts: torch.Tensor, shared_lens: torch.Tensor) -> int:
+    _need_i32(group_starts, shared_lens)
+    n = shared_lens.numel()
+    if shared_lens.dim() != 1 or group_starts.dim() != 1 or group_starts.numel() != n + 1:
+        raise _invalid(f"group_starts must hold one entry more than shared_lens, got "
+                       f"{tuple(group_starts.shape)} and {tuple(shared_lens.shape)}")
+    return n
+
+
+def paged_decode_window(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
+                        block_tables: torch.Tensor, context_lens: torch.Tensor, scale: float,
+                        max_context_len: int, window: int, sinks: int = 0, block_size: int = 16,
+                        out_dtype: torch.dtype | None = None, out: torch.Tensor | None = None,
+                        workspace: Workspace | None = None) -> torch.Tensor:
+    """paged_decode over the last ``window`` positions of each sequence, the new token's among them,
+    and the first ``sinks`` ones. Blocks without visible positions are not looked at."""
+    dev = _same_device(q, k_pool, v_pool, block_tables, context_lens, out)
+    _need_i32(block_tables, context_lens)
+    G, slots, D = _plain_pools(q, k_pool, v_pool, block_size)
+    B, H = _decode_q(q, D, G)
+    _lens(context_lens, B, "context_lens")
+    width = _table(block_tables, B, "block_tables")
+    out = _decode_out(out, q, out_dtype)
+    code = dtype_code(q.dtype)
+    ws = _scratch(workspace, _window_size(dev, B, 1, B, H, G, D, max_context_len, window, sinks,
+                                          code), q)
+    _launch(lib().flour_hip_paged_decode_window, dev, out.data_ptr(), dtype_code(out.dtype),
+            q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), block_tables.data_ptr(), width,
+            context_lens.data_ptr(), B, H, G, D, block_size, slots, max_context_len, window, sinks,
+            float(scale), code, ws.data_ptr(), ws.numel())
+    return out
+
+
+def varlen_prefill_window(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
+                          cu_seqlens_q: torch.Tensor, kv_lens: torch.Tensor,
+                          block_tables: torch.Tensor, max_seqlen_q: int, max_kv_len: int,
+                          scale: float, window: int, sinks: int = 0, block_size: int = 16,
+                          out_dtype: torch.dtype | None = None, out: torch.Tensor | None = None,
+                          workspace: Workspace | None = None) -> torch.Tensor:
+    """varlen_prefill in which a row at position p sees p - window + 1 .. p and the first ``sinks``
+    positions up to p. Packed q (total_q, num_heads, head_dim), any view with a unit last stride;
+    ``max_seqlen_q`` bounds the rows of a sequence, ``max_kv_len`` kv_lens; rows of q behind the last
+    sequence's (a padded batch) leave ``out`` as it was."""
+    dev = _same_device(q, k_pool, v_pool, cu_seqlens_q, kv_lens, block_tables, out)
+    _need_i32(cu_seqlens_q, kv_lens, block_tables)
+    G, slots, D = _plain_pools(q, k_pool, v_pool, block_size)
+    shape, strides = _prefill_q(q, D, G)
+    T, H, _ = shape
+    n = cu_seqlens_q.numel() - 1
+    _lens(kv_lens, n, "kv_lens")
+    width = _table(block_tables, n, "block_tables")
+    out = _out(out, shape, out_dtype or q.dtype, q.device)
+    out_strides = out.stride()
+    if out_strides[2] != 1:
+        raise _invalid("out must have a unit last stride")
+    code = dtype_code(q.dtype)
+    ws = _scratch(workspace, _window_size(dev, n, max_seqlen_q, T, H, G, D, max_kv_len, window,
+                                          sinks, code), q)
+    _launch(lib().flour_hip_varlen_prefill_window, dev, out.data_ptr(), dtype_code(out.dtype),
+            out_strides[0], out_strides[1], q.data_ptr(), strides[0], strides[1],
+            k_pool.data_ptr(), v_pool.data_ptr(), cu_seqlens_q.data_ptr(), kv_lens.data_ptr(),
+            block_tables.data_ptr(), width, n, max_seqlen_q, T, H, G, D, block_size, slots,
+            max_kv_len, window, sinks, float(scale), code, ws.data_ptr(), ws.numel())
+    return out
+
+
+def paged_decode_shared(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
+                        block_tables: torch.Tensor, context_lens: torch.Tensor,
+                        group_starts: torch.Tensor, shared_lens: torch.Tensor, scale: float,
+                        max_context_len: int, max_shared_len: int, block_size: int = 16,
+                        out_dtype: torch.dtype | None = None, out: torch.Tensor | None = None,
+                        workspace: Workspace | None = None) -> torch.Tensor:
+    """paged_decode for a batch in groups: sequences group_starts[g]:group_starts[g + 1] have the same
+    K/V at their first shared_lens[g] positions, which is computed once for all of the group's rows,
+    through its first sequence's table. ``max_shared_len`` bounds shared_lens."""
+    dev = _same_device(q, k_pool, v_pool, block_tables, context_lens, group_starts, shared_lens, out)
+    _need_i32(block_tables, context_lens)
+    G, slots, D = _plain_pools(q, k_pool, v_pool, block_size)
+    B, H = _decode_q(q, D, G)
+    _lens(context_lens, B, "context_lens")
+    width = _table(block_tables, B, "block_tables")
+    n = _groups(group_starts, shared_lens)
+    out = _decode_out(out, q, out_dtype)
+    code = dtype_code(q.dtype)
+    ws = _scratch(workspace, _shared_size(dev, B, n, 1, B, H, G, D, max_context_len,
+                                          max_shared_len, code), q)
+    _launch(lib().flour_hip_paged_decode_shared, dev, out.data_ptr(), dtype_code(out.dtype),
+            q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), block_tables.data_ptr(), width,
+            context_lens.data_ptr(), B, group_starts.data_ptr(), shared_lens.data_ptr(), n, H, G, D,
+            block_size, slots, max_context_len, max_shared_len, float(scale), code, ws.data_ptr(),
+            ws.numel())
+    return out
+
+
+def varlen_prefill_shared(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
+                          cu_seqlens_q: torch.Tensor, kv_lens: torch.Tensor,
+                          block_tables: torch.Tensor, group_starts: torch.Tensor,
+                          shared_lens: torch.Tensor, max_seqlen_q: int, max_kv_len: int,
+                          max_shared_len: int, scale: float, block_size: int = 16,
+                          out_dtype: torch.dtype | None = None, out: torch.Tensor | None = None,
+                          workspace: Workspace | None = None) -> torch.Tensor:
+    """varlen_prefill for a batch in groups with shared prefixes, as in paged_decode_shared: several
+    rows a sequence (drafted tokens, turns), packed, with the bounds of varlen_prefill_window."""
+    dev = _same_device(q, k_pool, v_pool, cu_seqlens_q, kv_lens, block_tables, group_starts,
+                       shared_lens, out)
+    _need_i32(cu_seqlens_q, kv_lens, block_tables)
+    G, slots, D = _plain_pools(q, k_pool, v_pool, block_size)
+    shape, strides = _prefill_q(q, D, G)
+    T, H, _ = shape
+    n = cu_seqlens_q.numel() - 1
+    _lens(kv_lens, n, "kv_lens")
+    width = _table(block_tables, n, "block_tables")
+    groups = _groups(group_starts, shared_lens)
+    out = _out(out, shape, out_dtype or q.dtype, q.device)
+    out_strides = out.stride()
+    if out_strides[2] != 1:
+        raise _invalid("out must have a unit last stride")
+    code = dtype_code(q.dtype)
+    ws = _scratch(workspace, _shared_size(dev, n, groups, max_seqlen_q, T, H, G, D, max_kv_len,
+                                          max_shared_len, code), q)
+    _launch(lib().flour_hip_varlen_prefill_shared, dev, out.data_ptr(), dtype_code(out.dtype),
+            out_strides[0], out_strides[1], q.data_ptr(), strides[0], strides[1],
+            k_pool.data_ptr(), v_pool.data_ptr(), cu_seqlens_q.data_ptr(), kv_lens.data_ptr(),
+            block_tables.data_ptr(), width, n, group_starts.data_ptr(), shared_lens.data_ptr(),
+            groups, max_seqlen_q, T, H, G, D, block_size, slots, max_kv_len, max_shared_len,
+            float(scale), code, ws.data_ptr(), ws.numel())
+    return out

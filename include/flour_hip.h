@@ -370,6 +370,87 @@ int flour_hip_kv_evict(void* k_pool, void* v_pool, float* k_scale, float* v_scal
                        int kv_heads, int head_dim, int block_size, int64_t num_slots,
                        int max_context_len, int max_keep_len, int recent, void* stream);
 
+/* ------------------------------------------------------------------------------------------
+ * Attention over a sliding window with sinks (no counterpart in the reference, whose models attend
+ * to every cached position). A row at position p sees the positions j <= p with p - j < window (its
+ * own and the window - 1 before it) and those with j < sinks, the first ones, which stay visible.
+ * window >= 1, sinks >= 0; a window at least as long as the context is plain causal attention.
+ * Positions that no row sees are not read for their values: blocks that hold none but those may be
+ * given back, their table entries left as any number. Visible positions' arithmetic is that of
+ * flour_hip_paged_decode and flour_hip_varlen_prefill; a row with a visible score of NaN or +inf reads
+ * NaN, in every type, one that sees no score above -inf is a zero row.
+ *
+ * The arguments are those of the plain calls, and max_kv_len, which bounds kv_lens (a longer sequence
+ * is taken to end there). Rows behind the last sequence's, where total_q is larger than
+ * cu_seqlens_q[num_seqs], leave out as it was. A workspace of flour_hip_window_workspace_size
+ * bytes (256-byte aligned, no initialisation needed; max_seqlen_q 1 and total_q = num_seqs = batch for
+ * a decode step) goes with the call, FLOUR_ERR_WORKSPACE where it is smaller; calls that share one must
+ * not overlap in time.
+ * ---------------------------------------------------------------------------------------- */
+int flour_hip_window_workspace_size(int num_seqs, int max_seqlen_q, int total_q, int num_heads,
+                                    int kv_heads, int head_dim, int max_kv_len, int window,
+                                    int sinks, int dtype, size_t* bytes);
+
+int flour_hip_paged_decode_window(void* out, int out_dtype, const void* q, const void* k_pool,
+                                  const void* v_pool, const int32_t* block_tables,
+                                  int max_blocks_per_seq, const int32_t* context_lens, int batch,
+                                  int num_heads, int kv_heads, int head_dim, int block_size,
+                                  int64_t num_slots, int max_context_len, int window, int sinks,
+                                  float scale, int dtype, void* workspace, size_t workspace_bytes,
+                                  void* stream);
+
+int flour_hip_varlen_prefill_window(void* out, int out_dtype, int64_t o_stride_tok,
+                                    int64_t o_stride_head, const void* q, int64_t q_stride_tok,
+                                    int64_t q_stride_head, const void* k_pool, const void* v_pool,
+                                    const int32_t* cu_seqlens_q, const int32_t* kv_lens,
+                                    const int32_t* block_tables, int max_blocks_per_seq,
+                                    int num_seqs, int max_seqlen_q, int total_q, int num_heads,
+                                    int kv_heads, int head_dim, int block_size, int64_t num_slots,
+                                    int max_kv_len, int window, int sinks, float scale, int dtype,
+                                    void* workspace, size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------------------------
+ * Attention of a batch whose sequences share long prefixes, each prefix computed once for all of its
+ * rows (the reference shares the prefix's blocks, prefix.rs, and attends to them once a sequence). The
+ * result is that of flour_hip_paged_decode / flour_hip_varlen_prefill over the same tables.
+ *
+ *   group_starts [num_groups + 1] int32: sequences group_starts[g] .. group_starts[g + 1] - 1 are group
+ *                g. They must not decrease; sequences before the first or behind the last are in no
+ *                group and attend to their own tables alone.
+ *   shared_lens  [num_groups] int32: the first shared_lens[g] positions of group g's sequences are the
+ *                same K/V. They are read through the table of the group's first sequence, which has to
+ *                name their blocks (whatever that sequence's own length), the rest through each
+ *                sequence's own. Any length counts, whole blocks or not; negative ones are 0, and
+ *                longer ones than max_shared_len are taken as that.
+ * A row sees positions up to its own, in the prefix too, so sequences may be shorter than their group's
+ * prefix. The other arguments are those of the plain calls; max_kv_len, rows behind the last sequence's,
+ * the workspace (flour_hip_shared_workspace_size) and scores of NaN or infinity are as above.
+ * ---------------------------------------------------------------------------------------- */
+int flour_hip_shared_workspace_size(int num_seqs, int num_groups, int max_seqlen_q, int total_q,
+                                    int num_heads, int kv_heads, int head_dim, int max_kv_len,
+                                    int max_shared_len, int dtype, size_t* bytes);
+
+int flour_hip_paged_decode_shared(void* out, int out_dtype, const void* q, const void* k_pool,
+                                  const void* v_pool, const int32_t* block_tables,
+                                  int max_blocks_per_seq, const int32_t* context_lens, int batch,
+                                  const int32_t* group_starts, const int32_t* shared_lens,
+                                  int num_groups, int num_heads, int kv_heads, int head_dim,
+                                  int block_size, int64_t num_slots, int max_context_len,
+                                  int max_shared_len, float scale, int dtype, void* workspace,
+                                  size_t workspace_bytes, void* stream);
+
+int flour_hip_varlen_prefill_shared(void* out, int out_dtype, int64_t o_stride_tok,
+                                    int64_t o_stride_head, const void* q, int64_t q_stride_tok,
+                                    int64_t q_stride_head, const void* k_pool, const void* v_pool,
+                                    const int32_t* cu_seqlens_q, const int32_t* kv_lens,
+                                    const int32_t* block_tables, int max_blocks_per_seq,
+                                    int num_seqs, const int32_t* group_starts,
+                                    const int32_t* shared_lens, int num_groups, int max_seqlen_q,
+                                    int total_q, int num_heads, int kv_heads, int head_dim,
+                                    int block_size, int64_t num_slots, int max_kv_len,
+                                    int max_shared_len, float scale, int dtype, void* workspace,
+                                    size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,6 +1,7 @@
 //! Raw FFI bindings of `libflour_hip.so`: the C-ABI declared in `include/flour_hip.h` (the
 //! attention hot path: KV-cache write, fused RoPE + KV write, paged decode, causal varlen
-//! prefill, the same over 8-bit caches, attention-weight sums and eviction by them) and `include/flour_cache.h` (block allocator, block table, per-sequence cache and
+//! prefill, the same over 8-bit caches, attention-weight sums and eviction by them, attention over a
+//! window with sinks and over shared prefixes) and `include/flour_cache.h` (block allocator, block table, per-sequence cache and
 //! many sequences over one device pool).
 //!
 //! These replace, in the flour crate, `paged_attention` (`src/backend/cpu.rs:57-112`),
@@ -141,6 +142,41 @@ extern "C" {
         keep_lens: *const i32, out_tables: *const i32, out_max_blocks: c_int, kept: *mut i32,
         batch: c_int, kv_heads: c_int, head_dim: c_int, block_size: c_int, num_slots: i64,
         max_context_len: c_int, max_keep_len: c_int, recent: c_int, stream: *mut c_void) -> c_int;
+    pub fn flour_hip_window_workspace_size(num_seqs: c_int, max_seqlen_q: c_int, total_q: c_int,
+        num_heads: c_int, kv_heads: c_int, head_dim: c_int, max_kv_len: c_int, window: c_int,
+        sinks: c_int, dtype: c_int, bytes: *mut usize) -> c_int;
+    pub fn flour_hip_paged_decode_window(out: *mut c_void, out_dtype: c_int, q: *const c_void,
+        k_pool: *const c_void, v_pool: *const c_void, block_tables: *const i32,
+        max_blocks_per_seq: c_int, context_lens: *const i32, batch: c_int, num_heads: c_int,
+        kv_heads: c_int, head_dim: c_int, block_size: c_int, num_slots: i64,
+        max_context_len: c_int, window: c_int, sinks: c_int, scale: f32, dtype: c_int,
+        workspace: *mut c_void, workspace_bytes: usize, stream: *mut c_void) -> c_int;
+    pub fn flour_hip_varlen_prefill_window(out: *mut c_void, out_dtype: c_int, o_stride_tok: i64,
+        o_stride_head: i64, q: *const c_void, q_stride_tok: i64, q_stride_head: i64,
+        k_pool: *const c_void, v_pool: *const c_void, cu_seqlens_q: *const i32,
+        kv_lens: *const i32, block_tables: *const i32, max_blocks_per_seq: c_int, num_seqs: c_int,
+        max_seqlen_q: c_int, total_q: c_int, num_heads: c_int, kv_heads: c_int, head_dim: c_int,
+        block_size: c_int, num_slots: i64, max_kv_len: c_int, window: c_int, sinks: c_int,
+        scale: f32, dtype: c_int, workspace: *mut c_void, workspace_bytes: usize,
+        stream: *mut c_void) -> c_int;
+    pub fn flour_hip_shared_workspace_size(num_seqs: c_int, num_groups: c_int,
+        max_seqlen_q: c_int, total_q: c_int, num_heads: c_int, kv_heads: c_int, head_dim: c_int,
+        max_kv_len: c_int, max_shared_len: c_int, dtype: c_int, bytes: *mut usize) -> c_int;
+    pub fn flour_hip_paged_decode_shared(out: *mut c_void, out_dtype: c_int, q: *const c_void,
+        k_pool: *const c_void, v_pool: *const c_void, block_tables: *const i32,
+        max_blocks_per_seq: c_int, context_lens: *const i32, batch: c_int,
+        group_starts: *const i32, shared_lens: *const i32, num_groups: c_int, num_heads: c_int,
+        kv_heads: c_int, head_dim: c_int, block_size: c_int, num_slots: i64,
+        max_context_len: c_int, max_shared_len: c_int, scale: f32, dtype: c_int,
+        workspace: *mut c_void, workspace_bytes: usize, stream: *mut c_void) -> c_int;
+    pub fn flour_hip_varlen_prefill_shared(out: *mut c_void, out_dtype: c_int, o_stride_tok: i64,
+        o_stride_head: i64, q: *const c_void, q_stride_tok: i64, q_stride_head: i64,
+        k_pool: *const c_void, v_pool: *const c_void, cu_seqlens_q: *const i32,
+        kv_lens: *const i32, block_tables: *const i32, max_blocks_per_seq: c_int, num_seqs: c_int,
+        group_starts: *const i32, shared_lens: *const i32, num_groups: c_int, max_seqlen_q: c_int,
+        total_q: c_int, num_heads: c_int, kv_heads: c_int, head_dim: c_int, block_size: c_int,
+        num_slots: i64, max_kv_len: c_int, max_shared_len: c_int, scale: f32, dtype: c_int,
+        workspace: *mut c_void, workspace_bytes: usize, stream: *mut c_void) -> c_int;
 }
 
 // include/flour_cache.h
