@@ -1,6 +1,10 @@
 // ranged_attn.cpp — C entries of the attention over a sliding window with sinks and over prefixes that
 // sequences share: argument checks, workspaces and the choice of the kernel.
-#include "ranged.h"
+#include <math.h>
+
+#include <algorithm>
+
+#include "ranged_tiles.h"
 
 namespace flour {
 
@@ -33,6 +37,91 @@ static bool check_shape(const char* what, const RangedAttn& a) {
     return true;
 }
 
+static size_t up256(size_t x) { return (x + 255) & ~(size_t)255; }
+
+// ---- the tile kernel
+// What the shape says of it; a call's tensors can still refuse it (tiles_take).
+static bool tiles_fit(int64_t rows, int num_heads, int kv_heads, int head_dim) {
+    // (columns and items counted in 32 bits, a merge workgroup four (row, head) pairs)
+    return (head_dim == 64 || head_dim == 128) && rows * num_heads < (int64_t)1 << 30 &&
+           kv_heads <= 65535;
+}
+
+static bool tiles_take(const RangedAttn& a) {
+    const int es = elem_bytes(a.dtype), oes = elem_bytes(a.out_dtype);
+    return tiles_fit(a.rows, a.num_heads, a.kv_heads, a.head_dim) && a.block_size % 16 == 0 &&
+           a.num_slots * a.head_dim * es <= (int64_t)0x7fffffff && a.scale > 0.0f &&
+           isfinite(a.scale * 1.4426950408889634f) &&
+           (((uint64_t)(uintptr_t)a.q | (uint64_t)(uintptr_t)a.out | (uint64_t)(uintptr_t)a.k_pool |
+             (uint64_t)(uintptr_t)a.v_pool | (uint64_t)(a.q_st * es) | (uint64_t)(a.q_sh * es) |
+             (uint64_t)(a.o_st * oes) | (uint64_t)(a.o_sh * oes)) & 15) == 0;
+}
+
+// How a launch over `units` units of up to unit_rows rows (rows in all) and unit_kv positions each is cut:
+// the grid's items, and the pieces of a pair, so that the launch has about two workgroups a CU.
+struct TilePlan {
+    int items, max_pieces, piece_tiles;
+    size_t bytes;  // of the pieces
+};
+static TilePlan tile_plan(int64_t units, int64_t unit_rows, int64_t rows, int64_t unit_kv, int num_heads,
+                          int kv_heads, int head_dim, int dtype, bool finals) {
+    const int64_t n_rep = num_heads / kv_heads, tt = rt_tokens(elem_bytes(dtype));
+    unit_rows = std::min(unit_rows, rows);
+    const int64_t tiles = std::min(rows * n_rep / RT_COLS + units,
+                                   units * ((unit_rows * n_rep + RT_COLS - 1) / RT_COLS));
+    TilePlan p;
+    p.items = (int)std::max<int64_t>(1, tiles * kv_heads);
+    const int64_t longest = unit_kv / tt + 3;  // (a front tile, and ends that are not whole)
+    const int64_t want = std::max<int64_t>(1, 2 * device_cus() / p.items);
+    // (a piece of fewer tiles costs more in its ends and its merge than it saves)
+    p.piece_tiles = (int)std::max<int64_t>(4, (longest + want - 1) / want);
+    p.max_pieces = (int)std::max<int64_t>(1, std::min<int64_t>(want, longest / p.piece_tiles));
+    p.bytes = finals && p.max_pieces == 1
+                  ? 0
+                  : up256((size_t)rows * num_heads * p.max_pieces * 2 * sizeof(float)) +
+                        up256((size_t)rows * num_heads * p.max_pieces * head_dim * sizeof(float));
+    return p;
+}
+
+static RtArgs tile_args(const RangedAttn& a, int kind, const TilePlan& p, bool finals, char* ws) {
+    RtArgs r{};
+    r.a = a, r.kind = kind, r.n_rep = a.num_heads / a.kv_heads;
+    r.scale_log2 = a.scale * 1.4426950408889634f;
+    r.max_pieces = p.max_pieces, r.piece_tiles = p.piece_tiles, r.finals = finals;
+    r.p_ml = reinterpret_cast<float*>(ws);
+    r.p_o = reinterpret_cast<float*>(
+        ws + up256((size_t)a.rows * a.num_heads * p.max_pieces * 2 * sizeof(float)));
+    return r;
+}
+
+static int launch_tiles(const RtArgs& r, const TilePlan& p, hipStream_t stream) {
+    auto launch = r.a.dtype == FLOUR_DTYPE_F32    ? launch_ranged_tiles_f32
+                  : r.a.dtype == FLOUR_DTYPE_BF16 ? launch_ranged_tiles_bf16
+                                                  : launch_ranged_tiles_f16;
+    return launch(r, p.items, stream);
+}
+
+// Rows over what they see: one launch, and a merge where pairs are cut.
+static TilePlan rows_plan(int num_seqs, int max_rows, int rows, int num_heads, int kv_heads, int head_dim,
+                          int max_kv, int window, int sinks, int dtype) {
+    const int64_t n_rep = num_heads / kv_heads;
+    const int64_t span = (int64_t)window + sinks + RT_COLS / n_rep + 2;
+    return tile_plan(num_seqs, max_rows, rows, std::min<int64_t>(max_kv, span), num_heads, kv_heads,
+                     head_dim, dtype, true);
+}
+
+// The prefixes by groups, then each sequence's own positions, then both together.
+struct SharedPlan {
+    TilePlan prefix, own;
+};
+static SharedPlan shared_plan(int num_seqs, int num_groups, int max_rows, int rows, int num_heads,
+                              int kv_heads, int head_dim, int max_kv, int max_shared, int dtype) {
+    return SharedPlan{tile_plan(num_groups, rows, rows, max_shared, num_heads, kv_heads, head_dim, dtype,
+                                false),
+                      tile_plan(num_seqs, max_rows, rows, max_kv, num_heads, kv_heads, head_dim, dtype,
+                                false)};
+}
+
 static int ranged_call(const char* what, const RangedAttn& a, bool shared, void* workspace,
                        size_t workspace_bytes, hipStream_t stream) {
     if (!check_shape(what, a)) return FLOUR_ERR_INVALID_ARGUMENT;
@@ -42,7 +131,35 @@ static int ranged_call(const char* what, const RangedAttn& a, bool shared, void*
         set_error("%s: null pointer", what);
         return FLOUR_ERR_INVALID_ARGUMENT;
     }
-    return launch_ranged_generic(a, stream);
+    size_t need = 0;
+    int rc = shared ? flour_hip_shared_workspace_size(a.num_seqs, a.num_groups, a.max_rows, a.rows,
+                                                      a.num_heads, a.kv_heads, a.head_dim, a.max_kv,
+                                                      a.max_shared, a.dtype, &need)
+                    : flour_hip_window_workspace_size(a.num_seqs, a.max_rows, a.rows, a.num_heads,
+                                                      a.kv_heads, a.head_dim, a.max_kv, a.window, a.sinks,
+                                                      a.dtype, &need);
+    if (rc != FLOUR_OK) return rc;
+    if (need > 0 && (!workspace || workspace_bytes < need || (uintptr_t)workspace % 256 != 0)) {
+        set_error("%s: workspace of %zu bytes (256-byte aligned) required, got %zu at %p", what, need,
+                  workspace_bytes, workspace);
+        return FLOUR_ERR_WORKSPACE;
+    }
+    if (!tiles_take(a) || (!a.cu && !shared)) return launch_ranged_generic(a, stream);
+    char* ws = static_cast<char*>(workspace);
+    if (!shared || a.num_groups == 0 || a.max_shared == 0) {
+        const TilePlan p = rows_plan(a.num_seqs, a.max_rows, a.rows, a.num_heads, a.kv_heads, a.head_dim,
+                                     a.max_kv, a.window, a.sinks, a.dtype);
+        const RtArgs r = tile_args(a, RT_ROWS, p, true, ws);
+        rc = launch_tiles(r, p, stream);
+        return rc != FLOUR_OK || p.max_pieces == 1 ? rc : launch_ranged_merge(r, nullptr, stream);
+    }
+    const SharedPlan p = shared_plan(a.num_seqs, a.num_groups, a.max_rows, a.rows, a.num_heads, a.kv_heads,
+                                     a.head_dim, a.max_kv, a.max_shared, a.dtype);
+    const RtArgs own = tile_args(a, RT_OWN, p.own, false, ws);
+    const RtArgs prefix = tile_args(a, RT_PREFIX, p.prefix, false, ws + p.own.bytes);
+    rc = launch_tiles(prefix, p.prefix, stream);
+    if (rc == FLOUR_OK) rc = launch_tiles(own, p.own, stream);
+    return rc != FLOUR_OK ? rc : launch_ranged_merge(own, &prefix, stream);
 }
 
 // A decode step's part of a call: one row a sequence, packed rows of all heads.
@@ -105,7 +222,10 @@ extern "C" int flour_hip_window_workspace_size(int num_seqs, int max_seqlen_q, i
         set_error("window_workspace_size: window %d with %d sinks", window, sinks);
         return FLOUR_ERR_INVALID_ARGUMENT;
     }
-    *bytes = 0;
+    *bytes = !tiles_fit(total_q, num_heads, kv_heads, head_dim)
+                 ? 0
+                 : rows_plan(num_seqs, max_seqlen_q, total_q, num_heads, kv_heads, head_dim, max_kv_len,
+                             window, sinks, dtype).bytes;
     return FLOUR_OK;
 }
 
@@ -123,6 +243,12 @@ extern "C" int flour_hip_shared_workspace_size(int num_seqs, int num_groups, int
         return FLOUR_ERR_INVALID_ARGUMENT;
     }
     *bytes = 0;
+    if (!tiles_fit(total_q, num_heads, kv_heads, head_dim)) return FLOUR_OK;
+    const SharedPlan p = shared_plan(num_seqs, num_groups, max_seqlen_q, total_q, num_heads, kv_heads,
+                                     head_dim, max_kv_len, max_shared_len, dtype);
+    const TilePlan alone = rows_plan(num_seqs, max_seqlen_q, total_q, num_heads, kv_heads, head_dim,
+                                     max_kv_len, 0x7fffffff, 0, dtype);
+    *bytes = std::max(p.prefix.bytes + p.own.bytes, alone.bytes);
     return FLOUR_OK;
 }
 

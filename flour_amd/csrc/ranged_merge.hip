@@ -1,0 +1,124 @@
+// ranged_merge.hip — joins the pieces of ranged_tiles.h: out = sum 2^(m_k - M) o_k / sum 2^(m_k - M) l_k over
+// the pieces k of a (row, query head), M their largest maximum.
+//
+// A wave a (row, head), four to a workgroup; a lane holds the maximum and sum of one piece and D / 64
+// dims of the output, over 8 pieces' rows at a time, all in flight together. It reads each piece once.
+#include "ranged_tiles.h"
+
+namespace flour {
+
+static constexpr int RM_WAVES = 4;
+
+struct RmPieces {
+    int n;
+    const float *ml, *o;
+};
+
+// The pieces of packed row `row`, head h in a launch.
+__device__ __forceinline__ RmPieces pieces_of(const RtArgs& ra, int seq, const RangedSeq& q, int row, int h,
+                                              int head_dim, int tt) {
+    const RangedAttn& a = ra.a;
+    const int gr = a.num_groups > 0 ? ranged_group(a, seq) : -1;
+    const int shared = ranged_shared_len(a, gr);
+    RmPieces p{0, nullptr, nullptr};
+    RtSpan sp;
+    if (ra.kind == RT_PREFIX) {
+        if (shared == 0) return p;
+        sp = rt_span(ra, RT_PREFIX, 0, shared, 0, 0, tt);
+    } else {
+        const int col = (row - q.row0) * ra.n_rep + h % ra.n_rep;
+        sp = rt_span(ra, ra.kind, q.rows, q.kv, col / RT_COLS, shared, tt);
+    }
+    p.n = rt_pieces(sp.tiles, ra.max_pieces, ra.piece_tiles);
+    const int64_t slot = ((int64_t)row * a.num_heads + h) * ra.max_pieces;
+    p.ml = ra.p_ml + 2 * slot;
+    p.o = ra.p_o + slot * head_dim;
+    return p;
+}
+
+template <int D>
+__global__ __launch_bounds__(64 * RM_WAVES) void ranged_merge_kernel(RtArgs first, RtArgs second,
+                                                                     bool two, int tt) {
+    constexpr int E = D / 64;
+    typedef typename std::conditional<E == 2, f32x2, float>::type RowV;
+    const RangedAttn& a = first.a;
+    const int lane = threadIdx.x & 63;
+    const int64_t item = (int64_t)blockIdx.x * RM_WAVES + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if (item >= (int64_t)a.rows * a.num_heads) return;
+    const int row = (int)(item / a.num_heads), h = (int)(item - (int64_t)row * a.num_heads);
+    int s = row;
+    if (a.cu) {
+        int x = 0, y = a.num_seqs;
+        while (y - x > 1) {
+            const int mid = (x + y) >> 1;
+            if (a.cu[mid] <= row)
+                x = mid;
+            else
+                y = mid;
+        }
+        s = x;
+    }
+    const RangedSeq q = ranged_seq(a, s);
+    if (row < q.row0 || row >= q.row0 + q.rows) return;  // (rows of no sequence)
+    const RmPieces set[2] = {pieces_of(first, s, q, row, h, D, tt),
+                             two ? pieces_of(second, s, q, row, h, D, tt) : RmPieces{0, nullptr, nullptr}};
+    if (first.finals && set[0].n == 1) return;
+    float M = DEC_M0, L = 0.0f, O[E] = {};
+#pragma unroll
+    for (int x = 0; x < 2; x++) {
+        const RmPieces& p = set[x];
+        for (int p0 = 0; p0 < p.n; p0 += 64) {
+            const bool on = p0 + lane < p.n;
+            const float mx = on ? p.ml[2 * (p0 + lane)] : DEC_M0, lx = on ? p.ml[2 * (p0 + lane) + 1] : 0.0f;
+            const float Mn = fmaxf(M, wave_max(mx));
+            const float w = on ? fast_exp2(mx - Mn) : 0.0f, old = fast_exp2(M - Mn);
+            L = L * old + wave_sum(w * lx);
+#pragma unroll
+            for (int e = 0; e < E; e++) O[e] *= old;
+            const int n = min(64, p.n - p0);
+            for (int y0 = 0; y0 < n; y0 += 8) {
+                RowV v[8];
+#pragma unroll
+                for (int y = 0; y < 8; y++)  // (past the last one: that again, for nothing)
+                    v[y] = *reinterpret_cast<const RowV*>(p.o + (int64_t)min(p0 + y0 + y, p.n - 1) * D +
+                                                          E * lane);
+#pragma unroll
+                for (int y = 0; y < 8; y++) {
+                    const float wy = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w), (y0 + y) & 63));
+                    if (y0 + y < n) {
+                        if constexpr (E == 2) {
+                            O[0] = fmaf(wy, v[y][0], O[0]);
+                            O[1] = fmaf(wy, v[y][1], O[1]);
+                        } else {
+                            O[0] = fmaf(wy, v[y], O[0]);
+                        }
+                    }
+                }
+            }
+            M = Mn;
+        }
+    }
+    const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+    const int64_t at = (int64_t)row * a.o_st + (int64_t)h * a.o_sh + E * lane;
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+        const float y = L == 0.0f ? 0.0f : O[e] * inv;
+        if (a.out_dtype == FLOUR_DTYPE_F32)
+            static_cast<float*>(a.out)[at + e] = y;
+        else if (a.out_dtype == FLOUR_DTYPE_BF16)
+            static_cast<bf16_t*>(a.out)[at + e] = from_f32<bf16_t>(y);
+        else
+            static_cast<f16_t*>(a.out)[at + e] = from_f32<f16_t>(y);
+    }
+}
+
+int launch_ranged_merge(const RtArgs& first, const RtArgs* second, hipStream_t stream) {
+    const int64_t items = (int64_t)first.a.rows * first.a.num_heads;
+    const dim3 grid((unsigned)((items + RM_WAVES - 1) / RM_WAVES));
+    const int tt = rt_tokens(elem_bytes(first.a.dtype));
+    auto kern = first.a.head_dim == 64 ? ranged_merge_kernel<64> : ranged_merge_kernel<128>;
+    kern<<<grid, dim3(64 * RM_WAVES), 0, stream>>>(first, second ? *second : first, second != nullptr, tt);
+    return check_hip(hipGetLastError(), "attention over ranges merge launch");
+}
+
+}  // namespace flour

@@ -1,0 +1,475 @@
+// ranged_tiles_kernel.h — the kernel of ranged_tiles.h.
+//
+// An item is 128 columns = (row, query head) pairs of one kv head, in the order row * n_rep + head, so
+// any group size fills the tiles and a wave's 32 columns span few rows: the band of positions that
+// they see is narrow, and tiles outside of it are skipped wave by wave. Four waves, a column a lane
+// pair (l, l + 32); the item's positions come through LDS in tiles, double-buffered, loaded one tile ahead.
+// Two workgroups a CU, whose waves are in different phases: the matrix cores of one run beside the
+// softmax of the other.
+//
+//  * S^T = K Q^T on v_mfma_f32_32x32x16: K rows from LDS (A), Q^T in registers (B). A lane holds its
+//    column's scores at positions 8 (e / 4) + 4 (l / 32) + e % 4 of 32.
+//  * These registers, rounded to f16, are the B operand of O^T = V^T P^T as they stand, its k index
+//    running over the positions in that order. V lies in LDS row by row; the transposed A operand comes
+//    from ds_read_b64_tr_b16, which hands 16 lanes a 4 x 16 block by columns.
+//  * Softmax in the exp2 domain, with a reference maximum that may lag by 2^8.
+//  * bf16 V goes to f16 on its way to LDS: exact for 2^-17 <= |v| <= 65,504. P in f16 keeps 11 bits where
+//    bf16 would keep 8. A column that is not finite at its end, or whose root mean square is below
+//    2^-25 / 5e-4 (smaller values lost bits), has its item computed again with bf16 V and P as two bf16 parts.
+//  * A column that is not finite after that is computed again alone, position by position: a weight of 0
+//    times a V row of NaN or infinity that other columns of the tile see is NaN in the products.
+//  * fp32: v_mfma_f32_32x32x2 throughout, tiles of 32 positions.
+#pragma once
+
+#include "ranged_tiles.h"
+
+namespace flour {
+
+typedef __attribute__((ext_vector_type(4))) short s16x4;
+
+__device__ __forceinline__ u32x2 lds_read_tr16(const void* p) {
+    return __builtin_bit_cast(
+        u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                   (__attribute__((address_space(3))) s16x4*)p));
+}
+
+__device__ __forceinline__ int wave_min_i32(int x) { return -wave_max_i32(-x); }
+
+template <typename T, int D>
+__global__ __launch_bounds__(64 * RT_WAVES, 2) void ranged_tiles_kernel(RtArgs ra) {
+    constexpr bool F32 = std::is_same<T, float>::value;
+    constexpr bool BF16 = std::is_same<T, bf16_t>::value;
+    constexpr int ES = sizeof(T), ROW = D * ES;       // bytes of a K / V row
+    constexpr int TT = rt_tokens(ES), NB = TT / 32;   // positions of a tile, blocks of 32
+    constexpr int NO = D / 32;                        // 32-dim blocks of the output
+    constexpr int KP = ROW + 16;                      // LDS pitches (bytes): 16-byte reads of 16 rows,
+    constexpr int VP = F32 ? ROW + 32 : (D == 128 ? 320 : 192);  // and V's, spread over the banks
+    constexpr int LPR = ROW / 16, RPP = 64 * RT_WAVES / LPR, NP = TT / RPP;  // staging: lanes a row, rows
+                                                                            // and passes of 16 bytes a thread
+    __shared__ __attribute__((aligned(16))) unsigned char k_lds[2][TT * KP];
+    __shared__ __attribute__((aligned(16))) unsigned char v_lds[2][TT * VP];
+    const RangedAttn& a = ra.a;
+    const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, l32 = lane & 31;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int n_rep = ra.n_rep;
+
+    // ---- the item: (unit, column tile), kv head fastest (neighbouring workgroups, one an XCD, have
+    // different heads, so each XCD's L2 holds its own heads' K/V)
+    const int g = blockIdx.x % a.kv_heads, want = blockIdx.x / a.kv_heads;
+    const int units = ra.kind == RT_PREFIX ? a.num_groups : a.num_seqs;
+    int unit = -1, ctile = 0, row0 = 0, rows = 0, kv = 0;
+    {
+        int before = 0;
+        for (int u0 = 0; u0 < units; u0 += 64) {
+            const int u = u0 + lane;
+            int ur0 = 0, un = 0, ukv = 0;
+            if (u < units) {
+                if (ra.kind == RT_PREFIX) {
+                    const int s0 = max(0, min(a.group_starts[u], a.num_seqs));
+                    const int s1 = max(s0, min(a.group_starts[u + 1], a.num_seqs));
+                    ukv = max(0, min(a.shared_lens[u], a.max_shared));
+                    ur0 = a.cu ? a.cu[s0] : s0;
+                    un = ukv > 0 ? (a.cu ? a.cu[s1] : s1) - ur0 : 0;
+                } else {
+                    const RangedSeq q = ranged_seq(a, u);
+                    ur0 = q.row0, un = q.rows, ukv = q.kv;
+                }
+            }
+            const int nt = un > 0 ? (int)(((int64_t)un * n_rep + RT_COLS - 1) / RT_COLS) : 0;
+            const int incl = wave_incl_sum(nt);
+            const uint64_t hit = __ballot(before + incl > want);
+            if (hit) {
+                const int w = __builtin_ctzll(hit);
+                unit = u0 + w;
+                ctile = want - before - (__builtin_amdgcn_readlane(incl, w) - __builtin_amdgcn_readlane(nt, w));
+                row0 = __builtin_amdgcn_readlane(ur0, w);
+                rows = __builtin_amdgcn_readlane(un, w);
+                kv = __builtin_amdgcn_readlane(ukv, w);
+                break;
+            }
+            before += __builtin_amdgcn_readlane(incl, 63);
+        }
+    }
+    if (unit < 0) return;
+    const int ncols = rows * n_rep;
+    const int seq = ra.kind == RT_PREFIX ? max(0, min(a.group_starts[unit], a.num_seqs - 1)) : unit;
+    const int32_t* bt = a.block_tables + (int64_t)seq * a.max_blocks;
+
+    // ---- the lane's column, and which positions t it sees: t < hi and (t >= lo or t < sinks)
+    const int col0 = ctile * RT_COLS + 32 * wave;
+    const bool live = col0 < ncols;  // (waves past the columns only stage)
+    const int col = min(col0 + l32, ncols - 1);
+    const bool real = col0 + l32 < ncols;
+    const int row_i = col / n_rep, head = g * n_rep + (col - row_i * n_rep);
+    const int row = row0 + row_i;
+    const int sinks = ra.kind == RT_ROWS ? a.sinks : 0;
+    int hi, lo = 0, own = 0;
+    if (ra.kind == RT_PREFIX) {
+        int s = row;
+        if (a.cu) {
+            int x = 0, y = a.num_seqs;
+            while (y - x > 1) {
+                const int mid = (x + y) >> 1;
+                if (a.cu[mid] <= row)
+                    x = mid;
+                else
+                    y = mid;
+            }
+            s = x;
+        }
+        const RangedSeq q = ranged_seq(a, s);
+        hi = q.kv > 0 ? min(kv, q.kv - q.rows + (row - q.row0) + 1) : 0;
+    } else {
+        hi = kv > 0 ? kv - rows + row_i + 1 : 0;
+        if (ra.kind == RT_ROWS)
+            lo = max(0, hi - a.window);
+        else
+            lo = own = ranged_shared_len(a, ranged_group(a, seq));
+    }
+    const RtSpan sp = rt_span(ra, ra.kind, rows, kv, ctile, own, TT);
+    const int front = sp.front, from = sp.from, to = sp.to, all_tiles = sp.tiles;
+    auto tok_of = [&](int v) -> int { return sp.tok(v, TT); };
+
+    // ---- this workgroup's piece of the tiles
+    const int pieces = rt_pieces(all_tiles, ra.max_pieces, ra.piece_tiles), piece = blockIdx.y;
+    if (piece >= pieces) return;
+    const int t_begin = (int)((int64_t)all_tiles * piece / pieces);
+    const int t_end = (int)((int64_t)all_tiles * (piece + 1) / pieces);
+
+    const int min_hi = wave_min_i32(hi), max_hi = wave_max_i32(hi);
+    const int min_lo = wave_min_i32(lo), max_lo = wave_max_i32(lo);
+
+    // ---- page slots of 16-position runs, 64 at a time, one a lane
+    constexpr int UPT = TT / 16, WIN = 64 / UPT;  // runs a tile, tiles a refill
+    const int max_id = (int)(a.num_slots / a.block_size - 1);
+    const int last_run = (to - 1) & ~15;
+    auto load_slots = [&](int t0) -> uint32_t {  // byte offsets
+        const int v = t0 + lane / UPT;
+        const int tok = min(tok_of(min(v, max(all_tiles - 1, 0))) + 16 * (lane % UPT), last_run);
+        const int lb = a.block_size == 16 ? tok >> 4 : tok / a.block_size;
+        int id = bt[lb];
+        id = id < 0 ? 0 : (id > max_id ? max_id : id);  // a bad block id never leaves the pool
+        return (uint32_t)(id * a.block_size + (tok - lb * a.block_size)) * (uint32_t)ROW;
+    };
+
+    const uint32_t head_bytes = (uint32_t)(a.num_slots * ROW);
+    const __amdgpu_buffer_rsrc_t k_rsrc = __builtin_amdgcn_make_buffer_rsrc(
+        (void*)(static_cast<const char*>(a.k_pool) + (int64_t)g * a.num_slots * ROW), (short)0,
+        (int)head_bytes, BUF_DWORD3);
+    const __amdgpu_buffer_rsrc_t v_rsrc = __builtin_amdgcn_make_buffer_rsrc(
+        (void*)(static_cast<const char*>(a.v_pool) + (int64_t)g * a.num_slots * ROW), (short)0,
+        (int)head_bytes, BUF_DWORD3);
+    const int s_row = tid / LPR, s_col = (tid % LPR) * 16;  // staging: row of a pass, byte of the row
+    const int w_row = wave * (64 / LPR);                    // the wave's first row of a pass
+    u32x4 kreg[NP], vreg[NP];
+    auto load_tile = [&](uint32_t slots, int t) __attribute__((always_inline)) {
+        const int s0 = ((t - t_begin) % WIN) * UPT;
+#pragma unroll
+        for (int k = 0; k < NP; k++) {
+            const uint32_t soff = __builtin_amdgcn_readlane(slots, s0 + (k * RPP + w_row) / 16);
+            const uint32_t voff = (uint32_t)(((k * RPP + s_row) & 15) * ROW + s_col);
+            kreg[k] = __builtin_amdgcn_raw_buffer_load_b128(k_rsrc, voff, soff, 0);
+            vreg[k] = __builtin_amdgcn_raw_buffer_load_b128(v_rsrc, voff, soff, 0);
+        }
+    };
+    auto stage_tile = [&](auto exact, int t, int buf) __attribute__((always_inline)) {
+        const int tok0 = tok_of(t);
+        // positions that no column sees: no bits of theirs
+        const bool edge = tok0 + TT > to || (tok0 < from && tok0 + TT > front);
+#pragma unroll
+        for (int k = 0; k < NP; k++) {
+            const int r = k * RPP + s_row, tok = tok0 + r;
+            *reinterpret_cast<u32x4*>(&k_lds[buf][r * KP + s_col]) = kreg[k];
+            u32x4 v = vreg[k];
+            if (edge && !(tok < to && (tok >= from || tok < front))) v = u32x4{0, 0, 0, 0};
+            if constexpr (BF16 && !decltype(exact)::value)
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    v[e] = pack2<f16_t>(lo_f32<bf16_t>(v[e]), hi_f32<bf16_t>(v[e]));
+            *reinterpret_cast<u32x4*>(&v_lds[buf][r * VP + s_col]) = v;
+        }
+    };
+
+    // ---- Q^T as the B operand: dims 16 kk + 8 half .. + 7 for product kk; fp32: dims D/2 half + s for
+    // product s
+    constexpr int NQ = F32 ? D / 8 : D / 16;
+    u32x4 qb[NQ];
+    {
+        const T* q = static_cast<const T*>(a.q) + (int64_t)row * a.q_st + (int64_t)head * a.q_sh;
+#pragma unroll
+        for (int kk = 0; kk < NQ; kk++)
+            qb[kk] = live ? *reinterpret_cast<const u32x4*>(
+                                q + (F32 ? D / 2 * half + 4 * kk : 16 * kk + 8 * half))
+                          : u32x4{0, 0, 0, 0};
+    }
+
+    float m, l;
+    f32x16 acc[NO];
+    auto compute = [&](auto exact, int t, int buf) __attribute__((always_inline)) {
+        const int tok0 = tok_of(t);
+        if (!live || tok0 >= max_hi || (tok0 + TT <= min_lo && tok0 >= sinks)) return;
+        f32x16 s[NB];
+#pragma unroll
+        for (int b = 0; b < NB; b++) {
+#pragma unroll
+            for (int e = 0; e < 16; e++) s[b][e] = 0.0f;
+            const unsigned char* kr = &k_lds[buf][(32 * b + l32) * KP];
+            if constexpr (F32) {
+                f32x16 s1 = s[b];
+#pragma unroll
+                for (int kk = 0; kk < NQ; kk++) {
+                    const f32x4 x = *reinterpret_cast<const f32x4*>(kr + ROW / 2 * half + 16 * kk);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        f32x16& y = e & 1 ? s1 : s[b];
+                        y = __builtin_amdgcn_mfma_f32_32x32x2f32(x[e], __uint_as_float(qb[kk][e]), y, 0,
+                                                                 0, 0);
+                    }
+                }
+                s[b] += s1;
+            } else {
+#pragma unroll
+                for (int kk = 0; kk < NQ; kk++)
+                    s[b] = mfma32x32x16<T>(*reinterpret_cast<const u32x4*>(kr + 32 * kk + 16 * half),
+                                           qb[kk], s[b]);
+            }
+        }
+        const bool full = tok0 + TT <= min_hi && (tok0 >= max_lo || tok0 + TT <= sinks);
+        if (!full) {
+#pragma unroll
+            for (int b = 0; b < NB; b++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) {
+                    const int tok = tok0 + 32 * b + 8 * (e >> 2) + 4 * half + (e & 3);
+                    if (!(tok < hi && (tok >= lo || tok < sinks))) s[b][e] = -INFINITY;
+                }
+        }
+        float top = s[0][0];
+#pragma unroll
+        for (int b = 0; b < NB; b++)
+#pragma unroll
+            for (int e = 0; e < 16; e++)
+                if (b + e > 0) top = vmax(top, s[b][e]);
+        top = max_across_halves(top) * ra.scale_log2;
+        constexpr float LAG = F32 ? 0.0f : 8.0f;
+        const bool up = top > m + LAG;
+        if (__builtin_amdgcn_ballot_w64(up) != 0) {
+            const float m_new = up ? top : m, alpha = fast_exp2(m - m_new);
+            m = m_new;
+            l *= alpha;
+#pragma unroll
+            for (int o = 0; o < NO; o++) acc[o] *= alpha;
+        }
+#pragma unroll
+        for (int b = 0; b < NB; b++) {
+            float p[16];
+#pragma unroll
+            for (int e = 0; e < 16; e++) p[e] = fast_exp2(fmaf(s[b][e], ra.scale_log2, -m));
+            if constexpr (F32) {
+                float x = 0.0f, y = 0.0f;
+#pragma unroll
+                for (int e = 0; e < 16; e += 2) x += p[e], y += p[e + 1];
+                l += x + y;
+#pragma unroll
+                for (int o = 0; o < NO; o++) {
+                    // (the tile's sum by itself, then added: a long context's sum is one of sums)
+                    f32x16 z;
+#pragma unroll
+                    for (int e = 0; e < 16; e++) z[e] = 0.0f;
+#pragma unroll
+                    for (int e = 0; e < 16; e++)
+                        z = __builtin_amdgcn_mfma_f32_32x32x2f32(
+                            *reinterpret_cast<const float*>(
+                                &v_lds[buf][(32 * b + 8 * (e >> 2) + 4 * half + (e & 3)) * VP +
+                                            4 * (32 * o + l32)]),
+                            p[e], z, 0, 0, 0);
+                    acc[o] += z;
+                }
+            } else {
+                typedef typename std::conditional<BF16 && !decltype(exact)::value, f16_t, T>::type TP;
+                constexpr bool SPLIT = BF16 && decltype(exact)::value;
+                u32x4 ph[2], pl[2];
+#pragma unroll
+                for (int x = 0; x < 2; x++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const float p0 = p[8 * x + 2 * e], p1 = p[8 * x + 2 * e + 1];
+                        const uint32_t hi16 = pack2<TP>(p0, p1);
+                        ph[x][e] = hi16;
+                        if constexpr (SPLIT) {
+                            pl[x][e] = pack2<TP>(p0 - lo_f32<TP>(hi16), p1 - hi_f32<TP>(hi16));
+                            l += p0 + p1;
+                        } else {  // (the rounded weights that enter the product)
+                            l = __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, hi16), f16x2{1, 1}, l, false);
+                        }
+                    }
+                // V^T: 16 lanes read rows 4 half .. + 3 of 16 dims, and the rows 8 behind
+                const unsigned char* vr =
+                    &v_lds[buf][(32 * b + 4 * half + ((lane >> 2) & 3)) * VP + 32 * ((lane >> 4) & 1) +
+                                8 * (lane & 3)];
+#pragma unroll
+                for (int x = 0; x < 2; x++)
+#pragma unroll
+                    for (int o = 0; o < NO; o++) {
+                        const u32x2 v0 = lds_read_tr16(vr + 16 * x * VP + 64 * o);
+                        const u32x2 v1 = lds_read_tr16(vr + (16 * x + 8) * VP + 64 * o);
+                        const u32x4 A = {v0[0], v0[1], v1[0], v1[1]};
+                        acc[o] = mfma32x32x16<TP>(A, ph[x], acc[o]);
+                        if constexpr (SPLIT) acc[o] = mfma32x32x16<TP>(A, pl[x], acc[o]);
+                    }
+            }
+        }
+    };
+
+    auto pass = [&](auto exact) __attribute__((always_inline)) {
+        m = DEC_M0, l = 0.0f;
+#pragma unroll
+        for (int o = 0; o < NO; o++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) acc[o][e] = 0.0f;
+        if (t_begin >= t_end) return;
+        uint32_t slots = load_slots(t_begin), next = slots;
+        if (t_begin + WIN < t_end) next = load_slots(t_begin + WIN);
+        load_tile(slots, t_begin);
+        stage_tile(exact, t_begin, 0);
+        __syncthreads();
+        for (int t = t_begin; t < t_end; t++) {
+            const int buf = (t - t_begin) & 1;
+            if (t + 1 < t_end) {
+                if ((t + 1 - t_begin) % WIN == 0) {
+                    slots = next;
+                    if (t + 1 + WIN < t_end) next = load_slots(t + 1 + WIN);
+                }
+                load_tile(slots, t + 1);
+            }
+            compute(exact, t, buf);
+            if (t + 1 < t_end) stage_tile(exact, t + 1, buf ^ 1);
+            __syncthreads();
+        }
+        l = sum_across_halves(l);
+    };
+    using yes = std::integral_constant<bool, true>;
+    using no = std::integral_constant<bool, false>;
+    pass(no{});
+
+    // ---- columns to compute again
+    auto finite = [&]() -> bool {
+        float x = l - l;  // 0, or NaN where it is not finite
+#pragma unroll
+        for (int o = 0; o < NO; o++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) x = fmaf(acc[o][e], 0.0f, x);
+        return x == 0.0f;
+    };
+    if constexpr (BF16) {
+        float sq = 0.0f;
+#pragma unroll
+        for (int o = 0; o < NO; o++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) sq = fmaf(acc[o][e], acc[o][e], sq);
+        sq = sum_across_halves(sq);
+        const float least = 2.0f / (32768.0f * 1024.0f * 5e-4f * 2.0f);  // 2^-25 / 5e-4
+        const bool again = live && real && l != 0.0f && !(sq >= D * least * least * l * l && finite());
+        if (__syncthreads_or(again)) pass(yes{});
+    }
+
+    // ---- out: a lane holds dims 32 o + 8 (e / 4) + 4 half + e % 4 of its column
+    const bool final_out = ra.finals && pieces == 1;
+    const int64_t slot = ((int64_t)row * a.num_heads + head) * ra.max_pieces + piece;
+    const int64_t out_at = (int64_t)row * a.o_st + (int64_t)head * a.o_sh;
+    const bool bad = live && real && !finite();
+    if (live && real && !bad) {
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+        for (int o = 0; o < NO; o++)
+#pragma unroll
+            for (int e = 0; e < 16; e += 4) {
+                const int d = 32 * o + 2 * e + 4 * half;
+                float v[4];
+#pragma unroll
+                for (int x = 0; x < 4; x++) v[x] = final_out ? acc[o][e + x] * inv : acc[o][e + x];
+                if (final_out)
+                    store_run<4>(a.out, a.out_dtype, out_at + d, v);
+                else
+                    *reinterpret_cast<f32x4*>(ra.p_o + slot * D + d) = f32x4{v[0], v[1], v[2], v[3]};
+            }
+        if (!final_out && half == 0) {
+            ra.p_ml[2 * slot] = m;
+            ra.p_ml[2 * slot + 1] = l;
+        }
+    }
+
+    // ---- columns with numbers that are not finite, one at a time: 64 positions at once, one a lane, then
+    // a lane's D / 64 dims over those that the column sees
+    uint64_t todo = __ballot(bad);
+    todo = (todo | (todo >> 32)) & 0xffffffffu;
+    while (todo) {
+        const int c = __builtin_ctzll(todo);
+        todo &= todo - 1;
+        const int c_row = __builtin_amdgcn_readlane(row, c), c_head = __builtin_amdgcn_readlane(head, c);
+        const int c_hi = __builtin_amdgcn_readlane(hi, c), c_lo = __builtin_amdgcn_readlane(lo, c);
+        const T* q = static_cast<const T*>(a.q) + (int64_t)c_row * a.q_st + (int64_t)c_head * a.q_sh;
+        const T* kp = static_cast<const T*>(a.k_pool) + (int64_t)g * a.num_slots * D;
+        const T* vp = static_cast<const T*>(a.v_pool) + (int64_t)g * a.num_slots * D;
+        float cm = DEC_M0, cl = 0.0f, co[D / 64] = {};
+        for (int t = t_begin; t < t_end; t++) {
+            const int tok = tok_of(t) + lane;
+            const bool sees = lane < TT && tok < c_hi && (tok >= c_lo || tok < sinks);
+            float sc = -INFINITY;
+            int slot_j = 0;
+            if (sees) {
+                const int lb = tok / a.block_size;
+                int id = bt[lb];
+                id = id < 0 ? 0 : (id > max_id ? max_id : id);
+                slot_j = id * a.block_size + (tok - lb * a.block_size);
+                float dot = 0.0f;
+                for (int d = 0; d < D; d++) dot = fmaf(to_f32(q[d]), to_f32(kp[(int64_t)slot_j * D + d]), dot);
+                sc = dot * ra.scale_log2;
+            }
+            const float m_new = fmaxf(cm, wave_max(sc)), alpha = fast_exp2(cm - m_new);
+            const float p = sees ? fast_exp2(sc - m_new) : 0.0f;
+            cl = cl * alpha + wave_sum(p);
+#pragma unroll
+            for (int x = 0; x < D / 64; x++) co[x] *= alpha;
+            for (uint64_t left = __ballot(sees); left; left &= left - 1) {
+                const int j = __builtin_ctzll(left);
+                const float pj = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(p), j));
+                const int64_t v_at = (int64_t)__builtin_amdgcn_readlane(slot_j, j) * D + D / 64 * lane;
+#pragma unroll
+                for (int x = 0; x < D / 64; x++) co[x] = fmaf(pj, to_f32(vp[v_at + x]), co[x]);
+            }
+            cm = m_new;
+        }
+        const int64_t c_slot = ((int64_t)c_row * a.num_heads + c_head) * ra.max_pieces + piece;
+        const float inv = cl == 0.0f ? 0.0f : 1.0f / cl;
+#pragma unroll
+        for (int x = 0; x < D / 64; x++) {
+            const int d = D / 64 * lane + x;
+            if (final_out) {
+                const int64_t at = (int64_t)c_row * a.o_st + (int64_t)c_head * a.o_sh + d;
+                const float y = cl == 0.0f ? 0.0f : co[x] * inv;
+                if (a.out_dtype == FLOUR_DTYPE_F32)
+                    static_cast<float*>(a.out)[at] = y;
+                else if (a.out_dtype == FLOUR_DTYPE_BF16)
+                    static_cast<bf16_t*>(a.out)[at] = from_f32<bf16_t>(y);
+                else
+                    static_cast<f16_t*>(a.out)[at] = from_f32<f16_t>(y);
+            } else {
+                ra.p_o[c_slot * D + d] = co[x];
+            }
+        }
+        if (!final_out && lane == 0) {
+            ra.p_ml[2 * c_slot] = cm;
+            ra.p_ml[2 * c_slot + 1] = cl;
+        }
+    }
+}
+
+template <typename T>
+static int launch_ranged_tiles(const RtArgs& r, int items, hipStream_t stream) {
+    auto kern = r.a.head_dim == 64 ? ranged_tiles_kernel<T, 64> : ranged_tiles_kernel<T, 128>;
+    kern<<<dim3(items, r.max_pieces), dim3(64 * RT_WAVES), 0, stream>>>(r);
+    return check_hip(hipGetLastError(), "attention over ranges launch");
+}
+
+}  // namespace flour
