@@ -286,6 +286,15 @@ __device__ __forceinline__ void store_run(void* out, int out_dtype, int64_t idx,
     }
 }
 
+__device__ __forceinline__ void store_1(void* out, int out_dtype, int64_t idx, float v) {
+    if (out_dtype == FLOUR_DTYPE_F32)
+        static_cast<float*>(out)[idx] = v;
+    else if (out_dtype == FLOUR_DTYPE_BF16)
+        static_cast<bf16_t*>(out)[idx] = from_f32<bf16_t>(v);
+    else
+        static_cast<f16_t*>(out)[idx] = from_f32<f16_t>(v);
+}
+
 // The place of token t of 16 in a V^T row: bits 2 and 3 swapped, the order in which the score
 // registers of S^T = K Q^T hold a row's positions.
 __device__ __forceinline__ int sigma16(int t) {

@@ -38,6 +38,26 @@ __device__ __forceinline__ RangedSeq ranged_seq(const RangedAttn& a, int s) {
     return RangedSeq{r0, max(n, 0), kv >= n && kv > 0 ? kv : 0};
 }
 
+// The group of sequence s (-1: none): the last one that starts at or before it, if it has not ended.
+__device__ __forceinline__ int ranged_group(const int32_t* starts, int num_groups, int s) {
+    if (num_groups == 0 || starts[0] > s) return -1;
+    int lo = 0, hi = num_groups;  // the last g with starts[g] <= s
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (starts[mid] <= s)
+            lo = mid;
+        else
+            hi = mid;
+    }
+    return s < starts[lo + 1] ? lo : -1;
+}
+__device__ __forceinline__ int ranged_shared_len(const int32_t* shared_lens, int max_shared, int g) {
+    return g < 0 ? 0 : max(0, min(shared_lens[g], max_shared));
+}
+__device__ __forceinline__ int ranged_shared_of(const RangedAttn& a, int s) {
+    return ranged_shared_len(a.shared_lens, a.max_shared, ranged_group(a.group_starts, a.num_groups, s));
+}
+
 // Takes every shape (ranged_generic.hip).
 int launch_ranged_generic(const RangedAttn& a, hipStream_t stream);
 

@@ -39,6 +39,54 @@ static bool check_shape(const char* what, const RangedAttn& a) {
 
 static size_t up256(size_t x) { return (x + 255) & ~(size_t)255; }
 
+// ---- the decode stream
+static bool stream_fits(int batch, int num_heads, int kv_heads, int head_dim) {
+    return (head_dim == 64 || head_dim == 128) && num_heads / kv_heads <= 16 &&
+           batch <= DEC_MAX_BATCH && num_heads <= 65535;
+}
+
+static bool stream_takes(const RangedAttn& a) {
+    const int es = elem_bytes(a.dtype);
+    return stream_fits(a.num_seqs, a.num_heads, a.kv_heads, a.head_dim) && a.block_size % 16 == 0 &&
+           a.num_slots * a.head_dim * es <= (int64_t)0x7fffffff &&
+           (((uintptr_t)a.q | (uintptr_t)a.out | (uintptr_t)a.k_pool | (uintptr_t)a.v_pool) & 15) == 0;
+}
+
+// Its workspace, behind prefixes with the places of pairs that one wave finishes.
+static size_t stream_bytes(int batch, int num_heads, int kv_heads, int head_dim, bool own) {
+    const size_t pairs = (size_t)batch * num_heads;
+    return decode_ws_bytes(decode_workgroups(FLOUR_DTYPE_F32), num_heads / kv_heads, head_dim, batch) +
+           (own ? up256(pairs * 2 * sizeof(float)) + up256(pairs * head_dim * sizeof(float)) : 0);
+}
+
+static RangedStream stream_args(const RangedAttn& a, bool own, char* ws) {
+    const int n_rep = a.num_heads / a.kv_heads, nwg = decode_workgroups(a.dtype);
+    RangedStream st{};
+    st.ws = decode_ws_at(ws, nwg, n_rep, a.head_dim);
+    st.ws.rng.window = a.window, st.ws.rng.sinks = a.sinks, st.ws.rng.out_dtype = a.out_dtype;
+    if (own) {
+        const size_t pairs = (size_t)a.num_seqs * a.num_heads;
+        char* at = ws + stream_bytes(a.num_seqs, a.num_heads, a.kv_heads, a.head_dim, false);
+        st.ws.rng.group_starts = a.group_starts, st.ws.rng.shared_lens = a.shared_lens;
+        st.ws.rng.num_groups = a.num_groups, st.ws.rng.max_shared = a.max_shared;
+        st.ws.rng.pair_ml = reinterpret_cast<float*>(at);
+        st.ws.rng.pair_o = reinterpret_cast<float*>(at + up256(pairs * 2 * sizeof(float)));
+    }
+    // no more waves than ranges (range_count) for the longest visible parts
+    const int64_t chunk = dec_chunk(elem_bytes(a.dtype));
+    const int64_t span = std::min<int64_t>(a.max_kv, (int64_t)a.window + a.sinks + 2 * chunk);
+    const int64_t half = (int64_t)a.num_seqs * a.kv_heads * ((span + chunk - 1) / chunk) / 2;
+    st.grid = (int)std::max<int64_t>(1, std::min<int64_t>(half, nwg));
+    return st;
+}
+
+static int launch_stream(const RangedAttn& a, const RangedStream& st, hipStream_t stream) {
+    auto launch = a.dtype == FLOUR_DTYPE_F32    ? launch_ranged_decode_f32
+                  : a.dtype == FLOUR_DTYPE_BF16 ? launch_ranged_decode_bf16
+                                                : launch_ranged_decode_f16;
+    return launch(a, st, stream);
+}
+
 // ---- the tile kernel
 // What the shape says of it; a call's tensors can still refuse it (tiles_take).
 static bool tiles_fit(int64_t rows, int num_heads, int kv_heads, int head_dim) {
@@ -144,22 +192,34 @@ static int ranged_call(const char* what, const RangedAttn& a, bool shared, void*
                   workspace_bytes, workspace);
         return FLOUR_ERR_WORKSPACE;
     }
-    if (!tiles_take(a) || (!a.cu && !shared)) return launch_ranged_generic(a, stream);
     char* ws = static_cast<char*>(workspace);
+    const bool step = !a.cu && stream_takes(a);
+    if (step && (!shared || a.num_groups == 0 || a.max_shared == 0))
+        return launch_stream(a, stream_args(a, false, ws), stream);
+    if (!tiles_take(a)) return launch_ranged_generic(a, stream);
     if (!shared || a.num_groups == 0 || a.max_shared == 0) {
         const TilePlan p = rows_plan(a.num_seqs, a.max_rows, a.rows, a.num_heads, a.kv_heads, a.head_dim,
                                      a.max_kv, a.window, a.sinks, a.dtype);
         const RtArgs r = tile_args(a, RT_ROWS, p, true, ws);
         rc = launch_tiles(r, p, stream);
-        return rc != FLOUR_OK || p.max_pieces == 1 ? rc : launch_ranged_merge(r, nullptr, stream);
+        return rc != FLOUR_OK || p.max_pieces == 1 ? rc : launch_ranged_merge(r, nullptr, nullptr, stream);
     }
     const SharedPlan p = shared_plan(a.num_seqs, a.num_groups, a.max_rows, a.rows, a.num_heads, a.kv_heads,
                                      a.head_dim, a.max_kv, a.max_shared, a.dtype);
+    if (step) {
+        const RangedStream st = stream_args(a, true, ws);
+        const RtArgs prefix = tile_args(
+            a, RT_PREFIX, p.prefix, false,
+            ws + stream_bytes(a.num_seqs, a.num_heads, a.kv_heads, a.head_dim, true));
+        rc = launch_tiles(prefix, p.prefix, stream);
+        if (rc == FLOUR_OK) rc = launch_stream(a, st, stream);
+        return rc != FLOUR_OK ? rc : launch_ranged_merge(prefix, nullptr, &st, stream);
+    }
     const RtArgs own = tile_args(a, RT_OWN, p.own, false, ws);
     const RtArgs prefix = tile_args(a, RT_PREFIX, p.prefix, false, ws + p.own.bytes);
     rc = launch_tiles(prefix, p.prefix, stream);
     if (rc == FLOUR_OK) rc = launch_tiles(own, p.own, stream);
-    return rc != FLOUR_OK ? rc : launch_ranged_merge(own, &prefix, stream);
+    return rc != FLOUR_OK ? rc : launch_ranged_merge(own, &prefix, nullptr, stream);
 }
 
 // A decode step's part of a call: one row a sequence, packed rows of all heads.
@@ -222,10 +282,13 @@ extern "C" int flour_hip_window_workspace_size(int num_seqs, int max_seqlen_q, i
         set_error("window_workspace_size: window %d with %d sinks", window, sinks);
         return FLOUR_ERR_INVALID_ARGUMENT;
     }
-    *bytes = !tiles_fit(total_q, num_heads, kv_heads, head_dim)
-                 ? 0
-                 : rows_plan(num_seqs, max_seqlen_q, total_q, num_heads, kv_heads, head_dim, max_kv_len,
-                             window, sinks, dtype).bytes;
+    size_t n = 0;
+    if (tiles_fit(total_q, num_heads, kv_heads, head_dim))
+        n = rows_plan(num_seqs, max_seqlen_q, total_q, num_heads, kv_heads, head_dim, max_kv_len, window,
+                      sinks, dtype).bytes;
+    if (total_q == num_seqs && stream_fits(num_seqs, num_heads, kv_heads, head_dim))  // a decode step
+        n = std::max(n, stream_bytes(num_seqs, num_heads, kv_heads, head_dim, false));
+    *bytes = n;
     return FLOUR_OK;
 }
 
@@ -248,7 +311,10 @@ extern "C" int flour_hip_shared_workspace_size(int num_seqs, int num_groups, int
                                      head_dim, max_kv_len, max_shared_len, dtype);
     const TilePlan alone = rows_plan(num_seqs, max_seqlen_q, total_q, num_heads, kv_heads, head_dim,
                                      max_kv_len, 0x7fffffff, 0, dtype);
-    *bytes = std::max(p.prefix.bytes + p.own.bytes, alone.bytes);
+    size_t n = std::max(p.prefix.bytes + p.own.bytes, alone.bytes);
+    if (total_q == num_seqs && stream_fits(num_seqs, num_heads, kv_heads, head_dim))
+        n = std::max(n, p.prefix.bytes + stream_bytes(num_seqs, num_heads, kv_heads, head_dim, true));
+    *bytes = n;
     return FLOUR_OK;
 }
 

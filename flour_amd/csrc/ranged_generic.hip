@@ -106,12 +106,7 @@ __global__ __launch_bounds__(RG_THREADS) void ranged_generic_kernel(RangedAttn a
         if (d < head_dim) {
             const int64_t to = r * a.o_st + h * a.o_sh + d;
             const float y = l == 0.0f ? 0.0f : acc[e] * inv;
-            if (a.out_dtype == FLOUR_DTYPE_F32)
-                static_cast<float*>(a.out)[to] = y;
-            else if (a.out_dtype == FLOUR_DTYPE_BF16)
-                static_cast<bf16_t*>(a.out)[to] = from_f32<bf16_t>(y);
-            else
-                static_cast<f16_t*>(a.out)[to] = from_f32<f16_t>(y);
+            store_1(a.out, a.out_dtype, to, y);
         }
     }
 }

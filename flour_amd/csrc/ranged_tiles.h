@@ -9,6 +9,7 @@
 
 #include "decode_ranges.h"
 #include "ranged.h"
+#include "ranged_decode.h"
 
 namespace flour {
 
@@ -41,23 +42,6 @@ __host__ __device__ constexpr int rt_tokens(int elem_bytes) { return elem_bytes 
 __host__ __device__ __forceinline__ int rt_pieces(int tiles, int max_pieces, int piece_tiles) {
     const int n = (tiles + piece_tiles - 1) / piece_tiles;
     return n < 1 ? 1 : (n < max_pieces ? n : max_pieces);
-}
-
-// The group of sequence s (-1: none): the last one that starts at or before it and has not ended.
-__device__ __forceinline__ int ranged_group(const RangedAttn& a, int s) {
-    if (a.num_groups == 0 || a.group_starts[0] > s) return -1;
-    int lo = 0, hi = a.num_groups;  // the last g with starts[g] <= s
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (a.group_starts[mid] <= s)
-            lo = mid;
-        else
-            hi = mid;
-    }
-    return s < a.group_starts[lo + 1] ? lo : -1;
-}
-__device__ __forceinline__ int ranged_shared_len(const RangedAttn& a, int g) {
-    return g < 0 ? 0 : max(0, min(a.shared_lens[g], a.max_shared));
 }
 
 // The positions that a column tile of a unit goes through: [0, front) and [from, to), the second behind the
@@ -93,9 +77,10 @@ __device__ __forceinline__ RtSpan rt_span(const RtArgs& ra, int kind, int rows, 
     return s;
 }
 
-// Joins pieces: of `first`, and (or null) of `second`, whose launch had the same rows. Where first.finals
-// is set, rows of one piece are left alone.
-int launch_ranged_merge(const RtArgs& first, const RtArgs* second, hipStream_t stream);
+// Joins pieces: of `first`, and (or null) of `second`, whose launch had the same rows, or of a step's
+// stream. Where first.finals is set, rows of one piece are left alone.
+int launch_ranged_merge(const RtArgs& first, const RtArgs* second, const RangedStream* st,
+                        hipStream_t stream);
 
 int launch_ranged_tiles_f32(const RtArgs& r, int items, hipStream_t stream);
 int launch_ranged_tiles_bf16(const RtArgs& r, int items, hipStream_t stream);

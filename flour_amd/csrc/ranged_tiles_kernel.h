@@ -124,7 +124,7 @@ __global__ __launch_bounds__(64 * RT_WAVES, 2) void ranged_tiles_kernel(RtArgs r
         if (ra.kind == RT_ROWS)
             lo = max(0, hi - a.window);
         else
-            lo = own = ranged_shared_len(a, ranged_group(a, seq));
+            lo = own = ranged_shared_of(a, seq);
     }
     const RtSpan sp = rt_span(ra, ra.kind, rows, kv, ctile, own, TT);
     const int front = sp.front, from = sp.from, to = sp.to, all_tiles = sp.tiles;
@@ -448,12 +448,7 @@ __global__ __launch_bounds__(64 * RT_WAVES, 2) void ranged_tiles_kernel(RtArgs r
             if (final_out) {
                 const int64_t at = (int64_t)c_row * a.o_st + (int64_t)c_head * a.o_sh + d;
                 const float y = cl == 0.0f ? 0.0f : co[x] * inv;
-                if (a.out_dtype == FLOUR_DTYPE_F32)
-                    static_cast<float*>(a.out)[at] = y;
-                else if (a.out_dtype == FLOUR_DTYPE_BF16)
-                    static_cast<bf16_t*>(a.out)[at] = from_f32<bf16_t>(y);
-                else
-                    static_cast<f16_t*>(a.out)[at] = from_f32<f16_t>(y);
+                store_1(a.out, a.out_dtype, at, y);
             } else {
                 ra.p_o[c_slot * D + d] = co[x];
             }
