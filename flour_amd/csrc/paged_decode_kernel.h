@@ -39,17 +39,11 @@ static_assert(DEC_WAVES_PER_CU_F32 >= DEC_WAVES_PER_CU, "the workspace is sized 
 __host__ __device__ constexpr int dec_kpitch(int d, int elem_bytes) { return d * elem_bytes + 16; }
 
 // A step that looks at parts of its contexts (the kernels' RNG instantiations): the first `sinks` and the
-// last `window` positions, or with groups what lies behind the shared prefix of the sequence's group. The
-// list of chunks holds those that have visible positions: of the sinks, and from the last multiple of 16
-// before the window (or behind the prefix) on.
+// last `window` positions. The list of chunks holds those that have visible positions: of the sinks, and
+// from the last multiple of 16 before the window on.
 struct DecodeRange {
     int window, sinks;
-    const int32_t *group_starts, *shared_lens;  // null: a window
-    int num_groups, max_shared;
     int out_dtype;  // of AnyOut outputs
-    // Behind a prefix a pair that one wave finishes leaves (max, sum) and accumulator too, at slot b *
-    // num_heads + head.
-    float *pair_ml, *pair_o;
 };
 // The output's type is a field of the call.
 struct AnyOut {
@@ -60,13 +54,16 @@ struct AnyOut {
 template <int CHUNK>
 struct DecodePart {
     int ctx, lo, front;
-    __device__ __forceinline__ DecodePart(int ctx_, int lo_, int sinks)
-        : ctx(ctx_), lo(lo_), front(lo_ > 0 ? min(sinks, lo_) : 0) {}
+    __device__ __forceinline__ DecodePart(int ctx_, const DecodeRange& r) : ctx(ctx_) {
+        lo = max(0, ctx - r.window);
+        if (lo <= r.sinks) lo = 0;
+        front = lo > 0 ? r.sinks : 0;
+    }
     __device__ __forceinline__ int front_chunks() const { return (front + CHUNK - 1) / CHUNK; }
     __device__ __forceinline__ int base() const { return max(lo & ~15, front_chunks() * CHUNK); }
     __device__ __forceinline__ int chunks() const {
         const int b = base();
-        return ctx <= 0 || ctx <= lo ? 0 : front_chunks() + (ctx > b ? (ctx - b + CHUNK - 1) / CHUNK : 0);
+        return ctx <= 0 ? 0 : front_chunks() + (ctx > b ? (ctx - b + CHUNK - 1) / CHUNK : 0);
     }
     __device__ __forceinline__ int tok(int c) const {  // the first position of chunk c
         const int f = front_chunks();
@@ -175,34 +172,16 @@ __global__ __launch_bounds__(64, 2) void paged_decode_mfma_kernel(
     // is a ballot and scalar lane reads: no LDS search, no second read of a context length.
     // (16-token pages: with other page sizes those two registers spill)
     const bool in_lanes = BS16 && batch <= 64;
-    // RNG: where sequence b's positions start behind the sinks (0: all of them are visible)
     const DecodeRange& rng = ws.rng;
-    int* const lds_lo = pre + batch + 1;
-    auto part_lo = [&](int b, int ctx) -> int {
-        if (rng.group_starts)
-            return ranged_shared_len(rng.shared_lens, rng.max_shared,
-                                     ranged_group(rng.group_starts, rng.num_groups, b));
-        const int lo = max(0, ctx - rng.window);
-        return lo <= rng.sinks ? 0 : lo;
+    auto part = [&](int ctx) { return DecodePart<CHUNK>(ctx, rng); };
+    auto chunks_of = [&](int ctx) -> int {
+        if constexpr (RNG) return part(min(ctx, max_ctx)).chunks();
+        return decode_chunks<CHUNK>(ctx, max_ctx);
     };
-    auto part = [&](int ctx, int lo) { return DecodePart<CHUNK>(ctx, lo, rng.sinks); };
-    int my_ctx = 0, my_pre = 0, my_lo = 0, all_chunks;
+    int my_ctx = 0, my_pre = 0, all_chunks;
     if (in_lanes) {
         my_ctx = lane < batch ? min(context_lens[lane], max_ctx) : 0;
-        if constexpr (RNG) {
-            if (rng.group_starts && rng.num_groups <= 64) {
-                // one group a lane; then every group's range in turn (fewer steps of memory than a search)
-                const bool on = lane < rng.num_groups;
-                const int st = on ? rng.group_starts[lane] : 0, en = on ? rng.group_starts[lane + 1] : 0;
-                const int len = on ? ranged_shared_len(rng.shared_lens, rng.max_shared, lane) : 0;
-                for (int x = 0; x < rng.num_groups; x++)
-                    if (lane >= __builtin_amdgcn_readlane(st, x) && lane < __builtin_amdgcn_readlane(en, x))
-                        my_lo = __builtin_amdgcn_readlane(len, x);
-            } else if (lane < batch) {
-                my_lo = part_lo(lane, my_ctx);
-            }
-        }
-        const int n = RNG ? part(my_ctx, my_lo).chunks() : decode_chunks<CHUNK>(my_ctx, max_ctx);
+        const int n = chunks_of(my_ctx);
         const int incl = wave_incl_sum(n);
         my_pre = incl - n;
         all_chunks = __builtin_amdgcn_readlane(incl, 63);
@@ -220,15 +199,7 @@ __global__ __launch_bounds__(64, 2) void paged_decode_mfma_kernel(
         int local = 0;
         for (int i = 0; i < per; i++) {
             const int b = lane * per + i;
-            if constexpr (RNG) {
-                if (b < batch) {
-                    const int ctx = min(context_lens[b], max_ctx), lo = part_lo(b, ctx);
-                    lds_lo[b] = lo;
-                    local += part(ctx, lo).chunks();
-                }
-            } else {
-                if (b < batch) local += decode_chunks<CHUNK>(context_lens[b], max_ctx);
-            }
+            if (b < batch) local += chunks_of(context_lens[b]);
         }
         const int incl = wave_incl_sum(local);
         int run = incl - local;
@@ -236,10 +207,7 @@ __global__ __launch_bounds__(64, 2) void paged_decode_mfma_kernel(
             const int b = lane * per + i;
             if (b < batch) {
                 pre[b] = run;
-                if constexpr (RNG)
-                    run += part(min(context_lens[b], max_ctx), lds_lo[b]).chunks();
-                else
-                    run += decode_chunks<CHUNK>(context_lens[b], max_ctx);
+                run += chunks_of(context_lens[b]);
             }
         }
         if (lane == 63) pre[batch] = incl;
@@ -284,8 +252,7 @@ __global__ __launch_bounds__(64, 2) void paged_decode_mfma_kernel(
     // The wave's range is a stream of segments: up to DEC_SEG consecutive chunks of one
     // (sequence, kv head) pair. Consecutive segments of the same pair form one piece.
     struct Seg {
-        int b, g, cb, ce, nch, tok_end;
-        int lo;  // RNG (tok_end is the context's)
+        int b, g, cb, ce, nch, tok_end;  // RNG: tok_end is the context's
     };
     auto seg_at = [&](int at) -> Seg {
         const int64_t x = lo + at;
@@ -296,12 +263,7 @@ __global__ __launch_bounds__(64, 2) void paged_decode_mfma_kernel(
             sg.b = __popcll(le) - 1;
             before = __builtin_amdgcn_readlane(my_pre, sg.b);
             ctx = __builtin_amdgcn_readlane(my_ctx, sg.b);
-            if constexpr (RNG) {
-                sg.lo = __builtin_amdgcn_readlane(my_lo, sg.b);
-                sg.nch = part(ctx, sg.lo).chunks();
-            } else {
-                sg.nch = decode_chunks<CHUNK>(ctx, max_ctx);
-            }
+            sg.nch = chunks_of(ctx);
         } else {
             int l0 = 0, h0 = batch;
             while (h0 - l0 > 1) {
@@ -315,10 +277,7 @@ __global__ __launch_bounds__(64, 2) void paged_decode_mfma_kernel(
             before = __builtin_amdgcn_readfirstlane(pre[l0]);
             sg.nch = __builtin_amdgcn_readfirstlane(pre[l0 + 1]) - before;
             ctx = min(context_lens[sg.b], max_ctx);
-            if constexpr (RNG) {
-                ctx = __builtin_amdgcn_readfirstlane(ctx);
-                sg.lo = __builtin_amdgcn_readfirstlane(lds_lo[l0]);
-            }
+            if constexpr (RNG) ctx = __builtin_amdgcn_readfirstlane(ctx);
         }
         const int64_t rel = x - (int64_t)kv_heads * before;
         sg.g = __builtin_amdgcn_readfirstlane(narrow ? (int)((uint32_t)rel / (uint32_t)sg.nch)
@@ -343,7 +302,7 @@ __global__ __launch_bounds__(64, 2) void paged_decode_mfma_kernel(
         const int32_t* bt = block_tables + (int64_t)sg.b * max_blocks;
         const int last_tile_tok0 = ((sg.tok_end - 1) >> 4) << 4;
         int first = sg.cb * CHUNK + lane * 16;
-        if constexpr (RNG) first = part(sg.tok_end, sg.lo).tok(sg.cb + lane / TILES) + lane % TILES * 16;
+        if constexpr (RNG) first = part(sg.tok_end).tok(sg.cb + lane / TILES) + lane % TILES * 16;
         const int tok0 = min(first, last_tile_tok0);
         const int lb = BS16 ? (tok0 >> 4) : tok0 / block_size;
         return Slots{bt[lb], BS16 ? 0 : tok0 - lb * block_size};
@@ -406,12 +365,13 @@ __global__ __launch_bounds__(64, 2) void paged_decode_mfma_kernel(
 #pragma unroll
     for (int nn = 0; nn < NV; nn++) acc[nn] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 
-    auto compute_chunk = [&](int c, int tok_end, int tok_lo, Ld (*ka)[4], Ld (*va)[4]) {
-        int tok0 = c * CHUNK, front = 0;
+    auto compute_chunk = [&](int c, int tok_end, Ld (*ka)[4], Ld (*va)[4]) {
+        int tok0 = c * CHUNK, tok_lo = 0, front = 0;
         bool full = tok0 + CHUNK <= tok_end;
         if constexpr (RNG) {
-            const DecodePart<CHUNK> pt = part(tok_end, tok_lo);
+            const DecodePart<CHUNK> pt = part(tok_end);
             tok0 = pt.tok(c);
+            tok_lo = pt.lo;
             front = pt.front;
             full = tok0 + CHUNK <= tok_end && (tok0 >= tok_lo || tok0 + CHUNK <= front);
         }
@@ -565,20 +525,7 @@ __global__ __launch_bounds__(64, 2) void paged_decode_mfma_kernel(
         if (lc < n_rep) {
             // F32: undefined sums give zero rows (RNG hands them on)
             constexpr bool CLEAR = F32 && !RNG;
-            if (RNG && complete && rng.group_starts) {
-                const int64_t pidx = (int64_t)b * num_heads + (int64_t)g * n_rep + lc;
-                float* o = rng.pair_o + pidx * D + (F32 ? 16 : D / 4) * lgo;
-#pragma unroll
-                for (int r = 0; r < 4; r++)
-#pragma unroll
-                    for (int h4 = 0; h4 < NV; h4 += 4)
-                        *reinterpret_cast<f32x4*>(o + (F32 ? 16 * h4 + 4 * r : NV * r + h4)) =
-                            f32x4{acc[h4][r], acc[h4 + 1][r], acc[h4 + 2][r], acc[h4 + 3][r]};
-                if (lg == 0) {
-                    rng.pair_ml[2 * pidx] = m;
-                    rng.pair_ml[2 * pidx + 1] = lsum;
-                }
-            } else if (complete) {  // whole pair in this range: final output
+            if (complete) {  // whole pair in this range: final output
                 if constexpr (WTS)
                     if (lg == 0) {
                         float* ml = ws.row_ml + 2 * ((int64_t)b * num_heads + (int64_t)g * n_rep + lc);
@@ -772,7 +719,7 @@ __global__ __launch_bounds__(64, 2) void paged_decode_mfma_kernel(
             const int ptile = in_cur ? TILES * (c + 1 - cur.cb) : 0;
             load_chunk(pg, pslots, ptile, kn, vn);
         }
-        compute_chunk(c, cur.tok_end, RNG ? cur.lo : 0, kc, vc);
+        compute_chunk(c, cur.tok_end, kc, vc);
         if (!seg_end) {
             c += 1;
             return;

@@ -4,6 +4,7 @@
 
 #include <algorithm>
 
+#include "ranged_decode.h"
 #include "ranged_tiles.h"
 
 namespace flour {
@@ -52,35 +53,20 @@ static bool stream_takes(const RangedAttn& a) {
            (((uintptr_t)a.q | (uintptr_t)a.out | (uintptr_t)a.k_pool | (uintptr_t)a.v_pool) & 15) == 0;
 }
 
-// Its workspace, behind prefixes with the places of pairs that one wave finishes.
-static size_t stream_bytes(int batch, int num_heads, int kv_heads, int head_dim, bool own) {
-    const size_t pairs = (size_t)batch * num_heads;
-    return decode_ws_bytes(decode_workgroups(FLOUR_DTYPE_F32), num_heads / kv_heads, head_dim, batch) +
-           (own ? up256(pairs * 2 * sizeof(float)) + up256(pairs * head_dim * sizeof(float)) : 0);
+static size_t stream_bytes(int batch, int num_heads, int kv_heads, int head_dim) {
+    return decode_ws_bytes(decode_workgroups(FLOUR_DTYPE_F32), num_heads / kv_heads, head_dim, batch);
 }
 
-static RangedStream stream_args(const RangedAttn& a, bool own, char* ws) {
-    const int n_rep = a.num_heads / a.kv_heads, nwg = decode_workgroups(a.dtype);
+static int launch_stream(const RangedAttn& a, void* workspace, hipStream_t stream) {
+    const int nwg = decode_workgroups(a.dtype);
     RangedStream st{};
-    st.ws = decode_ws_at(ws, nwg, n_rep, a.head_dim);
-    st.ws.rng.window = a.window, st.ws.rng.sinks = a.sinks, st.ws.rng.out_dtype = a.out_dtype;
-    if (own) {
-        const size_t pairs = (size_t)a.num_seqs * a.num_heads;
-        char* at = ws + stream_bytes(a.num_seqs, a.num_heads, a.kv_heads, a.head_dim, false);
-        st.ws.rng.group_starts = a.group_starts, st.ws.rng.shared_lens = a.shared_lens;
-        st.ws.rng.num_groups = a.num_groups, st.ws.rng.max_shared = a.max_shared;
-        st.ws.rng.pair_ml = reinterpret_cast<float*>(at);
-        st.ws.rng.pair_o = reinterpret_cast<float*>(at + up256(pairs * 2 * sizeof(float)));
-    }
+    st.ws = decode_ws_at(workspace, nwg, a.num_heads / a.kv_heads, a.head_dim);
+    st.ws.rng = DecodeRange{a.window, a.sinks, a.out_dtype};
     // no more waves than ranges (range_count) for the longest visible parts
     const int64_t chunk = dec_chunk(elem_bytes(a.dtype));
     const int64_t span = std::min<int64_t>(a.max_kv, (int64_t)a.window + a.sinks + 2 * chunk);
     const int64_t half = (int64_t)a.num_seqs * a.kv_heads * ((span + chunk - 1) / chunk) / 2;
     st.grid = (int)std::max<int64_t>(1, std::min<int64_t>(half, nwg));
-    return st;
-}
-
-static int launch_stream(const RangedAttn& a, const RangedStream& st, hipStream_t stream) {
     auto launch = a.dtype == FLOUR_DTYPE_F32    ? launch_ranged_decode_f32
                   : a.dtype == FLOUR_DTYPE_BF16 ? launch_ranged_decode_bf16
                                                 : launch_ranged_decode_f16;
@@ -111,6 +97,9 @@ struct TilePlan {
     int items, max_pieces, piece_tiles;
     size_t bytes;  // of the pieces
 };
+static int g_ranged_wgs = 4, g_ranged_min = 4;
+// Prefixes as a part of their own: 1 always, 0 never, -1 by prefer_shared (a test switch).
+static int g_ranged_shared = -1;
 static TilePlan tile_plan(int64_t units, int64_t unit_rows, int64_t rows, int64_t unit_kv, int num_heads,
                           int kv_heads, int head_dim, int dtype, bool finals) {
     const int64_t n_rep = num_heads / kv_heads, tt = rt_tokens(elem_bytes(dtype));
@@ -120,9 +109,9 @@ static TilePlan tile_plan(int64_t units, int64_t unit_rows, int64_t rows, int64_
     TilePlan p;
     p.items = (int)std::max<int64_t>(1, tiles * kv_heads);
     const int64_t longest = unit_kv / tt + 3;  // (a front tile, and ends that are not whole)
-    const int64_t want = std::max<int64_t>(1, 2 * device_cus() / p.items);
+    const int64_t want = std::max<int64_t>(1, g_ranged_wgs * device_cus() / 2 / p.items);
     // (a piece of fewer tiles costs more in its ends and its merge than it saves)
-    p.piece_tiles = (int)std::max<int64_t>(4, (longest + want - 1) / want);
+    p.piece_tiles = (int)std::max<int64_t>(g_ranged_min, (longest + want - 1) / want);
     p.max_pieces = (int)std::max<int64_t>(1, std::min<int64_t>(want, longest / p.piece_tiles));
     p.bytes = finals && p.max_pieces == 1
                   ? 0
@@ -131,22 +120,26 @@ static TilePlan tile_plan(int64_t units, int64_t unit_rows, int64_t rows, int64_
     return p;
 }
 
-static RtArgs tile_args(const RangedAttn& a, int kind, const TilePlan& p, bool finals, char* ws) {
+static RtArgs tile_args(const RangedAttn& a) {
     RtArgs r{};
-    r.a = a, r.kind = kind, r.n_rep = a.num_heads / a.kv_heads;
+    r.a = a, r.n_rep = a.num_heads / a.kv_heads;
     r.scale_log2 = a.scale * 1.4426950408889634f;
-    r.max_pieces = p.max_pieces, r.piece_tiles = p.piece_tiles, r.finals = finals;
-    r.p_ml = reinterpret_cast<float*>(ws);
-    r.p_o = reinterpret_cast<float*>(
-        ws + up256((size_t)a.rows * a.num_heads * p.max_pieces * 2 * sizeof(float)));
     return r;
 }
+static void add_part(RtArgs* r, int kind, const TilePlan& p, bool finals, char* ws) {
+    RtPart& t = r->part[r->parts++];
+    t.kind = kind, t.items = p.items, t.max_pieces = p.max_pieces, t.piece_tiles = p.piece_tiles;
+    t.finals = finals;
+    t.p_ml = reinterpret_cast<float*>(ws);
+    t.p_o = reinterpret_cast<float*>(
+        ws + up256((size_t)r->a.rows * r->a.num_heads * p.max_pieces * 2 * sizeof(float)));
+}
 
-static int launch_tiles(const RtArgs& r, const TilePlan& p, hipStream_t stream) {
+static int launch_tiles(const RtArgs& r, hipStream_t stream) {
     auto launch = r.a.dtype == FLOUR_DTYPE_F32    ? launch_ranged_tiles_f32
                   : r.a.dtype == FLOUR_DTYPE_BF16 ? launch_ranged_tiles_bf16
                                                   : launch_ranged_tiles_f16;
-    return launch(r, p.items, stream);
+    return launch(r, stream);
 }
 
 // Rows over what they see: one launch, and a merge where pairs are cut.
@@ -168,6 +161,38 @@ static SharedPlan shared_plan(int num_seqs, int num_groups, int max_rows, int ro
                                 false),
                       tile_plan(num_seqs, max_rows, rows, max_kv, num_heads, kv_heads, head_dim, dtype,
                                 false)};
+}
+
+// Whether prefixes are worth a part of their own, by an estimate of both ways in us from the host's bounds.
+// A tile step (128 columns, 32 KB of K / V at head_dim 128 in 16 bits) takes the chip 4.7-5.9 ns; pieces are
+// written and read at about 8 TB/s. Decode steps alone are streamed: what several sequences read comes from
+// the caches for the most part. Fitted on 32 / 8 heads of 128, bf16, prefix + own, us alone / shared:
+//   64 sequences of one prefix 256 + 64 15.6 / 19.9, 1,024 + 64 31.5 / 20.7, 4,096 + 256 91 / 38,
+//   16,384 + 128 313 / 48; of 32 prefixes 256 + 64 18.5 / 26.7, 1,024 + 64 45.9 / 39.1;
+//   4 sequences of one prefix 1,024 + 1,024 15.6 / 16.7, 16,384 + 128 29.2 / 28.9
+static bool prefer_shared(int num_seqs, int num_groups, int max_rows, int rows, int num_heads, int kv_heads,
+                          int head_dim, int max_kv, int max_shared, int dtype, const SharedPlan& p) {
+    if (num_groups == 0 || max_shared == 0 || g_ranged_shared >= 0)
+        return num_groups > 0 && max_shared > 0 && g_ranged_shared > 0;
+    const double es = elem_bytes(dtype), G = kv_heads, n_rep = num_heads / kv_heads;
+    const double tt = rt_tokens((int)es), row = 2.0 * G * head_dim * es;  // K and V of a position
+    const double ns = 5e-3 * (dtype == FLOUR_DTYPE_F32 ? 2.0 : 1.0) * head_dim / 128;  // a tile step
+    const double own = std::max(1, max_kv - max_shared), S = num_seqs;
+    const double groups = std::min(num_groups, num_seqs);
+    const double seq_tiles =
+        std::min(S * ceil((double)max_rows * n_rep / RT_COLS), rows * n_rep / RT_COLS + S);
+    const double group_tiles = rows * n_rep / RT_COLS + groups;
+    const double pieces =
+        (double)rows * num_heads * (head_dim + 2) * 4.0 *
+        (std::min<double>(p.prefix.max_pieces, ceil(max_shared / tt / p.prefix.piece_tiles)) +
+         std::min<double>(p.own.max_pieces, ceil(own / tt / p.own.piece_tiles)));
+    const double shared_us = 14.0 + ns * G * (group_tiles * max_shared / tt + seq_tiles * (own / tt + 0.5)) +
+                             2.0 * pieces / 8e6;
+    const double unique = (groups * max_shared + S * own) * row, all = S * max_kv * row;
+    const double alone_us = max_rows <= 1 && n_rep <= 16
+                                ? 8.0 + unique / 5.5e6 + std::max(0.0, all - unique) / 12e6
+                                : 8.0 + ns * G * seq_tiles * (max_kv / tt + 0.5);
+    return shared_us < alone_us;
 }
 
 static int ranged_call(const char* what, const RangedAttn& a, bool shared, void* workspace,
@@ -193,33 +218,26 @@ static int ranged_call(const char* what, const RangedAttn& a, bool shared, void*
         return FLOUR_ERR_WORKSPACE;
     }
     char* ws = static_cast<char*>(workspace);
-    const bool step = !a.cu && stream_takes(a);
-    if (step && (!shared || a.num_groups == 0 || a.max_shared == 0))
-        return launch_stream(a, stream_args(a, false, ws), stream);
-    if (!tiles_take(a)) return launch_ranged_generic(a, stream);
-    if (!shared || a.num_groups == 0 || a.max_shared == 0) {
-        const TilePlan p = rows_plan(a.num_seqs, a.max_rows, a.rows, a.num_heads, a.kv_heads, a.head_dim,
-                                     a.max_kv, a.window, a.sinks, a.dtype);
-        const RtArgs r = tile_args(a, RT_ROWS, p, true, ws);
-        rc = launch_tiles(r, p, stream);
-        return rc != FLOUR_OK || p.max_pieces == 1 ? rc : launch_ranged_merge(r, nullptr, nullptr, stream);
+    const bool step = !a.cu && stream_takes(a), tiles = tiles_take(a);
+    if (!step && !tiles) return launch_ranged_generic(a, stream);
+    RtArgs r = tile_args(a);
+    if (tiles && shared) {
+        const SharedPlan p = shared_plan(a.num_seqs, a.num_groups, a.max_rows, a.rows, a.num_heads,
+                                         a.kv_heads, a.head_dim, a.max_kv, a.max_shared, a.dtype);
+        if (prefer_shared(a.num_seqs, a.num_groups, a.max_rows, a.rows, a.num_heads, a.kv_heads,
+                          a.head_dim, a.max_kv, a.max_shared, a.dtype, p)) {
+            add_part(&r, RT_PREFIX, p.prefix, false, ws);
+            add_part(&r, RT_OWN, p.own, false, ws + p.prefix.bytes);
+            rc = launch_tiles(r, stream);
+            return rc != FLOUR_OK ? rc : launch_ranged_merge(r, stream);
+        }
     }
-    const SharedPlan p = shared_plan(a.num_seqs, a.num_groups, a.max_rows, a.rows, a.num_heads, a.kv_heads,
-                                     a.head_dim, a.max_kv, a.max_shared, a.dtype);
-    if (step) {
-        const RangedStream st = stream_args(a, true, ws);
-        const RtArgs prefix = tile_args(
-            a, RT_PREFIX, p.prefix, false,
-            ws + stream_bytes(a.num_seqs, a.num_heads, a.kv_heads, a.head_dim, true));
-        rc = launch_tiles(prefix, p.prefix, stream);
-        if (rc == FLOUR_OK) rc = launch_stream(a, st, stream);
-        return rc != FLOUR_OK ? rc : launch_ranged_merge(prefix, nullptr, &st, stream);
-    }
-    const RtArgs own = tile_args(a, RT_OWN, p.own, false, ws);
-    const RtArgs prefix = tile_args(a, RT_PREFIX, p.prefix, false, ws + p.own.bytes);
-    rc = launch_tiles(prefix, p.prefix, stream);
-    if (rc == FLOUR_OK) rc = launch_tiles(own, p.own, stream);
-    return rc != FLOUR_OK ? rc : launch_ranged_merge(own, &prefix, nullptr, stream);
+    if (step) return launch_stream(a, ws, stream);
+    const TilePlan p = rows_plan(a.num_seqs, a.max_rows, a.rows, a.num_heads, a.kv_heads, a.head_dim,
+                                 a.max_kv, a.window, a.sinks, a.dtype);
+    add_part(&r, RT_ROWS, p, true, ws);
+    rc = launch_tiles(r, stream);
+    return rc != FLOUR_OK || p.max_pieces == 1 ? rc : launch_ranged_merge(r, stream);
 }
 
 // A decode step's part of a call: one row a sequence, packed rows of all heads.
@@ -287,7 +305,7 @@ extern "C" int flour_hip_window_workspace_size(int num_seqs, int max_seqlen_q, i
         n = rows_plan(num_seqs, max_seqlen_q, total_q, num_heads, kv_heads, head_dim, max_kv_len, window,
                       sinks, dtype).bytes;
     if (total_q == num_seqs && stream_fits(num_seqs, num_heads, kv_heads, head_dim))  // a decode step
-        n = std::max(n, stream_bytes(num_seqs, num_heads, kv_heads, head_dim, false));
+        n = std::max(n, stream_bytes(num_seqs, num_heads, kv_heads, head_dim));
     *bytes = n;
     return FLOUR_OK;
 }
@@ -305,15 +323,18 @@ extern "C" int flour_hip_shared_workspace_size(int num_seqs, int num_groups, int
                   max_shared_len);
         return FLOUR_ERR_INVALID_ARGUMENT;
     }
-    *bytes = 0;
-    if (!tiles_fit(total_q, num_heads, kv_heads, head_dim)) return FLOUR_OK;
-    const SharedPlan p = shared_plan(num_seqs, num_groups, max_seqlen_q, total_q, num_heads, kv_heads,
-                                     head_dim, max_kv_len, max_shared_len, dtype);
-    const TilePlan alone = rows_plan(num_seqs, max_seqlen_q, total_q, num_heads, kv_heads, head_dim,
-                                     max_kv_len, 0x7fffffff, 0, dtype);
-    size_t n = std::max(p.prefix.bytes + p.own.bytes, alone.bytes);
-    if (total_q == num_seqs && stream_fits(num_seqs, num_heads, kv_heads, head_dim))
-        n = std::max(n, p.prefix.bytes + stream_bytes(num_seqs, num_heads, kv_heads, head_dim, true));
+    size_t n = 0;
+    if (tiles_fit(total_q, num_heads, kv_heads, head_dim)) {
+        const SharedPlan p = shared_plan(num_seqs, num_groups, max_seqlen_q, total_q, num_heads, kv_heads,
+                                         head_dim, max_kv_len, max_shared_len, dtype);
+        n = prefer_shared(num_seqs, num_groups, max_seqlen_q, total_q, num_heads, kv_heads, head_dim,
+                          max_kv_len, max_shared_len, dtype, p)
+                ? p.prefix.bytes + p.own.bytes
+                : rows_plan(num_seqs, max_seqlen_q, total_q, num_heads, kv_heads, head_dim, max_kv_len,
+                            0x7fffffff, 0, dtype).bytes;
+    }
+    if (total_q == num_seqs && stream_fits(num_seqs, num_heads, kv_heads, head_dim))  // a decode step
+        n = std::max(n, stream_bytes(num_seqs, num_heads, kv_heads, head_dim));
     *bytes = n;
     return FLOUR_OK;
 }
@@ -392,4 +413,17 @@ extern "C" int flour_hip_varlen_prefill_shared(
     }
     return ranged_call("varlen_prefill_shared", a, true, workspace, workspace_bytes,
                        static_cast<hipStream_t>(stream));
+}
+
+extern "C" int flour_hip_set_shared_prefix(int mode) {
+    if (mode < -1 || mode > 1) return FLOUR_ERR_INVALID_ARGUMENT;
+    g_ranged_shared = mode;
+    switch_set();
+    return FLOUR_OK;
+}
+
+extern "C" int flour_hip_set_ranged(int wgs, int least) {
+    g_ranged_wgs = wgs, g_ranged_min = least;
+    switch_set();
+    return 0;
 }

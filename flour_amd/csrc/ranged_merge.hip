@@ -9,72 +9,35 @@ namespace flour {
 
 static constexpr int RM_WAVES = 4;
 
-// Piece k > 0 of a row is k steps behind ml and o, piece 0 has a place of its own.
 struct RmPieces {
     int n;
-    const float *ml0, *o0, *ml, *o;
-    int64_t ml_step, o_step;
+    const float *ml, *o;
 };
 
 // The pieces of packed row `row`, head h in a tile launch; `shared`: the length of its group's prefix.
-__device__ __forceinline__ RmPieces tile_pieces(const RtArgs& ra, const RangedSeq& q, int shared, int row,
-                                                int h, int head_dim, int tt) {
+__device__ __forceinline__ RmPieces tile_pieces(const RtArgs& ra, const RtPart& pt, const RangedSeq& q,
+                                                int shared, int row, int h, int head_dim, int tt) {
     RmPieces p{};
     RtSpan sp;
-    if (ra.kind == RT_PREFIX) {
+    if (pt.kind == RT_PREFIX) {
         if (shared == 0) return p;
-        sp = rt_span(ra, RT_PREFIX, 0, shared, 0, 0, tt);
+        sp = rt_span(ra, RT_PREFIX, 0, shared, 0, 0);
     } else {
         const int col = (row - q.row0) * ra.n_rep + h % ra.n_rep;
-        sp = rt_span(ra, ra.kind, q.rows, q.kv, col / RT_COLS, shared, tt);
+        sp = rt_span(ra, pt.kind, q.rows, q.kv, col / RT_COLS, shared);
     }
-    p.n = rt_pieces(sp.tiles, ra.max_pieces, ra.piece_tiles);
-    const int64_t slot = ((int64_t)row * ra.a.num_heads + h) * ra.max_pieces;
-    p.ml0 = p.ml = ra.p_ml + 2 * slot;
-    p.o0 = p.o = ra.p_o + slot * head_dim;
-    p.ml_step = 2, p.o_step = head_dim;
-    return p;
-}
-
-// The pieces of batch entry b, head h in a step's stream: of the wave ranges that its chunks lie in, two
-// slots each, or the slot of its own where one wave has them all.
-__device__ __forceinline__ RmPieces stream_pieces(const RangedStream& st, const RangedAttn& a, int b, int h,
-                                                  int n_rep) {
-    const DecodeWs& ws = st.ws;
-    RmPieces p{};
-    const int before = ws.pre[b], nch = ws.pre[b + 1] - before, all = ws.pre[a.num_seqs];
-    if (nch == 0) return p;
-    const int g = h / n_rep, hh = h - g * n_rep;
-    const int64_t total = (int64_t)a.kv_heads * all, nwg = range_count(total, st.grid);
-    const int64_t s = (int64_t)a.kv_heads * before + (int64_t)g * nch, e = s + nch;
-    const bool narrow = ranges_narrow(total, nwg, ws.xcd_w);
-    const WaveRanges<uint32_t> r32(narrow ? total : 1, nwg, ws.xcd_w);
-    const WaveRanges<int64_t> r64(total, nwg, ws.xcd_w);
-    const int64_t f = narrow ? (int64_t)r32.owner((uint32_t)s) : r64.owner(s);
-    const int64_t l = narrow ? (int64_t)r32.owner((uint32_t)(e - 1)) : r64.owner(e - 1);
-    const int D = a.head_dim;
-    if (f == l) {
-        const int64_t slot = (int64_t)b * a.num_heads + h;
-        p.n = 1;
-        p.ml0 = p.ml = ws.rng.pair_ml + 2 * slot;
-        p.o0 = p.o = ws.rng.pair_o + slot * D;
-        return p;
-    }
-    const bool f_first = s == (narrow ? (int64_t)r32.lo((uint32_t)f) : r64.lo(f));
-    const int64_t slot = 2 * f * n_rep + hh, slot0 = slot + (f_first ? 0 : n_rep);
-    p.n = (int)(l - f + 1);
-    p.ml = ws.ml + 2 * slot, p.ml0 = ws.ml + 2 * slot0;
-    p.o = ws.o + slot * D, p.o0 = ws.o + slot0 * D;
-    p.ml_step = 4 * n_rep, p.o_step = (int64_t)2 * n_rep * D;
+    p.n = rt_pieces(sp.tiles(tt), pt.max_pieces, pt.piece_tiles);
+    const int64_t slot = ((int64_t)row * ra.a.num_heads + h) * pt.max_pieces;
+    p.ml = pt.p_ml + 2 * slot;
+    p.o = pt.p_o + slot * head_dim;
     return p;
 }
 
 template <int D>
-__global__ __launch_bounds__(64 * RM_WAVES) void ranged_merge_kernel(RtArgs first, RtArgs second,
-                                                                     bool two, RangedStream st, int tt) {
+__global__ __launch_bounds__(64 * RM_WAVES) void ranged_merge_kernel(RtArgs ra, int tt) {
     constexpr int E = D / 64;
     typedef typename std::conditional<E == 2, f32x2, float>::type RowV;
-    const RangedAttn& a = first.a;
+    const RangedAttn& a = ra.a;
     const int lane = threadIdx.x & 63;
     const int64_t item = (int64_t)blockIdx.x * RM_WAVES + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     if (item >= (int64_t)a.rows * a.num_heads) return;
@@ -94,19 +57,17 @@ __global__ __launch_bounds__(64 * RM_WAVES) void ranged_merge_kernel(RtArgs firs
     const RangedSeq q = ranged_seq(a, s);
     if (row < q.row0 || row >= q.row0 + q.rows) return;  // (rows of no sequence)
     const int shared = a.num_groups > 0 ? ranged_shared_of(a, s) : 0;
-    const RmPieces set[2] = {tile_pieces(first, q, shared, row, h, D, tt),
-                             two           ? tile_pieces(second, q, shared, row, h, D, tt)
-                             : st.grid > 0 ? stream_pieces(st, a, s, h, first.n_rep)
-                                           : RmPieces{}};
-    if (first.finals && set[0].n == 1) return;
+    const RmPieces set[2] = {tile_pieces(ra, ra.part[0], q, shared, row, h, D, tt),
+                             ra.parts > 1 ? tile_pieces(ra, ra.part[1], q, shared, row, h, D, tt)
+                                          : RmPieces{}};
+    if (ra.part[0].finals && set[0].n == 1) return;
     float M = DEC_M0, L = 0.0f, O[E] = {};
 #pragma unroll
     for (int x = 0; x < 2; x++) {
         const RmPieces& p = set[x];
         for (int p0 = 0; p0 < p.n; p0 += 64) {
             const bool on = p0 + lane < p.n;
-            const float* ml = p0 + lane == 0 ? p.ml0 : p.ml + (int64_t)(p0 + lane) * p.ml_step;
-            const float mx = on ? ml[0] : DEC_M0, lx = on ? ml[1] : 0.0f;
+            const float mx = on ? p.ml[2 * (p0 + lane)] : DEC_M0, lx = on ? p.ml[2 * (p0 + lane) + 1] : 0.0f;
             const float Mn = fmaxf(M, wave_max(mx));
             const float w = on ? fast_exp2(mx - Mn) : 0.0f, old = fast_exp2(M - Mn);
             L = L * old + wave_sum(w * lx);
@@ -116,10 +77,9 @@ __global__ __launch_bounds__(64 * RM_WAVES) void ranged_merge_kernel(RtArgs firs
             for (int y0 = 0; y0 < n; y0 += 8) {
                 RowV v[8];
 #pragma unroll
-                for (int y = 0; y < 8; y++) {  // (past the last one: that again, for nothing)
-                    const int k = min(p0 + y0 + y, p.n - 1);
-                    v[y] = *reinterpret_cast<const RowV*>((k == 0 ? p.o0 : p.o + k * p.o_step) + E * lane);
-                }
+                for (int y = 0; y < 8; y++)  // (past the last one: that again, for nothing)
+                    v[y] = *reinterpret_cast<const RowV*>(p.o + (int64_t)min(p0 + y0 + y, p.n - 1) * D +
+                                                          E * lane);
 #pragma unroll
                 for (int y = 0; y < 8; y++) {
                     const float wy = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w), (y0 + y) & 63));
@@ -145,14 +105,12 @@ __global__ __launch_bounds__(64 * RM_WAVES) void ranged_merge_kernel(RtArgs firs
     }
 }
 
-int launch_ranged_merge(const RtArgs& first, const RtArgs* second, const RangedStream* st,
-                        hipStream_t stream) {
-    const int64_t items = (int64_t)first.a.rows * first.a.num_heads;
+int launch_ranged_merge(const RtArgs& r, hipStream_t stream) {
+    const int64_t items = (int64_t)r.a.rows * r.a.num_heads;
     const dim3 grid((unsigned)((items + RM_WAVES - 1) / RM_WAVES));
-    const int tt = rt_tokens(elem_bytes(first.a.dtype));
-    auto kern = first.a.head_dim == 64 ? ranged_merge_kernel<64> : ranged_merge_kernel<128>;
-    kern<<<grid, dim3(64 * RM_WAVES), 0, stream>>>(first, second ? *second : first, second != nullptr,
-                                                   st ? *st : RangedStream{}, tt);
+    const int tt = rt_tokens(elem_bytes(r.a.dtype));
+    auto kern = r.a.head_dim == 64 ? ranged_merge_kernel<64> : ranged_merge_kernel<128>;
+    kern<<<grid, dim3(64 * RM_WAVES), 0, stream>>>(r, tt);
     return check_hip(hipGetLastError(), "attention over ranges merge launch");
 }
 

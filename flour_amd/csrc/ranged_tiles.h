@@ -9,7 +9,6 @@
 
 #include "decode_ranges.h"
 #include "ranged.h"
-#include "ranged_decode.h"
 
 namespace flour {
 
@@ -20,18 +19,22 @@ enum RtKind {
     RT_OWN,     // a unit is a sequence: its rows over the positions behind its group's prefix
 };
 
-struct RtArgs {
-    RangedAttn a;
-    int kind;
-    int n_rep;
-    float scale_log2;
-    // A pair's tiles are cut into up to max_pieces pieces of at least piece_tiles. A pair of one piece is
-    // written out where finals is set; otherwise piece k of packed row r, head h leaves its maximum and
-    // sum (exp2 domain) and accumulator at slot (r * num_heads + h) * max_pieces + k.
-    int max_pieces, piece_tiles;
+// One kind's part of a launch: `items` (unit, column tile, kv head) triples at most, each of which has its
+// tiles cut into up to max_pieces pieces of at least piece_tiles. A triple of one piece is written out
+// where finals is set; otherwise piece k of packed row r, head h leaves its maximum and sum (exp2
+// domain) and accumulator at slot (r * num_heads + h) * max_pieces + k.
+struct RtPart {
+    int kind, items, max_pieces, piece_tiles;
     bool finals;
     float* p_ml;  // [slot][2]
     float* p_o;   // [slot][D]
+};
+struct RtArgs {
+    RangedAttn a;
+    int n_rep;
+    float scale_log2;
+    int parts;
+    RtPart part[2];  // the first one's workgroups come first
 };
 
 static constexpr int RT_WAVES = 4;              // waves of 32 columns each
@@ -44,17 +47,18 @@ __host__ __device__ __forceinline__ int rt_pieces(int tiles, int max_pieces, int
     return n < 1 ? 1 : (n < max_pieces ? n : max_pieces);
 }
 
-// The positions that a column tile of a unit goes through: [0, front) and [from, to), the second behind the
-// first, in tiles of tt positions (the second's start at a run of 16).
+// The positions that a column tile of a unit goes through, in runs of 16: those of [0, front), then those of
+// [from, to) from the last multiple of 16 on; a tile is RT tokens / 16 of these runs.
 struct RtSpan {
-    int front, from, to, ft, base, tiles;
-    __device__ __forceinline__ int tok(int v, int tt) const {
-        return v < ft ? v * tt : base + (v - ft) * tt;
+    int front, from, to, front_runs, base, runs;
+    __device__ __forceinline__ int tok(int run) const {
+        return run < front_runs ? 16 * run : base + 16 * (run - front_runs);
     }
+    __device__ __forceinline__ int tiles(int tt) const { return (16 * runs + tt - 1) / tt; }
 };
 // rows and kv: the unit's. own: where the positions of RT_OWN start.
 __device__ __forceinline__ RtSpan rt_span(const RtArgs& ra, int kind, int rows, int kv, int ctile,
-                                          int own, int tt) {
+                                          int own) {
     RtSpan s;
     const int sinks = kind == RT_ROWS ? ra.a.sinks : 0;
     s.from = 0, s.to = kv;
@@ -71,19 +75,18 @@ __device__ __forceinline__ RtSpan rt_span(const RtArgs& ra, int kind, int rows, 
         }
     }
     s.front = s.from > 0 ? min(sinks, s.to) : 0;
-    s.ft = (s.front + tt - 1) / tt;
-    s.base = max(s.from & ~15, s.ft * tt);
-    s.tiles = s.ft + (s.to > s.base ? (s.to - s.base + tt - 1) / tt : 0);
+    s.front_runs = (s.front + 15) >> 4;
+    s.base = max(s.from & ~15, 16 * s.front_runs);
+    s.runs = s.front_runs + (s.to > s.base ? (s.to - s.base + 15) >> 4 : 0);
     return s;
 }
 
-// Joins pieces: of `first`, and (or null) of `second`, whose launch had the same rows, or of a step's
-// stream. Where first.finals is set, rows of one piece are left alone.
-int launch_ranged_merge(const RtArgs& first, const RtArgs* second, const RangedStream* st,
-                        hipStream_t stream);
+// Joins the pieces of a launch's parts. Where the first part's finals is set, rows of one piece are left
+// alone.
+int launch_ranged_merge(const RtArgs& r, hipStream_t stream);
 
-int launch_ranged_tiles_f32(const RtArgs& r, int items, hipStream_t stream);
-int launch_ranged_tiles_bf16(const RtArgs& r, int items, hipStream_t stream);
-int launch_ranged_tiles_f16(const RtArgs& r, int items, hipStream_t stream);
+int launch_ranged_tiles_f32(const RtArgs& r, hipStream_t stream);
+int launch_ranged_tiles_bf16(const RtArgs& r, hipStream_t stream);
+int launch_ranged_tiles_f16(const RtArgs& r, hipStream_t stream);
 
 }  // namespace flour

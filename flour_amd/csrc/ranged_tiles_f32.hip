@@ -3,8 +3,8 @@
 
 namespace flour {
 
-int launch_ranged_tiles_f32(const RtArgs& r, int items, hipStream_t stream) {
-    return launch_ranged_tiles<float>(r, items, stream);
+int launch_ranged_tiles_f32(const RtArgs& r, hipStream_t stream) {
+    return launch_ranged_tiles<float>(r, stream);
 }
 
 }  // namespace flour

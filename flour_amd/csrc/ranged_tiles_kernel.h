@@ -55,8 +55,12 @@ __global__ __launch_bounds__(64 * RT_WAVES, 2) void ranged_tiles_kernel(RtArgs r
 
     // ---- the item: (unit, column tile), kv head fastest (neighbouring workgroups, one an XCD, have
     // different heads, so each XCD's L2 holds its own heads' K/V)
-    const int g = blockIdx.x % a.kv_heads, want = blockIdx.x / a.kv_heads;
-    const int units = ra.kind == RT_PREFIX ? a.num_groups : a.num_seqs;
+    const bool second = blockIdx.x >= (unsigned)(ra.part[0].items * ra.part[0].max_pieces);
+    const RtPart pt = ra.part[second ? 1 : 0];
+    const int wg = (int)blockIdx.x - (second ? ra.part[0].items * ra.part[0].max_pieces : 0);
+    const int piece = wg / pt.items, item = wg - piece * pt.items;
+    const int g = item % a.kv_heads, want = item / a.kv_heads;
+    const int units = pt.kind == RT_PREFIX ? a.num_groups : a.num_seqs;
     int unit = -1, ctile = 0, row0 = 0, rows = 0, kv = 0;
     {
         int before = 0;
@@ -64,7 +68,7 @@ __global__ __launch_bounds__(64 * RT_WAVES, 2) void ranged_tiles_kernel(RtArgs r
             const int u = u0 + lane;
             int ur0 = 0, un = 0, ukv = 0;
             if (u < units) {
-                if (ra.kind == RT_PREFIX) {
+                if (pt.kind == RT_PREFIX) {
                     const int s0 = max(0, min(a.group_starts[u], a.num_seqs));
                     const int s1 = max(s0, min(a.group_starts[u + 1], a.num_seqs));
                     ukv = max(0, min(a.shared_lens[u], a.max_shared));
@@ -92,7 +96,7 @@ __global__ __launch_bounds__(64 * RT_WAVES, 2) void ranged_tiles_kernel(RtArgs r
     }
     if (unit < 0) return;
     const int ncols = rows * n_rep;
-    const int seq = ra.kind == RT_PREFIX ? max(0, min(a.group_starts[unit], a.num_seqs - 1)) : unit;
+    const int seq = pt.kind == RT_PREFIX ? max(0, min(a.group_starts[unit], a.num_seqs - 1)) : unit;
     const int32_t* bt = a.block_tables + (int64_t)seq * a.max_blocks;
 
     // ---- the lane's column, and which positions t it sees: t < hi and (t >= lo or t < sinks)
@@ -102,9 +106,9 @@ __global__ __launch_bounds__(64 * RT_WAVES, 2) void ranged_tiles_kernel(RtArgs r
     const bool real = col0 + l32 < ncols;
     const int row_i = col / n_rep, head = g * n_rep + (col - row_i * n_rep);
     const int row = row0 + row_i;
-    const int sinks = ra.kind == RT_ROWS ? a.sinks : 0;
+    const int sinks = pt.kind == RT_ROWS ? a.sinks : 0;
     int hi, lo = 0, own = 0;
-    if (ra.kind == RT_PREFIX) {
+    if (pt.kind == RT_PREFIX) {
         int s = row;
         if (a.cu) {
             int x = 0, y = a.num_seqs;
@@ -121,17 +125,16 @@ __global__ __launch_bounds__(64 * RT_WAVES, 2) void ranged_tiles_kernel(RtArgs r
         hi = q.kv > 0 ? min(kv, q.kv - q.rows + (row - q.row0) + 1) : 0;
     } else {
         hi = kv > 0 ? kv - rows + row_i + 1 : 0;
-        if (ra.kind == RT_ROWS)
+        if (pt.kind == RT_ROWS)
             lo = max(0, hi - a.window);
         else
             lo = own = ranged_shared_of(a, seq);
     }
-    const RtSpan sp = rt_span(ra, ra.kind, rows, kv, ctile, own, TT);
-    const int front = sp.front, from = sp.from, to = sp.to, all_tiles = sp.tiles;
-    auto tok_of = [&](int v) -> int { return sp.tok(v, TT); };
+    const RtSpan sp = rt_span(ra, pt.kind, rows, kv, ctile, own);
+    const int front = sp.front, from = sp.from, to = sp.to, all_tiles = sp.tiles(TT);
 
     // ---- this workgroup's piece of the tiles
-    const int pieces = rt_pieces(all_tiles, ra.max_pieces, ra.piece_tiles), piece = blockIdx.y;
+    const int pieces = rt_pieces(all_tiles, pt.max_pieces, pt.piece_tiles);
     if (piece >= pieces) return;
     const int t_begin = (int)((int64_t)all_tiles * piece / pieces);
     const int t_end = (int)((int64_t)all_tiles * (piece + 1) / pieces);
@@ -144,8 +147,7 @@ __global__ __launch_bounds__(64 * RT_WAVES, 2) void ranged_tiles_kernel(RtArgs r
     const int max_id = (int)(a.num_slots / a.block_size - 1);
     const int last_run = (to - 1) & ~15;
     auto load_slots = [&](int t0) -> uint32_t {  // byte offsets
-        const int v = t0 + lane / UPT;
-        const int tok = min(tok_of(min(v, max(all_tiles - 1, 0))) + 16 * (lane % UPT), last_run);
+        const int tok = min(sp.tok(min(t0 * UPT + lane, sp.runs - 1)), last_run);
         const int lb = a.block_size == 16 ? tok >> 4 : tok / a.block_size;
         int id = bt[lb];
         id = id < 0 ? 0 : (id > max_id ? max_id : id);  // a bad block id never leaves the pool
@@ -172,22 +174,24 @@ __global__ __launch_bounds__(64 * RT_WAVES, 2) void ranged_tiles_kernel(RtArgs r
             vreg[k] = __builtin_amdgcn_raw_buffer_load_b128(v_rsrc, voff, soff, 0);
         }
     };
-    auto stage_tile = [&](auto exact, int t, int buf) __attribute__((always_inline)) {
-        const int tok0 = tok_of(t);
-        // positions that no column sees: no bits of theirs
-        const bool edge = tok0 + TT > to || (tok0 < from && tok0 + TT > front);
+    // positions of a loaded tile that no column sees: no bits of theirs
+    auto cut_tile = [&](int t) __attribute__((always_inline)) {
+        if (sp.tok(t * UPT) >= from && sp.tok(t * UPT + UPT - 1) + 16 <= to) return;
 #pragma unroll
         for (int k = 0; k < NP; k++) {
-            const int r = k * RPP + s_row, tok = tok0 + r;
-            *reinterpret_cast<u32x4*>(&k_lds[buf][r * KP + s_col]) = kreg[k];
-            u32x4 v = vreg[k];
-            if (edge && !(tok < to && (tok >= from || tok < front))) v = u32x4{0, 0, 0, 0};
-            if constexpr (BF16 && !decltype(exact)::value)
-#pragma unroll
-                for (int e = 0; e < 4; e++)
-                    v[e] = pack2<f16_t>(lo_f32<bf16_t>(v[e]), hi_f32<bf16_t>(v[e]));
-            *reinterpret_cast<u32x4*>(&v_lds[buf][r * VP + s_col]) = v;
+            const int tok = sp.tok(t * UPT + (k * RPP + w_row) / 16) + ((k * RPP + s_row) & 15);
+            if (!(tok < to && (tok >= from || tok < front))) vreg[k] = u32x4{0, 0, 0, 0};
         }
+    };
+    auto stage_rows = [&](auto exact, int k, int buf) __attribute__((always_inline)) {
+        const int r = k * RPP + s_row;
+        *reinterpret_cast<u32x4*>(&k_lds[buf][r * KP + s_col]) = kreg[k];
+        u32x4 v = vreg[k];
+        if constexpr (BF16 && !decltype(exact)::value)
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                v[e] = pack2<f16_t>(lo_f32<bf16_t>(v[e]), hi_f32<bf16_t>(v[e]));
+        *reinterpret_cast<u32x4*>(&v_lds[buf][r * VP + s_col]) = v;
     };
 
     // ---- Q^T as the B operand: dims 16 kk + 8 half .. + 7 for product kk; fp32: dims D/2 half + s for
@@ -205,42 +209,69 @@ __global__ __launch_bounds__(64 * RT_WAVES, 2) void ranged_tiles_kernel(RtArgs r
 
     float m, l;
     f32x16 acc[NO];
-    auto compute = [&](auto exact, int t, int buf) __attribute__((always_inline)) {
-        const int tok0 = tok_of(t);
-        if (!live || tok0 >= max_hi || (tok0 + TT <= min_lo && tok0 >= sinks)) return;
+    // Tile t, and meanwhile the next one's rows from registers to the other buffer, which frees the registers
+    // for request().
+    auto compute = [&](auto exact, int t, int buf, auto request) __attribute__((always_inline)) {
+        const int tok0 = sp.tok(t * UPT), tok_end = sp.tok(t * UPT + UPT - 1) + 16;
+        if (!live || tok0 >= max_hi || (tok_end <= min_lo && tok0 >= sinks)) {
+#pragma unroll
+            for (int k = 0; k < NP; k++) stage_rows(exact, k, buf ^ 1);
+            request();
+            return;
+        }
         f32x16 s[NB];
 #pragma unroll
-        for (int b = 0; b < NB; b++) {
+        for (int b = 0; b < NB; b++)
 #pragma unroll
             for (int e = 0; e < 16; e++) s[b][e] = 0.0f;
-            const unsigned char* kr = &k_lds[buf][(32 * b + l32) * KP];
-            if constexpr (F32) {
-                f32x16 s1 = s[b];
+        const unsigned char* kr = &k_lds[buf][l32 * KP];
+        if constexpr (F32) {
 #pragma unroll
-                for (int kk = 0; kk < NQ; kk++) {
-                    const f32x4 x = *reinterpret_cast<const f32x4*>(kr + ROW / 2 * half + 16 * kk);
+            for (int k = 0; k < NP; k++) stage_rows(exact, k, buf ^ 1);
+            f32x16 s1 = s[0];
 #pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        f32x16& y = e & 1 ? s1 : s[b];
-                        y = __builtin_amdgcn_mfma_f32_32x32x2f32(x[e], __uint_as_float(qb[kk][e]), y, 0,
-                                                                 0, 0);
-                    }
+            for (int kk = 0; kk < NQ; kk++) {
+                const f32x4 x = *reinterpret_cast<const f32x4*>(kr + ROW / 2 * half + 16 * kk);
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    f32x16& y = e & 1 ? s1 : s[0];
+                    y = __builtin_amdgcn_mfma_f32_32x32x2f32(x[e], __uint_as_float(qb[kk][e]), y, 0, 0, 0);
                 }
-                s[b] += s1;
-            } else {
-#pragma unroll
-                for (int kk = 0; kk < NQ; kk++)
-                    s[b] = mfma32x32x16<T>(*reinterpret_cast<const u32x4*>(kr + 32 * kk + 16 * half),
-                                           qb[kk], s[b]);
             }
+            s[0] += s1;
+        } else {
+            // K fragments three steps ahead (left alone, the reads come right before their products)
+            constexpr int AHEAD = 3;
+            u32x4 kf[AHEAD][NB];
+            auto read_k = [&](int kk) __attribute__((always_inline)) {
+#pragma unroll
+                for (int b = 0; b < NB; b++)
+                    kf[kk % AHEAD][b] =
+                        *reinterpret_cast<const u32x4*>(kr + 32 * b * KP + 32 * kk + 16 * half);
+            };
+            __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+            for (int kk = 0; kk < AHEAD; kk++) read_k(kk);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int kk = 0; kk < NQ; kk++) {
+#pragma unroll
+                for (int b = 0; b < NB; b++) s[b] = mfma32x32x16<T>(kf[kk % AHEAD][b], qb[kk], s[b]);
+                if (kk + AHEAD < NQ) read_k(kk + AHEAD);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            __builtin_amdgcn_s_setprio(0);
+#pragma unroll
+            for (int k = 0; k < NP; k++) stage_rows(exact, k, buf ^ 1);
         }
-        const bool full = tok0 + TT <= min_hi && (tok0 >= max_lo || tok0 + TT <= sinks);
+        request();  // the tile after the next one
+        const bool full = tok_end <= min_hi && (tok0 >= max_lo || tok_end <= sinks);
         if (!full) {
 #pragma unroll
             for (int b = 0; b < NB; b++)
 #pragma unroll
                 for (int e = 0; e < 16; e++) {
-                    const int tok = tok0 + 32 * b + 8 * (e >> 2) + 4 * half + (e & 3);
+                    const int tok = sp.tok(t * UPT + 2 * b + (e >> 3)) + 8 * ((e >> 2) & 1) + 4 * half + (e & 3);
                     if (!(tok < hi && (tok >= lo || tok < sinks))) s[b][e] = -INFINITY;
                 }
         }
@@ -260,64 +291,71 @@ __global__ __launch_bounds__(64 * RT_WAVES, 2) void ranged_tiles_kernel(RtArgs r
 #pragma unroll
             for (int o = 0; o < NO; o++) acc[o] *= alpha;
         }
+        if constexpr (F32) {
+            float p[16], x = 0.0f, y = 0.0f;
 #pragma unroll
-        for (int b = 0; b < NB; b++) {
-            float p[16];
+            for (int e = 0; e < 16; e++) p[e] = fast_exp2(fmaf(s[0][e], ra.scale_log2, -m));
 #pragma unroll
-            for (int e = 0; e < 16; e++) p[e] = fast_exp2(fmaf(s[b][e], ra.scale_log2, -m));
-            if constexpr (F32) {
-                float x = 0.0f, y = 0.0f;
+            for (int e = 0; e < 16; e += 2) x += p[e], y += p[e + 1];
+            l += x + y;
 #pragma unroll
-                for (int e = 0; e < 16; e += 2) x += p[e], y += p[e + 1];
-                l += x + y;
+            for (int o = 0; o < NO; o++) {
+                // (the tile's sum by itself, then added: a long context's sum is one of sums)
+                f32x16 z;
 #pragma unroll
-                for (int o = 0; o < NO; o++) {
-                    // (the tile's sum by itself, then added: a long context's sum is one of sums)
-                    f32x16 z;
+                for (int e = 0; e < 16; e++) z[e] = 0.0f;
 #pragma unroll
-                    for (int e = 0; e < 16; e++) z[e] = 0.0f;
-#pragma unroll
-                    for (int e = 0; e < 16; e++)
-                        z = __builtin_amdgcn_mfma_f32_32x32x2f32(
-                            *reinterpret_cast<const float*>(
-                                &v_lds[buf][(32 * b + 8 * (e >> 2) + 4 * half + (e & 3)) * VP +
-                                            4 * (32 * o + l32)]),
-                            p[e], z, 0, 0, 0);
-                    acc[o] += z;
-                }
-            } else {
-                typedef typename std::conditional<BF16 && !decltype(exact)::value, f16_t, T>::type TP;
-                constexpr bool SPLIT = BF16 && decltype(exact)::value;
-                u32x4 ph[2], pl[2];
-#pragma unroll
-                for (int x = 0; x < 2; x++)
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        const float p0 = p[8 * x + 2 * e], p1 = p[8 * x + 2 * e + 1];
-                        const uint32_t hi16 = pack2<TP>(p0, p1);
-                        ph[x][e] = hi16;
-                        if constexpr (SPLIT) {
-                            pl[x][e] = pack2<TP>(p0 - lo_f32<TP>(hi16), p1 - hi_f32<TP>(hi16));
-                            l += p0 + p1;
-                        } else {  // (the rounded weights that enter the product)
-                            l = __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, hi16), f16x2{1, 1}, l, false);
-                        }
-                    }
-                // V^T: 16 lanes read rows 4 half .. + 3 of 16 dims, and the rows 8 behind
-                const unsigned char* vr =
-                    &v_lds[buf][(32 * b + 4 * half + ((lane >> 2) & 3)) * VP + 32 * ((lane >> 4) & 1) +
-                                8 * (lane & 3)];
-#pragma unroll
-                for (int x = 0; x < 2; x++)
-#pragma unroll
-                    for (int o = 0; o < NO; o++) {
-                        const u32x2 v0 = lds_read_tr16(vr + 16 * x * VP + 64 * o);
-                        const u32x2 v1 = lds_read_tr16(vr + (16 * x + 8) * VP + 64 * o);
-                        const u32x4 A = {v0[0], v0[1], v1[0], v1[1]};
-                        acc[o] = mfma32x32x16<TP>(A, ph[x], acc[o]);
-                        if constexpr (SPLIT) acc[o] = mfma32x32x16<TP>(A, pl[x], acc[o]);
-                    }
+                for (int e = 0; e < 16; e++)
+                    z = __builtin_amdgcn_mfma_f32_32x32x2f32(
+                        *reinterpret_cast<const float*>(
+                            &v_lds[buf][(8 * (e >> 2) + 4 * half + (e & 3)) * VP + 4 * (32 * o + l32)]),
+                        p[e], z, 0, 0, 0);
+                acc[o] += z;
             }
+        } else {
+            typedef typename std::conditional<BF16 && !decltype(exact)::value, f16_t, T>::type TP;
+            constexpr bool SPLIT = BF16 && decltype(exact)::value;
+            // V^T: 16 lanes read rows 4 half .. + 3 of 16 dims, and the rows 8 behind; fragment n is of
+            // positions 16 (n / NO) .. + 15 and dims 32 (n % NO) .. + 31
+            const unsigned char* vr = &v_lds[buf][(4 * half + ((lane >> 2) & 3)) * VP +
+                                                  32 * ((lane >> 4) & 1) + 8 * (lane & 3)];
+            constexpr int NF = 2 * NB * NO, AHEAD = 4;
+            u32x4 vf[AHEAD];
+            auto read_v = [&](int n) __attribute__((always_inline)) {
+                const unsigned char* at = vr + 16 * (n / NO) * VP + 64 * (n % NO);
+                const u32x2 v0 = lds_read_tr16(at), v1 = lds_read_tr16(at + 8 * VP);
+                vf[n % AHEAD] = u32x4{v0[0], v0[1], v1[0], v1[1]};
+            };
+#pragma unroll
+            for (int n = 0; n < AHEAD; n++) read_v(n);
+            u32x4 ph[2 * NB], pl[2 * NB];
+#pragma unroll
+            for (int x = 0; x < 2 * NB; x++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const int at = 8 * (x & 1) + 2 * e;
+                    const float p0 = fast_exp2(fmaf(s[x >> 1][at], ra.scale_log2, -m));
+                    const float p1 = fast_exp2(fmaf(s[x >> 1][at + 1], ra.scale_log2, -m));
+                    const uint32_t hi16 = pack2<TP>(p0, p1);
+                    ph[x][e] = hi16;
+                    if constexpr (SPLIT) {
+                        pl[x][e] = pack2<TP>(p0 - lo_f32<TP>(hi16), p1 - hi_f32<TP>(hi16));
+                        l += p0 + p1;
+                    } else {  // (the rounded weights that enter the product)
+                        l = __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, hi16), f16x2{1, 1}, l, false);
+                    }
+                }
+            __builtin_amdgcn_sched_barrier(0);
+            __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+            for (int n = 0; n < NF; n++) {
+                f32x16& o = acc[n % NO];
+                o = mfma32x32x16<TP>(vf[n % AHEAD], ph[n / NO], o);
+                if constexpr (SPLIT) o = mfma32x32x16<TP>(vf[n % AHEAD], pl[n / NO], o);
+                if (n + AHEAD < NF) read_v(n + AHEAD);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            __builtin_amdgcn_s_setprio(0);
         }
     };
 
@@ -331,19 +369,22 @@ __global__ __launch_bounds__(64 * RT_WAVES, 2) void ranged_tiles_kernel(RtArgs r
         uint32_t slots = load_slots(t_begin), next = slots;
         if (t_begin + WIN < t_end) next = load_slots(t_begin + WIN);
         load_tile(slots, t_begin);
-        stage_tile(exact, t_begin, 0);
+        cut_tile(t_begin);
+#pragma unroll
+        for (int k = 0; k < NP; k++) stage_rows(exact, k, 0);
+        if (t_begin + 1 < t_end) load_tile(slots, t_begin + 1);
         __syncthreads();
         for (int t = t_begin; t < t_end; t++) {
-            const int buf = (t - t_begin) & 1;
-            if (t + 1 < t_end) {
-                if ((t + 1 - t_begin) % WIN == 0) {
+            // (behind the last tile whatever the registers hold goes to a buffer that nobody reads)
+            if (t + 1 < t_end) cut_tile(t + 1);
+            compute(exact, t, (t - t_begin) & 1, [&]() __attribute__((always_inline)) {
+                if (t + 2 >= t_end) return;
+                if ((t + 2 - t_begin) % WIN == 0) {
                     slots = next;
-                    if (t + 1 + WIN < t_end) next = load_slots(t + 1 + WIN);
+                    if (t + 2 + WIN < t_end) next = load_slots(t + 2 + WIN);
                 }
-                load_tile(slots, t + 1);
-            }
-            compute(exact, t, buf);
-            if (t + 1 < t_end) stage_tile(exact, t + 1, buf ^ 1);
+                load_tile(slots, t + 2);
+            });
             __syncthreads();
         }
         l = sum_across_halves(l);
@@ -374,8 +415,8 @@ __global__ __launch_bounds__(64 * RT_WAVES, 2) void ranged_tiles_kernel(RtArgs r
     }
 
     // ---- out: a lane holds dims 32 o + 8 (e / 4) + 4 half + e % 4 of its column
-    const bool final_out = ra.finals && pieces == 1;
-    const int64_t slot = ((int64_t)row * a.num_heads + head) * ra.max_pieces + piece;
+    const bool final_out = pt.finals && pieces == 1;
+    const int64_t slot = ((int64_t)row * a.num_heads + head) * pt.max_pieces + piece;
     const int64_t out_at = (int64_t)row * a.o_st + (int64_t)head * a.o_sh;
     const bool bad = live && real && !finite();
     if (live && real && !bad) {
@@ -391,11 +432,11 @@ __global__ __launch_bounds__(64 * RT_WAVES, 2) void ranged_tiles_kernel(RtArgs r
                 if (final_out)
                     store_run<4>(a.out, a.out_dtype, out_at + d, v);
                 else
-                    *reinterpret_cast<f32x4*>(ra.p_o + slot * D + d) = f32x4{v[0], v[1], v[2], v[3]};
+                    *reinterpret_cast<f32x4*>(pt.p_o + slot * D + d) = f32x4{v[0], v[1], v[2], v[3]};
             }
         if (!final_out && half == 0) {
-            ra.p_ml[2 * slot] = m;
-            ra.p_ml[2 * slot + 1] = l;
+            pt.p_ml[2 * slot] = m;
+            pt.p_ml[2 * slot + 1] = l;
         }
     }
 
@@ -413,7 +454,7 @@ __global__ __launch_bounds__(64 * RT_WAVES, 2) void ranged_tiles_kernel(RtArgs r
         const T* vp = static_cast<const T*>(a.v_pool) + (int64_t)g * a.num_slots * D;
         float cm = DEC_M0, cl = 0.0f, co[D / 64] = {};
         for (int t = t_begin; t < t_end; t++) {
-            const int tok = tok_of(t) + lane;
+            const int tok = sp.tok(t * UPT + lane / 16) + lane % 16;
             const bool sees = lane < TT && tok < c_hi && (tok >= c_lo || tok < sinks);
             float sc = -INFINITY;
             int slot_j = 0;
@@ -440,7 +481,7 @@ __global__ __launch_bounds__(64 * RT_WAVES, 2) void ranged_tiles_kernel(RtArgs r
             }
             cm = m_new;
         }
-        const int64_t c_slot = ((int64_t)c_row * a.num_heads + c_head) * ra.max_pieces + piece;
+        const int64_t c_slot = ((int64_t)c_row * a.num_heads + c_head) * pt.max_pieces + piece;
         const float inv = cl == 0.0f ? 0.0f : 1.0f / cl;
 #pragma unroll
         for (int x = 0; x < D / 64; x++) {
@@ -450,20 +491,22 @@ __global__ __launch_bounds__(64 * RT_WAVES, 2) void ranged_tiles_kernel(RtArgs r
                 const float y = cl == 0.0f ? 0.0f : co[x] * inv;
                 store_1(a.out, a.out_dtype, at, y);
             } else {
-                ra.p_o[c_slot * D + d] = co[x];
+                pt.p_o[c_slot * D + d] = co[x];
             }
         }
         if (!final_out && lane == 0) {
-            ra.p_ml[2 * c_slot] = cm;
-            ra.p_ml[2 * c_slot + 1] = cl;
+            pt.p_ml[2 * c_slot] = cm;
+            pt.p_ml[2 * c_slot + 1] = cl;
         }
     }
 }
 
 template <typename T>
-static int launch_ranged_tiles(const RtArgs& r, int items, hipStream_t stream) {
+static int launch_ranged_tiles(const RtArgs& r, hipStream_t stream) {
     auto kern = r.a.head_dim == 64 ? ranged_tiles_kernel<T, 64> : ranged_tiles_kernel<T, 128>;
-    kern<<<dim3(items, r.max_pieces), dim3(64 * RT_WAVES), 0, stream>>>(r);
+    int64_t grid = 0;
+    for (int i = 0; i < r.parts; i++) grid += (int64_t)r.part[i].items * r.part[i].max_pieces;
+    kern<<<dim3((unsigned)grid), dim3(64 * RT_WAVES), 0, stream>>>(r);
     return check_hip(hipGetLastError(), "attention over ranges launch");
 }
 

@@ -11,6 +11,15 @@ from flour_amd import _lib, ops
 
 pytestmark = pytest.mark.gpu
 
+
+@pytest.fixture(autouse=True)
+def prefixes_on_their_own():
+    """Small batches would not be cut at their prefixes: here they are, but for check_shared's other modes."""
+    _lib.lib().flour_hip_set_shared_prefix(1)
+    yield
+    _lib.lib().flour_hip_set_shared_prefix(-1)
+
+
 DT = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
 # What a weight is rounded to on the way into a product: two bf16 or f16 parts in decode steps of up to 16
 # query heads a kv head (half a step of 8 bits, twice: 2^-8 of 2^-8), one f16 number elsewhere (half a step,
@@ -49,6 +58,17 @@ def check(got, b, scale, eps, window=R.EVERY, sinks=0):
     want, mag, top, seen = R.expected(b, scale, window, sinks)
     v_max = float(b.v_pool[torch.isfinite(b.v_pool)].double().abs().max())
     R.close(got, want, R.bound(mag, top, seen, b.q.shape[2], eps, v_max))
+
+
+def check_shared(b, scale, eps, **kw):
+    """The prefixes once for their groups, without, and as the library chooses."""
+    lib = _lib.lib()
+    try:
+        for mode in (1, 0, -1):
+            assert lib.flour_hip_set_shared_prefix(mode) == 0
+            check(run(b, scale, **kw), b, scale, eps)
+    finally:
+        lib.flour_hip_set_shared_prefix(1)
 
 
 HEADS = [(8, 8, 64), (14, 2, 64), (32, 8, 128), (28, 4, 128)]
@@ -142,7 +162,7 @@ def test_decode_shared(dt, heads, starts, shared):
     kv = [450, 33, 0, 161, 1200]
     b = R.batch(DT[dt], *heads, 16, [1] * 5, kv, seed=len(starts), starts=starts, shared=shared)
     scale = heads[2] ** -0.5
-    check(run(b, scale, decode=True), b, scale, TILE_EPS[dt])
+    check_shared(b, scale, TILE_EPS[dt], decode=True)
 
 
 @pytest.mark.parametrize("dt", DT)
@@ -153,7 +173,7 @@ def test_prefill_shared(dt, heads, starts, shared, rows):
     kv = [450, 33, 5, 161, 1200]
     b = R.batch(DT[dt], *heads, 16, rows, kv, seed=len(starts), starts=starts, shared=shared)
     scale = heads[2] ** -0.5
-    check(run(b, scale), b, scale, TILE_EPS[dt])
+    check_shared(b, scale, TILE_EPS[dt])
 
 
 @pytest.mark.parametrize("bs", [1, 7, 32, 48])
@@ -163,7 +183,7 @@ def test_shared_other_pages(dt, bs):
         rows = [1] * 4 if decode else [4, 1, 7, 2]
         b = R.batch(DT[dt], 8, 2, 64, bs, rows, [300, 250, 260, 500], seed=bs, starts=[0, 3, 4],
                     shared=[245, 77])
-        check(run(b, 0.125, decode=decode), b, 0.125, TILE_EPS[dt])
+        check_shared(b, 0.125, TILE_EPS[dt], decode=decode)
 
 
 @pytest.mark.parametrize("dt", DT)
@@ -178,12 +198,12 @@ def test_shared_large_batches(dt, n, groups):
         rows = [1] * n if decode else [1 + s % 4 for s in range(n)]
         kv = [max(L, r) for L, r in zip(kv, rows)]
         b = R.batch(DT[dt], 8, 2, 128, 16, rows, kv, seed=n, starts=starts, shared=shared)
-        check(run(b, 0.09, decode=decode), b, 0.09, TILE_EPS[dt])
+        check_shared(b, 0.09, TILE_EPS[dt], decode=decode)
 
 
 def test_no_groups_is_plain_attention():
     b = R.batch(torch.bfloat16, 8, 2, 128, 16, [1] * 3, [100, 7, 650], seed=1, starts=[0], shared=[])
-    check(run(b, 0.09, decode=True), b, 0.09, TILE_EPS["bf16"])
+    check_shared(b, 0.09, TILE_EPS["bf16"], decode=True)
 
 
 # ------------------------------------------------------------------ values that are not numbers
@@ -364,10 +384,10 @@ def test_table_entries_that_are_not_visible_may_be_anything(dt):
 def test_other_scales(dt, scale):
     b = R.batch(DT[dt], 8, 2, 64, 16, [40, 3], [100, 300], seed=12, starts=[0, 2], shared=[64])
     check(run(b, scale, 50, 2), b, scale, TILE_EPS[dt], 50, 2)
-    check(run(b, scale), b, scale, TILE_EPS[dt])
+    check_shared(b, scale, TILE_EPS[dt])
     b = R.batch(DT[dt], 8, 2, 64, 16, [1, 1], [100, 300], seed=12, starts=[0, 2], shared=[64])
     check(run(b, scale, 50, 2, decode=True), b, scale, DECODE_EPS[dt], 50, 2)
-    check(run(b, scale, decode=True), b, scale, TILE_EPS[dt])
+    check_shared(b, scale, TILE_EPS[dt], decode=True)
 
 
 def calls(b, d):
