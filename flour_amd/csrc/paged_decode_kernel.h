@@ -45,6 +45,9 @@ struct DecodeRange {
     int window, sinks;
     int out_dtype;  // of AnyOut outputs
 };
+// How a launch's waves share the chunks. DEC_PAIRS (windows): a workgroup a (sequence, kv head), whose waves
+// take equal parts of its chunks and fold their states through LDS, so nothing is left to merge.
+enum DecodeSplit { DEC_RANGES, DEC_PAIRS };
 // The output's type is a field of the call.
 struct AnyOut {
     uint8_t bits;
@@ -143,11 +146,20 @@ __device__ __forceinline__ f32x4 mfma16x16x4_f32(float a, float b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
 }
 
+// Waves of a DEC_PAIRS workgroup at most, and a wave's LDS there: its K tile, then its state.
+static constexpr int DEC_PAIR_WAVES = 8;
+__host__ __device__ constexpr int dec_pair_lds(int d, int elem_bytes) {
+    const int k = 16 * dec_kpitch(d, elem_bytes), state = 64 * (d * 16 / 64 + 2) * 4;
+    return k > state ? k : state;
+}
+
 // One wave per workgroup; each wave owns one contiguous range of the chunk list. D is the head
 // dim, 128 or 64. A lane's K/V share of a 16-token tile is rows 4lg .. 4lg + 3 at 16-byte
 // (D 128: dims 8lc ..) or 8-byte (D 64: dims 4lc ..) width, so a wave reads whole rows.
-template <typename T, typename TO, bool BS16, int D, bool FUSE, bool WTS, bool RNG = false>
-__global__ __launch_bounds__(64, 2) void paged_decode_mfma_kernel(
+// RNG: the context is looked at through ws.rng.
+template <typename T, typename TO, bool BS16, int D, bool FUSE, bool WTS, bool RNG = false,
+          int SPLIT = DEC_RANGES>
+__global__ __launch_bounds__(SPLIT == DEC_PAIRS ? 64 * DEC_PAIR_WAVES : 64, 2) void paged_decode_mfma_kernel(
     TO* __restrict__ out, const T* __restrict__ q, const T* __restrict__ k_pool,
     const T* __restrict__ v_pool, const int32_t* __restrict__ block_tables, int max_blocks,
     const int32_t* __restrict__ context_lens, int batch, int num_heads, int kv_heads, int n_rep,
@@ -163,9 +175,14 @@ __global__ __launch_bounds__(64, 2) void paged_decode_mfma_kernel(
     // so an instruction reads four 256-byte row segments in every form (128 at D 64, 16-bit).
     constexpr int NL = F32 ? D / 64 : TILES;
     typedef typename std::conditional<F32 || D == 128, u32x4, u32x2>::type Ld;
-    extern __shared__ int pre[];  // pre[b] = chunks of sequences 0..b-1; pre[batch] = all
-    __shared__ __attribute__((aligned(16))) unsigned char kt[16 * KP];  // one K tile
-    const int lane = threadIdx.x, lg = lane >> 4, lc = lane & 15;
+    constexpr bool PAIRS = SPLIT == DEC_PAIRS;
+    // pre[b] = chunks of sequences 0..b-1; pre[batch] = all. PAIRS: the waves' LDS instead.
+    extern __shared__ __attribute__((aligned(16))) int pre[];
+    __shared__ __attribute__((aligned(16))) unsigned char kt_one[PAIRS ? 16 : 16 * KP];  // one K tile
+    const int lane = PAIRS ? threadIdx.x & 63 : threadIdx.x, lg = lane >> 4, lc = lane & 15;
+    const int w_id = PAIRS ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0;
+    unsigned char* const kt = PAIRS ? reinterpret_cast<unsigned char*>(pre) + w_id * dec_pair_lds(D, sizeof(T))
+                                    : kt_one;
 
     // ---- exclusive prefix sum of per-sequence chunk counts. Up to 64 sequences stay in
     // registers, one per lane (clamped context length and prefix), so that locating a segment
@@ -178,8 +195,9 @@ __global__ __launch_bounds__(64, 2) void paged_decode_mfma_kernel(
         if constexpr (RNG) return part(min(ctx, max_ctx)).chunks();
         return decode_chunks<CHUNK>(ctx, max_ctx);
     };
-    int my_ctx = 0, my_pre = 0, all_chunks;
-    if (in_lanes) {
+    int my_ctx = 0, my_pre = 0, all_chunks = 0;
+    if (PAIRS) {
+    } else if (in_lanes) {
         my_ctx = lane < batch ? min(context_lens[lane], max_ctx) : 0;
         const int n = chunks_of(my_ctx);
         const int incl = wave_incl_sum(n);
@@ -218,7 +236,7 @@ __global__ __launch_bounds__(64, 2) void paged_decode_mfma_kernel(
     }
     const int64_t total = (int64_t)kv_heads * all_chunks;
     const int64_t nwg = range_count(total, gridDim.x), wgi = blockIdx.x;
-    if (total == 0 || wgi >= nwg) return;
+    if (!PAIRS && (total == 0 || wgi >= nwg)) return;
     // 32-bit divisions whenever they fit: a 64-bit one is ~0.3 us of instructions, and the
     // range bounds and the first segments stand before the wave's first load
     const bool narrow = ranges_narrow(total, nwg, ws.xcd_w);
@@ -228,7 +246,16 @@ __global__ __launch_bounds__(64, 2) void paged_decode_mfma_kernel(
     // buffer load that takes its offset into a per-lane loop.
     int64_t lo;
     int len;
-    if (narrow) {
+    // PAIRS: the pair, its context, its chunks
+    int pb = 0, pg = 0, p_ctx = 0, p_nch = 0;
+    if constexpr (PAIRS) {
+        pb = blockIdx.x / kv_heads, pg = blockIdx.x - pb * kv_heads;
+        p_ctx = min(__builtin_amdgcn_readfirstlane(context_lens[pb]), max_ctx);
+        p_nch = chunks_of(p_ctx);
+        const int waves = blockDim.x >> 6;
+        lo = (int64_t)p_nch * w_id / waves;
+        len = (int)((int64_t)p_nch * (w_id + 1) / waves - lo);
+    } else if (narrow) {
         const WaveRanges<uint32_t> wr(total, nwg, ws.xcd_w);
         const uint32_t a = wr.lo((uint32_t)wgi);
         lo = (uint32_t)__builtin_amdgcn_readfirstlane((int)a);
@@ -257,6 +284,12 @@ __global__ __launch_bounds__(64, 2) void paged_decode_mfma_kernel(
     auto seg_at = [&](int at) -> Seg {
         const int64_t x = lo + at;
         Seg sg;
+        if constexpr (PAIRS) {
+            sg.b = pb, sg.g = pg, sg.nch = p_nch, sg.tok_end = p_ctx;
+            sg.cb = (int)x;
+            sg.ce = sg.cb + min(DEC_SEG, len - at);
+            return sg;
+        }
         int before, ctx;  // chunks per head before sequence b, its clamped context length
         if (in_lanes) {   // largest b with kv_heads * pre[b] <= x
             const uint64_t le = __ballot(lane < batch && (int64_t)kv_heads * my_pre <= x);
@@ -516,6 +549,7 @@ __global__ __launch_bounds__(64, 2) void paged_decode_mfma_kernel(
     // Piece epilogue from registers: lane (lg, lc) holds head lc, dims (D / 4) lg + NV r + nn
     // (r < 4, nn < NV): D / 4 contiguous dims; fp32 pools: dims 64i + 16lg + 4r + e for nn = 4i + e.
     auto epilogue = [&](int b, int g, bool complete, bool first_piece) {
+        if constexpr (PAIRS) return;  // (at the end, all waves together)
         lsum = sum_across_rows(lsum);
         // lg made opaque here, so the per-lane output addresses are formed at the store instead
         // of being hoisted out of the stream as 64-bit values (which spill, and a spill reload
@@ -668,6 +702,52 @@ __global__ __launch_bounds__(64, 2) void paged_decode_mfma_kernel(
         }
     };
 
+    // PAIRS: the waves' states through LDS, then wave w writes dims (D / 4) lg + NV r .. of r = w, w + waves ..
+    // (fp32: 64 i + 16 lg + 4 r ..), folded over the waves.
+    auto fold = [&]() {
+        constexpr int WAVE = dec_pair_lds(D, sizeof(T)) / 4;
+        float* const all = reinterpret_cast<float*>(pre);
+        lsum = sum_across_rows(lsum);
+        float* const mine = all + w_id * WAVE;
+#pragma unroll
+        for (int nn = 0; nn < NV; nn++) *reinterpret_cast<f32x4*>(mine + (nn * 64 + lane) * 4) = acc[nn];
+        mine[NV * 256 + lane] = m;
+        mine[NV * 256 + 64 + lane] = lsum;
+        __syncthreads();
+        const int waves = blockDim.x >> 6;
+        if (w_id >= 4) return;
+        float M = DEC_M0, L = 0.0f;
+        for (int x = 0; x < waves; x++) M = fmaxf(M, all[x * WAVE + NV * 256 + lane]);
+        for (int x = 0; x < waves; x++)
+            L += fast_exp2(all[x * WAVE + NV * 256 + lane] - M) * all[x * WAVE + NV * 256 + 64 + lane];
+        const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+        if (lc >= n_rep) return;
+        const int64_t o_at = ((int64_t)pb * num_heads + (int64_t)pg * n_rep + lc) * D + (F32 ? 16 : D / 4) * lg;
+        for (int r = w_id; r < 4; r += waves) {
+            float o[NV];
+#pragma unroll
+            for (int nn = 0; nn < NV; nn++) o[nn] = 0.0f;
+            for (int x = 0; x < waves; x++) {
+                const float* from = all + x * WAVE;
+                const float w = fast_exp2(from[NV * 256 + lane] - M) * inv;
+#pragma unroll
+                for (int nn = 0; nn < NV; nn++) o[nn] = fmaf(w, from[(nn * 64 + lane) * 4 + r], o[nn]);
+            }
+            if (L == 0.0f)
+#pragma unroll
+                for (int nn = 0; nn < NV; nn++) o[nn] = 0.0f;
+#pragma unroll
+            for (int h4 = 0; h4 < NV; h4 += 4)
+                store_run<4>(out, rng.out_dtype, o_at + (F32 ? 16 * h4 + 4 * r : NV * r + h4), o + h4);
+        }
+    };
+    if constexpr (PAIRS) {
+        if (len == 0) {  // (fewer chunks than waves, or an empty context: zero rows)
+            fold();
+            return;
+        }
+    }
+
     Seg cur = seg_at(0);
     NewRows nr{};
     if constexpr (FUSE) {
@@ -725,7 +805,7 @@ __global__ __launch_bounds__(64, 2) void paged_decode_mfma_kernel(
             return;
         }
         // end of a segment
-        const bool piece_end = !has_nxt || nxt.b != cur.b || nxt.g != cur.g;
+        const bool piece_end = !PAIRS && (!has_nxt || nxt.b != cur.b || nxt.g != cur.g);
         if (piece_end) epilogue(cur.b, cur.g, pc0 == 0 && cur.ce == cur.nch, first_piece);
         if (!has_nxt) return;
         if (piece_end) {
@@ -769,6 +849,7 @@ __global__ __launch_bounds__(64, 2) void paged_decode_mfma_kernel(
     } else {
         step(pf_off{}, ka, va, kb, vb);
     }
+    if constexpr (PAIRS) fold();
 }
 
 // Merge of the pieces of pairs cut by wave ranges, and zero rows for empty contexts: one

@@ -57,6 +57,22 @@ static size_t stream_bytes(int batch, int num_heads, int kv_heads, int head_dim)
     return decode_ws_bytes(decode_workgroups(FLOUR_DTYPE_F32), num_heads / kv_heads, head_dim, batch);
 }
 
+// Windows: whether each (sequence, kv head) is a workgroup of four waves with nothing to merge, rather than a
+// part of the ranges of one wave each. A workgroup's time goes with its chunks (0.19-0.26 us each over 16-bit
+// pools, 0.25 / 0.75 over fp32 ones of 64 / 128 dims), the ranges' with the bytes of all and a second launch.
+// 32 / 8 heads of 128 in bf16, ranges / workgroups in us: 1 sequence, window 128 9.3 / 6.5, 1,024 10.6 / 13.8;
+// 16, 1,024 20.1 / 20.1; 40, 128 14.7 / 9.9, 1,024 41.2 / 39.1. 8 / 8 of 64: 64, 1,024 34.5 / 27.0, 4 of 4,096
+// 13.3 / 30.2. Eight waves are within 10% of four, two behind them but on large batches.
+static constexpr int PAIR_WAVES = 4;
+static int g_window_pairs = -1;  // 1 always, 0 never, -1 by this (a test switch)
+static bool prefer_pairs(int64_t pairs, int64_t chunks, int head_dim, int dtype) {
+    if (pairs > 0x7fffffff || g_window_pairs >= 0) return pairs <= 0x7fffffff && g_window_pairs > 0;
+    if (dtype == FLOUR_DTYPE_F32 && head_dim == 128) return chunks <= 8;
+    const double per = dtype == FLOUR_DTYPE_F32 ? 0.25 : head_dim == 64 ? 0.19 : 0.26;
+    const double bytes = 2.0 * dec_chunk(elem_bytes(dtype)) * head_dim * elem_bytes(dtype);
+    return 5.0 + per * chunks <= 9.3 + pairs * chunks * bytes / 5.5e6;
+}
+
 static int launch_stream(const RangedAttn& a, void* workspace, hipStream_t stream) {
     const int nwg = decode_workgroups(a.dtype);
     RangedStream st{};
@@ -67,6 +83,9 @@ static int launch_stream(const RangedAttn& a, void* workspace, hipStream_t strea
     const int64_t span = std::min<int64_t>(a.max_kv, (int64_t)a.window + a.sinks + 2 * chunk);
     const int64_t half = (int64_t)a.num_seqs * a.kv_heads * ((span + chunk - 1) / chunk) / 2;
     st.grid = (int)std::max<int64_t>(1, std::min<int64_t>(half, nwg));
+    const int64_t pairs = (int64_t)a.num_seqs * a.kv_heads;
+    if (prefer_pairs(pairs, (span + chunk - 1) / chunk, a.head_dim, a.dtype))
+        st.grid = (int)pairs, st.pair_waves = PAIR_WAVES;
     auto launch = a.dtype == FLOUR_DTYPE_F32    ? launch_ranged_decode_f32
                   : a.dtype == FLOUR_DTYPE_BF16 ? launch_ranged_decode_bf16
                                                 : launch_ranged_decode_f16;
@@ -91,28 +110,31 @@ static bool tiles_take(const RangedAttn& a) {
              (uint64_t)(a.o_st * oes) | (uint64_t)(a.o_sh * oes)) & 15) == 0;
 }
 
-// How a launch over `units` units of up to unit_rows rows (rows in all) and unit_kv positions each is cut:
-// the grid's items, and the pieces of a pair, so that the launch has about two workgroups a CU.
+// A launch's items and the pieces that their tiles are cut into.
 struct TilePlan {
     int items, max_pieces, piece_tiles;
     size_t bytes;  // of the pieces
 };
-static int g_ranged_wgs = 4, g_ranged_min = 4;
-// Prefixes as a part of their own: 1 always, 0 never, -1 by prefer_shared (a test switch).
-static int g_ranged_shared = -1;
-static TilePlan tile_plan(int64_t units, int64_t unit_rows, int64_t rows, int64_t unit_kv, int num_heads,
-                          int kv_heads, int head_dim, int dtype, bool finals) {
-    const int64_t n_rep = num_heads / kv_heads, tt = rt_tokens(elem_bytes(dtype));
+static int g_ranged_wgs = 3, g_ranged_min = 4, g_ranged_fmin = 12;
+// Units of up to unit_rows rows (rows in all), an item for each of their column tiles and kv heads.
+static int64_t tile_items(int64_t units, int64_t unit_rows, int64_t rows, int64_t n_rep, int64_t kv_heads) {
     unit_rows = std::min(unit_rows, rows);
     const int64_t tiles = std::min(rows * n_rep / RT_COLS + units,
                                    units * ((unit_rows * n_rep + RT_COLS - 1) / RT_COLS));
+    return std::max<int64_t>(1, tiles * kv_heads);
+}
+// Tiles of a piece, so that `steps` of them come to two workgroups a CU, `least` at least: a shorter piece
+// costs more in its ends and its merge than it saves.
+static int64_t tiles_of_piece(int64_t steps, int64_t least) {
+    const int64_t slots = g_ranged_wgs * device_cus() / 2;
+    return std::max(least, (steps + slots - 1) / slots);
+}
+static TilePlan tile_plan(int64_t items, int64_t longest, int64_t piece_tiles, int64_t rows, int num_heads,
+                          int head_dim, bool finals) {
     TilePlan p;
-    p.items = (int)std::max<int64_t>(1, tiles * kv_heads);
-    const int64_t longest = unit_kv / tt + 3;  // (a front tile, and ends that are not whole)
-    const int64_t want = std::max<int64_t>(1, g_ranged_wgs * device_cus() / 2 / p.items);
-    // (a piece of fewer tiles costs more in its ends and its merge than it saves)
-    p.piece_tiles = (int)std::max<int64_t>(g_ranged_min, (longest + want - 1) / want);
-    p.max_pieces = (int)std::max<int64_t>(1, std::min<int64_t>(want, longest / p.piece_tiles));
+    p.items = (int)items;
+    p.piece_tiles = (int)piece_tiles;
+    p.max_pieces = (int)((longest + piece_tiles - 1) / piece_tiles);
     p.bytes = finals && p.max_pieces == 1
                   ? 0
                   : up256((size_t)rows * num_heads * p.max_pieces * 2 * sizeof(float)) +
@@ -142,25 +164,34 @@ static int launch_tiles(const RtArgs& r, hipStream_t stream) {
     return launch(r, stream);
 }
 
-// Rows over what they see: one launch, and a merge where pairs are cut.
+// Rows over what they see: one launch, and a merge where items are cut.
 static TilePlan rows_plan(int num_seqs, int max_rows, int rows, int num_heads, int kv_heads, int head_dim,
                           int max_kv, int window, int sinks, int dtype) {
-    const int64_t n_rep = num_heads / kv_heads;
+    const int64_t n_rep = num_heads / kv_heads, tt = rt_tokens(elem_bytes(dtype));
+    const int64_t items = tile_items(num_seqs, max_rows, rows, n_rep, kv_heads);
     const int64_t span = (int64_t)window + sinks + RT_COLS / n_rep + 2;
-    return tile_plan(num_seqs, max_rows, rows, std::min<int64_t>(max_kv, span), num_heads, kv_heads,
-                     head_dim, dtype, true);
+    const int64_t longest = std::min<int64_t>(max_kv, span) / tt + 2;  // (ends that are not whole tiles)
+    return tile_plan(items, longest, tiles_of_piece(items * longest, g_ranged_fmin), rows, num_heads, head_dim,
+                     true);
 }
 
-// The prefixes by groups, then each sequence's own positions, then both together.
+// Prefixes as a part of their own: 1 always, 0 never, -1 by prefer_shared (a test switch).
+static int g_ranged_shared = -1;
+
+// The prefixes by groups and each sequence's own positions, cut alike.
 struct SharedPlan {
     TilePlan prefix, own;
 };
 static SharedPlan shared_plan(int num_seqs, int num_groups, int max_rows, int rows, int num_heads,
                               int kv_heads, int head_dim, int max_kv, int max_shared, int dtype) {
-    return SharedPlan{tile_plan(num_groups, rows, rows, max_shared, num_heads, kv_heads, head_dim, dtype,
-                                false),
-                      tile_plan(num_seqs, max_rows, rows, max_kv, num_heads, kv_heads, head_dim, dtype,
-                                false)};
+    const int64_t n_rep = num_heads / kv_heads, tt = rt_tokens(elem_bytes(dtype));
+    const int64_t items_p = tile_items(num_groups, rows, rows, n_rep, kv_heads);
+    const int64_t items_o = tile_items(num_seqs, max_rows, rows, n_rep, kv_heads);
+    // (a sequence of a group with a shorter prefix can have more of its own: its pieces are longer)
+    const int64_t long_p = max_shared / tt + 1, long_o = std::max(0, max_kv - max_shared) / tt + 2;
+    const int64_t piece = tiles_of_piece(items_p * long_p + items_o * long_o, g_ranged_min);
+    return SharedPlan{tile_plan(items_p, long_p, piece, rows, num_heads, head_dim, false),
+                      tile_plan(items_o, long_o, piece, rows, num_heads, head_dim, false)};
 }
 
 // Whether prefixes are worth a part of their own, by an estimate of both ways in us from the host's bounds.
@@ -422,8 +453,14 @@ extern "C" int flour_hip_set_shared_prefix(int mode) {
     return FLOUR_OK;
 }
 
-extern "C" int flour_hip_set_ranged(int wgs, int least) {
-    g_ranged_wgs = wgs, g_ranged_min = least;
+extern "C" int flour_hip_set_window_pairs(int mode) {
+    if (mode < -1 || mode > 1) return FLOUR_ERR_INVALID_ARGUMENT;
+    g_window_pairs = mode;
+    return FLOUR_OK;
+}
+
+extern "C" int flour_hip_set_ranged(int wgs, int least, int fleast) {
+    g_ranged_wgs = wgs, g_ranged_min = least, g_ranged_fmin = fleast;
     switch_set();
     return 0;
 }

@@ -71,6 +71,19 @@ def check_shared(b, scale, eps, **kw):
         lib.flour_hip_set_shared_prefix(1)
 
 
+def check_steps(b, scale, eps, window, sinks):
+    """Workgroups of a (sequence, kv head), ranges of chunks, and as the library chooses."""
+    lib = _lib.lib()
+    try:
+        for mode in (1, 0, -1):
+            assert lib.flour_hip_set_window_pairs(mode) == 0
+            got = run(b, scale, window, sinks, decode=True)
+            check(got, b, scale, eps, window, sinks)
+    finally:
+        lib.flour_hip_set_window_pairs(-1)
+    return got
+
+
 HEADS = [(8, 8, 64), (14, 2, 64), (32, 8, 128), (28, 4, 128)]
 
 
@@ -82,9 +95,8 @@ def test_decode_window(dt, heads, window, sinks):
     kv = [0, 1, 2, window, window + 1, window + sinks, window + sinks + 1, 63, 64, 65, 500, 777]
     b = R.batch(DT[dt], *heads, 16, [1] * len(kv), kv, seed=window)
     scale = heads[2] ** -0.5
-    got = run(b, scale, window, sinks, decode=True)
+    got = check_steps(b, scale, decode_eps(dt, heads), window, sinks)
     assert got.dtype == DT[dt]
-    check(got, b, scale, decode_eps(dt, heads), window, sinks)
     assert not bool(got[0].any())
 
 
@@ -92,7 +104,7 @@ def test_decode_window(dt, heads, window, sinks):
 @pytest.mark.parametrize("dt", DT)
 def test_decode_window_other_pages(dt, bs):
     b = R.batch(DT[dt], 8, 2, 64, bs, [1] * 5, [3, 200, 1000, 333, 97], seed=bs)
-    check(run(b, 0.125, 90, 5, decode=True), b, 0.125, DECODE_EPS[dt], 90, 5)
+    check_steps(b, 0.125, DECODE_EPS[dt], 90, 5)
 
 
 @pytest.mark.parametrize("dt,odt", [("bf16", "f32"), ("f16", "bf16"), ("f32", "f16")])
@@ -108,7 +120,7 @@ def test_decode_window_output_types(dt, odt):
 def test_decode_window_batches(dt, n):
     kv = [(s * 7919) % 3000 for s in range(n)]
     b = R.batch(DT[dt], 8, 4, 128, 16, [1] * n, kv, seed=n)
-    check(run(b, 0.09, 600, 20, decode=True), b, 0.09, DECODE_EPS[dt], 600, 20)
+    check_steps(b, 0.09, DECODE_EPS[dt], 600, 20)
 
 
 # ------------------------------------------------------------------ prefill, window
@@ -227,8 +239,7 @@ def test_what_no_row_sees_does_not_matter(dt, heads, value):
     for window, sinks in ((5, 0), (40, 3), (100, 20)):
         kv = [1, 30, 39, 41, 120, 121, 700]
         b = R.batch(DT[dt], *heads, 16, [1] * 7, kv, seed=2)
-        check(run(poison(b, window, sinks, value), scale, window, sinks, decode=True), b, scale,
-              DECODE_EPS[dt], window, sinks)
+        check_steps(poison(b, window, sinks, value), scale, DECODE_EPS[dt], window, sinks)
         b = R.batch(DT[dt], *heads, 16, [1, 30, 4, 1, 70, 1, 90], kv, seed=2)
         check(run(poison(b, window, sinks, value), scale, window, sinks), b, scale, TILE_EPS[dt],
               window, sinks)
