@@ -228,6 +228,7 @@ EXTRA_SIGNATURES: dict[str, tuple] = {
     "flour_hip_set_prefill_q8": (_c_int, [_c_int]),
     "flour_hip_set_shared_prefix": (_c_int, [_c_int]),
     "flour_hip_set_window_pairs": (_c_int, [_c_int]),
+    "flour_hip_set_tile_halves": (_c_int, [_c_int]),
     "flour_hip_set_batch_split": (_c_int, [_c_int]),
     "flour_hip_set_batch_fuse": (_c_int, [_c_int]),
     "flour_hip_empty_launch": (_c_int, [_vp]),

@@ -112,26 +112,33 @@ static bool tiles_take(const RangedAttn& a) {
 
 // A launch's items and the pieces that their tiles are cut into.
 struct TilePlan {
-    int items, max_pieces, piece_tiles;
+    int items, max_pieces, piece_tiles, halves;
     size_t bytes;  // of the pieces
 };
-static int g_ranged_wgs = 3, g_ranged_min = 4, g_ranged_fmin = 12;
+// Waves that share 32 columns: 1 or 2, 0 by the plans' rules (a test switch).
+static int g_tile_halves = 0;
+// Three workgroups for two CUs are aimed at: 2 / 3 / 4 for two in us: 64 sequences of one prefix 8,192 + up to
+// 512 57.0 / 44.6 / 48.9, drafted rows 55.6 / 50.3 / 55.6, fp32 28.7 / 23.3 / 23.1. Pieces have four tiles at
+// least, twelve where a launch could do without any (which saves the merge).
+static constexpr int WGS_OF_TWO_CUS = 3, LEAST_TILES = 4, LEAST_TILES_FINAL = 12;
 // Units of up to unit_rows rows (rows in all), an item for each of their column tiles and kv heads.
-static int64_t tile_items(int64_t units, int64_t unit_rows, int64_t rows, int64_t n_rep, int64_t kv_heads) {
+static int64_t tile_items(int64_t units, int64_t unit_rows, int64_t rows, int64_t n_rep, int64_t kv_heads,
+                          int64_t cols) {
     unit_rows = std::min(unit_rows, rows);
-    const int64_t tiles = std::min(rows * n_rep / RT_COLS + units,
-                                   units * ((unit_rows * n_rep + RT_COLS - 1) / RT_COLS));
+    const int64_t tiles =
+        std::min(rows * n_rep / cols + units, units * ((unit_rows * n_rep + cols - 1) / cols));
     return std::max<int64_t>(1, tiles * kv_heads);
 }
-// Tiles of a piece, so that `steps` of them come to two workgroups a CU, `least` at least: a shorter piece
-// costs more in its ends and its merge than it saves.
+// Tiles of a piece, so that `steps` of them come to so many workgroups, `least` at least: a shorter piece costs
+// more in its ends and its merge than it saves.
 static int64_t tiles_of_piece(int64_t steps, int64_t least) {
-    const int64_t slots = g_ranged_wgs * device_cus() / 2;
+    const int64_t slots = WGS_OF_TWO_CUS * device_cus() / 2;
     return std::max(least, (steps + slots - 1) / slots);
 }
-static TilePlan tile_plan(int64_t items, int64_t longest, int64_t piece_tiles, int64_t rows, int num_heads,
-                          int head_dim, bool finals) {
+static TilePlan tile_plan(int halves, int64_t items, int64_t longest, int64_t piece_tiles, int64_t rows,
+                          int num_heads, int head_dim, bool finals) {
     TilePlan p;
+    p.halves = halves;
     p.items = (int)items;
     p.piece_tiles = (int)piece_tiles;
     p.max_pieces = (int)((longest + piece_tiles - 1) / piece_tiles);
@@ -142,8 +149,9 @@ static TilePlan tile_plan(int64_t items, int64_t longest, int64_t piece_tiles, i
     return p;
 }
 
-static RtArgs tile_args(const RangedAttn& a) {
+static RtArgs tile_args(const RangedAttn& a, int halves) {
     RtArgs r{};
+    r.cols = rt_cols(halves), r.tile = rt_tokens(elem_bytes(a.dtype), halves);
     r.a = a, r.n_rep = a.num_heads / a.kv_heads;
     r.scale_log2 = a.scale * 1.4426950408889634f;
     return r;
@@ -157,21 +165,31 @@ static void add_part(RtArgs* r, int kind, const TilePlan& p, bool finals, char* 
         ws + up256((size_t)r->a.rows * r->a.num_heads * p.max_pieces * 2 * sizeof(float)));
 }
 
-static int launch_tiles(const RtArgs& r, hipStream_t stream) {
+static int launch_tiles(const RtArgs& r, int halves, hipStream_t stream) {
     auto launch = r.a.dtype == FLOUR_DTYPE_F32    ? launch_ranged_tiles_f32
                   : r.a.dtype == FLOUR_DTYPE_BF16 ? launch_ranged_tiles_bf16
                                                   : launch_ranged_tiles_f16;
-    return launch(r, stream);
+    return launch(r, halves, stream);
 }
 
 // Rows over what they see: one launch, and a merge where items are cut.
 static TilePlan rows_plan(int num_seqs, int max_rows, int rows, int num_heads, int kv_heads, int head_dim,
                           int max_kv, int window, int sinks, int dtype) {
-    const int64_t n_rep = num_heads / kv_heads, tt = rt_tokens(elem_bytes(dtype));
-    const int64_t items = tile_items(num_seqs, max_rows, rows, n_rep, kv_heads);
-    const int64_t span = (int64_t)window + sinks + RT_COLS / n_rep + 2;
+    const int64_t n_rep = num_heads / kv_heads;
+    // Two waves for 32 columns while that leaves the chip unfilled: half the time of an item, 1.3 times that of
+    // all. Waves of 64 positions / half of them in us: 16 bits, 32 / 8 heads of 128, window 512, 80 items (of
+    // 128 columns) 24.9 / 20.5, 256 27.5 / 27.5, 416 35.2 / 44.7; 8 / 8 of 64, 256 22.6 / 20.6, 384 32.2 / 26.6;
+    // 14 / 2, 660 41.3 / 39.1; fp32, 8 / 8 of 64, 128 52.6 / 39.2, 384 107.8 / 109.5; 32 / 8 of 128, 80 79.9 /
+    // 59.0, 256 124 / 116 (window 128: 48.9 / 54.3), 416 162 / 188.
+    const int64_t few = dtype == FLOUR_DTYPE_F32 ? (head_dim == 64 ? 384 : 128) : (head_dim == 64 ? 640 : 256);
+    int halves = tile_items(num_seqs, max_rows, rows, n_rep, kv_heads, rt_cols(1)) <= few ? 2 : 1;
+    if (g_tile_halves > 0) halves = g_tile_halves;
+    const int cols = rt_cols(halves);
+    const int64_t tt = rt_tokens(elem_bytes(dtype), halves);
+    const int64_t items = tile_items(num_seqs, max_rows, rows, n_rep, kv_heads, cols);
+    const int64_t span = (int64_t)window + sinks + cols / n_rep + 2;
     const int64_t longest = std::min<int64_t>(max_kv, span) / tt + 2;  // (ends that are not whole tiles)
-    return tile_plan(items, longest, tiles_of_piece(items * longest, g_ranged_fmin), rows, num_heads, head_dim,
+    return tile_plan(halves, items, longest, tiles_of_piece(items * longest, LEAST_TILES_FINAL), rows, num_heads, head_dim,
                      true);
 }
 
@@ -184,14 +202,23 @@ struct SharedPlan {
 };
 static SharedPlan shared_plan(int num_seqs, int num_groups, int max_rows, int rows, int num_heads,
                               int kv_heads, int head_dim, int max_kv, int max_shared, int dtype) {
-    const int64_t n_rep = num_heads / kv_heads, tt = rt_tokens(elem_bytes(dtype));
-    const int64_t items_p = tile_items(num_groups, rows, rows, n_rep, kv_heads);
-    const int64_t items_o = tile_items(num_seqs, max_rows, rows, n_rep, kv_heads);
+    const int64_t n_rep = num_heads / kv_heads;
+    // Two waves for 32 columns, unless large groups make the prefixes' products the most of the work. Waves of
+    // 64 positions / half of them in us, 32 / 8 heads of 128 in bf16: 64 sequences of one prefix 4,096 + 256
+    // 41.2 / 36.1, 1,024 + 1,024 84 / 72, 16,384 + 128 55.5 / 61.0; of eight 4,096 + 256 59.7 / 51.1; 64 / 8
+    // heads, one prefix and six rows each 115.6 / 132.0.
+    const int64_t tiles_p = tile_items(num_groups, rows, rows, n_rep, kv_heads, rt_cols(1)) * (max_shared / 64);
+    int halves = rows * n_rep >= (int64_t)192 * num_groups && tiles_p >= 3000 ? 1 : 2;
+    if (g_tile_halves > 0) halves = g_tile_halves;
+    const int cols = rt_cols(halves);
+    const int64_t tt = rt_tokens(elem_bytes(dtype), halves);
+    const int64_t items_p = tile_items(num_groups, rows, rows, n_rep, kv_heads, cols);
+    const int64_t items_o = tile_items(num_seqs, max_rows, rows, n_rep, kv_heads, cols);
     // (a sequence of a group with a shorter prefix can have more of its own: its pieces are longer)
     const int64_t long_p = max_shared / tt + 1, long_o = std::max(0, max_kv - max_shared) / tt + 2;
-    const int64_t piece = tiles_of_piece(items_p * long_p + items_o * long_o, g_ranged_min);
-    return SharedPlan{tile_plan(items_p, long_p, piece, rows, num_heads, head_dim, false),
-                      tile_plan(items_o, long_o, piece, rows, num_heads, head_dim, false)};
+    const int64_t piece = tiles_of_piece(items_p * long_p + items_o * long_o, LEAST_TILES);
+    return SharedPlan{tile_plan(halves, items_p, long_p, piece, rows, num_heads, head_dim, false),
+                      tile_plan(halves, items_o, long_o, piece, rows, num_heads, head_dim, false)};
 }
 
 // Whether prefixes are worth a part of their own, by an estimate of both ways in us from the host's bounds.
@@ -206,13 +233,13 @@ static bool prefer_shared(int num_seqs, int num_groups, int max_rows, int rows, 
     if (num_groups == 0 || max_shared == 0 || g_ranged_shared >= 0)
         return num_groups > 0 && max_shared > 0 && g_ranged_shared > 0;
     const double es = elem_bytes(dtype), G = kv_heads, n_rep = num_heads / kv_heads;
-    const double tt = rt_tokens((int)es), row = 2.0 * G * head_dim * es;  // K and V of a position
+    const double cols = rt_cols(1), tt = rt_tokens((int)es, 1), row = 2.0 * G * head_dim * es;  // K and V of a position
     const double ns = 5e-3 * (dtype == FLOUR_DTYPE_F32 ? 2.0 : 1.0) * head_dim / 128;  // a tile step
     const double own = std::max(1, max_kv - max_shared), S = num_seqs;
     const double groups = std::min(num_groups, num_seqs);
     const double seq_tiles =
-        std::min(S * ceil((double)max_rows * n_rep / RT_COLS), rows * n_rep / RT_COLS + S);
-    const double group_tiles = rows * n_rep / RT_COLS + groups;
+        std::min(S * ceil((double)max_rows * n_rep / cols), rows * n_rep / cols + S);
+    const double group_tiles = rows * n_rep / cols + groups;
     const double pieces =
         (double)rows * num_heads * (head_dim + 2) * 4.0 *
         (std::min<double>(p.prefix.max_pieces, ceil(max_shared / tt / p.prefix.piece_tiles)) +
@@ -251,23 +278,24 @@ static int ranged_call(const char* what, const RangedAttn& a, bool shared, void*
     char* ws = static_cast<char*>(workspace);
     const bool step = !a.cu && stream_takes(a), tiles = tiles_take(a);
     if (!step && !tiles) return launch_ranged_generic(a, stream);
-    RtArgs r = tile_args(a);
     if (tiles && shared) {
         const SharedPlan p = shared_plan(a.num_seqs, a.num_groups, a.max_rows, a.rows, a.num_heads,
                                          a.kv_heads, a.head_dim, a.max_kv, a.max_shared, a.dtype);
         if (prefer_shared(a.num_seqs, a.num_groups, a.max_rows, a.rows, a.num_heads, a.kv_heads,
                           a.head_dim, a.max_kv, a.max_shared, a.dtype, p)) {
+            RtArgs r = tile_args(a, p.own.halves);
             add_part(&r, RT_PREFIX, p.prefix, false, ws);
             add_part(&r, RT_OWN, p.own, false, ws + p.prefix.bytes);
-            rc = launch_tiles(r, stream);
+            rc = launch_tiles(r, p.own.halves, stream);
             return rc != FLOUR_OK ? rc : launch_ranged_merge(r, stream);
         }
     }
     if (step) return launch_stream(a, ws, stream);
     const TilePlan p = rows_plan(a.num_seqs, a.max_rows, a.rows, a.num_heads, a.kv_heads, a.head_dim,
                                  a.max_kv, a.window, a.sinks, a.dtype);
+    RtArgs r = tile_args(a, p.halves);
     add_part(&r, RT_ROWS, p, true, ws);
-    rc = launch_tiles(r, stream);
+    rc = launch_tiles(r, p.halves, stream);
     return rc != FLOUR_OK || p.max_pieces == 1 ? rc : launch_ranged_merge(r, stream);
 }
 
@@ -459,8 +487,9 @@ extern "C" int flour_hip_set_window_pairs(int mode) {
     return FLOUR_OK;
 }
 
-extern "C" int flour_hip_set_ranged(int wgs, int least, int fleast) {
-    g_ranged_wgs = wgs, g_ranged_min = least, g_ranged_fmin = fleast;
+extern "C" int flour_hip_set_tile_halves(int halves) {
+    if (halves < 0 || halves > 2) return FLOUR_ERR_INVALID_ARGUMENT;
+    g_tile_halves = halves;
     switch_set();
-    return 0;
+    return FLOUR_OK;
 }

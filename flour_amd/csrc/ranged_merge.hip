@@ -16,7 +16,7 @@ struct RmPieces {
 
 // The pieces of packed row `row`, head h in a tile launch; `shared`: the length of its group's prefix.
 __device__ __forceinline__ RmPieces tile_pieces(const RtArgs& ra, const RtPart& pt, const RangedSeq& q,
-                                                int shared, int row, int h, int head_dim, int tt) {
+                                                int shared, int row, int h, int head_dim) {
     RmPieces p{};
     RtSpan sp;
     if (pt.kind == RT_PREFIX) {
@@ -24,9 +24,9 @@ __device__ __forceinline__ RmPieces tile_pieces(const RtArgs& ra, const RtPart& 
         sp = rt_span(ra, RT_PREFIX, 0, shared, 0, 0);
     } else {
         const int col = (row - q.row0) * ra.n_rep + h % ra.n_rep;
-        sp = rt_span(ra, pt.kind, q.rows, q.kv, col / RT_COLS, shared);
+        sp = rt_span(ra, pt.kind, q.rows, q.kv, col / ra.cols, shared);
     }
-    p.n = rt_pieces(sp.tiles(tt), pt.max_pieces, pt.piece_tiles);
+    p.n = rt_pieces(sp.tiles(ra.tile), pt.max_pieces, pt.piece_tiles);
     const int64_t slot = ((int64_t)row * ra.a.num_heads + h) * pt.max_pieces;
     p.ml = pt.p_ml + 2 * slot;
     p.o = pt.p_o + slot * head_dim;
@@ -34,7 +34,7 @@ __device__ __forceinline__ RmPieces tile_pieces(const RtArgs& ra, const RtPart& 
 }
 
 template <int D>
-__global__ __launch_bounds__(64 * RM_WAVES) void ranged_merge_kernel(RtArgs ra, int tt) {
+__global__ __launch_bounds__(64 * RM_WAVES) void ranged_merge_kernel(RtArgs ra) {
     constexpr int E = D / 64;
     typedef typename std::conditional<E == 2, f32x2, float>::type RowV;
     const RangedAttn& a = ra.a;
@@ -57,8 +57,8 @@ __global__ __launch_bounds__(64 * RM_WAVES) void ranged_merge_kernel(RtArgs ra, 
     const RangedSeq q = ranged_seq(a, s);
     if (row < q.row0 || row >= q.row0 + q.rows) return;  // (rows of no sequence)
     const int shared = a.num_groups > 0 ? ranged_shared_of(a, s) : 0;
-    const RmPieces set[2] = {tile_pieces(ra, ra.part[0], q, shared, row, h, D, tt),
-                             ra.parts > 1 ? tile_pieces(ra, ra.part[1], q, shared, row, h, D, tt)
+    const RmPieces set[2] = {tile_pieces(ra, ra.part[0], q, shared, row, h, D),
+                             ra.parts > 1 ? tile_pieces(ra, ra.part[1], q, shared, row, h, D)
                                           : RmPieces{}};
     if (ra.part[0].finals && set[0].n == 1) return;
     float M = DEC_M0, L = 0.0f, O[E] = {};
@@ -108,9 +108,8 @@ __global__ __launch_bounds__(64 * RM_WAVES) void ranged_merge_kernel(RtArgs ra, 
 int launch_ranged_merge(const RtArgs& r, hipStream_t stream) {
     const int64_t items = (int64_t)r.a.rows * r.a.num_heads;
     const dim3 grid((unsigned)((items + RM_WAVES - 1) / RM_WAVES));
-    const int tt = rt_tokens(elem_bytes(r.a.dtype));
     auto kern = r.a.head_dim == 64 ? ranged_merge_kernel<64> : ranged_merge_kernel<128>;
-    kern<<<grid, dim3(64 * RM_WAVES), 0, stream>>>(r, tt);
+    kern<<<grid, dim3(64 * RM_WAVES), 0, stream>>>(r);
     return check_hip(hipGetLastError(), "attention over ranges merge launch");
 }
 

@@ -33,14 +33,19 @@ struct RtArgs {
     RangedAttn a;
     int n_rep;
     float scale_log2;
+    int cols, tile;  // columns of an item, positions of a tile (rt_cols, rt_tokens)
     int parts;
     RtPart part[2];  // the first one's workgroups come first
 };
 
-static constexpr int RT_WAVES = 4;              // waves of 32 columns each
-static constexpr int RT_COLS = 32 * RT_WAVES;   // columns of a tile: (row, query head of the kv head)
-// Cached positions of a step: 64 of a 16-bit pool, 32 of an fp32 one.
-__host__ __device__ constexpr int rt_tokens(int elem_bytes) { return elem_bytes == 4 ? 32 : 64; }
+// Four waves a workgroup, of 32 columns = (row, query head of the kv head) pairs each. halves 2: two waves
+// share 32 columns, each with every second block of 32 positions.
+static constexpr int RT_WAVES = 4;
+__host__ __device__ constexpr int rt_cols(int halves) { return 32 * RT_WAVES / halves; }
+// Cached positions of a step: 64, but 32 of fp32 pools where a wave has all of a tile.
+__host__ __device__ constexpr int rt_tokens(int elem_bytes, int halves) {
+    return elem_bytes == 4 && halves == 1 ? 32 : 64;
+}
 
 __host__ __device__ __forceinline__ int rt_pieces(int tiles, int max_pieces, int piece_tiles) {
     const int n = (tiles + piece_tiles - 1) / piece_tiles;
@@ -48,7 +53,7 @@ __host__ __device__ __forceinline__ int rt_pieces(int tiles, int max_pieces, int
 }
 
 // The positions that a column tile of a unit goes through, in runs of 16: those of [0, front), then those of
-// [from, to) from the last multiple of 16 on; a tile is RT tokens / 16 of these runs.
+// [from, to) from the last multiple of 16 on; a tile is as many of these runs as it has positions / 16.
 struct RtSpan {
     int front, from, to, front_runs, base, runs;
     __device__ __forceinline__ int tok(int run) const {
@@ -63,8 +68,8 @@ __device__ __forceinline__ RtSpan rt_span(const RtArgs& ra, int kind, int rows, 
     const int sinks = kind == RT_ROWS ? ra.a.sinks : 0;
     s.from = 0, s.to = kv;
     if (kind != RT_PREFIX) {
-        const int i0 = ctile * RT_COLS / ra.n_rep;
-        const int i1 = min(rows * ra.n_rep - 1, ctile * RT_COLS + RT_COLS - 1) / ra.n_rep;
+        const int i0 = ctile * ra.cols / ra.n_rep;
+        const int i1 = min(rows * ra.n_rep - 1, ctile * ra.cols + ra.cols - 1) / ra.n_rep;
         s.to = kv > 0 ? kv - rows + i1 + 1 : 0;
         if (kind == RT_ROWS) {
             s.from = kv > 0 ? max(0, kv - rows + i0 + 1 - ra.a.window) : 0;
@@ -85,8 +90,8 @@ __device__ __forceinline__ RtSpan rt_span(const RtArgs& ra, int kind, int rows, 
 // alone.
 int launch_ranged_merge(const RtArgs& r, hipStream_t stream);
 
-int launch_ranged_tiles_f32(const RtArgs& r, hipStream_t stream);
-int launch_ranged_tiles_bf16(const RtArgs& r, hipStream_t stream);
-int launch_ranged_tiles_f16(const RtArgs& r, hipStream_t stream);
+int launch_ranged_tiles_f32(const RtArgs& r, int halves, hipStream_t stream);
+int launch_ranged_tiles_bf16(const RtArgs& r, int halves, hipStream_t stream);
+int launch_ranged_tiles_f16(const RtArgs& r, int halves, hipStream_t stream);
 
 }  // namespace flour

@@ -35,12 +35,15 @@ __device__ __forceinline__ u32x2 lds_read_tr16(const void* p) {
 
 __device__ __forceinline__ int wave_min_i32(int x) { return -wave_max_i32(-x); }
 
-template <typename T, int D>
-__global__ __launch_bounds__(64 * RT_WAVES, 2) void ranged_tiles_kernel(RtArgs ra) {
+template <typename T, int D, int HALVES>
+__global__ __launch_bounds__(64 * RT_WAVES, (sizeof(T) * D * HALVES > 512 ? 1 : 2)) void ranged_tiles_kernel(
+    RtArgs ra) {
     constexpr bool F32 = std::is_same<T, float>::value;
     constexpr bool BF16 = std::is_same<T, bf16_t>::value;
     constexpr int ES = sizeof(T), ROW = D * ES;       // bytes of a K / V row
-    constexpr int TT = rt_tokens(ES), NB = TT / 32;   // positions of a tile, blocks of 32
+    constexpr int COLS = rt_cols(HALVES);
+    constexpr int TT = rt_tokens(ES, HALVES);         // positions of a tile
+    constexpr int NB = TT / 32 / HALVES;              // the wave's blocks of 32
     constexpr int NO = D / 32;                        // 32-dim blocks of the output
     constexpr int KP = ROW + 16;                      // LDS pitches (bytes): 16-byte reads of 16 rows,
     constexpr int VP = F32 ? ROW + 32 : (D == 128 ? 320 : 192);  // and V's, spread over the banks
@@ -79,7 +82,7 @@ __global__ __launch_bounds__(64 * RT_WAVES, 2) void ranged_tiles_kernel(RtArgs r
                     ur0 = q.row0, un = q.rows, ukv = q.kv;
                 }
             }
-            const int nt = un > 0 ? (int)(((int64_t)un * n_rep + RT_COLS - 1) / RT_COLS) : 0;
+            const int nt = un > 0 ? (int)(((int64_t)un * n_rep + COLS - 1) / COLS) : 0;
             const int incl = wave_incl_sum(nt);
             const uint64_t hit = __ballot(before + incl > want);
             if (hit) {
@@ -100,7 +103,8 @@ __global__ __launch_bounds__(64 * RT_WAVES, 2) void ranged_tiles_kernel(RtArgs r
     const int32_t* bt = a.block_tables + (int64_t)seq * a.max_blocks;
 
     // ---- the lane's column, and which positions t it sees: t < hi and (t >= lo or t < sinks)
-    const int col0 = ctile * RT_COLS + 32 * wave;
+    const int col0 = ctile * COLS + 32 * (wave / HALVES);
+    const int tok_half = 32 * NB * (wave % HALVES);  // of a tile, where the wave's positions start
     const bool live = col0 < ncols;  // (waves past the columns only stage)
     const int col = min(col0 + l32, ncols - 1);
     const bool real = col0 + l32 < ncols;
@@ -132,6 +136,12 @@ __global__ __launch_bounds__(64 * RT_WAVES, 2) void ranged_tiles_kernel(RtArgs r
     }
     const RtSpan sp = rt_span(ra, pt.kind, rows, kv, ctile, own);
     const int front = sp.front, from = sp.from, to = sp.to, all_tiles = sp.tiles(TT);
+    // Tiles from `plain` on hold consecutive positions, tok_off + TT t .. ; those before hold sinks.
+    const int plain = (sp.front_runs + TT / 16 - 1) / (TT / 16), tok_off = sp.base - 16 * sp.front_runs;
+    auto tile_tok = [&](int t) -> int { return t >= plain ? tok_off + TT * t : sp.tok(t * (TT / 16)); };
+    auto tile_end = [&](int t) -> int {
+        return t >= plain ? tok_off + TT * t + TT : sp.tok(t * (TT / 16) + TT / 16 - 1) + 16;
+    };
 
     // ---- this workgroup's piece of the tiles
     const int pieces = rt_pieces(all_tiles, pt.max_pieces, pt.piece_tiles);
@@ -176,11 +186,13 @@ __global__ __launch_bounds__(64 * RT_WAVES, 2) void ranged_tiles_kernel(RtArgs r
     };
     // positions of a loaded tile that no column sees: no bits of theirs
     auto cut_tile = [&](int t) __attribute__((always_inline)) {
-        if (sp.tok(t * UPT) >= from && sp.tok(t * UPT + UPT - 1) + 16 <= to) return;
+        if (tile_tok(t) >= from && tile_end(t) <= to) return;
 #pragma unroll
         for (int k = 0; k < NP; k++) {
             const int tok = sp.tok(t * UPT + (k * RPP + w_row) / 16) + ((k * RPP + s_row) & 15);
-            if (!(tok < to && (tok >= from || tok < front))) vreg[k] = u32x4{0, 0, 0, 0};
+            const bool keep = (tok < to) & ((tok >= from) | (tok < front));
+#pragma unroll
+            for (int e = 0; e < 4; e++) vreg[k][e] = keep ? vreg[k][e] : 0;
         }
     };
     auto stage_rows = [&](auto exact, int k, int buf) __attribute__((always_inline)) {
@@ -212,7 +224,7 @@ __global__ __launch_bounds__(64 * RT_WAVES, 2) void ranged_tiles_kernel(RtArgs r
     // Tile t, and meanwhile the next one's rows from registers to the other buffer, which frees the registers
     // for request().
     auto compute = [&](auto exact, int t, int buf, auto request) __attribute__((always_inline)) {
-        const int tok0 = sp.tok(t * UPT), tok_end = sp.tok(t * UPT + UPT - 1) + 16;
+        const int tok0 = tile_tok(t), tok_end = tile_end(t);
         if (!live || tok0 >= max_hi || (tok_end <= min_lo && tok0 >= sinks)) {
 #pragma unroll
             for (int k = 0; k < NP; k++) stage_rows(exact, k, buf ^ 1);
@@ -224,7 +236,7 @@ __global__ __launch_bounds__(64 * RT_WAVES, 2) void ranged_tiles_kernel(RtArgs r
         for (int b = 0; b < NB; b++)
 #pragma unroll
             for (int e = 0; e < 16; e++) s[b][e] = 0.0f;
-        const unsigned char* kr = &k_lds[buf][l32 * KP];
+        const unsigned char* kr = &k_lds[buf][(tok_half + l32) * KP];
         if constexpr (F32) {
 #pragma unroll
             for (int k = 0; k < NP; k++) stage_rows(exact, k, buf ^ 1);
@@ -240,8 +252,8 @@ __global__ __launch_bounds__(64 * RT_WAVES, 2) void ranged_tiles_kernel(RtArgs r
             }
             s[0] += s1;
         } else {
-            // K fragments three steps ahead (left alone, the reads come right before their products)
-            constexpr int AHEAD = 3;
+            // K fragments two steps ahead (left alone, the reads come right before their products)
+            constexpr int AHEAD = 2;
             u32x4 kf[AHEAD][NB];
             auto read_k = [&](int kk) __attribute__((always_inline)) {
 #pragma unroll
@@ -266,13 +278,26 @@ __global__ __launch_bounds__(64 * RT_WAVES, 2) void ranged_tiles_kernel(RtArgs r
         }
         request();  // the tile after the next one
         const bool full = tok_end <= min_hi && (tok0 >= max_lo || tok_end <= sinks);
-        if (!full) {
+        // (positions of a register are known up to where the tile and the lane's half start)
+        if (!full && t >= plain) {
+            const int at = tok0 + tok_half + 4 * half, r_hi = hi - at, r_lo = lo - at, r_sinks = sinks - at;
 #pragma unroll
             for (int b = 0; b < NB; b++)
 #pragma unroll
                 for (int e = 0; e < 16; e++) {
-                    const int tok = sp.tok(t * UPT + 2 * b + (e >> 3)) + 8 * ((e >> 2) & 1) + 4 * half + (e & 3);
-                    if (!(tok < hi && (tok >= lo || tok < sinks))) s[b][e] = -INFINITY;
+                    const int x = 32 * b + 8 * (e >> 2) + (e & 3);
+                    const bool sees = (x < r_hi) & ((x >= r_lo) | (x < r_sinks));
+                    s[b][e] = sees ? s[b][e] : -INFINITY;
+                }
+        } else if (!full) {
+#pragma unroll
+            for (int b = 0; b < NB; b++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) {
+                    const int tok = sp.tok(t * UPT + tok_half / 16 + 2 * b + (e >> 3)) + 8 * ((e >> 2) & 1) +
+                                    4 * half + (e & 3);
+                    const bool sees = (tok < hi) & ((tok >= lo) | (tok < sinks));
+                    s[b][e] = sees ? s[b][e] : -INFINITY;
                 }
         }
         float top = s[0][0];
@@ -308,7 +333,8 @@ __global__ __launch_bounds__(64 * RT_WAVES, 2) void ranged_tiles_kernel(RtArgs r
                 for (int e = 0; e < 16; e++)
                     z = __builtin_amdgcn_mfma_f32_32x32x2f32(
                         *reinterpret_cast<const float*>(
-                            &v_lds[buf][(8 * (e >> 2) + 4 * half + (e & 3)) * VP + 4 * (32 * o + l32)]),
+                            &v_lds[buf][(tok_half + 8 * (e >> 2) + 4 * half + (e & 3)) * VP +
+                                        4 * (32 * o + l32)]),
                         p[e], z, 0, 0, 0);
                 acc[o] += z;
             }
@@ -317,7 +343,7 @@ __global__ __launch_bounds__(64 * RT_WAVES, 2) void ranged_tiles_kernel(RtArgs r
             constexpr bool SPLIT = BF16 && decltype(exact)::value;
             // V^T: 16 lanes read rows 4 half .. + 3 of 16 dims, and the rows 8 behind; fragment n is of
             // positions 16 (n / NO) .. + 15 and dims 32 (n % NO) .. + 31
-            const unsigned char* vr = &v_lds[buf][(4 * half + ((lane >> 2) & 3)) * VP +
+            const unsigned char* vr = &v_lds[buf][(tok_half + 4 * half + ((lane >> 2) & 3)) * VP +
                                                   32 * ((lane >> 4) & 1) + 8 * (lane & 3)];
             constexpr int NF = 2 * NB * NO, AHEAD = 4;
             u32x4 vf[AHEAD];
@@ -388,7 +414,37 @@ __global__ __launch_bounds__(64 * RT_WAVES, 2) void ranged_tiles_kernel(RtArgs r
             __syncthreads();
         }
         l = sum_across_halves(l);
+        if constexpr (HALVES == 2) {  // the second wave's state to the first, through LDS
+            float* const st = reinterpret_cast<float*>(&v_lds[0][0]) + (wave / 2) * (64 * (16 * NO + 2));
+            if (wave & 1) {
+#pragma unroll
+                for (int o = 0; o < NO; o++)
+#pragma unroll
+                    for (int e = 0; e < 16; e += 4)
+                        *reinterpret_cast<f32x4*>(st + (4 * o + e / 4) * 256 + 4 * lane) =
+                            f32x4{acc[o][e], acc[o][e + 1], acc[o][e + 2], acc[o][e + 3]};
+                st[16 * NO * 64 + lane] = m;
+                st[16 * NO * 64 + 64 + lane] = l;
+            }
+            __syncthreads();
+            if (!(wave & 1)) {
+                const float m1 = st[16 * NO * 64 + lane], l1 = st[16 * NO * 64 + 64 + lane];
+                const float mn = fmaxf(m, m1), w0 = fast_exp2(m - mn), w1 = fast_exp2(m1 - mn);
+                l = l * w0 + l1 * w1;
+                m = mn;
+#pragma unroll
+                for (int o = 0; o < NO; o++)
+#pragma unroll
+                    for (int e = 0; e < 16; e += 4) {
+                        const f32x4 y = *reinterpret_cast<const f32x4*>(st + (4 * o + e / 4) * 256 + 4 * lane);
+#pragma unroll
+                        for (int x = 0; x < 4; x++) acc[o][e + x] = acc[o][e + x] * w0 + y[x] * w1;
+                    }
+            }
+            __syncthreads();  // (another pass stages there)
+        }
     };
+    const bool owner = HALVES == 1 || !(wave & 1);  // of its columns' states
     using yes = std::integral_constant<bool, true>;
     using no = std::integral_constant<bool, false>;
     pass(no{});
@@ -410,7 +466,7 @@ __global__ __launch_bounds__(64 * RT_WAVES, 2) void ranged_tiles_kernel(RtArgs r
             for (int e = 0; e < 16; e++) sq = fmaf(acc[o][e], acc[o][e], sq);
         sq = sum_across_halves(sq);
         const float least = 2.0f / (32768.0f * 1024.0f * 5e-4f * 2.0f);  // 2^-25 / 5e-4
-        const bool again = live && real && l != 0.0f && !(sq >= D * least * least * l * l && finite());
+        const bool again = live && owner && real && l != 0.0f && !(sq >= D * least * least * l * l && finite());
         if (__syncthreads_or(again)) pass(yes{});
     }
 
@@ -418,8 +474,8 @@ __global__ __launch_bounds__(64 * RT_WAVES, 2) void ranged_tiles_kernel(RtArgs r
     const bool final_out = pt.finals && pieces == 1;
     const int64_t slot = ((int64_t)row * a.num_heads + head) * pt.max_pieces + piece;
     const int64_t out_at = (int64_t)row * a.o_st + (int64_t)head * a.o_sh;
-    const bool bad = live && real && !finite();
-    if (live && real && !bad) {
+    const bool bad = live && owner && real && !finite();
+    if (live && owner && real && !bad) {
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
         for (int o = 0; o < NO; o++)
@@ -502,8 +558,10 @@ __global__ __launch_bounds__(64 * RT_WAVES, 2) void ranged_tiles_kernel(RtArgs r
 }
 
 template <typename T>
-static int launch_ranged_tiles(const RtArgs& r, hipStream_t stream) {
-    auto kern = r.a.head_dim == 64 ? ranged_tiles_kernel<T, 64> : ranged_tiles_kernel<T, 128>;
+static int launch_ranged_tiles(const RtArgs& r, int halves, hipStream_t stream) {
+    auto kern = r.a.head_dim == 64
+                    ? (halves == 2 ? ranged_tiles_kernel<T, 64, 2> : ranged_tiles_kernel<T, 64, 1>)
+                    : (halves == 2 ? ranged_tiles_kernel<T, 128, 2> : ranged_tiles_kernel<T, 128, 1>);
     int64_t grid = 0;
     for (int i = 0; i < r.parts; i++) grid += (int64_t)r.part[i].items * r.part[i].max_pieces;
     kern<<<dim3((unsigned)grid), dim3(64 * RT_WAVES), 0, stream>>>(r);

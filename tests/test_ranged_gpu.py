@@ -20,6 +20,20 @@ def prefixes_on_their_own():
     _lib.lib().flour_hip_set_shared_prefix(-1)
 
 
+@pytest.fixture
+def both_halves():
+    """A function that runs another with a wave's columns its own and shared with a second one."""
+    lib = _lib.lib()
+
+    def each(f):
+        for halves in (1, 2):
+            assert lib.flour_hip_set_tile_halves(halves) == 0
+            f()
+
+    yield each
+    lib.flour_hip_set_tile_halves(0)
+
+
 DT = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
 # What a weight is rounded to on the way into a product: two bf16 or f16 parts in decode steps of up to 16
 # query heads a kv head (half a step of 8 bits, twice: 2^-8 of 2^-8), one f16 number elsewhere (half a step,
@@ -127,21 +141,25 @@ def test_decode_window_batches(dt, n):
 @pytest.mark.parametrize("dt", DT)
 @pytest.mark.parametrize("heads", HEADS + [(40, 2, 128), (6, 3, 96), (2, 1, 40)], ids=str)
 @pytest.mark.parametrize("window,sinks", [(1, 0), (1, 2), (17, 5), (64, 0), (200, 70)])
-def test_prefill_window(dt, heads, window, sinks):
+def test_prefill_window(dt, heads, window, sinks, both_halves):
     rows = [1, 0, 33, 128, 5, 200, 2, 64]
     kv = [1, 9, 33, 300, 4, 200, 900, 65]  # (the fifth has fewer positions than rows: zeros)
     b = R.batch(DT[dt], *heads, 16, rows, kv, seed=window)
     scale = heads[2] ** -0.5
-    got = run(b, scale, window, sinks)
-    check(got, b, scale, TILE_EPS[dt], window, sinks)
-    assert not bool(got[b.cu[4]:b.cu[5]].any())
+
+    def one():
+        got = run(b, scale, window, sinks)
+        check(got, b, scale, TILE_EPS[dt], window, sinks)
+        assert not bool(got[b.cu[4]:b.cu[5]].any())
+
+    both_halves(one)
 
 
 @pytest.mark.parametrize("bs", [1, 7, 8, 32, 48, 80])
 @pytest.mark.parametrize("dt", DT)
-def test_prefill_window_other_pages(dt, bs):
+def test_prefill_window_other_pages(dt, bs, both_halves):
     b = R.batch(DT[dt], 8, 2, 64, bs, [150, 20, 1], [150, 400, 111], seed=bs)
-    check(run(b, 0.125, 60, 5), b, 0.125, TILE_EPS[dt], 60, 5)
+    both_halves(lambda: check(run(b, 0.125, 60, 5), b, 0.125, TILE_EPS[dt], 60, 5))
 
 
 @pytest.mark.parametrize("dt,odt", [("bf16", "f32"), ("f16", "bf16"), ("f32", "f16")])
@@ -169,23 +187,23 @@ GROUPS = [([0, 5], [160]), ([0, 2, 5], [32, 400]), ([1, 3, 3, 4], [100, 7, 0]), 
 @pytest.mark.parametrize("dt", DT)
 @pytest.mark.parametrize("heads", HEADS + [(40, 2, 128), (6, 3, 96), (2, 1, 40)], ids=str)
 @pytest.mark.parametrize("starts,shared", GROUPS, ids=str)
-def test_decode_shared(dt, heads, starts, shared):
+def test_decode_shared(dt, heads, starts, shared, both_halves):
     # (sequences longer and shorter than their prefixes, one of no position)
     kv = [450, 33, 0, 161, 1200]
     b = R.batch(DT[dt], *heads, 16, [1] * 5, kv, seed=len(starts), starts=starts, shared=shared)
     scale = heads[2] ** -0.5
-    check_shared(b, scale, TILE_EPS[dt], decode=True)
+    both_halves(lambda: check_shared(b, scale, TILE_EPS[dt], decode=True))
 
 
 @pytest.mark.parametrize("dt", DT)
 @pytest.mark.parametrize("heads", HEADS + [(40, 2, 128), (6, 3, 96), (2, 1, 40)], ids=str)
 @pytest.mark.parametrize("starts,shared", GROUPS, ids=str)
 @pytest.mark.parametrize("rows", [[3, 8, 0, 5, 1], [150, 30, 9, 64, 200]], ids=["few", "many"])
-def test_prefill_shared(dt, heads, starts, shared, rows):
+def test_prefill_shared(dt, heads, starts, shared, rows, both_halves):
     kv = [450, 33, 5, 161, 1200]
     b = R.batch(DT[dt], *heads, 16, rows, kv, seed=len(starts), starts=starts, shared=shared)
     scale = heads[2] ** -0.5
-    check_shared(b, scale, TILE_EPS[dt])
+    both_halves(lambda: check_shared(b, scale, TILE_EPS[dt]))
 
 
 @pytest.mark.parametrize("bs", [1, 7, 32, 48])
@@ -249,7 +267,7 @@ def test_what_no_row_sees_does_not_matter(dt, heads, value):
 @pytest.mark.parametrize("dt", DT)
 @pytest.mark.parametrize("heads", [(14, 2, 64), (32, 8, 128), (6, 3, 96)], ids=str)
 @pytest.mark.parametrize("where", ["k", "v"])
-def test_a_bad_row_spoils_those_who_see_it(dt, heads, value, where):
+def test_a_bad_row_spoils_those_who_see_it(dt, heads, value, where, both_halves):
     """Rows beside it in a tile, which do not see it, keep their numbers."""
     scale = heads[2] ** -0.5
     b = R.batch(DT[dt], *heads, 16, [200, 30], [260, 400], seed=4)
@@ -260,13 +278,13 @@ def test_a_bad_row_spoils_those_who_see_it(dt, heads, value, where):
         b.q[:, :, 0] = b.q[:, :, 0].abs() + 1
         b.q[:, :, 1:] = 0
     want, mag, top, seen = R.expected(b, scale, 40, 3)
-    got = run(b, scale, 40, 3)
     if where == "k":
         top = torch.nan_to_num(top, nan=0.0, posinf=0.0)
         rows = torch.isfinite(want).all(2).all(1)
         top[rows] = R.expected(_finite(b), scale, 40, 3)[2][rows]
-    R.close(got, want, torch.nan_to_num(
-        R.bound(mag, top, seen, heads[2], TILE_EPS[dt], 8.0), nan=0.0, posinf=0.0, neginf=0.0))
+    err = torch.nan_to_num(R.bound(mag, top, seen, heads[2], TILE_EPS[dt], 8.0), nan=0.0, posinf=0.0,
+                           neginf=0.0)
+    both_halves(lambda: R.close(run(b, scale, 40, 3), want, err))
 
 
 def _finite(b):
@@ -290,18 +308,17 @@ def test_scores_of_minus_infinity_weigh_nothing(dt):
 
 @pytest.mark.parametrize("size", [2.0 ** -20, 2.0 ** -40, 0.0, 2.0 ** 17, 2.0 ** 100])
 @pytest.mark.parametrize("heads", [(14, 2, 64), (8, 2, 128)], ids=str)
-def test_bf16_values_of_any_size(size, heads):
+def test_bf16_values_of_any_size(size, heads, both_halves):
     """Values beyond f16's numbers, above and below."""
     scale = heads[2] ** -0.5
     b = R.batch(torch.bfloat16, *heads, 16, [150, 3], [200, 300], seed=6, v_scale=size, starts=[0, 2],
                 shared=[50])
     for kw in (dict(window=64, sinks=2), {}):
         want, mag, top, seen = R.expected(b, scale, kw.get("window", R.EVERY), kw.get("sinks", 0))
-        got = run(b, scale, out_dtype=torch.float32, **kw)
         err = R.bound(mag, top, seen, heads[2], 2.0 ** -11, 4.5 * size)
         # values below f16's numbers: off by what is small beside the block's root mean square
         err = err - 2.0 ** -25 + min(2.0 ** -25, 5e-4 * 4.5 * size)
-        R.close(got, want, err)
+        both_halves(lambda: R.close(run(b, scale, out_dtype=torch.float32, **kw), want, err))
 
 
 # ------------------------------------------------------------------ layouts, tables, streams, graphs
