@@ -38,6 +38,19 @@ __device__ __forceinline__ RangedSeq ranged_seq(const RangedAttn& a, int s) {
     return RangedSeq{r0, max(n, 0), kv >= n && kv > 0 ? kv : 0};
 }
 
+// The sequence of packed row `row`: the last one that starts at or before it.
+__device__ __forceinline__ int ranged_seq_of(const RangedAttn& a, int row) {
+    int lo = 0, hi = a.num_seqs;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (a.cu[mid] <= row)
+            lo = mid;
+        else
+            hi = mid;
+    }
+    return lo;
+}
+
 // The group of sequence s (-1: none): the last one that starts at or before it, if it has not ended.
 __device__ __forceinline__ int ranged_group(const int32_t* starts, int num_groups, int s) {
     if (num_groups == 0 || starts[0] > s) return -1;

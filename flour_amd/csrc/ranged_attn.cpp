@@ -119,8 +119,8 @@ struct TilePlan {
 static int g_tile_halves = 0;
 // Three workgroups for two CUs are aimed at: 2 / 3 / 4 for two in us: 64 sequences of one prefix 8,192 + up to
 // 512 57.0 / 44.6 / 48.9, drafted rows 55.6 / 50.3 / 55.6, fp32 28.7 / 23.3 / 23.1. Pieces have four tiles at
-// least, twelve where a launch could do without any (which saves the merge).
-static constexpr int WGS_OF_TWO_CUS = 3, LEAST_TILES = 4, LEAST_TILES_FINAL = 12;
+// least, eight where a launch could do without any (which saves the merge).
+static constexpr int WGS_OF_TWO_CUS = 3, LEAST_TILES = 4, LEAST_TILES_FINAL = 8;
 // Units of up to unit_rows rows (rows in all), an item for each of their column tiles and kv heads.
 static int64_t tile_items(int64_t units, int64_t unit_rows, int64_t rows, int64_t n_rep, int64_t kv_heads,
                           int64_t cols) {
@@ -177,20 +177,33 @@ static TilePlan rows_plan(int num_seqs, int max_rows, int rows, int num_heads, i
                           int max_kv, int window, int sinks, int dtype) {
     const int64_t n_rep = num_heads / kv_heads;
     // Two waves for 32 columns while that leaves the chip unfilled: half the time of an item, 1.3 times that of
-    // all. Waves of 64 positions / half of them in us: 16 bits, 32 / 8 heads of 128, window 512, 80 items (of
-    // 128 columns) 24.9 / 20.5, 256 27.5 / 27.5, 416 35.2 / 44.7; 8 / 8 of 64, 256 22.6 / 20.6, 384 32.2 / 26.6;
-    // 14 / 2, 660 41.3 / 39.1; fp32, 8 / 8 of 64, 128 52.6 / 39.2, 384 107.8 / 109.5; 32 / 8 of 128, 80 79.9 /
-    // 59.0, 256 124 / 116 (window 128: 48.9 / 54.3), 416 162 / 188.
-    const int64_t few = dtype == FLOUR_DTYPE_F32 ? (head_dim == 64 ? 384 : 128) : (head_dim == 64 ? 640 : 256);
-    int halves = tile_items(num_seqs, max_rows, rows, n_rep, kv_heads, rt_cols(1)) <= few ? 2 : 1;
-    if (g_tile_halves > 0) halves = g_tile_halves;
-    const int cols = rt_cols(halves);
-    const int64_t tt = rt_tokens(elem_bytes(dtype), halves);
-    const int64_t items = tile_items(num_seqs, max_rows, rows, n_rep, kv_heads, cols);
-    const int64_t span = (int64_t)window + sinks + cols / n_rep + 2;
-    const int64_t longest = std::min<int64_t>(max_kv, span) / tt + 2;  // (ends that are not whole tiles)
-    return tile_plan(halves, items, longest, tiles_of_piece(items * longest, LEAST_TILES_FINAL), rows, num_heads, head_dim,
-                     true);
+    // all. Waves of 64 positions / half of them in us, by items (of 128 columns): bf16, 8 / 8 heads of 64,
+    // window 512, 64 items 22.7 / 17.3, 384 30.0 / 25.1; 14 / 2, 352 22.9 / 21.3, 660 29.9 / 38.4; 32 / 8 of 128,
+    // 80 23.5 / 21.2, 256 26.1 / 26.7; fp32, 8 / 8 of 64, 64 64.0 / 37.3, 384 107.2 / 108.0; 32 / 8 of 128,
+    // 80 94.4 / 58.8, 224 86.1 / 91.6.
+    const int64_t few = dtype == FLOUR_DTYPE_F32 ? (head_dim == 64 ? 384 : 128) : (head_dim == 64 ? 384 : 256);
+    const int64_t cus = device_cus();
+    int halves = 1;
+    int64_t items = 0, longest = 0, piece = 0;
+    // An item of many tiles is cut along the keys while the items leave CUs idle. Whole / cut in us, by items and
+    // their tiles: 8 / 8 heads of 64 in bf16, 16 items of 10 tiles 11.4 / 18.4, of 34 23.0 / 15.8; 28 / 4 of
+    // 128, 136 of 34 36.7 / 36.4, 220 of 34 59.6 / 67.4, of 130 133.9 / 120.1; 14 / 2 of 64, 352 of 130
+    // 113.6 / 140.9; fp32, 32 / 8 of 128, 224 of 66 206 / 193.
+    auto cut = [&](int h) {
+        halves = h;
+        const int cols = rt_cols(h);
+        const int64_t tt = rt_tokens(elem_bytes(dtype), h);
+        items = tile_items(num_seqs, max_rows, rows, n_rep, kv_heads, cols);
+        const int64_t span = (int64_t)window + sinks + cols / n_rep + 2;
+        longest = std::min<int64_t>(max_kv, span) / tt + 2;  // (ends that are not whole tiles)
+        const bool idle = longest >= 64 ? items <= cus : longest >= 24 && 2 * items <= cus;
+        piece = idle ? tiles_of_piece(items * longest, LEAST_TILES_FINAL) : longest;
+    };
+    cut(1);
+    // (whole columns where the cut fills the chip: fp32, 32 / 8 of 128, 80 items of 258 tiles 258 / 277)
+    const bool filled = longest >= 64 && 8 * items >= cus && 2 * items <= cus;
+    if (g_tile_halves > 0 ? g_tile_halves == 2 : items <= few && !filled) cut(2);
+    return tile_plan(halves, items, longest, piece, rows, num_heads, head_dim, true);
 }
 
 // Prefixes as a part of their own: 1 always, 0 never, -1 by prefer_shared (a test switch).
@@ -203,12 +216,16 @@ struct SharedPlan {
 static SharedPlan shared_plan(int num_seqs, int num_groups, int max_rows, int rows, int num_heads,
                               int kv_heads, int head_dim, int max_kv, int max_shared, int dtype) {
     const int64_t n_rep = num_heads / kv_heads;
-    // Two waves for 32 columns, unless large groups make the prefixes' products the most of the work. Waves of
-    // 64 positions / half of them in us, 32 / 8 heads of 128 in bf16: 64 sequences of one prefix 4,096 + 256
-    // 41.2 / 36.1, 1,024 + 1,024 84 / 72, 16,384 + 128 55.5 / 61.0; of eight 4,096 + 256 59.7 / 51.1; 64 / 8
-    // heads, one prefix and six rows each 115.6 / 132.0.
+    // Two waves for 32 columns, except at head_dim 128 in 16 bits, which they keep from two workgroups a CU, and
+    // where large groups make the prefixes' products the most of the work. Waves of 64 positions / half of them
+    // in us, 64 sequences: bf16, 32 / 8 heads of 128, one prefix 16,384 + 128 60.3 / 67.4, of eight 4,096 + 256
+    // 59.5 / 67.7; of 64, 1,024 + 1,024 35.8 / 33.2; fp32, 8 / 8 of 64, 4,096 + 256 64.4 / 47.5; 64 / 8 of
+    // 128, 16,384 418 / 499.
     const int64_t tiles_p = tile_items(num_groups, rows, rows, n_rep, kv_heads, rt_cols(1)) * (max_shared / 64);
-    int halves = rows * n_rep >= (int64_t)192 * num_groups && tiles_p >= 3000 ? 1 : 2;
+    int halves = (dtype != FLOUR_DTYPE_F32 && head_dim == 128) ||
+                         (rows * n_rep >= (int64_t)192 * num_groups && tiles_p >= 3000)
+                     ? 1
+                     : 2;
     if (g_tile_halves > 0) halves = g_tile_halves;
     const int cols = rt_cols(halves);
     const int64_t tt = rt_tokens(elem_bytes(dtype), halves);

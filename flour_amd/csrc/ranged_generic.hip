@@ -37,18 +37,7 @@ __global__ __launch_bounds__(RG_THREADS) void ranged_generic_kernel(RangedAttn a
     __shared__ float red[RG_THREADS / 64];
     const int r = blockIdx.x, h = blockIdx.y, tid = threadIdx.x;
     const int head_dim = a.head_dim, block_size = a.block_size;
-    int s = r;
-    if (a.cu) {
-        int lo = 0, hi = a.num_seqs;
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            if (a.cu[mid] <= r)
-                lo = mid;
-            else
-                hi = mid;
-        }
-        s = lo;
-    }
+    const int s = a.cu ? ranged_seq_of(a, r) : r;
     const RangedSeq sq = ranged_seq(a, s);
     const int i = r - sq.row0;
     if (i < 0 || i >= sq.rows) return;  // (rows of no sequence)

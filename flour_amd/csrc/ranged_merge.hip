@@ -42,18 +42,7 @@ __global__ __launch_bounds__(64 * RM_WAVES) void ranged_merge_kernel(RtArgs ra) 
     const int64_t item = (int64_t)blockIdx.x * RM_WAVES + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     if (item >= (int64_t)a.rows * a.num_heads) return;
     const int row = (int)(item / a.num_heads), h = (int)(item - (int64_t)row * a.num_heads);
-    int s = row;
-    if (a.cu) {
-        int x = 0, y = a.num_seqs;
-        while (y - x > 1) {
-            const int mid = (x + y) >> 1;
-            if (a.cu[mid] <= row)
-                x = mid;
-            else
-                y = mid;
-        }
-        s = x;
-    }
+    const int s = a.cu ? ranged_seq_of(a, row) : row;
     const RangedSeq q = ranged_seq(a, s);
     if (row < q.row0 || row >= q.row0 + q.rows) return;  // (rows of no sequence)
     const int shared = a.num_groups > 0 ? ranged_shared_of(a, s) : 0;

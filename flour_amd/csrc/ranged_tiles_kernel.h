@@ -4,8 +4,10 @@
 // any group size fills the tiles and a wave's 32 columns span few rows: the band of positions that
 // they see is narrow, and tiles outside of it are skipped wave by wave. Four waves, a column a lane
 // pair (l, l + 32); the item's positions come through LDS in tiles, double-buffered, loaded one tile ahead.
-// Two workgroups a CU, whose waves are in different phases: the matrix cores of one run beside the
-// softmax of the other.
+// Two workgroups a CU (three of 16-bit pools at head_dim 64), whose waves are in different phases: the matrix
+// cores of one run beside the softmax of the other. One wave a SIMD with twice the columns, its products
+// and vector work interleaved by hand, took 1.6 times as long at head_dim 64 and did not fit the
+// registers at 128.
 //
 //  * S^T = K Q^T on v_mfma_f32_32x32x16: K rows from LDS (A), Q^T in registers (B). A lane holds its
 //    column's scores at positions 8 (e / 4) + 4 (l / 32) + e % 4 of 32.
@@ -36,7 +38,7 @@ __device__ __forceinline__ u32x2 lds_read_tr16(const void* p) {
 __device__ __forceinline__ int wave_min_i32(int x) { return -wave_max_i32(-x); }
 
 template <typename T, int D, int HALVES>
-__global__ __launch_bounds__(64 * RT_WAVES, (sizeof(T) * D * HALVES > 512 ? 1 : 2)) void ranged_tiles_kernel(
+__global__ __launch_bounds__(64 * RT_WAVES, rt_workgroups(sizeof(T), D, HALVES)) void ranged_tiles_kernel(
     RtArgs ra) {
     constexpr bool F32 = std::is_same<T, float>::value;
     constexpr bool BF16 = std::is_same<T, bf16_t>::value;
@@ -113,19 +115,7 @@ __global__ __launch_bounds__(64 * RT_WAVES, (sizeof(T) * D * HALVES > 512 ? 1 : 
     const int sinks = pt.kind == RT_ROWS ? a.sinks : 0;
     int hi, lo = 0, own = 0;
     if (pt.kind == RT_PREFIX) {
-        int s = row;
-        if (a.cu) {
-            int x = 0, y = a.num_seqs;
-            while (y - x > 1) {
-                const int mid = (x + y) >> 1;
-                if (a.cu[mid] <= row)
-                    x = mid;
-                else
-                    y = mid;
-            }
-            s = x;
-        }
-        const RangedSeq q = ranged_seq(a, s);
+        const RangedSeq q = ranged_seq(a, a.cu ? ranged_seq_of(a, row) : row);
         hi = q.kv > 0 ? min(kv, q.kv - q.rows + (row - q.row0) + 1) : 0;
     } else {
         hi = kv > 0 ? kv - rows + row_i + 1 : 0;
