@@ -28,14 +28,18 @@ struct RangedAttn {
     int num_groups, max_shared;
 };
 
+// Where the rows of sequence s start (those of num_seqs: where they end). Whatever cu holds, rows are the call's.
+__device__ __forceinline__ int ranged_row(const RangedAttn& a, int s) {
+    return a.cu ? max(0, min(a.cu[s], a.rows)) : s;
+}
 // Rows of sequence s, its kv length (0 where its rows see nothing).
 struct RangedSeq {
     int row0, rows, kv;
 };
 __device__ __forceinline__ RangedSeq ranged_seq(const RangedAttn& a, int s) {
-    const int r0 = a.cu ? a.cu[s] : s, n = a.cu ? a.cu[s + 1] - r0 : 1;
+    const int r0 = ranged_row(a, s), n = max(0, ranged_row(a, s + 1) - r0);
     const int kv = min(a.kv_lens[s], a.max_kv);
-    return RangedSeq{r0, max(n, 0), kv >= n && kv > 0 ? kv : 0};
+    return RangedSeq{r0, n, kv >= n && kv > 0 ? kv : 0};
 }
 
 // The sequence of packed row `row`: the last one that starts at or before it.

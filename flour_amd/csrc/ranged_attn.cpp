@@ -124,7 +124,7 @@ static constexpr int WGS_OF_TWO_CUS = 3, LEAST_TILES = 4, LEAST_TILES_FINAL = 8;
 // Units of up to unit_rows rows (rows in all), an item for each of their column tiles and kv heads.
 static int64_t tile_items(int64_t units, int64_t unit_rows, int64_t rows, int64_t n_rep, int64_t kv_heads,
                           int64_t cols) {
-    unit_rows = std::min(unit_rows, rows);
+    unit_rows = std::min(unit_rows, rows), units = std::min(units, rows);  // (of those that have rows)
     const int64_t tiles =
         std::min(rows * n_rep / cols + units, units * ((unit_rows * n_rep + cols - 1) / cols));
     return std::max<int64_t>(1, tiles * kv_heads);
@@ -252,7 +252,7 @@ static bool prefer_shared(int num_seqs, int num_groups, int max_rows, int rows, 
     const double es = elem_bytes(dtype), G = kv_heads, n_rep = num_heads / kv_heads;
     const double cols = rt_cols(1), tt = rt_tokens((int)es, 1), row = 2.0 * G * head_dim * es;  // K and V of a position
     const double ns = 5e-3 * (dtype == FLOUR_DTYPE_F32 ? 2.0 : 1.0) * head_dim / 128;  // a tile step
-    const double own = std::max(1, max_kv - max_shared), S = num_seqs;
+    const double own = std::max(1, max_kv - max_shared), S = std::min(num_seqs, rows);
     const double groups = std::min(num_groups, num_seqs);
     const double seq_tiles =
         std::min(S * ceil((double)max_rows * n_rep / cols), rows * n_rep / cols + S);

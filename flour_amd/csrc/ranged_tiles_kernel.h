@@ -77,8 +77,8 @@ __global__ __launch_bounds__(64 * RT_WAVES, rt_workgroups(sizeof(T), D, HALVES))
                     const int s0 = max(0, min(a.group_starts[u], a.num_seqs));
                     const int s1 = max(s0, min(a.group_starts[u + 1], a.num_seqs));
                     ukv = max(0, min(a.shared_lens[u], a.max_shared));
-                    ur0 = a.cu ? a.cu[s0] : s0;
-                    un = ukv > 0 ? (a.cu ? a.cu[s1] : s1) - ur0 : 0;
+                    ur0 = ranged_row(a, s0);
+                    un = ukv > 0 ? ranged_row(a, s1) - ur0 : 0;
                 } else {
                     const RangedSeq q = ranged_seq(a, u);
                     ur0 = q.row0, un = q.rows, ukv = q.kv;
@@ -188,6 +188,8 @@ __global__ __launch_bounds__(64 * RT_WAVES, rt_workgroups(sizeof(T), D, HALVES))
     auto stage_rows = [&](auto exact, int k, int buf) __attribute__((always_inline)) {
         const int r = k * RPP + s_row;
         *reinterpret_cast<u32x4*>(&k_lds[buf][r * KP + s_col]) = kreg[k];
+        // (or the conversion moves up to the branch that compute() begins with, and with it the wait for the rows)
+        if constexpr (!F32) asm volatile("" : "+v"(vreg[k]));
         u32x4 v = vreg[k];
         if constexpr (BF16 && !decltype(exact)::value)
 #pragma unroll
@@ -290,6 +292,9 @@ __global__ __launch_bounds__(64 * RT_WAVES, rt_workgroups(sizeof(T), D, HALVES))
                     s[b][e] = sees ? s[b][e] : -INFINITY;
                 }
         }
+        // (one register for a score whether the masks above ran or not, or every tile copies them)
+#pragma unroll
+        for (int b = 0; b < NB; b++) asm volatile("" : "+v"(s[b]));
         float top = s[0][0];
 #pragma unroll
         for (int b = 0; b < NB; b++)

@@ -379,6 +379,22 @@ def test_rows_behind_the_last_sequence_stay(dt):
         assert bool((out[32:] == 7.0).all())
 
 
+@pytest.mark.parametrize("head_dim", [64, 80])  # the tile kernel, the one for every shape
+@pytest.mark.parametrize("dt", DT)
+def test_row_starts_behind_the_calls_rows_are_cut(dt, head_dim):
+    """q's rows bound the sequences': the memory behind out is not theirs."""
+    b = R.batch(DT[dt], 8, 2, head_dim, 16, [30, 2], [60, 300], seed=19, starts=[0, 2], shared=[48])
+    args = (b.q.cuda(), b.k_pool.cuda(), b.v_pool.cuda(), i32([0, 30, 2 ** 31 - 1]), i32(b.kv), b.tables.cuda())
+    for window in (True, False):
+        memory = torch.full((64, 8, head_dim), 7.0, dtype=DT[dt], device="cuda")
+        if window:
+            ops.varlen_prefill_window(*args, 30, 300, 0.09, 33, 1, out=memory[:32])
+        else:
+            ops.varlen_prefill_shared(*args, i32(b.starts), i32(b.shared), 30, 300, 48, 0.09, out=memory[:32])
+        check(memory[:32], b, 0.09, TILE_EPS[dt], 33 if window else R.EVERY, 1 if window else 0)
+        assert bool((memory[32:] == 7.0).all())
+
+
 @pytest.mark.parametrize("dt", DT)
 def test_bounds_cut_longer_sequences_and_prefixes(dt):
     b = R.batch(DT[dt], 8, 2, 128, 16, [1, 1, 1], [600, 200, 90], seed=10, starts=[0, 3], shared=[80])
