@@ -270,6 +270,11 @@ __global__ __launch_bounds__(64 * RT_WAVES, rt_workgroups(sizeof(T), D, HALVES))
         }
         request();  // the tile after the next one
         const bool full = tok_end <= min_hi && (tok0 >= max_lo || tok_end <= sinks);
+        // Masked scores are handed on whole: element by element, tiles without a mask would copy theirs too.
+        auto masked = [&]() __attribute__((always_inline)) {
+#pragma unroll
+            for (int b = 0; b < NB; b++) asm volatile("" : "+v"(s[b]));
+        };
         // (positions of a register are known up to where the tile and the lane's half start)
         if (!full && t >= plain) {
             const int at = tok0 + tok_half + 4 * half, r_hi = hi - at, r_lo = lo - at, r_sinks = sinks - at;
@@ -281,6 +286,7 @@ __global__ __launch_bounds__(64 * RT_WAVES, rt_workgroups(sizeof(T), D, HALVES))
                     const bool sees = (x < r_hi) & ((x >= r_lo) | (x < r_sinks));
                     s[b][e] = sees ? s[b][e] : -INFINITY;
                 }
+            masked();
         } else if (!full) {
 #pragma unroll
             for (int b = 0; b < NB; b++)
@@ -291,10 +297,8 @@ __global__ __launch_bounds__(64 * RT_WAVES, rt_workgroups(sizeof(T), D, HALVES))
                     const bool sees = (tok < hi) & ((tok >= lo) | (tok < sinks));
                     s[b][e] = sees ? s[b][e] : -INFINITY;
                 }
+            masked();
         }
-        // (one register for a score whether the masks above ran or not, or every tile copies them)
-#pragma unroll
-        for (int b = 0; b < NB; b++) asm volatile("" : "+v"(s[b]));
         float top = s[0][0];
 #pragma unroll
         for (int b = 0; b < NB; b++)
