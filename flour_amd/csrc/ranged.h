@@ -42,31 +42,30 @@ __device__ __forceinline__ RangedSeq ranged_seq(const RangedAttn& a, int s) {
     return RangedSeq{r0, n, kv >= n && kv > 0 ? kv : 0};
 }
 
-// The sequence of packed row `row`: the last one that starts at or before it.
-__device__ __forceinline__ int ranged_seq_of(const RangedAttn& a, int row) {
-    int lo = 0, hi = a.num_seqs;
+// The last i in [lo, hi) with at[i] <= x (lo if there is none), at not decreasing; by a whole wave, the same x
+// and bounds in every lane: 64 of the range in a round.
+__device__ __forceinline__ int wave_last_at(const int32_t* at, int lo, int hi, int x) {
+    const int lane = threadIdx.x & 63;
     while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (a.cu[mid] <= row)
-            lo = mid;
-        else
-            hi = mid;
+        const int step = (hi - lo + 63) >> 6, i = lo + min(lane * step, hi - lo);
+        const int below = __builtin_popcountll(__ballot(i < hi && at[i] <= x));
+        hi = min(hi, lo + max(1, below) * step);
+        lo += max(0, below - 1) * step;
     }
     return lo;
 }
 
-// The group of sequence s (-1: none): the last one that starts at or before it, if it has not ended.
+// The sequence of packed row `row`, one for the wave: the last one that starts at or before it.
+__device__ __forceinline__ int ranged_seq_of(const RangedAttn& a, int row) {
+    return wave_last_at(a.cu, 0, a.num_seqs, row);
+}
+
+// The group of sequence s, one for the wave (-1: none): the last one that starts at or before it, if it has
+// not ended.
 __device__ __forceinline__ int ranged_group(const int32_t* starts, int num_groups, int s) {
     if (num_groups == 0 || starts[0] > s) return -1;
-    int lo = 0, hi = num_groups;  // the last g with starts[g] <= s
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (starts[mid] <= s)
-            lo = mid;
-        else
-            hi = mid;
-    }
-    return s < starts[lo + 1] ? lo : -1;
+    const int g = wave_last_at(starts, 0, num_groups, s);
+    return s < starts[g + 1] ? g : -1;
 }
 __device__ __forceinline__ int ranged_shared_len(const int32_t* shared_lens, int max_shared, int g) {
     return g < 0 ? 0 : max(0, min(shared_lens[g], max_shared));

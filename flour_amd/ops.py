@@ -805,8 +805,8 @@ def paged_decode_shared(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Ten
                         out_dtype: torch.dtype | None = None, out: torch.Tensor | None = None,
                         workspace: Workspace | None = None) -> torch.Tensor:
     """paged_decode for a batch in groups: sequences group_starts[g]:group_starts[g + 1] have the same
-    K/V at their first shared_lens[g] positions, which is computed once for all of the group's rows,
-    through its first sequence's table. ``max_shared_len`` bounds shared_lens."""
+    K/V at their first shared_lens[g] positions, which is computed once for all of the group's rows
+    where that is faster, through its first sequence's table. ``max_shared_len`` bounds shared_lens."""
     dev = _same_device(q, k_pool, v_pool, block_tables, context_lens, group_starts, shared_lens, out)
     _need_i32(block_tables, context_lens)
     G, slots, D = _plain_pools(q, k_pool, v_pool, block_size)

@@ -418,10 +418,10 @@ int flour_hip_varlen_prefill_window(void* out, int out_dtype, int64_t o_stride_t
  *                g. They must not decrease; sequences before the first or behind the last are in no
  *                group and attend to their own tables alone.
  *   shared_lens  [num_groups] int32: the first shared_lens[g] positions of group g's sequences are the
- *                same K/V. They are read through the table of the group's first sequence, which has to
- *                name their blocks (whatever that sequence's own length), the rest through each
- *                sequence's own. Any length counts, whole blocks or not; negative ones are 0, and
- *                longer ones than max_shared_len are taken as that.
+ *                same K/V. Every sequence's table names its positions as for the plain calls, the group's
+ *                first one all of the prefix's, whatever its own length; which of these tables a call
+ *                reads the prefix through is its choice. Any length counts, whole blocks or not; negative
+ *                ones are 0, and longer ones than max_shared_len are taken as that.
  * A row sees positions up to its own, in the prefix too, so sequences may be shorter than their group's
  * prefix. The other arguments are those of the plain calls; max_kv_len, rows behind the last sequence's,
  * the workspace (flour_hip_shared_workspace_size) and scores of NaN or infinity are as above.
