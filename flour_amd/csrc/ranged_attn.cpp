@@ -117,10 +117,8 @@ struct TilePlan {
 };
 // Waves that share 32 columns: 1 or 2, 0 by the plans' rules (a test switch).
 static int g_tile_halves = 0;
-// Three workgroups for two CUs are aimed at: 2 / 3 / 4 for two in us: 64 sequences of one prefix 8,192 + up to
-// 512 57.0 / 44.6 / 48.9, drafted rows 55.6 / 50.3 / 55.6, fp32 28.7 / 23.3 / 23.1. Pieces have four tiles at
-// least, eight where a launch could do without any (which saves the merge).
-static constexpr int WGS_OF_TWO_CUS = 3, LEAST_TILES = 4, LEAST_TILES_FINAL = 8;
+// Pieces have four tiles at least, eight where a launch could do without any (which saves the merge).
+static constexpr int LEAST_TILES = 4, LEAST_TILES_FINAL = 8;
 // Units of up to unit_rows rows (rows in all), an item for each of their column tiles and kv heads.
 static int64_t tile_items(int64_t units, int64_t unit_rows, int64_t rows, int64_t n_rep, int64_t kv_heads,
                           int64_t cols) {
@@ -129,10 +127,14 @@ static int64_t tile_items(int64_t units, int64_t unit_rows, int64_t rows, int64_
         std::min(rows * n_rep / cols + units, units * ((unit_rows * n_rep + cols - 1) / cols));
     return std::max<int64_t>(1, tiles * kv_heads);
 }
-// Tiles of a piece, so that `steps` of them come to so many workgroups, `least` at least: a shorter piece costs
-// more in its ends and its merge than it saves.
-static int64_t tiles_of_piece(int64_t steps, int64_t least) {
-    const int64_t slots = WGS_OF_TWO_CUS * device_cus() / 2;
+// Tiles of a piece, so that `steps` of them come to seven workgroups for four CUs (fp32: eight), and `least` at
+// least: more workgroups than are at work at once leave a last round of few and longer merges, fewer leave long
+// pieces. 5 / 6 / 7 / 8 / 9 / 10 for four in us, 64 sequences of one prefix 4,096 + 64-1,024: bf16, 32 / 8 heads
+// of 128 58.7 / 57.6 / 55.6 / 59.1 / 58.9 / 59.6, 28 / 4, eight rows each 69.5 / 67.1 / 65.3 / 76.8 / 77.0 / 76.8;
+// the mean of 68 such batches 1 / 0.964 / 0.946 / 0.953 / 0.977 / 0.997, 35 of 14 / 2 heads of 64 1 / 0.975 / 0.956 /
+// 0.964 / 0.955 / 0.953, 35 in fp32, 8 / 8 of 64, 1 / 0.929 / 0.889 / 0.868 / 0.861 / 0.865.
+static int64_t tiles_of_piece(int64_t steps, int64_t least, int dtype) {
+    const int64_t slots = (dtype == FLOUR_DTYPE_F32 ? 8 : 7) * device_cus() / 4;
     return std::max(least, (steps + slots - 1) / slots);
 }
 static TilePlan tile_plan(int halves, int64_t items, int64_t longest, int64_t piece_tiles, int64_t rows,
@@ -197,7 +199,7 @@ static TilePlan rows_plan(int num_seqs, int max_rows, int rows, int num_heads, i
         const int64_t span = (int64_t)window + sinks + cols / n_rep + 2;
         longest = std::min<int64_t>(max_kv, span) / tt + 2;  // (ends that are not whole tiles)
         const bool idle = longest >= 64 ? items <= cus : longest >= 24 && 2 * items <= cus;
-        piece = idle ? tiles_of_piece(items * longest, LEAST_TILES_FINAL) : longest;
+        piece = idle ? tiles_of_piece(items * longest, LEAST_TILES_FINAL, dtype) : longest;
     };
     cut(1);
     // (whole columns where the cut fills the chip: fp32, 32 / 8 of 128, 80 items of 258 tiles 258 / 277)
@@ -233,7 +235,7 @@ static SharedPlan shared_plan(int num_seqs, int num_groups, int max_rows, int ro
     const int64_t items_o = tile_items(num_seqs, max_rows, rows, n_rep, kv_heads, cols);
     // (a sequence of a group with a shorter prefix can have more of its own: its pieces are longer)
     const int64_t long_p = max_shared / tt + 1, long_o = std::max(0, max_kv - max_shared) / tt + 2;
-    const int64_t piece = tiles_of_piece(items_p * long_p + items_o * long_o, LEAST_TILES);
+    const int64_t piece = tiles_of_piece(items_p * long_p + items_o * long_o, LEAST_TILES, dtype);
     return SharedPlan{tile_plan(halves, items_p, long_p, piece, rows, num_heads, head_dim, false),
                       tile_plan(halves, items_o, long_o, piece, rows, num_heads, head_dim, false)};
 }

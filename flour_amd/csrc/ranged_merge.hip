@@ -2,14 +2,14 @@
 // the pieces k of a (row, query head), M their largest maximum.
 //
 // A wave a (row, head), four to a workgroup; a lane holds the maximum and sum of one piece and D / 64
-// dims of the output, over 8 pieces' rows at a time, all in flight together. It reads each piece once. 64 rows of
+// dims of the output, over 16 pieces' rows at a time, all in flight together. It reads each piece once. 64 rows of
 // 32 heads of 128, up to 10 pieces each: 6.7 us; 165 rows 10.6; 16 rows of 8 heads of 64 4.3, which is its
 // launch and two dependent reads.
 #include "ranged_tiles.h"
 
 namespace flour {
 
-static constexpr int RM_WAVES = 4;
+static constexpr int RM_WAVES = 4, RM_ROWS = 16;
 
 struct RmPieces {
     int n;
@@ -57,14 +57,17 @@ __global__ __launch_bounds__(64 * RM_WAVES) void ranged_merge_kernel(RtArgs ra) 
         const int n = min(64, all - p0), mine = min(p0 + lane, all - 1);
         const float* at = mine < p.n ? p.ml + 2 * mine : p2.ml + 2 * (mine - p.n);
         const float mx = at[0], lx = at[1];
-        RowV v[8];
+        RowV v[RM_ROWS];
         auto request = [&](int y0) __attribute__((always_inline)) {
 #pragma unroll
-            for (int y = 0; y < 8; y++) {  // (past the last one: that again, for nothing)
-                const int k = min(p0 + y0 + y, all - 1);
-                const float* o = k < p.n ? p.o + (int64_t)k * D : p2.o + (int64_t)(k - p.n) * D;
-                v[y] = *reinterpret_cast<const RowV*>(o + E * lane);
-            }
+            for (int x = 0; x < RM_ROWS; x += 4)
+                if (y0 + x < n)
+#pragma unroll
+                    for (int y = x; y < x + 4; y++) {  // (past the last one: that again, for nothing)
+                        const int k = min(p0 + y0 + y, all - 1);
+                        const float* o = k < p.n ? p.o + (int64_t)k * D : p2.o + (int64_t)(k - p.n) * D;
+                        v[y] = *reinterpret_cast<const RowV*>(o + E * lane);
+                    }
         };
         request(0);  // (beside the maxima)
         const bool on = lane < n;
@@ -73,10 +76,10 @@ __global__ __launch_bounds__(64 * RM_WAVES) void ranged_merge_kernel(RtArgs ra) 
         L = L * old + wave_sum(on ? w * lx : 0.0f);
 #pragma unroll
         for (int e = 0; e < E; e++) O[e] *= old;
-        for (int y0 = 0; y0 < n; y0 += 8) {
+        for (int y0 = 0; y0 < n; y0 += RM_ROWS) {
             if (y0 > 0) request(y0);
 #pragma unroll
-            for (int y = 0; y < 8; y++) {
+            for (int y = 0; y < RM_ROWS; y++) {
                 const float wy = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w), (y0 + y) & 63));
                 if (y0 + y < n) {
                     if constexpr (E == 2) {
