@@ -115,7 +115,8 @@ struct TilePlan {
     int items, max_pieces, piece_tiles, halves;
     size_t bytes;  // of the pieces
 };
-// Waves that share 32 columns: 1 or 2, 0 by the plans' rules (a test switch).
+// Waves that share 32 columns: 1 or 2, 0 by the plans' rules, 3 one but two of own positions where the
+// rules may say that (a test switch).
 static int g_tile_halves = 0;
 // Pieces have four tiles at least, eight where a launch could do without any (which saves the merge).
 static constexpr int LEAST_TILES = 4, LEAST_TILES_FINAL = 8;
@@ -151,9 +152,8 @@ static TilePlan tile_plan(int halves, int64_t items, int64_t longest, int64_t pi
     return p;
 }
 
-static RtArgs tile_args(const RangedAttn& a, int halves) {
+static RtArgs tile_args(const RangedAttn& a) {
     RtArgs r{};
-    r.cols = rt_cols(halves), r.tile = rt_tokens(elem_bytes(a.dtype), halves);
     r.a = a, r.n_rep = a.num_heads / a.kv_heads;
     r.scale_log2 = a.scale * 1.4426950408889634f;
     return r;
@@ -161,17 +161,18 @@ static RtArgs tile_args(const RangedAttn& a, int halves) {
 static void add_part(RtArgs* r, int kind, const TilePlan& p, bool finals, char* ws) {
     RtPart& t = r->part[r->parts++];
     t.kind = kind, t.items = p.items, t.max_pieces = p.max_pieces, t.piece_tiles = p.piece_tiles;
+    t.cols = rt_cols(p.halves), t.tile = rt_tokens(elem_bytes(r->a.dtype), p.halves);
     t.finals = finals;
     t.p_ml = reinterpret_cast<float*>(ws);
     t.p_o = reinterpret_cast<float*>(
         ws + up256((size_t)r->a.rows * r->a.num_heads * p.max_pieces * 2 * sizeof(float)));
 }
 
-static int launch_tiles(const RtArgs& r, int halves, hipStream_t stream) {
+static int launch_tiles(const RtArgs& r, int halves, int last, hipStream_t stream) {
     auto launch = r.a.dtype == FLOUR_DTYPE_F32    ? launch_ranged_tiles_f32
                   : r.a.dtype == FLOUR_DTYPE_BF16 ? launch_ranged_tiles_bf16
                                                   : launch_ranged_tiles_f16;
-    return launch(r, halves, stream);
+    return launch(r, halves, last, stream);
 }
 
 // Rows over what they see: one launch, and a merge where items are cut.
@@ -228,16 +229,23 @@ static SharedPlan shared_plan(int num_seqs, int num_groups, int max_rows, int ro
                          (rows * n_rep >= (int64_t)192 * num_groups && tiles_p >= 3000)
                      ? 1
                      : 2;
-    if (g_tile_halves > 0) halves = g_tile_halves;
-    const int cols = rt_cols(halves);
-    const int64_t tt = rt_tokens(elem_bytes(dtype), halves);
-    const int64_t items_p = tile_items(num_groups, rows, rows, n_rep, kv_heads, cols);
-    const int64_t items_o = tile_items(num_seqs, max_rows, rows, n_rep, kv_heads, cols);
+    if (g_tile_halves > 0) halves = g_tile_halves == 2 ? 2 : 1;
+    // Own positions of up to 64 columns a sequence: two waves anyway, since items of 128 would be half empty, or
+    // more. Prefixes and own positions by waves of 64 / the latter by half of them in us: 64 sequences of four
+    // prefixes 4,096 + 64-1,024, eight rows each, bf16, 32 / 8 heads 99.1 / 91.2, one row 61.7 / 59.3; of one
+    // 16,384 + 6-100, 64 / 8 heads, 72.1 / 68.9. (fp32 at 128 would keep one workgroup a CU for it.)
+    const bool narrow = max_rows * n_rep <= rt_cols(2) && rt_mixes(elem_bytes(dtype), head_dim);
+    const int own = narrow && (g_tile_halves == 0 || g_tile_halves == 3) ? 2 : halves;
+    auto items = [&](int64_t units, int unit_rows, int h) {
+        return tile_items(units, unit_rows, rows, n_rep, kv_heads, rt_cols(h));
+    };
+    const int es = elem_bytes(dtype), tt = rt_tokens(es, halves), tt_own = rt_tokens(es, own);
+    const int64_t items_p = items(num_groups, rows, halves), items_o = items(num_seqs, max_rows, own);
     // (a sequence of a group with a shorter prefix can have more of its own: its pieces are longer)
-    const int64_t long_p = max_shared / tt + 1, long_o = std::max(0, max_kv - max_shared) / tt + 2;
+    const int64_t long_p = max_shared / tt + 1, long_o = std::max(0, max_kv - max_shared) / tt_own + 2;
     const int64_t piece = tiles_of_piece(items_p * long_p + items_o * long_o, LEAST_TILES, dtype);
     return SharedPlan{tile_plan(halves, items_p, long_p, piece, rows, num_heads, head_dim, false),
-                      tile_plan(halves, items_o, long_o, piece, rows, num_heads, head_dim, false)};
+                      tile_plan(own, items_o, long_o, piece, rows, num_heads, head_dim, false)};
 }
 
 // Whether prefixes are worth a part of their own, by an estimate of both ways in us from the host's bounds.
@@ -302,19 +310,19 @@ static int ranged_call(const char* what, const RangedAttn& a, bool shared, void*
                                          a.kv_heads, a.head_dim, a.max_kv, a.max_shared, a.dtype);
         if (prefer_shared(a.num_seqs, a.num_groups, a.max_rows, a.rows, a.num_heads, a.kv_heads,
                           a.head_dim, a.max_kv, a.max_shared, a.dtype, p)) {
-            RtArgs r = tile_args(a, p.own.halves);
+            RtArgs r = tile_args(a);
             add_part(&r, RT_PREFIX, p.prefix, false, ws);
             add_part(&r, RT_OWN, p.own, false, ws + p.prefix.bytes);
-            rc = launch_tiles(r, p.own.halves, stream);
+            rc = launch_tiles(r, p.prefix.halves, p.own.halves, stream);
             return rc != FLOUR_OK ? rc : launch_ranged_merge(r, stream);
         }
     }
     if (step) return launch_stream(a, ws, stream);
     const TilePlan p = rows_plan(a.num_seqs, a.max_rows, a.rows, a.num_heads, a.kv_heads, a.head_dim,
                                  a.max_kv, a.window, a.sinks, a.dtype);
-    RtArgs r = tile_args(a, p.halves);
+    RtArgs r = tile_args(a);
     add_part(&r, RT_ROWS, p, true, ws);
-    rc = launch_tiles(r, p.halves, stream);
+    rc = launch_tiles(r, p.halves, p.halves, stream);
     return rc != FLOUR_OK || p.max_pieces == 1 ? rc : launch_ranged_merge(r, stream);
 }
 
@@ -507,7 +515,7 @@ extern "C" int flour_hip_set_window_pairs(int mode) {
 }
 
 extern "C" int flour_hip_set_tile_halves(int halves) {
-    if (halves < 0 || halves > 2) return FLOUR_ERR_INVALID_ARGUMENT;
+    if (halves < 0 || halves > 3) return FLOUR_ERR_INVALID_ARGUMENT;
     g_tile_halves = halves;
     switch_set();
     return FLOUR_OK;

@@ -23,12 +23,12 @@ __device__ __forceinline__ RmPieces tile_pieces(const RtArgs& ra, const RtPart& 
     RtSpan sp;
     if (pt.kind == RT_PREFIX) {
         if (shared == 0) return p;
-        sp = rt_span(ra, RT_PREFIX, 0, shared, 0, 0);
+        sp = rt_span(ra, pt, 0, shared, 0, 0);
     } else {
         const int col = (row - q.row0) * ra.n_rep + h % ra.n_rep;
-        sp = rt_span(ra, pt.kind, q.rows, q.kv, col / ra.cols, shared);
+        sp = rt_span(ra, pt, q.rows, q.kv, col / pt.cols, shared);
     }
-    p.n = rt_pieces(sp.tiles(ra.tile), pt.max_pieces, pt.piece_tiles);
+    p.n = rt_pieces(sp.tiles(pt.tile), pt.max_pieces, pt.piece_tiles);
     const int64_t slot = ((int64_t)row * ra.a.num_heads + h) * pt.max_pieces;
     p.ml = pt.p_ml + 2 * slot;
     p.o = pt.p_o + slot * head_dim;

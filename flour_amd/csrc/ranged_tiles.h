@@ -25,6 +25,7 @@ enum RtKind {
 // domain) and accumulator at slot (r * num_heads + h) * max_pieces + k.
 struct RtPart {
     int kind, items, max_pieces, piece_tiles;
+    int cols, tile;  // columns of an item, positions of a tile (rt_cols, rt_tokens)
     bool finals;
     float* p_ml;  // [slot][2]
     float* p_o;   // [slot][D]
@@ -33,7 +34,6 @@ struct RtArgs {
     RangedAttn a;
     int n_rep;
     float scale_log2;
-    int cols, tile;  // columns of an item, positions of a tile (rt_cols, rt_tokens)
     int parts;
     RtPart part[2];  // the first one's workgroups come first
 };
@@ -54,6 +54,11 @@ __host__ __device__ constexpr int rt_workgroups(int elem_bytes, int head_dim, in
     return row == 128 ? 3 : row * halves > 512 ? 1 : 2;
 }
 
+// Whether a launch's parts may differ in their halves.
+constexpr bool rt_mixes(int elem_bytes, int head_dim) {
+    return rt_workgroups(elem_bytes, head_dim, 2) == rt_workgroups(elem_bytes, head_dim, 1);
+}
+
 __host__ __device__ __forceinline__ int rt_pieces(int tiles, int max_pieces, int piece_tiles) {
     const int n = (tiles + piece_tiles - 1) / piece_tiles;
     return n < 1 ? 1 : (n < max_pieces ? n : max_pieces);
@@ -69,14 +74,14 @@ struct RtSpan {
     __device__ __forceinline__ int tiles(int tt) const { return (16 * runs + tt - 1) / tt; }
 };
 // rows and kv: the unit's. own: where the positions of RT_OWN start.
-__device__ __forceinline__ RtSpan rt_span(const RtArgs& ra, int kind, int rows, int kv, int ctile,
+__device__ __forceinline__ RtSpan rt_span(const RtArgs& ra, const RtPart& pt, int rows, int kv, int ctile,
                                           int own) {
     RtSpan s;
-    const int sinks = kind == RT_ROWS ? ra.a.sinks : 0;
+    const int kind = pt.kind, sinks = kind == RT_ROWS ? ra.a.sinks : 0;
     s.from = 0, s.to = kv;
     if (kind != RT_PREFIX) {
-        const int i0 = ctile * ra.cols / ra.n_rep;
-        const int i1 = min(rows * ra.n_rep - 1, ctile * ra.cols + ra.cols - 1) / ra.n_rep;
+        const int i0 = ctile * pt.cols / ra.n_rep;
+        const int i1 = min(rows * ra.n_rep - 1, ctile * pt.cols + pt.cols - 1) / ra.n_rep;
         s.to = kv > 0 ? kv - rows + i1 + 1 : 0;
         if (kind == RT_ROWS) {
             s.from = kv > 0 ? max(0, kv - rows + i0 + 1 - ra.a.window) : 0;
@@ -97,8 +102,9 @@ __device__ __forceinline__ RtSpan rt_span(const RtArgs& ra, int kind, int rows, 
 // alone.
 int launch_ranged_merge(const RtArgs& r, hipStream_t stream);
 
-int launch_ranged_tiles_f32(const RtArgs& r, int halves, hipStream_t stream);
-int launch_ranged_tiles_bf16(const RtArgs& r, int halves, hipStream_t stream);
-int launch_ranged_tiles_f16(const RtArgs& r, int halves, hipStream_t stream);
+// halves: of the first part's items, last: of the last part's (the same, or 2 behind 1 where rt_mixes).
+int launch_ranged_tiles_f32(const RtArgs& r, int halves, int last, hipStream_t stream);
+int launch_ranged_tiles_bf16(const RtArgs& r, int halves, int last, hipStream_t stream);
+int launch_ranged_tiles_f16(const RtArgs& r, int halves, int last, hipStream_t stream);
 
 }  // namespace flour

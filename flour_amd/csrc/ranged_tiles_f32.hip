@@ -3,8 +3,8 @@
 
 namespace flour {
 
-int launch_ranged_tiles_f32(const RtArgs& r, int halves, hipStream_t stream) {
-    return launch_ranged_tiles<float>(r, halves, stream);
+int launch_ranged_tiles_f32(const RtArgs& r, int halves, int last, hipStream_t stream) {
+    return launch_ranged_tiles<float>(r, halves, last, stream);
 }
 
 }  // namespace flour

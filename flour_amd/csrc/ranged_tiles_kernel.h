@@ -44,9 +44,19 @@ __device__ __forceinline__ u32x2 lds_read_tr16(const void* p) {
 
 __device__ __forceinline__ int wave_min_i32(int x) { return -wave_max_i32(-x); }
 
+// LDS pitches (bytes) of K and V rows: 16-byte reads of 16 rows, and V's, spread over the banks.
+template <typename T, int D>
+static constexpr int RT_KP = D * sizeof(T) + 16;
+template <typename T, int D>
+static constexpr int RT_VP = sizeof(T) == 4 ? D * 4 + 32 : (D == 128 ? 320 : 192);
+template <typename T, int D>
+__host__ __device__ constexpr int rt_lds(int halves) {
+    return 2 * rt_tokens(sizeof(T), halves) * (RT_KP<T, D> + RT_VP<T, D>);
+}
+
+// Workgroup wg of a part.
 template <typename T, int D, int HALVES>
-__global__ __launch_bounds__(64 * RT_WAVES, rt_workgroups(sizeof(T), D, HALVES)) void ranged_tiles_kernel(
-    RtArgs ra) {
+__device__ __forceinline__ void ranged_tiles_body(const RtArgs& ra, const RtPart pt, int wg, unsigned char* lds) {
     constexpr bool F32 = std::is_same<T, float>::value;
     constexpr bool BF16 = std::is_same<T, bf16_t>::value;
     constexpr int ES = sizeof(T), ROW = D * ES;       // bytes of a K / V row
@@ -54,12 +64,11 @@ __global__ __launch_bounds__(64 * RT_WAVES, rt_workgroups(sizeof(T), D, HALVES))
     constexpr int TT = rt_tokens(ES, HALVES);         // positions of a tile
     constexpr int NB = TT / 32 / HALVES;              // the wave's blocks of 32
     constexpr int NO = D / 32;                        // 32-dim blocks of the output
-    constexpr int KP = ROW + 16;                      // LDS pitches (bytes): 16-byte reads of 16 rows,
-    constexpr int VP = F32 ? ROW + 32 : (D == 128 ? 320 : 192);  // and V's, spread over the banks
+    constexpr int KP = RT_KP<T, D>, VP = RT_VP<T, D>;
     constexpr int LPR = ROW / 16, RPP = 64 * RT_WAVES / LPR, NP = TT / RPP;  // staging: lanes a row, rows
                                                                             // and passes of 16 bytes a thread
-    __shared__ __attribute__((aligned(16))) unsigned char k_lds[2][TT * KP];
-    __shared__ __attribute__((aligned(16))) unsigned char v_lds[2][TT * VP];
+    unsigned char (*const k_lds)[TT * KP] = reinterpret_cast<unsigned char (*)[TT * KP]>(lds);
+    unsigned char (*const v_lds)[TT * VP] = reinterpret_cast<unsigned char (*)[TT * VP]>(lds + 2 * TT * KP);
     const RangedAttn& a = ra.a;
     const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, l32 = lane & 31;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -67,9 +76,6 @@ __global__ __launch_bounds__(64 * RT_WAVES, rt_workgroups(sizeof(T), D, HALVES))
 
     // ---- the item: (unit, column tile), kv head fastest (neighbouring workgroups, one an XCD, have
     // different heads, so each XCD's L2 holds its own heads' K/V)
-    const bool second = blockIdx.x >= (unsigned)(ra.part[0].items * ra.part[0].max_pieces);
-    const RtPart pt = ra.part[second ? 1 : 0];
-    const int wg = (int)blockIdx.x - (second ? ra.part[0].items * ra.part[0].max_pieces : 0);
     const int piece = wg / pt.items, item = wg - piece * pt.items;
     const int g = item % a.kv_heads, want = item / a.kv_heads;
     const int units = pt.kind == RT_PREFIX ? a.num_groups : a.num_seqs;
@@ -141,7 +147,7 @@ __global__ __launch_bounds__(64 * RT_WAVES, rt_workgroups(sizeof(T), D, HALVES))
         else
             lo = own = ranged_shared_of(a, seq);
     }
-    const RtSpan sp = rt_span(ra, pt.kind, rows, kv, ctile, own);
+    const RtSpan sp = rt_span(ra, pt, rows, kv, ctile, own);
     const int front = sp.front, from = sp.from, to = sp.to, all_tiles = sp.tiles(TT);
     // Tiles from `plain` on hold consecutive positions, tok_off + TT t .. ; those before hold sinks.
     const int plain = (sp.front_runs + TT / 16 - 1) / (TT / 16), tok_off = sp.base - 16 * sp.front_runs;
@@ -573,15 +579,37 @@ __global__ __launch_bounds__(64 * RT_WAVES, rt_workgroups(sizeof(T), D, HALVES))
     }
 }
 
-template <typename T>
-static int launch_ranged_tiles(const RtArgs& r, int halves, hipStream_t stream) {
-    auto kern = r.a.head_dim == 64
-                    ? (halves == 2 ? ranged_tiles_kernel<T, 64, 2> : ranged_tiles_kernel<T, 64, 1>)
-                    : (halves == 2 ? ranged_tiles_kernel<T, 128, 2> : ranged_tiles_kernel<T, 128, 1>);
+template <typename T, int D, int HALVES, int LAST>
+__global__ __launch_bounds__(64 * RT_WAVES, std::min(rt_workgroups(sizeof(T), D, HALVES),
+                                                     rt_workgroups(sizeof(T), D, LAST))) void
+ranged_tiles_kernel(RtArgs ra) {
+    __shared__ __attribute__((aligned(16))) unsigned char
+        lds[std::max(rt_lds<T, D>(HALVES), rt_lds<T, D>(LAST))];
+    const int first = ra.part[0].items * ra.part[0].max_pieces;
+    const bool second = blockIdx.x >= (unsigned)first;
+    if (HALVES == LAST)
+        ranged_tiles_body<T, D, HALVES>(ra, ra.part[second ? 1 : 0], (int)blockIdx.x - (second ? first : 0), lds);
+    else if (second)
+        ranged_tiles_body<T, D, LAST>(ra, ra.part[1], (int)blockIdx.x - first, lds);
+    else
+        ranged_tiles_body<T, D, HALVES>(ra, ra.part[0], (int)blockIdx.x, lds);
+}
+
+template <typename T, int D>
+static int launch_ranged_tiles_d(const RtArgs& r, int halves, int last, hipStream_t stream) {
+    auto kern = halves == 2 ? ranged_tiles_kernel<T, D, 2, 2> : ranged_tiles_kernel<T, D, 1, 1>;
+    if constexpr (rt_mixes(sizeof(T), D))
+        if (halves < last) kern = ranged_tiles_kernel<T, D, 1, 2>;
     int64_t grid = 0;
     for (int i = 0; i < r.parts; i++) grid += (int64_t)r.part[i].items * r.part[i].max_pieces;
     kern<<<dim3((unsigned)grid), dim3(64 * RT_WAVES), 0, stream>>>(r);
     return check_hip(hipGetLastError(), "attention over ranges launch");
+}
+
+template <typename T>
+static int launch_ranged_tiles(const RtArgs& r, int halves, int last, hipStream_t stream) {
+    return r.a.head_dim == 64 ? launch_ranged_tiles_d<T, 64>(r, halves, last, stream)
+                              : launch_ranged_tiles_d<T, 128>(r, halves, last, stream);
 }
 
 }  // namespace flour

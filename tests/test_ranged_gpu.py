@@ -22,11 +22,12 @@ def prefixes_on_their_own():
 
 @pytest.fixture
 def both_halves():
-    """A function that runs another with a wave's columns its own and shared with a second one."""
+    """A function that runs another with a wave's columns its own, shared with a second one, and the latter
+    behind prefixes only."""
     lib = _lib.lib()
 
     def each(f):
-        for halves in (1, 2):
+        for halves in (1, 2, 3):
             assert lib.flour_hip_set_tile_halves(halves) == 0
             f()
 
