@@ -112,7 +112,7 @@ static bool tiles_take(const RangedAttn& a) {
 
 // A launch's items and the pieces that their tiles are cut into.
 struct TilePlan {
-    int items, max_pieces, piece_tiles, halves;
+    int items, max_pieces, piece_tiles, longest, halves;
     size_t bytes;  // of the pieces
 };
 // Waves that share 32 columns: 1 or 2, 0 by the plans' rules, 3 one but two of own positions where the
@@ -143,7 +143,7 @@ static TilePlan tile_plan(int halves, int64_t items, int64_t longest, int64_t pi
     TilePlan p;
     p.halves = halves;
     p.items = (int)items;
-    p.piece_tiles = (int)piece_tiles;
+    p.piece_tiles = (int)piece_tiles, p.longest = (int)longest;
     p.max_pieces = (int)((longest + piece_tiles - 1) / piece_tiles);
     p.bytes = finals && p.max_pieces == 1
                   ? 0
@@ -248,35 +248,40 @@ static SharedPlan shared_plan(int num_seqs, int num_groups, int max_rows, int ro
                       tile_plan(own, items_o, long_o, piece, rows, num_heads, head_dim, false)};
 }
 
-// Whether prefixes are worth a part of their own, by an estimate of both ways in us from the host's bounds.
-// A tile step (128 columns, 32 KB of K / V at head_dim 128 in 16 bits) takes the chip 4.7-5.9 ns; pieces are
-// written and read at about 8 TB/s. Decode steps alone are streamed: what several sequences read comes from
-// the caches for the most part. Fitted on 32 / 8 heads of 128, bf16, prefix + own, us alone / shared:
-//   64 sequences of one prefix 256 + 64 15.6 / 19.9, 1,024 + 64 31.5 / 20.7, 4,096 + 256 91 / 38,
-//   16,384 + 128 313 / 48; of 32 prefixes 256 + 64 18.5 / 26.7, 1,024 + 64 45.9 / 39.1;
-//   4 sequences of one prefix 1,024 + 1,024 15.6 / 16.7, 16,384 + 128 29.2 / 28.9
+// Whether prefixes are worth a part of their own, by an estimate of both ways in us from the host's bounds,
+// fitted on 412 batches of up to 64 sequences (the rms of an estimate is 15%, the chosen way takes 1.006 times the
+// better one in the mean). A step is 64 positions of 128 columns: `step` us of a CU; a piece's steps, one
+// behind the other, take twice that, or a third where a prefix has its CU to itself, and pieces are written
+// and read. Streamed decode steps are read at 5-6 TB/s, several times that where many sequences read the same.
+// 32 / 8 heads of 128, bf16, prefix + own, us alone / shared: 64 sequences of one prefix 512 + 64 15.0 / 23.4,
+// 2,048 + 256 39.6 / 32.6, 8,192 + 512 136 / 51; of eight, eight rows each, 512 + 64 25.9 / 41.1, 2,048 + 512
+// 79.9 / 66.4; 2 of one 2,048 + 512, eight rows, 23.1 / 19.8; 16, 64 rows, 69.5 / 84.8.
 static bool prefer_shared(int num_seqs, int num_groups, int max_rows, int rows, int num_heads, int kv_heads,
                           int head_dim, int max_kv, int max_shared, int dtype, const SharedPlan& p) {
     if (num_groups == 0 || max_shared == 0 || g_ranged_shared >= 0)
         return num_groups > 0 && max_shared > 0 && g_ranged_shared > 0;
-    const double es = elem_bytes(dtype), G = kv_heads, n_rep = num_heads / kv_heads;
-    const double cols = rt_cols(1), tt = rt_tokens((int)es, 1), row = 2.0 * G * head_dim * es;  // K and V of a position
-    const double ns = 5e-3 * (dtype == FLOUR_DTYPE_F32 ? 2.0 : 1.0) * head_dim / 128;  // a tile step
-    const double own = std::max(1, max_kv - max_shared), S = std::min(num_seqs, rows);
-    const double groups = std::min(num_groups, num_seqs);
-    const double seq_tiles =
-        std::min(S * ceil((double)max_rows * n_rep / cols), rows * n_rep / cols + S);
-    const double group_tiles = rows * n_rep / cols + groups;
-    const double pieces =
-        (double)rows * num_heads * (head_dim + 2) * 4.0 *
-        (std::min<double>(p.prefix.max_pieces, ceil(max_shared / tt / p.prefix.piece_tiles)) +
-         std::min<double>(p.own.max_pieces, ceil(own / tt / p.own.piece_tiles)));
-    const double shared_us = 14.0 + ns * G * (group_tiles * max_shared / tt + seq_tiles * (own / tt + 0.5)) +
-                             2.0 * pieces / 8e6;
-    const double unique = (groups * max_shared + S * own) * row, all = S * max_kv * row;
-    const double alone_us = max_rows <= 1 && n_rep <= 16
-                                ? 8.0 + unique / 5.5e6 + std::max(0.0, all - unique) / 12e6
-                                : 8.0 + ns * G * seq_tiles * (max_kv / tt + 0.5);
+    const int es = elem_bytes(dtype), n_rep = num_heads / kv_heads;
+    const bool f32 = dtype == FLOUR_DTYPE_F32;
+    const double step = f32 ? (head_dim == 64 ? 3.2 : 6.4) : (head_dim == 64 ? 0.7 : 1.15);
+    auto chain = [&](const TilePlan& t) {
+        return step * std::min(t.piece_tiles, t.longest) * rt_tokens(es, t.halves) / (64.0 * t.halves);
+    };
+    auto work = [&](const TilePlan& t) {
+        return step * t.items * t.longest * rt_tokens(es, t.halves) / (64.0 * t.halves) / device_cus();
+    };
+    auto merge = [&](const TilePlan& t) { return 2.0 * t.max_pieces * rows * num_heads * (head_dim + 2) * 4 / 8e6; };
+    const double shared_us = 12.5 + (f32 ? 1.2 : 0.34) * std::max(chain(p.prefix), chain(p.own)) + work(p.prefix) +
+                             (f32 ? 0.87 : 1.85) * work(p.own) + 2.0 * (merge(p.prefix) + merge(p.own));
+    double alone_us;
+    if (max_rows <= 1 && n_rep <= 16) {
+        const double bytes = 2.0 * num_seqs * max_kv * kv_heads * head_dim * es;
+        const double sharers = std::max(1.0, (double)num_seqs / num_groups);
+        alone_us = 7.0 + bytes / ((f32 ? 5e6 : 6e6) * (1.0 + 0.25 * log2(sharers) * std::min(1.0, num_seqs / 64.0)));
+    } else {
+        const TilePlan t = rows_plan(num_seqs, max_rows, rows, num_heads, kv_heads, head_dim, max_kv, 0x7fffffff,
+                                     0, dtype);
+        alone_us = 6.5 + std::max(1.95 * chain(t), work(t)) + (t.max_pieces > 1 ? 6.5 + 4.2 * merge(t) : 0.0);
+    }
     return shared_us < alone_us;
 }
 
