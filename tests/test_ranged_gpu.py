@@ -115,6 +115,13 @@ def test_decode_window(dt, heads, window, sinks):
     assert not bool(got[0].any())
 
 
+@pytest.mark.parametrize("dt", DT)
+@pytest.mark.parametrize("window,sinks", [(2 ** 31 - 1, 5), (3, 2 ** 31 - 1), (2 ** 31 - 1, 2 ** 31 - 1)])
+def test_decode_window_over_everything(dt, window, sinks):
+    b = R.batch(DT[dt], 8, 2, 64, 16, [1] * 4, [0, 1, 333, 2000], seed=24)
+    check_steps(b, 0.125, DECODE_EPS[dt], window, sinks)
+
+
 @pytest.mark.parametrize("bs", [1, 7, 8, 32, 48, 80])
 @pytest.mark.parametrize("dt", DT)
 def test_decode_window_other_pages(dt, bs):
@@ -178,6 +185,26 @@ def test_prefill_window_many_sequences(dt, n):
     rows = [min(L, (s * 31) % 40) for s, L in enumerate(kv)]
     b = R.batch(DT[dt], 14, 2, 64, 16, rows, kv, seed=n)
     check(run(b, 0.125, 50, 3), b, 0.125, TILE_EPS[dt], 50, 3)
+
+
+@pytest.mark.parametrize("dt", DT)
+@pytest.mark.parametrize("heads", [(8, 2, 64), (7, 1, 128), (130, 1, 64)], ids=str)
+@pytest.mark.parametrize("window,sinks", [(3000, 20), (2 ** 31 - 1, 0), (5, 2 ** 31 - 1)])
+def test_prefill_window_few_rows_over_many_positions(dt, heads, window, sinks, both_halves):
+    """Items cut along the positions, and (130 heads) rows that fill more than one item."""
+    b = R.batch(DT[dt], *heads, 16, [5, 0, 1, 20], [5000, 9, 4100, 20], seed=21)
+    both_halves(lambda: check(run(b, 0.1, window, sinks), b, 0.1, TILE_EPS[dt], min(window, R.EVERY), sinks))
+
+
+def test_thousands_of_sequences():
+    n, per = 4200, 60  # (more than the decode stream takes, and than two rounds of a wave's search)
+    starts, shared = list(range(0, n + 1, per)), [16 * (g % 3) for g in range(n // per)]
+    kv = [shared[s // per] + s % 5 for s in range(n)]
+    for decode in (True, False):
+        rows = [1] * n if decode else [min(L, s % 3) for s, L in enumerate(kv)]
+        b = R.batch(torch.bfloat16, 2, 1, 64, 16, rows, kv, seed=22, starts=starts, shared=shared)
+        check(run(b, 0.125, decode=decode), b, 0.125, TILE_EPS["bf16"])
+        check(run(b, 0.125, 7, 2, decode=decode), b, 0.125, TILE_EPS["bf16"], 7, 2)
 
 
 # ------------------------------------------------------------------ shared prefixes
