@@ -22,8 +22,8 @@
 //    times a V row of NaN or infinity that other columns of the tile see is NaN in the products.
 //  * fp32: v_mfma_f32_32x32x2 throughout, tiles of 32 positions.
 //
-// 16,384 tokens, window 2,048, 28 / 4 heads of 128 in bf16: 547-569 us, 795-827 TFLOP/s of visible products at
-// a clock of 1.9 GHz. Matrix cores are busy for 40% of the cycles, vector instructions issue in 50%
+// 16,384 tokens, window 2,048, 28 / 4 heads of 128 in bf16: 536-558 us, 810-844 TFLOP/s of visible products at
+// a clock of 1.9 GHz. Matrix cores are busy for 41% of the cycles, vector instructions issue in 47%
 // (180 a wave and tile of 32 products: weights 96, V to f16 48, maximum 19), hardly ever both at once; LDS reads
 // have no bank conflicts. Eight prompts (256-2,048 rows, window 512, 32 / 8 heads): 77 us, where an item is ten
 // tiles and its first one waits for tables, queries and rows. K rows straight to LDS (no registers, 16 fewer
