@@ -60,18 +60,24 @@ __device__ __forceinline__ int ranged_seq_of(const RangedAttn& a, int row) {
     return wave_last_at(a.cu, 0, a.num_seqs, row);
 }
 
-// The group of sequence s, one for the wave (-1: none): the last one that starts at or before it, if it has
-// not ended.
-__device__ __forceinline__ int ranged_group(const int32_t* starts, int num_groups, int s) {
-    if (num_groups == 0 || starts[0] > s) return -1;
-    const int g = wave_last_at(starts, 0, num_groups, s);
-    return s < starts[g + 1] ? g : -1;
+// Groups first + lane: where they start and end, and their prefixes' lengths.
+struct RangedGroups {
+    int start, end, len;
+};
+__device__ __forceinline__ RangedGroups ranged_groups(const RangedAttn& a, int first) {
+    const int g = first + (threadIdx.x & 63);
+    if (g >= a.num_groups) return RangedGroups{0, 0, 0};
+    return RangedGroups{a.group_starts[g], a.group_starts[g + 1], a.shared_lens[g]};
 }
-__device__ __forceinline__ int ranged_shared_len(const int32_t* shared_lens, int max_shared, int g) {
-    return g < 0 ? 0 : max(0, min(shared_lens[g], max_shared));
+// The length of the prefix of sequence s, one for the wave, which is in one of these groups (0: in none).
+__device__ __forceinline__ int ranged_shared_in(const RangedAttn& a, const RangedGroups& x, int s) {
+    const uint64_t hit = __ballot(x.start <= s && s < x.end);
+    return hit ? max(0, min(__builtin_amdgcn_readlane(x.len, __builtin_ctzll(hit)), a.max_shared)) : 0;
 }
-__device__ __forceinline__ int ranged_shared_of(const RangedAttn& a, int s) {
-    return ranged_shared_len(a.shared_lens, a.max_shared, ranged_group(a.group_starts, a.num_groups, s));
+// The same of all groups, whose first 64 have been read.
+__device__ __forceinline__ int ranged_shared_of(const RangedAttn& a, const RangedGroups& x, int s) {
+    if (a.num_groups <= 64) return ranged_shared_in(a, x, s);
+    return ranged_shared_in(a, ranged_groups(a, wave_last_at(a.group_starts, 0, a.num_groups, s)), s);
 }
 
 // Takes every shape (ranged_generic.hip).

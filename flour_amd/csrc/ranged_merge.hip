@@ -44,10 +44,11 @@ __global__ __launch_bounds__(64 * RM_WAVES) void ranged_merge_kernel(RtArgs ra) 
     const int64_t item = (int64_t)blockIdx.x * RM_WAVES + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     if (item >= (int64_t)a.rows * a.num_heads) return;
     const int row = (int)(item / a.num_heads), h = (int)(item - (int64_t)row * a.num_heads);
+    const RangedGroups groups = ranged_groups(a, 0);  // (beside the sequence's search)
     const int s = a.cu ? ranged_seq_of(a, row) : row;
     const RangedSeq q = ranged_seq(a, s);
     if (row < q.row0 || row >= q.row0 + q.rows) return;  // (rows of no sequence)
-    const int shared = a.num_groups > 0 ? ranged_shared_of(a, s) : 0;
+    const int shared = ranged_shared_of(a, groups, s);
     const RmPieces p = tile_pieces(ra, ra.part[0], q, shared, row, h, D);
     const RmPieces p2 = ra.parts > 1 ? tile_pieces(ra, ra.part[1], q, shared, row, h, D) : RmPieces{};
     if (ra.part[0].finals && p.n == 1) return;

@@ -79,18 +79,20 @@ __device__ __forceinline__ void ranged_tiles_body(const RtArgs& ra, const RtPart
     const int piece = wg / pt.items, item = wg - piece * pt.items;
     const int g = item % a.kv_heads, want = item / a.kv_heads;
     const int units = pt.kind == RT_PREFIX ? a.num_groups : a.num_seqs;
-    int unit = -1, ctile = 0, row0 = 0, rows = 0, kv = 0;
+    int unit = -1, ctile = 0, row0 = 0, rows = 0, kv = 0, seq = 0;
+    // (what a prefix ends at, asked for beside the units)
+    const RangedGroups groups = pt.kind == RT_OWN ? ranged_groups(a, 0) : RangedGroups{};
     {
         int before = 0;
         for (int u0 = 0; u0 < units; u0 += 64) {
             const int u = u0 + lane;
-            int ur0 = 0, un = 0, ukv = 0;
+            int ur0 = 0, un = 0, ukv = 0, us = u;
             if (u < units) {
                 if (pt.kind == RT_PREFIX) {
-                    const int s0 = max(0, min(a.group_starts[u], a.num_seqs));
-                    const int s1 = max(s0, min(a.group_starts[u + 1], a.num_seqs));
+                    us = max(0, min(a.group_starts[u], a.num_seqs));
+                    const int s1 = max(us, min(a.group_starts[u + 1], a.num_seqs));
                     ukv = max(0, min(a.shared_lens[u], a.max_shared));
-                    ur0 = ranged_row(a, s0);
+                    ur0 = ranged_row(a, us);
                     un = ukv > 0 ? ranged_row(a, s1) - ur0 : 0;
                 } else {
                     const RangedSeq q = ranged_seq(a, u);
@@ -107,6 +109,7 @@ __device__ __forceinline__ void ranged_tiles_body(const RtArgs& ra, const RtPart
                 row0 = __builtin_amdgcn_readlane(ur0, w);
                 rows = __builtin_amdgcn_readlane(un, w);
                 kv = __builtin_amdgcn_readlane(ukv, w);
+                seq = __builtin_amdgcn_readlane(us, w);  // (a group with rows starts before num_seqs)
                 break;
             }
             before += __builtin_amdgcn_readlane(incl, 63);
@@ -114,39 +117,11 @@ __device__ __forceinline__ void ranged_tiles_body(const RtArgs& ra, const RtPart
     }
     if (unit < 0) return;
     const int ncols = rows * n_rep;
-    const int seq = pt.kind == RT_PREFIX ? max(0, min(a.group_starts[unit], a.num_seqs - 1)) : unit;
     const int32_t* bt = a.block_tables + (int64_t)seq * a.max_blocks;
 
-    // ---- the lane's column, and which positions t it sees: t < hi and (t >= lo or t < sinks)
-    const int col0 = ctile * COLS + 32 * (wave / HALVES);
-    const int tok_half = 32 * NB * (wave % HALVES);  // of a tile, where the wave's positions start
-    const bool live = col0 < ncols;  // (waves past the columns only stage)
-    const int col = min(col0 + l32, ncols - 1);
-    const bool real = col0 + l32 < ncols;
-    const int row_i = col / n_rep, head = g * n_rep + (col - row_i * n_rep);
-    const int row = row0 + row_i;
+    // ---- the positions
+    const int own = pt.kind == RT_OWN ? ranged_shared_of(a, groups, seq) : 0;
     const int sinks = pt.kind == RT_ROWS ? a.sinks : 0;
-    int hi, lo = 0, own = 0;
-    if (pt.kind == RT_PREFIX) {
-        int s = row;
-        if (a.cu) {  // the sequences from the wave's first row's to its last row's
-            const int s0 = ranged_seq_of(a, __builtin_amdgcn_readfirstlane(row));
-            const int s1 = ranged_seq_of(a, __builtin_amdgcn_readlane(row, 31));
-            s = s0;
-            for (int f = s0; f < s1; f += 64) {
-                const int next = a.cu[min(f + 1 + lane, a.num_seqs)], n = min(64, s1 - f);
-                for (int k = 0; k < n; k++) s += __builtin_amdgcn_readlane(next, k) <= row;
-            }
-        }
-        const RangedSeq q = ranged_seq(a, s);
-        hi = q.kv > 0 ? min(kv, q.kv - q.rows + (row - q.row0) + 1) : 0;
-    } else {
-        hi = kv > 0 ? kv - rows + row_i + 1 : 0;
-        if (pt.kind == RT_ROWS)
-            lo = max(0, hi - a.window);
-        else
-            lo = own = ranged_shared_of(a, seq);
-    }
     const RtSpan sp = rt_span(ra, pt, rows, kv, ctile, own);
     const int front = sp.front, from = sp.from, to = sp.to, all_tiles = sp.tiles(TT);
     // Tiles from `plain` on hold consecutive positions, tok_off + TT t .. ; those before hold sinks.
@@ -159,11 +134,8 @@ __device__ __forceinline__ void ranged_tiles_body(const RtArgs& ra, const RtPart
     // ---- this workgroup's piece of the tiles
     const int pieces = rt_pieces(all_tiles, pt.max_pieces, pt.piece_tiles);
     if (piece >= pieces) return;
-    const int t_begin = (int)((int64_t)all_tiles * piece / pieces);
-    const int t_end = (int)((int64_t)all_tiles * (piece + 1) / pieces);
-
-    const int min_hi = wave_min_i32(hi), max_hi = wave_max_i32(hi);
-    const int min_lo = wave_min_i32(lo), max_lo = wave_max_i32(lo);
+    const int share = all_tiles / pieces, more = all_tiles - share * pieces;  // (the first `more`: one more)
+    const int t_begin = share * piece + min(piece, more), t_end = t_begin + share + (piece < more);
 
     // ---- page slots of 16-position runs, 64 at a time, one a lane
     constexpr int UPT = TT / 16, WIN = 64 / UPT;  // runs a tile, tiles a refill
@@ -220,6 +192,48 @@ __device__ __forceinline__ void ranged_tiles_body(const RtArgs& ra, const RtPart
                 v[e] = pack2<f16_t>(lo_f32<bf16_t>(v[e]), hi_f32<bf16_t>(v[e]));
         *reinterpret_cast<u32x4*>(&v_lds[buf][r * VP + s_col]) = v;
     };
+
+    // ---- the first tile is asked for before what the columns see, which can take a few reads
+    uint32_t slots = 0, next = 0;
+    auto begin = [&]() __attribute__((always_inline)) {
+        if (t_begin >= t_end) return;
+        slots = next = load_slots(t_begin);
+        if (t_begin + WIN < t_end) next = load_slots(t_begin + WIN);
+        load_tile(slots, t_begin);
+    };
+    begin();
+
+    // ---- the lane's column, and which positions t it sees: t < hi and (t >= lo or t < sinks)
+    const int col0 = ctile * COLS + 32 * (wave / HALVES);
+    const int tok_half = 32 * NB * (wave % HALVES);  // of a tile, where the wave's positions start
+    const bool live = col0 < ncols;  // (waves past the columns only stage)
+    const int col = min(col0 + l32, ncols - 1);
+    const bool real = col0 + l32 < ncols;
+    const int row_i = col / n_rep, head = g * n_rep + (col - row_i * n_rep);
+    const int row = row0 + row_i;
+    int hi, lo = 0;
+    if (pt.kind == RT_PREFIX) {
+        int s = row;
+        if (a.cu) {  // the sequences from the wave's first row's to its last row's
+            const int s0 = ranged_seq_of(a, __builtin_amdgcn_readfirstlane(row));
+            const int s1 = ranged_seq_of(a, __builtin_amdgcn_readlane(row, 31));
+            s = s0;
+            for (int f = s0; f < s1; f += 64) {
+                const int next = a.cu[min(f + 1 + lane, a.num_seqs)], n = min(64, s1 - f);
+                for (int k = 0; k < n; k++) s += __builtin_amdgcn_readlane(next, k) <= row;
+            }
+        }
+        const RangedSeq q = ranged_seq(a, s);
+        hi = q.kv > 0 ? min(kv, q.kv - q.rows + (row - q.row0) + 1) : 0;
+    } else {
+        hi = kv > 0 ? kv - rows + row_i + 1 : 0;
+        if (pt.kind == RT_ROWS)
+            lo = max(0, hi - a.window);
+        else
+            lo = own;
+    }
+    const int min_hi = wave_min_i32(hi), max_hi = wave_max_i32(hi);
+    const int min_lo = wave_min_i32(lo), max_lo = wave_max_i32(lo);
 
     // ---- Q^T as the B operand: dims 16 kk + 8 half .. + 7 for product kk; fp32: dims D/2 half + s for
     // product s
@@ -414,9 +428,6 @@ __device__ __forceinline__ void ranged_tiles_body(const RtArgs& ra, const RtPart
 #pragma unroll
             for (int e = 0; e < 16; e++) acc[o][e] = 0.0f;
         if (t_begin >= t_end) return;
-        uint32_t slots = load_slots(t_begin), next = slots;
-        if (t_begin + WIN < t_end) next = load_slots(t_begin + WIN);
-        load_tile(slots, t_begin);
         cut_tile(t_begin);
 #pragma unroll
         for (int k = 0; k < NP; k++) stage_rows(exact, k, 0);
@@ -489,7 +500,10 @@ __device__ __forceinline__ void ranged_tiles_body(const RtArgs& ra, const RtPart
         sq = sum_across_halves(sq);
         const float least = 2.0f / (32768.0f * 1024.0f * 5e-4f * 2.0f);  // 2^-25 / 5e-4
         const bool again = live && owner && real && l != 0.0f && !(sq >= D * least * least * l * l && finite());
-        if (__syncthreads_or(again)) pass(yes{});
+        if (__syncthreads_or(again)) {
+            begin();
+            pass(yes{});
+        }
     }
 
     // ---- out: a lane holds dims 32 o + 8 (e / 4) + 4 half + e % 4 of its column
