@@ -156,12 +156,16 @@ static RtArgs tile_args(const RangedAttn& a) {
     RtArgs r{};
     r.a = a, r.n_rep = a.num_heads / a.kv_heads;
     r.scale_log2 = a.scale * 1.4426950408889634f;
+    r.max_id = (int)(a.num_slots / a.block_size - 1);
+    r.by_rep = rt_div(r.n_rep), r.by_heads = rt_div(a.num_heads), r.by_kv_heads = rt_div(a.kv_heads);
+    r.by_block = rt_div(a.block_size);
     return r;
 }
 static void add_part(RtArgs* r, int kind, const TilePlan& p, bool finals, char* ws) {
     RtPart& t = r->part[r->parts++];
     t.kind = kind, t.items = p.items, t.max_pieces = p.max_pieces, t.piece_tiles = p.piece_tiles;
     t.cols = rt_cols(p.halves), t.tile = rt_tokens(elem_bytes(r->a.dtype), p.halves);
+    t.by_items = rt_div(p.items), t.by_piece = rt_div(p.piece_tiles);
     t.finals = finals;
     t.p_ml = reinterpret_cast<float*>(ws);
     t.p_o = reinterpret_cast<float*>(

@@ -25,10 +25,10 @@ __device__ __forceinline__ RmPieces tile_pieces(const RtArgs& ra, const RtPart& 
         if (shared == 0) return p;
         sp = rt_span(ra, pt, 0, shared, 0, 0);
     } else {
-        const int col = (row - q.row0) * ra.n_rep + h % ra.n_rep;
-        sp = rt_span(ra, pt, q.rows, q.kv, col / pt.cols, shared);
+        const int col = (row - q.row0) * ra.n_rep + h - ra.by_rep(h) * ra.n_rep;
+        sp = rt_span(ra, pt, q.rows, q.kv, col >> (pt.cols == 128 ? 7 : 6), shared);
     }
-    p.n = rt_pieces(sp.tiles(pt.tile), pt.max_pieces, pt.piece_tiles);
+    p.n = rt_pieces(sp.tiles(pt.tile), pt);
     const int64_t slot = ((int64_t)row * ra.a.num_heads + h) * pt.max_pieces;
     p.ml = pt.p_ml + 2 * slot;
     p.o = pt.p_o + slot * head_dim;
@@ -41,9 +41,9 @@ __global__ __launch_bounds__(64 * RM_WAVES) void ranged_merge_kernel(RtArgs ra) 
     typedef typename std::conditional<E == 2, f32x2, float>::type RowV;
     const RangedAttn& a = ra.a;
     const int lane = threadIdx.x & 63;
-    const int64_t item = (int64_t)blockIdx.x * RM_WAVES + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    if (item >= (int64_t)a.rows * a.num_heads) return;
-    const int row = (int)(item / a.num_heads), h = (int)(item - (int64_t)row * a.num_heads);
+    const int item = (int)blockIdx.x * RM_WAVES + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if (item >= a.rows * a.num_heads) return;  // (rows * num_heads < 2^30)
+    const int row = ra.by_heads(item), h = item - row * a.num_heads;
     const RangedGroups groups = ranged_groups(a, 0);  // (beside the sequence's search)
     const int s = a.cu ? ranged_seq_of(a, row) : row;
     const RangedSeq q = ranged_seq(a, s);

@@ -12,6 +12,22 @@
 
 namespace flour {
 
+// x / d of 0 <= x < 2^31 without a division: with 2^(s - 1) < d <= 2^s and mul = ceil(2^(31 + s) / d), mul * d is
+// less than 2^s above 2^(31 + s), so mul * x / 2^(31 + s) is less than 1 / d above x / d. A workgroup has about
+// eight to do before its first tile (compiled divisions: 150-1,000 cycles each).
+struct RtDiv {
+    uint32_t mul;
+    int shift;  // 31 + s
+    __device__ __forceinline__ int operator()(int x) const {
+        return (int)(((uint64_t)(uint32_t)x * mul) >> shift);
+    }
+};
+inline RtDiv rt_div(int64_t d) {
+    int s = 0;
+    while (((int64_t)1 << s) < d) s++;
+    return RtDiv{(uint32_t)((((uint64_t)1 << (31 + s)) + d - 1) / d), 31 + s};
+}
+
 // What a launch attends: a unit's rows over a unit's positions.
 enum RtKind {
     RT_ROWS,    // a unit is a sequence: its rows over what they see (window and sinks)
@@ -25,6 +41,7 @@ enum RtKind {
 // domain) and accumulator at slot (r * num_heads + h) * max_pieces + k.
 struct RtPart {
     int kind, items, max_pieces, piece_tiles;
+    RtDiv by_items, by_piece;
     int cols, tile;  // columns of an item, positions of a tile (rt_cols, rt_tokens)
     bool finals;
     float* p_ml;  // [slot][2]
@@ -32,7 +49,8 @@ struct RtPart {
 };
 struct RtArgs {
     RangedAttn a;
-    int n_rep;
+    int n_rep, max_id;  // max_id: the last block
+    RtDiv by_rep, by_heads, by_kv_heads, by_block;
     float scale_log2;
     int parts;
     RtPart part[2];  // the first one's workgroups come first
@@ -59,9 +77,8 @@ constexpr bool rt_mixes(int elem_bytes, int head_dim) {
     return rt_workgroups(elem_bytes, head_dim, 2) == rt_workgroups(elem_bytes, head_dim, 1);
 }
 
-__host__ __device__ __forceinline__ int rt_pieces(int tiles, int max_pieces, int piece_tiles) {
-    const int n = (tiles + piece_tiles - 1) / piece_tiles;
-    return n < 1 ? 1 : (n < max_pieces ? n : max_pieces);
+__device__ __forceinline__ int rt_pieces(int tiles, const RtPart& pt) {
+    return max(1, min(pt.by_piece(tiles + pt.piece_tiles - 1), pt.max_pieces));
 }
 
 // The positions that a column tile of a unit goes through, in runs of 16: those of [0, front), then those of
@@ -71,7 +88,7 @@ struct RtSpan {
     __device__ __forceinline__ int tok(int run) const {
         return run < front_runs ? 16 * run : base + 16 * (run - front_runs);
     }
-    __device__ __forceinline__ int tiles(int tt) const { return (16 * runs + tt - 1) / tt; }
+    __device__ __forceinline__ int tiles(int tt) const { return (16 * runs + tt - 1) >> (tt == 64 ? 6 : 5); }
 };
 // rows and kv: the unit's. own: where the positions of RT_OWN start.
 __device__ __forceinline__ RtSpan rt_span(const RtArgs& ra, const RtPart& pt, int rows, int kv, int ctile,
@@ -80,8 +97,8 @@ __device__ __forceinline__ RtSpan rt_span(const RtArgs& ra, const RtPart& pt, in
     const int kind = pt.kind, sinks = kind == RT_ROWS ? ra.a.sinks : 0;
     s.from = 0, s.to = kv;
     if (kind != RT_PREFIX) {
-        const int i0 = ctile * pt.cols / ra.n_rep;
-        const int i1 = min(rows * ra.n_rep - 1, ctile * pt.cols + pt.cols - 1) / ra.n_rep;
+        const int i0 = ra.by_rep(ctile * pt.cols);
+        const int i1 = ra.by_rep(max(0, min(rows * ra.n_rep, ctile * pt.cols + pt.cols) - 1));
         s.to = kv > 0 ? kv - rows + i1 + 1 : 0;
         if (kind == RT_ROWS) {
             s.from = kv > 0 ? max(0, kv - rows + i0 + 1 - ra.a.window) : 0;

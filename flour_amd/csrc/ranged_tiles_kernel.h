@@ -76,8 +76,8 @@ __device__ __forceinline__ void ranged_tiles_body(const RtArgs& ra, const RtPart
 
     // ---- the item: (unit, column tile), kv head fastest (neighbouring workgroups, one an XCD, have
     // different heads, so each XCD's L2 holds its own heads' K/V)
-    const int piece = wg / pt.items, item = wg - piece * pt.items;
-    const int g = item % a.kv_heads, want = item / a.kv_heads;
+    const int piece = pt.by_items(wg), item = wg - piece * pt.items;
+    const int want = ra.by_kv_heads(item), g = item - want * a.kv_heads;
     const int units = pt.kind == RT_PREFIX ? a.num_groups : a.num_seqs;
     int unit = -1, ctile = 0, row0 = 0, rows = 0, kv = 0, seq = 0;
     // (what a prefix ends at, asked for beside the units)
@@ -99,7 +99,7 @@ __device__ __forceinline__ void ranged_tiles_body(const RtArgs& ra, const RtPart
                     ur0 = q.row0, un = q.rows, ukv = q.kv;
                 }
             }
-            const int nt = un > 0 ? (int)(((int64_t)un * n_rep + COLS - 1) / COLS) : 0;
+            const int nt = (un * n_rep + COLS - 1) / COLS;  // (rows * heads < 2^30)
             const int incl = wave_incl_sum(nt);
             const uint64_t hit = __ballot(before + incl > want);
             if (hit) {
@@ -126,24 +126,23 @@ __device__ __forceinline__ void ranged_tiles_body(const RtArgs& ra, const RtPart
     const int front = sp.front, from = sp.from, to = sp.to, all_tiles = sp.tiles(TT);
     // Tiles from `plain` on hold consecutive positions, tok_off + TT t .. ; those before hold sinks.
     const int plain = (sp.front_runs + TT / 16 - 1) / (TT / 16), tok_off = sp.base - 16 * sp.front_runs;
-    auto tile_tok = [&](int t) -> int { return t >= plain ? tok_off + TT * t : sp.tok(t * (TT / 16)); };
-    auto tile_end = [&](int t) -> int {
-        return t >= plain ? tok_off + TT * t + TT : sp.tok(t * (TT / 16) + TT / 16 - 1) + 16;
-    };
 
     // ---- this workgroup's piece of the tiles
-    const int pieces = rt_pieces(all_tiles, pt.max_pieces, pt.piece_tiles);
+    const int pieces = rt_pieces(all_tiles, pt);
     if (piece >= pieces) return;
-    const int share = all_tiles / pieces, more = all_tiles - share * pieces;  // (the first `more`: one more)
-    const int t_begin = share * piece + min(piece, more), t_end = t_begin + share + (piece < more);
+    int t_begin = 0, t_end = all_tiles;
+    if (pieces > 1) {
+        const int share = all_tiles / pieces, more = all_tiles - share * pieces;  // (the first `more`: one more)
+        t_begin = share * piece + min(piece, more), t_end = t_begin + share + (piece < more);
+    }
 
     // ---- page slots of 16-position runs, 64 at a time, one a lane
     constexpr int UPT = TT / 16, WIN = 64 / UPT;  // runs a tile, tiles a refill
-    const int max_id = (int)(a.num_slots / a.block_size - 1);
+    const int max_id = ra.max_id;
     const int last_run = (to - 1) & ~15;
     auto load_slots = [&](int t0) -> uint32_t {  // byte offsets
         const int tok = min(sp.tok(min(t0 * UPT + lane, sp.runs - 1)), last_run);
-        const int lb = a.block_size == 16 ? tok >> 4 : tok / a.block_size;
+        const int lb = ra.by_block(tok);
         int id = bt[lb];
         id = id < 0 ? 0 : (id > max_id ? max_id : id);  // a bad block id never leaves the pool
         return (uint32_t)(id * a.block_size + (tok - lb * a.block_size)) * (uint32_t)ROW;
@@ -160,10 +159,14 @@ __device__ __forceinline__ void ranged_tiles_body(const RtArgs& ra, const RtPart
     const int w_row = wave * (64 / LPR);                    // the wave's first row of a pass
     u32x4 kreg[NP], vreg[NP];
     auto load_tile = [&](uint32_t slots, int t) __attribute__((always_inline)) {
-        const int s0 = ((t - t_begin) % WIN) * UPT;
+        const int s0 = ((unsigned)(t - t_begin) % WIN) * UPT;
+        uint32_t at[NP];
+#pragma unroll
+        for (int k = 0; k < NP; k++) at[k] = __builtin_amdgcn_readlane(slots, s0 + (k * RPP + w_row) / 16);
+        __builtin_amdgcn_sched_barrier(0);  // (each load would wait for its readlane otherwise)
 #pragma unroll
         for (int k = 0; k < NP; k++) {
-            const uint32_t soff = __builtin_amdgcn_readlane(slots, s0 + (k * RPP + w_row) / 16);
+            const uint32_t soff = at[k];
             const uint32_t voff = (uint32_t)(((k * RPP + s_row) & 15) * ROW + s_col);
             kreg[k] = __builtin_amdgcn_raw_buffer_load_b128(k_rsrc, voff, soff, 0);
             vreg[k] = __builtin_amdgcn_raw_buffer_load_b128(v_rsrc, voff, soff, 0);
@@ -171,7 +174,7 @@ __device__ __forceinline__ void ranged_tiles_body(const RtArgs& ra, const RtPart
     };
     // positions of a loaded tile that no column sees: no bits of theirs
     auto cut_tile = [&](int t) __attribute__((always_inline)) {
-        if (tile_tok(t) >= from && tile_end(t) <= to) return;
+        if (t > plain && t < all_tiles - 1) return;
 #pragma unroll
         for (int k = 0; k < NP; k++) {
             const int tok = sp.tok(t * UPT + (k * RPP + w_row) / 16) + ((k * RPP + s_row) & 15);
@@ -209,7 +212,7 @@ __device__ __forceinline__ void ranged_tiles_body(const RtArgs& ra, const RtPart
     const bool live = col0 < ncols;  // (waves past the columns only stage)
     const int col = min(col0 + l32, ncols - 1);
     const bool real = col0 + l32 < ncols;
-    const int row_i = col / n_rep, head = g * n_rep + (col - row_i * n_rep);
+    const int row_i = ra.by_rep(col), head = g * n_rep + (col - row_i * n_rep);
     const int row = row0 + row_i;
     int hi, lo = 0;
     if (pt.kind == RT_PREFIX) {
@@ -232,8 +235,13 @@ __device__ __forceinline__ void ranged_tiles_body(const RtArgs& ra, const RtPart
         else
             lo = own;
     }
-    const int min_hi = wave_min_i32(hi), max_hi = wave_max_i32(hi);
-    const int min_lo = wave_min_i32(lo), max_lo = wave_max_i32(lo);
+    // (lanes are columns in the order of their rows; a prefix's rows are of several sequences)
+    int min_hi = __builtin_amdgcn_readfirstlane(hi), max_hi = __builtin_amdgcn_readlane(hi, 31);
+    if (pt.kind == RT_PREFIX) {
+        min_hi = __builtin_amdgcn_readfirstlane(wave_min_i32(hi));
+        max_hi = __builtin_amdgcn_readfirstlane(wave_max_i32(hi));
+    }
+    const int min_lo = __builtin_amdgcn_readfirstlane(lo), max_lo = __builtin_amdgcn_readlane(lo, 31);
 
     // ---- Q^T as the B operand: dims 16 kk + 8 half .. + 7 for product kk; fp32: dims D/2 half + s for
     // product s
@@ -253,7 +261,11 @@ __device__ __forceinline__ void ranged_tiles_body(const RtArgs& ra, const RtPart
     // Tile t, and meanwhile the next one's rows from registers to the other buffer, which frees the registers
     // for request().
     auto compute = [&](auto exact, int t, int buf, auto request) __attribute__((always_inline)) {
-        const int tok0 = tile_tok(t), tok_end = tile_end(t);
+        int tok0 = tok_off + TT * t, tok_end = tok0 + TT;
+        if (t < plain) {
+            tok0 = sp.tok(t * UPT), tok_end = sp.tok(t * UPT + UPT - 1) + 16;
+            asm volatile("" : "+s"(tok0), "+s"(tok_end));  // (a branch: every tile would compute both)
+        }
         if (!live || tok0 >= max_hi || (tok_end <= min_lo && tok0 >= sinks)) {
 #pragma unroll
             for (int k = 0; k < NP; k++) stage_rows(exact, k, buf ^ 1);
@@ -438,7 +450,7 @@ __device__ __forceinline__ void ranged_tiles_body(const RtArgs& ra, const RtPart
             if (t + 1 < t_end) cut_tile(t + 1);
             compute(exact, t, (t - t_begin) & 1, [&]() __attribute__((always_inline)) {
                 if (t + 2 >= t_end) return;
-                if ((t + 2 - t_begin) % WIN == 0) {
+                if ((unsigned)(t + 2 - t_begin) % WIN == 0) {
                     slots = next;
                     if (t + 2 + WIN < t_end) next = load_slots(t + 2 + WIN);
                 }
@@ -483,7 +495,18 @@ __device__ __forceinline__ void ranged_tiles_body(const RtArgs& ra, const RtPart
     pass(no{});
 
     // ---- columns to compute again
-    auto finite = [&]() -> bool {
+    auto squares = [&]() -> float {
+        float x[4] = {};
+#pragma unroll
+        for (int o = 0; o < NO; o++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) x[e & 3] = fmaf(acc[o][e], acc[o][e], x[e & 3]);
+        return (x[0] + x[1]) + (x[2] + x[3]);
+    };
+    // (sq: the lane's squares. They can overflow where the numbers do not.)
+    auto finite = [&](float sq) -> bool {
+        const bool good = sq - sq == 0.0f && l - l == 0.0f;
+        if (__ballot(!good) == 0) return true;
         float x = l - l;  // 0, or NaN where it is not finite
 #pragma unroll
         for (int o = 0; o < NO; o++)
@@ -491,18 +514,23 @@ __device__ __forceinline__ void ranged_tiles_body(const RtArgs& ra, const RtPart
             for (int e = 0; e < 16; e++) x = fmaf(acc[o][e], 0.0f, x);
         return x == 0.0f;
     };
+    const bool mine = live && owner && real;
+    float sq = squares();
+    bool good = finite(sq);
     if constexpr (BF16) {
-        float sq = 0.0f;
-#pragma unroll
-        for (int o = 0; o < NO; o++)
-#pragma unroll
-            for (int e = 0; e < 16; e++) sq = fmaf(acc[o][e], acc[o][e], sq);
-        sq = sum_across_halves(sq);
         const float least = 2.0f / (32768.0f * 1024.0f * 5e-4f * 2.0f);  // 2^-25 / 5e-4
-        const bool again = live && owner && real && l != 0.0f && !(sq >= D * least * least * l * l && finite());
-        if (__syncthreads_or(again)) {
+        const bool again = mine && l != 0.0f && !(sum_across_halves(sq) >= D * least * least * l * l && good);
+        int* const flags = reinterpret_cast<int*>(lds);  // (K's memory, which nobody reads any more)
+        const bool any = __ballot(again) != 0;
+        if (lane == 0) flags[wave] = any;
+        __syncthreads();
+        const u32x4 f = *reinterpret_cast<const u32x4*>(flags);
+        if (__builtin_amdgcn_readfirstlane(f[0] | f[1] | f[2] | f[3]) != 0) {
+            __syncthreads();  // (the pass stages there)
             begin();
             pass(yes{});
+            sq = squares();
+            good = finite(sq);
         }
     }
 
@@ -510,25 +538,45 @@ __device__ __forceinline__ void ranged_tiles_body(const RtArgs& ra, const RtPart
     const bool final_out = pt.finals && pieces == 1;
     const int64_t slot = ((int64_t)row * a.num_heads + head) * pt.max_pieces + piece;
     const int64_t out_at = (int64_t)row * a.o_st + (int64_t)head * a.o_sh;
-    const bool bad = live && owner && real && !finite();
-    if (live && owner && real && !bad) {
-        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    const bool bad = mine && !good;
+    auto emit = [&](float by, auto store) __attribute__((always_inline)) {
 #pragma unroll
         for (int o = 0; o < NO; o++)
 #pragma unroll
-            for (int e = 0; e < 16; e += 4) {
-                const int d = 32 * o + 2 * e + 4 * half;
-                float v[4];
+            for (int e = 0; e < 16; e += 4)
+                store(32 * o + 2 * e, f32x4{acc[o][e] * by, acc[o][e + 1] * by, acc[o][e + 2] * by, acc[o][e + 3] * by});
+    };
+    // 16 bits: a lane and the one of the other half swap runs of 4 dims, so that each has 8 in a row
+    auto emit16 = [&](auto type, float by) __attribute__((always_inline)) {
+        using TO = decltype(type);
+        TO* const to = static_cast<TO*>(a.out) + out_at + 8 * half;
 #pragma unroll
-                for (int x = 0; x < 4; x++) v[x] = final_out ? acc[o][e + x] * inv : acc[o][e + x];
-                if (final_out)
-                    store_run<4>(a.out, a.out_dtype, out_at + d, v);
-                else
-                    *reinterpret_cast<f32x4*>(pt.p_o + slot * D + d) = f32x4{v[0], v[1], v[2], v[3]};
+        for (int o = 0; o < NO; o++)
+#pragma unroll
+            for (int e = 0; e < 16; e += 8) {
+                uint32_t w[4];
+#pragma unroll
+                for (int x = 0; x < 4; x++)
+                    w[x] = pack2<TO>(acc[o][e + 2 * x] * by, acc[o][e + 2 * x + 1] * by);
+                const auto a0 = __builtin_amdgcn_permlane32_swap(w[0], w[2], false, false);
+                const auto a1 = __builtin_amdgcn_permlane32_swap(w[1], w[3], false, false);
+                if (mine && !bad) *reinterpret_cast<u32x4*>(to + 32 * o + 2 * e) = u32x4{a0[0], a1[0], a0[1], a1[1]};
             }
-        if (!final_out && half == 0) {
-            pt.p_ml[2 * slot] = m;
-            pt.p_ml[2 * slot + 1] = l;
+    };
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    if (final_out && a.out_dtype != FLOUR_DTYPE_F32) {
+        if (a.out_dtype == FLOUR_DTYPE_BF16)
+            emit16(bf16_t{}, inv);
+        else
+            emit16(f16_t{}, inv);
+    } else if (mine && !bad) {
+        if (!final_out) {
+            float* const to = pt.p_o + slot * D + 4 * half;
+            emit(1.0f, [&](int d, f32x4 v) { *reinterpret_cast<f32x4*>(to + d) = v; });
+            if (half == 0) *reinterpret_cast<f32x2*>(pt.p_ml + 2 * slot) = f32x2{m, l};
+        } else {
+            float* const to = static_cast<float*>(a.out) + out_at + 4 * half;
+            emit(inv, [&](int d, f32x4 v) { *reinterpret_cast<f32x4*>(to + d) = v; });
         }
     }
 
@@ -551,7 +599,7 @@ __device__ __forceinline__ void ranged_tiles_body(const RtArgs& ra, const RtPart
             float sc = -INFINITY;
             int slot_j = 0;
             if (sees) {
-                const int lb = tok / a.block_size;
+                const int lb = ra.by_block(tok);
                 int id = bt[lb];
                 id = id < 0 ? 0 : (id > max_id ? max_id : id);
                 slot_j = id * a.block_size + (tok - lb * a.block_size);
