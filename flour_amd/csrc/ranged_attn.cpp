@@ -118,8 +118,10 @@ struct TilePlan {
 // Waves that share 32 columns: 1 or 2, 0 by the plans' rules, 3 one but two of own positions where the
 // rules may say that (a test switch).
 static int g_tile_halves = 0;
-// Pieces have four tiles at least, eight where a launch could do without any (which saves the merge).
-static constexpr int LEAST_TILES = 4, LEAST_TILES_FINAL = 8;
+// Pieces have four tiles at least; five, and up to eight while that is one for a CU, where a launch could do
+// without any (which saves the merge). 5 / 8 / 12 in us: 4 rows, window 2,000, 32 / 8 heads of 128 in bf16 16.1 /
+// 18.7 / 21.4, in fp32 38.6 / 53.8 / 68.3; 100 rows (392 / 280 / 168 workgroups) 24.9 / 24.2 / 25.8 and 66.4 / 58.4 / 70.7.
+static constexpr int LEAST_TILES = 4, LEAST_TILES_FINAL = 5, MOST_TILES_FINAL = 8;
 // Units of up to unit_rows rows (rows in all), an item for each of their column tiles and kv heads.
 static int64_t tile_items(int64_t units, int64_t unit_rows, int64_t rows, int64_t n_rep, int64_t kv_heads,
                           int64_t cols) {
@@ -192,10 +194,12 @@ static TilePlan rows_plan(int num_seqs, int max_rows, int rows, int num_heads, i
     const int64_t cus = device_cus();
     int halves = 1;
     int64_t items = 0, longest = 0, piece = 0;
-    // An item of many tiles is cut along the keys while the items leave CUs idle. Whole / cut in us, by items and
-    // their tiles: 8 / 8 heads of 64 in bf16, 16 items of 10 tiles 11.4 / 18.4, of 34 23.0 / 15.8; 28 / 4 of
-    // 128, 136 of 34 36.7 / 36.4, 220 of 34 59.6 / 67.4, of 130 133.9 / 120.1; 14 / 2 of 64, 352 of 130
-    // 113.6 / 140.9; fp32, 32 / 8 of 128, 224 of 66 206 / 193.
+    // An item of several tiles is cut along the keys while the items leave CUs idle. Whole / cut in us, by items and
+    // their tiles: bf16, 14 / 2 heads of 64, 44 items of 10 tiles 13.4 / 14.4, of 13 15.8 / 13.9, of 18 19.8 / 14.6;
+    // 32 / 8 of 128, 8 of 13 18.3 / 14.8; fp32, 8 / 8 of 64, 16 of 10 32.9 / 24.7, of 18 55.1 / 24.9; many items: bf16,
+    // 28 / 4 of 128, 220 of 34 59.6 / 67.4, of 130 133.9 / 120.1; 14 / 2 of 64, 352 of 130 113.6 / 140.9; fp32,
+    // 32 / 8 of 128, 224 of 66 206 / 193.
+    const int several = dtype == FLOUR_DTYPE_F32 ? 10 : 12;
     auto cut = [&](int h) {
         halves = h;
         const int cols = rt_cols(h);
@@ -203,8 +207,9 @@ static TilePlan rows_plan(int num_seqs, int max_rows, int rows, int num_heads, i
         items = tile_items(num_seqs, max_rows, rows, n_rep, kv_heads, cols);
         const int64_t span = (int64_t)window + sinks + cols / n_rep + 2;
         longest = std::min<int64_t>(max_kv, span) / tt + 2;  // (ends that are not whole tiles)
-        const bool idle = longest >= 64 ? items <= cus : longest >= 24 && 2 * items <= cus;
-        piece = idle ? tiles_of_piece(items * longest, LEAST_TILES_FINAL, dtype) : longest;
+        const bool idle = longest >= 64 ? items <= cus : longest >= several && 2 * items <= cus;
+        const int64_t steps = items * longest, even = std::max<int64_t>(LEAST_TILES_FINAL, (steps + cus - 1) / cus);
+        piece = idle ? tiles_of_piece(steps, std::min<int64_t>(even, MOST_TILES_FINAL), dtype) : longest;
     };
     cut(1);
     // (whole columns where the cut fills the chip: fp32, 32 / 8 of 128, 80 items of 258 tiles 258 / 277)
