@@ -313,11 +313,11 @@ __device__ __forceinline__ void ranged_tiles_body(const RtArgs& ra, const RtPart
 #pragma unroll
                 for (int b = 0; b < NB; b++) s[b] = mfma32x32x16<T>(kf[kk % AHEAD][b], qb[kk], s[b]);
                 if (kk + AHEAD < NQ) read_k(kk + AHEAD);
+                if (kk & 1) stage_rows(exact, kk / 2, buf ^ 1);  // (beside the products)
                 __builtin_amdgcn_sched_barrier(0);
             }
+            static_assert(NP == NQ / 2, "rows staged under the score products");
             __builtin_amdgcn_s_setprio(0);
-#pragma unroll
-            for (int k = 0; k < NP; k++) stage_rows(exact, k, buf ^ 1);
         }
         request();  // the tile after the next one
         const bool full = tok_end <= min_hi && (tok0 >= max_lo || tok_end <= sinks);
