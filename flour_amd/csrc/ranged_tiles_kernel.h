@@ -404,23 +404,23 @@ __device__ __forceinline__ void ranged_tiles_body(const RtArgs& ra, const RtPart
             };
 #pragma unroll
             for (int n = 0; n < AHEAD; n++) read_v(n);
+            // weights 2 e and 2 e + 1 of the eight that the lane has of 16 positions
             u32x4 ph[2 * NB], pl[2 * NB];
-#pragma unroll
-            for (int x = 0; x < 2 * NB; x++)
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const int at = 8 * (x & 1) + 2 * e;
-                    const float p0 = fast_exp2(fmaf(s[x >> 1][at], ra.scale_log2, -m));
-                    const float p1 = fast_exp2(fmaf(s[x >> 1][at + 1], ra.scale_log2, -m));
-                    const uint32_t hi16 = pack2<TP>(p0, p1);
-                    ph[x][e] = hi16;
-                    if constexpr (SPLIT) {
-                        pl[x][e] = pack2<TP>(p0 - lo_f32<TP>(hi16), p1 - hi_f32<TP>(hi16));
-                        l += p0 + p1;
-                    } else {  // (the rounded weights that enter the product)
-                        l = __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, hi16), f16x2{1, 1}, l, false);
-                    }
+            auto weigh = [&](int x, int e) __attribute__((always_inline)) {
+                const int at = 8 * (x & 1) + 2 * e;
+                const float p0 = fast_exp2(fmaf(s[x >> 1][at], ra.scale_log2, -m));
+                const float p1 = fast_exp2(fmaf(s[x >> 1][at + 1], ra.scale_log2, -m));
+                const uint32_t hi16 = pack2<TP>(p0, p1);
+                ph[x][e] = hi16;
+                if constexpr (SPLIT) {
+                    pl[x][e] = pack2<TP>(p0 - lo_f32<TP>(hi16), p1 - hi_f32<TP>(hi16));
+                    l += p0 + p1;
+                } else {  // (the rounded weights that enter the product)
+                    l = __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, hi16), f16x2{1, 1}, l, false);
                 }
+            };
+#pragma unroll
+            for (int e = 0; e < 4; e++) weigh(0, e);
             __builtin_amdgcn_sched_barrier(0);
             __builtin_amdgcn_s_setprio(1);
 #pragma unroll
@@ -429,6 +429,9 @@ __device__ __forceinline__ void ranged_tiles_body(const RtArgs& ra, const RtPart
                 o = mfma32x32x16<TP>(vf[n % AHEAD], ph[n / NO], o);
                 if constexpr (SPLIT) o = mfma32x32x16<TP>(vf[n % AHEAD], pl[n / NO], o);
                 if (n + AHEAD < NF) read_v(n + AHEAD);
+                if (n / NO + 1 < 2 * NB)  // the next 16 positions' weights beside the products
+#pragma unroll
+                    for (int e = n % NO * 4 / NO; e < (n % NO + 1) * 4 / NO; e++) weigh(n / NO + 1, e);
                 __builtin_amdgcn_sched_barrier(0);
             }
             __builtin_amdgcn_s_setprio(0);
