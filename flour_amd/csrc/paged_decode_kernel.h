@@ -557,7 +557,8 @@ __global__ __launch_bounds__(SPLIT == DEC_PAIRS ? 64 * DEC_PAIR_WAVES : 64, 2) v
         int lgo = lg;
         asm volatile("" : "+v"(lgo));
         if (lc < n_rep) {
-            // F32: undefined sums give zero rows (RNG hands them on)
+            // F32: undefined sums give zero rows (RNG hands them on, and clears where no score is above -inf: its
+            // accumulators are 0 times values that may be NaN)
             constexpr bool CLEAR = F32 && !RNG;
             if (complete) {  // whole pair in this range: final output
                 if constexpr (WTS)
@@ -571,7 +572,7 @@ __global__ __launch_bounds__(SPLIT == DEC_PAIRS ? 64 * DEC_PAIR_WAVES : 64, 2) v
                                      (F32 ? 16 : D / 4) * lgo;
                 TO* o = out + o_at;
                 const float inv = 1.0f / divisor<CLEAR>(lsum);
-                if (CLEAR && !(lsum > 0.0f))
+                if (RNG ? lsum == 0.0f : CLEAR && !(lsum > 0.0f))
 #pragma unroll
                     for (int nn = 0; nn < NV; nn++) acc[nn] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
@@ -1022,7 +1023,7 @@ __global__ __launch_bounds__(64 * DEC_MERGE_WAVES) void paged_decode_merge_kerne
     for (int i = 0; i < E; i++) {
         const float x = O[i] / divisor<F32>(L);
         if constexpr (ANY)
-            store_1(out, ws.rng.out_dtype, o_at + i, x);
+            store_1(out, ws.rng.out_dtype, o_at + i, L == 0.0f ? 0.0f : x);
         else
             o[i] = from_f32<TO>(F32 && !(L > 0.0f) ? 0.0f : x);
     }
