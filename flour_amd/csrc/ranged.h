@@ -80,6 +80,29 @@ __device__ __forceinline__ int ranged_shared_of(const RangedAttn& a, const Range
     return ranged_shared_in(a, ranged_groups(a, wave_last_at(a.group_starts, 0, a.num_groups, s)), s);
 }
 
+// The lengths of the prefixes of sequences s, one a lane.
+__device__ __forceinline__ int ranged_shared_each(const RangedAttn& a, const RangedGroups& x, int s) {
+    int len = 0;
+    if (a.num_groups <= 64) {
+        for (int g = 0; g < a.num_groups; g++) {
+            const int start = __builtin_amdgcn_readlane(x.start, g), end = __builtin_amdgcn_readlane(x.end, g);
+            const int n = __builtin_amdgcn_readlane(x.len, g);
+            len = start <= s && s < end ? n : len;
+        }
+    } else {
+        int lo = 0, hi = a.num_groups;
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (a.group_starts[mid] <= s)
+                lo = mid;
+            else
+                hi = mid;
+        }
+        if (a.group_starts[lo] <= s && s < a.group_starts[lo + 1]) len = a.shared_lens[lo];
+    }
+    return max(0, min(len, a.max_shared));
+}
+
 // Takes every shape (ranged_generic.hip).
 int launch_ranged_generic(const RangedAttn& a, hipStream_t stream);
 

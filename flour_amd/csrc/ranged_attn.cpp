@@ -113,6 +113,7 @@ static bool tiles_take(const RangedAttn& a) {
 // A launch's items and the pieces that their tiles are cut into.
 struct TilePlan {
     int items, max_pieces, piece_tiles, longest, halves;
+    int extra, pitch;  // of RtPart
     size_t bytes;  // of the pieces
 };
 // Waves that share 32 columns: 1 or 2, 0 by the plans' rules, 3 one but two of own positions where the
@@ -140,17 +141,32 @@ static int64_t tiles_of_piece(int64_t steps, int64_t least, int dtype) {
     const int64_t slots = (dtype == FLOUR_DTYPE_F32 ? 8 : 7) * device_cus() / 4;
     return std::max(least, (steps + slots - 1) / slots);
 }
+// A part's memory: RT_OVER numbers where it can have extra pieces, the pieces' maxima and sums, their accumulators.
+struct PieceBytes {
+    size_t over, ml, o;
+};
+static PieceBytes piece_bytes(int64_t rows, int num_heads, int pitch, int head_dim, int extra) {
+    const size_t slots = (size_t)rows * num_heads * pitch;
+    return PieceBytes{extra > 0 ? RT_OVER * sizeof(int) : 0, up256(slots * 2 * sizeof(float)),
+                      up256(slots * head_dim * sizeof(float))};
+}
+// most: tiles of a unit, where it can have more than the longest that is planned for. A workgroup a CU for these: they
+// cost a call that has none nothing (0.1 us of 15-44, as one of them does), and 1 of 64 sequences with 16,640 positions
+// to itself, the others behind a prefix of 16,384, takes 331 us without, 86 / 71 / 70 with 64 / 128 / 256 of them, 4
+// of 64 with 8,000 (prefix 8,192) 176 and 108 / 79 / 66, 16 of 64 with up to 8,192 172 and 172 / 114 / 98.
 static TilePlan tile_plan(int halves, int64_t items, int64_t longest, int64_t piece_tiles, int64_t rows,
-                          int num_heads, int head_dim, bool finals) {
+                          int num_heads, int head_dim, bool finals, int64_t most = 0) {
     TilePlan p;
     p.halves = halves;
     p.items = (int)items;
     p.piece_tiles = (int)piece_tiles, p.longest = (int)longest;
     p.max_pieces = (int)((longest + piece_tiles - 1) / piece_tiles);
-    p.bytes = finals && p.max_pieces == 1
-                  ? 0
-                  : up256((size_t)rows * num_heads * p.max_pieces * 2 * sizeof(float)) +
-                        up256((size_t)rows * num_heads * p.max_pieces * head_dim * sizeof(float));
+    const int cus = std::min(device_cus(), 0xffff);
+    p.pitch = (int)std::max<int64_t>(p.max_pieces, std::min((most + piece_tiles - 1) / piece_tiles,
+                                                            (int64_t)p.max_pieces + cus));
+    p.extra = p.pitch > p.max_pieces ? cus : 0;
+    const PieceBytes b = piece_bytes(rows, num_heads, p.pitch, head_dim, p.extra);
+    p.bytes = finals && p.max_pieces == 1 ? 0 : b.over + b.ml + b.o;
     return p;
 }
 
@@ -166,12 +182,13 @@ static RtArgs tile_args(const RangedAttn& a) {
 static void add_part(RtArgs* r, int kind, const TilePlan& p, bool finals, char* ws) {
     RtPart& t = r->part[r->parts++];
     t.kind = kind, t.items = p.items, t.max_pieces = p.max_pieces, t.piece_tiles = p.piece_tiles;
+    t.extra = (uint16_t)p.extra, t.pitch = p.pitch;
     t.cols = rt_cols(p.halves), t.tile = rt_tokens(elem_bytes(r->a.dtype), p.halves);
     t.by_items = rt_div(p.items), t.by_piece = rt_div(p.piece_tiles);
     t.finals = finals;
-    t.p_ml = reinterpret_cast<float*>(ws);
-    t.p_o = reinterpret_cast<float*>(
-        ws + up256((size_t)r->a.rows * r->a.num_heads * p.max_pieces * 2 * sizeof(float)));
+    const PieceBytes b = piece_bytes(r->a.rows, r->a.num_heads, p.pitch, r->a.head_dim, p.extra);
+    t.p_ml = reinterpret_cast<float*>(ws + b.over);
+    t.p_o = reinterpret_cast<float*>(ws + b.over + b.ml);
 }
 
 static int launch_tiles(const RtArgs& r, int halves, int last, hipStream_t stream) {
@@ -250,11 +267,11 @@ static SharedPlan shared_plan(int num_seqs, int num_groups, int max_rows, int ro
     };
     const int es = elem_bytes(dtype), tt = rt_tokens(es, halves), tt_own = rt_tokens(es, own);
     const int64_t items_p = items(num_groups, rows, halves), items_o = items(num_seqs, max_rows, own);
-    // (a sequence of a group with a shorter prefix can have more of its own: its pieces are longer)
+    // (a sequence of no group, or of one with a shorter prefix, can have more of its own: RtPart's extra)
     const int64_t long_p = max_shared / tt + 1, long_o = std::max(0, max_kv - max_shared) / tt_own + 2;
     const int64_t piece = tiles_of_piece(items_p * long_p + items_o * long_o, LEAST_TILES, dtype);
     return SharedPlan{tile_plan(halves, items_p, long_p, piece, rows, num_heads, head_dim, false),
-                      tile_plan(own, items_o, long_o, piece, rows, num_heads, head_dim, false)};
+                      tile_plan(own, items_o, long_o, piece, rows, num_heads, head_dim, false, max_kv / tt_own + 2)};
 }
 
 // Whether prefixes are worth a part of their own, by an estimate of both ways in us from the host's bounds,

@@ -29,7 +29,9 @@ __device__ __forceinline__ RmPieces tile_pieces(const RtArgs& ra, const RtPart& 
         sp = rt_span(ra, pt, q.rows, q.kv, col >> (pt.cols == 128 ? 7 : 6), shared);
     }
     p.n = rt_pieces(sp.tiles(pt.tile), pt);
-    const int64_t slot = ((int64_t)row * ra.a.num_heads + h) * pt.max_pieces;
+    const int tiles = rt_own_tiles(pt, q.kv, shared);
+    if (tiles > rt_planned(pt)) p.n = rt_over_pieces(pt, tiles, *rt_over(pt));
+    const int64_t slot = ((int64_t)row * ra.a.num_heads + h) * pt.pitch;
     p.ml = pt.p_ml + 2 * slot;
     p.o = pt.p_o + slot * head_dim;
     return p;

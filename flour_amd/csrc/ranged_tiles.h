@@ -38,15 +38,28 @@ enum RtKind {
 // One kind's part of a launch: `items` (unit, column tile, kv head) triples at most, each of which has its
 // tiles cut into up to max_pieces pieces of at least piece_tiles. A triple of one piece is written out
 // where finals is set; otherwise piece k of packed row r, head h leaves its maximum and sum (exp2
-// domain) and accumulator at slot (r * num_heads + h) * max_pieces + k.
+// domain) and accumulator at slot (r * num_heads + h) * pitch + k.
+//
+// RT_OWN: a sequence of no group, or of one with a shorter prefix than another's, can have more tiles than its
+// max_pieces pieces are planned for. It is cut into more, of as many tiles as it takes that `extra` workgroups behind
+// the others are enough for them (left for the merge at rt_over, by the first of these).
 struct RtPart {
     int kind, items, max_pieces, piece_tiles;
     RtDiv by_items, by_piece;
     int cols, tile;  // columns of an item, positions of a tile (rt_cols, rt_tokens)
     bool finals;
+    uint16_t extra;
+    int pitch;    // slots of a (row, head): pieces at most
     float* p_ml;  // [slot][2]
     float* p_o;   // [slot][D]
 };
+// (a launch's two parts at 96 bytes each: 0.3 us more of every call)
+static_assert(sizeof(RtPart) == 64, "a part is one scalar load");
+static constexpr int RT_OVER = 64;  // numbers before p_ml
+__device__ __forceinline__ int* rt_over(const RtPart& pt) { return reinterpret_cast<int*>(pt.p_ml) - RT_OVER; }
+__device__ __forceinline__ int rt_planned(const RtPart& pt) {
+    return pt.extra > 0 ? pt.max_pieces * pt.piece_tiles : 0x7fffffff;
+}
 struct RtArgs {
     RangedAttn a;
     int n_rep, max_id;  // max_id: the last block
@@ -79,6 +92,17 @@ constexpr bool rt_mixes(int elem_bytes, int head_dim) {
 
 __device__ __forceinline__ int rt_pieces(int tiles, const RtPart& pt) {
     return max(1, min(pt.by_piece(tiles + pt.piece_tiles - 1), pt.max_pieces));
+}
+
+// RT_OWN: the tiles of a sequence of kv positions, the first `own` of them its group's.
+__device__ __forceinline__ int rt_own_tiles(const RtPart& pt, int kv, int own) {
+    const int runs = (max(0, kv - (own & ~15)) + 15) >> 4;
+    return (16 * runs + pt.tile - 1) >> (pt.tile == 64 ? 6 : 5);
+}
+// Pieces of the items of a sequence with more tiles than planned. (Theirs are cut alike, so those behind max_pieces
+// are fewer than tiles / over an item, less than `extra` in all.)
+__device__ __forceinline__ int rt_over_pieces(const RtPart& pt, int tiles, int over) {
+    return max(pt.max_pieces, min((tiles + over - 1) / max(1, over), pt.pitch));
 }
 
 // The positions that a column tile of a unit goes through, in runs of 16: those of [0, front), then those of

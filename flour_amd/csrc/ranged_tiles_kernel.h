@@ -57,8 +57,8 @@ __host__ __device__ constexpr int rt_lds(int halves) {
     return 2 * rt_tokens(sizeof(T), halves) * (RT_KP<T, D> + RT_VP<T, D>);
 }
 
-// Workgroup wg of a part.
-template <typename T, int D, int HALVES>
+// Workgroup wg of a part (EXTRA: which can be RT_OWN).
+template <typename T, int D, int HALVES, bool EXTRA>
 __device__ __forceinline__ void ranged_tiles_body(const RtArgs& ra, const RtPart pt, int wg, unsigned char* lds) {
     constexpr bool F32 = std::is_same<T, float>::value;
     constexpr bool BF16 = std::is_same<T, bf16_t>::value;
@@ -79,13 +79,15 @@ __device__ __forceinline__ void ranged_tiles_body(const RtArgs& ra, const RtPart
 
     // ---- the item: (unit, column tile), kv head fastest (neighbouring workgroups, one an XCD, have
     // different heads, so each XCD's L2 holds its own heads' K/V)
-    const int piece = pt.by_items(wg), item = wg - piece * pt.items;
-    const int want = ra.by_kv_heads(item), g = item - want * a.kv_heads;
+    int piece = pt.by_items(wg);
+    const int item = wg - piece * pt.items;
+    int want = ra.by_kv_heads(item), g = item - want * a.kv_heads;
     const int units = pt.kind == RT_PREFIX ? a.num_groups : a.num_seqs;
     int unit = -1, ctile = 0, row0 = 0, rows = 0, kv = 0, seq = 0;
     // (what a prefix ends at, asked for beside the units)
     const RangedGroups groups = pt.kind == RT_OWN ? ranged_groups(a, 0) : RangedGroups{};
-    {
+    const int extra = EXTRA && pt.extra > 0 ? wg - pt.items * pt.max_pieces : -1;
+    if (extra < 0) {
         int before = 0;
         for (int u0 = 0; u0 < units; u0 += 64) {
             const int u = u0 + lane;
@@ -117,13 +119,64 @@ __device__ __forceinline__ void ranged_tiles_body(const RtArgs& ra, const RtPart
             }
             before += __builtin_amdgcn_readlane(incl, 63);
         }
+        if (unit < 0) return;
     }
-    if (unit < 0) return;
+    int own = 0;
+    if (pt.kind == RT_OWN && extra < 0) own = __builtin_amdgcn_readfirstlane(ranged_shared_of(a, groups, seq));
+    // ---- an extra workgroup, or an item of more tiles than planned: all such sequences' tiles say how many a piece
+    // has, then the extra workgroup's piece is found by counting
+    int over = 0;
+    if (EXTRA && (extra >= 0 || rt_own_tiles(pt, kv, own) > rt_planned(pt))) {
+        struct Beyond {
+            RangedSeq q;
+            int own, nt, tiles;  // tiles: 0 where they are not more than planned
+        };
+        auto beyond = [&](int u0) -> Beyond {
+            Beyond x;
+            x.own = ranged_shared_each(a, groups, u0 + lane);
+            x.q = ranged_seq(a, min(u0 + lane, units - 1));
+            x.nt = u0 + lane < units ? (x.q.rows * n_rep + COLS - 1) / COLS : 0;
+            x.tiles = rt_own_tiles(pt, x.q.kv, x.own);
+            if (x.tiles <= rt_planned(pt)) x.tiles = 0;
+            return x;
+        };
+        double sum = 0.0;  // (whole numbers below 2^53: the same in every workgroup)
+#pragma unroll 1
+        for (int u0 = 0; u0 < units; u0 += 64) {
+            const Beyond x = beyond(u0);
+            sum += (double)x.nt * (double)x.tiles;
+        }
+        if (__ballot(sum > 0.0) == 0) return;
+        for (int x = 32; x > 0; x >>= 1) sum += __shfl_xor(sum, x, 64);
+        const double share = min(sum * a.kv_heads / pt.extra, (double)(1 << 30));
+        over = __builtin_amdgcn_readfirstlane(max(pt.piece_tiles, (int)share + 1));
+        if (extra == 0 && tid == 0) *rt_over(pt) = over;
+        int before = 0;
+#pragma unroll 1
+        for (int u0 = 0; u0 < units && extra >= 0 && unit < 0; u0 += 64) {
+            const Beyond x = beyond(u0);
+            const int n = x.tiles > 0 ? (rt_over_pieces(pt, x.tiles, over) - pt.max_pieces) * x.nt * a.kv_heads : 0;
+            const int incl = wave_incl_sum(n);
+            const uint64_t hit = __ballot(before + incl > extra);
+            if (hit) {
+                const int w = __builtin_ctzll(hit), u_nt = __builtin_amdgcn_readlane(x.nt, w);
+                const int k = extra - before - (__builtin_amdgcn_readlane(incl, w) - __builtin_amdgcn_readlane(n, w));
+                const int by_head = ra.by_kv_heads(k), p = by_head / u_nt;
+                g = k - by_head * a.kv_heads, ctile = by_head - p * u_nt, piece = pt.max_pieces + p;
+                unit = seq = u0 + w;
+                row0 = __builtin_amdgcn_readlane(x.q.row0, w);
+                rows = __builtin_amdgcn_readlane(x.q.rows, w);
+                kv = __builtin_amdgcn_readlane(x.q.kv, w);
+                own = __builtin_amdgcn_readlane(x.own, w);
+            }
+            before += __builtin_amdgcn_readlane(incl, 63);
+        }
+        if (unit < 0) return;
+    }
     const int ncols = rows * n_rep;
     const int32_t* bt = a.block_tables + (int64_t)seq * a.max_blocks;
 
     // ---- the positions
-    const int own = pt.kind == RT_OWN ? ranged_shared_of(a, groups, seq) : 0;
     const int sinks = pt.kind == RT_ROWS ? a.sinks : 0;
     const RtSpan sp = rt_span(ra, pt, rows, kv, ctile, own);
     const int front = sp.front, from = sp.from, to = sp.to, all_tiles = sp.tiles(TT);
@@ -131,7 +184,7 @@ __device__ __forceinline__ void ranged_tiles_body(const RtArgs& ra, const RtPart
     const int plain = (sp.front_runs + TT / 16 - 1) / (TT / 16), tok_off = sp.base - 16 * sp.front_runs;
 
     // ---- this workgroup's piece of the tiles
-    const int pieces = rt_pieces(all_tiles, pt);
+    const int pieces = over > 0 ? rt_over_pieces(pt, rt_own_tiles(pt, kv, own), over) : rt_pieces(all_tiles, pt);
     if (piece >= pieces) return;
     int t_begin = 0, t_end = all_tiles;
     if (pieces > 1) {
@@ -542,7 +595,7 @@ __device__ __forceinline__ void ranged_tiles_body(const RtArgs& ra, const RtPart
 
     // ---- out: a lane holds dims 32 o + 8 (e / 4) + 4 half + e % 4 of its column
     const bool final_out = pt.finals && pieces == 1;
-    const int64_t slot = ((int64_t)row * a.num_heads + head) * pt.max_pieces + piece;
+    const int64_t slot = ((int64_t)row * a.num_heads + head) * pt.pitch + piece;
     const int64_t out_at = (int64_t)row * a.o_st + (int64_t)head * a.o_sh;
     const bool bad = mine && !good;
     auto emit = [&](float by, auto store) __attribute__((always_inline)) {
@@ -627,7 +680,7 @@ __device__ __forceinline__ void ranged_tiles_body(const RtArgs& ra, const RtPart
             }
             cm = m_new;
         }
-        const int64_t c_slot = ((int64_t)c_row * a.num_heads + c_head) * pt.max_pieces + piece;
+        const int64_t c_slot = ((int64_t)c_row * a.num_heads + c_head) * pt.pitch + piece;
         const float inv = cl == 0.0f ? 0.0f : 1.0f / cl;
 #pragma unroll
         for (int x = 0; x < D / 64; x++) {
@@ -656,11 +709,11 @@ ranged_tiles_kernel(RtArgs ra) {
     const int first = ra.part[0].items * ra.part[0].max_pieces;
     const bool second = blockIdx.x >= (unsigned)first;
     if (HALVES == LAST)
-        ranged_tiles_body<T, D, HALVES>(ra, ra.part[second ? 1 : 0], (int)blockIdx.x - (second ? first : 0), lds);
+        ranged_tiles_body<T, D, HALVES, true>(ra, ra.part[second ? 1 : 0], (int)blockIdx.x - (second ? first : 0), lds);
     else if (second)
-        ranged_tiles_body<T, D, LAST>(ra, ra.part[1], (int)blockIdx.x - first, lds);
+        ranged_tiles_body<T, D, LAST, true>(ra, ra.part[1], (int)blockIdx.x - first, lds);
     else
-        ranged_tiles_body<T, D, HALVES>(ra, ra.part[0], (int)blockIdx.x, lds);
+        ranged_tiles_body<T, D, HALVES, false>(ra, ra.part[0], (int)blockIdx.x, lds);
 }
 
 template <typename T, int D>
@@ -669,7 +722,7 @@ static int launch_ranged_tiles_d(const RtArgs& r, int halves, int last, hipStrea
     if constexpr (rt_mixes(sizeof(T), D))
         if (halves < last) kern = ranged_tiles_kernel<T, D, 1, 2>;
     int64_t grid = 0;
-    for (int i = 0; i < r.parts; i++) grid += (int64_t)r.part[i].items * r.part[i].max_pieces;
+    for (int i = 0; i < r.parts; i++) grid += (int64_t)r.part[i].items * r.part[i].max_pieces + r.part[i].extra;
     kern<<<dim3((unsigned)grid), dim3(64 * RT_WAVES), 0, stream>>>(r);
     return check_hip(hipGetLastError(), "attention over ranges launch");
 }
