@@ -282,8 +282,9 @@ static SharedPlan shared_plan(int num_seqs, int num_groups, int max_rows, int ro
 // 32 / 8 heads of 128, bf16, prefix + own, us alone / shared: 64 sequences of one prefix 512 + 64 15.0 / 23.4,
 // 2,048 + 256 39.6 / 32.6, 8,192 + 512 136 / 51; of eight, eight rows each, 512 + 64 25.9 / 41.1, 2,048 + 512
 // 79.9 / 66.4; 2 of one 2,048 + 512, eight rows, 23.1 / 19.8; 16, 64 rows, 69.5 / 84.8.
-static bool prefer_shared(int num_seqs, int num_groups, int max_rows, int rows, int num_heads, int kv_heads,
-                          int head_dim, int max_kv, int max_shared, int dtype, const SharedPlan& p) {
+// as_step: the other way is the decode stream (a packed call of one row a sequence has row tiles).
+static bool prefer_shared(bool as_step, int num_seqs, int num_groups, int max_rows, int rows, int num_heads,
+                          int kv_heads, int head_dim, int max_kv, int max_shared, int dtype, const SharedPlan& p) {
     if (num_groups == 0 || max_shared == 0 || g_ranged_shared >= 0)
         return num_groups > 0 && max_shared > 0 && g_ranged_shared > 0;
     const int es = elem_bytes(dtype), n_rep = num_heads / kv_heads;
@@ -299,7 +300,7 @@ static bool prefer_shared(int num_seqs, int num_groups, int max_rows, int rows, 
     const double shared_us = 12.5 + (f32 ? 1.2 : 0.34) * std::max(chain(p.prefix), chain(p.own)) + work(p.prefix) +
                              (f32 ? 0.87 : 1.85) * work(p.own) + 2.0 * (merge(p.prefix) + merge(p.own));
     double alone_us;
-    if (max_rows <= 1 && n_rep <= 16) {
+    if (as_step) {
         const double bytes = 2.0 * num_seqs * max_kv * kv_heads * head_dim * es;
         const double sharers = std::max(1.0, (double)num_seqs / num_groups);
         alone_us = 7.0 + bytes / ((f32 ? 5e6 : 6e6) * (1.0 + 0.25 * log2(sharers) * std::min(1.0, num_seqs / 64.0)));
@@ -339,7 +340,7 @@ static int ranged_call(const char* what, const RangedAttn& a, bool shared, void*
     if (tiles && shared) {
         const SharedPlan p = shared_plan(a.num_seqs, a.num_groups, a.max_rows, a.rows, a.num_heads,
                                          a.kv_heads, a.head_dim, a.max_kv, a.max_shared, a.dtype);
-        if (prefer_shared(a.num_seqs, a.num_groups, a.max_rows, a.rows, a.num_heads, a.kv_heads,
+        if (prefer_shared(step, a.num_seqs, a.num_groups, a.max_rows, a.rows, a.num_heads, a.kv_heads,
                           a.head_dim, a.max_kv, a.max_shared, a.dtype, p)) {
             RtArgs r = tile_args(a);
             add_part(&r, RT_PREFIX, p.prefix, false, ws);
@@ -440,18 +441,23 @@ extern "C" int flour_hip_shared_workspace_size(int num_seqs, int num_groups, int
                   max_shared_len);
         return FLOUR_ERR_INVALID_ARGUMENT;
     }
+    // (whether it can be a decode step; if so a call of either form fits)
+    const bool step = total_q == num_seqs && stream_fits(num_seqs, num_heads, kv_heads, head_dim);
     size_t n = 0;
     if (tiles_fit(total_q, num_heads, kv_heads, head_dim)) {
         const SharedPlan p = shared_plan(num_seqs, num_groups, max_seqlen_q, total_q, num_heads, kv_heads,
                                          head_dim, max_kv_len, max_shared_len, dtype);
-        n = prefer_shared(num_seqs, num_groups, max_seqlen_q, total_q, num_heads, kv_heads, head_dim,
-                          max_kv_len, max_shared_len, dtype, p)
-                ? p.prefix.bytes + p.own.bytes
-                : rows_plan(num_seqs, max_seqlen_q, total_q, num_heads, kv_heads, head_dim, max_kv_len,
-                            0x7fffffff, 0, dtype).bytes;
+        const auto prefer = [&](bool as_step) {
+            return prefer_shared(as_step, num_seqs, num_groups, max_seqlen_q, total_q, num_heads, kv_heads,
+                                 head_dim, max_kv_len, max_shared_len, dtype, p);
+        };
+        const bool rows = prefer(false);
+        if (rows || (step && prefer(true))) n = p.prefix.bytes + p.own.bytes;
+        if (!rows)
+            n = std::max(n, rows_plan(num_seqs, max_seqlen_q, total_q, num_heads, kv_heads, head_dim, max_kv_len,
+                                      0x7fffffff, 0, dtype).bytes);
     }
-    if (total_q == num_seqs && stream_fits(num_seqs, num_heads, kv_heads, head_dim))  // a decode step
-        n = std::max(n, stream_bytes(num_seqs, num_heads, kv_heads, head_dim));
+    if (step) n = std::max(n, stream_bytes(num_seqs, num_heads, kv_heads, head_dim));
     *bytes = n;
     return FLOUR_OK;
 }

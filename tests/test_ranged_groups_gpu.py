@@ -129,3 +129,15 @@ def test_a_graph_replayed_with_other_groups(dt):
             check(out, b, 0.09, TILE_EPS[dt])
     finally:
         lib.flour_hip_set_shared_prefix(-1)
+
+
+@pytest.mark.parametrize("dt", DT)
+@pytest.mark.parametrize("heads", [(8, 8, 64), (32, 8, 128), (40, 2, 128)], ids=str)
+@pytest.mark.parametrize("n", [1, 16, 64])
+def test_packed_calls_of_one_row_a_sequence(dt, heads, n):
+    """In the way that the library chooses for them, with the workspace that it asks for; as a step too."""
+    for P, own in ((64, 16), (512, 64)):
+        b = R.batch(DT[dt], *heads, 16, [1] * n, [P + 1 + s % own for s in range(n)], seed=45, starts=[0, n],
+                    shared=[P])
+        every_way(b, dt, heads[2] ** -0.5, False, (1, 0, -1))
+        every_way(b, dt, heads[2] ** -0.5, True, (-1,))
