@@ -690,6 +690,16 @@ def kv_evict(k_pool: torch.Tensor, v_pool: torch.Tensor, weights: torch.Tensor,
 # ------------------------------------------------------------------ parts of the cache
 # A sliding window with sinks, and prefixes that groups of sequences share. These too run on the
 # tensors' own device, on its current stream.
+_EVERY = 2 ** 31 - 1  # positions are int32: a window of as many is one over everything
+
+
+def _span(window: int, sinks: int) -> tuple[int, int]:
+    """A window and its sinks as the library's 32 bits hold them."""
+    if window < 1 or sinks < 0:
+        raise _invalid(f"window {window} with {sinks} sinks: a row sees its own position at least")
+    return min(window, _EVERY), min(sinks, _EVERY)
+
+
 def _window_size(dev: int, *shape: int) -> int:
     return _size("flour_hip_window_workspace_size", dev, switches(), *shape)
 
@@ -703,6 +713,8 @@ def window_workspace_bytes(num_seqs: int, max_seqlen_q: int, total_q: int, num_h
                            dtype: torch.dtype) -> int:
     """Bytes of workspace of varlen_prefill_window on the current device, and of
     paged_decode_window (max_seqlen_q 1, total_q = num_seqs)."""
+    if not (0 < window <= _EVERY and 0 <= sinks <= _EVERY):
+        window, sinks = _span(window, sinks)
     return _window_size(_device_in_use(), num_seqs, max_seqlen_q, total_q, num_heads, kv_heads,
                         head_dim, max_kv_len, window, sinks, dtype_code(dtype))
 
@@ -748,6 +760,8 @@ def paged_decode_window(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Ten
                         workspace: Workspace | None = None) -> torch.Tensor:
     """paged_decode over the last ``window`` positions of each sequence, the new token's among them,
     and the first ``sinks`` ones. Blocks without visible positions are not looked at."""
+    if not (0 < window <= _EVERY and 0 <= sinks <= _EVERY):
+        window, sinks = _span(window, sinks)
     dev = _same_device(q, k_pool, v_pool, block_tables, context_lens, out)
     _need_i32(block_tables, context_lens)
     G, slots, D = _plain_pools(q, k_pool, v_pool, block_size)
@@ -775,6 +789,8 @@ def varlen_prefill_window(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.T
     positions up to p. Packed q (total_q, num_heads, head_dim), any view with a unit last stride;
     ``max_seqlen_q`` bounds the rows of a sequence, ``max_kv_len`` kv_lens; rows of q behind the last
     sequence's (a padded batch) leave ``out`` as it was."""
+    if not (0 < window <= _EVERY and 0 <= sinks <= _EVERY):
+        window, sinks = _span(window, sinks)
     dev = _same_device(q, k_pool, v_pool, cu_seqlens_q, kv_lens, block_tables, out)
     _need_i32(cu_seqlens_q, kv_lens, block_tables)
     G, slots, D = _plain_pools(q, k_pool, v_pool, block_size)

@@ -92,3 +92,18 @@ def test_ops_refuse_cpu_tensors():
               lambda: ops.varlen_prefill_shared(q, p, p, c, n, t, c, n, 1, 64, 16, 1.0)):
         with pytest.raises(_lib.FlourError, match="device tensors"):
             f()
+
+
+@pytest.mark.parametrize("more", [0, 1, 2 ** 31, 2 ** 31 + 5, 2 ** 40, 2 ** 62])
+def test_windows_and_sinks_beyond_32_bits_are_everything(more):
+    """(A C int would hold their lowest 32 bits: a window of 2^32 + 4 as one of 4.)"""
+    def size(window, sinks):
+        return ops.window_workspace_bytes(2, 8, 16, 8, 2, 64, 5000, window, sinks, torch.bfloat16)
+
+    every = 2 ** 31 - 1
+    assert size(every, 0) != size(4, 0)
+    assert size(every + more, 0) == size(every, 0) and size(4, every + more) == size(4, every)
+    for bad in ((0 - more, 0), (1, -1 - more)):
+        with pytest.raises(_lib.FlourError) as e:
+            size(*bad)
+        assert e.value.code == _lib.ERR_INVALID_ARGUMENT
