@@ -146,8 +146,9 @@ __device__ __forceinline__ f32x4 mfma16x16x4_f32(float a, float b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
 }
 
-// Waves of a DEC_PAIRS workgroup at most, and a wave's LDS there: its K tile, then its state.
-static constexpr int DEC_PAIR_WAVES = 8;
+// Waves of a DEC_PAIRS workgroup (eight are within 10% of four, two behind them but on large batches), and a wave's
+// LDS there: its K tile, then its state.
+static constexpr int DEC_PAIR_WAVES = 4;
 __host__ __device__ constexpr int dec_pair_lds(int d, int elem_bytes) {
     const int k = 16 * dec_kpitch(d, elem_bytes), state = 64 * (d * 16 / 64 + 2) * 4;
     return k > state ? k : state;
@@ -252,9 +253,8 @@ __global__ __launch_bounds__(SPLIT == DEC_PAIRS ? 64 * DEC_PAIR_WAVES : 64, 2) v
         pb = blockIdx.x / kv_heads, pg = blockIdx.x - pb * kv_heads;
         p_ctx = min(__builtin_amdgcn_readfirstlane(context_lens[pb]), max_ctx);
         p_nch = chunks_of(p_ctx);
-        const int waves = blockDim.x >> 6;
-        lo = (int64_t)p_nch * w_id / waves;
-        len = (int)((int64_t)p_nch * (w_id + 1) / waves - lo);
+        lo = (int64_t)p_nch * w_id / DEC_PAIR_WAVES;
+        len = (int)((int64_t)p_nch * (w_id + 1) / DEC_PAIR_WAVES - lo);
     } else if (narrow) {
         const WaveRanges<uint32_t> wr(total, nwg, ws.xcd_w);
         const uint32_t a = wr.lo((uint32_t)wgi);
@@ -703,8 +703,8 @@ __global__ __launch_bounds__(SPLIT == DEC_PAIRS ? 64 * DEC_PAIR_WAVES : 64, 2) v
         }
     };
 
-    // PAIRS: the waves' states through LDS, then wave w writes dims (D / 4) lg + NV r .. of r = w, w + waves ..
-    // (fp32: 64 i + 16 lg + 4 r ..), folded over the waves.
+    // PAIRS: the waves' states through LDS, then wave r writes dims (D / 4) lg + NV r .. (fp32: 64 i + 16 lg + 4 r ..),
+    // folded over the waves.
     auto fold = [&]() {
         constexpr int WAVE = dec_pair_lds(D, sizeof(T)) / 4;
         float* const all = reinterpret_cast<float*>(pre);
@@ -715,32 +715,29 @@ __global__ __launch_bounds__(SPLIT == DEC_PAIRS ? 64 * DEC_PAIR_WAVES : 64, 2) v
         mine[NV * 256 + lane] = m;
         mine[NV * 256 + 64 + lane] = lsum;
         __syncthreads();
-        const int waves = blockDim.x >> 6;
-        if (w_id >= 4) return;
+        static_assert(DEC_PAIR_WAVES == 4, "a wave for each of the four runs of a lane's dims");
         float M = DEC_M0, L = 0.0f;
-        for (int x = 0; x < waves; x++) M = fmaxf(M, all[x * WAVE + NV * 256 + lane]);
-        for (int x = 0; x < waves; x++)
+        for (int x = 0; x < DEC_PAIR_WAVES; x++) M = fmaxf(M, all[x * WAVE + NV * 256 + lane]);
+        for (int x = 0; x < DEC_PAIR_WAVES; x++)
             L += fast_exp2(all[x * WAVE + NV * 256 + lane] - M) * all[x * WAVE + NV * 256 + 64 + lane];
         const float inv = L == 0.0f ? 0.0f : 1.0f / L;
         if (lc >= n_rep) return;
         const int64_t o_at = ((int64_t)pb * num_heads + (int64_t)pg * n_rep + lc) * D + (F32 ? 16 : D / 4) * lg;
-        for (int r = w_id; r < 4; r += waves) {
-            float o[NV];
+        float o[NV];
+#pragma unroll
+        for (int nn = 0; nn < NV; nn++) o[nn] = 0.0f;
+        for (int x = 0; x < DEC_PAIR_WAVES; x++) {
+            const float* from = all + x * WAVE;
+            const float w = fast_exp2(from[NV * 256 + lane] - M) * inv;
+#pragma unroll
+            for (int nn = 0; nn < NV; nn++) o[nn] = fmaf(w, from[(nn * 64 + lane) * 4 + w_id], o[nn]);
+        }
+        if (L == 0.0f)
 #pragma unroll
             for (int nn = 0; nn < NV; nn++) o[nn] = 0.0f;
-            for (int x = 0; x < waves; x++) {
-                const float* from = all + x * WAVE;
-                const float w = fast_exp2(from[NV * 256 + lane] - M) * inv;
 #pragma unroll
-                for (int nn = 0; nn < NV; nn++) o[nn] = fmaf(w, from[(nn * 64 + lane) * 4 + r], o[nn]);
-            }
-            if (L == 0.0f)
-#pragma unroll
-                for (int nn = 0; nn < NV; nn++) o[nn] = 0.0f;
-#pragma unroll
-            for (int h4 = 0; h4 < NV; h4 += 4)
-                store_run<4>(out, rng.out_dtype, o_at + (F32 ? 16 * h4 + 4 * r : NV * r + h4), o + h4);
-        }
+        for (int h4 = 0; h4 < NV; h4 += 4)
+            store_run<4>(out, rng.out_dtype, o_at + (F32 ? 16 * h4 + 4 * w_id : NV * w_id + h4), o + h4);
     };
     if constexpr (PAIRS) {
         if (len == 0) {  // (fewer chunks than waves, or an empty context: zero rows)

@@ -62,8 +62,7 @@ static size_t stream_bytes(int batch, int num_heads, int kv_heads, int head_dim)
 // pools, 0.25 / 0.75 over fp32 ones of 64 / 128 dims), the ranges' with the bytes of all and a second launch.
 // 32 / 8 heads of 128 in bf16, ranges / workgroups in us: 1 sequence, window 128 9.3 / 6.5, 1,024 10.6 / 13.8;
 // 16, 1,024 20.1 / 20.1; 40, 128 14.7 / 9.9, 1,024 41.2 / 39.1. 8 / 8 of 64: 64, 1,024 34.5 / 27.0, 4 of 4,096
-// 13.3 / 30.2. Eight waves are within 10% of four, two behind them but on large batches.
-static constexpr int PAIR_WAVES = 4;
+// 13.3 / 30.2.
 static int g_window_pairs = -1;  // 1 always, 0 never, -1 by this (a test switch)
 static bool prefer_pairs(int64_t pairs, int64_t chunks, int head_dim, int dtype) {
     if (pairs > 0x7fffffff || g_window_pairs >= 0) return pairs <= 0x7fffffff && g_window_pairs > 0;
@@ -85,7 +84,7 @@ static int launch_stream(const RangedAttn& a, void* workspace, hipStream_t strea
     st.grid = (int)std::max<int64_t>(1, std::min<int64_t>(half, nwg));
     const int64_t pairs = (int64_t)a.num_seqs * a.kv_heads;
     if (prefer_pairs(pairs, (span + chunk - 1) / chunk, a.head_dim, a.dtype))
-        st.grid = (int)pairs, st.pair_waves = PAIR_WAVES;
+        st.grid = (int)pairs, st.pairs = true;
     auto launch = a.dtype == FLOUR_DTYPE_F32    ? launch_ranged_decode_f32
                   : a.dtype == FLOUR_DTYPE_BF16 ? launch_ranged_decode_bf16
                                                 : launch_ranged_decode_f16;

@@ -8,11 +8,12 @@
 
 namespace flour {
 
-// The stream of a step: its workspace's parts, its workgroups, and (0: waves of ranges) the waves of a
-// workgroup a pair.
+// The stream of a step: its workspace's parts, its workgroups, and whether those are a pair each (or waves of
+// ranges).
 struct RangedStream {
     DecodeWs ws;
-    int grid, pair_waves;
+    int grid;
+    bool pairs;
 };
 
 int launch_ranged_decode_f32(const RangedAttn& a, const RangedStream& st, hipStream_t stream);
@@ -22,13 +23,13 @@ int launch_ranged_decode_f16(const RangedAttn& a, const RangedStream& st, hipStr
 template <typename T, int D>
 static void launch_ranged_decode_d(const RangedAttn& a, const RangedStream& st, hipStream_t stream) {
     auto kern = a.block_size == 16
-                    ? (st.pair_waves ? paged_decode_mfma_kernel<T, AnyOut, true, D, false, false, true, DEC_PAIRS>
+                    ? (st.pairs ? paged_decode_mfma_kernel<T, AnyOut, true, D, false, false, true, DEC_PAIRS>
                                      : paged_decode_mfma_kernel<T, AnyOut, true, D, false, false, true>)
-                    : (st.pair_waves ? paged_decode_mfma_kernel<T, AnyOut, false, D, false, false, true, DEC_PAIRS>
+                    : (st.pairs ? paged_decode_mfma_kernel<T, AnyOut, false, D, false, false, true, DEC_PAIRS>
                                      : paged_decode_mfma_kernel<T, AnyOut, false, D, false, false, true>);
-    const size_t lds = st.pair_waves ? (size_t)st.pair_waves * dec_pair_lds(D, sizeof(T))
+    const size_t lds = st.pairs ? (size_t)DEC_PAIR_WAVES * dec_pair_lds(D, sizeof(T))
                                      : (size_t)(a.num_seqs + 1) * sizeof(int);
-    kern<<<dim3(st.grid), dim3(st.pair_waves ? 64 * st.pair_waves : 64), lds, stream>>>(
+    kern<<<dim3(st.grid), dim3(st.pairs ? 64 * DEC_PAIR_WAVES : 64), lds, stream>>>(
         static_cast<AnyOut*>(a.out), static_cast<const T*>(a.q), static_cast<const T*>(a.k_pool),
         static_cast<const T*>(a.v_pool), a.block_tables, a.max_blocks, a.kv_lens, a.num_seqs, a.num_heads,
         a.kv_heads, a.num_heads / a.kv_heads, a.block_size, a.num_slots, a.max_kv, a.scale * LOG2E, st.ws);
@@ -41,7 +42,7 @@ static int launch_ranged_decode(const RangedAttn& a, const RangedStream& st, hip
     else
         launch_ranged_decode_d<T, 128>(a, st, stream);
     const int rc = check_hip(hipGetLastError(), "decode over a window launch");
-    if (rc != FLOUR_OK || st.pair_waves) return rc;
+    if (rc != FLOUR_OK || st.pairs) return rc;
     const int batch = a.num_seqs, n_rep = a.num_heads / a.kv_heads;
     auto merge = a.head_dim == 64 ? paged_decode_merge_kernel<AnyOut, 64, false, false>
                                   : paged_decode_merge_kernel<AnyOut, 128, false, false>;
