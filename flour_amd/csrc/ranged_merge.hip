@@ -16,7 +16,9 @@ struct RmPieces {
     const float *ml, *o;
 };
 
-// The pieces of packed row `row`, head h in a tile launch; `shared`: the length of its group's prefix.
+// The pieces of packed row `row`, head h in a tile launch; `shared`: the length of its group's prefix. OWN: the part
+// can be RT_OWN.
+template <bool OWN>
 __device__ __forceinline__ RmPieces tile_pieces(const RtArgs& ra, const RtPart& pt, const RangedSeq& q,
                                                 int shared, int row, int h, int head_dim) {
     RmPieces p{};
@@ -28,12 +30,12 @@ __device__ __forceinline__ RmPieces tile_pieces(const RtArgs& ra, const RtPart& 
         const int col = (row - q.row0) * ra.n_rep + h - ra.by_rep(h) * ra.n_rep;
         sp = rt_span(ra, pt, q.rows, q.kv, col >> (pt.cols == 128 ? 7 : 6), shared);
     }
-    p.n = rt_pieces(sp.tiles(pt.tile), pt);
-    const int tiles = rt_own_tiles(pt, q.kv, shared);
-    if (tiles > rt_planned(pt)) p.n = rt_over_pieces(pt, tiles, *rt_over(pt));
     const int64_t slot = ((int64_t)row * ra.a.num_heads + h) * pt.pitch;
+    p.n = rt_pieces(sp.tiles(pt.tile), pt);
     p.ml = pt.p_ml + 2 * slot;
     p.o = pt.p_o + slot * head_dim;
+    if (OWN && __builtin_expect(rt_own_tiles(pt, q.kv, shared) > rt_planned(pt), 0))
+        p.n = rt_over_pieces(pt, rt_own_tiles(pt, q.kv, shared), *rt_over(pt));
     return p;
 }
 
@@ -51,8 +53,8 @@ __global__ __launch_bounds__(64 * RM_WAVES) void ranged_merge_kernel(RtArgs ra) 
     const RangedSeq q = ranged_seq(a, s);
     if (row < q.row0 || row >= q.row0 + q.rows) return;  // (rows of no sequence)
     const int shared = ranged_shared_of(a, groups, s);
-    const RmPieces p = tile_pieces(ra, ra.part[0], q, shared, row, h, D);
-    const RmPieces p2 = ra.parts > 1 ? tile_pieces(ra, ra.part[1], q, shared, row, h, D) : RmPieces{};
+    const RmPieces p = tile_pieces<false>(ra, ra.part[0], q, shared, row, h, D);
+    const RmPieces p2 = ra.parts > 1 ? tile_pieces<true>(ra, ra.part[1], q, shared, row, h, D) : RmPieces{};
     if (ra.part[0].finals && p.n == 1) return;
     const int all = p.n + p2.n;
     float M = DEC_M0, L = 0.0f, O[E] = {};

@@ -159,3 +159,26 @@ def test_steps_streamed_by_sequences_keep_both_parts_of_their_weights(dt, heads)
     scale = heads[2] ** -0.5
     b = R.batch(DT[dt], *heads, 16, [1] * 5, [450, 33, 0, 161, 1200], seed=34, starts=[0, 5], shared=[160])
     each_way(lambda eps: check(run(b, scale, decode=True, out_dtype=torch.float32), b, scale, eps[dt]), True, False)
+
+
+@pytest.mark.parametrize("value", [math.nan, math.inf])
+@pytest.mark.parametrize("dt", DT)
+@pytest.mark.parametrize("heads", [(8, 2, 64), (7, 1, 128)], ids=str)
+def test_bad_rows_in_items_cut_along_the_positions(dt, heads, value):
+    """Few rows over a long window: pieces of numbers that are not finite, rows beside them that see them no more."""
+    scale, lib = heads[2] ** -0.5, _lib.lib()
+    b = R.batch(DT[dt], *heads, 16, [5, 0, 1, 20], [5000, 9, 4100, 20], seed=35)
+    b.v_pool[0, b.slots(0, 5000)[1998], 9] = value  # the first three rows' windows hold it
+    b.v_pool[0, b.slots(2, 4100)[10], 3] = value    # a sink
+    b.k_pool[0, b.slots(0, 5000)[500]] = value      # nobody's
+    want, mag, top, seen = R.expected(b, scale, 3000, 20)
+    bad = ~torch.isfinite(want).all(2).all(1)
+    assert bad.tolist() == [True] * 3 + [False] * 2 + [True] + [False] * 20
+    mag, top = (torch.nan_to_num(x, nan=0.0, posinf=0.0) for x in (mag, top))
+    err = R.bound(mag, top, seen, heads[2], TILE_EPS[dt], 8.0)
+    try:
+        for halves in (1, 2, 0):
+            assert lib.flour_hip_set_tile_halves(halves) == 0
+            R.close(run(b, scale, 3000, 20), want, err)
+    finally:
+        lib.flour_hip_set_tile_halves(0)
