@@ -149,8 +149,8 @@ static PieceBytes piece_bytes(int64_t rows, int num_heads, int pitch, int head_d
     return PieceBytes{extra > 0 ? RT_OVER * sizeof(int) : 0, up256(slots * 2 * sizeof(float)),
                       up256(slots * head_dim * sizeof(float))};
 }
-// most: tiles of a unit, where it can have more than the longest that is planned for. A workgroup a CU for these: they
-// cost a call that has none nothing (0.1 us of 15-44, as one of them does), and 1 of 64 sequences with 16,640 positions
+// most: tiles of a unit, where it can have more than the longest that is planned for. A workgroup a CU for these: a
+// call that has none takes 0-0.5 us of 15-46 more, as with one of them. 1 of 64 sequences with 16,640 positions
 // to itself, the others behind a prefix of 16,384, takes 331 us without, 86 / 71 / 70 with 64 / 128 / 256 of them, 4
 // of 64 with 8,000 (prefix 8,192) 176 and 108 / 79 / 66, 16 of 64 with up to 8,192 172 and 172 / 114 / 98.
 static TilePlan tile_plan(int halves, int64_t items, int64_t longest, int64_t piece_tiles, int64_t rows,
@@ -280,7 +280,10 @@ static SharedPlan shared_plan(int num_seqs, int num_groups, int max_rows, int ro
 // and read. Streamed decode steps are read at 5-6 TB/s, several times that where many sequences read the same.
 // 32 / 8 heads of 128, bf16, prefix + own, us alone / shared: 64 sequences of one prefix 512 + 64 15.0 / 23.4,
 // 2,048 + 256 39.6 / 32.6, 8,192 + 512 136 / 51; of eight, eight rows each, 512 + 64 25.9 / 41.1, 2,048 + 512
-// 79.9 / 66.4; 2 of one 2,048 + 512, eight rows, 23.1 / 19.8; 16, 64 rows, 69.5 / 84.8.
+// 79.9 / 66.4; 2 of one 2,048 + 512, eight rows, 23.1 / 19.8; 16, 64 rows, 69.5 / 84.8. Packed batches of one row,
+// 1-128 sequences: 1.002 times the better one in the mean of 204. The bounds stand for every sequence, so own positions
+// of thousands, or one such sequence, can still be judged too long: 64 over 8,192 + up to 8,192 370 / 289 (the other
+// 63 up to 256: 202 / 180), chosen alone.
 // as_step: the other way is the decode stream (a packed call of one row a sequence has row tiles).
 static bool prefer_shared(bool as_step, int num_seqs, int num_groups, int max_rows, int rows, int num_heads,
                           int kv_heads, int head_dim, int max_kv, int max_shared, int dtype, const SharedPlan& p) {

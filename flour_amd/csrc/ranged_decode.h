@@ -1,7 +1,7 @@
 // ranged_decode.h — decode steps over a window with sinks: the stream of paged_decode.hip over the chunks that
 // hold visible positions. Instantiated per type in ranged_decode_*.hip. Bound by memory: 64 x 512-4,096 tokens,
-// window 1,024, 32 / 8 heads of 128 in bf16 42.9 us (6.0 TB/s of the 259 MB that are visible); 8 x 16-32K, window
-// 4,096 with 4 sinks, 64 / 8 heads in f16 25.5 us (5.3) and its merge 5.0.
+// window 1,024, 32 / 8 heads of 128 in bf16 42.0 us (6.2 TB/s of the 259 MB that are visible); 8 x 16-32K, window
+// 4,096 with 16 sinks, 64 / 8 heads in f16 26.5 us (5.1) and its merge 4.6.
 #pragma once
 
 #include "paged_decode_kernel.h"

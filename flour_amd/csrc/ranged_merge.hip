@@ -3,7 +3,7 @@
 //
 // A wave a (row, head), four to a workgroup; a lane holds the maximum and sum of one piece and D / 64
 // dims of the output, over 16 pieces' rows at a time, all in flight together. It reads each piece once. 64 rows of
-// 32 heads of 128, nine pieces each: 5.2 us; 165 rows, five, 6.9; 16 rows of 8 heads of 64 4.0, which is its
+// 32 heads of 128, nine pieces each: 5.1 us; 165 rows, five, 7.2; 16 rows of 8 heads of 64 4.0, which is its
 // launch and its dependent reads (the row's sequence, its group, the pieces).
 #include "ranged_tiles.h"
 

@@ -22,14 +22,14 @@
 //    times a V row of NaN or infinity that other columns of the tile see is NaN in the products.
 //  * fp32: v_mfma_f32_32x32x2 throughout, tiles of 32 positions.
 //
-// 16,384 tokens, window 2,048, 28 / 4 heads of 128 in bf16: 501-511 us, 885-902 TFLOP/s of visible products at
-// a clock of 1.9 GHz. Matrix cores are busy for 44% of the cycles, vector instructions issue in 49%
-// (187 a wave and tile of 32 products: weights 96, V to f16 48, maximum 19), hardly ever both at once: a wave's
-// tile was 3,750 cycles of steps one behind the other (barrier and loop 250, scores 800, V to f16 and rows to LDS
-// 600, asking for the next 400, checks 290, maximum 250, weights and V products 1,180) before the third and three
-// quarters of the weights moved between the products (508 -> 501 us, 16 turns behind prefixes 106.2 -> 104.7).
-// LDS reads have no bank conflicts. Eight prompts (256-2,048 rows, window 512, 32 / 8 heads): 69-72 us, where an item is ten tiles and
-// waits 4 us for its first one. K rows straight to LDS (no registers, 16 fewer LDS writes a workgroup and tile)
+// 16,384 tokens, window 2,048, 28 / 4 heads of 128 in bf16: 501-527 us on several cards, 857-902 TFLOP/s of visible
+// products. Matrix cores are busy for 47% of the cycles, vector instructions issue in 52% (187 a wave and tile of 32
+// products: weights 96, V to f16 48, maximum 19), hardly ever both at once: a wave's tile is 4,100 cycles of steps one
+// behind the other (barrier and loop 340, edge check 190, scores with V to f16 and rows to LDS between them 1,250,
+// asking for the next 540, masks 260, maximum 270, the first weights 130, V products with the others between them
+// 1,100).
+// LDS reads have no bank conflicts. Eight prompts (256-2,048 rows, window 512, 32 / 8 heads): 69-72 us, where an item is
+// ten tiles, of 4,000-4,800 cycles, and waits 10,000 for its first one. K rows straight to LDS (no registers, 16 fewer LDS writes a workgroup and tile)
 // are even.
 #pragma once
 

@@ -376,12 +376,20 @@ int flour_hip_kv_evict(void* k_pool, void* v_pool, float* k_scale, float* v_scal
  * own and the window - 1 before it) and those with j < sinks, the first ones, which stay visible.
  * window >= 1, sinks >= 0; a window at least as long as the context is plain causal attention.
  * Positions that no row sees are not read for their values: blocks that hold none but those may be
- * given back, their table entries left as any number. Visible positions' arithmetic is that of
- * flour_hip_paged_decode and flour_hip_varlen_prefill; a row with a visible score of NaN or +inf reads
+ * given back, their table entries left as any number. A row with a visible score of NaN or +inf reads
  * NaN, in every type, one that sees no score above -inf is a zero row.
  *
+ * Scores, maxima and sums are fp32. The weights that V is multiplied with are, over 16-bit pools, two 16-bit
+ * parts in decode steps of up to 16 query heads a kv head (as in flour_hip_paged_decode: 2^-16 of a weight),
+ * and one f16 number in prefill and in steps of larger groups (2^-11 of a weight, 2^-25 of the largest one
+ * where they are smaller than f16's normal numbers; bf16 V is f16 there too, off by 2^-25 at most, unless a row's
+ * result is not finite or its root mean square below 6e-5, when it is computed again with bf16 V and weights in
+ * two parts, as in flour_hip_varlen_prefill). Dims of V that are far smaller than their row's others keep these
+ * errors. Shapes that the matrix cores do not take (the plain calls' limits) have fp32 weights.
+ *
  * The arguments are those of the plain calls, and max_kv_len, which bounds kv_lens (a longer sequence
- * is taken to end there). Rows behind the last sequence's, where total_q is larger than
+ * is taken to end there). One-row sequences among longer ones take a prefill's time for a tile of rows each: a
+ * batch with many of them is faster as a decode call and a prefill call. Rows behind the last sequence's, where total_q is larger than
  * cu_seqlens_q[num_seqs], leave out as it was. A workspace of flour_hip_window_workspace_size
  * bytes (256-byte aligned, no initialisation needed; max_seqlen_q 1 and total_q = num_seqs = batch for
  * a decode step) goes with the call, FLOUR_ERR_WORKSPACE where it is smaller; calls that share one must
@@ -412,7 +420,9 @@ int flour_hip_varlen_prefill_window(void* out, int out_dtype, int64_t o_stride_t
 /* ------------------------------------------------------------------------------------------
  * Attention of a batch whose sequences share long prefixes, each prefix computed once for all of its
  * rows (the reference shares the prefix's blocks, prefix.rs, and attends to them once a sequence). The
- * result is that of flour_hip_paged_decode / flour_hip_varlen_prefill over the same tables.
+ * result is attention over each sequence's own table, as of flour_hip_paged_decode / flour_hip_varlen_prefill,
+ * with the roundings of a prefill above, in steps too, where prefixes are computed for their groups; where that
+ * would be slower (the library's choice, from the bounds alone), with those of the calls with a window.
  *
  *   group_starts [num_groups + 1] int32: sequences group_starts[g] .. group_starts[g + 1] - 1 are group
  *                g. They must not decrease; sequences before the first or behind the last are in no
@@ -423,7 +433,8 @@ int flour_hip_varlen_prefill_window(void* out, int out_dtype, int64_t o_stride_t
  *                reads the prefix through is its choice. Any length counts, whole blocks or not; negative
  *                ones are 0, and longer ones than max_shared_len are taken as that.
  * A row sees positions up to its own, in the prefix too, so sequences may be shorter than their group's
- * prefix. The other arguments are those of the plain calls; max_kv_len, rows behind the last sequence's,
+ * prefix, and sequences of no group as long as any. The choice takes max_kv_len - max_shared_len for what every
+ * sequence has of its own: a single very long one can make a call read all prefixes once a sequence. The other arguments are those of the plain calls; max_kv_len, rows behind the last sequence's,
  * the workspace (flour_hip_shared_workspace_size) and scores of NaN or infinity are as above.
  * ---------------------------------------------------------------------------------------- */
 int flour_hip_shared_workspace_size(int num_seqs, int num_groups, int max_seqlen_q, int total_q,
