@@ -281,7 +281,9 @@ static SharedPlan shared_plan(int num_seqs, int num_groups, int max_rows, int ro
 // 32 / 8 heads of 128, bf16, prefix + own, us alone / shared: 64 sequences of one prefix 512 + 64 15.0 / 23.4,
 // 2,048 + 256 39.6 / 32.6, 8,192 + 512 136 / 51; of eight, eight rows each, 512 + 64 25.9 / 41.1, 2,048 + 512
 // 79.9 / 66.4; 2 of one 2,048 + 512, eight rows, 23.1 / 19.8; 16, 64 rows, 69.5 / 84.8. Packed batches of one row,
-// 1-128 sequences: 1.002 times the better one in the mean of 204. The bounds stand for every sequence, so own positions
+// 1-128 sequences: 1.002 times the better one in the mean of 204. Batches of 96-4,096 sequences, on which it was not
+// fitted: 1.007 in the mean of 417, but where thousands have hundreds of short prefixes, since every workgroup walks all
+// sequences (fp32, 4,096 of 512 prefixes 256 + 32: 504 alone, 1,460 shared and chosen). The bounds stand for every sequence, so own positions
 // of thousands, or one such sequence, can still be judged too long: 64 over 8,192 + up to 8,192 370 / 289 (the other
 // 63 up to 256: 202 / 180), chosen alone.
 // as_step: the other way is the decode stream (a packed call of one row a sequence has row tiles).
